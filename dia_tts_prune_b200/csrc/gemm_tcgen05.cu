@@ -29,7 +29,6 @@
 #include <algorithm>
 #include <atomic>
 
-#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -37,6 +36,7 @@
 #include "engine_internal.h"
 #include "gemm_tcgen05.h"
 #include "attention_split.h"
+#include "tensor_cores.cuh"
 
 namespace dia {
 
@@ -55,35 +55,12 @@ constexpr int kGemmBars = 2 * kASlots + 2 * kBSlots + 4;
 constexpr int kGemmSmem = kASlots * kTileBytes + kBSlots * kBTileBytes + 1024 /* alignment slack */ + 256 /* barriers */;
 static_assert(kGemmBars * 8 + 8 <= 256, "barrier region");
 
-__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
-    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-                 ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1)
-                 : "memory");
-}
 __device__ __forceinline__ void mbar_wait_bounded(uint64_t* bar, uint32_t parity) {
     unsigned polls = 0;
     while (!mbar_try_wait(bar, parity)) {
         if (++polls > 20000000u) __trap();                  // seconds: the pipeline is stuck
     }
 }
-// K-major, 128-byte swizzle: rows of 128 B, 8-row groups 1024 B apart (stride byte offset), version 1 (sm_100)
-__device__ __forceinline__ uint64_t umma_desc(uint32_t smem_addr) {
-    const uint32_t lo = ((smem_addr & 0x3FFFFu) >> 4) | (1u << 16);
-    const uint32_t hi = (1024u >> 4) | (1u << 14) | (2u << 29);
-    return ((uint64_t)hi << 32) | lo;
-}
-__device__ __forceinline__ void umma_bf16(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-        ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
-__device__ __forceinline__ void umma_commit(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
-
 }  // namespace
 
 // gelu in its tanh form, as z sigmoid(2 u) with u = sqrt(2 / pi) (z + 0.044715 z^3): 0.5 (1 + tanh u) = sigmoid(2 u).  Fast
@@ -543,43 +520,6 @@ unsigned& gemm_pair_polls() {
     return polls;
 }
 
-__device__ __forceinline__ uint32_t at_rank(const void* local, uint32_t rank) {
-    uint32_t a;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(local)), "r"(rank));
-    return a;
-}
-__device__ __forceinline__ bool pair_wait(uint64_t* bar, uint32_t parity, unsigned polls) {       // one answer for a converged warp
-    for (unsigned i = 0; i < polls; ++i)
-        if (__any_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
-    return false;
-}
-__device__ __forceinline__ bool lane_wait(uint64_t* bar, uint32_t parity, unsigned polls) {
-    for (unsigned i = 0; i < polls; ++i)
-        if (mbar_try_wait(bar, parity)) return true;
-    return false;
-}
-// a load of this CTA that counts on a barrier of the pair's leader
-__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
-    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-                 ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1)
-                 : "memory");
-}
-__device__ __forceinline__ void umma_bf16_pair(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-        ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
-__device__ __forceinline__ void umma_commit_pair(uint64_t* bar) {                // the barrier at this place in both CTAs
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
-                 ::"r"(smem_u32(bar)), "h"((uint16_t)3) : "memory");
-}
-__device__ __forceinline__ void cluster_sync_all() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-
 // NaN for rows [row0, row0 + rows) and columns [c0, c1) of a product that has no result (a multiple of 4 columns)
 template <bool GLU>
 __device__ __noinline__ void pair_no_result(const PairProduct& p, int row0, int rows, int c0, int c1, int lane) {
@@ -596,15 +536,6 @@ __device__ __noinline__ void pair_no_result(const PairProduct& p, int row0, int 
 // the inverse of a column's scale 2^(14 - e), where its largest magnitude lies in [2^e, 2^(e + 1)) (0 for a column of zeros)
 __device__ __forceinline__ float column_inverse(float magnitude) {
     return __uint_as_float((uint32_t)max((int)(__float_as_uint(magnitude) >> 23) - 14, 0) << 23);
-}
-
-__device__ __forceinline__ void tmem_columns16(uint32_t addr, uint32_t (&v)[16]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
-          "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
-        : "r"(addr)
-        : "memory");
 }
 
 // GLU: the weights' rows are [gate (N / 2) | up (N / 2)], and a tile is 128 columns of either: the leader's half of the weight tile holds gate rows, the other's
@@ -924,21 +855,6 @@ dia_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512));
     }
-}
-
-__device__ __forceinline__ float load_remote(const float* local, uint32_t rank) {
-    uint32_t a;
-    float v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(local)), "r"(rank));
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
-    return v;
-}
-__device__ __forceinline__ float4 load_remote4(const float* local, uint32_t rank) {
-    uint32_t a;
-    float4 v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(local)), "r"(rank));
-    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a) : "memory");
-    return v;
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -1327,22 +1243,6 @@ __global__ void __launch_bounds__(256) split3_heads_kernel(const float* __restri
 }
 
 // ---- host side ---------------------------------------------------------------------------------------------------
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-static EncodeTiledFn encode_tiled() {
-    static EncodeTiledFn fn = nullptr;
-    if (!fn) {
-        void* p = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-            q == cudaDriverEntryPointSuccess)
-            fn = reinterpret_cast<EncodeTiledFn>(p);
-    }
-    return fn;
-}
-
 // a [rows][K] bf16 matrix, K contiguous, read in [box_rows x 64 k] boxes with the 128-byte swizzle
 static bool make_map(CUtensorMap* map, const void* base, long long rows, int K, int box_rows) {
     EncodeTiledFn enc = encode_tiled();
