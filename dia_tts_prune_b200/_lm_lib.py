@@ -22,6 +22,7 @@ GATE_SIGMOID, GATE_NONE, GATE_SILU, GATE_SIGMOID_HEAD = 0, 1, 2, 3
 ROT_INTERLEAVED, ROT_HALF = 0, 1
 ABI_VERSION = 6
 PRECISION_FP32, PRECISION_BF16 = 0, 1
+TYPE_FP32, TYPE_BF16, TYPE_FP16 = 0, 1, 2
 E_OK, E_INVAL, E_CUDA, E_NOMEM, E_UNSUPPORTED = 0, -1, -2, -3, -5
 
 _vp, _i, _f = C.c_void_p, C.c_int32, C.c_float
@@ -89,6 +90,12 @@ _SIGNATURES = {
     "lm_b200_op_linear": (_ci, [_vp, _vp, _vp, _ci, _ci, _ci, _vp]),
     "lm_b200_op_linear_tc": (_ci, [_vp, _vp, _vp, _vp, _ci, _ci, _ci, _vp]),
     "lm_b200_op_gated_tc": (_ci, [_vp, _vp, _vp, _vp, _vp, _ci, _ci, _ci, _ci, _cf, _ci, _vp, _ci, _vp, _vp]),
+    "lm_b200_mxfp4_code_bytes": (C.c_size_t, [_ci, _ci]),
+    "lm_b200_mxfp4_scale_bytes": (C.c_size_t, [_ci, _ci]),
+    "lm_b200_op_mxfp4_quantize": (_ci, [_vp, _ci, C.c_int64, _ci, _ci, _vp, _vp, _vp]),
+    "lm_b200_op_mxfp4_dequantize": (_ci, [_vp, _vp, _ci, _ci, _vp, _ci, _vp]),
+    "lm_b200_op_linear_mxfp4_work_bytes": (C.c_size_t, [_ci, _ci, _ci]),
+    "lm_b200_op_linear_mxfp4": (_ci, [_vp, _ci, C.c_int64, _vp, _vp, _vp, _ci, _ci, _ci, _ci, _vp, C.c_size_t, _vp]),
     "lm_b200_argmax_rows": (_ci, [_vp, _ci, _ci, _vp, _vp]),
 }
 

@@ -1,0 +1,123 @@
+"""Operators of the language models for callers that hold rows of their own: matrices in 4 bits and their products.
+
+They stand beside ``lm_engine.linear``: torch tensors on a CUDA device in, new tensors out, queued on the current stream of the tensors'
+device.  Workspaces come from torch's allocator for the length of a call, so calls on several streams and in captured graphs do not share
+any.  Arguments are checked on the host (``ValueError``, ``TypeError``); there is no CPU fallback.
+"""
+
+from __future__ import annotations
+
+from dataclasses import dataclass
+
+import torch
+
+from . import _lm_lib
+from .lm_engine import _stream
+
+_TYPES = {torch.float32: _lm_lib.TYPE_FP32, torch.bfloat16: _lm_lib.TYPE_BF16, torch.float16: _lm_lib.TYPE_FP16}
+
+
+def _check_rows(x: torch.Tensor, name: str, types=tuple(_TYPES)) -> None:
+    if not isinstance(x, torch.Tensor):
+        raise TypeError(f"{name} must be a tensor")
+    if x.dtype not in types:
+        raise TypeError(f"{name} must be one of {', '.join(str(t) for t in types)}, not {x.dtype}")
+    if not x.is_cuda:
+        raise ValueError(f"{name} must live on a CUDA device (there is no CPU fallback)")
+
+
+def _as_rows(x: torch.Tensor) -> torch.Tensor:
+    """``x [..., K]`` as rows with neighbouring channels (a view where the strides allow one)."""
+    x = x.reshape(-1, x.shape[-1])
+    # (overlapping or backward rows are copied; a row stride is only read where there are several rows)
+    return x if (x.shape[1] == 1 or x.stride(1) == 1) and (x.shape[0] <= 1 or x.stride(0) >= x.shape[1]) else x.contiguous()
+
+
+def _no_grad(what: str, *tensors: torch.Tensor) -> None:
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise ValueError(f"{what} has no gradient: detach its inputs or call it under torch.no_grad()")
+
+
+@dataclass(frozen=True)
+class Mxfp4:
+    """Rows ``[rows, width]`` in microscaled 4-bit numbers: blocks of 32 channels share a power of two (E8M0), elements are E2M1.
+    ``codes`` and ``scales`` are uint8 buffers in the kernels' layout."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+    rows: int
+    width: int
+
+    @property
+    def shape(self) -> torch.Size:
+        return torch.Size((self.rows, self.width))
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+    @property
+    def nbytes(self) -> int:
+        return self.codes.numel() + self.scales.numel()
+
+    def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+        """The values ``[rows, width]`` that the 4-bit numbers stand for."""
+        if dtype not in _TYPES:
+            raise TypeError(f"dtype must be one of {', '.join(str(t) for t in _TYPES)}, not {dtype}")
+        out = torch.empty((self.rows, self.width), dtype=dtype, device=self.device)
+        if out.numel():
+            with torch.cuda.device(self.device):
+                _lm_lib.check(_lm_lib.load().lm_b200_op_mxfp4_dequantize(self.codes.data_ptr(), self.scales.data_ptr(), self.rows, self.width,
+                                                                         out.data_ptr(), _TYPES[dtype], _stream(self.device)), "mxfp4_dequantize")
+        return out
+
+
+def quantize_mxfp4(x: torch.Tensor) -> Mxfp4:
+    """``x [rows, width]`` (float32, bfloat16 or float16; rows of any stride) in MXFP4, rounded as the OCP Microscaling specification
+    says: a block's scale is ``2 ** (floor(log2(largest magnitude)) - 2)``, at least ``2 ** -127``; elements go to the nearest of 0, 0.5,
+    1, 1.5, 2, 3, 4, 6 times the scale, half way to the even code, what lies beyond 6 to 6.  A block with an infinity or a NaN stands
+    for NaNs.  The last block of a row may be short."""
+    _check_rows(x, "x")
+    if x.dim() != 2:
+        raise ValueError(f"x must have two dimensions, not {x.dim()}")
+    _no_grad("quantize_mxfp4", x)
+    rows, width = x.shape
+    lib = _lm_lib.load()
+    codes = torch.empty(lib.lm_b200_mxfp4_code_bytes(rows, width), dtype=torch.uint8, device=x.device)
+    scales = torch.empty(lib.lm_b200_mxfp4_scale_bytes(rows, width), dtype=torch.uint8, device=x.device)
+    if x.numel():
+        x = _as_rows(x)
+        with torch.cuda.device(x.device):
+            _lm_lib.check(lib.lm_b200_op_mxfp4_quantize(x.data_ptr(), _TYPES[x.dtype], x.stride(0), rows, width, codes.data_ptr(),
+                                                        scales.data_ptr(), _stream(x.device)), "mxfp4_quantize")
+    return Mxfp4(codes, scales, rows, width)
+
+
+def linear_mxfp4(a: torch.Tensor, w: Mxfp4, out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """``a [..., width] @ w [out, width]^T`` with both sides in MXFP4: the rows of ``a`` are rounded on the way (as
+    :func:`quantize_mxfp4` does), products are exact and sums float32, and the result has ``a``'s type unless ``out_dtype`` says another.
+    For serving: it has no gradient."""
+    _check_rows(a, "a")
+    if not isinstance(w, Mxfp4):
+        raise TypeError("w must be an Mxfp4 (see quantize_mxfp4)")
+    if a.dim() < 1 or a.shape[-1] != w.width:
+        raise ValueError(f"a has rows of {a.shape[-1] if a.dim() else 0} channels, w of {w.width}")
+    if a.device != w.device:
+        raise ValueError(f"a lives on {a.device}, w on {w.device}")
+    out_dtype = a.dtype if out_dtype is None else out_dtype
+    if out_dtype not in _TYPES:
+        raise TypeError(f"out_dtype must be one of {', '.join(str(t) for t in _TYPES)}, not {out_dtype}")
+    _no_grad("linear_mxfp4", a)
+    y = torch.empty((*a.shape[:-1], w.rows), dtype=out_dtype, device=a.device)
+    if not y.numel():
+        return y
+    if not w.width:
+        return y.zero_()
+    lib, rows = _lm_lib.load(), _as_rows(a)
+    M = rows.shape[0]
+    need = lib.lm_b200_op_linear_mxfp4_work_bytes(M, w.rows, w.width)
+    work = torch.empty(need, dtype=torch.uint8, device=a.device)
+    with torch.cuda.device(a.device):
+        _lm_lib.check(lib.lm_b200_op_linear_mxfp4(rows.data_ptr(), _TYPES[a.dtype], rows.stride(0), w.codes.data_ptr(), w.scales.data_ptr(),
+                                                  y.data_ptr(), _TYPES[out_dtype], M, w.rows, w.width, work.data_ptr() if need else None, need,
+                                                  _stream(a.device)), "linear_mxfp4")
+    return y

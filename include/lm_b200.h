@@ -296,6 +296,24 @@ int lm_b200_op_gated_tc(const float *A, const void *W_bf16, void *a_bf16, float 
 /* greedy sampling: out[r] = index of the largest of logits[r][0 .. V) (ties: the lowest index) */
 int lm_b200_argmax_rows(const float *logits, int M, int V, int32_t *out, void *stream);
 
+
+/* ---- matrices and rows in microscaled 4-bit numbers (MXFP4), for callers with rows of their own ----
+ * Blocks of 32 channels along a row share a power of two 2^(floor(log2(largest magnitude)) - 2), at least 2^-127; the elements are E2M1 (0, 0.5, 1, 1.5, 2, 3, 4, 6),
+ * to the nearest, half way to the even code, 6 beyond.  A block with an infinity or a NaN stands for NaNs.  Two channels a byte in `codes`, one byte a block in `scales`;
+ * both are laid out for the kernels (see csrc/lm_mxfp4.h) and sized by: */
+enum lm_b200_type { LM_B200_FP32 = 0, LM_B200_BF16 = 1, LM_B200_FP16 = 2 };
+size_t lm_b200_mxfp4_code_bytes(int rows, int K);
+size_t lm_b200_mxfp4_scale_bytes(int rows, int K);
+/* x [rows][K] of `type`, `ld` elements from one row to the next; codes and scales 16-byte aligned */
+int lm_b200_op_mxfp4_quantize(const void *x, int type, int64_t ld, int rows, int K, void *codes, void *scales, void *stream);
+/* out [rows][K] of `type`: the values (bf16 and fp32 hold them as they are down to their smallest number; fp16 rounds) */
+int lm_b200_op_mxfp4_dequantize(const void *codes, const void *scales, int rows, int K, void *out, int type, void *stream);
+/* Y [M][N] of y_type = round(A) . W^T: the rows of A [M][K] (a_type, row stride lda) are rounded to MXFP4 as above, W [N][K] is in it; products are exact, sums fp32.
+ * work: lm_b200_op_linear_mxfp4_work_bytes(M, N, K) bytes, 128-byte aligned (none: NULL) */
+size_t lm_b200_op_linear_mxfp4_work_bytes(int M, int N, int K);
+int lm_b200_op_linear_mxfp4(const void *A, int a_type, int64_t lda, const void *w_codes, const void *w_scales, void *Y, int y_type, int M, int N, int K, void *work,
+                            size_t work_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

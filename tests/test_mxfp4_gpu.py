@@ -1,0 +1,125 @@
+"""Rows in MXFP4 and products with them (csrc/lm_mxfp4.cu) against the definition in 64 bits."""
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+MAGNITUDES = np.array([0, 0.5, 1, 1.5, 2, 3, 4, 6])
+
+
+def values(x: torch.Tensor) -> torch.Tensor:
+    """What the rows stand for in MXFP4, in 64 bits: every element's nearest magnitude, of two as near the one with the even code."""
+    a = x.detach().cpu().double().numpy()
+    rows, width = a.shape
+    a = np.concatenate([a, np.zeros((rows, -width % 32))], 1).reshape(rows, -1, 32)
+    with np.errstate(invalid="ignore", divide="ignore"):
+        most = np.abs(a).max(-1, keepdims=True)
+        finite = np.isfinite(most)
+        _, e = np.frexp(np.where(finite & (most > 0), most, 2.0 ** -126))
+        unit = np.ldexp(1.0, np.maximum(e - 3, -127))
+        r = np.where(finite, np.abs(a) / unit, 0)
+        gap = np.abs(np.minimum(r, 6)[..., None] - MAGNITUDES)
+        gap[..., 1::2] += 1e-12                                  # (halves of E2M1's steps are multiples of 0.25: far more than this)
+        v = np.sign(a) * MAGNITUDES[gap.argmin(-1)] * unit
+        v = np.where(finite, v, np.nan)
+    return torch.from_numpy(v.reshape(rows, -1)[:, :width].copy())
+
+
+def rows_of(m, k, seed, dtype=torch.float32):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(m, k, generator=g) * torch.exp(2 * torch.randn(m, 1, generator=g))
+    return x.to(dtype).cuda()
+
+
+def same(got, want):
+    got = got.double().cpu()
+    return bool(((got == want) | (got.isnan() & want.isnan())).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m,k", [(1, 1), (1, 32), (2, 31), (3, 33), (7, 128), (128, 129), (129, 256), (5, 1000), (300, 2048), (1, 8192)])
+def test_values_are_the_definitions(m, k, dtype):
+    from dia_tts_prune_b200 import lm_ops
+    x = rows_of(m, k, m + k, dtype)
+    q = lm_ops.quantize_mxfp4(x)
+    assert q.shape == (m, k)
+    assert same(q.dequantize(), values(x))
+    assert same(q.dequantize(torch.bfloat16), values(x))          # (4 significant bits: bfloat16 holds them)
+
+
+def test_borders_and_extremes():
+    """All halves between two magnitudes with either sign, the smallest and largest scales, subnormal numbers, signed zeros."""
+    from dia_tts_prune_b200 import lm_ops
+    half = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 5.5, 6.0, 6.5, 7.0, 7.99])
+    row = torch.cat([half, -half, torch.tensor([4.0, 0.0, -0.0, 1e-30, -1e-30, 2 ** -149, 0.2499999, 0.2500001])])
+    x = torch.stack([row * 2.0 ** s for s in (0, 1, -3, 100, 125, -100, -126, -140)])
+    x[4] = x[4].clamp(-3.4e38, 3.4e38)
+    x = torch.cat([x, torch.zeros(1, 32), torch.full((1, 32), 2.0 ** -149), torch.full((1, 32), 3.4028234e38)])
+    x = torch.cat([x, torch.randn(11, 32)], 1).cuda()
+    assert same(lm_ops.quantize_mxfp4(x).dequantize(), values(x))
+
+
+def test_blocks_that_are_not_finite_stand_for_nan_alone():
+    from dia_tts_prune_b200 import lm_ops
+    x = rows_of(130, 160, 3)
+    x[0, 5], x[1, 40], x[129, 159], x[7, 96] = math.inf, math.nan, -math.inf, math.nan
+    got = lm_ops.quantize_mxfp4(x).dequantize().cpu()
+    assert same(got, values(x))
+    assert int(got.isnan().sum()) == 4 * 32
+    w = rows_of(64, 160, 4)
+    y = lm_ops.linear_mxfp4(x, lm_ops.quantize_mxfp4(w)).cpu()
+    assert y[[0, 1, 7, 129]].isnan().all() and y.isnan().sum() == 4 * 64
+    y = lm_ops.linear_mxfp4(w, lm_ops.quantize_mxfp4(x)).cpu()
+    assert y[:, [0, 1, 7, 129]].isnan().all() and y.isnan().sum() == 4 * 64
+
+
+def test_strides():
+    """Rows that stand apart, rows that do not start at 16 bytes, and neighbours along the other axis."""
+    from dia_tts_prune_b200 import lm_ops
+    big = rows_of(40, 301, 9, torch.bfloat16)
+    w = lm_ops.quantize_mxfp4(rows_of(33, 100, 10))
+    for x in (big[:, :100], big[::3, 1:101], big[:, 201:], rows_of(100, 40, 11).T, big[:1, :100].expand(5, 100)):
+        assert same(lm_ops.quantize_mxfp4(x).dequantize(), values(x))
+        assert torch.equal(lm_ops.linear_mxfp4(x, w), lm_ops.linear_mxfp4(x.contiguous().clone(), w))
+
+
+def check(x, w, y):
+    """Products are exact; a tensor core adds 64 of them at a time to a float32 sum and cuts off, which loses at most 2^-22 of the
+    magnitudes summed so far at each of K / 64 steps (2^-23 for the sum and as much for the products that are lined up with it); and the
+    result's own rounding: half a step, which is eps / 2 of a normal number and eps / 2 of the smallest normal number below that (float16:
+    2^-25; a result of 3e-5 stood 2.96e-8 off)."""
+    a, b = values(x), values(w)
+    want, most, t = a @ b.T, a.abs() @ b.abs().T, torch.finfo(y.dtype)
+    bound = (x.shape[1] / 64 + 2) * 2.0 ** -22 * most + t.eps / 2 * (want.abs() + t.smallest_normal)
+    assert y.dtype == x.dtype and y.shape == want.shape
+    worst = ((y.double().cpu() - want).abs() - bound).max()
+    assert worst <= 0, float(worst)
+
+
+SIZES = [(1, 1, 1), (1, 2048, 2048), (2, 5, 33), (3, 130, 256), (8, 1028, 200), (9, 64, 384), (16, 257, 4096), (17, 300, 1000), (32, 128, 128), (33, 96, 640),
+         (64, 2048, 1024), (65, 129, 129), (128, 128, 128), (129, 127, 500), (257, 384, 1152), (333, 1028, 2000), (1000, 640, 520)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m,n,k", SIZES)
+def test_products_against_64_bits(m, n, k, dtype):
+    from dia_tts_prune_b200 import lm_ops
+    x, w = rows_of(m, k, m, dtype) * 0.25, rows_of(n, k, n, torch.bfloat16) / k ** 0.5
+    if m > 2:
+        x[m // 2] = 0
+    check(x, w, lm_ops.linear_mxfp4(x, lm_ops.quantize_mxfp4(w)))
+
+
+def test_many_tiles_on_every_sm_and_leading_dimensions():
+    from dia_tts_prune_b200 import lm_ops
+    x, w = rows_of(1030, 320, 1, torch.bfloat16) * 0.25, rows_of(8200, 320, 2, torch.bfloat16)
+    q = lm_ops.quantize_mxfp4(w)
+    y = lm_ops.linear_mxfp4(x.view(5, 206, 320), q)
+    assert y.shape == (5, 206, 8200)
+    check(x, w, y.view(1030, 8200))
+    assert lm_ops.linear_mxfp4(x[0], q).shape == (8200,)
+    assert lm_ops.linear_mxfp4(x[:3], q, out_dtype=torch.float32).dtype == torch.float32
