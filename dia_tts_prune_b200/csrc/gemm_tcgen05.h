@@ -60,6 +60,9 @@ inline long long& extra_launches() {
     return n;
 }
 
+// how often a wait of the kernels on pairs of SMs (and of those of 4-bit numbers) looks at its barrier, in launches of this thread
+unsigned& gemm_pair_polls();
+
 inline bool gemm_tcgen05_shape_ok(int M, int N, int K) { return M > 0 && N > 0 && K >= 8 && K % 8 == 0 && N % 4 == 0; }
 
 cudaError_t launch_gemm_tcgen05_bf16(const void* a_bf16, int terms, const void* wt, long long wt_rows, float* y, int M, int N,

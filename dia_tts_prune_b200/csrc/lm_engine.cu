@@ -98,6 +98,7 @@
 #include "gemm_tcgen05.h"
 #include "lm_b200.h"
 #include "lm_internal.h"
+#include "lm_loss.h"
 #include "lm_mxfp4.h"
 
 namespace {
@@ -132,6 +133,14 @@ inline cudaStream_t S(void* s) { return reinterpret_cast<cudaStream_t>(s); }
 
 constexpr int kMostChannels = 1 << 24;           // of a row that an operator takes (offsets inside a row stay in 32 bits)
 inline bool known_type(int t) { return t == LM_B200_FP32 || t == LM_B200_BF16 || t == LM_B200_FP16; }
+inline bool loss_shape(lm::LossShape& s, const void* h, int h_type, int64_t ldh, const void* W, int64_t ldw, int M, int V, int K) {
+    constexpr int most = 0x7fffffff - 256;       // (tiles of 256 are counted in 32 bits)
+    if (!h || !W || M <= 0 || M > most || V <= 0 || V > most || K <= 0 || K > kMostChannels || (M > 1 && ldh < K) || (V > 1 && ldw < K) ||
+        (h_type != LM_B200_FP32 && h_type != LM_B200_BF16))
+        return false;
+    s = lm::LossShape{h, h_type, M > 1 ? ldh : K, W, V > 1 ? ldw : K, nullptr, 0, 0, M, V, K, 1.f};
+    return true;
+}
 inline bool aligned(const void* p, unsigned to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
 inline lm::NormW N(const lm_b200_norm& n) { return lm::NormW{n.w, n.b, n.alpha}; }
 
@@ -1743,6 +1752,38 @@ int lm_b200_op_linear_mxfp4(const void* A, int a_type, int64_t lda, const void* 
         !aligned(w_codes, 16) || !aligned(w_scales, 16) || !aligned(work, 128) || work_bytes < lm_b200_op_linear_mxfp4_work_bytes(M, N, K) || (work_bytes && !work))
         return LM_B200_EINVAL;
     LCK(lm::launch_mxfp4_linear(lm::Mxfp4Product{A, a_type, M > 1 ? lda : K, w_codes, w_scales, Y, y_type, M, N, K, nullptr, 0}, work, S(stream)));
+    return LM_B200_OK;
+}
+
+size_t lm_b200_op_loss_work_bytes(const void* h, int h_type, int64_t ldh, const void* W, int64_t ldw, int M, int V, int K) {
+    lm::LossShape s;
+    return loss_shape(s, h, h_type, ldh, W, ldw, M, V, K) ? lm::loss_work_bytes(s) : 0;
+}
+
+int lm_b200_op_loss(const void* h, int h_type, int64_t ldh, const void* W, int64_t ldw, const void* targets, int targets64, int64_t ignore, int M, int V, int K, float scale,
+                    float* loss, float* lse, float* totals, void* work, size_t work_bytes, void* stream) {
+    lm::LossShape s;
+    if (!loss_shape(s, h, h_type, ldh, W, ldw, M, V, K) || !targets || !(scale > 0.f) || !std::isfinite(scale) || !loss || !lse || !totals || !work || !aligned(work, 256) ||
+        work_bytes < lm::loss_work_bytes(s))
+        return LM_B200_EINVAL;
+    s.targets = targets; s.targets64 = targets64; s.ignore = ignore; s.scale = scale;
+    LCK(lm::launch_loss(s, loss, lse, totals, work, S(stream)));
+    return LM_B200_OK;
+}
+
+size_t lm_b200_op_loss_grad_work_bytes(const void* h, int64_t ldh, const void* W, int64_t ldw, int M, int V, int K, int rows, int head) {
+    lm::LossShape s;
+    return loss_shape(s, h, LM_B200_BF16, ldh, W, ldw, M, V, K) ? lm::loss_grad_work_bytes(s, rows != 0, head != 0) : 0;
+}
+
+int lm_b200_op_loss_grad(const void* h, int64_t ldh, const void* W, int64_t ldw, const void* targets, int targets64, int64_t ignore, int M, int V, int K, float scale,
+                         const float* lse, const float* grad, int grad_stride, const float* count, void* dh, void* dW, void* work, size_t work_bytes, void* stream) {
+    lm::LossShape s;
+    if (!loss_shape(s, h, LM_B200_BF16, ldh, W, ldw, M, V, K) || !targets || !(scale > 0.f) || !std::isfinite(scale) || !lse || !grad || grad_stride < 0 || (!dh && !dW) ||
+        !work || !aligned(work, 256) || work_bytes < lm::loss_grad_work_bytes(s, dh != nullptr, dW != nullptr))
+        return LM_B200_EINVAL;
+    s.targets = targets; s.targets64 = targets64; s.ignore = ignore; s.scale = scale;
+    LCK(lm::launch_loss_grad(s, lse, grad, grad_stride, count, dh, dW, work, S(stream)));
     return LM_B200_OK;
 }
 

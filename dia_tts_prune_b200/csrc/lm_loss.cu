@@ -1,0 +1,678 @@
+// lm_loss.cu - cross entropy of rows h [M][K] under a head w [V][K], and its gradient, without the logits in memory.
+//
+//   z = scale h w^T,  loss_i = log sum_j exp z_ij - z_i,target        P = (softmax(z) - onehot) g scale,  dh = P w,  dw = P^T h
+//
+// Forward: one product whose epilogue keeps of a 256 x 256 tile of logits, per row, the largest one, the sum of the exponentials below it and the target's, all in fp32;
+// a second kernel joins the tiles of a row.  Backward: the vocabulary goes in pieces.  The product is taken again for a piece, its epilogue turns logits into P (bf16, a
+// piece of at most 64 MB or 4096 columns: it stays in L2), and two products take P to dh (fp32 sums over the pieces) and to the piece's rows of dw.
+//
+// All four are one kernel on pairs of SMs: a cluster of two CTAs owns a 256 x 256 tile, tcgen05.mma (cta_group::2) multiplies the 256 rows of both by the 256 columns of
+// both, and the accumulators (two per CTA: a tile is taken out while the next is multiplied) live in tensor memory.
+//   warp 0    one lane per CTA: TMA loads of its halves into a ring of stages; every byte of both CTAs counts on the leader's barrier
+//   warp 1    leader only: one elected lane issues the pair's MMAs, commits to the barriers of both CTAs
+//   warps 2-5 epilogue of the CTA's 128 rows
+// P w contracts over rows of w and P^T h over rows of both: those operands lie with the contraction along their rows in memory, and the MMA takes them so
+// (MN-major descriptors); nothing is transposed.
+#include <algorithm>
+
+#include <cuda_bf16.h>
+
+#include "attention_split.h"
+#include "engine_internal.h"
+#include "gemm_tcgen05.h"
+#include "lm_loss.h"
+#include "lm_mxfp4.h"
+#include "tensor_cores.cuh"
+
+namespace lm {
+namespace {
+
+using namespace dia;
+
+enum Kind { kStats, kProbs, kRows, kHead };
+
+constexpr int kTileN = 256, kBK = 64, kTileBytes = 128 * kBK * 2;          // 16 KB: 128 rows of an operand, 64 of the contraction
+constexpr int kThreads = 192, kStagesMost = 6, kTurn = 4 * 4096;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+template <int TERMS>
+struct Ring {
+    static constexpr int kStage = (TERMS + 1) * kTileBytes, kStages = TERMS == 1 ? 6 : 3;
+    static constexpr int kSmem = kStages * kStage + kTurn + 1024 + 256;
+};
+
+struct LossTiles {
+    int M, N, K;                     // rows and columns of the product, length of the contraction
+    int splits;                      // kRows: pairs that share the contraction of a tile
+    const void* targets; int targets64; long long ignore;
+    float c;                         // scale log2(e)
+    unsigned* arrived;               // kStats: set to zero for the kernel that joins the tiles
+    float2* part; float* hit;        // kStats: [M][column tiles] largest c z and sum of 2^(c z - it); [M] z of the target
+    const float *lse, *grad, *count; int grad_stride; float scale; int v0, V;      // kProbs: columns v0 .. of the head
+    __nv_bfloat16* p; int ldp;
+    float* acc; int ld_acc, add;     // kRows: [splits][M][ld_acc]; add: to what is there
+    __nv_bfloat16* out; int wide;    // kHead: [M][N]; wide: 16-byte stores
+    int* ran_out;
+    unsigned polls;
+};
+
+__device__ __forceinline__ long long target_of(const void* t, int wide, int i) {
+    return wide ? reinterpret_cast<const long long*>(t)[i] : (long long)reinterpret_cast<const int*>(t)[i];
+}
+
+// An operand whose contraction lies along memory rows: [64 k][64 channels] boxes of 128-byte rows with the 128-byte swizzle.  Eight rows of k are 1024 bytes apart
+// (stride byte offset), 64 channels further the next box begins, 8192 bytes on (leading byte offset).
+__device__ __forceinline__ uint64_t umma_desc_mn(uint32_t smem_addr) {
+    const uint32_t lo = ((smem_addr & 0x3FFFFu) >> 4) | ((8192u >> 4) << 16);
+    const uint32_t hi = (1024u >> 4) | (1u << 14) | (2u << 29);
+    return ((uint64_t)hi << 32) | lo;
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// 32 rows (lane = row) x 64 columns of bf16 through shared memory: whole lines of out [..][ld] from (row0, c0) on, `rows` and `cols` of them
+__device__ __forceinline__ void store_64(unsigned char* blk, const uint32_t (&y)[32], __nv_bfloat16* out, long long ld, long long row0, int rows, int c0, int cols, bool wide,
+                                         int lane) {
+    const int rr = lane >> 3, ch = lane & 7;
+    // its 16-byte piece c goes to place c ^ (row % 8) of the row's 128 bytes, and is read a row per eight lanes
+#pragma unroll
+    for (int c = 0; c < 8; ++c)
+        *reinterpret_cast<uint4*>(blk + lane * 128 + ((c ^ (lane & 7)) << 4)) = make_uint4(y[4 * c], y[4 * c + 1], y[4 * c + 2], y[4 * c + 3]);
+    __syncwarp();
+    if (wide) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int r = 4 * e + rr;
+            if (r < rows && 8 * ch < cols)
+                *reinterpret_cast<uint4*>(out + (row0 + r) * ld + c0 + 8 * ch) = *reinterpret_cast<const uint4*>(blk + r * 128 + ((ch ^ (r & 7)) << 4));
+        }
+    } else {
+        for (int r = 0; r < rows; ++r)
+#pragma unroll
+            for (int c = lane; c < 64; c += 32)
+                if (c < cols)
+                    reinterpret_cast<uint16_t*>(out)[(row0 + r) * ld + c0 + c] = *reinterpret_cast<const uint16_t*>(blk + r * 128 + (((c >> 3) ^ (r & 7)) << 4) + 2 * (c & 7));
+    }
+    __syncwarp();
+}
+
+template <int KIND, int TERMS>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+loss_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ LossTiles p) {
+    constexpr bool kAmn = KIND == kHead, kBmn = KIND == kRows || KIND == kHead;
+    constexpr int kStage = Ring<TERMS>::kStage, kStages = Ring<TERMS>::kStages;
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    unsigned char* turn = smem + kStages * kStage;
+    uint64_t* full = reinterpret_cast<uint64_t*>(turn + kTurn);              // (the leader's alone)
+    uint64_t* empty = full + kStagesMost;
+    uint64_t* t_full = empty + kStagesMost;
+    uint64_t* t_empty = t_full + 2;                                          // (the leader's alone)
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(t_empty + 2);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = blockIdx.x & 1;
+    const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+    const int kb_all = (p.K + kBK - 1) / kBK, splits = KIND == kRows ? p.splits : 1, kb_per = (kb_all + splits - 1) / splits;
+    const int tiles_m = (p.M + 255) / 256, tiles_n = (p.N + kTileN - 1) / kTileN, n_tiles = tiles_m * tiles_n * splits;
+    // tile t: row block t % tiles_m, then the column block, then the share of the contraction
+    const auto first_kb = [&](int t) { return KIND == kRows ? t / (tiles_m * tiles_n) * kb_per : 0; };
+    const auto last_kb = [&](int t) { return KIND == kRows ? min(first_kb(t) + kb_per, kb_all) : kb_all; };
+
+    if (KIND == kStats && blockIdx.x == 0 && threadIdx.x == 0) *p.arrived = 0u;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kStages; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&t_full[i], 1); mbar_init(&t_empty[i], 8); }
+        fence_mbar_init();
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::);
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    cluster_sync_all();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem_base = *tmem_slot;
+    bool ok = true;
+    if (warp == 0) {
+        if (lane == 0) {
+            unsigned i = 0;
+            for (int t = pair; t < n_tiles && ok; t += pairs) {
+                const int tn = t / tiles_m % tiles_n, a0 = t % tiles_m * 256 + (int)rank * 128, b0 = tn * kTileN + (int)rank * 128;
+                for (int kb = first_kb(t); kb < last_kb(t); ++kb, ++i) {
+                    const unsigned s = i % kStages;
+                    if (!lane_wait(&empty[s], ((i / kStages) & 1u) ^ 1u, p.polls)) { ok = false; break; }
+                    if (rank == 0) mbar_arrive_expect_tx(&full[s], 2u * kStage);
+                    const uint32_t bar = at_rank(&full[s], 0), dst = smem_u32(smem + s * kStage), k = kb * kBK;
+                    if constexpr (kBmn) {                     // (of the head in kRows: the piece's rows)
+                        tma_load_2d_pair(dst + TERMS * kTileBytes, &map_b, bar, b0, p.v0 + k);
+                        tma_load_2d_pair(dst + TERMS * kTileBytes + kTileBytes / 2, &map_b, bar, b0 + 64, p.v0 + k);
+                    } else {
+                        tma_load_2d_pair(dst + TERMS * kTileBytes, &map_b, bar, k, p.v0 + b0);
+                    }
+                    if constexpr (kAmn) {
+                        tma_load_2d_pair(dst, &map_a, bar, a0, k);
+                        tma_load_2d_pair(dst + kTileBytes / 2, &map_a, bar, a0 + 64, k);
+                    } else {
+#pragma unroll
+                        for (int tm = 0; tm < TERMS; ++tm) tma_load_2d_pair(dst + tm * kTileBytes, &map_a, bar, k, tm * p.M + a0);
+                    }
+                }
+            }
+            // (the leader's last commits arrive here: not after this CTA has gone)
+            for (unsigned j = i > (unsigned)kStages ? i - kStages : 0; j < i && ok; ++j) ok = lane_wait(&empty[j % kStages], (j / kStages) & 1u, p.polls);
+            // (nor do copies arrive that were issued before a wait ran out)
+            for (unsigned j = i > (unsigned)kStages ? i - kStages : 0; j < i && !ok && rank == 0; ++j) (void)lane_wait(&full[j % kStages], (j / kStages) & 1u, p.polls);
+        }
+    } else if (warp == 1) {
+        if (rank == 0) {
+            // fp32 accumulators, bf16 operands, which of them are MN-major, N = 256, M = 256
+            const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((kAmn ? 1u : 0u) << 15) | ((kBmn ? 1u : 0u) << 16) | ((uint32_t)(kTileN >> 3) << 17) | (16u << 24);
+            constexpr uint32_t a_step = kAmn ? 2048 >> 4 : 2, b_step = kBmn ? 2048 >> 4 : 2;        // 16 of the contraction, in descriptor units
+            unsigned i = 0, it = 0;
+            for (int t = pair; t < n_tiles && ok; t += pairs, ++it) {
+                if (!pair_wait(&t_empty[it & 1u], ((it >> 1) & 1u) ^ 1u, p.polls)) { ok = false; break; }
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint32_t d = tmem_base + (it & 1u) * kTileN;
+                const int kb0 = first_kb(t), kb1 = last_kb(t);
+                for (int kb = kb0; kb < kb1; ++kb, ++i) {
+                    const unsigned s = i % kStages;
+                    if (!pair_wait(&full[s], (i / kStages) & 1u, p.polls)) { ok = false; break; }
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint32_t at = smem_u32(smem + s * kStage);
+                    const uint64_t bdesc = kBmn ? umma_desc_mn(at + TERMS * kTileBytes) : umma_desc(at + TERMS * kTileBytes);
+                    if (elect_one_sync()) {
+#pragma unroll
+                        for (int u = 0; u < TERMS; ++u) {
+                            const uint32_t a_at = at + (TERMS - 1 - u) * kTileBytes;                 // the smallest term first
+                            const uint64_t adesc = kAmn ? umma_desc_mn(a_at) : umma_desc(a_at);
+#pragma unroll
+                            for (int j = 0; j < kBK / 16; ++j)
+                                umma_bf16_pair(d, adesc + a_step * j, bdesc + b_step * j, idesc, (u | j) != 0 || kb != kb0 ? 1u : 0u);
+                        }
+                        umma_commit_pair(&empty[s]);
+                        if (kb == kb1 - 1) umma_commit_pair(&t_full[it & 1u]);
+                    }
+                    __syncwarp();
+                }
+            }
+        }
+    } else {
+        const int q = warp & 3;
+        unsigned char* const blk = turn + (warp - 2) * 4096;
+        unsigned it = 0;
+        for (int t = pair; t < n_tiles; t += pairs, ++it) {
+            const int tn = t / tiles_m % tiles_n, n0 = tn * kTileN, row0 = t % tiles_m * 256 + (int)rank * 128 + q * 32, rows = min(32, p.M - row0), row = row0 + lane;
+            const bool mine = row < p.M;
+            ok = ok && pair_wait(&t_full[it & 1u], (it >> 1) & 1u, p.polls);
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const uint32_t from = tmem_base + ((uint32_t)(q * 32) << 16) + (it & 1u) * kTileN;
+            if constexpr (KIND == kStats) {
+                const long long target = mine ? target_of(p.targets, p.targets64, row) : -1;
+                float most = -CUDART_INF_F, sum = 0.f;        // of c z, of 2^(c z - most)
+#pragma unroll 1
+                for (int cb = 0; cb < kTileN / 32; ++cb) {
+                    const int c0 = n0 + cb * 32;
+                    if (c0 >= p.N || rows <= 0) break;        // (uniform)
+                    uint32_t v[32];
+                    tmem_columns32(from + cb * 32, v);
+                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                    if (c0 + 32 > p.N) {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) if (c0 + e >= p.N) v[e] = __float_as_uint(-CUDART_INF_F);
+                    }
+                    float top[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) top[e & 3] = fmaxf(top[e & 3], __uint_as_float(v[e]));
+                    const float now = fmaxf(most, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * p.c);
+                    const float below = now == -CUDART_INF_F ? 0.f : now;        // (nothing but minus infinities so far)
+                    float add[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) add[e & 3] += exp2_fast(fmaf(__uint_as_float(v[e]), p.c, -below));
+                    sum = (most == -CUDART_INF_F ? 0.f : sum * exp2_fast(most - now)) + ((add[0] + add[1]) + (add[2] + add[3]));
+                    most = now;
+                    if (target >= c0 && target < c0 + 32 && target < p.N) {
+                        float z = 0.f;
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) z = target == c0 + e ? __uint_as_float(v[e]) : z;
+                        p.hit[row] = ok ? z : CUDART_NAN_F;
+                    }
+                }
+                if (mine) p.part[(size_t)row * tiles_n + tn] = ok ? make_float2(most, sum) : make_float2(CUDART_NAN_F, CUDART_NAN_F);      // (no result)
+            } else if constexpr (KIND == kProbs) {
+                // a row's number in front of the exponential, and the factor behind it
+                float g = 0.f, base = 0.f;
+                int target = -1;
+                if (mine) {
+                    const long long to = target_of(p.targets, p.targets64, row);
+                    if (to != p.ignore) {
+                        g = p.grad[(size_t)row * p.grad_stride] * p.scale;
+                        if (p.count) g /= *p.count;
+                        base = p.lse[row] * kLog2e;
+                        if (!ok || to < 0 || to >= p.V) g = CUDART_NAN_F;
+                        else target = (int)to - p.v0;
+                    }
+                }
+                const bool none = target == -1 && g == 0.f;   // (not a row that counts: nothing of it enters, whatever it holds)
+#pragma unroll 1
+                for (int cb = 0; cb < kTileN / 64; ++cb) {
+                    if (rows <= 0) break;
+                    uint32_t v[2][32], y[32];
+                    tmem_columns32(from + cb * 64, v[0]);
+                    tmem_columns32(from + cb * 64 + 32, v[1]);
+                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                    const int at = target - (n0 + cb * 64);
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) {
+                        float f[2];
+#pragma unroll
+                        for (int o = 0; o < 2; ++o) {
+                            const int col = 2 * e + o;
+                            const float s = exp2_fast(fmaf(__uint_as_float(v[col >> 5][col & 31]), p.c, -base));
+                            f[o] = none ? 0.f : (at == col ? s - 1.f : s) * g;
+                        }
+                        const __nv_bfloat162 b = __floats2bfloat162_rn(f[0], f[1]);
+                        y[e] = *reinterpret_cast<const uint32_t*>(&b);
+                    }
+                    store_64(blk, y, p.p, p.ldp, row0, rows, n0 + cb * 64, 64, true, lane);
+                }
+            } else if constexpr (KIND == kRows) {
+                const int rr = lane >> 3, ch = lane & 7;
+                float* const acc = p.acc + (size_t)(t / (tiles_m * tiles_n)) * p.M * p.ld_acc;
+#pragma unroll 1
+                for (int cb = 0; cb < kTileN / 32; ++cb) {
+                    const int n = n0 + cb * 32 + 4 * ch;
+                    if (n0 + cb * 32 >= p.ld_acc || rows <= 0) break;
+                    uint32_t v[32];
+                    tmem_columns32(from + cb * 32, v);
+                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+                    for (int c = 0; c < 8; ++c)
+                        *reinterpret_cast<uint4*>(blk + lane * 128 + ((c ^ (lane & 7)) << 4)) = make_uint4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+                    __syncwarp();
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const int r = 4 * e + rr;
+                        if (r >= rows || n >= p.ld_acc) break;
+                        float4 f = *reinterpret_cast<const float4*>(blk + r * 128 + ((ch ^ (r & 7)) << 4));
+                        float4* const to = reinterpret_cast<float4*>(acc + (size_t)(row0 + r) * p.ld_acc + n);
+                        if (!ok) f.x = f.y = f.z = f.w = CUDART_NAN_F;
+                        if (p.add) {
+                            const float4 o = *to;
+                            f.x += o.x; f.y += o.y; f.z += o.z; f.w += o.w;
+                        }
+                        *to = f;
+                    }
+                    __syncwarp();
+                }
+            } else {
+#pragma unroll 1
+                for (int cb = 0; cb < kTileN / 64; ++cb) {
+                    const int c0 = n0 + cb * 64;
+                    if (c0 >= p.N || rows <= 0) break;
+                    uint32_t v[2][32], y[32];
+                    tmem_columns32(from + cb * 64, v[0]);
+                    tmem_columns32(from + cb * 64 + 32, v[1]);
+                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) {
+                        const float lo = __uint_as_float(v[e >> 4][2 * e & 31]), hi = __uint_as_float(v[e >> 4][(2 * e & 31) + 1]);
+                        const __nv_bfloat162 b = __floats2bfloat162_rn(ok ? lo : CUDART_NAN_F, ok ? hi : CUDART_NAN_F);
+                        y[e] = *reinterpret_cast<const uint32_t*>(&b);
+                    }
+                    store_64(blk, y, p.out, p.N, row0, rows, c0, p.N - c0, p.wide, lane);
+                }
+            }
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(at_rank(&t_empty[it & 1u], 0)) : "memory");
+        }
+    }
+    if (!ok && lane == 0 && p.ran_out) {
+        *reinterpret_cast<volatile int*>(p.ran_out) = 1;
+        __threadfence_system();
+    }
+    __syncwarp();
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    cluster_sync_all();                                       // neither CTA's memory goes while the other still reads it or arrives there
+    if (warp == 1) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512));
+    }
+}
+
+// The tiles of a row joined, a warp per row; the last block to come sums the rows, in their order.
+constexpr int kJoinWarps = 8;
+__global__ void __launch_bounds__(32 * kJoinWarps) loss_join_kernel(const float2* __restrict__ part, const float* __restrict__ hit, int M, int V, int tiles, const void* targets,
+                                                                    int targets64, long long ignore, float c, float* loss, float* __restrict__ lse, float* __restrict__ totals,
+                                                                    unsigned* arrived) {
+    const int lane = threadIdx.x & 31, row = blockIdx.x * kJoinWarps + (threadIdx.x >> 5);
+    if (row < M) {
+        const float2* const p = part + (size_t)row * tiles;
+        float most = -CUDART_INF_F, sum = 0.f;
+        bool bad = false;
+        for (int i = lane; i < tiles; i += 32) {
+            const float2 x = p[i];
+            const float now = fmaxf(most, x.x);
+            bad = bad || x.y != x.y || x.x != x.x;
+            if (now > -CUDART_INF_F) sum = sum * exp2f(most - now) + x.y * exp2f(x.x - now);
+            most = now;
+        }
+#pragma unroll
+        for (int o = 16; o; o >>= 1) {
+            const float other = __shfl_xor_sync(0xffffffffu, most, o), add = __shfl_xor_sync(0xffffffffu, sum, o), now = fmaxf(most, other);
+            if (now > -CUDART_INF_F) sum = sum * exp2f(most - now) + add * exp2f(other - now);
+            most = now;
+        }
+        bad = __any_sync(0xffffffffu, bad);
+        if (lane == 0) {
+            const long long t = target_of(targets, targets64, row);
+            const float below = bad ? CUDART_NAN_F : log2f(sum);
+            lse[row] = (most + below) * kLn2;
+            // (the target's distance from the largest is taken before it meets the logarithm: losses near zero keep their digits)
+            loss[row] = t == ignore ? 0.f : t < 0 || t >= V ? CUDART_NAN_F : (below - fmaf(hit[row], c, -most)) * kLn2;
+        }
+    }
+    __shared__ bool last;
+    __shared__ int counts[kJoinWarps];
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) last = atomicAdd(arrived, 1u) == gridDim.x - 1;
+    __syncthreads();
+    if (!last) return;
+    __threadfence();
+    // every thread its rows in double precision, then a fixed tree
+    double s = 0.0;
+    int n = 0;
+    for (int i = threadIdx.x; i < M; i += 32 * kJoinWarps)
+        if (target_of(targets, targets64, i) != ignore) {
+            s += (double)__ldcg(loss + i);
+            ++n;
+        }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+        s += __shfl_xor_sync(0xffffffffu, s, o);
+        n += __shfl_xor_sync(0xffffffffu, n, o);
+    }
+    __shared__ double parts[kJoinWarps];
+    if (lane == 0) { parts[threadIdx.x >> 5] = s; counts[threadIdx.x >> 5] = n; }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        s = 0.0;
+        n = 0;
+        for (int i = 0; i < kJoinWarps; ++i) { s += parts[i]; n += counts[i]; }
+        totals[0] = (float)s;
+        totals[1] = (float)n;
+        totals[2] = n ? (float)(s / n) : 0.f;
+    }
+}
+
+// Rows as operands: out [TERMS][M][ld_out] bf16, zeros from K on.  TERMS 3: fp32 rows as three bf16 terms (24 bits).  targets: rows whose target is `ignore` are zeros
+// (what they hold, a NaN among it, stays out of the head's gradient).
+template <int TERMS, bool F32>
+__global__ void __launch_bounds__(256) loss_pack_kernel(const void* __restrict__ x, long long ld, int M, int K, __nv_bfloat16* __restrict__ out, int ld_out, const void* targets,
+                                                        int targets64, long long ignore) {
+    const int per_row = ld_out / 8;
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x, r = i / per_row;
+    if (r >= M) return;
+    const int k = (int)(i - r * per_row) * 8;
+    const bool out_of_it = targets && target_of(targets, targets64, (int)r) == ignore;
+    __nv_bfloat16 t[TERMS][8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        float v = 0.f;
+        if (k + e < K && !out_of_it) v = F32 ? reinterpret_cast<const float*>(x)[r * ld + k + e] : __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(x)[r * ld + k + e]);
+        t[0][e] = TERMS == 1 ? __float2bfloat16_rn(v) : __float2bfloat16_rz(v);
+        if (TERMS == 3) {                                     // rounded towards zero first: the largest numbers do not become infinities
+            const float f = __bfloat162float(t[0][e]), r1 = fabsf(f) <= 3.402823466e38f ? v - f : 0.f;
+            t[TERMS > 1][e] = __float2bfloat16_rn(r1);
+            t[TERMS - 1][e] = __float2bfloat16_rn(r1 - __bfloat162float(t[TERMS > 1][e]));
+        }
+    }
+#pragma unroll
+    for (int q = 0; q < TERMS; ++q) *reinterpret_cast<uint4*>(out + ((size_t)q * M + r) * ld_out + k) = *reinterpret_cast<const uint4*>(t[q]);
+}
+
+// dh = the sum of the shares of the contraction
+__global__ void __launch_bounds__(256) loss_rows_out_kernel(const float* __restrict__ acc, int splits, int M, int K, int ld, __nv_bfloat16* __restrict__ out, int wide) {
+    const int per_row = ld / 4;
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x, r = i / per_row;
+    if (r >= M) return;
+    const int k = (int)(i - r * per_row) * 4;
+    float4 v = *reinterpret_cast<const float4*>(acc + r * ld + k);
+    for (int s = 1; s < splits; ++s) {
+        const float4 o = *reinterpret_cast<const float4*>(acc + ((size_t)s * M + r) * ld + k);
+        v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
+    }
+    const __nv_bfloat16 h[4] = {__float2bfloat16_rn(v.x), __float2bfloat16_rn(v.y), __float2bfloat16_rn(v.z), __float2bfloat16_rn(v.w)};
+    __nv_bfloat16* const o = out + (size_t)r * K + k;
+    if (wide) {
+        *reinterpret_cast<uint2*>(o) = *reinterpret_cast<const uint2*>(h);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) if (k + e < K) o[e] = h[e];
+    }
+}
+
+// ---- host side -------------------------------------------------------------------------------------------------------------------------------
+
+// bf16 [rows][cols], ld elements apart, in boxes of box_rows x 64 columns
+bool bf16_map(CUtensorMap* map, const void* base, long long rows, long long cols, long long ld, int box_rows) {
+    const EncodeTiledFn enc = encode_tiled();
+    if (!enc) return false;
+    const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)ld * 2};
+    const cuuint32_t box[2] = {kBK, (cuuint32_t)box_rows}, estr[2] = {1, 1};
+    return enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int KIND, int TERMS>
+cudaError_t pairs_of(int dev, int* out) {
+    static std::atomic<int> known[64];
+    if (dev >= 0 && dev < 64 && (*out = known[dev].load(std::memory_order_relaxed)) > 0) return cudaSuccess;
+    const auto kernel = loss_product_kernel<KIND, TERMS>;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(2);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = Ring<TERMS>::kSmem;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = 2;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Ring<TERMS>::kSmem);
+    if (e == cudaSuccess) e = cudaOccupancyMaxActiveClusters(out, kernel, &cfg);
+    if (e != cudaSuccess) return e;
+    if (*out < 1) return cudaErrorNotSupported;
+    if (dev >= 0 && dev < 64) known[dev].store(*out, std::memory_order_relaxed);
+    return cudaSuccess;
+}
+
+template <int KIND, int TERMS>
+cudaError_t run_tiles(const CUtensorMap& a, const CUtensorMap& b, LossTiles p, int dev, cudaStream_t st) {
+    int pairs = 0;
+    const cudaError_t e = pairs_of<KIND, TERMS>(dev, &pairs);
+    if (e != cudaSuccess) return e;
+    p.polls = gemm_pair_polls();
+    p.ran_out = split_attention_ran_out(dev, st);
+    const long long tiles = (long long)((p.M + 255) / 256) * ((p.N + kTileN - 1) / kTileN) * (KIND == kRows ? p.splits : 1);
+    if (tiles > 0x3fffffffLL) return cudaErrorNotSupported;
+    loss_product_kernel<KIND, TERMS><<<2 * (int)std::min<long long>(tiles, pairs), kThreads, Ring<TERMS>::kSmem, st>>>(a, b, p);
+    return cudaGetLastError();
+}
+
+int padded(int K) { return (K + 7) / 8 * 8; }
+bool in_place(const void* x, long long ld) { return (reinterpret_cast<uintptr_t>(x) & 15) == 0 && ld % 8 == 0; }
+size_t up(size_t n) { return (n + 255) / 256 * 256; }
+
+template <int TERMS, bool F32>
+cudaError_t pack(const void* x, long long ld, int M, int K, void* out, const LossShape* counts, cudaStream_t st) {
+    const long long blocks = ((long long)M * (padded(K) / 8) + 255) / 256;
+    if (blocks > 0x7fffffffLL) return cudaErrorNotSupported;
+    loss_pack_kernel<TERMS, F32><<<(unsigned)blocks, 256, 0, st>>>(x, ld, M, K, reinterpret_cast<__nv_bfloat16*>(out), padded(K), counts ? counts->targets : nullptr,
+                                                                   counts ? counts->targets64 : 0, counts ? counts->ignore : 0);
+    ++extra_launches();
+    return cudaGetLastError();
+}
+
+// Shares of a contraction of `length`, none of them empty, where `most` are asked for
+int shares_of(int length, int most) {
+    const int kb = (length + kBK - 1) / kBK, per = (kb + most - 1) / most;
+    return (kb + per - 1) / per;
+}
+
+// What a call keeps in its workspace, one after the other
+struct Room {
+    size_t h = 0, w = 0, part = 0, hit = 0, arrived = 0, p = 0, acc = 0, all = 0;      // offsets
+    int piece = 0, splits = 1;                                                          // columns of a piece of the vocabulary, shares of dh's contraction
+};
+Room room_of(const LossShape& s, bool grad, bool rows, bool head) {
+    Room r;
+    size_t at = 0;
+    const auto take = [&](size_t bytes) { const size_t was = at; at += up(bytes); return was; };
+    const size_t row = (size_t)s.M * padded(s.K) * 2;
+    r.h = take(grad ? (head || !in_place(s.h, s.ldh) ? row : 0) : s.h_type == kTypeF32 ? 3 * row : in_place(s.h, s.ldh) ? 0 : row);
+    r.w = take(in_place(s.w, s.ldw) ? 0 : (size_t)s.V * padded(s.K) * 2);
+    if (!grad) {
+        r.part = take((size_t)s.M * ((s.V + kTileN - 1) / kTileN) * 8);
+        r.hit = take((size_t)s.M * 4);
+        r.arrived = take(4);
+    } else {
+        const long long all = (s.V + 255) / 256 * 256LL, fit = (64LL << 20) / 2 / s.M / 256 * 256;
+        r.piece = (int)std::min(all, std::max(4096LL, fit));
+        // shares of dh's contraction where its tiles leave most of the chip idle
+        const long long tiles = (long long)((s.M + 255) / 256) * ((s.K + 255) / 256);
+        while (r.splits < 16 && 2 * r.splits * tiles <= 74 && r.piece / kBK >= 16 * r.splits) r.splits *= 2;
+        r.splits = shares_of(r.piece, r.splits);
+        r.p = take((size_t)s.M * r.piece * 2);
+        r.acc = take(rows ? (size_t)r.splits * s.M * ((s.K + 3) / 4 * 4) * 4 : 0);
+    }
+    r.all = at;
+    return r;
+}
+
+LossTiles tiles_of(const LossShape& s) {
+    LossTiles p{};
+    p.splits = 1;
+    p.targets = s.targets; p.targets64 = s.targets64; p.ignore = s.ignore;
+    p.c = s.scale * kLog2e; p.scale = s.scale; p.V = s.V;
+    return p;
+}
+
+}  // namespace
+
+size_t loss_work_bytes(const LossShape& s) { return room_of(s, false, false, false).all; }
+size_t loss_grad_work_bytes(const LossShape& s, bool rows, bool head) { return room_of(s, true, rows, head).all; }
+
+cudaError_t launch_loss(const LossShape& s, float* loss, float* lse, float* totals, void* work, cudaStream_t st) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (take_ran_out(dev, st)) return cudaErrorLaunchTimeout;
+    const Room r = room_of(s, false, false, false);
+    unsigned char* const base = reinterpret_cast<unsigned char*>(work);
+    const void *h = s.h, *w = s.w;
+    long long ldh = s.ldh, ldw = s.ldw;
+    const bool f32 = s.h_type == kTypeF32;
+    if (f32 || !in_place(s.h, s.ldh)) {
+        h = base + r.h;
+        ldh = padded(s.K);
+        e = f32 ? pack<3, true>(s.h, s.ldh, s.M, s.K, base + r.h, nullptr, st) : pack<1, false>(s.h, s.ldh, s.M, s.K, base + r.h, nullptr, st);
+    }
+    if (e == cudaSuccess && !in_place(s.w, s.ldw)) {
+        w = base + r.w;
+        ldw = padded(s.K);
+        e = pack<1, false>(s.w, s.ldw, s.V, s.K, base + r.w, nullptr, st);
+    }
+    if (e != cudaSuccess) return e;
+    unsigned* const arrived = reinterpret_cast<unsigned*>(base + r.arrived);
+    CUtensorMap ma, mb;
+    if (!bf16_map(&ma, h, (long long)s.M * (f32 ? 3 : 1), s.K, ldh, 128) || !bf16_map(&mb, w, s.V, s.K, ldw, 128)) return cudaErrorNotSupported;
+    LossTiles p = tiles_of(s);
+    p.M = s.M; p.N = s.V; p.K = s.K;
+    p.part = reinterpret_cast<float2*>(base + r.part);
+    p.hit = reinterpret_cast<float*>(base + r.hit);
+    p.arrived = arrived;
+    e = f32 ? run_tiles<kStats, 3>(ma, mb, p, dev, st) : run_tiles<kStats, 1>(ma, mb, p, dev, st);
+    if (e != cudaSuccess) return e;
+    ++extra_launches();
+    loss_join_kernel<<<(s.M + kJoinWarps - 1) / kJoinWarps, 32 * kJoinWarps, 0, st>>>(p.part, p.hit, s.M, s.V, (s.V + kTileN - 1) / kTileN, s.targets, s.targets64, s.ignore,
+                                                                                    p.c, loss, lse, totals, arrived);
+    return cudaGetLastError();
+}
+
+cudaError_t launch_loss_grad(const LossShape& s, const float* lse, const float* grad, int grad_stride, const float* count, void* dh, void* dw, void* work, cudaStream_t st) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (take_ran_out(dev, st)) return cudaErrorLaunchTimeout;
+    const Room r = room_of(s, true, dh != nullptr, dw != nullptr);
+    unsigned char* const base = reinterpret_cast<unsigned char*>(work);
+    const void *h = s.h, *w = s.w;
+    long long ldh = s.ldh, ldw = s.ldw;
+    if (dw || !in_place(s.h, s.ldh)) {                        // (rows that do not count are zeros here)
+        h = base + r.h;
+        ldh = padded(s.K);
+        e = pack<1, false>(s.h, s.ldh, s.M, s.K, base + r.h, &s, st);
+    }
+    if (e == cudaSuccess && !in_place(s.w, s.ldw)) {
+        w = base + r.w;
+        ldw = padded(s.K);
+        e = pack<1, false>(s.w, s.ldw, s.V, s.K, base + r.w, nullptr, st);
+    }
+    if (e != cudaSuccess) return e;
+    __nv_bfloat16* const probs = reinterpret_cast<__nv_bfloat16*>(base + r.p);
+    float* const acc = reinterpret_cast<float*>(base + r.acc);
+    const int ld_acc = (s.K + 3) / 4 * 4;
+    CUtensorMap h_rows, w_rows, p_rows, h_cols, w_cols, p_cols;
+    // rows along the contraction, and (the last two products) channels of a row in boxes of 64 x 64
+    if (!bf16_map(&h_rows, h, s.M, s.K, ldh, 128) || !bf16_map(&w_rows, w, s.V, s.K, ldw, 128) || !bf16_map(&p_rows, probs, s.M, r.piece, r.piece, 128) ||
+        !bf16_map(&h_cols, h, s.M, s.K, ldh, kBK) || !bf16_map(&w_cols, w, s.V, s.K, ldw, kBK) || !bf16_map(&p_cols, probs, s.M, r.piece, r.piece, kBK))
+        return cudaErrorNotSupported;
+    for (int v0 = 0; v0 < s.V; v0 += r.piece) {
+        const int cols = std::min(r.piece, s.V - v0);
+        LossTiles p = tiles_of(s);
+        p.v0 = v0;
+        p.M = s.M; p.N = cols; p.K = s.K;
+        p.lse = lse; p.grad = grad; p.grad_stride = grad_stride; p.count = count;
+        p.p = probs; p.ldp = r.piece;
+        e = run_tiles<kProbs, 1>(h_rows, w_rows, p, dev, st);
+        if (e != cudaSuccess) return e;
+        ++extra_launches();
+        if (dh) {
+            LossTiles q = tiles_of(s);
+            q.v0 = v0;
+            q.M = s.M; q.N = s.K; q.K = cols;
+            q.splits = shares_of(cols, r.splits); q.acc = acc; q.ld_acc = ld_acc; q.add = v0 > 0;
+            e = run_tiles<kRows, 1>(p_rows, w_cols, q, dev, st);
+            if (e != cudaSuccess) return e;
+            ++extra_launches();
+        }
+        if (dw) {
+            LossTiles q = tiles_of(s);
+            q.M = cols; q.N = s.K; q.K = s.M;
+            q.out = reinterpret_cast<__nv_bfloat16*>(dw) + (size_t)v0 * s.K;
+            q.wide = s.K % 8 == 0 && (reinterpret_cast<uintptr_t>(dw) & 15) == 0;
+            e = run_tiles<kHead, 1>(p_cols, h_cols, q, dev, st);
+            if (e != cudaSuccess) return e;
+            ++extra_launches();
+        }
+    }
+    if (dh) {
+        const long long blocks = ((long long)s.M * (ld_acc / 4) + 255) / 256;
+        if (blocks > 0x7fffffffLL) return cudaErrorNotSupported;
+        loss_rows_out_kernel<<<(unsigned)blocks, 256, 0, st>>>(acc, r.splits, s.M, s.K, ld_acc, reinterpret_cast<__nv_bfloat16*>(dh),
+                                                              s.K % 4 == 0 && (reinterpret_cast<uintptr_t>(dh) & 7) == 0);
+        ++extra_launches();
+        e = cudaGetLastError();
+    }
+    --extra_launches();                                       // (the caller counts one)
+    return e;
+}
+
+}  // namespace lm

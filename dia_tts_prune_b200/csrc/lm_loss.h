@@ -1,0 +1,29 @@
+// lm_loss.h - cross entropy of rows under a head and its gradient, the logits in pieces that stay on the chip.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace lm {
+
+// z[i][j] = scale h_i . w_j; loss_i = log sum_j exp z[i][j] - z[i][target_i], zero where the target is `ignore`
+struct LossShape {
+    const void* h; int h_type; long long ldh;    // [M][K] fp32 or bf16
+    const void* w; long long ldw;                // [V][K] bf16
+    const void* targets; int targets64;          // [M] int64 or int32
+    long long ignore;
+    int M, V, K;
+    float scale;
+};
+// The operands that are laid out again in the workspace: rows that are fp32 or not of 16 bytes, a head whose rows are not
+size_t loss_work_bytes(const LossShape& s);
+// loss [M], lse [M]: log sum_j exp z[i][j]; totals [3]: the sum of the losses, how many rows count, their mean (0 where none does)
+cudaError_t launch_loss(const LossShape& s, float* loss, float* lse, float* totals, void* work, cudaStream_t st);
+
+// The gradient by rows (dh [M][K] bf16) and by the head (dw [V][K] bf16), either or both; h is bf16.  grad: of every loss, grad_stride floats apart (0: one for all);
+// count: divides it where not null (totals + 1 of a mean)
+size_t loss_grad_work_bytes(const LossShape& s, bool rows, bool head);
+cudaError_t launch_loss_grad(const LossShape& s, const float* lse, const float* grad, int grad_stride, const float* count, void* dh, void* dw, void* work,
+                             cudaStream_t st);
+
+}  // namespace lm

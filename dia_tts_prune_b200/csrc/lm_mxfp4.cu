@@ -174,7 +174,6 @@ constexpr int kStages = 5;
 constexpr int kThreads4 = 192;
 constexpr int kTurnBytes = 4 * 4096;
 constexpr int kSmem4 = kStages * kStageBytes + kTurnBytes + 1024 + 256;
-constexpr unsigned kPolls = 4000000u;                         // looks at a barrier until a wait has run out: a few seconds
 
 // scales of 128 rows x 128 channels in shared memory: 8 rows of 16 bytes after one another, no swizzle
 __device__ __forceinline__ uint64_t scale_desc(uint32_t smem_addr) {
@@ -387,7 +386,7 @@ cudaError_t launch_mxfp4_linear(Mxfp4Product p, void* work, cudaStream_t st) {
     cudaError_t e = current_sms(&dev, &sms);
     if (e != cudaSuccess) return e;
     p.ran_out = split_attention_ran_out(dev, st);
-    p.polls = kPolls;
+    p.polls = gemm_pair_polls();
     if (take_ran_out(dev, st)) return cudaErrorLaunchTimeout;
     uint8_t* const codes = reinterpret_cast<uint8_t*>(work);
     uint8_t* const scales = codes + (mx_code_bytes(p.M, p.K) + 127) / 128 * 128;

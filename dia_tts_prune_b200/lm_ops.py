@@ -1,4 +1,5 @@
-"""Operators of the language models for callers that hold rows of their own: matrices in 4 bits and their products.
+"""Operators of the language models for callers that hold rows of their own: matrices in 4 bits and their products, and the cross
+entropy of rows under a head with its gradient.
 
 They stand beside ``lm_engine.linear``: torch tensors on a CUDA device in, new tensors out, queued on the current stream of the tensors'
 device.  Workspaces come from torch's allocator for the length of a call, so calls on several streams and in captured graphs do not share
@@ -121,3 +122,91 @@ def linear_mxfp4(a: torch.Tensor, w: Mxfp4, out_dtype: torch.dtype | None = None
                                                   y.data_ptr(), _TYPES[out_dtype], M, w.rows, w.width, work.data_ptr() if need else None, need,
                                                   _stream(a.device)), "linear_mxfp4")
     return y
+
+
+def _loss_operands(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor):
+    _check_rows(hidden, "hidden", (torch.float32, torch.bfloat16))
+    _check_rows(weight, "weight", (torch.bfloat16,))
+    if not isinstance(targets, torch.Tensor):
+        raise TypeError("targets must be a tensor")
+    if targets.dtype not in (torch.int64, torch.int32):
+        raise TypeError(f"targets must be int64 or int32, not {targets.dtype}")
+    if hidden.dim() < 1 or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1]:
+        raise ValueError(f"hidden {tuple(hidden.shape)} and weight {tuple(weight.shape)} do not share a width")
+    if targets.shape != hidden.shape[:-1]:
+        raise ValueError(f"targets {tuple(targets.shape)} do not go with hidden {tuple(hidden.shape)}")
+    if weight.device != hidden.device or targets.device != hidden.device:
+        raise ValueError("hidden, weight and targets must live on one device")
+    if not weight.numel():
+        raise ValueError("weight is empty")
+
+
+class _LinearCrossEntropy(torch.autograd.Function):
+    """Losses of rows, or (mean, sum) their total; rows are two-dimensional here."""
+
+    @staticmethod
+    def forward(ctx, hidden, weight, targets, scale, ignore_index, reduction):
+        lib = _lm_lib.load()
+        (M, K), V, device = hidden.shape, weight.shape[0], hidden.device
+        loss, lse, totals = (torch.empty(n, dtype=torch.float32, device=device) for n in (M, M, 3))
+        h, w, t = _as_rows(hidden), _as_rows(weight), targets.contiguous()
+        args = h.data_ptr(), _TYPES[h.dtype], h.stride(0), w.data_ptr(), w.stride(0)
+        need = lib.lm_b200_op_loss_work_bytes(*args, M, V, K)
+        work = torch.empty(need, dtype=torch.uint8, device=device)
+        with torch.cuda.device(device):
+            _lm_lib.check(lib.lm_b200_op_loss(*args, t.data_ptr(), t.dtype == torch.int64, ignore_index, M, V, K, scale, loss.data_ptr(),
+                                              lse.data_ptr(), totals.data_ptr(), work.data_ptr(), need, _stream(device)), "loss")
+        ctx.save_for_backward(hidden, weight, t, lse)
+        # (the count stands beside the result, which may be changed in place: not a saved tensor)
+        ctx.args = scale, ignore_index, totals[1:2].detach() if reduction == "mean" else None
+        return loss if reduction == "none" else totals[2 if reduction == "mean" else 0]
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        hidden, weight, t, lse = ctx.saved_tensors
+        scale, ignore_index, count = ctx.args
+        need_h, need_w = ctx.needs_input_grad[:2]
+        if hidden.dtype != torch.bfloat16:
+            raise TypeError("gradients need hidden in bfloat16")
+        lib = _lm_lib.load()
+        (M, K), V, device = hidden.shape, weight.shape[0], hidden.device
+        h, w, grad = _as_rows(hidden), _as_rows(weight), grad.to(torch.float32)
+        if grad.dim() and grad.stride(0) < 0:
+            grad = grad.contiguous()
+        dh = torch.empty((M, K), dtype=hidden.dtype, device=device) if need_h else None
+        dw = torch.empty((V, K), dtype=weight.dtype, device=device) if need_w else None
+        args = h.data_ptr(), h.stride(0), w.data_ptr(), w.stride(0)
+        need = lib.lm_b200_op_loss_grad_work_bytes(*args, M, V, K, need_h, need_w)
+        work = torch.empty(need, dtype=torch.uint8, device=device)
+        with torch.cuda.device(device):
+            _lm_lib.check(lib.lm_b200_op_loss_grad(
+                *args, t.data_ptr(), t.dtype == torch.int64, ignore_index, M, V, K, scale, lse.data_ptr(), grad.data_ptr(),
+                grad.stride(0) if grad.dim() else 0, count.data_ptr() if count is not None else None,
+                dh.data_ptr() if need_h else None, dw.data_ptr() if need_w else None, work.data_ptr(), need, _stream(device)), "loss_grad")
+        return dh, dw, None, None, None, None
+
+
+def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, *, scale: float = 1.0,
+                         ignore_index: int = -100, reduction: str = "mean") -> torch.Tensor:
+    """The cross entropy of ``targets [...]`` under the logits ``scale * hidden [..., width] @ weight [vocab, width]^T``, float32, without
+    the logits in memory: ``"none"`` every token's loss, ``"sum"`` or ``"mean"`` over the tokens whose target is not ``ignore_index`` (0
+    where there is none).  A token that does not count has loss 0; one whose target is neither ``ignore_index`` nor in ``[0, vocab)`` NaN.
+
+    ``weight`` is bfloat16; ``hidden`` is bfloat16, or float32, which is then multiplied as it is (24 bits) and has no gradient.  The
+    gradients by ``hidden`` and ``weight`` take the vocabulary in pieces; rows that do not count have no part in them, whatever they hold.
+    """
+    _loss_operands(hidden, weight, targets)
+    if reduction not in ("none", "sum", "mean"):
+        raise ValueError("reduction must be 'none', 'sum' or 'mean'")
+    scale, ignore_index = float(scale), int(ignore_index)
+    if not 0.0 < scale < float("inf"):
+        raise ValueError("scale must be positive and finite")
+    if hidden.dtype == torch.float32 and torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
+        raise ValueError("gradients need hidden in bfloat16")
+    if not targets.numel():
+        rows = hidden.new_zeros(targets.shape, dtype=torch.float32)
+        return rows if reduction == "none" else rows.sum()
+    K = hidden.shape[-1]
+    loss = _LinearCrossEntropy.apply(hidden.reshape(-1, K), weight, targets.reshape(-1), scale, ignore_index, reduction)
+    return loss.view(targets.shape) if reduction == "none" else loss

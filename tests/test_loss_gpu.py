@@ -1,0 +1,197 @@
+"""The cross entropy of rows under a head and its gradient (csrc/lm_loss.cu) against the definition in 64 bits."""
+
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def operands(m, v, k, seed, dtype=torch.bfloat16, ignored=0.2, lean=6.0):
+    g = torch.Generator().manual_seed(seed)
+    w = (torch.randn(v, k, generator=g) / k ** 0.5).bfloat16()
+    t = torch.randint(0, v, (m,), generator=g)
+    h = torch.randn(m, k, generator=g) + lean * torch.rand(m, 1, generator=g) * w[t].float()
+    t[torch.rand(m, generator=g) < ignored] = -100
+    return h.to(dtype).cuda(), w.cuda(), t.cuda()
+
+
+class Exact:
+    """Losses, probabilities and gradients in 64 bits, and how far off the kernels' may be.
+
+    A logit is a sum of exact products; the tensor core adds 16 at a time to a float32 sum and cuts off, at most 2^-22 of the magnitudes
+    so far at each of K / 16 steps (float32 rows: three times as many, and 2^-22 of each product beyond their three terms): ``dz``.  A loss
+    moves by twice the largest of them, by 2^-20 for the exponentials and logarithms and by a few roundings of its parts."""
+
+    def __init__(self, h, w, t, scale=1.0):
+        self.h, self.w, t = h.detach().double().cpu(), w.detach().double().cpu(), t.cpu().long()
+        self.keep, self.scale, k = t != -100, scale, h.shape[1]
+        z = scale * self.h @ self.w.T
+        self.steps = (k / 16 + 2) * (3 if h.dtype == torch.float32 else 1) * 2.0 ** -22
+        self.dz = self.steps * scale * (self.h.abs() @ self.w.abs().T).amax(1)
+        logp, at = torch.log_softmax(z, 1), torch.where(self.keep, t, 0)[:, None]
+        self.loss = torch.where(self.keep, -logp.gather(1, at)[:, 0], 0.0)
+        self.loss_off = torch.where(self.keep, 2 * self.dz + 2.0 ** -20 + 2.0 ** -22 * (z.abs().amax(1) + self.loss), 0.0)
+        self.p, self.onehot = logp.exp(), torch.zeros_like(z).scatter_(1, at, 1.0)
+
+    def gradient(self, g):
+        """(by rows, by the head) and their bounds: P is off by 2^-8 of itself (bfloat16) and by its probability's 4 dz + 2^-18; the sums of V
+        (or M) products lose as the logits do, in pieces; and the results are bfloat16."""
+        g = (g.double().cpu() * self.keep * self.scale)[:, None]
+        P = (self.p - self.onehot) * g
+        dP = 2.0 ** -8 * P.abs() + (self.p * g).abs() * (4 * self.dz[:, None] + 2.0 ** -18) + P.abs() * 2.0 ** -18
+        out = []
+        for a, da, b in ((P, dP, self.w), (P.T, dP.T, self.h)):
+            want, lost = a @ b, (a.shape[1] / 16 + 2) * 2.0 ** -22
+            out.append((want, 1.01 * (da @ b.abs()) + lost * (a.abs() @ b.abs()) + 2.0 ** -8 * want.abs() + 2.0 ** -133))
+        return out
+
+
+def within(got, want, bound):
+    off = (got.detach().double().cpu() - want).abs() - bound
+    assert not off.isnan().any() and off.max() <= 0, float(off.max())
+
+
+SIZES = [(1, 1, 1), (1, 2, 8), (1, 256, 64), (2, 257, 65), (3, 300, 52), (127, 64, 128), (129, 1000, 100), (256, 511, 72), (257, 1025, 200), (5, 20000, 64),
+         (300, 9000, 96), (40, 640, 2048), (700, 300, 1001),
+         (8200, 4500, 40)]                                        # two pieces of the vocabulary
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("m,v,k", SIZES)
+def test_losses(m, v, k, dtype):
+    from dia_tts_prune_b200.lm_ops import linear_cross_entropy
+    h, w, t = operands(m, v, k, m + v, dtype)
+    for scale in (1.0, 0.25):
+        e = Exact(h, w, t, scale)
+        within(linear_cross_entropy(h, w, t, scale=scale, reduction="none"), e.loss, e.loss_off)
+        n = max(int(e.keep.sum()), 1)
+        for reduction, by in (("sum", 1), ("mean", n)):
+            got = linear_cross_entropy(h, w, t.int(), scale=scale, reduction=reduction)
+            within(got, e.loss.sum() / by, e.loss_off.sum() / by + 2.0 ** -23 * e.loss.sum() / by)
+
+
+@pytest.mark.parametrize("m,v,k", SIZES)
+def test_gradients(m, v, k):
+    from dia_tts_prune_b200.lm_ops import linear_cross_entropy
+    h, w, t = operands(m, v, k, 2 * m + v)
+    h.requires_grad_(True), w.requires_grad_(True)
+    e = Exact(h, w, t, 0.5)
+    loss = linear_cross_entropy(h, w, t, scale=0.5)
+    dh, dw = torch.autograd.grad(loss, (h, w))
+    n = max(int(e.keep.sum()), 1)
+    (want_h, off_h), (want_w, off_w) = e.gradient(torch.full((m,), 1.0 / n))
+    assert dh.dtype == dw.dtype == torch.bfloat16
+    within(dh, want_h, off_h)
+    within(dw, want_w, off_w)
+    # every token's own factor, through an expanded and a strided gradient, one input at a time
+    g = torch.randn(m, generator=torch.Generator().manual_seed(m)).cuda()
+    (want_h, off_h), (want_w, off_w) = e.gradient(g)
+    loss = linear_cross_entropy(h, w.detach(), t, scale=0.5, reduction="none")
+    within(torch.autograd.grad(loss, h, torch.stack([g, g], 1)[:, 0])[0], want_h, off_h)
+    loss = linear_cross_entropy(h.detach(), w, t, scale=0.5, reduction="none")
+    within(torch.autograd.grad(loss, w, g)[0], want_w, off_w)
+    loss = linear_cross_entropy(h, w, t, scale=0.5, reduction="none")
+    (want_h, off_h), _ = e.gradient(torch.ones(m))
+    within(torch.autograd.grad(loss.sum(), h)[0], want_h, off_h)
+
+
+def test_gradient_against_differences():
+    """Central differences of the loss in 64 bits along random directions, and the gradient's own product with them: the two differ by the
+    gradient's bound (see Exact) times the direction and by the third derivative's step^2 / 6 < 1e-6 of a loss whose logits move by less than one."""
+    from dia_tts_prune_b200.lm_ops import linear_cross_entropy
+    h, w, t = operands(33, 700, 48, 5)
+    h.requires_grad_(True), w.requires_grad_(True)
+    dh, dw = torch.autograd.grad(linear_cross_entropy(h, w, t, reduction="sum"), (h, w))
+    e = Exact(h, w, t)
+    (_, off_h), (_, off_w) = e.gradient(torch.ones(33))
+
+    def loss(a, b):
+        return torch.nn.functional.cross_entropy(a @ b.T, t.cpu(), reduction="sum")
+
+    g = torch.Generator().manual_seed(0)
+    for _ in range(4):
+        u, s = torch.randn(e.h.shape, generator=g).double(), 1e-4
+        slope = (loss(e.h + s * u, e.w) - loss(e.h - s * u, e.w)) / (2 * s)
+        assert abs(slope - (dh.double().cpu() * u).sum()) <= (off_h * u.abs()).sum() + 1e-4
+        u = torch.randn(e.w.shape, generator=g).double()
+        slope = (loss(e.h, e.w + s * u) - loss(e.h, e.w - s * u)) / (2 * s)
+        assert abs(slope - (dw.double().cpu() * u).sum()) <= (off_w * u.abs()).sum() + 1e-4
+
+
+def test_rows_that_do_not_count_and_bad_targets():
+    from dia_tts_prune_b200.lm_ops import linear_cross_entropy
+    h, w, t = operands(40, 500, 64, 7, ignored=0.0)
+    t[3], t[17], t[39] = -100, -100, -100
+    clean = h.clone()
+    h[3], h[17, 5], h[39, 0] = math.nan, math.inf, -math.inf
+    clean[[3, 17, 39]] = 0
+    a, b = h.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    loss = linear_cross_entropy(a, b, t)
+    dh, dw = torch.autograd.grad(loss, (a, b))
+    a0, b0 = clean.requires_grad_(True), w.clone().requires_grad_(True)
+    loss0 = linear_cross_entropy(a0, b0, t)
+    dh0, dw0 = torch.autograd.grad(loss0, (a0, b0))
+    assert loss.isfinite() and torch.equal(loss, loss0) and torch.equal(dh, dh0) and torch.equal(dw, dw0) and not dh[[3, 17, 39]].any()
+    # nothing counts: zero, with gradients of zeros
+    none = torch.full_like(t, -100)
+    loss = linear_cross_entropy(a, b, none)
+    dh, dw = torch.autograd.grad(loss, (a, b))
+    assert loss == 0 and not dh.any() and not dw.any()
+    assert linear_cross_entropy(a, b, none, reduction="sum") == 0 and not linear_cross_entropy(a, b, none, reduction="none").any()
+    # a target outside the vocabulary shows, in its row alone
+    bad = t.clone()
+    bad[5], bad[6] = 500, -1
+    rows = linear_cross_entropy(a0, b0, bad, reduction="none")
+    assert rows.isnan().nonzero()[:, 0].tolist() == [5, 6]
+    dh, = torch.autograd.grad(rows[:5].sum() + rows[7:].sum(), a0)
+    assert torch.equal(dh[0], torch.autograd.grad(linear_cross_entropy(a0, b0, t, reduction="sum"), a0)[0][0])
+    # another number for the rows that do not count
+    assert torch.equal(linear_cross_entropy(a0, b0, torch.where(t == -100, 7, t), ignore_index=7, reduction="none")[3], rows[3])
+
+
+def test_infinities_and_far_logits():
+    """Logits of hundreds, a head row of minus infinities (probability zero) and a loss next to zero, which keeps its digits."""
+    from dia_tts_prune_b200.lm_ops import linear_cross_entropy
+    h, w, t = operands(20, 400, 64, 8, ignored=0.0)
+    far = (h.float() * 64).bfloat16()
+    e = Exact(far, w, t)
+    within(linear_cross_entropy(far, w, t, reduction="none"), e.loss, e.loss_off)
+    pos = h.abs() + 0.5
+    w2 = w.clone()
+    w2[11] = -math.inf
+    w2[64:96] = -math.inf                                          # (a whole block of columns)
+    t2 = torch.where((t == 11) | ((t >= 64) & (t < 96)), 0, t)
+    kept = torch.tensor([j for j in range(400) if j != 11 and not 64 <= j < 96])
+    at = torch.searchsorted(kept, t2.cpu())
+    e = Exact(pos, w[kept.cuda()], at)
+    within(linear_cross_entropy(pos, w2, t2, reduction="none"), e.loss, e.loss_off)
+    sure, one = torch.zeros(1, 64, dtype=torch.bfloat16, device="cuda"), torch.zeros(3, 64, dtype=torch.bfloat16, device="cuda")
+    sure[0, 0], one[1, 0] = 16.0, 1.0
+    got = linear_cross_entropy(sure, one, torch.tensor([1], device="cuda"), reduction="none")
+    want = math.log1p(2 * math.exp(-16.0))                         # 2.25e-7; float32's sum 1 + that is off by 2^-24 (6e-8) at most
+    assert abs(float(got) - want) <= 2.0 ** -23
+
+
+def test_strides_leading_dimensions_and_empty():
+    from dia_tts_prune_b200.lm_ops import linear_cross_entropy
+    h, w, t = operands(24, 300, 104, 9)
+    want = linear_cross_entropy(h, w, t, reduction="none")
+    big = torch.zeros(24, 333, dtype=torch.bfloat16, device="cuda")
+    big[:, 8:112] = h
+    wide = torch.zeros(300, 120, dtype=torch.bfloat16, device="cuda")
+    wide[:, :104] = w
+    odd = torch.zeros(600, 107, dtype=torch.bfloat16, device="cuda")
+    odd[::2, 1:105] = w
+    for a in (big[:, 8:112], h.T.contiguous().T):
+        for b in (wide[:, :104], odd[::2, 1:105], w.T.contiguous().T):
+            assert torch.equal(linear_cross_entropy(a, b, t, reduction="none"), want)
+            x, y = a.detach().requires_grad_(True), b.detach().requires_grad_(True)
+            p, q = h.clone().requires_grad_(True), w.clone().requires_grad_(True)
+            for got, ref in zip(torch.autograd.grad(linear_cross_entropy(x, y, t), (x, y)), torch.autograd.grad(linear_cross_entropy(p, q, t), (p, q))):
+                assert torch.equal(got, ref)
+    assert torch.equal(linear_cross_entropy(h.view(4, 6, 104), w, t.view(4, 6), reduction="none"), want.view(4, 6))
+    assert torch.equal(linear_cross_entropy(h[0], w, t[0], reduction="none"), want[0])
+    assert linear_cross_entropy(h[:0], w, t[:0], reduction="none").shape == (0,)
+    assert linear_cross_entropy(h[:0], w, t[:0]) == 0
