@@ -1761,13 +1761,13 @@ size_t lm_b200_op_loss_work_bytes(const void* h, int h_type, int64_t ldh, const 
 }
 
 int lm_b200_op_loss(const void* h, int h_type, int64_t ldh, const void* W, int64_t ldw, const void* targets, int targets64, int64_t ignore, int M, int V, int K, float scale,
-                    float* loss, float* lse, float* totals, void* work, size_t work_bytes, void* stream) {
+                    float* loss, float* kept, float* totals, void* work, size_t work_bytes, void* stream) {
     lm::LossShape s;
-    if (!loss_shape(s, h, h_type, ldh, W, ldw, M, V, K) || !targets || !(scale > 0.f) || !std::isfinite(scale) || !loss || !lse || !totals || !work || !aligned(work, 256) ||
+    if (!loss_shape(s, h, h_type, ldh, W, ldw, M, V, K) || !targets || !(scale > 0.f) || !std::isfinite(scale) || !kept || !totals || !work || !aligned(work, 256) ||
         work_bytes < lm::loss_work_bytes(s))
         return LM_B200_EINVAL;
     s.targets = targets; s.targets64 = targets64; s.ignore = ignore; s.scale = scale;
-    LCK(lm::launch_loss(s, loss, lse, totals, work, S(stream)));
+    LCK(lm::launch_loss(s, loss, kept, totals, work, S(stream)));
     return LM_B200_OK;
 }
 
@@ -1777,13 +1777,13 @@ size_t lm_b200_op_loss_grad_work_bytes(const void* h, int64_t ldh, const void* W
 }
 
 int lm_b200_op_loss_grad(const void* h, int64_t ldh, const void* W, int64_t ldw, const void* targets, int targets64, int64_t ignore, int M, int V, int K, float scale,
-                         const float* lse, const float* grad, int grad_stride, const float* count, void* dh, void* dW, void* work, size_t work_bytes, void* stream) {
+                         const float* kept, const float* grad, int grad_stride, const float* count, void* dh, void* dW, void* work, size_t work_bytes, void* stream) {
     lm::LossShape s;
-    if (!loss_shape(s, h, LM_B200_BF16, ldh, W, ldw, M, V, K) || !targets || !(scale > 0.f) || !std::isfinite(scale) || !lse || !grad || grad_stride < 0 || (!dh && !dW) ||
+    if (!loss_shape(s, h, LM_B200_BF16, ldh, W, ldw, M, V, K) || !targets || !(scale > 0.f) || !std::isfinite(scale) || !kept || !grad || grad_stride < 0 || (!dh && !dW) ||
         !work || !aligned(work, 256) || work_bytes < lm::loss_grad_work_bytes(s, dh != nullptr, dW != nullptr))
         return LM_B200_EINVAL;
     s.targets = targets; s.targets64 = targets64; s.ignore = ignore; s.scale = scale;
-    LCK(lm::launch_loss_grad(s, lse, grad, grad_stride, count, dh, dW, work, S(stream)));
+    LCK(lm::launch_loss_grad(s, kept, lm::LossGrad{grad, grad_stride, count}, dh, dW, work, S(stream)));
     return LM_B200_OK;
 }
 

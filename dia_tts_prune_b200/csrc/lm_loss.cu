@@ -1,10 +1,13 @@
 // lm_loss.cu - cross entropy of rows h [M][K] under a head w [V][K], and its gradient, without the logits in memory.
 //
-//   z = scale h w^T,  loss_i = log sum_j exp z_ij - z_i,target        P = (softmax(z) - onehot) g scale,  dh = P w,  dw = P^T h
+//   z = scale h w^T,  loss_i = log sum_j exp z_ij - z_i,target        P = softmax(z) - onehot,  dh_i = scale g_i P_i w,  dw = P^T (scale g h)
 //
 // Forward: one product whose epilogue keeps of a 256 x 256 tile of logits, per row, the largest one, the sum of the exponentials below it and the target's, all in fp32;
 // a second kernel joins the tiles of a row.  Backward: the vocabulary goes in pieces.  The product is taken again for a piece, its epilogue turns logits into P (bf16, a
-// piece of at most 64 MB or 4096 columns: it stays in L2), and two products take P to dh (fp32 sums over the pieces) and to the piece's rows of dw.
+// piece of at most 64 MB or 4096 columns: it stays in L2), and two products take P to dh (fp32 sums over the pieces) and to the piece's rows of dw.  P is rounded without
+// g: 1 - p of a row's target, which is most of its gradient, then lies just below a power of two where steps are fine, and the roundings of the rows do not go one way
+// (8192 rows: 1.7e-3 to 1.9e-3 of the gradients' norm, of which the results' own rounding is 1.66e-3; with g inside 3.0e-3).  One g for all rows multiplies the sums; rows with
+// their own take it into h for dw (rounded to bf16) and behind the sums for dh.
 //
 // All four are one kernel on pairs of SMs: a cluster of two CTAs owns a 256 x 256 tile, tcgen05.mma (cta_group::2) multiplies the 256 rows of both by the 256 columns of
 // both, and the accumulators (two per CTA: a tile is taken out while the next is multiplied) live in tensor memory.
@@ -32,12 +35,13 @@ using namespace dia;
 enum Kind { kStats, kProbs, kRows, kHead };
 
 constexpr int kTileN = 256, kBK = 64, kTileBytes = 128 * kBK * 2;          // 16 KB: 128 rows of an operand, 64 of the contraction
-constexpr int kThreads = 192, kStagesMost = 6, kTurn = 4 * 4096;
+constexpr int kWarps = 8, kThreads = 64 + 32 * kWarps, kStagesMost = 6, kTurn = kWarps * 4096;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 template <int TERMS>
 struct Ring {
     static constexpr int kStage = (TERMS + 1) * kTileBytes, kStages = TERMS == 1 ? 6 : 3;
+    static constexpr int kChunk = TERMS == 1 ? 16 : 8;       // kStats: k-blocks of an accumulator
     static constexpr int kSmem = kStages * kStage + kTurn + 1024 + 256;
 };
 
@@ -47,11 +51,12 @@ struct LossTiles {
     const void* targets; int targets64; long long ignore;
     float c;                         // scale log2(e)
     unsigned* arrived;               // kStats: set to zero for the kernel that joins the tiles
-    float2* part; float* hit;        // kStats: [M][column tiles] largest c z and sum of 2^(c z - it); [M] z of the target
-    const float *lse, *grad, *count; int grad_stride; float scale; int v0, V;      // kProbs: columns v0 .. of the head
+    float2* part; float* hit;        // kStats: [M][2 column tiles] largest c z and sum of 2^(c z - it); [M] z of the target
+    const float2* kept; int v0, V;   // kProbs: [M] lse and loss; columns v0 .. of the head
     __nv_bfloat16* p; int ldp;
     float* acc; int ld_acc, add;     // kRows: [splits][M][ld_acc]; add: to what is there
     __nv_bfloat16* out; int wide;    // kHead: [M][N]; wide: 16-byte stores
+    const float *grad, *count; float scale;        // kHead: what the sums are multiplied by (grad null: nothing)
     int* ran_out;
     unsigned polls;
 };
@@ -104,7 +109,8 @@ template <int KIND, int TERMS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 loss_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ LossTiles p) {
     constexpr bool kAmn = KIND == kHead, kBmn = KIND == kRows || KIND == kHead;
-    constexpr int kStage = Ring<TERMS>::kStage, kStages = Ring<TERMS>::kStages;
+    constexpr bool kStats_ = KIND == kStats;
+    constexpr int kStage = Ring<TERMS>::kStage, kStages = Ring<TERMS>::kStages, kChunk = Ring<TERMS>::kChunk;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     unsigned char* turn = smem + kStages * kStage;
@@ -126,7 +132,7 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
     if (KIND == kStats && blockIdx.x == 0 && threadIdx.x == 0) *p.arrived = 0u;
     if (threadIdx.x == 0) {
         for (int i = 0; i < kStages; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
-        for (int i = 0; i < 2; ++i) { mbar_init(&t_full[i], 1); mbar_init(&t_empty[i], 8); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&t_full[i], 1); mbar_init(&t_empty[i], 2 * kWarps); }
         fence_mbar_init();
     }
     if (warp == 1) {
@@ -173,13 +179,16 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
             // fp32 accumulators, bf16 operands, which of them are MN-major, N = 256, M = 256
             const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((kAmn ? 1u : 0u) << 15) | ((kBmn ? 1u : 0u) << 16) | ((uint32_t)(kTileN >> 3) << 17) | (16u << 24);
             constexpr uint32_t a_step = kAmn ? 2048 >> 4 : 2, b_step = kBmn ? 2048 >> 4 : 2;        // 16 of the contraction, in descriptor units
-            unsigned i = 0, it = 0;
-            for (int t = pair; t < n_tiles && ok; t += pairs, ++it) {
-                if (!pair_wait(&t_empty[it & 1u], ((it >> 1) & 1u) ^ 1u, p.polls)) { ok = false; break; }
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint32_t d = tmem_base + (it & 1u) * kTileN;
+            unsigned i = 0, it = 0;                           // k-blocks and uses of an accumulator so far
+            for (int t = pair; t < n_tiles && ok; t += pairs) {
                 const int kb0 = first_kb(t), kb1 = last_kb(t);
                 for (int kb = kb0; kb < kb1; ++kb, ++i) {
+                    const bool first = kStats_ ? kb % kChunk == 0 : kb == kb0, last = kb == kb1 - 1 || (kStats_ && kb % kChunk == kChunk - 1);
+                    if (first) {
+                        if (!pair_wait(&t_empty[it & 1u], ((it >> 1) & 1u) ^ 1u, p.polls)) { ok = false; break; }
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    }
+                    const uint32_t d = tmem_base + (it & 1u) * kTileN;
                     const unsigned s = i % kStages;
                     if (!pair_wait(&full[s], (i / kStages) & 1u, p.polls)) { ok = false; break; }
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -192,78 +201,100 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                             const uint64_t adesc = kAmn ? umma_desc_mn(a_at) : umma_desc(a_at);
 #pragma unroll
                             for (int j = 0; j < kBK / 16; ++j)
-                                umma_bf16_pair(d, adesc + a_step * j, bdesc + b_step * j, idesc, (u | j) != 0 || kb != kb0 ? 1u : 0u);
+                                umma_bf16_pair(d, adesc + a_step * j, bdesc + b_step * j, idesc, (u | j) != 0 || !first ? 1u : 0u);
                         }
                         umma_commit_pair(&empty[s]);
-                        if (kb == kb1 - 1) umma_commit_pair(&t_full[it & 1u]);
+                        if (last) umma_commit_pair(&t_full[it & 1u]);
                     }
                     __syncwarp();
+                    if (last) ++it;
                 }
             }
         }
     } else {
-        const int q = warp & 3;
+        const int q = warp & 3, c_half = (warp - 2) >> 2 << 7;               // (a warp reads the 32 lanes of its number mod 4) and its half of the columns
         unsigned char* const blk = turn + (warp - 2) * 4096;
+        float factor = 1.f;
+        if (KIND == kHead && p.grad) {
+            factor = *p.grad * p.scale;
+            if (p.count) factor /= fmaxf(*p.count, 1.f);
+        }
         unsigned it = 0;
-        for (int t = pair; t < n_tiles; t += pairs, ++it) {
-            const int tn = t / tiles_m % tiles_n, n0 = tn * kTileN, row0 = t % tiles_m * 256 + (int)rank * 128 + q * 32, rows = min(32, p.M - row0), row = row0 + lane;
+        const auto taken = [&]() {                            // this warp has read the accumulator
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(at_rank(&t_empty[it & 1u], 0)) : "memory");
+            ++it;
+        };
+        for (int t = pair; t < n_tiles; t += pairs) {
+            const int tn = t / tiles_m % tiles_n, n0 = tn * kTileN + c_half, row0 = t % tiles_m * 256 + (int)rank * 128 + q * 32, rows = min(32, p.M - row0);
+            const int row = row0 + lane;
             const bool mine = row < p.M;
-            ok = ok && pair_wait(&t_full[it & 1u], (it >> 1) & 1u, p.polls);
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const uint32_t from = tmem_base + ((uint32_t)(q * 32) << 16) + (it & 1u) * kTileN;
+            const auto from = [&]() { return tmem_base + ((uint32_t)(q * 32) << 16) + (it & 1u) * kTileN + c_half; };
+            const auto wait = [&]() {
+                ok = ok && pair_wait(&t_full[it & 1u], (it >> 1) & 1u, p.polls);
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            };
             if constexpr (KIND == kStats) {
                 const long long target = mine ? target_of(p.targets, p.targets64, row) : -1;
-                float most = -CUDART_INF_F, sum = 0.f;        // of c z, of 2^(c z - most)
-#pragma unroll 1
-                for (int cb = 0; cb < kTileN / 32; ++cb) {
-                    const int c0 = n0 + cb * 32;
-                    if (c0 >= p.N || rows <= 0) break;        // (uniform)
-                    uint32_t v[32];
-                    tmem_columns32(from + cb * 32, v);
-                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                    if (c0 + 32 > p.N) {
+                // The tensor core cuts its sum off at every step, so an accumulator lives for a piece of the contraction and the pieces meet in registers.
+                float z[128];
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) if (c0 + e >= p.N) v[e] = __float_as_uint(-CUDART_INF_F);
+                for (int e = 0; e < 128; ++e) z[e] = 0.f;
+                for (int kb = 0; kb < kb_all; kb += kChunk) {
+                    wait();
+#pragma unroll
+                    for (int cb = 0; cb < 4; ++cb) {
+                        uint32_t v[32];
+                        tmem_columns32(from() + cb * 32, v);
+                        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) z[cb * 32 + e] += __uint_as_float(v[e]);
                     }
-                    float top[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) top[e & 3] = fmaxf(top[e & 3], __uint_as_float(v[e]));
-                    const float now = fmaxf(most, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * p.c);
-                    const float below = now == -CUDART_INF_F ? 0.f : now;        // (nothing but minus infinities so far)
-                    float add[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) add[e & 3] += exp2_fast(fmaf(__uint_as_float(v[e]), p.c, -below));
-                    sum = (most == -CUDART_INF_F ? 0.f : sum * exp2_fast(most - now)) + ((add[0] + add[1]) + (add[2] + add[3]));
-                    most = now;
-                    if (target >= c0 && target < c0 + 32 && target < p.N) {
-                        float z = 0.f;
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) z = target == c0 + e ? __uint_as_float(v[e]) : z;
-                        p.hit[row] = ok ? z : CUDART_NAN_F;
-                    }
+                    taken();
                 }
-                if (mine) p.part[(size_t)row * tiles_n + tn] = ok ? make_float2(most, sum) : make_float2(CUDART_NAN_F, CUDART_NAN_F);      // (no result)
+                if (mine && target >= n0 && target < n0 + 128 && target < p.N) {
+                    float at = 0.f;
+#pragma unroll
+                    for (int e = 0; e < 128; ++e) at = target == n0 + e ? z[e] : at;
+                    p.hit[row] = ok ? at : CUDART_NAN_F;
+                }
+                if (n0 + 128 > p.N) {
+#pragma unroll
+                    for (int e = 0; e < 128; ++e) if (n0 + e >= p.N) z[e] = -CUDART_INF_F;
+                }
+                float top[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F}, sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int e = 0; e < 128; ++e) top[e & 3] = fmaxf(top[e & 3], z[e]);
+                const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * p.c;
+                const float below = most == -CUDART_INF_F ? 0.f : most;              // (nothing but minus infinities)
+#pragma unroll
+                for (int e = 0; e < 128; ++e) sum[e & 3] += exp2_fast(fmaf(z[e], p.c, -below));
+                if (mine)
+                    p.part[(size_t)row * (2 * tiles_n) + 2 * tn + (c_half >> 7)] =
+                        ok ? make_float2(most, (sum[0] + sum[1]) + (sum[2] + sum[3])) : make_float2(CUDART_NAN_F, CUDART_NAN_F);      // (no result)
             } else if constexpr (KIND == kProbs) {
-                // a row's number in front of the exponential, and the factor behind it
-                float g = 0.f, base = 0.f;
+                // rows that do not count are zeros, whatever they hold; one with a target that is not there NaN
+                float base = 0.f, own = 0.f;
                 int target = -1;
+                bool counts = false;
                 if (mine) {
                     const long long to = target_of(p.targets, p.targets64, row);
-                    if (to != p.ignore) {
-                        g = p.grad[(size_t)row * p.grad_stride] * p.scale;
-                        if (p.count) g /= *p.count;
-                        base = p.lse[row] * kLog2e;
-                        if (!ok || to < 0 || to >= p.V) g = CUDART_NAN_F;
-                        else target = (int)to - p.v0;
-                    }
+                    counts = to != p.ignore;
+                    const float2 kept = p.kept[row];
+                    const bool there = to >= 0 && to < p.V;
+                    base = there ? kept.x * kLog2e : CUDART_NAN_F;
+                    own = expm1f(-kept.y);                    // p - 1 of the target: keeps its digits where p is next to one
+                    if (there) target = (int)to - p.v0;
                 }
-                const bool none = target == -1 && g == 0.f;   // (not a row that counts: nothing of it enters, whatever it holds)
+                wait();
+                if (!ok) base = own = CUDART_NAN_F;
 #pragma unroll 1
-                for (int cb = 0; cb < kTileN / 64; ++cb) {
+                for (int cb = 0; cb < 2; ++cb) {
                     if (rows <= 0) break;
                     uint32_t v[2][32], y[32];
-                    tmem_columns32(from + cb * 64, v[0]);
-                    tmem_columns32(from + cb * 64 + 32, v[1]);
+                    tmem_columns32(from() + cb * 64, v[0]);
+                    tmem_columns32(from() + cb * 64 + 32, v[1]);
                     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
                     const int at = target - (n0 + cb * 64);
 #pragma unroll
@@ -273,22 +304,24 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                         for (int o = 0; o < 2; ++o) {
                             const int col = 2 * e + o;
                             const float s = exp2_fast(fmaf(__uint_as_float(v[col >> 5][col & 31]), p.c, -base));
-                            f[o] = none ? 0.f : (at == col ? s - 1.f : s) * g;
+                            f[o] = counts ? (at == col ? own : s) : 0.f;
                         }
                         const __nv_bfloat162 b = __floats2bfloat162_rn(f[0], f[1]);
                         y[e] = *reinterpret_cast<const uint32_t*>(&b);
                     }
                     store_64(blk, y, p.p, p.ldp, row0, rows, n0 + cb * 64, 64, true, lane);
                 }
+                taken();
             } else if constexpr (KIND == kRows) {
                 const int rr = lane >> 3, ch = lane & 7;
                 float* const acc = p.acc + (size_t)(t / (tiles_m * tiles_n)) * p.M * p.ld_acc;
+                wait();
 #pragma unroll 1
-                for (int cb = 0; cb < kTileN / 32; ++cb) {
+                for (int cb = 0; cb < 4; ++cb) {
                     const int n = n0 + cb * 32 + 4 * ch;
                     if (n0 + cb * 32 >= p.ld_acc || rows <= 0) break;
                     uint32_t v[32];
-                    tmem_columns32(from + cb * 32, v);
+                    tmem_columns32(from() + cb * 32, v);
                     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
                     for (int c = 0; c < 8; ++c)
@@ -309,27 +342,27 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                     }
                     __syncwarp();
                 }
+                taken();
             } else {
+                wait();
+                if (!ok) factor = CUDART_NAN_F;
 #pragma unroll 1
-                for (int cb = 0; cb < kTileN / 64; ++cb) {
+                for (int cb = 0; cb < 2; ++cb) {
                     const int c0 = n0 + cb * 64;
                     if (c0 >= p.N || rows <= 0) break;
                     uint32_t v[2][32], y[32];
-                    tmem_columns32(from + cb * 64, v[0]);
-                    tmem_columns32(from + cb * 64 + 32, v[1]);
+                    tmem_columns32(from() + cb * 64, v[0]);
+                    tmem_columns32(from() + cb * 64 + 32, v[1]);
                     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
                     for (int e = 0; e < 32; ++e) {
-                        const float lo = __uint_as_float(v[e >> 4][2 * e & 31]), hi = __uint_as_float(v[e >> 4][(2 * e & 31) + 1]);
-                        const __nv_bfloat162 b = __floats2bfloat162_rn(ok ? lo : CUDART_NAN_F, ok ? hi : CUDART_NAN_F);
+                        const __nv_bfloat162 b = __floats2bfloat162_rn(__uint_as_float(v[e >> 4][2 * e & 31]) * factor, __uint_as_float(v[e >> 4][(2 * e & 31) + 1]) * factor);
                         y[e] = *reinterpret_cast<const uint32_t*>(&b);
                     }
                     store_64(blk, y, p.out, p.N, row0, rows, c0, p.N - c0, p.wide, lane);
                 }
+                taken();
             }
-            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(at_rank(&t_empty[it & 1u], 0)) : "memory");
         }
     }
     if (!ok && lane == 0 && p.ran_out) {
@@ -348,7 +381,7 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
 // The tiles of a row joined, a warp per row; the last block to come sums the rows, in their order.
 constexpr int kJoinWarps = 8;
 __global__ void __launch_bounds__(32 * kJoinWarps) loss_join_kernel(const float2* __restrict__ part, const float* __restrict__ hit, int M, int V, int tiles, const void* targets,
-                                                                    int targets64, long long ignore, float c, float* loss, float* __restrict__ lse, float* __restrict__ totals,
+                                                                    int targets64, long long ignore, float c, float* __restrict__ loss, float2* kept, float* __restrict__ totals,
                                                                     unsigned* arrived) {
     const int lane = threadIdx.x & 31, row = blockIdx.x * kJoinWarps + (threadIdx.x >> 5);
     if (row < M) {
@@ -372,9 +405,10 @@ __global__ void __launch_bounds__(32 * kJoinWarps) loss_join_kernel(const float2
         if (lane == 0) {
             const long long t = target_of(targets, targets64, row);
             const float below = bad ? CUDART_NAN_F : log2f(sum);
-            lse[row] = (most + below) * kLn2;
             // (the target's distance from the largest is taken before it meets the logarithm: losses near zero keep their digits)
-            loss[row] = t == ignore ? 0.f : t < 0 || t >= V ? CUDART_NAN_F : (below - fmaf(hit[row], c, -most)) * kLn2;
+            const float l = t == ignore ? 0.f : t < 0 || t >= V ? CUDART_NAN_F : (below - fmaf(hit[row], c, -most)) * kLn2;
+            kept[row] = make_float2((most + below) * kLn2, l);
+            if (loss) loss[row] = l;
         }
     }
     __shared__ bool last;
@@ -390,7 +424,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) loss_join_kernel(const float2
     int n = 0;
     for (int i = threadIdx.x; i < M; i += 32 * kJoinWarps)
         if (target_of(targets, targets64, i) != ignore) {
-            s += (double)__ldcg(loss + i);
+            s += (double)__ldcg(&kept[i].y);
             ++n;
         }
 #pragma unroll
@@ -412,20 +446,26 @@ __global__ void __launch_bounds__(32 * kJoinWarps) loss_join_kernel(const float2
 }
 
 // Rows as operands: out [TERMS][M][ld_out] bf16, zeros from K on.  TERMS 3: fp32 rows as three bf16 terms (24 bits).  targets: rows whose target is `ignore` are zeros
-// (what they hold, a NaN among it, stays out of the head's gradient).
+// (what they hold, a NaN among it, stays out of the head's gradient).  grad: the others times grad scale [/ *count] of their own.
 template <int TERMS, bool F32>
 __global__ void __launch_bounds__(256) loss_pack_kernel(const void* __restrict__ x, long long ld, int M, int K, __nv_bfloat16* __restrict__ out, int ld_out, const void* targets,
-                                                        int targets64, long long ignore) {
+                                                        int targets64, long long ignore, const float* grad, int grad_stride, const float* count, float scale) {
     const int per_row = ld_out / 8;
     const long long i = (long long)blockIdx.x * 256 + threadIdx.x, r = i / per_row;
     if (r >= M) return;
     const int k = (int)(i - r * per_row) * 8;
     const bool out_of_it = targets && target_of(targets, targets64, (int)r) == ignore;
+    float factor = 1.f;
+    if (grad) {
+        factor = grad[r * grad_stride] * scale;
+        if (count) factor /= fmaxf(*count, 1.f);
+    }
     __nv_bfloat16 t[TERMS][8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
         float v = 0.f;
         if (k + e < K && !out_of_it) v = F32 ? reinterpret_cast<const float*>(x)[r * ld + k + e] : __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(x)[r * ld + k + e]);
+        if (grad && !out_of_it) v *= factor;
         t[0][e] = TERMS == 1 ? __float2bfloat16_rn(v) : __float2bfloat16_rz(v);
         if (TERMS == 3) {                                     // rounded towards zero first: the largest numbers do not become infinities
             const float f = __bfloat162float(t[0][e]), r1 = fabsf(f) <= 3.402823466e38f ? v - f : 0.f;
@@ -437,8 +477,10 @@ __global__ void __launch_bounds__(256) loss_pack_kernel(const void* __restrict__
     for (int q = 0; q < TERMS; ++q) *reinterpret_cast<uint4*>(out + ((size_t)q * M + r) * ld_out + k) = *reinterpret_cast<const uint4*>(t[q]);
 }
 
-// dh = the sum of the shares of the contraction
-__global__ void __launch_bounds__(256) loss_rows_out_kernel(const float* __restrict__ acc, int splits, int M, int K, int ld, __nv_bfloat16* __restrict__ out, int wide) {
+// dh = the sum of the shares of the contraction, times grad scale [/ *count]
+__global__ void __launch_bounds__(256) loss_rows_out_kernel(const float* __restrict__ acc, int splits, int M, int K, int ld, __nv_bfloat16* __restrict__ out, int wide,
+                                                            const float* __restrict__ grad, int grad_stride, const float* __restrict__ count, float scale, const void* targets,
+                                                            int targets64, long long ignore) {
     const int per_row = ld / 4;
     const long long i = (long long)blockIdx.x * 256 + threadIdx.x, r = i / per_row;
     if (r >= M) return;
@@ -448,6 +490,10 @@ __global__ void __launch_bounds__(256) loss_rows_out_kernel(const float* __restr
         const float4 o = *reinterpret_cast<const float4*>(acc + ((size_t)s * M + r) * ld + k);
         v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
     }
+    float f = grad[r * grad_stride] * scale;
+    if (count) f /= fmaxf(*count, 1.f);
+    if (target_of(targets, targets64, (int)r) == ignore) f = 0.f;
+    v.x *= f; v.y *= f; v.z *= f; v.w *= f;
     const __nv_bfloat16 h[4] = {__float2bfloat16_rn(v.x), __float2bfloat16_rn(v.y), __float2bfloat16_rn(v.z), __float2bfloat16_rn(v.w)};
     __nv_bfloat16* const o = out + (size_t)r * K + k;
     if (wide) {
@@ -511,11 +557,12 @@ bool in_place(const void* x, long long ld) { return (reinterpret_cast<uintptr_t>
 size_t up(size_t n) { return (n + 255) / 256 * 256; }
 
 template <int TERMS, bool F32>
-cudaError_t pack(const void* x, long long ld, int M, int K, void* out, const LossShape* counts, cudaStream_t st) {
+cudaError_t pack(const void* x, long long ld, int M, int K, void* out, const LossShape* counts, cudaStream_t st, const LossGrad* by = nullptr) {
     const long long blocks = ((long long)M * (padded(K) / 8) + 255) / 256;
     if (blocks > 0x7fffffffLL) return cudaErrorNotSupported;
     loss_pack_kernel<TERMS, F32><<<(unsigned)blocks, 256, 0, st>>>(x, ld, M, K, reinterpret_cast<__nv_bfloat16*>(out), padded(K), counts ? counts->targets : nullptr,
-                                                                   counts ? counts->targets64 : 0, counts ? counts->ignore : 0);
+                                                                   counts ? counts->targets64 : 0, counts ? counts->ignore : 0, by ? by->grad : nullptr, by ? by->grad_stride : 0,
+                                                                   by ? by->count : nullptr, counts ? counts->scale : 1.f);
     ++extra_launches();
     return cudaGetLastError();
 }
@@ -528,7 +575,7 @@ int shares_of(int length, int most) {
 
 // What a call keeps in its workspace, one after the other
 struct Room {
-    size_t h = 0, w = 0, part = 0, hit = 0, arrived = 0, p = 0, acc = 0, all = 0;      // offsets
+    size_t h = 0, h_dw = 0, w = 0, part = 0, hit = 0, arrived = 0, p = 0, acc = 0, all = 0;      // offsets
     int piece = 0, splits = 1;                                                          // columns of a piece of the vocabulary, shares of dh's contraction
 };
 Room room_of(const LossShape& s, bool grad, bool rows, bool head) {
@@ -536,10 +583,11 @@ Room room_of(const LossShape& s, bool grad, bool rows, bool head) {
     size_t at = 0;
     const auto take = [&](size_t bytes) { const size_t was = at; at += up(bytes); return was; };
     const size_t row = (size_t)s.M * padded(s.K) * 2;
-    r.h = take(grad ? (head || !in_place(s.h, s.ldh) ? row : 0) : s.h_type == kTypeF32 ? 3 * row : in_place(s.h, s.ldh) ? 0 : row);
+    r.h = take(s.h_type == kTypeF32 ? 3 * row : in_place(s.h, s.ldh) ? 0 : row);
+    r.h_dw = take(grad && head ? row : 0);
     r.w = take(in_place(s.w, s.ldw) ? 0 : (size_t)s.V * padded(s.K) * 2);
     if (!grad) {
-        r.part = take((size_t)s.M * ((s.V + kTileN - 1) / kTileN) * 8);
+        r.part = take((size_t)s.M * ((s.V + kTileN - 1) / kTileN) * 16);
         r.hit = take((size_t)s.M * 4);
         r.arrived = take(4);
     } else {
@@ -560,7 +608,7 @@ LossTiles tiles_of(const LossShape& s) {
     LossTiles p{};
     p.splits = 1;
     p.targets = s.targets; p.targets64 = s.targets64; p.ignore = s.ignore;
-    p.c = s.scale * kLog2e; p.scale = s.scale; p.V = s.V;
+    p.c = s.scale * kLog2e; p.V = s.V;
     return p;
 }
 
@@ -569,7 +617,7 @@ LossTiles tiles_of(const LossShape& s) {
 size_t loss_work_bytes(const LossShape& s) { return room_of(s, false, false, false).all; }
 size_t loss_grad_work_bytes(const LossShape& s, bool rows, bool head) { return room_of(s, true, rows, head).all; }
 
-cudaError_t launch_loss(const LossShape& s, float* loss, float* lse, float* totals, void* work, cudaStream_t st) {
+cudaError_t launch_loss(const LossShape& s, float* loss, float* kept, float* totals, void* work, cudaStream_t st) {
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
@@ -601,12 +649,12 @@ cudaError_t launch_loss(const LossShape& s, float* loss, float* lse, float* tota
     e = f32 ? run_tiles<kStats, 3>(ma, mb, p, dev, st) : run_tiles<kStats, 1>(ma, mb, p, dev, st);
     if (e != cudaSuccess) return e;
     ++extra_launches();
-    loss_join_kernel<<<(s.M + kJoinWarps - 1) / kJoinWarps, 32 * kJoinWarps, 0, st>>>(p.part, p.hit, s.M, s.V, (s.V + kTileN - 1) / kTileN, s.targets, s.targets64, s.ignore,
-                                                                                    p.c, loss, lse, totals, arrived);
+    loss_join_kernel<<<(s.M + kJoinWarps - 1) / kJoinWarps, 32 * kJoinWarps, 0, st>>>(p.part, p.hit, s.M, s.V, 2 * ((s.V + kTileN - 1) / kTileN), s.targets, s.targets64,
+                                                                                    s.ignore, p.c, loss, reinterpret_cast<float2*>(kept), totals, arrived);
     return cudaGetLastError();
 }
 
-cudaError_t launch_loss_grad(const LossShape& s, const float* lse, const float* grad, int grad_stride, const float* count, void* dh, void* dw, void* work, cudaStream_t st) {
+cudaError_t launch_loss_grad(const LossShape& s, const float* kept, const LossGrad& by, void* dh, void* dw, void* work, cudaStream_t st) {
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
@@ -615,11 +663,13 @@ cudaError_t launch_loss_grad(const LossShape& s, const float* lse, const float* 
     unsigned char* const base = reinterpret_cast<unsigned char*>(work);
     const void *h = s.h, *w = s.w;
     long long ldh = s.ldh, ldw = s.ldw;
-    if (dw || !in_place(s.h, s.ldh)) {                        // (rows that do not count are zeros here)
+    if (!in_place(s.h, s.ldh)) {
         h = base + r.h;
         ldh = padded(s.K);
-        e = pack<1, false>(s.h, s.ldh, s.M, s.K, base + r.h, &s, st);
+        e = pack<1, false>(s.h, s.ldh, s.M, s.K, base + r.h, nullptr, st);
     }
+    // the rows as dw takes them: those that do not count are zeros, factors of their own are in them
+    if (e == cudaSuccess && dw) e = pack<1, false>(s.h, s.ldh, s.M, s.K, base + r.h_dw, &s, st, by.grad_stride ? &by : nullptr);
     if (e == cudaSuccess && !in_place(s.w, s.ldw)) {
         w = base + r.w;
         ldw = padded(s.K);
@@ -632,14 +682,14 @@ cudaError_t launch_loss_grad(const LossShape& s, const float* lse, const float* 
     CUtensorMap h_rows, w_rows, p_rows, h_cols, w_cols, p_cols;
     // rows along the contraction, and (the last two products) channels of a row in boxes of 64 x 64
     if (!bf16_map(&h_rows, h, s.M, s.K, ldh, 128) || !bf16_map(&w_rows, w, s.V, s.K, ldw, 128) || !bf16_map(&p_rows, probs, s.M, r.piece, r.piece, 128) ||
-        !bf16_map(&h_cols, h, s.M, s.K, ldh, kBK) || !bf16_map(&w_cols, w, s.V, s.K, ldw, kBK) || !bf16_map(&p_cols, probs, s.M, r.piece, r.piece, kBK))
+        (dw && !bf16_map(&h_cols, base + r.h_dw, s.M, s.K, padded(s.K), kBK)) || !bf16_map(&w_cols, w, s.V, s.K, ldw, kBK) || !bf16_map(&p_cols, probs, s.M, r.piece, r.piece, kBK))
         return cudaErrorNotSupported;
     for (int v0 = 0; v0 < s.V; v0 += r.piece) {
         const int cols = std::min(r.piece, s.V - v0);
         LossTiles p = tiles_of(s);
         p.v0 = v0;
         p.M = s.M; p.N = cols; p.K = s.K;
-        p.lse = lse; p.grad = grad; p.grad_stride = grad_stride; p.count = count;
+        p.kept = reinterpret_cast<const float2*>(kept);
         p.p = probs; p.ldp = r.piece;
         e = run_tiles<kProbs, 1>(h_rows, w_rows, p, dev, st);
         if (e != cudaSuccess) return e;
@@ -657,6 +707,7 @@ cudaError_t launch_loss_grad(const LossShape& s, const float* lse, const float* 
             LossTiles q = tiles_of(s);
             q.M = cols; q.N = s.K; q.K = s.M;
             q.out = reinterpret_cast<__nv_bfloat16*>(dw) + (size_t)v0 * s.K;
+            if (!by.grad_stride) q.grad = by.grad, q.count = by.count, q.scale = s.scale;      // (else the rows have theirs)
             q.wide = s.K % 8 == 0 && (reinterpret_cast<uintptr_t>(dw) & 15) == 0;
             e = run_tiles<kHead, 1>(p_cols, h_cols, q, dev, st);
             if (e != cudaSuccess) return e;
@@ -667,7 +718,8 @@ cudaError_t launch_loss_grad(const LossShape& s, const float* lse, const float* 
         const long long blocks = ((long long)s.M * (ld_acc / 4) + 255) / 256;
         if (blocks > 0x7fffffffLL) return cudaErrorNotSupported;
         loss_rows_out_kernel<<<(unsigned)blocks, 256, 0, st>>>(acc, r.splits, s.M, s.K, ld_acc, reinterpret_cast<__nv_bfloat16*>(dh),
-                                                              s.K % 4 == 0 && (reinterpret_cast<uintptr_t>(dh) & 7) == 0);
+                                                              s.K % 4 == 0 && (reinterpret_cast<uintptr_t>(dh) & 7) == 0, by.grad, by.grad_stride, by.count, s.scale, s.targets,
+                                                              s.targets64, s.ignore);
         ++extra_launches();
         e = cudaGetLastError();
     }

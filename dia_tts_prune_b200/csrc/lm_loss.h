@@ -17,13 +17,15 @@ struct LossShape {
 };
 // The operands that are laid out again in the workspace: rows that are fp32 or not of 16 bytes, a head whose rows are not
 size_t loss_work_bytes(const LossShape& s);
-// loss [M], lse [M]: log sum_j exp z[i][j]; totals [3]: the sum of the losses, how many rows count, their mean (0 where none does)
-cudaError_t launch_loss(const LossShape& s, float* loss, float* lse, float* totals, void* work, cudaStream_t st);
+// loss [M] (or null), kept [M][2]: log sum_j exp z[i][j] and the loss, for the gradient; totals [3]: the sum of the losses, how many rows count, their mean (0 where none does)
+cudaError_t launch_loss(const LossShape& s, float* loss, float* kept, float* totals, void* work, cudaStream_t st);
 
-// The gradient by rows (dh [M][K] bf16) and by the head (dw [V][K] bf16), either or both; h is bf16.  grad: of every loss, grad_stride floats apart (0: one for all);
-// count: divides it where not null (totals + 1 of a mean)
+// The gradient by rows (dh [M][K] bf16) and by the head (dw [V][K] bf16), either or both; h is bf16
+struct LossGrad {
+    const float* grad; int grad_stride;          // of every loss, grad_stride floats apart (0: one for all)
+    const float* count;                          // divides it where not null (totals + 1 of a mean)
+};
 size_t loss_grad_work_bytes(const LossShape& s, bool rows, bool head);
-cudaError_t launch_loss_grad(const LossShape& s, const float* lse, const float* grad, int grad_stride, const float* count, void* dh, void* dw, void* work,
-                             cudaStream_t st);
+cudaError_t launch_loss_grad(const LossShape& s, const float* kept, const LossGrad& by, void* dh, void* dw, void* work, cudaStream_t st);
 
 }  // namespace lm

@@ -148,15 +148,16 @@ class _LinearCrossEntropy(torch.autograd.Function):
     def forward(ctx, hidden, weight, targets, scale, ignore_index, reduction):
         lib = _lm_lib.load()
         (M, K), V, device = hidden.shape, weight.shape[0], hidden.device
-        loss, lse, totals = (torch.empty(n, dtype=torch.float32, device=device) for n in (M, M, 3))
+        loss = torch.empty(M, dtype=torch.float32, device=device) if reduction == "none" else None
+        kept, totals = torch.empty(2 * M, dtype=torch.float32, device=device), torch.empty(3, dtype=torch.float32, device=device)
         h, w, t = _as_rows(hidden), _as_rows(weight), targets.contiguous()
         args = h.data_ptr(), _TYPES[h.dtype], h.stride(0), w.data_ptr(), w.stride(0)
         need = lib.lm_b200_op_loss_work_bytes(*args, M, V, K)
         work = torch.empty(need, dtype=torch.uint8, device=device)
         with torch.cuda.device(device):
-            _lm_lib.check(lib.lm_b200_op_loss(*args, t.data_ptr(), t.dtype == torch.int64, ignore_index, M, V, K, scale, loss.data_ptr(),
-                                              lse.data_ptr(), totals.data_ptr(), work.data_ptr(), need, _stream(device)), "loss")
-        ctx.save_for_backward(hidden, weight, t, lse)
+            _lm_lib.check(lib.lm_b200_op_loss(*args, t.data_ptr(), t.dtype == torch.int64, ignore_index, M, V, K, scale,
+                                              None if loss is None else loss.data_ptr(), kept.data_ptr(), totals.data_ptr(), work.data_ptr(), need, _stream(device)), "loss")
+        ctx.save_for_backward(hidden, weight, t, kept)
         # (the count stands beside the result, which may be changed in place: not a saved tensor)
         ctx.args = scale, ignore_index, totals[1:2].detach() if reduction == "mean" else None
         return loss if reduction == "none" else totals[2 if reduction == "mean" else 0]
@@ -164,7 +165,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        hidden, weight, t, lse = ctx.saved_tensors
+        hidden, weight, t, kept = ctx.saved_tensors
         scale, ignore_index, count = ctx.args
         need_h, need_w = ctx.needs_input_grad[:2]
         if hidden.dtype != torch.bfloat16:
@@ -181,7 +182,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
         work = torch.empty(need, dtype=torch.uint8, device=device)
         with torch.cuda.device(device):
             _lm_lib.check(lib.lm_b200_op_loss_grad(
-                *args, t.data_ptr(), t.dtype == torch.int64, ignore_index, M, V, K, scale, lse.data_ptr(), grad.data_ptr(),
+                *args, t.data_ptr(), t.dtype == torch.int64, ignore_index, M, V, K, scale, kept.data_ptr(), grad.data_ptr(),
                 grad.stride(0) if grad.dim() else 0, count.data_ptr() if count is not None else None,
                 dh.data_ptr() if need_h else None, dw.data_ptr() if need_w else None, work.data_ptr(), need, _stream(device)), "loss_grad")
         return dh, dw, None, None, None, None

@@ -35,14 +35,15 @@ class Exact:
         self.loss_off = torch.where(self.keep, 2 * self.dz + 2.0 ** -20 + 2.0 ** -22 * (z.abs().amax(1) + self.loss), 0.0)
         self.p, self.onehot = logp.exp(), torch.zeros_like(z).scatter_(1, at, 1.0)
 
-    def gradient(self, g):
+    def gradient(self, g, own=False):
         """(by rows, by the head) and their bounds: P is off by 2^-8 of itself (bfloat16) and by its probability's 4 dz + 2^-18; the sums of V
-        (or M) products lose as the logits do, in pieces; and the results are bfloat16."""
+        (or M) products lose as the logits do, in pieces; and the results are bfloat16.  own: rows with factors of their own take them into
+        h for the head's gradient, which is rounded once more (2^-8, and 2^-8 of that of P)."""
         g = (g.double().cpu() * self.keep * self.scale)[:, None]
         P = (self.p - self.onehot) * g
         dP = 2.0 ** -8 * P.abs() + (self.p * g).abs() * (4 * self.dz[:, None] + 2.0 ** -18) + P.abs() * 2.0 ** -18
         out = []
-        for a, da, b in ((P, dP, self.w), (P.T, dP.T, self.h)):
+        for a, da, b in ((P, dP, self.w), (P.T, dP.T + (1.01 * 2.0 ** -8 * P.T.abs() if own else 0), self.h)):
             want, lost = a @ b, (a.shape[1] / 16 + 2) * 2.0 ** -22
             out.append((want, 1.01 * (da @ b.abs()) + lost * (a.abs() @ b.abs()) + 2.0 ** -8 * want.abs() + 2.0 ** -133))
         return out
@@ -87,7 +88,7 @@ def test_gradients(m, v, k):
     within(dw, want_w, off_w)
     # every token's own factor, through an expanded and a strided gradient, one input at a time
     g = torch.randn(m, generator=torch.Generator().manual_seed(m)).cuda()
-    (want_h, off_h), (want_w, off_w) = e.gradient(g)
+    (want_h, off_h), (want_w, off_w) = e.gradient(g, own=True)
     loss = linear_cross_entropy(h, w.detach(), t, scale=0.5, reduction="none")
     within(torch.autograd.grad(loss, h, torch.stack([g, g], 1)[:, 0])[0], want_h, off_h)
     loss = linear_cross_entropy(h.detach(), w, t, scale=0.5, reduction="none")
