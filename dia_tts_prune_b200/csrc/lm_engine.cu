@@ -1744,7 +1744,7 @@ int lm_b200_op_mxfp4_dequantize(const void* codes, const void* scales, int rows,
     return LM_B200_OK;
 }
 
-size_t lm_b200_op_linear_mxfp4_work_bytes(int M, int N, int K) { return M > 0 && N > 0 && K > 0 ? lm::mxfp4_linear_work_bytes(M, K) : 0; }
+size_t lm_b200_op_linear_mxfp4_work_bytes(int M, int N, int K) { return M > 0 && N > 0 && K > 0 ? lm::mxfp4_linear_work_bytes(M, N, K) : 0; }
 
 int lm_b200_op_linear_mxfp4(const void* A, int a_type, int64_t lda, const void* w_codes, const void* w_scales, void* Y, int y_type, int M, int N, int K, void* work,
                             size_t work_bytes, void* stream) {
@@ -1763,7 +1763,7 @@ size_t lm_b200_op_loss_work_bytes(const void* h, int h_type, int64_t ldh, const 
 int lm_b200_op_loss(const void* h, int h_type, int64_t ldh, const void* W, int64_t ldw, const void* targets, int targets64, int64_t ignore, int M, int V, int K, float scale,
                     float* loss, float* kept, float* totals, void* work, size_t work_bytes, void* stream) {
     lm::LossShape s;
-    if (!loss_shape(s, h, h_type, ldh, W, ldw, M, V, K) || !targets || !(scale > 0.f) || !std::isfinite(scale) || !kept || !totals || !work || !aligned(work, 256) ||
+    if (!loss_shape(s, h, h_type, ldh, W, ldw, M, V, K) || !targets || !(scale > 0.f) || !std::isfinite(scale) || !work || !aligned(work, 256) ||
         work_bytes < lm::loss_work_bytes(s))
         return LM_B200_EINVAL;
     s.targets = targets; s.targets64 = targets64; s.ignore = ignore; s.scale = scale;

@@ -143,6 +143,7 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
     cluster_sync_all();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem_base = *tmem_slot;
+    if (KIND == kStats) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     bool ok = true;
     if (warp == 0) {
         if (lane == 0) {
@@ -378,12 +379,175 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
     }
 }
 
-// The tiles of a row joined, a warp per row; the last block to come sums the rows, in their order.
+// Few rows (a token or some, up to 32): the head is the 128-row operand and streams once, the rows are the columns; float32 rows have a column for each of their three
+// terms.  A CTA walks tiles of 128 head rows, and a thread keeps for its head row of every tile, per row of h, the largest logit and the sum of the exponentials below it;
+// at the end the CTA's 128 threads meet.
+//   warp 0    one lane: the head's tile [128 x 64] of a k-block and the rows' [columns x 64] into a ring; the head's first ones before the kernel's predecessor has ended
+//             (nothing that lets its successor start early writes a head)
+//   warp 1    MMAs (M = 128, N = the columns), an accumulator for 16 k-blocks
+//   warps 2-5 take the accumulators out
+// Bound: the head's bytes.  Tensor memory is taken behind the wait for the predecessor and in front of the signal to the successor (see the few rows of 4-bit numbers).
+constexpr int kFewMost = 32, kFewThreads = 192, kFewCols = 256, kFewSlotsMost = 6, kFewChunk = 16;
+
+template <int NB, int TERMS>
+struct Few {
+    static constexpr int kCols = NB * TERMS, kSlot = kTileBytes + kCols * 128, kFit = 110 * 1024 / kSlot, kSlots = kFit < kFewSlotsMost ? kFit : kFewSlotsMost;
+    static constexpr int kSmem = kSlots * kSlot + 1024;
+    static_assert(2 * kCols <= kFewCols && 2 * kFewCols <= 512 && 3 * kSmem > 228 * 1024, "two CTAs on an SM");
+};
+
+template <int NB, int TERMS>
+__global__ void __launch_bounds__(kFewThreads, 2) loss_few_rows_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_constant__ CUtensorMap map_w,
+                                                                       const __grid_constant__ LossTiles p) {
+    constexpr int kCols = Few<NB, TERMS>::kCols, kSlot = Few<NB, TERMS>::kSlot, kSlots = Few<NB, TERMS>::kSlots;
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    __shared__ uint64_t full[kSlots], empty[kSlots], t_full[2], t_empty[2];
+    __shared__ uint32_t tmem_slot;
+    __shared__ int targets[NB];
+    __shared__ float2 meet[4][NB];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, M = p.M;
+    const int n_kb = (p.K + kBK - 1) / kBK, n_tiles = (p.N + 127) / 128, mine = (n_tiles - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x, blocks = mine * n_kb;
+    const auto head_tile = [&](int i) {
+        const int slot = i % kSlots, t = blockIdx.x + i / n_kb * gridDim.x;
+        mbar_arrive_expect_tx(&full[slot], kSlot);
+        tma_load_2d(smem_u32(smem + slot * kSlot), &map_w, smem_u32(&full[slot]), i % n_kb * kBK, t * 128);
+    };
+    const auto row_tile = [&](int i) {
+        const int slot = i % kSlots;
+#pragma unroll
+        for (int tm = 0; tm < TERMS; ++tm)
+            tma_load_2d(smem_u32(smem + slot * kSlot + kTileBytes + tm * NB * 128), &map_h, smem_u32(&full[slot]), i % n_kb * kBK, tm * M);
+    };
+    if (tid == 0) {
+        for (int i = 0; i < kSlots; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&t_full[i], 1); mbar_init(&t_empty[i], 4); }
+        fence_mbar_init();
+        for (int i = 0; i < min(blocks, kSlots); ++i) head_tile(i);
+    }
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (blockIdx.x == 0 && tid == 0) *p.arrived = 0u;
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(kFewCols));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+    }
+    if (tid < NB) {
+        const long long t = tid < M ? target_of(p.targets, p.targets64, tid) : -1;
+        targets[tid] = t >= 0 && t < p.N ? (int)t : -1;
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const uint32_t tmem = tmem_slot;
+    bool ok = true;
+    if (warp == 0) {
+        if (lane == 0) {
+            int i = 0;
+            for (; i < min(blocks, kSlots); ++i) row_tile(i);
+            for (; i < blocks; ++i) {
+                if (!lane_wait(&empty[i % kSlots], ((i / kSlots) & 1u) ^ 1u, p.polls)) { ok = false; break; }
+                head_tile(i);
+                row_tile(i);
+            }
+            // (copies in flight arrive before the CTA goes)
+            for (int j = max(0, i - kSlots); j < i && !ok; ++j) (void)lane_wait(&full[j % kSlots], (j / kSlots) & 1u, p.polls);
+        }
+    } else if (warp == 1) {
+        const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(kCols >> 3) << 17) | (8u << 24);
+        unsigned it = 0;
+        for (int i = 0; i < blocks && ok; ++i) {
+            const int kb = i % n_kb, slot = i % kSlots;
+            const bool first = kb % kFewChunk == 0, last = kb == n_kb - 1 || kb % kFewChunk == kFewChunk - 1;
+            if (first) ok = pair_wait(&t_empty[it & 1u], ((it >> 1) & 1u) ^ 1u, p.polls);
+            ok = ok && pair_wait(&full[slot], (i / kSlots) & 1u, p.polls);
+            if (!ok) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const uint32_t at = smem_u32(smem + slot * kSlot);
+            const uint64_t adesc = umma_desc(at), bdesc = umma_desc(at + kTileBytes);
+            if (elect_one_sync()) {
+#pragma unroll
+                for (int j = 0; j < kBK / 16; ++j) umma_bf16(tmem + (it & 1u) * kCols, adesc + 2 * j, bdesc + 2 * j, idesc, j != 0 || !first ? 1u : 0u);
+                umma_commit(&empty[slot]);
+                if (last) umma_commit(&t_full[it & 1u]);
+            }
+            __syncwarp();
+            if (last) ++it;
+        }
+    } else {
+        const int q = warp & 3, c = q * 32 + lane;
+        float most[NB], sum[NB];                              // of c z, of 2^(c z - most)
+#pragma unroll
+        for (int m = 0; m < NB; ++m) most[m] = -CUDART_INF_F, sum[m] = 0.f;
+        unsigned it = 0;
+        for (int j = 0; j < mine; ++j) {
+            const int n = (blockIdx.x + j * gridDim.x) * 128 + c;
+            float z[NB];
+#pragma unroll
+            for (int m = 0; m < NB; ++m) z[m] = 0.f;
+            for (int kb = 0; kb < n_kb; kb += kFewChunk, ++it) {
+                ok = ok && pair_wait(&t_full[it & 1u], (it >> 1) & 1u, p.polls);
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+                for (int tm = TERMS - 1; tm >= 0; --tm)
+#pragma unroll
+                    for (int m0 = 0; m0 < NB; m0 += 16) {
+                        uint32_t v[16];
+                        tmem_columns16(tmem + ((uint32_t)(q * 32) << 16) + (it & 1u) * kCols + tm * NB + m0, v);
+                        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) z[m0 + e] += __uint_as_float(v[e]);
+                    }
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&t_empty[it & 1u]);
+            }
+#pragma unroll
+            for (int m = 0; m < NB; ++m) {
+                if (m >= M) break;
+                if (targets[m] == n) p.hit[m] = ok ? z[m] : CUDART_NAN_F;
+                const float x = n < p.N ? z[m] * p.c : -CUDART_INF_F, now = fmaxf(most[m], x);
+                if (now > -CUDART_INF_F) sum[m] = sum[m] * exp2_fast(most[m] - now) + exp2_fast(n < p.N ? fmaf(z[m], p.c, -now) : -CUDART_INF_F);
+                else sum[m] += x != x ? x : 0.f;
+                most[m] = now;
+            }
+        }
+#pragma unroll
+        for (int m = 0; m < NB; ++m) {
+            if (m >= M) break;
+            if (!ok) most[m] = sum[m] = CUDART_NAN_F;
+#pragma unroll
+            for (int o = 16; o; o >>= 1) {
+                const float other = __shfl_xor_sync(0xffffffffu, most[m], o), add = __shfl_xor_sync(0xffffffffu, sum[m], o), now = fmaxf(most[m], other);
+                if (now > -CUDART_INF_F) sum[m] = sum[m] * exp2_fast(most[m] - now) + add * exp2_fast(other - now);
+                else sum[m] += add;
+                most[m] = now;
+            }
+            if (lane == 0) meet[q][m] = make_float2(most[m], sum[m]);
+        }
+    }
+    if (!ok && lane == 0 && p.ran_out) {
+        *reinterpret_cast<volatile int*>(p.ran_out) = 1;
+        __threadfence_system();
+    }
+    __syncwarp();
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (warp == 1) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kFewCols));
+    }
+    for (int i = tid; i < 4 * M; i += kFewThreads) p.part[((size_t)(i >> 2) * gridDim.x + blockIdx.x) * 4 + (i & 3)] = meet[i & 3][i >> 2];
+}
+
+// The tiles of a row joined, a warp per row; where totals are asked for, the last block to come sums the rows, in their order.
 constexpr int kJoinWarps = 8;
 __global__ void __launch_bounds__(32 * kJoinWarps) loss_join_kernel(const float2* __restrict__ part, const float* __restrict__ hit, int M, int V, int tiles, const void* targets,
                                                                     int targets64, long long ignore, float c, float* __restrict__ loss, float2* kept, float* __restrict__ totals,
                                                                     unsigned* arrived) {
     const int lane = threadIdx.x & 31, row = blockIdx.x * kJoinWarps + (threadIdx.x >> 5);
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");        // (launched while the tiles are on their way)
     if (row < M) {
         const float2* const p = part + (size_t)row * tiles;
         float most = -CUDART_INF_F, sum = 0.f;
@@ -411,6 +575,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) loss_join_kernel(const float2
             if (loss) loss[row] = l;
         }
     }
+    if (!totals) return;
     __shared__ bool last;
     __shared__ int counts[kJoinWarps];
     __threadfence();
@@ -552,6 +717,25 @@ cudaError_t run_tiles(const CUtensorMap& a, const CUtensorMap& b, LossTiles p, i
     return cudaGetLastError();
 }
 
+template <int NB, int TERMS>
+cudaError_t run_few(const CUtensorMap& h, const CUtensorMap& w, LossTiles p, int grid, int dev, cudaStream_t st) {
+    const cudaError_t e = ask_smem<loss_few_rows_kernel<NB, TERMS>>(dev, Few<NB, TERMS>::kSmem);
+    if (e != cudaSuccess) return e;
+    p.polls = gemm_pair_polls();
+    p.ran_out = split_attention_ran_out(dev, st);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(kFewThreads);
+    cfg.dynamicSmemBytes = Few<NB, TERMS>::kSmem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, loss_few_rows_kernel<NB, TERMS>, h, w, p);
+}
+
 int padded(int K) { return (K + 7) / 8 * 8; }
 bool in_place(const void* x, long long ld) { return (reinterpret_cast<uintptr_t>(x) & 15) == 0 && ld % 8 == 0; }
 size_t up(size_t n) { return (n + 255) / 256 * 256; }
@@ -575,10 +759,12 @@ int shares_of(int length, int most) {
 
 // What a call keeps in its workspace, one after the other
 struct Room {
-    size_t h = 0, h_dw = 0, w = 0, part = 0, hit = 0, arrived = 0, p = 0, acc = 0, all = 0;      // offsets
+    size_t h = 0, h_dw = 0, w = 0, part = 0, hit = 0, arrived = 0, kept = 0, p = 0, acc = 0, all = 0;      // offsets
+    bool few = false;
+    int parts = 0;                                                                      // of a row's logits
     int piece = 0, splits = 1;                                                          // columns of a piece of the vocabulary, shares of dh's contraction
 };
-Room room_of(const LossShape& s, bool grad, bool rows, bool head) {
+Room room_of(const LossShape& s, bool grad, bool rows, bool head, int sms) {
     Room r;
     size_t at = 0;
     const auto take = [&](size_t bytes) { const size_t was = at; at += up(bytes); return was; };
@@ -587,9 +773,12 @@ Room room_of(const LossShape& s, bool grad, bool rows, bool head) {
     r.h_dw = take(grad && head ? row : 0);
     r.w = take(in_place(s.w, s.ldw) ? 0 : (size_t)s.V * padded(s.K) * 2);
     if (!grad) {
-        r.part = take((size_t)s.M * ((s.V + kTileN - 1) / kTileN) * 16);
+        r.few = s.M <= kFewMost;
+        r.parts = r.few ? (int)std::min<long long>((s.V + 127) / 128, 2 * sms) * 4 : 2 * ((s.V + kTileN - 1) / kTileN);
+        r.part = take((size_t)s.M * r.parts * 8);
         r.hit = take((size_t)s.M * 4);
         r.arrived = take(4);
+        r.kept = take((size_t)s.M * 8);
     } else {
         const long long all = (s.V + 255) / 256 * 256LL, fit = (64LL << 20) / 2 / s.M / 256 * 256;
         r.piece = (int)std::min(all, std::max(4096LL, fit));
@@ -614,15 +803,18 @@ LossTiles tiles_of(const LossShape& s) {
 
 }  // namespace
 
-size_t loss_work_bytes(const LossShape& s) { return room_of(s, false, false, false).all; }
-size_t loss_grad_work_bytes(const LossShape& s, bool rows, bool head) { return room_of(s, true, rows, head).all; }
+size_t loss_work_bytes(const LossShape& s) {
+    int dev = 0, sms = 0;
+    return current_sms(&dev, &sms) == cudaSuccess ? room_of(s, false, false, false, sms).all : 0;
+}
+size_t loss_grad_work_bytes(const LossShape& s, bool rows, bool head) { return room_of(s, true, rows, head, 0).all; }
 
 cudaError_t launch_loss(const LossShape& s, float* loss, float* kept, float* totals, void* work, cudaStream_t st) {
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
+    int dev = 0, sms = 0;
+    cudaError_t e = current_sms(&dev, &sms);
     if (e != cudaSuccess) return e;
     if (take_ran_out(dev, st)) return cudaErrorLaunchTimeout;
-    const Room r = room_of(s, false, false, false);
+    const Room r = room_of(s, false, false, false, sms);
     unsigned char* const base = reinterpret_cast<unsigned char*>(work);
     const void *h = s.h, *w = s.w;
     long long ldh = s.ldh, ldw = s.ldw;
@@ -638,20 +830,30 @@ cudaError_t launch_loss(const LossShape& s, float* loss, float* kept, float* tot
         e = pack<1, false>(s.w, s.ldw, s.V, s.K, base + r.w, nullptr, st);
     }
     if (e != cudaSuccess) return e;
-    unsigned* const arrived = reinterpret_cast<unsigned*>(base + r.arrived);
+    const int columns = s.M <= 16 ? 16 : 32;
     CUtensorMap ma, mb;
-    if (!bf16_map(&ma, h, (long long)s.M * (f32 ? 3 : 1), s.K, ldh, 128) || !bf16_map(&mb, w, s.V, s.K, ldw, 128)) return cudaErrorNotSupported;
+    if (!bf16_map(&ma, h, (long long)s.M * (f32 ? 3 : 1), s.K, ldh, r.few ? columns : 128) || !bf16_map(&mb, w, s.V, s.K, ldw, 128)) return cudaErrorNotSupported;
     LossTiles p = tiles_of(s);
     p.M = s.M; p.N = s.V; p.K = s.K;
     p.part = reinterpret_cast<float2*>(base + r.part);
     p.hit = reinterpret_cast<float*>(base + r.hit);
-    p.arrived = arrived;
-    e = f32 ? run_tiles<kStats, 3>(ma, mb, p, dev, st) : run_tiles<kStats, 1>(ma, mb, p, dev, st);
+    p.arrived = reinterpret_cast<unsigned*>(base + r.arrived);
+    if (!r.few) e = f32 ? run_tiles<kStats, 3>(ma, mb, p, dev, st) : run_tiles<kStats, 1>(ma, mb, p, dev, st);
+    else if (columns == 16) e = f32 ? run_few<16, 3>(ma, mb, p, r.parts / 4, dev, st) : run_few<16, 1>(ma, mb, p, r.parts / 4, dev, st);
+    else e = f32 ? run_few<32, 3>(ma, mb, p, r.parts / 4, dev, st) : run_few<32, 1>(ma, mb, p, r.parts / 4, dev, st);
     if (e != cudaSuccess) return e;
     ++extra_launches();
-    loss_join_kernel<<<(s.M + kJoinWarps - 1) / kJoinWarps, 32 * kJoinWarps, 0, st>>>(p.part, p.hit, s.M, s.V, 2 * ((s.V + kTileN - 1) / kTileN), s.targets, s.targets64,
-                                                                                    s.ignore, p.c, loss, reinterpret_cast<float2*>(kept), totals, arrived);
-    return cudaGetLastError();
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((s.M + kJoinWarps - 1) / kJoinWarps);
+    cfg.blockDim = dim3(32 * kJoinWarps);
+    cfg.stream = st;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, loss_join_kernel, (const float2*)p.part, (const float*)p.hit, s.M, s.V, r.parts, s.targets, s.targets64, s.ignore, p.c, loss,
+                              kept ? reinterpret_cast<float2*>(kept) : reinterpret_cast<float2*>(base + r.kept), totals, p.arrived);
 }
 
 cudaError_t launch_loss_grad(const LossShape& s, const float* kept, const LossGrad& by, void* dh, void* dw, void* work, cudaStream_t st) {
@@ -659,7 +861,7 @@ cudaError_t launch_loss_grad(const LossShape& s, const float* kept, const LossGr
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     if (take_ran_out(dev, st)) return cudaErrorLaunchTimeout;
-    const Room r = room_of(s, true, dh != nullptr, dw != nullptr);
+    const Room r = room_of(s, true, dh != nullptr, dw != nullptr, 0);
     unsigned char* const base = reinterpret_cast<unsigned char*>(work);
     const void *h = s.h, *w = s.w;
     long long ldh = s.ldh, ldw = s.ldw;

@@ -17,7 +17,7 @@ struct LossShape {
 };
 // The operands that are laid out again in the workspace: rows that are fp32 or not of 16 bytes, a head whose rows are not
 size_t loss_work_bytes(const LossShape& s);
-// loss [M] (or null), kept [M][2]: log sum_j exp z[i][j] and the loss, for the gradient; totals [3]: the sum of the losses, how many rows count, their mean (0 where none does)
+// loss [M] (or null), kept [M][2]: log sum_j exp z[i][j] and the loss, for the gradient, or null; totals [3]: the sum of the losses, how many rows count, their mean (0 where none does), or null
 cudaError_t launch_loss(const LossShape& s, float* loss, float* kept, float* totals, void* work, cudaStream_t st);
 
 // The gradient by rows (dh [M][K] bf16) and by the head (dw [V][K] bf16), either or both; h is bf16

@@ -4,6 +4,7 @@
 // E2M1 number, 6), at least 2^-127; its elements are x 2^-e to the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6 (half way: to the even code), 6 beyond.  Both steps are exact
 // but for that last one, so every implementation of the rule has the same bits.
 #include <algorithm>
+#include <type_traits>
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -336,6 +337,184 @@ mxfp4_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
     }
 }
 
+// Few rows (decoding, a short portion): the weights are the 128-row operand and stream once, the rows are the columns.  A cluster of S CTAs owns 128 weight rows, each
+// CTA a range of stages.
+//   warp 0    requests the CTA's weight codes and scales ahead of the rows - before the kernel's predecessor has ended (nothing that lets its successor start early
+//             writes weights)
+//   all warps round the CTA's share of the rows to MXFP4, straight into the layout of the MMA (the rows are read S times less than once per CTA)
+//   warp 1    per stage the scales into tensor memory and its MMAs (M = 128, N = NB)
+//   warps 2-5 take the accumulator out (weight row = lane); with S > 1 the shares meet in shared memory, in the order of the ranges
+// Bound: the weights' bytes where there are many, latency else.  Tensor memory is taken behind the wait for the predecessor and in front of the signal to the successor:
+// a CTA that waits for another kernel holds none of it, so neither can wait for the other.  Shared memory is asked for such that an SM holds three CTAs at most, whose
+// tensor memory fits at the same time: CTAs of a cluster wait for one another.
+constexpr int kFewMost = 64, kFewCols = 128, kFewSmemMost = 226 * 1024, kFewSmemLeast = 58 * 1024, kFewSlotsMost = 12;
+static_assert(4 * kFewSmemLeast > 228 * 1024 && 4 * kFewCols <= 512, "CTAs on an SM");
+
+struct FewProduct {
+    const void* a; long long lda; int a_type, wide;
+    const uint8_t* w_scales;
+    void* y; int y_type;
+    int M, N, K, per, slots;                                  // stages of a CTA, of the ring
+    int* ran_out;
+    unsigned polls;
+};
+
+__device__ __forceinline__ void put1(void* y, int type, size_t at, float v) {
+    if (type == kTypeF32) reinterpret_cast<float*>(y)[at] = v;
+    else if (type == kTypeBf16) reinterpret_cast<__nv_bfloat16*>(y)[at] = __float2bfloat16_rn(v);
+    else reinterpret_cast<__half*>(y)[at] = __float2half_rn(v);
+}
+
+template <int NB>
+__global__ void __launch_bounds__(kThreads4, 1) mxfp4_few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ FewProduct p) {
+    constexpr int kSlot = kCodeTile + 1024, kRows = NB * 128 + 1024;       // a stage of weights, of rows
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    __shared__ uint64_t full[kFewSlotsMost], empty[kFewSlotsMost], t_full;
+    __shared__ uint32_t tmem_slot;
+    unsigned char* const ring = smem;
+    unsigned char* const rows = ring + p.slots * kSlot;                     // [per][NB x 128 bytes | 2 x 512 bytes of scales]
+    float* const part = reinterpret_cast<float*>(rows + p.per * kRows);     // [NB][128]
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, S = gridDim.y, rank = blockIdx.y, n0 = blockIdx.x * 128, M = p.M;
+    const int pieces = (p.K + 127) / 128, n_stage = (pieces + 1) / 2, s0 = rank * p.per, stages = max(0, min(p.per, n_stage - s0));
+    const auto request = [&](int s, int slot) {
+        unsigned char* const dst = ring + slot * kSlot;
+        const uint32_t sc = kMxScaleBytes * min(2, pieces - 2 * (s0 + s));
+        mbar_arrive_expect_tx(&full[slot], kCodeTile + sc);
+        tma_load_2d(smem_u32(dst), &map_w, smem_u32(&full[slot]), (s0 + s) * (kStageK / 2), n0);
+        bulk_g2s(dst + kCodeTile, p.w_scales + ((size_t)blockIdx.x * pieces + 2 * (s0 + s)) * kMxScaleBytes, sc, &full[slot]);
+    };
+    if (tid == 0) {
+        for (int i = 0; i < p.slots; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
+        mbar_init(&t_full, 1);
+        fence_mbar_init();
+        for (int s = 0; s < min(stages, p.slots); ++s) request(s, s);
+    }
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(kFewCols));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+    }
+    // ---- the rows: eight channels an item, four neighbours a block; kBatch loads in flight (one after the other, 8 rows x 2048 took 11 of 18 us) ----
+    const int per_row = stages * 32, items = M * per_row;
+    const auto place = [&](int m, int c) { return rows + (c >> 5) * kRows + (m >> 3) * 1024 + (m & 7) * 128 + ((((c & 31) >> 2) ^ (m & 7)) << 4) + (c & 3) * 4; };
+    const auto take = [&](auto type) {
+        constexpr int TYPE = decltype(type)::value, kBatch = TYPE == kTypeF32 ? 4 : 8;
+        for (int i0 = tid; i0 < items; i0 += kThreads4 * kBatch) {           // (a warp is in or out as a whole)
+            float v[kBatch][8];
+#pragma unroll
+            for (int b = 0; b < kBatch; ++b) {
+                const int i = i0 + b * kThreads4, m = i / per_row, k = s0 * kStageK + 8 * (i - m * per_row);
+                load8<TYPE>(reinterpret_cast<const char*>(p.a) + (long long)m * p.lda * (TYPE == kTypeF32 ? 4 : 2), k, i < items ? p.K - k : 0, p.wide, v[b]);
+            }
+#pragma unroll
+            for (int b = 0; b < kBatch; ++b) {
+                const int i = i0 + b * kThreads4, m = i / per_row, c = i - m * per_row;
+                if (i >= items) break;
+                uint32_t scale;
+                *reinterpret_cast<uint32_t*>(place(m, c)) = round_block(v[b], scale);
+                if ((c & 3) == 0) rows[(c >> 5) * kRows + NB * 128 + ((c & 31) >> 4) * kMxScaleBytes + (m & 31) * 16 + (m >> 5) * 4 + ((c >> 2) & 3)] = (uint8_t)scale;
+            }
+        }
+    };
+    if (p.a_type == kTypeF32) take(std::integral_constant<int, kTypeF32>());
+    else if (p.a_type == kTypeBf16) take(std::integral_constant<int, kTypeBf16>());
+    else take(std::integral_constant<int, kTypeF16>());
+    for (int i = tid; i < (NB - M) * per_row; i += kThreads4) {               // columns that no row uses
+        const int m = M + i / per_row, c = i % per_row;
+        *reinterpret_cast<uint32_t*>(place(m, c)) = 0u;
+        if ((c & 3) == 0) rows[(c >> 5) * kRows + NB * 128 + ((c & 31) >> 4) * kMxScaleBytes + (m & 31) * 16 + (m >> 5) * 4 + ((c >> 2) & 3)] = 0;
+    }
+    fence_proxy_async();
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const uint32_t tmem = tmem_slot;
+    bool ok = true;
+    if (warp == 0) {
+        if (lane == 0) {
+            for (int s = p.slots; s < stages && ok; ++s) {
+                const int slot = s % p.slots;
+                ok = lane_wait(&empty[slot], ((s / p.slots) & 1u) ^ 1u, p.polls);
+                if (ok) request(s, slot);
+            }
+            if (!ok)                                          // (copies in flight arrive before the CTA goes)
+                for (int s = 0; s < min(stages, p.slots); ++s) (void)lane_wait(&full[s], 0, p.polls);
+        }
+    } else if (warp == 1) {
+        const uint32_t idesc[2] = {mx_idesc(NB, 0), mx_idesc(NB, 1)};
+        for (int s = 0; s < stages && ok; ++s) {
+            const int slot = s % p.slots;
+            if (!pair_wait(&full[slot], (s / p.slots) & 1u, p.polls)) { ok = false; break; }
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const uint32_t wa = smem_u32(ring + slot * kSlot), ra = smem_u32(rows + s * kRows);
+            const uint64_t adesc = umma_desc(wa), bdesc = umma_desc(ra);
+            const uint32_t sa = tmem + 64 + (s & 3) * 16, sb = sa + 8;
+            const int here = min(2, pieces - 2 * (s0 + s));
+            if (elect_one_sync()) {
+                for (int c = 0; c < here; ++c) {
+                    scales_to_tmem(sa + 4 * c, scale_desc(wa + kCodeTile + c * kMxScaleBytes));
+                    scales_to_tmem(sb + 4 * c, scale_desc(ra + NB * 128 + c * kMxScaleBytes));
+                }
+                for (int c = 0; c < here; ++c)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+                        umma_mxfp4(tmem, adesc + 4 * c + 2 * j, bdesc + 4 * c + 2 * j, idesc[j], sa + 4 * c, sb + 4 * c, (s | c | j) != 0 ? 1u : 0u);
+                umma_commit(&empty[slot]);
+                if (s == stages - 1) umma_commit(&t_full);
+            }
+            __syncwarp();
+        }
+    } else {
+        ok = stages == 0 || pair_wait(&t_full, 0, p.polls);   // (the last CTAs of a cluster may have none: zeros)
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const int c = (warp & 3) * 32 + lane;
+        const int n = n0 + c;
+#pragma unroll
+        for (int m0 = 0; m0 < NB; m0 += 16) {
+            if (m0 >= M) break;
+            uint32_t v[16];
+            tmem_columns16(tmem + ((uint32_t)((warp & 3) * 32) << 16) + m0, v);
+            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const float f = !ok ? CUDART_NAN_F : stages ? __uint_as_float(v[e]) : 0.f;          // (NaN: no result)
+                if (S > 1) part[(m0 + e) * 128 + c] = f;
+                else if (m0 + e < M && n < p.N) put1(p.y, p.y_type, (size_t)(m0 + e) * p.N + n, f);
+            }
+        }
+    }
+    if (!ok && lane == 0 && p.ran_out) {
+        *reinterpret_cast<volatile int*>(p.ran_out) = 1;
+        __threadfence_system();
+    }
+    __syncwarp();
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (warp == 1) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kFewCols));
+    }
+    if (S > 1) {
+        cluster_sync_all();
+        // the outputs of the tile, dealt to the cluster's CTAs
+        for (int i = rank * kThreads4 + tid; i < M * 128; i += S * kThreads4) {
+            const int m = i >> 7, n = n0 + (i & 127);
+            if (n >= p.N) continue;
+            float u[8];
+#pragma unroll
+            for (int r = 0; r < 8; ++r) u[r] = r < S ? load_remote(part + i, r) : 0.f;
+            float v = u[0];
+#pragma unroll
+            for (int r = 1; r < 8; ++r)
+                if (r < S) v += u[r];
+            put1(p.y, p.y_type, (size_t)m * p.N + n, v);
+        }
+        cluster_sync_all();                                   // (the shares stay until every CTA has read them)
+    }
+}
+
 // codes [rows][stride / 2] in boxes of box_rows x 128 bytes
 bool codes_map(CUtensorMap* map, const void* codes, int rows, int K, int box_rows) {
     const EncodeTiledFn enc = encode_tiled();
@@ -359,6 +538,54 @@ cudaError_t run_tiled(const Mxfp4Product& p, const uint8_t* a_codes, const uint8
     return cudaGetLastError();
 }
 
+// CTAs of a cluster, and what they hold: as many CTAs as the chip has SMs, two stages each while there are that many (one beyond that would cost more in joining
+// shares than it saves)
+bool few_plan(int M, int N, int K, int& NB, int& S, int& per, int& slots, size_t& smem) {
+    if (M > kFewMost) return false;
+    NB = M <= 16 ? 16 : M <= 32 ? 32 : 64;
+    const long long tiles = (N + 127) / 128, n_stage = (mx_stride(K) / 128 + 1) / 2;
+    const size_t slot = kCodeTile + 1024, row = NB * 128 + 1024;
+    for (S = 1; S < 8 && n_stage >= 2 * S && tiles * S < 120; S *= 2) {}
+    for (;; S *= 2) {
+        if (S > 8) return false;
+        const long long each = (n_stage + S - 1) / S;
+        const size_t fixed = 1024 + each * row + (S > 1 ? NB * 512 : 0);
+        if (fixed + std::min<long long>(each, 2) * slot > (size_t)kFewSmemMost) continue;
+        per = (int)each;
+        slots = (int)std::min<long long>(each, kFewSlotsMost);
+        // two CTAs on an SM where four stages fit: the next launch's weights are then requested while this one runs
+        while (slots > 4 && fixed + slots * slot > (size_t)kFewSmemMost / 2) --slots;
+        while (fixed + slots * slot > (size_t)kFewSmemMost) --slots;
+        smem = std::max<size_t>(fixed + slots * slot, kFewSmemLeast);
+        return tiles <= 0x7fffffffLL;
+    }
+}
+
+template <int NB>
+cudaError_t run_few(const Mxfp4Product& p, int S, int per, int slots, size_t smem, int dev, cudaStream_t st) {
+    const cudaError_t e = ask_smem<mxfp4_few_rows_kernel<NB>>(dev, kFewSmemMost);
+    if (e != cudaSuccess) return e;
+    CUtensorMap mw;
+    if (!codes_map(&mw, p.w_codes, p.N, p.K, 128)) return cudaErrorNotSupported;
+    const int wide = (reinterpret_cast<uintptr_t>(p.a) & 15) == 0 && p.lda * type_bytes(p.a_type) % 16 == 0;
+    const FewProduct q{p.a, p.lda, p.a_type, wide, reinterpret_cast<const uint8_t*>(p.w_scales), p.y, p.y_type, p.M, p.N, p.K, per, slots, p.ran_out, p.polls};
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((p.N + 127) / 128, S);
+    cfg.blockDim = dim3(kThreads4);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = 1;
+    attr[1].val.clusterDim.y = S;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = S > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, mxfp4_few_rows_kernel<NB>, mw, q);
+}
+
 }  // namespace
 
 cudaError_t launch_mxfp4_quantize(const void* x, int type, long long ld, int rows, int K, void* codes, void* scales, cudaStream_t st) {
@@ -379,7 +606,12 @@ cudaError_t launch_mxfp4_dequantize(const void* codes, const void* scales, int r
     return cudaGetLastError();
 }
 
-size_t mxfp4_linear_work_bytes(int M, int K) { return (mx_code_bytes(M, K) + 127) / 128 * 128 + mx_scale_bytes(M, K); }
+size_t mxfp4_linear_work_bytes(int M, int N, int K) {
+    int NB, S, per, slots;
+    size_t smem;
+    if (few_plan(M, N, K, NB, S, per, slots, smem)) return 0;
+    return (mx_code_bytes(M, K) + 127) / 128 * 128 + mx_scale_bytes(M, K);
+}
 
 cudaError_t launch_mxfp4_linear(Mxfp4Product p, void* work, cudaStream_t st) {
     int dev = 0, sms = 0;
@@ -388,6 +620,10 @@ cudaError_t launch_mxfp4_linear(Mxfp4Product p, void* work, cudaStream_t st) {
     p.ran_out = split_attention_ran_out(dev, st);
     p.polls = gemm_pair_polls();
     if (take_ran_out(dev, st)) return cudaErrorLaunchTimeout;
+    int NB, S, per, slots;
+    size_t smem;
+    if (few_plan(p.M, p.N, p.K, NB, S, per, slots, smem))
+        return NB == 16 ? run_few<16>(p, S, per, slots, smem, dev, st) : NB == 32 ? run_few<32>(p, S, per, slots, smem, dev, st) : run_few<64>(p, S, per, slots, smem, dev, st);
     uint8_t* const codes = reinterpret_cast<uint8_t*>(work);
     uint8_t* const scales = codes + (mx_code_bytes(p.M, p.K) + 127) / 128 * 128;
     e = launch_mxfp4_quantize(p.a, p.a_type, p.lda, p.M, p.K, codes, scales, st);

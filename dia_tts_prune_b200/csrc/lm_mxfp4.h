@@ -32,7 +32,7 @@ struct Mxfp4Product {
     int* ran_out;
     unsigned polls;
 };
-size_t mxfp4_linear_work_bytes(int M, int K);
+size_t mxfp4_linear_work_bytes(int M, int N, int K);
 cudaError_t launch_mxfp4_linear(Mxfp4Product p, void* work, cudaStream_t st);
 
 }  // namespace lm

@@ -8,45 +8,86 @@ any.  Arguments are checked on the host (``ValueError``, ``TypeError``); there i
 
 from __future__ import annotations
 
-from dataclasses import dataclass
+from functools import lru_cache
 
 import torch
 
 from . import _lm_lib
-from .lm_engine import _stream
 
 _TYPES = {torch.float32: _lm_lib.TYPE_FP32, torch.bfloat16: _lm_lib.TYPE_BF16, torch.float16: _lm_lib.TYPE_FP16}
 
 
-def _check_rows(x: torch.Tensor, name: str, types=tuple(_TYPES)) -> None:
+def _names(types) -> str:
+    return ", ".join(str(t) for t in types)
+
+
+def _check_rows(x: torch.Tensor, name: str, types=_TYPES) -> None:
     if not isinstance(x, torch.Tensor):
         raise TypeError(f"{name} must be a tensor")
     if x.dtype not in types:
-        raise TypeError(f"{name} must be one of {', '.join(str(t) for t in types)}, not {x.dtype}")
+        raise TypeError(f"{name} must be one of {_names(types)}, not {x.dtype}")
     if not x.is_cuda:
         raise ValueError(f"{name} must live on a CUDA device (there is no CPU fallback)")
 
 
+def _call(what: str, device: torch.device, *args) -> None:
+    """The library's function ``lm_b200_op_<what>`` on the device's current stream, as its last argument."""
+    fn, stream = getattr(_lm_lib.load(), "lm_b200_op_" + what), torch._C._cuda_getCurrentRawStream(device.index)
+    if torch.cuda.current_device() == device.index:
+        rc = fn(*args, stream)
+    else:
+        with torch.cuda.device(device.index):
+            rc = fn(*args, stream)
+    if rc:
+        _lm_lib.check(rc, what)
+
+
+# Bytes of a call's workspace go by its sizes and by whether its operands can be read where they are, which the library decides; the answers
+# are kept (asking takes the host 1 to 2 us).  Of an address only the alignment counts.
+@lru_cache(maxsize=1024)
+def _linear_work_bytes(m: int, n: int, k: int) -> int:
+    return _lm_lib.load().lm_b200_op_linear_mxfp4_work_bytes(m, n, k)
+
+
+@lru_cache(maxsize=1024)
+def _loss_work_bytes(h_at: int, h_type: int, ldh: int, w_at: int, ldw: int, m: int, v: int, k: int, device: int) -> int:
+    with torch.cuda.device(device):
+        return _lm_lib.load().lm_b200_op_loss_work_bytes(h_at | 4096, h_type, ldh, w_at | 4096, ldw, m, v, k)
+
+
+@lru_cache(maxsize=1024)
+def _loss_grad_work_bytes(h_at: int, ldh: int, w_at: int, ldw: int, m: int, v: int, k: int, rows: bool, head: bool) -> int:
+    return _lm_lib.load().lm_b200_op_loss_grad_work_bytes(h_at | 4096, ldh, w_at | 4096, ldw, m, v, k, rows, head)
+
+
 def _as_rows(x: torch.Tensor) -> torch.Tensor:
     """``x [..., K]`` as rows with neighbouring channels (a view where the strides allow one)."""
-    x = x.reshape(-1, x.shape[-1])
+    if x.dim() != 2:
+        x = x.reshape(-1, x.shape[-1])
+    rows, width = x.shape
+    if rows > 0x7fffff00 or width > 1 << 24:
+        raise ValueError(f"{rows} rows of {width} channels are more than an operator takes")
+    apart, step = x.stride()
     # (overlapping or backward rows are copied; a row stride is only read where there are several rows)
-    return x if (x.shape[1] == 1 or x.stride(1) == 1) and (x.shape[0] <= 1 or x.stride(0) >= x.shape[1]) else x.contiguous()
+    return x if (width == 1 or step == 1) and (rows <= 1 or apart >= width) else x.contiguous()
 
 
-def _no_grad(what: str, *tensors: torch.Tensor) -> None:
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
-        raise ValueError(f"{what} has no gradient: detach its inputs or call it under torch.no_grad()")
+def _no_grad(what: str, x: torch.Tensor) -> None:
+    if x.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{what} has no gradient: detach its rows or call it under torch.no_grad()")
 
 
-@dataclass(frozen=True)
 class Mxfp4:
     """Rows ``[rows, width]`` in microscaled 4-bit numbers: blocks of 32 channels share a power of two (E8M0), elements are E2M1.
-    ``codes`` and ``scales`` are uint8 buffers in the kernels' layout."""
-    codes: torch.Tensor
-    scales: torch.Tensor
-    rows: int
-    width: int
+    ``data`` holds the codes and, from ``scales_at`` on, the scales, both as the kernels read them (4.25 bits a channel)."""
+    __slots__ = ("data", "rows", "width", "scales_at")
+
+    def __init__(self, rows: int, width: int, device: torch.device):
+        """Room for so many rows (their numbers are not set; see :func:`quantize_mxfp4`)."""
+        stride = (width + 127) // 128 * 128
+        self.rows, self.width = rows, width
+        self.scales_at = (rows * (stride // 2) + 127) // 128 * 128
+        self.data = torch.empty(self.scales_at + (rows + 127) // 128 * (stride // 128) * 512, dtype=torch.uint8, device=device)
 
     @property
     def shape(self) -> torch.Size:
@@ -54,21 +95,21 @@ class Mxfp4:
 
     @property
     def device(self) -> torch.device:
-        return self.codes.device
+        return self.data.device
 
     @property
     def nbytes(self) -> int:
-        return self.codes.numel() + self.scales.numel()
+        return self.data.numel()
 
     def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
         """The values ``[rows, width]`` that the 4-bit numbers stand for."""
         if dtype not in _TYPES:
-            raise TypeError(f"dtype must be one of {', '.join(str(t) for t in _TYPES)}, not {dtype}")
-        out = torch.empty((self.rows, self.width), dtype=dtype, device=self.device)
-        if out.numel():
-            with torch.cuda.device(self.device):
-                _lm_lib.check(_lm_lib.load().lm_b200_op_mxfp4_dequantize(self.codes.data_ptr(), self.scales.data_ptr(), self.rows, self.width,
-                                                                         out.data_ptr(), _TYPES[dtype], _stream(self.device)), "mxfp4_dequantize")
+            raise TypeError(f"dtype must be one of {_names(_TYPES)}, not {dtype}")
+        device = self.data.device
+        out = torch.empty((self.rows, self.width), dtype=dtype, device=device)
+        if self.rows and self.width:
+            at = self.data.data_ptr()
+            _call("mxfp4_dequantize", device, at, at + self.scales_at, self.rows, self.width, out.data_ptr(), _TYPES[dtype])
         return out
 
 
@@ -76,21 +117,18 @@ def quantize_mxfp4(x: torch.Tensor) -> Mxfp4:
     """``x [rows, width]`` (float32, bfloat16 or float16; rows of any stride) in MXFP4, rounded as the OCP Microscaling specification
     says: a block's scale is ``2 ** (floor(log2(largest magnitude)) - 2)``, at least ``2 ** -127``; elements go to the nearest of 0, 0.5,
     1, 1.5, 2, 3, 4, 6 times the scale, half way to the even code, what lies beyond 6 to 6.  A block with an infinity or a NaN stands
-    for NaNs.  The last block of a row may be short."""
+    for NaNs.  The last block of a row may be short.  It has no gradient."""
     _check_rows(x, "x")
     if x.dim() != 2:
         raise ValueError(f"x must have two dimensions, not {x.dim()}")
     _no_grad("quantize_mxfp4", x)
-    rows, width = x.shape
-    lib = _lm_lib.load()
-    codes = torch.empty(lib.lm_b200_mxfp4_code_bytes(rows, width), dtype=torch.uint8, device=x.device)
-    scales = torch.empty(lib.lm_b200_mxfp4_scale_bytes(rows, width), dtype=torch.uint8, device=x.device)
-    if x.numel():
-        x = _as_rows(x)
-        with torch.cuda.device(x.device):
-            _lm_lib.check(lib.lm_b200_op_mxfp4_quantize(x.data_ptr(), _TYPES[x.dtype], x.stride(0), rows, width, codes.data_ptr(),
-                                                        scales.data_ptr(), _stream(x.device)), "mxfp4_quantize")
-    return Mxfp4(codes, scales, rows, width)
+    x = _as_rows(x)
+    (rows, width), device = x.shape, x.device
+    q = Mxfp4(rows, width, device)
+    if rows and width:
+        at = q.data.data_ptr()
+        _call("mxfp4_quantize", device, x.data_ptr(), _TYPES[x.dtype], x.stride(0), rows, width, at, at + q.scales_at)
+    return q
 
 
 def linear_mxfp4(a: torch.Tensor, w: Mxfp4, out_dtype: torch.dtype | None = None) -> torch.Tensor:
@@ -100,27 +138,27 @@ def linear_mxfp4(a: torch.Tensor, w: Mxfp4, out_dtype: torch.dtype | None = None
     _check_rows(a, "a")
     if not isinstance(w, Mxfp4):
         raise TypeError("w must be an Mxfp4 (see quantize_mxfp4)")
-    if a.dim() < 1 or a.shape[-1] != w.width:
+    if not a.dim() or a.shape[-1] != w.width:
         raise ValueError(f"a has rows of {a.shape[-1] if a.dim() else 0} channels, w of {w.width}")
-    if a.device != w.device:
-        raise ValueError(f"a lives on {a.device}, w on {w.device}")
-    out_dtype = a.dtype if out_dtype is None else out_dtype
-    if out_dtype not in _TYPES:
-        raise TypeError(f"out_dtype must be one of {', '.join(str(t) for t in _TYPES)}, not {out_dtype}")
+    device = a.device
+    if device != w.data.device:
+        raise ValueError(f"a lives on {device}, w on {w.data.device}")
+    if out_dtype is None:
+        out_dtype = a.dtype
+    elif out_dtype not in _TYPES:
+        raise TypeError(f"out_dtype must be one of {_names(_TYPES)}, not {out_dtype}")
     _no_grad("linear_mxfp4", a)
-    y = torch.empty((*a.shape[:-1], w.rows), dtype=out_dtype, device=a.device)
-    if not y.numel():
-        return y
+    y = torch.empty((*a.shape[:-1], w.rows), dtype=out_dtype, device=device)
     if not w.width:
         return y.zero_()
-    lib, rows = _lm_lib.load(), _as_rows(a)
-    M = rows.shape[0]
-    need = lib.lm_b200_op_linear_mxfp4_work_bytes(M, w.rows, w.width)
-    work = torch.empty(need, dtype=torch.uint8, device=a.device)
-    with torch.cuda.device(a.device):
-        _lm_lib.check(lib.lm_b200_op_linear_mxfp4(rows.data_ptr(), _TYPES[a.dtype], rows.stride(0), w.codes.data_ptr(), w.scales.data_ptr(),
-                                                  y.data_ptr(), _TYPES[out_dtype], M, w.rows, w.width, work.data_ptr() if need else None, need,
-                                                  _stream(a.device)), "linear_mxfp4")
+    if not y.numel():
+        return y
+    rows = _as_rows(a)
+    M, at = rows.shape[0], w.data.data_ptr()
+    need = _linear_work_bytes(M, w.rows, w.width)
+    work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    _call("linear_mxfp4", device, rows.data_ptr(), _TYPES[a.dtype], rows.stride(0), at, at + w.scales_at, y.data_ptr(), _TYPES[out_dtype], M,
+          w.rows, w.width, work.data_ptr() if need else None, need)
     return y
 
 
@@ -131,7 +169,7 @@ def _loss_operands(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Te
         raise TypeError("targets must be a tensor")
     if targets.dtype not in (torch.int64, torch.int32):
         raise TypeError(f"targets must be int64 or int32, not {targets.dtype}")
-    if hidden.dim() < 1 or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1]:
+    if not hidden.dim() or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1]:
         raise ValueError(f"hidden {tuple(hidden.shape)} and weight {tuple(weight.shape)} do not share a width")
     if targets.shape != hidden.shape[:-1]:
         raise ValueError(f"targets {tuple(targets.shape)} do not go with hidden {tuple(hidden.shape)}")
@@ -141,26 +179,31 @@ def _loss_operands(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Te
         raise ValueError("weight is empty")
 
 
+def _losses(hidden, weight, targets, scale, ignore_index, reduction, keep):
+    """(losses or their sum or mean; with ``keep`` what the gradient needs: [log-sum, loss] of every row, and how many rows count)."""
+    h, w, t = _as_rows(hidden), _as_rows(weight), targets.contiguous()
+    (M, K), V, device = h.shape, w.shape[0], h.device
+    each = reduction == "none"
+    out = torch.empty(M if each else 3, dtype=torch.float32, device=device)
+    kept = torch.empty(2 * M, dtype=torch.float32, device=device) if keep else None
+    h_at, w_at, out_at, h_type, ldh, ldw = h.data_ptr(), w.data_ptr(), out.data_ptr(), _TYPES[h.dtype], h.stride(0), w.stride(0)
+    need = _loss_work_bytes(h_at & 255, h_type, ldh, w_at & 255, ldw, M, V, K, device.index)
+    work = torch.empty(need, dtype=torch.uint8, device=device)
+    _call("loss", device, h_at, h_type, ldh, w_at, ldw, t.data_ptr(), t.dtype == torch.int64, ignore_index, M, V, K, scale, out_at if each else None,
+          kept.data_ptr() if keep else None, None if each else out_at, work.data_ptr(), need)
+    return (out if each else out[2 if reduction == "mean" else 0]), t, kept, out
+
+
 class _LinearCrossEntropy(torch.autograd.Function):
     """Losses of rows, or (mean, sum) their total; rows are two-dimensional here."""
 
     @staticmethod
     def forward(ctx, hidden, weight, targets, scale, ignore_index, reduction):
-        lib = _lm_lib.load()
-        (M, K), V, device = hidden.shape, weight.shape[0], hidden.device
-        loss = torch.empty(M, dtype=torch.float32, device=device) if reduction == "none" else None
-        kept, totals = torch.empty(2 * M, dtype=torch.float32, device=device), torch.empty(3, dtype=torch.float32, device=device)
-        h, w, t = _as_rows(hidden), _as_rows(weight), targets.contiguous()
-        args = h.data_ptr(), _TYPES[h.dtype], h.stride(0), w.data_ptr(), w.stride(0)
-        need = lib.lm_b200_op_loss_work_bytes(*args, M, V, K)
-        work = torch.empty(need, dtype=torch.uint8, device=device)
-        with torch.cuda.device(device):
-            _lm_lib.check(lib.lm_b200_op_loss(*args, t.data_ptr(), t.dtype == torch.int64, ignore_index, M, V, K, scale,
-                                              None if loss is None else loss.data_ptr(), kept.data_ptr(), totals.data_ptr(), work.data_ptr(), need, _stream(device)), "loss")
+        out, t, kept, totals = _losses(hidden, weight, targets, scale, ignore_index, reduction, True)
         ctx.save_for_backward(hidden, weight, t, kept)
         # (the count stands beside the result, which may be changed in place: not a saved tensor)
         ctx.args = scale, ignore_index, totals[1:2].detach() if reduction == "mean" else None
-        return loss if reduction == "none" else totals[2 if reduction == "mean" else 0]
+        return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -168,23 +211,18 @@ class _LinearCrossEntropy(torch.autograd.Function):
         hidden, weight, t, kept = ctx.saved_tensors
         scale, ignore_index, count = ctx.args
         need_h, need_w = ctx.needs_input_grad[:2]
-        if hidden.dtype != torch.bfloat16:
-            raise TypeError("gradients need hidden in bfloat16")
-        lib = _lm_lib.load()
         (M, K), V, device = hidden.shape, weight.shape[0], hidden.device
         h, w, grad = _as_rows(hidden), _as_rows(weight), grad.to(torch.float32)
         if grad.dim() and grad.stride(0) < 0:
             grad = grad.contiguous()
         dh = torch.empty((M, K), dtype=hidden.dtype, device=device) if need_h else None
         dw = torch.empty((V, K), dtype=weight.dtype, device=device) if need_w else None
-        args = h.data_ptr(), h.stride(0), w.data_ptr(), w.stride(0)
-        need = lib.lm_b200_op_loss_grad_work_bytes(*args, M, V, K, need_h, need_w)
+        h_at, w_at, ldh, ldw = h.data_ptr(), w.data_ptr(), h.stride(0), w.stride(0)
+        need = _loss_grad_work_bytes(h_at & 255, ldh, w_at & 255, ldw, M, V, K, need_h, need_w)
         work = torch.empty(need, dtype=torch.uint8, device=device)
-        with torch.cuda.device(device):
-            _lm_lib.check(lib.lm_b200_op_loss_grad(
-                *args, t.data_ptr(), t.dtype == torch.int64, ignore_index, M, V, K, scale, kept.data_ptr(), grad.data_ptr(),
-                grad.stride(0) if grad.dim() else 0, count.data_ptr() if count is not None else None,
-                dh.data_ptr() if need_h else None, dw.data_ptr() if need_w else None, work.data_ptr(), need, _stream(device)), "loss_grad")
+        _call("loss_grad", device, h_at, ldh, w_at, ldw, t.data_ptr(), t.dtype == torch.int64, ignore_index, M, V, K, scale, kept.data_ptr(), grad.data_ptr(),
+              grad.stride(0) if grad.dim() else 0, None if count is None else count.data_ptr(), dh.data_ptr() if need_h else None,
+              dw.data_ptr() if need_w else None, work.data_ptr(), need)
         return dh, dw, None, None, None, None
 
 
@@ -203,11 +241,16 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
     scale, ignore_index = float(scale), int(ignore_index)
     if not 0.0 < scale < float("inf"):
         raise ValueError("scale must be positive and finite")
-    if hidden.dtype == torch.float32 and torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
+    with_grad = (hidden.requires_grad or weight.requires_grad) and torch.is_grad_enabled()
+    if with_grad and hidden.dtype != torch.bfloat16:
         raise ValueError("gradients need hidden in bfloat16")
     if not targets.numel():
         rows = hidden.new_zeros(targets.shape, dtype=torch.float32)
         return rows if reduction == "none" else rows.sum()
-    K = hidden.shape[-1]
-    loss = _LinearCrossEntropy.apply(hidden.reshape(-1, K), weight, targets.reshape(-1), scale, ignore_index, reduction)
-    return loss.view(targets.shape) if reduction == "none" else loss
+    rows = hidden if hidden.dim() == 2 else hidden.reshape(-1, hidden.shape[-1])
+    flat = targets if targets.dim() == 1 else targets.reshape(-1)
+    if with_grad:
+        loss = _LinearCrossEntropy.apply(rows, weight, flat, scale, ignore_index, reduction)
+    else:
+        loss = _losses(rows, weight, flat, scale, ignore_index, reduction, False)[0]
+    return loss.view(targets.shape) if reduction == "none" and targets.dim() != 1 else loss

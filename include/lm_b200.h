@@ -317,11 +317,12 @@ int lm_b200_op_linear_mxfp4(const void *A, int a_type, int64_t lda, const void *
 /* ---- cross entropy of rows under a head, and its gradient, without the logits in memory ----
  * z = scale h W^T (h [M][K] fp32 or bf16, row stride ldh; W [V][K] bf16, row stride ldw; scale > 0); loss[i] = log sum_j exp z[i][j] - z[i][target[i]], 0 for a row whose
  * target is `ignore`, NaN for one whose target is neither that nor in [0, V).  targets: int32, or int64 where targets64 != 0.  Operands of fp32 rows are exact to 24 bits
- * (three bf16 terms), sums fp32.  loss [M] may be NULL; kept [M][2]: log sum_j exp z[i][j] and the loss, for the gradient; totals [3]: the losses' sum, how many rows
- * count, their mean (0 where none does).
+ * (three bf16 terms), sums fp32.  loss [M] may be NULL; kept [M][2]: log sum_j exp z[i][j] and the loss, for the gradient, or NULL; totals [3]: the losses' sum, how many rows
+ * count, their mean (0 where none does), or NULL.
  * The gradient (h in bf16): P = softmax(z) - onehot, g = scale grad [/ max(*count, 1)], dh_i = g_i P_i W (bf16 [M][K]), dW = P^T (g h) (bf16 [V][K]), either may be NULL.  grad:
  * fp32, of every loss, grad_stride apart (0: one number).  Rows that do not count have no part in either, whatever they hold; a NaN loss has NaN gradients.
  * P is kept in bf16 for a piece of the vocabulary at a time.  work: 256-byte aligned. */
+/* (of h and W the alignment counts; the current device is asked for its SMs) */
 size_t lm_b200_op_loss_work_bytes(const void *h, int h_type, int64_t ldh, const void *W, int64_t ldw, int M, int V, int K);
 int lm_b200_op_loss(const void *h, int h_type, int64_t ldh, const void *W, int64_t ldw, const void *targets, int targets64, int64_t ignore, int M, int V, int K, float scale,
                     float *loss, float *kept, float *totals, void *work, size_t work_bytes, void *stream);
