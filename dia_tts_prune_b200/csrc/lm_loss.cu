@@ -32,7 +32,7 @@ namespace {
 
 using namespace dia;
 
-enum Kind { kStats, kProbs, kRows, kHead };
+enum Kind { kStats, kProbs, kGrads };
 
 constexpr int kTileN = 256, kBK = 64, kTileBytes = 128 * kBK * 2;          // 16 KB: 128 rows of an operand, 64 of the contraction
 constexpr int kWarps = 8, kThreads = 64 + 32 * kWarps, kStagesMost = 6, kTurn = kWarps * 4096;
@@ -45,18 +45,30 @@ struct Ring {
     static constexpr int kSmem = kStages * kStage + kTurn + 1024 + 256;
 };
 
-struct LossTiles {
+// Tiles of one product, and what they are made of (kGrads has two products)
+struct Tiles {
     int M, N, K;                     // rows and columns of the product, length of the contraction
-    int splits;                      // kRows: pairs that share the contraction of a tile
+    int splits;                      // pairs that share the contraction of a tile
+    __host__ __device__ int tiles_m() const { return (M + 255) / 256; }
+    __host__ __device__ int tiles_n() const { return (N + kTileN - 1) / kTileN; }
+    __host__ __device__ long long tiles() const { return N > 0 ? (long long)tiles_m() * tiles_n() * splits : 0; }
+    __host__ __device__ int blocks() const { return (K + kBK - 1) / kBK; }
+    __host__ __device__ int share() const { return (blocks() + splits - 1) / splits; }
+};
+
+struct LossTiles {
+    Tiles own;                       // kStats, kProbs: the logits; kGrads: dh
+    Tiles head;                      // kGrads: dw
+    int first_head, many, extra;     // kGrads: whether dw's tiles are the longer ones, which go first; tiles of the longer kind; the shorter ones as long as one of them
     const void* targets; int targets64; long long ignore;
     float c;                         // scale log2(e)
     unsigned* arrived;               // kStats: set to zero for the kernel that joins the tiles
     float2* part; float* hit;        // kStats: [M][2 column tiles] largest c z and sum of 2^(c z - it); [M] z of the target
     const float2* kept; int v0, V;   // kProbs: [M] lse and loss; columns v0 .. of the head
     __nv_bfloat16* p; int ldp;
-    float* acc; int ld_acc, add;     // kRows: [splits][M][ld_acc]; add: to what is there
-    __nv_bfloat16* out; int wide;    // kHead: [M][N]; wide: 16-byte stores
-    const float *grad, *count; float scale;        // kHead: what the sums are multiplied by (grad null: nothing)
+    float* acc; int ld_acc, add;     // kGrads, dh: [splits][M][ld_acc]; add: to what is there
+    __nv_bfloat16* out; int wide;    // dw: [M][N]; wide: 16-byte stores
+    const float *grad, *count; float scale;        // dw: what the sums are multiplied by (grad null: nothing)
     int* ran_out;
     unsigned polls;
 };
@@ -105,10 +117,45 @@ __device__ __forceinline__ void store_64(unsigned char* blk, const uint32_t (&y)
     __syncwarp();
 }
 
+struct Tile {
+    bool head;
+    int m, n, share, kb0, kb1;       // row and column block, share of the contraction and its k-blocks
+};
+// Tile k of a pair, false behind its last one.  Longer tiles are dealt first, one a round; the pairs that a last, partial round of them leaves out get `extra` shorter ones in
+// its place, the rest goes in rounds.  (One kind: pair, pair + pairs, ..)
+__device__ __forceinline__ bool tile_of(const LossTiles& p, int pair, int pairs, int k, Tile& t) {
+    const int all = (int)(p.own.tiles() + p.head.tiles()), few = all - p.many, left = p.many % pairs, rounds = (p.many - pair + pairs - 1) / pairs;
+    int i;
+    if (pair < p.many && k < rounds) {
+        i = pair + k * pairs;
+    } else {
+        k -= pair < p.many ? rounds : 0;
+        const int more = left ? p.extra : 0;
+        if (left && pair >= left && k < more) {
+            i = k * (pairs - left) + pair - left;
+        } else {
+            if (left && pair >= left) k -= more;
+            i = more * (pairs - left) + k * pairs + (pair - left + pairs) % pairs;
+        }
+        if (i >= few) return false;
+        i += p.many;
+    }
+    t.head = (i < p.many) == (p.first_head != 0);
+    if (i >= p.many) i -= p.many;
+    const Tiles& of = t.head ? p.head : p.own;
+    const int tm = of.tiles_m(), tn = of.tiles_n();
+    t.m = i % tm;
+    t.n = i / tm % tn;
+    t.share = i / (tm * tn);
+    t.kb0 = t.share * of.share();
+    t.kb1 = min(t.kb0 + of.share(), of.blocks());
+    return true;
+}
+
 template <int KIND, int TERMS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
-loss_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ LossTiles p) {
-    constexpr bool kAmn = KIND == kHead, kBmn = KIND == kRows || KIND == kHead;
+loss_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_ha,
+                    const __grid_constant__ CUtensorMap map_hb, const __grid_constant__ LossTiles p) {
     constexpr bool kStats_ = KIND == kStats;
     constexpr int kStage = Ring<TERMS>::kStage, kStages = Ring<TERMS>::kStages, kChunk = Ring<TERMS>::kChunk;
     extern __shared__ unsigned char smem_raw[];
@@ -123,12 +170,6 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = blockIdx.x & 1;
     const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
-    const int kb_all = (p.K + kBK - 1) / kBK, splits = KIND == kRows ? p.splits : 1, kb_per = (kb_all + splits - 1) / splits;
-    const int tiles_m = (p.M + 255) / 256, tiles_n = (p.N + kTileN - 1) / kTileN, n_tiles = tiles_m * tiles_n * splits;
-    // tile t: row block t % tiles_m, then the column block, then the share of the contraction
-    const auto first_kb = [&](int t) { return KIND == kRows ? t / (tiles_m * tiles_n) * kb_per : 0; };
-    const auto last_kb = [&](int t) { return KIND == kRows ? min(first_kb(t) + kb_per, kb_all) : kb_all; };
-
     if (KIND == kStats && blockIdx.x == 0 && threadIdx.x == 0) *p.arrived = 0u;
     if (threadIdx.x == 0) {
         for (int i = 0; i < kStages; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
@@ -148,25 +189,29 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
     if (warp == 0) {
         if (lane == 0) {
             unsigned i = 0;
-            for (int t = pair; t < n_tiles && ok; t += pairs) {
-                const int tn = t / tiles_m % tiles_n, a0 = t % tiles_m * 256 + (int)rank * 128, b0 = tn * kTileN + (int)rank * 128;
-                for (int kb = first_kb(t); kb < last_kb(t); ++kb, ++i) {
+            Tile t;
+            for (int n = 0; ok && tile_of(p, pair, pairs, n, t); ++n) {
+                const int a0 = t.m * 256 + (int)rank * 128, b0 = t.n * kTileN + (int)rank * 128;
+                for (int kb = t.kb0; kb < t.kb1; ++kb, ++i) {
                     const unsigned s = i % kStages;
                     if (!lane_wait(&empty[s], ((i / kStages) & 1u) ^ 1u, p.polls)) { ok = false; break; }
                     if (rank == 0) mbar_arrive_expect_tx(&full[s], 2u * kStage);
                     const uint32_t bar = at_rank(&full[s], 0), dst = smem_u32(smem + s * kStage), k = kb * kBK;
-                    if constexpr (kBmn) {                     // (of the head in kRows: the piece's rows)
-                        tma_load_2d_pair(dst + TERMS * kTileBytes, &map_b, bar, b0, p.v0 + k);
-                        tma_load_2d_pair(dst + TERMS * kTileBytes + kTileBytes / 2, &map_b, bar, b0 + 64, p.v0 + k);
+                    if constexpr (KIND == kGrads) {
+                        if (t.head) {
+                            tma_load_2d_pair(dst, &map_ha, bar, a0, k);
+                            tma_load_2d_pair(dst + kTileBytes / 2, &map_ha, bar, a0 + 64, k);
+                            tma_load_2d_pair(dst + kTileBytes, &map_hb, bar, b0, k);
+                            tma_load_2d_pair(dst + kTileBytes + kTileBytes / 2, &map_hb, bar, b0 + 64, k);
+                        } else {                              // (of the head the piece's rows)
+                            tma_load_2d_pair(dst, &map_a, bar, k, a0);
+                            tma_load_2d_pair(dst + kTileBytes, &map_b, bar, b0, p.v0 + k);
+                            tma_load_2d_pair(dst + kTileBytes + kTileBytes / 2, &map_b, bar, b0 + 64, p.v0 + k);
+                        }
                     } else {
                         tma_load_2d_pair(dst + TERMS * kTileBytes, &map_b, bar, k, p.v0 + b0);
-                    }
-                    if constexpr (kAmn) {
-                        tma_load_2d_pair(dst, &map_a, bar, a0, k);
-                        tma_load_2d_pair(dst + kTileBytes / 2, &map_a, bar, a0 + 64, k);
-                    } else {
 #pragma unroll
-                        for (int tm = 0; tm < TERMS; ++tm) tma_load_2d_pair(dst + tm * kTileBytes, &map_a, bar, k, tm * p.M + a0);
+                        for (int tm = 0; tm < TERMS; ++tm) tma_load_2d_pair(dst + tm * kTileBytes, &map_a, bar, k, tm * p.own.M + a0);
                     }
                 }
             }
@@ -177,14 +222,15 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
         }
     } else if (warp == 1) {
         if (rank == 0) {
-            // fp32 accumulators, bf16 operands, which of them are MN-major, N = 256, M = 256
-            const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((kAmn ? 1u : 0u) << 15) | ((kBmn ? 1u : 0u) << 16) | ((uint32_t)(kTileN >> 3) << 17) | (16u << 24);
-            constexpr uint32_t a_step = kAmn ? 2048 >> 4 : 2, b_step = kBmn ? 2048 >> 4 : 2;        // 16 of the contraction, in descriptor units
             unsigned i = 0, it = 0;                           // k-blocks and uses of an accumulator so far
-            for (int t = pair; t < n_tiles && ok; t += pairs) {
-                const int kb0 = first_kb(t), kb1 = last_kb(t);
-                for (int kb = kb0; kb < kb1; ++kb, ++i) {
-                    const bool first = kStats_ ? kb % kChunk == 0 : kb == kb0, last = kb == kb1 - 1 || (kStats_ && kb % kChunk == kChunk - 1);
+            Tile t;
+            for (int n = 0; ok && tile_of(p, pair, pairs, n, t); ++n) {
+                const bool a_mn = KIND == kGrads && t.head, b_mn = KIND == kGrads;
+                // fp32 accumulators, bf16 operands, which of them are MN-major, N = 256, M = 256
+                const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(kTileN >> 3) << 17) | (16u << 24);
+                const uint32_t a_step = a_mn ? 2048 >> 4 : 2, b_step = b_mn ? 2048 >> 4 : 2;        // 16 of the contraction, in descriptor units
+                for (int kb = t.kb0; kb < t.kb1; ++kb, ++i) {
+                    const bool first = kStats_ ? kb % kChunk == 0 : kb == t.kb0, last = kb == t.kb1 - 1 || (kStats_ && kb % kChunk == kChunk - 1);
                     if (first) {
                         if (!pair_wait(&t_empty[it & 1u], ((it >> 1) & 1u) ^ 1u, p.polls)) { ok = false; break; }
                         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -194,12 +240,12 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                     if (!pair_wait(&full[s], (i / kStages) & 1u, p.polls)) { ok = false; break; }
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     const uint32_t at = smem_u32(smem + s * kStage);
-                    const uint64_t bdesc = kBmn ? umma_desc_mn(at + TERMS * kTileBytes) : umma_desc(at + TERMS * kTileBytes);
+                    const uint64_t bdesc = b_mn ? umma_desc_mn(at + TERMS * kTileBytes) : umma_desc(at + TERMS * kTileBytes);
                     if (elect_one_sync()) {
 #pragma unroll
                         for (int u = 0; u < TERMS; ++u) {
                             const uint32_t a_at = at + (TERMS - 1 - u) * kTileBytes;                 // the smallest term first
-                            const uint64_t adesc = kAmn ? umma_desc_mn(a_at) : umma_desc(a_at);
+                            const uint64_t adesc = a_mn ? umma_desc_mn(a_at) : umma_desc(a_at);
 #pragma unroll
                             for (int j = 0; j < kBK / 16; ++j)
                                 umma_bf16_pair(d, adesc + a_step * j, bdesc + b_step * j, idesc, (u | j) != 0 || !first ? 1u : 0u);
@@ -216,7 +262,7 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
         const int q = warp & 3, c_half = (warp - 2) >> 2 << 7;               // (a warp reads the 32 lanes of its number mod 4) and its half of the columns
         unsigned char* const blk = turn + (warp - 2) * 4096;
         float factor = 1.f;
-        if (KIND == kHead && p.grad) {
+        if (KIND == kGrads && p.grad) {
             factor = *p.grad * p.scale;
             if (p.count) factor /= fmaxf(*p.count, 1.f);
         }
@@ -227,10 +273,11 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
             if (lane == 0) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(at_rank(&t_empty[it & 1u], 0)) : "memory");
             ++it;
         };
-        for (int t = pair; t < n_tiles; t += pairs) {
-            const int tn = t / tiles_m % tiles_n, n0 = tn * kTileN + c_half, row0 = t % tiles_m * 256 + (int)rank * 128 + q * 32, rows = min(32, p.M - row0);
-            const int row = row0 + lane;
-            const bool mine = row < p.M;
+        Tile t;
+        for (int tile = 0; tile_of(p, pair, pairs, tile, t); ++tile) {
+            const Tiles& of = KIND == kGrads && t.head ? p.head : p.own;
+            const int n0 = t.n * kTileN + c_half, row0 = t.m * 256 + (int)rank * 128 + q * 32, rows = min(32, of.M - row0), row = row0 + lane;
+            const bool mine = row < of.M;
             const auto from = [&]() { return tmem_base + ((uint32_t)(q * 32) << 16) + (it & 1u) * kTileN + c_half; };
             const auto wait = [&]() {
                 ok = ok && pair_wait(&t_full[it & 1u], (it >> 1) & 1u, p.polls);
@@ -242,7 +289,7 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                 float z[128];
 #pragma unroll
                 for (int e = 0; e < 128; ++e) z[e] = 0.f;
-                for (int kb = 0; kb < kb_all; kb += kChunk) {
+                for (int kb = 0; kb < of.blocks(); kb += kChunk) {
                     wait();
 #pragma unroll
                     for (int cb = 0; cb < 4; ++cb) {
@@ -254,15 +301,15 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                     }
                     taken();
                 }
-                if (mine && target >= n0 && target < n0 + 128 && target < p.N) {
+                if (mine && target >= n0 && target < n0 + 128 && target < of.N) {
                     float at = 0.f;
 #pragma unroll
                     for (int e = 0; e < 128; ++e) at = target == n0 + e ? z[e] : at;
                     p.hit[row] = ok ? at : CUDART_NAN_F;
                 }
-                if (n0 + 128 > p.N) {
+                if (n0 + 128 > of.N) {
 #pragma unroll
-                    for (int e = 0; e < 128; ++e) if (n0 + e >= p.N) z[e] = -CUDART_INF_F;
+                    for (int e = 0; e < 128; ++e) if (n0 + e >= of.N) z[e] = -CUDART_INF_F;
                 }
                 float top[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F}, sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -272,7 +319,7 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
 #pragma unroll
                 for (int e = 0; e < 128; ++e) sum[e & 3] += exp2_fast(fmaf(z[e], p.c, -below));
                 if (mine)
-                    p.part[(size_t)row * (2 * tiles_n) + 2 * tn + (c_half >> 7)] =
+                    p.part[(size_t)row * (2 * of.tiles_n()) + 2 * t.n + (c_half >> 7)] =
                         ok ? make_float2(most, (sum[0] + sum[1]) + (sum[2] + sum[3])) : make_float2(CUDART_NAN_F, CUDART_NAN_F);      // (no result)
             } else if constexpr (KIND == kProbs) {
                 // rows that do not count are zeros, whatever they hold; one with a target that is not there NaN
@@ -313,9 +360,9 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                     store_64(blk, y, p.p, p.ldp, row0, rows, n0 + cb * 64, 64, true, lane);
                 }
                 taken();
-            } else if constexpr (KIND == kRows) {
+            } else if (!t.head) {
                 const int rr = lane >> 3, ch = lane & 7;
-                float* const acc = p.acc + (size_t)(t / (tiles_m * tiles_n)) * p.M * p.ld_acc;
+                float* const acc = p.acc + (size_t)t.share * of.M * p.ld_acc;
                 wait();
 #pragma unroll 1
                 for (int cb = 0; cb < 4; ++cb) {
@@ -350,7 +397,7 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
 #pragma unroll 1
                 for (int cb = 0; cb < 2; ++cb) {
                     const int c0 = n0 + cb * 64;
-                    if (c0 >= p.N || rows <= 0) break;
+                    if (c0 >= of.N || rows <= 0) break;
                     uint32_t v[2][32], y[32];
                     tmem_columns32(from() + cb * 64, v[0]);
                     tmem_columns32(from() + cb * 64 + 32, v[1]);
@@ -360,7 +407,7 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                         const __nv_bfloat162 b = __floats2bfloat162_rn(__uint_as_float(v[e >> 4][2 * e & 31]) * factor, __uint_as_float(v[e >> 4][(2 * e & 31) + 1]) * factor);
                         y[e] = *reinterpret_cast<const uint32_t*>(&b);
                     }
-                    store_64(blk, y, p.out, p.N, row0, rows, c0, p.N - c0, p.wide, lane);
+                    store_64(blk, y, p.out, of.N, row0, rows, c0, of.N - c0, p.wide, lane);
                 }
                 taken();
             }
@@ -406,24 +453,26 @@ __global__ void __launch_bounds__(kFewThreads, 2) loss_few_rows_kernel(const __g
     __shared__ uint32_t tmem_slot;
     __shared__ int targets[NB];
     __shared__ float2 meet[4][NB];
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, M = p.M;
-    const int n_kb = (p.K + kBK - 1) / kBK, n_tiles = (p.N + 127) / 128, mine = (n_tiles - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x, blocks = mine * n_kb;
-    const auto head_tile = [&](int i) {
-        const int slot = i % kSlots, t = blockIdx.x + i / n_kb * gridDim.x;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, M = p.own.M;
+    const int n_kb = (p.own.K + kBK - 1) / kBK, n_tiles = (p.own.N + 127) / 128, mine = (n_tiles - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x, blocks = mine * n_kb;
+    const auto head_tile = [&](int slot, int t, int kb) {
         mbar_arrive_expect_tx(&full[slot], kSlot);
-        tma_load_2d(smem_u32(smem + slot * kSlot), &map_w, smem_u32(&full[slot]), i % n_kb * kBK, t * 128);
+        tma_load_2d(smem_u32(smem + slot * kSlot), &map_w, smem_u32(&full[slot]), kb * kBK, t * 128);
     };
-    const auto row_tile = [&](int i) {
-        const int slot = i % kSlots;
+    const auto row_tile = [&](int slot, int kb) {
 #pragma unroll
         for (int tm = 0; tm < TERMS; ++tm)
-            tma_load_2d(smem_u32(smem + slot * kSlot + kTileBytes + tm * NB * 128), &map_h, smem_u32(&full[slot]), i % n_kb * kBK, tm * M);
+            tma_load_2d(smem_u32(smem + slot * kSlot + kTileBytes + tm * NB * 128), &map_h, smem_u32(&full[slot]), kb * kBK, tm * M);
+    };
+    int t = blockIdx.x, kb = 0;                               // of the next block that is asked for
+    const auto next = [&]() {
+        if (++kb == n_kb) kb = 0, t += gridDim.x;
     };
     if (tid == 0) {
         for (int i = 0; i < kSlots; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
         for (int i = 0; i < 2; ++i) { mbar_init(&t_full[i], 1); mbar_init(&t_empty[i], 4); }
         fence_mbar_init();
-        for (int i = 0; i < min(blocks, kSlots); ++i) head_tile(i);
+        for (int i = 0; i < min(blocks, kSlots); ++i) { head_tile(i, t, kb); next(); }
     }
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (blockIdx.x == 0 && tid == 0) *p.arrived = 0u;
@@ -433,7 +482,7 @@ __global__ void __launch_bounds__(kFewThreads, 2) loss_few_rows_kernel(const __g
     }
     if (tid < NB) {
         const long long t = tid < M ? target_of(p.targets, p.targets64, tid) : -1;
-        targets[tid] = t >= 0 && t < p.N ? (int)t : -1;
+        targets[tid] = t >= 0 && t < p.own.N ? (int)t : -1;
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
@@ -444,11 +493,14 @@ __global__ void __launch_bounds__(kFewThreads, 2) loss_few_rows_kernel(const __g
     if (warp == 0) {
         if (lane == 0) {
             int i = 0;
-            for (; i < min(blocks, kSlots); ++i) row_tile(i);
+            t = blockIdx.x; kb = 0;
+            for (; i < min(blocks, kSlots); ++i) { row_tile(i, kb); next(); }
             for (; i < blocks; ++i) {
-                if (!lane_wait(&empty[i % kSlots], ((i / kSlots) & 1u) ^ 1u, p.polls)) { ok = false; break; }
-                head_tile(i);
-                row_tile(i);
+                const int slot = i % kSlots;
+                if (!lane_wait(&empty[slot], ((i / kSlots) & 1u) ^ 1u, p.polls)) { ok = false; break; }
+                head_tile(slot, t, kb);
+                row_tile(slot, kb);
+                next();
             }
             // (copies in flight arrive before the CTA goes)
             for (int j = max(0, i - kSlots); j < i && !ok; ++j) (void)lane_wait(&full[j % kSlots], (j / kSlots) & 1u, p.polls);
@@ -456,8 +508,9 @@ __global__ void __launch_bounds__(kFewThreads, 2) loss_few_rows_kernel(const __g
     } else if (warp == 1) {
         const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(kCols >> 3) << 17) | (8u << 24);
         unsigned it = 0;
-        for (int i = 0; i < blocks && ok; ++i) {
-            const int kb = i % n_kb, slot = i % kSlots;
+        kb = 0;
+        for (int i = 0; i < blocks && ok; ++i, kb = kb + 1 == n_kb ? 0 : kb + 1) {
+            const int slot = i % kSlots;
             const bool first = kb % kFewChunk == 0, last = kb == n_kb - 1 || kb % kFewChunk == kFewChunk - 1;
             if (first) ok = pair_wait(&t_empty[it & 1u], ((it >> 1) & 1u) ^ 1u, p.polls);
             ok = ok && pair_wait(&full[slot], (i / kSlots) & 1u, p.polls);
@@ -506,8 +559,8 @@ __global__ void __launch_bounds__(kFewThreads, 2) loss_few_rows_kernel(const __g
             for (int m = 0; m < NB; ++m) {
                 if (m >= M) break;
                 if (targets[m] == n) p.hit[m] = ok ? z[m] : CUDART_NAN_F;
-                const float x = n < p.N ? z[m] * p.c : -CUDART_INF_F, now = fmaxf(most[m], x);
-                if (now > -CUDART_INF_F) sum[m] = sum[m] * exp2_fast(most[m] - now) + exp2_fast(n < p.N ? fmaf(z[m], p.c, -now) : -CUDART_INF_F);
+                const float x = n < p.own.N ? z[m] * p.c : -CUDART_INF_F, now = fmaxf(most[m], x);
+                if (now > -CUDART_INF_F) sum[m] = sum[m] * exp2_fast(most[m] - now) + exp2_fast(n < p.own.N ? fmaf(z[m], p.c, -now) : -CUDART_INF_F);
                 else sum[m] += x != x ? x : 0.f;
                 most[m] = now;
             }
@@ -704,16 +757,21 @@ cudaError_t pairs_of(int dev, int* out) {
     return cudaSuccess;
 }
 
+// (hs, ht: the operands of dw in kGrads)
 template <int KIND, int TERMS>
-cudaError_t run_tiles(const CUtensorMap& a, const CUtensorMap& b, LossTiles p, int dev, cudaStream_t st) {
+cudaError_t run_tiles(const CUtensorMap& a, const CUtensorMap& b, LossTiles p, int dev, cudaStream_t st, const CUtensorMap* hs = nullptr, const CUtensorMap* ht = nullptr) {
     int pairs = 0;
     const cudaError_t e = pairs_of<KIND, TERMS>(dev, &pairs);
     if (e != cudaSuccess) return e;
     p.polls = gemm_pair_polls();
     p.ran_out = split_attention_ran_out(dev, st);
-    const long long tiles = (long long)((p.M + 255) / 256) * ((p.N + kTileN - 1) / kTileN) * (KIND == kRows ? p.splits : 1);
-    if (tiles > 0x3fffffffLL) return cudaErrorNotSupported;
-    loss_product_kernel<KIND, TERMS><<<2 * (int)std::min<long long>(tiles, pairs), kThreads, Ring<TERMS>::kSmem, st>>>(a, b, p);
+    const long long own = p.own.tiles(), head = p.head.tiles();
+    if (own + head > 0x3fffffffLL) return cudaErrorNotSupported;
+    const int long_own = p.own.share(), long_head = p.head.blocks();
+    p.first_head = own == 0 || (head > 0 && long_head > long_own);
+    p.many = (int)(p.first_head ? head : own);
+    p.extra = own && head ? std::max(1, (p.first_head ? long_head + long_own / 2 : long_own + long_head / 2) / (p.first_head ? long_own : long_head)) : 0;
+    loss_product_kernel<KIND, TERMS><<<2 * (int)std::min<long long>(own + head, pairs), kThreads, Ring<TERMS>::kSmem, st>>>(a, b, hs ? *hs : a, ht ? *ht : b, p);
     return cudaGetLastError();
 }
 
@@ -795,7 +853,7 @@ Room room_of(const LossShape& s, bool grad, bool rows, bool head, int sms) {
 
 LossTiles tiles_of(const LossShape& s) {
     LossTiles p{};
-    p.splits = 1;
+    p.own.splits = p.head.splits = 1;
     p.targets = s.targets; p.targets64 = s.targets64; p.ignore = s.ignore;
     p.c = s.scale * kLog2e; p.V = s.V;
     return p;
@@ -834,7 +892,7 @@ cudaError_t launch_loss(const LossShape& s, float* loss, float* kept, float* tot
     CUtensorMap ma, mb;
     if (!bf16_map(&ma, h, (long long)s.M * (f32 ? 3 : 1), s.K, ldh, r.few ? columns : 128) || !bf16_map(&mb, w, s.V, s.K, ldw, 128)) return cudaErrorNotSupported;
     LossTiles p = tiles_of(s);
-    p.M = s.M; p.N = s.V; p.K = s.K;
+    p.own.M = s.M; p.own.N = s.V; p.own.K = s.K;
     p.part = reinterpret_cast<float2*>(base + r.part);
     p.hit = reinterpret_cast<float*>(base + r.hit);
     p.arrived = reinterpret_cast<unsigned*>(base + r.arrived);
@@ -890,31 +948,27 @@ cudaError_t launch_loss_grad(const LossShape& s, const float* kept, const LossGr
         const int cols = std::min(r.piece, s.V - v0);
         LossTiles p = tiles_of(s);
         p.v0 = v0;
-        p.M = s.M; p.N = cols; p.K = s.K;
+        p.own.M = s.M; p.own.N = cols; p.own.K = s.K;
         p.kept = reinterpret_cast<const float2*>(kept);
         p.p = probs; p.ldp = r.piece;
         e = run_tiles<kProbs, 1>(h_rows, w_rows, p, dev, st);
         if (e != cudaSuccess) return e;
         ++extra_launches();
+        LossTiles q = tiles_of(s);
+        q.v0 = v0;
         if (dh) {
-            LossTiles q = tiles_of(s);
-            q.v0 = v0;
-            q.M = s.M; q.N = s.K; q.K = cols;
-            q.splits = shares_of(cols, r.splits); q.acc = acc; q.ld_acc = ld_acc; q.add = v0 > 0;
-            e = run_tiles<kRows, 1>(p_rows, w_cols, q, dev, st);
-            if (e != cudaSuccess) return e;
-            ++extra_launches();
+            q.own.M = s.M; q.own.N = s.K; q.own.K = cols; q.own.splits = shares_of(cols, r.splits);
+            q.acc = acc; q.ld_acc = ld_acc; q.add = v0 > 0;
         }
         if (dw) {
-            LossTiles q = tiles_of(s);
-            q.M = cols; q.N = s.K; q.K = s.M;
+            q.head.M = cols; q.head.N = s.K; q.head.K = s.M;
             q.out = reinterpret_cast<__nv_bfloat16*>(dw) + (size_t)v0 * s.K;
             if (!by.grad_stride) q.grad = by.grad, q.count = by.count, q.scale = s.scale;      // (else the rows have theirs)
             q.wide = s.K % 8 == 0 && (reinterpret_cast<uintptr_t>(dw) & 15) == 0;
-            e = run_tiles<kHead, 1>(p_cols, h_cols, q, dev, st);
-            if (e != cudaSuccess) return e;
-            ++extra_launches();
         }
+        e = run_tiles<kGrads, 1>(p_rows, w_cols, q, dev, st, &p_cols, dw ? &h_cols : nullptr);
+        if (e != cudaSuccess) return e;
+        ++extra_launches();
     }
     if (dh) {
         const long long blocks = ((long long)s.M * (ld_acc / 4) + 255) / 256;

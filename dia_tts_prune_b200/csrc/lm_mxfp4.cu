@@ -22,40 +22,54 @@ using namespace dia;
 
 // ---- rounding and values -------------------------------------------------------------------------------------------------------------------
 
-// eight neighbouring channels of a row; those at or beyond `n` are zero.  wide: 16-byte loads
-template <int TYPE>
-__device__ __forceinline__ void load8(const void* row, int k, int n, bool wide, float (&v)[8]) {
-    if (wide && n >= 8) {
-        if (TYPE == kTypeF32) {
-            const float4 a = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(row) + k)[0];
-            const float4 b = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(row) + k)[1];
-            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+// Eight neighbouring channels of a row as they lie in memory.  WIDE: rows of whole 16 bytes whose channels are a multiple of eight, all eight are there or none; else those
+// at or beyond `n` are zero.  (Fetching and widening are apart: widened at once, a load is waited for before the next one goes out.)
+template <int TYPE, bool WIDE>
+struct Eight {
+    uint4 w[TYPE == kTypeF32 ? 2 : 1];
+    __device__ __forceinline__ void fetch(const void* row, int k, int n) {
+        constexpr int kWords = TYPE == kTypeF32 ? 2 : 1;
+        if constexpr (WIDE) {
+#pragma unroll
+            for (int i = 0; i < kWords; ++i)
+                w[i] = n > 0 ? __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(row) + (size_t)k * (TYPE == kTypeF32 ? 4 : 2)) + i) : make_uint4(0u, 0u, 0u, 0u);
         } else {
-            const uint4 u = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(row) + k);
-            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+            uint32_t u[4 * kWords];
+#pragma unroll
+            for (int e = 0; e < 4 * kWords; ++e) {
+                if (TYPE == kTypeF32) {
+                    u[e] = e < n ? reinterpret_cast<const uint32_t*>(row)[k + e] : 0u;
+                } else {
+                    const uint32_t lo = 2 * e < n ? reinterpret_cast<const uint16_t*>(row)[k + 2 * e] : 0u, hi = 2 * e + 1 < n ? reinterpret_cast<const uint16_t*>(row)[k + 2 * e + 1] : 0u;
+                    u[e] = lo | hi << 16;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) w[i] = make_uint4(u[4 * i], u[4 * i + 1], u[4 * i + 2], u[4 * i + 3]);
+        }
+    }
+    __device__ __forceinline__ void widen(float (&v)[8]) const {
+        const uint32_t u[4] = {w[0].x, w[0].y, w[0].z, w[0].w};
+        if constexpr (TYPE == kTypeF32) {
+            const uint4 h = w[TYPE == kTypeF32];
+            v[0] = __uint_as_float(u[0]); v[1] = __uint_as_float(u[1]); v[2] = __uint_as_float(u[2]); v[3] = __uint_as_float(u[3]);
+            v[4] = __uint_as_float(h.x); v[5] = __uint_as_float(h.y); v[6] = __uint_as_float(h.z); v[7] = __uint_as_float(h.w);
+        } else {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 if (TYPE == kTypeBf16) {
-                    v[2 * e] = __uint_as_float(w[e] << 16);
-                    v[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+                    v[2 * e] = __uint_as_float(u[e] << 16);
+                    v[2 * e + 1] = __uint_as_float(u[e] & 0xffff0000u);
                 } else {
-                    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
+                    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[e]));
                     v[2 * e] = f.x;
                     v[2 * e + 1] = f.y;
                 }
             }
         }
-        return;
     }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        v[e] = 0.f;
-        if (e < n)
-            v[e] = TYPE == kTypeF32    ? reinterpret_cast<const float*>(row)[k + e]
-                   : TYPE == kTypeBf16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(row)[k + e])
-                                       : __half2float(reinterpret_cast<const __half*>(row)[k + e]);
-    }
-}
+};
+inline int wide_rows(const void* x, int type, long long ld, int K) { return (reinterpret_cast<uintptr_t>(x) & 15) == 0 && ld * type_bytes(type) % 16 == 0 && K % 8 == 0; }
 
 // The codes of eight channels and their block's scale, where the four lanes of a group of four hold the block's 32 channels.
 __device__ __forceinline__ uint32_t round_block(const float (&v)[8], uint32_t& scale) {
@@ -80,36 +94,43 @@ __device__ __forceinline__ uint32_t round_block(const float (&v)[8], uint32_t& s
     return codes;
 }
 
-// place of a scale in the pieces of 128 rows x 128 channels (block: 32 channels)
-__device__ __forceinline__ size_t scale_at(long long row, int block, int pieces) {
-    return ((size_t)(row >> 7) * pieces + (block >> 2)) * kMxScaleBytes + (row & 31) * 16 + ((row >> 5) & 3) * 4 + (block & 3);
-}
-
-// A thread takes eight channels, four neighbours a block.  Rows behind the last one of a piece get scales of zero.
-constexpr int kQuantThreads = 256, kQuantItems = 4;
-template <int TYPE>
-__global__ void __launch_bounds__(kQuantThreads) mxfp4_quantize_kernel(const void* __restrict__ x, long long ld, int rows, int K, int wide, uint32_t* __restrict__ codes,
-                                                                       uint8_t* __restrict__ scales) {
-    const int per_row = (int)((K + 127) / 128 * 16), pieces = per_row / 16;
-    const long long n = (long long)((rows + 127) / 128 * 128) * per_row;
-    const long long i0 = (long long)blockIdx.x * (kQuantThreads * kQuantItems) + threadIdx.x;
-    float v[kQuantItems][8];
+// A CTA takes 128 rows x 256 channels, a warp 16 rows of them, a lane eight channels (four neighbours a block): kAhead rows are on their way at a time, and the scales
+// leave as the two pieces that they are.  early: the successor, a product of these rows, may start now (never where the rows are a matrix to keep: products ask for
+// theirs before their predecessor has ended).  Rows behind the last one of a piece get scales of zero.  Bound: memory (32768 x 2048 bf16, 170 MB: 75 us with an index per eight
+// channels, whose scales went out byte by byte).
+constexpr int kQuantThreads = 256, kAhead = 8;
+template <int TYPE, bool WIDE>
+__global__ void __launch_bounds__(kQuantThreads) mxfp4_quantize_kernel(const void* __restrict__ x, long long ld, int rows, int K, uint32_t* __restrict__ codes,
+                                                                       uint8_t* __restrict__ scales, int early) {
+    if (early) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    __shared__ __align__(16) uint8_t staged[2 * kMxScaleBytes];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, pieces = (K + 127) / 128, c0 = blockIdx.x * 32 + lane, k = 8 * c0;
+    const long long row0 = (long long)blockIdx.y * 128 + warp * 16;
+    const bool kept = c0 < pieces * 16;                       // (a row's codes go on to the end of its last piece)
 #pragma unroll
-    for (int j = 0; j < kQuantItems; ++j) {
-        const long long i = i0 + j * kQuantThreads, r = i / per_row;
-        const int k = (int)(i - r * per_row) * 8;
-        load8<TYPE>(reinterpret_cast<const char*>(x) + r * ld * (TYPE == kTypeF32 ? 4 : 2), k, r < rows ? K - k : 0, wide, v[j]);
-    }
+    for (int r0 = 0; r0 < 16; r0 += kAhead) {
+        Eight<TYPE, WIDE> x8[kAhead];
 #pragma unroll
-    for (int j = 0; j < kQuantItems; ++j) {
-        const long long i = i0 + j * kQuantThreads, r = i / per_row;
-        const int c = (int)(i - r * per_row);
-        uint32_t scale;
-        const uint32_t code = round_block(v[j], scale);       // (n is a multiple of 32: a warp is in or out as a whole)
-        if (i >= n) continue;
-        if (r < rows) codes[i] = code;
-        if ((c & 3) == 0) scales[scale_at(r, c >> 2, pieces)] = (uint8_t)scale;
+        for (int j = 0; j < kAhead; ++j) {
+            const long long r = row0 + r0 + j;
+            x8[j].fetch(reinterpret_cast<const char*>(x) + r * ld * (TYPE == kTypeF32 ? 4 : 2), k, r < rows ? K - k : 0);
+        }
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            const int in = warp * 16 + r0 + j;
+            const long long r = row0 + r0 + j;
+            float v[8];
+            x8[j].widen(v);
+            uint32_t scale;
+            const uint32_t code = round_block(v, scale);
+            if (kept && r < rows) codes[r * (pieces * 16) + c0] = code;
+            if ((lane & 3) == 0) staged[(lane >> 4) * kMxScaleBytes + (in & 31) * 16 + (in >> 5) * 4 + ((lane >> 2) & 3)] = (uint8_t)scale;
+        }
     }
+    __syncthreads();
+    const int piece = 2 * blockIdx.x + (threadIdx.x >> 5);
+    if (threadIdx.x < 64 && piece < pieces)
+        reinterpret_cast<uint4*>(scales + ((size_t)blockIdx.y * pieces + piece) * kMxScaleBytes)[lane] = reinterpret_cast<const uint4*>(staged)[threadIdx.x];
 }
 
 // four neighbouring numbers of a row, those at or beyond `n` left out.  wide: one store of them all
@@ -145,25 +166,38 @@ __device__ __forceinline__ float2 two_values(uint32_t byte) {
 }
 __device__ __forceinline__ float scale_value(uint32_t scale) { return __uint_as_float(scale == 255u ? 0x7fffffffu : scale ? scale << 23 : 0x00400000u); }
 
+// The same shares; a lane takes four neighbouring channels of either half, so that whole lines of float32 are stored.
 template <int TYPE>
-__global__ void __launch_bounds__(256) mxfp4_dequantize_kernel(const uint32_t* __restrict__ codes, const uint8_t* __restrict__ scales, int rows, int K, void* __restrict__ out,
-                                                               int wide) {
-    const int per_row = (K + 7) / 8, stride = (int)((K + 127) / 128 * 16);
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x, r = i / per_row;
-    if (r >= rows) return;
-    const int c = (int)(i - r * per_row), k = 8 * c;
-    const uint32_t code = codes[r * stride + c];
-    const float f = scale_value(scales[scale_at(r, c >> 2, stride / 16)]);
-    float v[8];
+__global__ void __launch_bounds__(kQuantThreads) mxfp4_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int rows, int K,
+                                                                         void* __restrict__ out, int wide) {
+    __shared__ __align__(16) uint8_t staged[2 * kMxScaleBytes];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, pieces = (K + 127) / 128;
+    const long long row0 = (long long)blockIdx.y * 128 + warp * 16;
+    if (threadIdx.x < 64 && 2 * (int)blockIdx.x + warp < pieces)
+        reinterpret_cast<uint4*>(staged)[threadIdx.x] = reinterpret_cast<const uint4*>(scales + ((size_t)blockIdx.y * pieces + 2 * blockIdx.x + warp) * kMxScaleBytes)[lane];
+    __syncthreads();
+    const int n = (int)min(16LL, rows - row0);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        const float2 t = two_values((code >> (8 * e)) & 255u);
-        v[2 * e] = t.x * f;
-        v[2 * e + 1] = t.y * f;
+    for (int r0 = 0; r0 < 16; r0 += 4) {
+        uint32_t code[4][2];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int piece = 2 * blockIdx.x + h;
+                code[j][h] = r0 + j < n && piece < pieces ? reinterpret_cast<const uint16_t*>(codes + (row0 + r0 + j) * (pieces * 64) + piece * 64)[lane] : 0u;
+            }
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int in = warp * 16 + r0 + j, k = (2 * blockIdx.x + h) * 128 + 4 * lane;
+                if (r0 + j >= n || k >= K) continue;
+                const float f = scale_value(staged[h * kMxScaleBytes + (in & 31) * 16 + (in >> 5) * 4 + (lane >> 3)]);
+                const float2 a = two_values(code[j][h] & 255u), b = two_values(code[j][h] >> 8);
+                put4<TYPE>(out, (size_t)(row0 + r0 + j) * K + k, make_float4(a.x * f, a.y * f, b.x * f, b.y * f), K - k, wide);
+            }
     }
-    const size_t at = (size_t)r * K + k;
-    put4<TYPE>(out, at, make_float4(v[0], v[1], v[2], v[3]), K - k, wide);
-    put4<TYPE>(out, at + 4, make_float4(v[4], v[5], v[6], v[7]), K - k - 4, wide);
 }
 
 // ---- the product -----------------------------------------------------------------------------------------------------------------------------
@@ -240,20 +274,37 @@ mxfp4_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
     bool ok = true;
     if (warp == 0) {
         if (lane == 0) {
+            // a stage's weights, which do not wait for the kernel that rounds the rows, and its rows (t, s: its tile and place there)
+            const auto weights = [&](unsigned at, int t, int s) {
+                unsigned char* const dst = smem + at * kStageBytes;
+                const uint32_t sc = kMxScaleBytes * min(2, pieces - 2 * s);
+                const int tn = t / tiles_m;
+                mbar_arrive_expect_tx(&full[at], 2 * kCodeTile + 2 * sc);
+                tma_load_2d(smem_u32(dst + kCodeTile), &map_w, smem_u32(&full[at]), s * (kStageK / 2), tn * kBN);
+                bulk_g2s(dst + 2 * kCodeTile + 1024, p.w_scales + ((size_t)tn * pieces + 2 * s) * kMxScaleBytes, sc, &full[at]);
+            };
+            const auto rows = [&](unsigned at, int t, int s) {
+                unsigned char* const dst = smem + at * kStageBytes;
+                const int tm = t % tiles_m;
+                tma_load_2d(smem_u32(dst), &map_a, smem_u32(&full[at]), s * (kStageK / 2), tm * kBM);
+                bulk_g2s(dst + 2 * kCodeTile, p.a_scales + ((size_t)tm * pieces + 2 * s) * kMxScaleBytes, kMxScaleBytes * min(2, pieces - 2 * s), &full[at]);
+            };
             unsigned i = 0;
-            for (int t = blockIdx.x; t < n_tiles && ok; t += gridDim.x) {
-                const int tn = t / tiles_m, tm = t % tiles_m;
-                for (int s = 0; s < n_stage; ++s, ++i) {
-                    const unsigned at = i % kStages;
-                    if (!lane_wait(&empty[at], ((i / kStages) & 1u) ^ 1u, p.polls)) { ok = false; break; }
-                    unsigned char* const dst = smem + at * kStageBytes;
-                    const uint32_t sc = kMxScaleBytes * min(2, pieces - 2 * s);
-                    mbar_arrive_expect_tx(&full[at], 2 * kCodeTile + 2 * sc);
-                    tma_load_2d(smem_u32(dst), &map_a, smem_u32(&full[at]), s * (kStageK / 2), tm * kBM);
-                    tma_load_2d(smem_u32(dst + kCodeTile), &map_w, smem_u32(&full[at]), s * (kStageK / 2), tn * kBN);
-                    bulk_g2s(dst + 2 * kCodeTile, p.a_scales + ((size_t)tm * pieces + 2 * s) * kMxScaleBytes, sc, &full[at]);
-                    bulk_g2s(dst + 2 * kCodeTile + 1024, p.w_scales + ((size_t)tn * pieces + 2 * s) * kMxScaleBytes, sc, &full[at]);
-                }
+            int t = blockIdx.x, s = 0;
+            const auto next = [&]() {
+                ++i;
+                if (++s == n_stage) s = 0, t += gridDim.x;
+            };
+            while (i < kStages && t < n_tiles) { weights(i, t, s); next(); }
+            const unsigned ahead = i;
+            asm volatile("griddepcontrol.wait;" ::: "memory");
+            i = 0; t = blockIdx.x; s = 0;
+            while (i < ahead) { rows(i, t, s); next(); }
+            for (; t < n_tiles; next()) {
+                const unsigned at = i % kStages;
+                if (!lane_wait(&empty[at], ((i / kStages) & 1u) ^ 1u, p.polls)) { ok = false; break; }
+                weights(at, t, s);
+                rows(at, t, s);
             }
             // (copies in flight arrive before the CTA goes)
             for (unsigned j = i > (unsigned)kStages ? i - kStages : 0; j < i && !ok; ++j) (void)lane_wait(&full[j % kStages], (j / kStages) & 1u, p.polls);
@@ -337,17 +388,19 @@ mxfp4_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
     }
 }
 
-// Few rows (decoding, a short portion): the weights are the 128-row operand and stream once, the rows are the columns.  A cluster of S CTAs owns 128 weight rows, each
+// Few rows (decoding): the weights are the 128-row operand and stream once, the rows are the columns.  A cluster of S CTAs owns 128 weight rows, each
 // CTA a range of stages.
 //   warp 0    requests the CTA's weight codes and scales ahead of the rows - before the kernel's predecessor has ended (nothing that lets its successor start early
 //             writes weights)
-//   all warps round the CTA's share of the rows to MXFP4, straight into the layout of the MMA (the rows are read S times less than once per CTA)
+//   all warps round the CTA's share of the rows to MXFP4, straight into the layout of the MMA
 //   warp 1    per stage the scales into tensor memory and its MMAs (M = 128, N = NB)
 //   warps 2-5 take the accumulator out (weight row = lane); with S > 1 the shares meet in shared memory, in the order of the ranges
-// Bound: the weights' bytes where there are many, latency else.  Tensor memory is taken behind the wait for the predecessor and in front of the signal to the successor:
+// Bound: the weights' bytes where there are many, latency else.  Up to 16 rows: every CTA rounds the rows by itself, which beyond takes longer than a kernel that rounds
+// them once (us, here / rounded once and 128 x 128 tiles: 2048 x 2048 8 rows 5.6 / 9.1, 16 rows 6.1 / 9.7, 32 rows 8.0 / 10.2; 32768 x 2048 13.0 / 15.2, 14.5 / 15.3, 22.7 / 15.5;
+// 8192 x 4096 12.1 / 12.3, 13.9 / 12.8, 21.4 / 13.4).  Tensor memory is taken behind the wait for the predecessor and in front of the signal to the successor:
 // a CTA that waits for another kernel holds none of it, so neither can wait for the other.  Shared memory is asked for such that an SM holds three CTAs at most, whose
 // tensor memory fits at the same time: CTAs of a cluster wait for one another.
-constexpr int kFewMost = 64, kFewCols = 128, kFewSmemMost = 226 * 1024, kFewSmemLeast = 58 * 1024, kFewSlotsMost = 12;
+constexpr int kFewMost = 16, NB = 16, kFewCols = 128, kFewSmemMost = 226 * 1024, kFewSmemLeast = 58 * 1024, kFewSlotsMost = 12;
 static_assert(4 * kFewSmemLeast > 228 * 1024 && 4 * kFewCols <= 512, "CTAs on an SM");
 
 struct FewProduct {
@@ -365,7 +418,6 @@ __device__ __forceinline__ void put1(void* y, int type, size_t at, float v) {
     else reinterpret_cast<__half*>(y)[at] = __float2half_rn(v);
 }
 
-template <int NB>
 __global__ void __launch_bounds__(kThreads4, 1) mxfp4_few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ FewProduct p) {
     constexpr int kSlot = kCodeTile + 1024, kRows = NB * 128 + 1024;       // a stage of weights, of rows
     extern __shared__ unsigned char smem_raw[];
@@ -398,28 +450,35 @@ __global__ void __launch_bounds__(kThreads4, 1) mxfp4_few_rows_kernel(const __gr
     // ---- the rows: eight channels an item, four neighbours a block; kBatch loads in flight (one after the other, 8 rows x 2048 took 11 of 18 us) ----
     const int per_row = stages * 32, items = M * per_row;
     const auto place = [&](int m, int c) { return rows + (c >> 5) * kRows + (m >> 3) * 1024 + (m & 7) * 128 + ((((c & 31) >> 2) ^ (m & 7)) << 4) + (c & 3) * 4; };
-    const auto take = [&](auto type) {
+    const auto take = [&](auto type, auto wide) {
         constexpr int TYPE = decltype(type)::value, kBatch = TYPE == kTypeF32 ? 4 : 8;
+        constexpr bool WIDE = decltype(wide)::value;
         for (int i0 = tid; i0 < items; i0 += kThreads4 * kBatch) {           // (a warp is in or out as a whole)
-            float v[kBatch][8];
+            Eight<TYPE, WIDE> x8[kBatch];
 #pragma unroll
             for (int b = 0; b < kBatch; ++b) {
                 const int i = i0 + b * kThreads4, m = i / per_row, k = s0 * kStageK + 8 * (i - m * per_row);
-                load8<TYPE>(reinterpret_cast<const char*>(p.a) + (long long)m * p.lda * (TYPE == kTypeF32 ? 4 : 2), k, i < items ? p.K - k : 0, p.wide, v[b]);
+                x8[b].fetch(reinterpret_cast<const char*>(p.a) + (long long)m * p.lda * (TYPE == kTypeF32 ? 4 : 2), k, i < items ? p.K - k : 0);
             }
 #pragma unroll
             for (int b = 0; b < kBatch; ++b) {
                 const int i = i0 + b * kThreads4, m = i / per_row, c = i - m * per_row;
                 if (i >= items) break;
+                float v[8];
+                x8[b].widen(v);
                 uint32_t scale;
-                *reinterpret_cast<uint32_t*>(place(m, c)) = round_block(v[b], scale);
+                *reinterpret_cast<uint32_t*>(place(m, c)) = round_block(v, scale);
                 if ((c & 3) == 0) rows[(c >> 5) * kRows + NB * 128 + ((c & 31) >> 4) * kMxScaleBytes + (m & 31) * 16 + (m >> 5) * 4 + ((c >> 2) & 3)] = (uint8_t)scale;
             }
         }
     };
-    if (p.a_type == kTypeF32) take(std::integral_constant<int, kTypeF32>());
-    else if (p.a_type == kTypeBf16) take(std::integral_constant<int, kTypeBf16>());
-    else take(std::integral_constant<int, kTypeF16>());
+    const auto take_type = [&](auto type) {
+        if (p.wide) take(type, std::true_type());
+        else take(type, std::false_type());
+    };
+    if (p.a_type == kTypeF32) take_type(std::integral_constant<int, kTypeF32>());
+    else if (p.a_type == kTypeBf16) take_type(std::integral_constant<int, kTypeBf16>());
+    else take_type(std::integral_constant<int, kTypeF16>());
     for (int i = tid; i < (NB - M) * per_row; i += kThreads4) {               // columns that no row uses
         const int m = M + i / per_row, c = i % per_row;
         *reinterpret_cast<uint32_t*>(place(m, c)) = 0u;
@@ -471,18 +530,14 @@ __global__ void __launch_bounds__(kThreads4, 1) mxfp4_few_rows_kernel(const __gr
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const int c = (warp & 3) * 32 + lane;
         const int n = n0 + c;
+        uint32_t v[NB];
+        tmem_columns16(tmem + ((uint32_t)((warp & 3) * 32) << 16), v);
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-        for (int m0 = 0; m0 < NB; m0 += 16) {
-            if (m0 >= M) break;
-            uint32_t v[16];
-            tmem_columns16(tmem + ((uint32_t)((warp & 3) * 32) << 16) + m0, v);
-            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const float f = !ok ? CUDART_NAN_F : stages ? __uint_as_float(v[e]) : 0.f;          // (NaN: no result)
-                if (S > 1) part[(m0 + e) * 128 + c] = f;
-                else if (m0 + e < M && n < p.N) put1(p.y, p.y_type, (size_t)(m0 + e) * p.N + n, f);
-            }
+        for (int m = 0; m < NB; ++m) {
+            const float f = !ok ? CUDART_NAN_F : stages ? __uint_as_float(v[m]) : 0.f;              // (NaN: no result)
+            if (S > 1) part[m * 128 + c] = f;
+            else if (m < M && n < p.N) put1(p.y, p.y_type, (size_t)m * p.N + n, f);
         }
     }
     if (!ok && lane == 0 && p.ran_out) {
@@ -534,15 +589,23 @@ cudaError_t run_tiled(const Mxfp4Product& p, const uint8_t* a_codes, const uint8
     if (!codes_map(&ma, a_codes, p.M, p.K, kBM) || !codes_map(&mw, p.w_codes, p.N, p.K, kBN)) return cudaErrorNotSupported;
     const TiledProduct q{a_scales, reinterpret_cast<const uint8_t*>(p.w_scales), p.y, p.M, p.N, p.K, p.ran_out, p.polls};
     const long long n_tiles = (long long)((p.M + kBM - 1) / kBM) * ((p.N + kBN - 1) / kBN);
-    mxfp4_product_kernel<TYPE><<<(int)std::min<long long>(n_tiles, sms), kThreads4, kSmem4, st>>>(ma, mw, q);
-    return cudaGetLastError();
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)std::min<long long>(n_tiles, sms));
+    cfg.blockDim = dim3(kThreads4);
+    cfg.dynamicSmemBytes = kSmem4;
+    cfg.stream = st;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, mxfp4_product_kernel<TYPE>, ma, mw, q);
 }
 
 // CTAs of a cluster, and what they hold: as many CTAs as the chip has SMs, two stages each while there are that many (one beyond that would cost more in joining
 // shares than it saves)
-bool few_plan(int M, int N, int K, int& NB, int& S, int& per, int& slots, size_t& smem) {
+bool few_plan(int M, int N, int K, int& S, int& per, int& slots, size_t& smem) {
     if (M > kFewMost) return false;
-    NB = M <= 16 ? 16 : M <= 32 ? 32 : 64;
     const long long tiles = (N + 127) / 128, n_stage = (mx_stride(K) / 128 + 1) / 2;
     const size_t slot = kCodeTile + 1024, row = NB * 128 + 1024;
     for (S = 1; S < 8 && n_stage >= 2 * S && tiles * S < 120; S *= 2) {}
@@ -561,13 +624,12 @@ bool few_plan(int M, int N, int K, int& NB, int& S, int& per, int& slots, size_t
     }
 }
 
-template <int NB>
 cudaError_t run_few(const Mxfp4Product& p, int S, int per, int slots, size_t smem, int dev, cudaStream_t st) {
-    const cudaError_t e = ask_smem<mxfp4_few_rows_kernel<NB>>(dev, kFewSmemMost);
+    const cudaError_t e = ask_smem<mxfp4_few_rows_kernel>(dev, kFewSmemMost);
     if (e != cudaSuccess) return e;
     CUtensorMap mw;
     if (!codes_map(&mw, p.w_codes, p.N, p.K, 128)) return cudaErrorNotSupported;
-    const int wide = (reinterpret_cast<uintptr_t>(p.a) & 15) == 0 && p.lda * type_bytes(p.a_type) % 16 == 0;
+    const int wide = wide_rows(p.a, p.a_type, p.lda, p.K);
     const FewProduct q{p.a, p.lda, p.a_type, wide, reinterpret_cast<const uint8_t*>(p.w_scales), p.y, p.y_type, p.M, p.N, p.K, per, slots, p.ran_out, p.polls};
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((p.N + 127) / 128, S);
@@ -583,33 +645,53 @@ cudaError_t run_few(const Mxfp4Product& p, int S, int per, int slots, size_t sme
     attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = S > 1 ? 2 : 1;
-    return cudaLaunchKernelEx(&cfg, mxfp4_few_rows_kernel<NB>, mw, q);
+    return cudaLaunchKernelEx(&cfg, mxfp4_few_rows_kernel, mw, q);
+}
+
+// more rows than a grid has room for: 65535 x 128 at a time
+template <typename F>
+cudaError_t launch_in_parts(int rows, const F& launch) {
+    constexpr long long most = 65535LL * 128;
+    for (long long r0 = 0; r0 < rows; r0 += most) {
+        const cudaError_t e = launch(r0, (int)std::min(most, rows - r0));
+        if (e != cudaSuccess) return e;
+        if (r0) ++extra_launches();
+    }
+    return cudaSuccess;
 }
 
 }  // namespace
 
-cudaError_t launch_mxfp4_quantize(const void* x, int type, long long ld, int rows, int K, void* codes, void* scales, cudaStream_t st) {
-    const long long n = (long long)((rows + 127) / 128 * 128) * (mx_stride(K) / 8), per = kQuantThreads * kQuantItems, blocks = (n + per - 1) / per;
-    if (blocks > 0x7fffffffLL) return cudaErrorNotSupported;
-    const int wide = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && ld * type_bytes(type) % 16 == 0;
-    const auto kernel = type == kTypeF32 ? mxfp4_quantize_kernel<kTypeF32> : type == kTypeBf16 ? mxfp4_quantize_kernel<kTypeBf16> : mxfp4_quantize_kernel<kTypeF16>;
-    kernel<<<(unsigned)blocks, kQuantThreads, 0, st>>>(x, ld, rows, K, wide, reinterpret_cast<uint32_t*>(codes), reinterpret_cast<uint8_t*>(scales));
+cudaError_t launch_mxfp4_quantize(const void* x, int type, long long ld, int rows, int K, void* codes, void* scales, cudaStream_t st, bool early) {
+    const dim3 grid((K + 255) / 256, (rows + 127) / 128);
+    if (grid.y > 65535u) return launch_in_parts(rows, [&](long long r0, int n) {
+        return launch_mxfp4_quantize(reinterpret_cast<const char*>(x) + r0 * ld * type_bytes(type), type, ld, n, K, reinterpret_cast<uint8_t*>(codes) + mx_code_bytes(r0, K),
+                                     reinterpret_cast<uint8_t*>(scales) + mx_scale_bytes(r0, K), st);
+    });
+    const auto run = [&](auto kernel) { kernel<<<grid, kQuantThreads, 0, st>>>(x, ld, rows, K, reinterpret_cast<uint32_t*>(codes), reinterpret_cast<uint8_t*>(scales), early); };
+    const bool wide = wide_rows(x, type, ld, K);
+    if (type == kTypeF32) wide ? run(mxfp4_quantize_kernel<kTypeF32, true>) : run(mxfp4_quantize_kernel<kTypeF32, false>);
+    else if (type == kTypeBf16) wide ? run(mxfp4_quantize_kernel<kTypeBf16, true>) : run(mxfp4_quantize_kernel<kTypeBf16, false>);
+    else wide ? run(mxfp4_quantize_kernel<kTypeF16, true>) : run(mxfp4_quantize_kernel<kTypeF16, false>);
     return cudaGetLastError();
 }
 
 cudaError_t launch_mxfp4_dequantize(const void* codes, const void* scales, int rows, int K, void* out, int type, cudaStream_t st) {
-    const long long blocks = ((long long)rows * ((K + 7) / 8) + 255) / 256;
-    if (blocks > 0x7fffffffLL) return cudaErrorNotSupported;
-    const int wide = K % 8 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+    const dim3 grid((K + 255) / 256, (rows + 127) / 128);
+    if (grid.y > 65535u) return launch_in_parts(rows, [&](long long r0, int n) {
+        return launch_mxfp4_dequantize(reinterpret_cast<const uint8_t*>(codes) + mx_code_bytes(r0, K), reinterpret_cast<const uint8_t*>(scales) + mx_scale_bytes(r0, K), n, K,
+                                       reinterpret_cast<char*>(out) + (size_t)r0 * K * type_bytes(type), type, st);
+    });
+    const int wide = K % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
     const auto kernel = type == kTypeF32 ? mxfp4_dequantize_kernel<kTypeF32> : type == kTypeBf16 ? mxfp4_dequantize_kernel<kTypeBf16> : mxfp4_dequantize_kernel<kTypeF16>;
-    kernel<<<(unsigned)blocks, 256, 0, st>>>(reinterpret_cast<const uint32_t*>(codes), reinterpret_cast<const uint8_t*>(scales), rows, K, out, wide);
+    kernel<<<grid, kQuantThreads, 0, st>>>(reinterpret_cast<const uint8_t*>(codes), reinterpret_cast<const uint8_t*>(scales), rows, K, out, wide);
     return cudaGetLastError();
 }
 
 size_t mxfp4_linear_work_bytes(int M, int N, int K) {
-    int NB, S, per, slots;
+    int S, per, slots;
     size_t smem;
-    if (few_plan(M, N, K, NB, S, per, slots, smem)) return 0;
+    if (few_plan(M, N, K, S, per, slots, smem)) return 0;
     return (mx_code_bytes(M, K) + 127) / 128 * 128 + mx_scale_bytes(M, K);
 }
 
@@ -620,13 +702,12 @@ cudaError_t launch_mxfp4_linear(Mxfp4Product p, void* work, cudaStream_t st) {
     p.ran_out = split_attention_ran_out(dev, st);
     p.polls = gemm_pair_polls();
     if (take_ran_out(dev, st)) return cudaErrorLaunchTimeout;
-    int NB, S, per, slots;
+    int S, per, slots;
     size_t smem;
-    if (few_plan(p.M, p.N, p.K, NB, S, per, slots, smem))
-        return NB == 16 ? run_few<16>(p, S, per, slots, smem, dev, st) : NB == 32 ? run_few<32>(p, S, per, slots, smem, dev, st) : run_few<64>(p, S, per, slots, smem, dev, st);
+    if (few_plan(p.M, p.N, p.K, S, per, slots, smem)) return run_few(p, S, per, slots, smem, dev, st);
     uint8_t* const codes = reinterpret_cast<uint8_t*>(work);
     uint8_t* const scales = codes + (mx_code_bytes(p.M, p.K) + 127) / 128 * 128;
-    e = launch_mxfp4_quantize(p.a, p.a_type, p.lda, p.M, p.K, codes, scales, st);
+    e = launch_mxfp4_quantize(p.a, p.a_type, p.lda, p.M, p.K, codes, scales, st, true);
     if (e != cudaSuccess) return e;
     ++extra_launches();
     return p.y_type == kTypeF32    ? run_tiled<kTypeF32>(p, codes, scales, dev, sms, st)

@@ -19,8 +19,8 @@ inline long long mx_stride(long long K) { return (K + kMxStride - 1) / kMxStride
 inline size_t mx_code_bytes(long long rows, long long K) { return (size_t)rows * (mx_stride(K) / 2); }
 inline size_t mx_scale_bytes(long long rows, long long K) { return (size_t)((rows + 127) / 128) * (mx_stride(K) / kMxStride) * kMxScaleBytes; }
 
-// x [rows][K], row stride ld elements
-cudaError_t launch_mxfp4_quantize(const void* x, int type, long long ld, int rows, int K, void* codes, void* scales, cudaStream_t st);
+// x [rows][K], row stride ld elements.  early: a kernel launched behind it with programmatic serialization may start at once
+cudaError_t launch_mxfp4_quantize(const void* x, int type, long long ld, int rows, int K, void* codes, void* scales, cudaStream_t st, bool early = false);
 cudaError_t launch_mxfp4_dequantize(const void* codes, const void* scales, int rows, int K, void* out, int type, cudaStream_t st);
 
 // Y[M][N] = Q(A)[M][K] W[N][K]^T with W in MXFP4, Q the rounding of A's rows to it, fp32 sums, Y in y_type (row stride N)
