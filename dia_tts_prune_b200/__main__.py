@@ -2,6 +2,8 @@
 
   generate  --model DIR --prompt "1 2 3" [--prompt ...] [--max-new-tokens N] [--temperature T] ...
             continue prompts given as token ids with the model of DIR (chosen by its config.json)
+  score     --model DIR --tokens "1 2 3" [--tokens ...] [--head-format bfloat16|mxfp4]
+            log-probabilities of texts given as token ids, one JSON object per text
   trace     --model DIR --dtype bfloat16|float32 --out DIR --max-tokens N
             replay a trace of steps from standard input and write the logits asked for (``bin/trace_run``)
   build     compile the CUDA libraries
@@ -24,7 +26,7 @@ def _cmd_build(a) -> int:
 
 def _cmd_generate(a) -> int:
     from .registry import load_model
-    model = load_model(a.model, dtype=a.dtype, max_tokens=a.max_tokens)
+    model = load_model(a.model, dtype=a.dtype, max_tokens=a.max_tokens, head_format=a.head_format)
     if not hasattr(model, "generate") or not hasattr(model, "run_step"):
         print("generate: this command serves the language models; use the Dia API for speech", file=sys.stderr)
         return 2
@@ -33,6 +35,21 @@ def _cmd_generate(a) -> int:
                           top_k=a.top_k, eos=a.eos, seed=a.seed)
     for o in outs:
         print(" ".join(str(t) for t in o))
+    return 0
+
+
+def _cmd_score(a) -> int:
+    import math
+
+    from .registry import load_model
+    model = load_model(a.model, dtype=a.dtype, max_tokens=a.max_tokens, head_format=a.head_format)
+    if not hasattr(model, "score"):
+        print("score: this command serves the language models", file=sys.stderr)
+        return 2
+    for logprobs in model.score([[int(t) for t in p.replace(",", " ").split()] for p in a.tokens]):
+        total = math.fsum(logprobs)
+        print(json.dumps({"tokens": len(logprobs), "logprob": total, "perplexity": math.exp(-total / len(logprobs)) if logprobs else None,
+                          "logprobs": logprobs}))
     return 0
 
 
@@ -87,7 +104,15 @@ def main(argv=None) -> int:
     g.add_argument("--top-k", type=int, default=None)
     g.add_argument("--eos", type=int, default=None)
     g.add_argument("--seed", type=int, default=None)
+    g.add_argument("--head-format", default="bfloat16", choices=["bfloat16", "mxfp4"], help="how the head is kept")
     g.set_defaults(fn=_cmd_generate)
+    s = sub.add_parser("score", help="log-probabilities of token-id texts under a language model")
+    s.add_argument("--model", required=True)
+    s.add_argument("--tokens", action="append", required=True, help="token ids separated by blanks or commas")
+    s.add_argument("--dtype", default="bfloat16")
+    s.add_argument("--max-tokens", type=int, default=4096, help="tokens the sequence state holds")
+    s.add_argument("--head-format", default="bfloat16", choices=["bfloat16", "mxfp4"], help="how the head is kept")
+    s.set_defaults(fn=_cmd_score)
     t = sub.add_parser("trace", help="replay steps from standard input, write logits")
     t.add_argument("--model", required=True)
     t.add_argument("--dtype", default="bfloat16")

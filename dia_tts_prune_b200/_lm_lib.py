@@ -20,9 +20,10 @@ ACT_SILU_GLU, ACT_XIELU, ACT_CLAMPED_GLU, ACT_RELU2, ACT_GELU_GLU, ACT_GELU = 0,
 ROUTER_SIGMOID_INPUT, ROUTER_SOFTMAX_TOP, ROUTER_SOFTMAX_GROUPED = 0, 1, 2
 GATE_SIGMOID, GATE_NONE, GATE_SILU, GATE_SIGMOID_HEAD = 0, 1, 2, 3
 ROT_INTERLEAVED, ROT_HALF = 0, 1
-ABI_VERSION = 6
+ABI_VERSION = 7
 PRECISION_FP32, PRECISION_BF16 = 0, 1
 TYPE_FP32, TYPE_BF16, TYPE_FP16 = 0, 1, 2
+LOSS_EACH, LOSS_SUM, LOSS_MEAN = 0, 1, 2
 E_OK, E_INVAL, E_CUDA, E_NOMEM, E_UNSUPPORTED = 0, -1, -2, -3, -5
 
 _vp, _i, _f = C.c_void_p, C.c_int32, C.c_float
@@ -66,7 +67,7 @@ class Model(C.Structure):
                 ("n_slots", _i), ("max_rows", _i), ("eps", _f), ("precision", _i), ("embed", _vp), ("head", _vp),
                 ("final_norm", Norm), ("page_table", _vp), ("step_graphs", _i), ("logit_scale", _f), ("embed_scale", _f),
                 ("embed_norm", _vp), ("bigram", _vp), ("bigram_buckets", _i), ("bigram_mul_prev", _i), ("bigram_mul_cur", _i),
-                ("token_pages", _vp)]
+                ("token_pages", _vp), ("head_codes", _vp), ("head_scales", _vp)]
 
 
 _ci = C.c_int
@@ -80,6 +81,7 @@ _SIGNATURES = {
     "lm_b200_engine_workspace_bytes": (C.c_size_t, [_vp]),
     "lm_b200_check": (_ci, [_vp, _vp]),
     "lm_b200_forward": (_ci, [_vp, _vp, _ci, _ci, _ci, _vp, _vp, _vp]),
+    "lm_b200_forward_hidden": (_ci, [_vp, _vp, _ci, _ci, _ci, _vp, _vp]),
     "lm_b200_op_norm_tapmix": (_ci, [_vp, _ci, _ci, _vp, _vp, _ci, _ci, _vp, _vp]),
     "lm_b200_op_mixer": (_ci, [_vp, _ci, _vp, _vp, _ci, _ci, _vp, _vp]),
     "lm_b200_op_attention": (_ci, [_vp, _ci, _vp, _vp, _ci, _ci, _vp, _vp]),
@@ -97,7 +99,7 @@ _SIGNATURES = {
     "lm_b200_op_linear_mxfp4_work_bytes": (C.c_size_t, [_ci, _ci, _ci]),
     "lm_b200_op_linear_mxfp4": (_ci, [_vp, _ci, C.c_int64, _vp, _vp, _vp, _ci, _ci, _ci, _ci, _vp, C.c_size_t, _vp]),
     "lm_b200_op_loss_work_bytes": (C.c_size_t, [_vp, _ci, C.c_int64, _vp, C.c_int64, _ci, _ci, _ci]),
-    "lm_b200_op_loss": (_ci, [_vp, _ci, C.c_int64, _vp, C.c_int64, _vp, _ci, C.c_int64, _ci, _ci, _ci, _cf, _vp, _vp, _vp, _vp, C.c_size_t, _vp]),
+    "lm_b200_op_loss": (_ci, [_vp, _ci, C.c_int64, _vp, C.c_int64, _vp, _ci, C.c_int64, _ci, _ci, _ci, _cf, _ci, _vp, _vp, _vp, C.c_size_t, _vp]),
     "lm_b200_op_loss_grad_work_bytes": (C.c_size_t, [_vp, C.c_int64, _vp, C.c_int64, _ci, _ci, _ci, _ci, _ci]),
     "lm_b200_op_loss_grad": (_ci, [_vp, C.c_int64, _vp, C.c_int64, _vp, _ci, C.c_int64, _ci, _ci, _ci, _cf, _vp, _vp, _ci, _vp, _vp, _vp, _vp, C.c_size_t,
                                    _vp]),

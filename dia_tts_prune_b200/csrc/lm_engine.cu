@@ -191,6 +191,7 @@ struct lm_b200_engine {
     // steps of a few rows are captured once per (rows, sequences, wanted) into a CUDA graph over these fixed buffers
     int32_t* step_static = nullptr;
     float* logits_static = nullptr;
+    void* head_work = nullptr;                   // rounded rows of a head in MXFP4
     cudaStream_t capture_stream = nullptr;       // captures run here (the caller's stream may be the legacy default stream)
     struct StepGraph { cudaGraphExec_t exec; long long launches; };
     std::map<std::tuple<int, int, int>, StepGraph> graphs;
@@ -1096,7 +1097,8 @@ int lm_b200_engine_create(const lm_b200_model* model, const lm_b200_layer* layer
     const lm_b200_model& m = *model;
     if (m.n_layer <= 0 || m.width <= 0 || m.vocab <= 0 || m.taps < 0 || m.taps > lm::kMaxTaps || m.page_size <= 0 ||
         m.max_pages <= 0 || m.n_slots <= 0 || m.max_rows <= 0 ||
-        (m.precision != LM_B200_PRECISION_FP32 && m.precision != LM_B200_PRECISION_BF16) || !m.embed || !m.head || !m.final_norm.w ||
+        (m.precision != LM_B200_PRECISION_FP32 && m.precision != LM_B200_PRECISION_BF16) || !m.embed ||
+        (!m.head && !m.head_codes) || (m.head_codes != nullptr) != (m.head_scales != nullptr) || !aligned(m.head_codes, 16) || !aligned(m.head_scales, 16) || !m.final_norm.w ||
         (!m.final_norm.b && m.final_norm.kind != LM_B200_NORM_LAYER && m.final_norm.kind != LM_B200_NORM_RMS) || !m.page_table)
         return LM_B200_EINVAL;
     for (int i = 0; i < m.n_layer; ++i) {
@@ -1233,6 +1235,7 @@ int lm_b200_engine_create(const lm_b200_model* model, const lm_b200_layer* layer
     for (const lm_b200_layer& l : e->layers) max_heads = std::max(max_heads, (size_t)l.heads);
     const size_t arrived_bytes = (size_t)lm::kAttnRowsKernelMax * max_heads * 4, o_arrived = take(arrived_bytes);
     const size_t o_step = take((size_t)(8 * lm::kRowsKernelMax) * 4), o_logits = take((size_t)lm::kRowsKernelMax * m.vocab * 4);
+    const size_t o_head4 = take(m.head_codes ? lm::mxfp4_linear_work_bytes(m.max_rows, m.vocab, m.width) : 0);
     const bool tcb = m.precision == LM_B200_PRECISION_BF16;
     const size_t o_hb = take(tcb ? R * D * 2 : 0), o_attb = take(tcb ? R * att * 2 : 0), o_packb = take(tcb ? slots * D * 2 : 0),
                  o_midb = take(tcb ? slots * F * 2 : 0), o_smidb = take(tcb ? R * Sf * 2 : 0), o_hwb = take(tcb ? R * D * 2 : 0);
@@ -1283,6 +1286,7 @@ int lm_b200_engine_create(const lm_b200_model* model, const lm_b200_layer* layer
     }
     e->step_static = (int32_t*)(b + o_step);
     e->logits_static = (float*)(b + o_logits);
+    e->head_work = b + o_head4;
     *out = e;
     return LM_B200_OK;
 }
@@ -1316,21 +1320,27 @@ int lm_b200_step_sizes(lm_b200_engine* e, const int32_t* rows, const int32_t* fi
 
 namespace {
 
-// the final norm of the wanted rows of x [M][width] and the logits
-int head_rows(lm_b200_engine* e, const float* x, const StepView& v, int n_want, float* logits_out, cudaStream_t st) {
+// the final norm of the wanted rows of x [M][width] and the logits, or (hidden_out) those rows alone
+int head_rows(lm_b200_engine* e, const float* x, const StepView& v, int n_want, float* logits_out, float* hidden_out, cudaStream_t st) {
     const int D = e->m.width;
     if (n_want > 0) {
         // the head is the largest single weight stream: from kHeadTensorRowsMin wanted rows on (a batch of decoding
         // sequences) the tensor-core kernel reads it once for all rows, where the row kernel reads it once per row
-        const bool tc = e->m.precision == LM_B200_PRECISION_BF16 && n_want >= kHeadTensorRowsMin &&
+        const bool four = e->m.head_codes != nullptr;
+        const bool tc = !hidden_out && !four && e->m.precision == LM_B200_PRECISION_BF16 && n_want >= kHeadTensorRowsMin &&
                         dia::gemm_tcgen05_shape_ok(n_want, e->m.vocab, D) && (reinterpret_cast<uintptr_t>(logits_out) & 15) == 0;
+        float* const rows = hidden_out ? hidden_out : e->hw;
         if (e->m.final_norm.kind == LM_B200_NORM_LAYER || e->m.final_norm.kind == LM_B200_NORM_RMS)
             LCK(lm::launch_layernorm_rows(x, v.want, e->m.final_norm.w, e->m.final_norm.b, e->m.eps,
-                                          e->m.logit_scale != 0.f ? e->m.logit_scale : 1.f, e->hw, tc ? e->hwb : nullptr, n_want, D, st,
+                                          e->m.logit_scale != 0.f ? e->m.logit_scale : 1.f, rows, tc ? e->hwb : nullptr, n_want, D, st,
                                           e->m.final_norm.kind == LM_B200_NORM_RMS));
         else
-            LCK(lm::launch_dyt_gather(x, v.want, N(e->m.final_norm), e->hw, tc ? e->hwb : nullptr, n_want, D, st));
-        if (tc)
+            LCK(lm::launch_dyt_gather(x, v.want, N(e->m.final_norm), rows, tc ? e->hwb : nullptr, n_want, D, st));
+        if (hidden_out) return LM_B200_OK;
+        if (four)
+            LCK(lm::launch_mxfp4_linear(lm::Mxfp4Product{e->hw, lm::kTypeF32, D, e->m.head_codes, e->m.head_scales, logits_out, lm::kTypeF32, n_want, e->m.vocab, D, nullptr, 0},
+                                        e->head_work, st));
+        else if (tc)
             LCK(dia::launch_gemm_tcgen05_bf16(e->hwb, 1, e->m.head, e->m.vocab, logits_out, n_want, e->m.vocab, D, kPlain, nullptr, st));
         else
             LCK(linear_f32(e, e->hw, D, e->m.head, logits_out, e->m.vocab, n_want, e->m.vocab, D, st));
@@ -1437,13 +1447,13 @@ int run_stream_layers(lm_b200_engine* e, const StepView& v, int M, int n_seq, fl
 
 // the launch sequence of one step
 int run_step(lm_b200_engine* e, const int32_t* step, int M, int n_seq, int n_want, float* logits_out, float* layers_out,
-             cudaStream_t st) {
+             cudaStream_t st, float* hidden_out = nullptr) {
     const StepView v = view(e, step, M, n_seq, st);
     const int D = e->m.width;
     if (e->stream_form) {
         const int rc = run_stream_layers(e, v, M, n_seq, layers_out, st);
         if (rc) return rc;
-        return head_rows(e, e->layers[0].streams == 1 ? e->xs : e->x, v, n_want, logits_out, st);
+        return head_rows(e, e->layers[0].streams == 1 ? e->xs : e->x, v, n_want, logits_out, hidden_out, st);
     }
     LCK(lm::launch_embed(e->m.embed, v.token, e->x, M, e->m.vocab, D, st));
     bool keep_x0 = false;
@@ -1489,7 +1499,7 @@ int run_step(lm_b200_engine* e, const int32_t* step, int M, int n_seq, int n_wan
                 return cuda_fail(cudaGetLastError());
         }
     }
-    return head_rows(e, e->x, v, n_want, logits_out, st);
+    return head_rows(e, e->x, v, n_want, logits_out, hidden_out, st);
 }
 
 // A step of a few rows is some forty short dependent launches: it is captured once per (rows, sequences, wanted) over
@@ -1553,6 +1563,15 @@ int lm_b200_forward(lm_b200_engine* e, const int32_t* step, int M, int n_seq, in
     if (e->m.step_graphs && M <= lm::kRowsKernelMax && !layers_out)
         return run_step_graph(e, step, M, n_seq, n_want, logits_out, S(stream));
     return run_step(e, step, M, n_seq, n_want, logits_out, layers_out, S(stream));
+}
+
+int lm_b200_forward_hidden(lm_b200_engine* e, const int32_t* step, int M, int n_seq, int n_want, float* hidden_out, void* stream) {
+    const TakesSizes once{e};
+    if (!e || !step || M <= 0 || M > e->m.max_rows || n_seq <= 0 || n_seq > M || n_want < 0 || n_want > M || (n_want > 0 && !hidden_out)) return LM_B200_EINVAL;
+    Guard g(e->device);
+    if (!g.ok) return LM_B200_ECUDA;
+    if (dia::take_ran_out(e->device, S(stream))) return cuda_fail(cudaErrorLaunchTimeout);
+    return run_step(e, step, M, n_seq, n_want, nullptr, nullptr, S(stream), hidden_out);
 }
 
 int lm_b200_op_norm_tapmix(lm_b200_engine* e, int layer, int sub, const float* x, const int32_t* step, int M, int n_seq,
@@ -1761,13 +1780,13 @@ size_t lm_b200_op_loss_work_bytes(const void* h, int h_type, int64_t ldh, const 
 }
 
 int lm_b200_op_loss(const void* h, int h_type, int64_t ldh, const void* W, int64_t ldw, const void* targets, int targets64, int64_t ignore, int M, int V, int K, float scale,
-                    float* loss, float* kept, float* totals, void* work, size_t work_bytes, void* stream) {
+                    int reduction, float* out, float* kept, void* work, size_t work_bytes, void* stream) {
     lm::LossShape s;
-    if (!loss_shape(s, h, h_type, ldh, W, ldw, M, V, K) || !targets || !(scale > 0.f) || !std::isfinite(scale) || !work || !aligned(work, 256) ||
+    if (!loss_shape(s, h, h_type, ldh, W, ldw, M, V, K) || !targets || !(scale > 0.f) || !std::isfinite(scale) || reduction < LM_B200_LOSS_EACH || reduction > LM_B200_LOSS_MEAN || !out || !work || !aligned(work, 256) ||
         work_bytes < lm::loss_work_bytes(s))
         return LM_B200_EINVAL;
     s.targets = targets; s.targets64 = targets64; s.ignore = ignore; s.scale = scale;
-    LCK(lm::launch_loss(s, loss, kept, totals, work, S(stream)));
+    LCK(lm::launch_loss(s, reduction, out, kept, work, S(stream)));
     return LM_B200_OK;
 }
 

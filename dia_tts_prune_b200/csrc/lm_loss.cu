@@ -434,7 +434,7 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
 //   warp 1    MMAs (M = 128, N = the columns), an accumulator for 16 k-blocks
 //   warps 2-5 take the accumulators out
 // Bound: the head's bytes.  Tensor memory is taken behind the wait for the predecessor and in front of the signal to the successor (see the few rows of 4-bit numbers).
-constexpr int kFewMost = 32, kFewThreads = 192, kFewCols = 256, kFewSlotsMost = 6, kFewChunk = 16;
+constexpr int kFewMost = 32, kFewCtas = 2 * 148, kFewThreads = 192, kFewCols = 256, kFewSlotsMost = 6, kFewChunk = 16;
 
 template <int NB, int TERMS>
 struct Few {
@@ -593,10 +593,10 @@ __global__ void __launch_bounds__(kFewThreads, 2) loss_few_rows_kernel(const __g
     for (int i = tid; i < 4 * M; i += kFewThreads) p.part[((size_t)(i >> 2) * gridDim.x + blockIdx.x) * 4 + (i & 3)] = meet[i & 3][i >> 2];
 }
 
-// The tiles of a row joined, a warp per row; where totals are asked for, the last block to come sums the rows, in their order.
+// The tiles of a row joined, a warp per row; where their sum or mean is asked for, the last block to come sums the rows, in their order.
 constexpr int kJoinWarps = 8;
 __global__ void __launch_bounds__(32 * kJoinWarps) loss_join_kernel(const float2* __restrict__ part, const float* __restrict__ hit, int M, int V, int tiles, const void* targets,
-                                                                    int targets64, long long ignore, float c, float* __restrict__ loss, float2* kept, float* __restrict__ totals,
+                                                                    int targets64, long long ignore, float c, int reduction, float* __restrict__ out, float2* kept,
                                                                     unsigned* arrived) {
     const int lane = threadIdx.x & 31, row = blockIdx.x * kJoinWarps + (threadIdx.x >> 5);
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -625,10 +625,10 @@ __global__ void __launch_bounds__(32 * kJoinWarps) loss_join_kernel(const float2
             // (the target's distance from the largest is taken before it meets the logarithm: losses near zero keep their digits)
             const float l = t == ignore ? 0.f : t < 0 || t >= V ? CUDART_NAN_F : (below - fmaf(hit[row], c, -most)) * kLn2;
             kept[row] = make_float2((most + below) * kLn2, l);
-            if (loss) loss[row] = l;
+            if (reduction == kLossEach) out[row] = l;
         }
     }
-    if (!totals) return;
+    if (reduction == kLossEach) return;
     __shared__ bool last;
     __shared__ int counts[kJoinWarps];
     __threadfence();
@@ -657,9 +657,8 @@ __global__ void __launch_bounds__(32 * kJoinWarps) loss_join_kernel(const float2
         s = 0.0;
         n = 0;
         for (int i = 0; i < kJoinWarps; ++i) { s += parts[i]; n += counts[i]; }
-        totals[0] = (float)s;
-        totals[1] = (float)n;
-        totals[2] = n ? (float)(s / n) : 0.f;
+        *out = reduction == kLossSum ? (float)s : n ? (float)(s / n) : 0.f;
+        *reinterpret_cast<float*>(kept + M) = (float)n;
     }
 }
 
@@ -822,7 +821,7 @@ struct Room {
     int parts = 0;                                                                      // of a row's logits
     int piece = 0, splits = 1;                                                          // columns of a piece of the vocabulary, shares of dh's contraction
 };
-Room room_of(const LossShape& s, bool grad, bool rows, bool head, int sms) {
+Room room_of(const LossShape& s, bool grad, bool rows, bool head) {
     Room r;
     size_t at = 0;
     const auto take = [&](size_t bytes) { const size_t was = at; at += up(bytes); return was; };
@@ -832,11 +831,11 @@ Room room_of(const LossShape& s, bool grad, bool rows, bool head, int sms) {
     r.w = take(in_place(s.w, s.ldw) ? 0 : (size_t)s.V * padded(s.K) * 2);
     if (!grad) {
         r.few = s.M <= kFewMost;
-        r.parts = r.few ? (int)std::min<long long>((s.V + 127) / 128, 2 * sms) * 4 : 2 * ((s.V + kTileN - 1) / kTileN);
+        r.parts = r.few ? (int)std::min<long long>((s.V + 127LL) / 128, kFewCtas) * 4 : 2 * ((s.V + kTileN - 1) / kTileN);
         r.part = take((size_t)s.M * r.parts * 8);
         r.hit = take((size_t)s.M * 4);
         r.arrived = take(4);
-        r.kept = take((size_t)s.M * 8);
+        r.kept = take((size_t)s.M * 8 + 4);
     } else {
         const long long all = (s.V + 255) / 256 * 256LL, fit = (64LL << 20) / 2 / s.M / 256 * 256;
         r.piece = (int)std::min(all, std::max(4096LL, fit));
@@ -861,18 +860,15 @@ LossTiles tiles_of(const LossShape& s) {
 
 }  // namespace
 
-size_t loss_work_bytes(const LossShape& s) {
-    int dev = 0, sms = 0;
-    return current_sms(&dev, &sms) == cudaSuccess ? room_of(s, false, false, false, sms).all : 0;
-}
-size_t loss_grad_work_bytes(const LossShape& s, bool rows, bool head) { return room_of(s, true, rows, head, 0).all; }
+size_t loss_work_bytes(const LossShape& s) { return room_of(s, false, false, false).all; }
+size_t loss_grad_work_bytes(const LossShape& s, bool rows, bool head) { return room_of(s, true, rows, head).all; }
 
-cudaError_t launch_loss(const LossShape& s, float* loss, float* kept, float* totals, void* work, cudaStream_t st) {
-    int dev = 0, sms = 0;
-    cudaError_t e = current_sms(&dev, &sms);
+cudaError_t launch_loss(const LossShape& s, int reduction, float* out, float* kept, void* work, cudaStream_t st) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     if (take_ran_out(dev, st)) return cudaErrorLaunchTimeout;
-    const Room r = room_of(s, false, false, false, sms);
+    const Room r = room_of(s, false, false, false);
     unsigned char* const base = reinterpret_cast<unsigned char*>(work);
     const void *h = s.h, *w = s.w;
     long long ldh = s.ldh, ldw = s.ldw;
@@ -910,8 +906,8 @@ cudaError_t launch_loss(const LossShape& s, float* loss, float* kept, float* tot
     attr.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, loss_join_kernel, (const float2*)p.part, (const float*)p.hit, s.M, s.V, r.parts, s.targets, s.targets64, s.ignore, p.c, loss,
-                              kept ? reinterpret_cast<float2*>(kept) : reinterpret_cast<float2*>(base + r.kept), totals, p.arrived);
+    return cudaLaunchKernelEx(&cfg, loss_join_kernel, (const float2*)p.part, (const float*)p.hit, s.M, s.V, r.parts, s.targets, s.targets64, s.ignore, p.c, reduction, out,
+                              kept ? reinterpret_cast<float2*>(kept) : reinterpret_cast<float2*>(base + r.kept), p.arrived);
 }
 
 cudaError_t launch_loss_grad(const LossShape& s, const float* kept, const LossGrad& by, void* dh, void* dw, void* work, cudaStream_t st) {
@@ -919,7 +915,7 @@ cudaError_t launch_loss_grad(const LossShape& s, const float* kept, const LossGr
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     if (take_ran_out(dev, st)) return cudaErrorLaunchTimeout;
-    const Room r = room_of(s, true, dh != nullptr, dw != nullptr, 0);
+    const Room r = room_of(s, true, dh != nullptr, dw != nullptr);
     unsigned char* const base = reinterpret_cast<unsigned char*>(work);
     const void *h = s.h, *w = s.w;
     long long ldh = s.ldh, ldw = s.ldw;

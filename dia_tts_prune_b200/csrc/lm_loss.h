@@ -17,13 +17,15 @@ struct LossShape {
 };
 // The operands that are laid out again in the workspace: rows that are fp32 or not of 16 bytes, a head whose rows are not
 size_t loss_work_bytes(const LossShape& s);
-// loss [M] (or null), kept [M][2]: log sum_j exp z[i][j] and the loss, for the gradient, or null; totals [3]: the sum of the losses, how many rows count, their mean (0 where none does), or null
-cudaError_t launch_loss(const LossShape& s, float* loss, float* kept, float* totals, void* work, cudaStream_t st);
+// out: every loss [M], or the sum or the mean (0 where none counts) of those that count.  kept [M][2] and one more (or null), for the gradient: log sum_j exp z[i][j] and the
+// loss, and (not with kLossEach) how many rows count
+enum LossReduction { kLossEach = 0, kLossSum = 1, kLossMean = 2 };
+cudaError_t launch_loss(const LossShape& s, int reduction, float* out, float* kept, void* work, cudaStream_t st);
 
 // The gradient by rows (dh [M][K] bf16) and by the head (dw [V][K] bf16), either or both; h is bf16
 struct LossGrad {
     const float* grad; int grad_stride;          // of every loss, grad_stride floats apart (0: one for all)
-    const float* count;                          // divides it where not null (totals + 1 of a mean)
+    const float* count;                          // divides it where not null (kept + 2 M of a mean)
 };
 size_t loss_grad_work_bytes(const LossShape& s, bool rows, bool head);
 cudaError_t launch_loss_grad(const LossShape& s, const float* kept, const LossGrad& by, void* dh, void* dw, void* work, cudaStream_t st);

@@ -14,6 +14,7 @@ import torch
 
 from . import _lm_lib
 from .lm_layers import BigramEmbedding, DynamicTanh, LayerNorm, MixLayer, RmsNorm
+from .lm_ops import Mxfp4, linear_cross_entropy, quantize_mxfp4
 from .lm_state import PagedState, Sequence
 
 
@@ -29,8 +30,9 @@ class LMEngine:
     def __init__(self, layers: list, embed: torch.Tensor, head: torch.Tensor, final_norm: DynamicTanh | LayerNorm | RmsNorm, *,
                  width: int, vocab: int, taps: int, eps: float, state: PagedState, max_rows: int = 1024,
                  precision: str = "bfloat16", step_graphs: bool = True, logit_scale: float = 1.0, embed_scale: float = 1.0,
-                 embed_norm: torch.Tensor | None = None, bigram: BigramEmbedding | None = None):
-        """``layers``: the layer records in execution order (a layer that runs twice per token appears twice, each time
+                 embed_norm: torch.Tensor | None = None, bigram: BigramEmbedding | None = None, head_format: str = "bfloat16"):
+        """``head_format``: ``"bfloat16"``, or ``"mxfp4"`` for a head in microscaled 4-bit numbers, whose input rows are rounded to them
+        as well.  ``layers``: the layer records in execution order (a layer that runs twice per token appears twice, each time
         with the state record of its own index).  ``bigram``: a pair table added to the embedding rows (stream records; the
         state keeps the tokens)."""
         if not torch.cuda.is_available():
@@ -43,7 +45,10 @@ class LMEngine:
             self.device = torch.device("cuda", torch.cuda.current_device())
         self.layers, self.state = layers, state
         self.embed = embed.detach().to(device=self.device, dtype=torch.bfloat16).contiguous()
-        self.head = head.detach().to(device=self.device, dtype=torch.bfloat16).contiguous()
+        if head_format not in ("bfloat16", "mxfp4"):
+            raise ValueError("head_format must be 'bfloat16' or 'mxfp4'")
+        head = head.detach().to(device=self.device, dtype=torch.bfloat16).contiguous()
+        self.head = head if head_format == "bfloat16" else quantize_mxfp4(head)
         self.final_norm = final_norm
         self.width, self.vocab, self.max_rows = int(width), int(vocab), int(max_rows)
         self._zeros = np.zeros(64, dtype=np.int32)
@@ -59,7 +64,11 @@ class LMEngine:
             raise ValueError("precision must be 'bfloat16' or 'float32'")
         self.precision = precision
         m.precision = _lm_lib.PRECISION_BF16 if precision == "bfloat16" else _lm_lib.PRECISION_FP32
-        m.embed, m.head = self.embed.data_ptr(), self.head.data_ptr()
+        m.embed = self.embed.data_ptr()
+        if head_format == "bfloat16":
+            m.head = self.head.data_ptr()
+        else:
+            m.head_codes, m.head_scales = self.head.data.data_ptr(), self.head.data.data_ptr() + self.head.scales_at
         final_norm.fill(m.final_norm)
         m.page_table = state.page_table.data_ptr()
         m.step_graphs = 1 if step_graphs else 0
@@ -136,21 +145,28 @@ class LMEngine:
         """Behind a synchronisation: raises if a wait of a kernel ran out since the last look (what it wrote is NaN)."""
         _lm_lib.check(self.lib.lm_b200_check(self._h, _stream(self.device)), "check")
 
-    def _forward(self, parts, logits_out: torch.Tensor | None, layers_out: torch.Tensor | None = None) -> None:
+    def _forward(self, parts, out: torch.Tensor | None, layers_out: torch.Tensor | None = None, hidden: bool = False) -> None:
         buf, M, S, W = self._pack(parts)
         self.state.sync_table()
-        _lm_lib.check(self.lib.lm_b200_forward(
-            self._h, buf.data_ptr(), M, S, W, logits_out.data_ptr() if W else None,
-            layers_out.data_ptr() if layers_out is not None else None, _stream(self.device)), "forward")
+        at = out.data_ptr() if W else None
+        if hidden:
+            _lm_lib.check(self.lib.lm_b200_forward_hidden(self._h, buf.data_ptr(), M, S, W, at, _stream(self.device)), "forward_hidden")
+        else:
+            _lm_lib.check(self.lib.lm_b200_forward(
+                self._h, buf.data_ptr(), M, S, W, at, layers_out.data_ptr() if layers_out is not None else None,
+                _stream(self.device)), "forward")
         self._keep = buf                                        # stays alive until the next call is queued behind it
 
-    def step(self, entries: list[tuple[Sequence, list[int], list[int]]], keep_layers: bool = False):
+    def step(self, entries: list[tuple[Sequence, list[int], list[int]]], keep_layers: bool = False, hidden: bool = False):
         """entries: (sequence, its next tokens, indexes among them whose logits are wanted).  Appends the tokens to the
         sequences' state and returns float32 logits ``[wanted, vocab]`` in the order of the entries (and, with
-        ``keep_layers``, the residual stream after every layer for all rows)."""
+        ``keep_layers``, the residual stream after every layer for all rows).  ``hidden``: the rows that the head would be multiplied
+        with, ``[wanted, width]``, in place of the logits."""
+        if keep_layers and hidden:
+            raise ValueError("keep_layers goes with logits")
         n_want = sum(len(w) for _, _, w in entries)
         total = sum(len(t) for _, t, _ in entries)
-        logits = torch.empty((n_want, self.vocab), dtype=torch.float32, device=self.device)
+        logits = torch.empty((n_want, self.width if hidden else self.vocab), dtype=torch.float32, device=self.device)
         streams = torch.empty((len(self.layers), total, self.width), dtype=torch.float32, device=self.device) if keep_layers else None
         if keep_layers and total > self.max_rows:
             raise ValueError("keep_layers needs the whole step in one portion")
@@ -163,7 +179,7 @@ class LMEngine:
             if not parts:
                 return
             w = sum(len(p[3]) for p in parts)
-            self._forward(parts, logits[done:done + w] if w else None, streams)
+            self._forward(parts, logits[done:done + w] if w else None, streams, hidden)
             done += w
             parts, rows = [], 0
 
@@ -190,6 +206,16 @@ class LMEngine:
                 inverse[asked] = produced
             logits = logits[torch.tensor(inverse, device=self.device)]
         return (logits, streams) if keep_layers else logits
+
+    def token_losses(self, hidden: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:
+        """Cross entropy of ``targets [rows]`` under the logits of ``hidden`` (rows of :meth:`step` with ``hidden``), float32 ``[rows]``, the
+        logits never in memory.  As in a long step, the rows are multiplied in bfloat16 unless the model's precision is float32; in front
+        of a head in 4 bits they are rounded to 4 bits, whose values bfloat16 holds."""
+        if isinstance(self.head, Mxfp4):
+            rows, head = quantize_mxfp4(hidden).dequantize(torch.bfloat16), self.head.dequantize(torch.bfloat16)
+        else:
+            rows, head = hidden if self.precision == "float32" else hidden.to(torch.bfloat16), self.head
+        return linear_cross_entropy(rows, head, targets, reduction="none")
 
     def argmax(self, logits: torch.Tensor) -> torch.Tensor:
         out = torch.empty((logits.shape[0],), dtype=torch.int32, device=logits.device)

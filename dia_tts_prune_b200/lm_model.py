@@ -331,7 +331,9 @@ class Scheduler:
 class CausalLM:
     def __init__(self, cfg: PubopelConfig | KupelixConfig | LuketarConfig | FipadraConfig | LoduzenConfig | ForilornConfig,
                  weights: dict[str, torch.Tensor], dtype: str = "bfloat16", device=None, max_tokens: int = 4096, max_sequences: int = 8, page_size: int = 16, max_rows: int = 1024,
-                 max_sequence_tokens: int | None = None, step_graphs: bool = True):
+                 max_sequence_tokens: int | None = None, step_graphs: bool = True, head_format: str = "bfloat16"):
+        """``head_format``: ``"mxfp4"`` keeps the head (and rounds the rows in front of it) in microscaled 4-bit numbers, 3.76 times fewer
+        bytes for every step to read; :meth:`score` says what a text loses by it."""
         if dtype not in ("bfloat16", "float32"):
             raise ValueError("dtype must be 'bfloat16' or 'float32'")
         if not torch.cuda.is_available():
@@ -374,7 +376,7 @@ class CausalLM:
         self.engine = LMEngine(self.layers, weights["embed"], head, final_norm, width=cfg.width, vocab=cfg.vocab,
                                taps=taps, eps=cfg.norm.eps, state=self.state, max_rows=max_rows, precision=dtype,
                                step_graphs=step_graphs, logit_scale=logit_scale, embed_scale=embed_scale, embed_norm=embed_norm,
-                               bigram=bigram)
+                               bigram=bigram, head_format=head_format)
         self._draws = 0
 
     @classmethod
@@ -404,6 +406,47 @@ class CausalLM:
         for name in end:
             if name in self.state.sequences:
                 self.state.close(name)
+        return out
+
+    @torch.inference_mode()
+    def score(self, sequences: list[list[int]]) -> list[list[float]]:
+        """The log-probability of every token of ``sequences`` behind its first one, given those in front of it (teacher-forced; a
+        sequence of ``n`` tokens has ``n - 1``).  The logits are not kept: their cross entropy is taken as the head is multiplied.
+        Sequences go through together as far as slots and pages last."""
+        out: list[list[float]] = []
+        for tokens in sequences:
+            bad = [t for t in tokens if not 0 <= int(t) < self.engine.vocab]
+            if bad:
+                raise ValueError(f"token {bad[0]} is not in the vocabulary of {self.engine.vocab}")
+        while len(out) < len(sequences):
+            group, entries = [], []
+            try:
+                pages = self.state.free_pages
+                for tokens in sequences[len(out):]:
+                    n = max(len(tokens) - 1, 0)
+                    need = self.state.pages_needed(None, n)
+                    if group and (self.state.free_slots == 0 or need > pages):
+                        break
+                    pages -= need
+                    seq = self.state.open(f"score{self._draws}_{len(group)}")
+                    group.append((seq, tokens))
+                    if n:
+                        entries.append((seq, [int(t) for t in tokens[:-1]], list(range(n))))
+                losses = []
+                if entries:
+                    hidden = self.engine.step(entries, hidden=True)
+                    targets = torch.tensor([int(t) for _, tokens in group for t in tokens[1:]], dtype=torch.int32, device=self.device)
+                    losses = self.engine.token_losses(hidden, targets).tolist()
+                    self.engine.check()
+            finally:
+                for seq, _ in group:
+                    self.state.close(seq.name)
+                self._draws += 1
+            at = 0
+            for _, tokens in group:
+                n = max(len(tokens) - 1, 0)
+                out.append([-x for x in losses[at:at + n]])
+                at += n
         return out
 
     # ---- sampling ------------------------------------------------------------------------------------------------

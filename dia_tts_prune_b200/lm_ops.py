@@ -26,8 +26,14 @@ def _check_rows(x: torch.Tensor, name: str, types=_TYPES) -> None:
         raise TypeError(f"{name} must be a tensor")
     if x.dtype not in types:
         raise TypeError(f"{name} must be one of {_names(types)}, not {x.dtype}")
-    if not x.is_cuda:
-        raise ValueError(f"{name} must live on a CUDA device (there is no CPU fallback)")
+
+
+def _check_device(device: torch.device, *others: torch.Tensor) -> None:
+    for t in others:
+        if t.device != device:
+            raise ValueError(f"operands live on {device} and {t.device}: they must live on one device")
+    if device.type != "cuda":
+        raise ValueError(f"operands must live on a CUDA device, not {device} (there is no CPU fallback)")
 
 
 def _call(what: str, device: torch.device, *args) -> None:
@@ -50,9 +56,8 @@ def _linear_work_bytes(m: int, n: int, k: int) -> int:
 
 
 @lru_cache(maxsize=1024)
-def _loss_work_bytes(h_at: int, h_type: int, ldh: int, w_at: int, ldw: int, m: int, v: int, k: int, device: int) -> int:
-    with torch.cuda.device(device):
-        return _lm_lib.load().lm_b200_op_loss_work_bytes(h_at | 4096, h_type, ldh, w_at | 4096, ldw, m, v, k)
+def _loss_work_bytes(h_at: int, h_type: int, ldh: int, w_at: int, ldw: int, m: int, v: int, k: int) -> int:
+    return _lm_lib.load().lm_b200_op_loss_work_bytes(h_at | 4096, h_type, ldh, w_at | 4096, ldw, m, v, k)
 
 
 @lru_cache(maxsize=1024)
@@ -122,6 +127,7 @@ def quantize_mxfp4(x: torch.Tensor) -> Mxfp4:
     if x.dim() != 2:
         raise ValueError(f"x must have two dimensions, not {x.dim()}")
     _no_grad("quantize_mxfp4", x)
+    _check_device(x.device)
     x = _as_rows(x)
     (rows, width), device = x.shape, x.device
     q = Mxfp4(rows, width, device)
@@ -141,13 +147,12 @@ def linear_mxfp4(a: torch.Tensor, w: Mxfp4, out_dtype: torch.dtype | None = None
     if not a.dim() or a.shape[-1] != w.width:
         raise ValueError(f"a has rows of {a.shape[-1] if a.dim() else 0} channels, w of {w.width}")
     device = a.device
-    if device != w.data.device:
-        raise ValueError(f"a lives on {device}, w on {w.data.device}")
     if out_dtype is None:
         out_dtype = a.dtype
     elif out_dtype not in _TYPES:
         raise TypeError(f"out_dtype must be one of {_names(_TYPES)}, not {out_dtype}")
     _no_grad("linear_mxfp4", a)
+    _check_device(device, w.data)
     y = torch.empty((*a.shape[:-1], w.rows), dtype=out_dtype, device=device)
     if not w.width:
         return y.zero_()
@@ -173,25 +178,26 @@ def _loss_operands(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Te
         raise ValueError(f"hidden {tuple(hidden.shape)} and weight {tuple(weight.shape)} do not share a width")
     if targets.shape != hidden.shape[:-1]:
         raise ValueError(f"targets {tuple(targets.shape)} do not go with hidden {tuple(hidden.shape)}")
-    if weight.device != hidden.device or targets.device != hidden.device:
-        raise ValueError("hidden, weight and targets must live on one device")
     if not weight.numel():
         raise ValueError("weight is empty")
 
 
+_REDUCTIONS = {"none": _lm_lib.LOSS_EACH, "sum": _lm_lib.LOSS_SUM, "mean": _lm_lib.LOSS_MEAN}
+
+
 def _losses(hidden, weight, targets, scale, ignore_index, reduction, keep):
-    """(losses or their sum or mean; with ``keep`` what the gradient needs: [log-sum, loss] of every row, and how many rows count)."""
+    """(losses or their sum or mean; the targets as they were read; with ``keep`` what the gradient needs: [log-sum, loss] of every row and
+    how many rows count)."""
     h, w, t = _as_rows(hidden), _as_rows(weight), targets.contiguous()
     (M, K), V, device = h.shape, w.shape[0], h.device
-    each = reduction == "none"
-    out = torch.empty(M if each else 3, dtype=torch.float32, device=device)
-    kept = torch.empty(2 * M, dtype=torch.float32, device=device) if keep else None
-    h_at, w_at, out_at, h_type, ldh, ldw = h.data_ptr(), w.data_ptr(), out.data_ptr(), _TYPES[h.dtype], h.stride(0), w.stride(0)
-    need = _loss_work_bytes(h_at & 255, h_type, ldh, w_at & 255, ldw, M, V, K, device.index)
+    out = torch.empty(M if reduction == "none" else (), dtype=torch.float32, device=device)
+    kept = torch.empty(2 * M + 1, dtype=torch.float32, device=device) if keep else None
+    h_at, w_at, h_type, ldh, ldw = h.data_ptr(), w.data_ptr(), _TYPES[h.dtype], h.stride(0), w.stride(0)
+    need = _loss_work_bytes(h_at & 255, h_type, ldh, w_at & 255, ldw, M, V, K)
     work = torch.empty(need, dtype=torch.uint8, device=device)
-    _call("loss", device, h_at, h_type, ldh, w_at, ldw, t.data_ptr(), t.dtype == torch.int64, ignore_index, M, V, K, scale, out_at if each else None,
-          kept.data_ptr() if keep else None, None if each else out_at, work.data_ptr(), need)
-    return (out if each else out[2 if reduction == "mean" else 0]), t, kept, out
+    _call("loss", device, h_at, h_type, ldh, w_at, ldw, t.data_ptr(), t.dtype == torch.int64, ignore_index, M, V, K, scale,
+          _REDUCTIONS[reduction], out.data_ptr(), kept.data_ptr() if keep else None, work.data_ptr(), need)
+    return out, t, kept
 
 
 class _LinearCrossEntropy(torch.autograd.Function):
@@ -199,17 +205,16 @@ class _LinearCrossEntropy(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, hidden, weight, targets, scale, ignore_index, reduction):
-        out, t, kept, totals = _losses(hidden, weight, targets, scale, ignore_index, reduction, True)
+        out, t, kept = _losses(hidden, weight, targets, scale, ignore_index, reduction, True)
         ctx.save_for_backward(hidden, weight, t, kept)
-        # (the count stands beside the result, which may be changed in place: not a saved tensor)
-        ctx.args = scale, ignore_index, totals[1:2].detach() if reduction == "mean" else None
+        ctx.args = scale, ignore_index, reduction == "mean"
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
         hidden, weight, t, kept = ctx.saved_tensors
-        scale, ignore_index, count = ctx.args
+        scale, ignore_index, mean = ctx.args
         need_h, need_w = ctx.needs_input_grad[:2]
         (M, K), V, device = hidden.shape, weight.shape[0], hidden.device
         h, w, grad = _as_rows(hidden), _as_rows(weight), grad.to(torch.float32)
@@ -220,8 +225,9 @@ class _LinearCrossEntropy(torch.autograd.Function):
         h_at, w_at, ldh, ldw = h.data_ptr(), w.data_ptr(), h.stride(0), w.stride(0)
         need = _loss_grad_work_bytes(h_at & 255, ldh, w_at & 255, ldw, M, V, K, need_h, need_w)
         work = torch.empty(need, dtype=torch.uint8, device=device)
-        _call("loss_grad", device, h_at, ldh, w_at, ldw, t.data_ptr(), t.dtype == torch.int64, ignore_index, M, V, K, scale, kept.data_ptr(), grad.data_ptr(),
-              grad.stride(0) if grad.dim() else 0, None if count is None else count.data_ptr(), dh.data_ptr() if need_h else None,
+        kept_at = kept.data_ptr()
+        _call("loss_grad", device, h_at, ldh, w_at, ldw, t.data_ptr(), t.dtype == torch.int64, ignore_index, M, V, K, scale, kept_at,
+              grad.data_ptr(), grad.stride(0) if grad.dim() else 0, kept_at + 8 * M if mean else None, dh.data_ptr() if need_h else None,
               dw.data_ptr() if need_w else None, work.data_ptr(), need)
         return dh, dw, None, None, None, None
 
@@ -236,7 +242,7 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
     gradients by ``hidden`` and ``weight`` take the vocabulary in pieces; rows that do not count have no part in them, whatever they hold.
     """
     _loss_operands(hidden, weight, targets)
-    if reduction not in ("none", "sum", "mean"):
+    if reduction not in _REDUCTIONS:
         raise ValueError("reduction must be 'none', 'sum' or 'mean'")
     scale, ignore_index = float(scale), int(ignore_index)
     if not 0.0 < scale < float("inf"):
@@ -244,6 +250,7 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
     with_grad = (hidden.requires_grad or weight.requires_grad) and torch.is_grad_enabled()
     if with_grad and hidden.dtype != torch.bfloat16:
         raise ValueError("gradients need hidden in bfloat16")
+    _check_device(hidden.device, weight, targets)
     if not targets.numel():
         rows = hidden.new_zeros(targets.shape, dtype=torch.float32)
         return rows if reduction == "none" else rows.sum()

@@ -35,7 +35,7 @@
 extern "C" {
 #endif
 
-#define LM_B200_ABI_VERSION 6
+#define LM_B200_ABI_VERSION 7
 
 enum lm_b200_status { LM_B200_OK = 0, LM_B200_EINVAL = -1, LM_B200_ECUDA = -2, LM_B200_ENOMEM = -3, LM_B200_EUNSUPPORTED = -5 };
 
@@ -235,6 +235,8 @@ typedef struct lm_b200_model {
     const void *bigram;            /* bf16 [bigram_buckets + 1][width]; NULL: none */
     int32_t bigram_buckets, bigram_mul_prev, bigram_mul_cur;
     int32_t *token_pages;          /* [pages][page_size] token ids, on the page table of the keys and values */
+    /* The head in MXFP4 (both or neither; see lm_b200_op_mxfp4_quantize): `head` may then be NULL, the rows in front of it are rounded too */
+    const void *head_codes, *head_scales;
 } lm_b200_model;
 
 typedef struct lm_b200_engine lm_b200_engine;
@@ -262,6 +264,9 @@ int lm_b200_check(lm_b200_engine *e, void *stream);
  * float32 [n_layer][M][width]. */
 int lm_b200_forward(lm_b200_engine *e, const int32_t *step, int M, int n_seq, int n_want, float *logits_out,
                     float *layers_out, void *stream);
+
+/* The same without the head: the wanted rows behind the final norm (and the logit scale), float32 [n_want][width] - what a loss takes in place of the logits. */
+int lm_b200_forward_hidden(lm_b200_engine *e, const int32_t *step, int M, int n_seq, int n_want, float *hidden_out, void *stream);
 
 /* ---- the mechanisms one at a time (operator boundaries; `step` has the layout above with n_want = 0) ---- */
 /* out = tapmix(norm_in(x)) of sublayer `sub` (0 mixer, 1 feed-forward) of `layer`, and the tail update */
@@ -317,15 +322,16 @@ int lm_b200_op_linear_mxfp4(const void *A, int a_type, int64_t lda, const void *
 /* ---- cross entropy of rows under a head, and its gradient, without the logits in memory ----
  * z = scale h W^T (h [M][K] fp32 or bf16, row stride ldh; W [V][K] bf16, row stride ldw; scale > 0); loss[i] = log sum_j exp z[i][j] - z[i][target[i]], 0 for a row whose
  * target is `ignore`, NaN for one whose target is neither that nor in [0, V).  targets: int32, or int64 where targets64 != 0.  Operands of fp32 rows are exact to 24 bits
- * (three bf16 terms), sums fp32.  loss [M] may be NULL; kept [M][2]: log sum_j exp z[i][j] and the loss, for the gradient, or NULL; totals [3]: the losses' sum, how many rows
- * count, their mean (0 where none does), or NULL.
+ * (three bf16 terms), sums fp32.  out: every loss [M], or one number, the sum or the mean over the rows that count (0 where none does).  kept [2 M + 1] (or NULL), for the
+ * gradient: log sum_j exp z[i][j] and the loss of every row, and behind them (with a sum or a mean) how many rows count.
  * The gradient (h in bf16): P = softmax(z) - onehot, g = scale grad [/ max(*count, 1)], dh_i = g_i P_i W (bf16 [M][K]), dW = P^T (g h) (bf16 [V][K]), either may be NULL.  grad:
  * fp32, of every loss, grad_stride apart (0: one number).  Rows that do not count have no part in either, whatever they hold; a NaN loss has NaN gradients.
  * P is kept in bf16 for a piece of the vocabulary at a time.  work: 256-byte aligned. */
-/* (of h and W the alignment counts; the current device is asked for its SMs) */
+/* (of h and W the alignment counts) */
+enum lm_b200_loss_reduction { LM_B200_LOSS_EACH = 0, LM_B200_LOSS_SUM = 1, LM_B200_LOSS_MEAN = 2 };
 size_t lm_b200_op_loss_work_bytes(const void *h, int h_type, int64_t ldh, const void *W, int64_t ldw, int M, int V, int K);
 int lm_b200_op_loss(const void *h, int h_type, int64_t ldh, const void *W, int64_t ldw, const void *targets, int targets64, int64_t ignore, int M, int V, int K, float scale,
-                    float *loss, float *kept, float *totals, void *work, size_t work_bytes, void *stream);
+                    int reduction, float *out, float *kept, void *work, size_t work_bytes, void *stream);
 size_t lm_b200_op_loss_grad_work_bytes(const void *h, int64_t ldh, const void *W, int64_t ldw, int M, int V, int K, int rows, int head);
 int lm_b200_op_loss_grad(const void *h, int64_t ldh, const void *W, int64_t ldw, const void *targets, int targets64, int64_t ignore, int M, int V, int K, float scale,
                          const float *kept, const float *grad, int grad_stride, const float *count, void *dh, void *dW, void *work, size_t work_bytes, void *stream);

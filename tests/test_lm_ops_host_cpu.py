@@ -1,0 +1,129 @@
+"""What the operators of lm_ops refuse, and how their C entries answer what they do not take: without a GPU."""
+
+import ctypes as C
+import math
+
+import pytest
+import torch
+
+from dia_tts_prune_b200 import _lm_lib, lm_ops
+
+
+def test_rows_and_matrices_that_are_refused():
+    x = torch.randn(4, 64)
+    for bad in (x.double(), x.int(), x.to(torch.complex64)):
+        with pytest.raises(TypeError):
+            lm_ops.quantize_mxfp4(bad)
+    with pytest.raises(TypeError):
+        lm_ops.quantize_mxfp4([1.0])
+    for bad in (x[0], x[None]):
+        with pytest.raises(ValueError, match="two dimensions"):
+            lm_ops.quantize_mxfp4(bad)
+    with pytest.raises(ValueError, match="gradient"):
+        lm_ops.quantize_mxfp4(x.clone().requires_grad_(True))
+    with pytest.raises(ValueError, match="CUDA"):
+        lm_ops.quantize_mxfp4(x)
+
+
+def test_products_that_are_refused():
+    w = lm_ops.Mxfp4(8, 64, torch.device("cpu"))
+    x = torch.randn(4, 64)
+    with pytest.raises(TypeError):
+        lm_ops.linear_mxfp4(x, torch.randn(8, 64))
+    with pytest.raises(TypeError):
+        lm_ops.linear_mxfp4(x.long(), w)
+    with pytest.raises(TypeError):
+        lm_ops.linear_mxfp4(x, w, out_dtype=torch.float64)
+    for bad in (x[:, :63], torch.tensor(1.0)):
+        with pytest.raises(ValueError, match="channels"):
+            lm_ops.linear_mxfp4(bad, w)
+    with pytest.raises(ValueError, match="gradient"):
+        lm_ops.linear_mxfp4(x.clone().requires_grad_(True), w)
+    with pytest.raises(ValueError, match="CUDA"):
+        lm_ops.linear_mxfp4(x, w)
+    with pytest.raises(TypeError):
+        w.dequantize(torch.float64)
+    assert w.shape == (8, 64) and w.device.type == "cpu"
+    # 8 rows of 128 channels (64 are there) in half a byte each, one piece of 128 x 4 scales
+    assert w.nbytes == 8 * 64 + 512 and w.scales_at == 512
+
+
+def test_losses_that_are_refused():
+    h, w, t = torch.randn(6, 32).bfloat16(), torch.randn(10, 32).bfloat16(), torch.zeros(6, dtype=torch.long)
+    f = lm_ops.linear_cross_entropy
+    for a in ((h.half(), w, t), (h, w.float(), t), (h, w, t.float()), (h, w, t.bool()), (h, w, [0] * 6)):
+        with pytest.raises(TypeError):
+            f(*a)
+    for a in ((h[:, :31], w, t), (h, w[0], t), (h, w, t[:5]), (h, w, t[:, None]), (h, w[:0], t)):
+        with pytest.raises(ValueError):
+            f(*a)
+    for k in (dict(reduction="max"), dict(scale=0.0), dict(scale=-1.0), dict(scale=math.inf), dict(scale=math.nan)):
+        with pytest.raises(ValueError):
+            f(h, w, t, **k)
+    for a in ((h.float().requires_grad_(True), w, t), (h.float(), w.clone().requires_grad_(True), t)):
+        with pytest.raises(ValueError, match="bfloat16"):
+            f(*a)
+    with pytest.raises(ValueError, match="CUDA"):
+        f(h, w, t)
+    if torch.cuda.is_available():
+        with pytest.raises(ValueError, match="one device"):
+            f(h.cuda(), w, t)
+
+
+def test_c_entries_answer_bad_arguments():
+    """None of these reaches a device: 0 bytes, or LM_B200_EINVAL."""
+    lib = _lm_lib.load()
+    at, odd = 1 << 20, (1 << 20) + 8                               # (addresses that are never followed)
+    q = lib.lm_b200_op_mxfp4_quantize
+    for a in ((None, 0, 64, 4, 64, at, at), (at, 3, 64, 4, 64, at, at), (at, 0, 63, 4, 64, at, at), (at, 0, 64, 0, 64, at, at), (at, 0, 64, 4, 0, at, at),
+              (at, 0, 64, 4, 64, odd, at), (at, 0, 64, 4, 64, at, None), (at, 0, 1 << 30, 4, 1 << 25, at, at)):
+        assert q(*a, None) == _lm_lib.E_INVAL
+    for a in ((at, at, 0, 64, at, 0), (at, at, 4, 64, None, 0), (at, at, 4, 64, at, 7), (odd, at, 4, 64, at, 0)):
+        assert lib.lm_b200_op_mxfp4_dequantize(*a, None) == _lm_lib.E_INVAL
+    assert lib.lm_b200_mxfp4_code_bytes(0, 64) == 0 and lib.lm_b200_mxfp4_code_bytes(3, 65) == 3 * 64 and lib.lm_b200_mxfp4_scale_bytes(129, 129) == 2 * 2 * 512
+    need = lib.lm_b200_op_linear_mxfp4_work_bytes(200, 64, 64)
+    assert need >= 200 * 64 and lib.lm_b200_op_linear_mxfp4_work_bytes(0, 64, 64) == 0
+    f = lib.lm_b200_op_linear_mxfp4
+    good = [at, 1, 64, at, at, at, 1, 200, 64, 64, at, need]
+    for i, bad in ((0, None), (1, 5), (2, 63), (3, None), (3, odd), (4, None), (5, None), (6, -1), (7, 0), (8, 0), (9, 0), (10, None), (10, at + 64), (11, need - 1)):
+        a = list(good)
+        a[i] = bad
+        assert f(*a, None) == _lm_lib.E_INVAL, i
+    need = lib.lm_b200_op_loss_grad_work_bytes(at, 64, at, 64, 100, 300, 64, 1, 1)
+    assert need > 0 and lib.lm_b200_op_loss_grad_work_bytes(at, 63, at, 64, 100, 300, 64, 1, 1) == 0
+    f = lib.lm_b200_op_loss_grad
+    good = [at, 64, at, 64, at, 1, -100, 100, 300, 64, 1.0, at, at, 0, None, at, at, at, need]
+    for i, bad in ((0, None), (1, 63), (2, None), (3, 63), (4, None), (7, 0), (8, 0), (9, 0), (10, 0.0), (10, math.nan), (10, math.inf), (11, None), (12, None), (13, -1),
+                   (17, None), (17, at + 128), (18, need - 1)):
+        a = list(good)
+        a[i] = bad
+        assert f(*a, None) == _lm_lib.E_INVAL, i
+    a = list(good)
+    a[15] = a[16] = None
+    assert f(*a, None) == _lm_lib.E_INVAL
+    f = lib.lm_b200_op_loss
+    good = [at, 1, 64, at, 64, at, 1, -100, 100, 300, 64, 1.0, 2, at, at, at, 1 << 30]
+    for i, bad in ((0, None), (1, 2), (2, 63), (3, None), (4, 63), (5, None), (8, 0), (9, 0), (10, 0), (11, -1.0), (12, 3), (12, -1), (13, None), (15, None), (15, at + 8), (16, 0)):
+        a = list(good)
+        a[i] = bad
+        assert f(*a, None) == _lm_lib.E_INVAL, i
+    assert lib.lm_b200_forward_hidden(None, at, 1, 1, 1, at, None) == _lm_lib.E_INVAL
+
+
+def test_a_head_is_there_once():
+    """engine_create: a head, or codes with their scales"""
+    lib, out = _lm_lib.load(), C.c_void_p()
+    for codes, scales in ((None, None), (1 << 20, None), (None, 1 << 20), ((1 << 20) + 4, 1 << 20)):
+        m = _lm_lib.Model(n_layer=1, width=8, vocab=8, page_size=4, max_pages=1, n_slots=1, max_rows=1, embed=1 << 20, page_table=1 << 20)
+        m.final_norm.w = m.final_norm.b = 1 << 20
+        m.head_codes, m.head_scales = codes, scales
+        m.head = 1 << 20 if scales and not codes else None
+        assert lib.lm_b200_engine_create(C.byref(m), (_lm_lib.Layer * 1)(), 0, C.byref(out)) == _lm_lib.E_INVAL
+
+
+def test_score_command_parses():
+    from dia_tts_prune_b200.__main__ import main
+    with pytest.raises(SystemExit):
+        main(["score", "--model", "x"])
+    with pytest.raises(SystemExit):
+        main(["generate", "--model", "x", "--prompt", "1", "--head-format", "int4"])

@@ -1,0 +1,289 @@
+"""Scoring texts under served models, heads in 4 bits, and the operators one behind the other: captured, on other streams, twice at once."""
+
+import json
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def model(design="pubopel", dtype="float32", **kw):
+    from dia_tts_prune_b200 import lm_config as CFG
+    from dia_tts_prune_b200 import synthetic as SY
+    from dia_tts_prune_b200.lm_model import CausalLM
+    if design == "pubopel":
+        cfg = SY.pubopel_config(width=96, layers=2, heads=4, kv_heads=2, dim=24, experts=4, top=2, expert_ff=40, shared_ff=56, vocab=301, window=20, keep_first=3)
+        w, c = SY.pubopel_weights(cfg, 3), CFG.PubopelConfig.model_validate(cfg)
+    elif design == "fipadra":
+        cfg = SY.fipadra_config(width=64, kinds=["delta", "retention"], heads=4, dim=16, vdim=16, vocab=301, ff=96, logit_scale=0.5)
+        w, c = SY.fipadra_weights(cfg, 3), CFG.FipadraConfig.model_validate(cfg)
+    else:
+        cfg = SY.kupelix_config(width=64, kinds=["attention", "hgrn2"], heads=4, kv_heads=2, dim=16, vdim=16, vocab=301, ff=96)
+        w, c = SY.kupelix_weights(cfg, 3), CFG.KupelixConfig.model_validate(cfg)
+    return CausalLM(c, w, dtype=dtype, device="cuda:0", **{**dict(max_tokens=256, max_sequences=3, page_size=8, max_rows=64), **kw})
+
+
+def texts(lengths, seed=0, vocab=301):
+    g = torch.Generator().manual_seed(seed)
+    return [torch.randint(0, vocab, (n,), generator=g).tolist() for n in lengths]
+
+
+def rows_of(m, sequences):
+    """Per sequence the rows in front of the head, as the engine gives them."""
+    out = []
+    for s in sequences:
+        seq = m.state.open("x")
+        out.append(m.engine.step([(seq, s[:-1], list(range(len(s) - 1)))], hidden=True))
+        m.state.close("x")
+    return out
+
+
+def expected(hidden, head, sequence):
+    """log-probabilities in 64 bits and how far off float32 sums of exact products may be: a loss moves by twice a logit (2^-22 of the
+    magnitudes at each of K / 16 steps of three terms, see the losses' own tests) and by 2^-18 for exponentials and logarithms."""
+    h, w, t = hidden.double().cpu(), head.double().cpu(), torch.tensor(sequence[1:])
+    logp = torch.log_softmax(h @ w.T, 1).gather(1, t[:, None])[:, 0]
+    return logp, 2 * (3 * h.shape[1] / 16 + 6) * 2.0 ** -22 * (h.abs() @ w.abs().T).amax(1) + 2.0 ** -18
+
+
+@pytest.mark.parametrize("design", ["pubopel", "kupelix", "fipadra"])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_scores_of_served_models(design, dtype):
+    m = model(design, dtype)
+    sequences = texts((40, 2, 150, 1, 3, 0, 64, 90))              # more than there are slots, longer than a step, nothing to score
+    got = m.score(sequences)
+    assert [len(g) for g in got] == [39, 1, 149, 0, 2, 0, 63, 89]
+    assert m.state.free_slots == 3 and m.state.free_pages == m.state.n_pages and not m.state.sequences
+    head = m.engine.head
+    for s, g in zip(sequences, got):
+        if len(s) < 2:
+            continue
+        hidden, = rows_of(m, [s])
+        # a sequence of its own and the same one beside others go through kernels for other numbers of rows: hidden differs by their roundings,
+        # which float32 rows show as 2^-12 of the largest logit at most; bfloat16 products by the steps of bfloat16
+        want, off = expected(hidden if dtype == "float32" else hidden.bfloat16(), head, s)
+        slack = (2.0 ** -12 if dtype == "float32" else 2.0 ** -4) * (hidden.double().cpu() @ head.double().cpu().T).abs().amax(1)
+        assert ((torch.tensor(g, dtype=torch.float64) - want).abs() <= off + slack).all()
+        assert all(x <= 0 for x in g)
+
+
+@pytest.mark.parametrize("design", ["pubopel", "kupelix", "fipadra"])
+def test_hidden_rows_are_what_the_head_multiplies(design):
+    m = model(design)
+    for n in (1, 2, 40, 64):
+        s = texts((n,), seed=n)[0]
+        a, b = m.state.open("a"), m.state.open("b")
+        want = sorted({0, n // 2, n - 1})
+        logits = m.engine.step([(a, s, want)])
+        hidden = m.engine.step([(b, s, want)], hidden=True)
+        assert hidden.shape == (len(want), m.engine.width)
+        ref = hidden.double() @ m.engine.head.double().T
+        # (the rows of the two steps may come from a captured and an uncaptured pass of the same kernels; logits are float32 sums)
+        assert ((logits.double() - ref).abs() <= 2.0 ** -16 * (hidden.double().abs() @ m.engine.head.double().abs().T)).all()
+        m.state.close("a"), m.state.close("b")
+    with pytest.raises(ValueError):
+        m.engine.step([], keep_layers=True, hidden=True)
+
+
+def test_scores_refuse_and_leave_nothing():
+    from dia_tts_prune_b200.lm_state import OutOfPages
+    m = model()
+    for bad in ([1, 301], [-1, 2]):
+        with pytest.raises(ValueError):
+            m.score([[1, 2, 3], bad])
+    with pytest.raises(OutOfPages):
+        m.score(texts((300,)))
+    assert m.state.free_slots == 3 and m.state.free_pages == m.state.n_pages and not m.state.sequences
+    assert m.score([]) == []
+
+
+@pytest.mark.parametrize("design", ["pubopel", "fipadra"])
+def test_heads_in_4_bits(design):
+    """Logits are the product of the rounded rows and the rounded head (exact products, float32 sums); scores are their log-softmax; decoding
+    picks the largest; and the whole head's bytes shrink by 3.76."""
+    from dia_tts_prune_b200 import lm_ops
+    m, plain = model(design, head_format="mxfp4"), model(design)
+    head = m.engine.head.dequantize()
+    assert torch.equal(head, lm_ops.quantize_mxfp4(plain.engine.head).dequantize())
+    for n, wants in ((1, [0]), (40, [39]), (64, list(range(64)))):
+        s = texts((n,), seed=n)[0]
+        a = m.state.open("a")
+        logits = m.engine.step([(a, s, wants)])
+        m.state.close("a")
+        a = m.state.open("a")
+        hidden = m.engine.step([(a, s, wants)], hidden=True)
+        m.state.close("a")
+        rows = lm_ops.quantize_mxfp4(hidden).dequantize()
+        ref, most = rows.double() @ head.double().T, rows.double().abs() @ head.double().abs().T
+        # one step of 4 bits where the two passes' rows round to neighbours: a row may differ in a few elements by half its block's largest
+        close = (logits.double() - ref).abs() <= (hidden.shape[1] / 64 + 2) * 2.0 ** -22 * most
+        assert close.float().mean() > 0.9 and ((logits.double() - ref).abs() <= 0.25 * most).all()
+    got = m.score(texts((50, 33)))
+    for s, g in zip(texts((50, 33)), got):
+        hidden, = rows_of(m, [s])
+        want, off = expected(lm_ops.quantize_mxfp4(hidden).dequantize(), head, s)
+        assert ((torch.tensor(g, dtype=torch.float64) - want).abs() <= off + 0.25).all()
+    out = m.generate(texts((5, 9)), max_new_tokens=6)
+    assert [len(o) for o in out] == [6, 6] and all(0 <= t < 301 for o in out for t in o)
+    assert m.generate(texts((5, 9)), max_new_tokens=6) == out
+
+
+def test_score_command(tmp_path, capsys):
+    from dia_tts_prune_b200 import synthetic as SY
+    from dia_tts_prune_b200.__main__ import main
+    from dia_tts_prune_b200.checkpoint import save_safetensors
+    cfg = SY.pubopel_config(width=64, layers=1, heads=2, kv_heads=1, dim=32, experts=2, top=1, expert_ff=16, shared_ff=None, vocab=50)
+    (tmp_path / "config.json").write_text(json.dumps(cfg))
+    save_safetensors(tmp_path / "model.safetensors", SY.pubopel_weights(cfg, 1))
+    for fmt in ("bfloat16", "mxfp4"):
+        assert main(["score", "--model", str(tmp_path), "--tokens", "1 2 3 4", "--tokens", "7", "--head-format", fmt]) == 0
+        a, b = (json.loads(line) for line in capsys.readouterr().out.strip().splitlines())
+        assert a["tokens"] == 3 == len(a["logprobs"]) and abs(math.exp(-a["logprob"] / 3) - a["perplexity"]) < 1e-6
+        assert b == {"tokens": 0, "logprob": 0.0, "perplexity": None, "logprobs": []}
+
+
+# ---- the operators one behind the other ------------------------------------------------------------------------------------------------
+
+def chain(x, w4, head, t):
+    """A matrix in 4 bits, then the head's loss and both gradients."""
+    from dia_tts_prune_b200 import lm_ops
+    y = lm_ops.linear_mxfp4(x, w4).requires_grad_(True)
+    head = head.detach().requires_grad_(True)
+    loss = lm_ops.linear_cross_entropy(y, head, t)
+    return (loss.detach(), *torch.autograd.grad(loss, (y, head)), lm_ops.linear_cross_entropy(y.detach()[:5].float(), head.detach(), t[:5], reduction="none"),
+            lm_ops.linear_mxfp4(x[:3], w4))
+
+
+def inputs(m, seed):
+    from dia_tts_prune_b200 import lm_ops
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    x = torch.randn(m, 192, generator=g, device="cuda").bfloat16()
+    w4 = lm_ops.quantize_mxfp4(torch.randn(256, 192, generator=g, device="cuda") / 14)
+    head = (torch.randn(1111, 256, generator=g, device="cuda") / 16).bfloat16()
+    return x, w4, head, torch.randint(0, 1111, (m,), generator=g, device="cuda")
+
+
+def test_the_chain_is_reproducible_and_captured():
+    """The same bits every time, from a captured graph too, whose inputs may change between replays; two graphs share nothing."""
+    a, b = inputs(300, 1), inputs(300, 2)
+    want = [chain(*i) for i in (a, b)]
+    for i, w in ((a, want[0]), (b, want[1])):
+        assert all(torch.equal(u, v) for u, v in zip(chain(*i), w))
+    graphs = []
+    for i in (a, b):
+        x, w4, head, t = i[0].clone(), i[1], i[2].clone(), i[3].clone()
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            for _ in range(2):
+                chain(x, w4, head, t)
+        torch.cuda.current_stream().wait_stream(s)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = chain(x, w4, head, t)
+        graphs.append((g, out, x, head, t))
+    for _ in range(3):
+        for g, *_ in graphs:
+            g.replay()
+    torch.cuda.synchronize()
+    for (g, out, *_), w in zip(graphs, want):
+        assert all(torch.equal(u, v) for u, v in zip(out, w))
+    g, out, x, head, t = graphs[0]
+    x.copy_(b[0]), t.copy_(b[3])
+    g.replay()
+    for u, v in zip(out, chain(b[0], a[1], a[2], b[3])):
+        assert torch.equal(u, v)
+
+
+def test_two_streams_at_once():
+    a, b = inputs(150, 3), inputs(170, 4)
+    want = [chain(*i) for i in (a, b)]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    for _ in range(10):
+        for k, i in enumerate((a, b)):
+            with torch.cuda.stream(streams[k]):
+                got[k].append(chain(*i))
+    torch.cuda.synchronize()
+    for k in (0, 1):
+        for out in got[k]:
+            assert all(torch.equal(u, v) for u, v in zip(out, want[k]))
+
+
+def test_a_matrix_laid_out_right_before_its_product():
+    """Products ask for their weights before their predecessor has ended: not before one that writes them has."""
+    from dia_tts_prune_b200 import lm_ops
+    g = torch.Generator(device="cuda").manual_seed(5)
+    ws = [torch.randn(4096, 1024, generator=g, device="cuda") for _ in range(3)]
+    for m in (1, 40):
+        x = torch.randn(m, 1024, generator=g, device="cuda").bfloat16()
+        want = []
+        for w in ws:
+            q = lm_ops.quantize_mxfp4(w)
+            torch.cuda.synchronize()
+            want.append(lm_ops.linear_mxfp4(x, q))
+        torch.cuda.synchronize()
+        for _ in range(5):
+            got = []
+            for w in ws:
+                lm_ops.linear_mxfp4(x, q)
+                q = lm_ops.quantize_mxfp4(w)                       # (its memory is an earlier one's)
+                got.append(lm_ops.linear_mxfp4(x, q))
+            assert all(torch.equal(u, v) for u, v in zip(got, want))
+
+
+def test_results_do_not_alias_what_the_gradient_needs():
+    """A loss changed in place before its backward pass; hidden changed in place is noticed."""
+    from dia_tts_prune_b200.lm_ops import linear_cross_entropy
+    x, _, head, t = inputs(64, 6)
+    h = torch.randn(64, 256, device="cuda").bfloat16().requires_grad_(True)
+    head.requires_grad_(True)
+    want = torch.autograd.grad(linear_cross_entropy(h, head, t) * 0.5, (h, head))
+    loss = linear_cross_entropy(h, head, t)
+    loss *= 0.5
+    assert all(torch.equal(u, v) for u, v in zip(torch.autograd.grad(loss, (h, head)), want))
+    each = linear_cross_entropy(h, head, t, reduction="none")
+    each.mul_(0.0)
+    assert not torch.autograd.grad(each.sum(), h)[0].any()
+    k = h.detach().clone().requires_grad_(True)
+    loss = linear_cross_entropy(k, head, t)
+    with torch.no_grad():
+        k.add_(1)
+    with pytest.raises(RuntimeError, match="in-?place"):
+        loss.backward()
+    loss = linear_cross_entropy(h, head, t)
+    loss.backward(retain_graph=True)
+    once = h.grad.clone()
+    loss.backward()
+    assert torch.equal(h.grad, once * 2) and h.grad.dtype == head.grad.dtype == torch.bfloat16
+
+
+def test_a_wait_that_ran_out_shows():
+    """With no looks at any barrier every wait ends at once: results are NaN, the next call reports it, the one behind is whole again."""
+    import ctypes as C
+
+    from dia_tts_prune_b200 import _lm_lib, lm_ops
+    x, w4, head, t = inputs(300, 7)
+    polls = getattr(_lm_lib.load(), "_ZN3dia15gemm_pair_pollsEv")
+    polls.restype = C.POINTER(C.c_uint)
+    y = lm_ops.linear_mxfp4(x, w4)
+    calls = [lambda: lm_ops.linear_mxfp4(x, w4), lambda: lm_ops.linear_mxfp4(x[:2], w4), lambda: lm_ops.linear_cross_entropy(y, head, t, reduction="none"),
+             lambda: lm_ops.linear_cross_entropy(y[:2], head, t[:2], reduction="none")]
+    leaf = y.clone().requires_grad_(True)
+    loss = lm_ops.linear_cross_entropy(leaf, head, t)
+    kept = polls()[0]
+    for call in calls:
+        want = call()
+        polls()[0] = 0
+        try:
+            got = call()
+        finally:
+            polls()[0] = kept
+        torch.cuda.synchronize()
+        assert got.isnan().all()
+        with pytest.raises(RuntimeError):
+            call()
+        assert torch.equal(call(), want)
+    torch.autograd.grad(loss, leaf, retain_graph=True)
