@@ -206,8 +206,8 @@ constexpr int kBM = 128, kBN = 128, kStageK = 256;            // rows of A and o
 constexpr int kCodeTile = 128 * 128;                          // 128 rows x 256 channels, 16 KB
 constexpr int kStageBytes = 2 * kCodeTile + 2 * 1024;         // A, W, their scales
 constexpr int kStages = 5;
-constexpr int kThreads4 = 192;
-constexpr int kTurnBytes = 4 * 4096;
+constexpr int kFewThreads = 192, kWarps4 = 8, kThreads4 = 64 + 32 * kWarps4;
+constexpr int kTurnBytes = kWarps4 * 4096;
 constexpr int kSmem4 = kStages * kStageBytes + kTurnBytes + 1024 + 256;
 
 // scales of 128 rows x 128 channels in shared memory: 8 rows of 16 bytes after one another, no swizzle
@@ -239,10 +239,91 @@ struct TiledProduct {
     unsigned polls;
 };
 
+// 32 rows (lane = row) x 128 bytes of results - kUnit columns - from an accumulator, turned through shared memory so that whole lines are stored.
+template <int TYPE>
+struct Out {
+    static constexpr int kUnit = TYPE == kTypeF32 ? 32 : 64;
+    static constexpr int kBytes = TYPE == kTypeF32 ? 4 : 2;
+};
+__device__ __forceinline__ uint32_t pack16(int type, float lo, float hi) {
+    if (type == kTypeBf16) {
+        const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t*>(&b);
+    }
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <int TYPE>
+__device__ __forceinline__ void take_out(uint32_t from, unsigned char* blk, const TiledProduct& p, int row0, int rows, int n0, int lane, bool ok, bool wide) {
+    uint32_t w[32];
+    if constexpr (TYPE == kTypeF32) {
+        tmem_columns32(from, w);
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+    } else {
+        uint32_t v[2][32];
+        tmem_columns32(from, v[0]);
+        tmem_columns32(from + 32, v[1]);
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+        for (int e = 0; e < 32; ++e) w[e] = pack16(TYPE, __uint_as_float(v[e >> 4][2 * e & 31]), __uint_as_float(v[e >> 4][(2 * e & 31) + 1]));
+    }
+    if (!ok) {
+#pragma unroll
+        for (int e = 0; e < 32; ++e) w[e] = TYPE == kTypeF32 || TYPE == kTypeBf16 ? 0x7fff7fffu : 0x7e007e00u;      // (no result: NaN as one number or two)
+    }
+    // a row's 16-byte piece c goes to place c ^ (row % 8) of its 128 bytes
+#pragma unroll
+    for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(blk + lane * 128 + ((c ^ (lane & 7)) << 4)) = make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+    __syncwarp();
+    const int cols = min(Out<TYPE>::kUnit, p.N - n0), rr = lane >> 3, ch = lane & 7;
+    char* const y = reinterpret_cast<char*>(p.y) + ((size_t)row0 * p.N + n0) * Out<TYPE>::kBytes;
+    const size_t pitch = (size_t)p.N * Out<TYPE>::kBytes;
+    if (wide) {                                               // a row per eight lanes
+        uint4 u[8];
+#pragma unroll
+        for (int g = 0; g < 8; ++g) u[g] = *reinterpret_cast<const uint4*>(blk + (4 * g + rr) * 128 + ((ch ^ ((4 * g + rr) & 7)) << 4));
+        const bool in = ch * (16 / Out<TYPE>::kBytes) < cols;
+#pragma unroll
+        for (int g = 0; g < 8; ++g)
+            if (in && 4 * g + rr < rows) *reinterpret_cast<uint4*>(y + (4 * g + rr) * pitch + 16 * ch) = u[g];
+    } else {
+        // A row per warp, eight rows in flight, a 4-byte word per lane.  Where a row of 16-bit numbers begins half way into a word of memory, a lane's word is made of the
+        // second number of the lane in front and its own first one.
+#pragma unroll 1
+        for (int r0 = 0; r0 < rows; r0 += 8) {
+            uint32_t u[8];
+#pragma unroll
+            for (int g = 0; g < 8; ++g) u[g] = *reinterpret_cast<const uint32_t*>(blk + (r0 + g) * 128 + (((lane >> 2) ^ g) << 4) + 4 * (lane & 3));
+#pragma unroll
+            for (int g = 0; g < 8; ++g) {
+                char* const row = y + (r0 + g) * pitch;
+                if constexpr (TYPE == kTypeF32) {
+                    if (r0 + g < rows && lane < cols) *reinterpret_cast<uint32_t*>(row + 4 * lane) = u[g];
+                } else {
+                    const uint32_t front = __shfl_up_sync(0xffffffffu, u[g], 1);
+                    if (r0 + g >= rows) continue;
+                    const int off = (int)(reinterpret_cast<uintptr_t>(row) >> 1 & 1), c = 2 * lane - off;
+                    const uint32_t word = off ? __funnelshift_r(front, u[g], 16) : u[g];
+                    if (c >= 0 && c + 1 < cols) *reinterpret_cast<uint32_t*>(row + 2 * c) = word;
+                    // what stands alone at either end: the first number, the last one (of 64: a second store of the last lane)
+                    const bool front_end = c < 0, back_end = c == cols - 1, last = off && lane == 31 && cols == 64;
+                    if (front_end || back_end || last)
+                        *reinterpret_cast<uint16_t*>(row + 2 * (front_end ? 0 : back_end ? c : 63)) = (uint16_t)(front_end ? u[g] : back_end ? word : u[g] >> 16);
+                }
+            }
+        }
+    }
+    __syncwarp();
+}
+
+template <int TYPE>
+__device__ __forceinline__ bool whole_pieces(const TiledProduct& p) { return p.N * Out<TYPE>::kBytes % 16 == 0 && (reinterpret_cast<uintptr_t>(p.y) & 15) == 0; }
+
 // One CTA per SM walks 128 x 128 tiles.
 //   warp 0    one lane: a stage's codes (TMA, 128-byte swizzle) and scales (plain bulk copies)
 //   warp 1    one elected lane: the stage's scales into tensor memory, then its MMAs of 64 channels
-//   warps 2-5 take a finished accumulator out through shared memory while the next tile fills the other
+//   warps 2-9 take a finished accumulator out through shared memory while the next tile fills the other (with four of them 4096 x 16383 x 256, whose rows begin anywhere,
+//             took 102 us in fp32)
 template <int TYPE>
 __global__ void __launch_bounds__(kThreads4, 1)
 mxfp4_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ TiledProduct p) {
@@ -260,7 +341,7 @@ mxfp4_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < kStages; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
-        for (int i = 0; i < 2; ++i) { mbar_init(&t_full[i], 1); mbar_init(&t_empty[i], 4); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&t_full[i], 1); mbar_init(&t_empty[i], kWarps4); }
         fence_mbar_init();
     }
     if (warp == 1) {
@@ -340,36 +421,17 @@ mxfp4_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
             }
         }
     } else {
-        const int q = warp & 3, rr = lane >> 3, ch = lane & 7;
-        float* const blk = reinterpret_cast<float*>(turn + (warp - 2) * 4096);
-        const bool wide = p.N % 4 == 0 && (reinterpret_cast<uintptr_t>(p.y) & 15) == 0;
+        const int q = warp & 3, c_half = ((warp - 2) >> 2) * (kBN / 2);      // (a warp reads the 32 lanes of its number mod 4) and its half of the columns
+        unsigned char* const blk = turn + (warp - 2) * 4096;
+        const bool wide = whole_pieces<TYPE>(p);
         unsigned it = 0;
         for (int t = blockIdx.x; t < n_tiles; t += gridDim.x, ++it) {
             const int n0 = t / tiles_m * kBN, row0 = t % tiles_m * kBM + q * 32, rows = min(32, p.M - row0);
             ok = ok && pair_wait(&t_full[it & 1u], (it >> 1) & 1u, p.polls);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
-            for (int cb = 0; cb < kBN / 32; ++cb) {
-                const int n = n0 + cb * 32 + 4 * ch;
-                if (n0 + cb * 32 >= p.N || rows <= 0) break;
-                uint32_t v[32];
-                tmem_columns32(tmem + ((uint32_t)(q * 32) << 16) + (it & 1u) * kBN + cb * 32, v);
-                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                // lane = row: its 16-byte piece c goes to place c ^ (row % 8) of its 128 bytes, and is read a row per eight lanes
-#pragma unroll
-                for (int c = 0; c < 8; ++c)
-                    *reinterpret_cast<uint4*>(blk + lane * 32 + ((c ^ (lane & 7)) << 2)) = make_uint4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
-                __syncwarp();
-#pragma unroll
-                for (int g = 0; g < 8; ++g) {
-                    const int r = 4 * g + rr;
-                    if (r >= rows || n >= p.N) break;
-                    float4 f = *reinterpret_cast<const float4*>(blk + r * 32 + ((ch ^ (r & 7)) << 2));
-                    if (!ok) f = make_float4(CUDART_NAN_F, CUDART_NAN_F, CUDART_NAN_F, CUDART_NAN_F);      // (no result)
-                    put4<TYPE>(p.y, (size_t)(row0 + r) * p.N + n, f, p.N - n, wide);
-                }
-                __syncwarp();
-            }
+            for (int c = c_half; c < c_half + kBN / 2 && n0 + c < p.N && rows > 0; c += Out<TYPE>::kUnit)
+                take_out<TYPE>(tmem + ((uint32_t)(q * 32) << 16) + (it & 1u) * kBN + c, blk, p, row0, rows, n0 + c, lane, ok, wide);
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive(&t_empty[it & 1u]);
@@ -385,6 +447,169 @@ mxfp4_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
     if (warp == 1) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+    }
+}
+
+// The same on pairs of SMs: a cluster of two CTAs owns a 256 x 192 tile, an MMA of the pair multiplies the 256 rows of both by the 192 columns of both, so an SM takes 28 KB
+// of codes from L2 for 384 cycles of MMAs where the kernel above takes 32 KB for 256.  192 columns: two accumulators leave 128 columns of tensor memory for scales.  Each
+// SM needs the scales of its own 128 rows and of all 192 columns; those of an odd tile begin half way into a block of 128, two columns further.
+//   warp 0    one lane per CTA: codes and scales (TMA) of its halves; every byte of both CTAs counts on the leader's barrier
+//   warp 1    leader only: a stage's scales into the tensor memory of both, then the pair's MMAs; commits to the barriers of both
+//   warps 2-9 take the CTA's 128 rows of a finished accumulator out, half of the columns each
+constexpr int kPairN = 192, kPairStages = 6, kPairWarps = 8, kPairThreads = 64 + 32 * kPairWarps;
+constexpr int kPairCodes = kCodeTile + kPairN / 2 * 128, kPairStage = kPairCodes + 3 * 1024;
+constexpr int kPairSmem = kPairStages * kPairStage + kPairWarps * 4096 + 1024 + 256;
+static_assert(kPairStage % 1024 == 0 && kPairSmem <= 227 * 1024, "shared memory");
+
+__device__ __forceinline__ void scales_to_tmem_pair(uint32_t tmem, uint64_t desc) {
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+}
+__device__ __forceinline__ void umma_mxfp4_pair(uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t a_scales, uint32_t b_scales, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+        ::"r"(d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(a_scales), "r"(b_scales), "r"(accumulate)
+        : "memory");
+}
+
+template <int TYPE>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+mxfp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_as,
+                  const __grid_constant__ CUtensorMap map_ws, const __grid_constant__ TiledProduct p) {
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    unsigned char* turn = smem + kPairStages * kPairStage;
+    uint64_t* full = reinterpret_cast<uint64_t*>(turn + kPairWarps * 4096);  // (the leader's alone)
+    uint64_t* empty = full + kPairStages;
+    uint64_t* t_full = empty + kPairStages;
+    uint64_t* t_empty = t_full + 2;                                          // (the leader's alone)
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(t_empty + 2);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = blockIdx.x & 1;
+    const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+    const int pieces = (p.K + 127) / 128, n_stage = (pieces + 1) / 2;
+    const int tiles_m = (p.M + 255) / 256, n_tiles = tiles_m * ((p.N + kPairN - 1) / kPairN);
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kPairStages; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&t_full[i], 1); mbar_init(&t_empty[i], 2 * kPairWarps); }
+        fence_mbar_init();
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::);
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    cluster_sync_all();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = *tmem_slot;
+    bool ok = true;
+    if (warp == 0) {
+        if (lane == 0) {
+            // a stage's weights, which do not wait for the kernel that rounds the rows, and its rows (t, s: its tile and place there)
+            const auto weights = [&](unsigned at, int t, int s) {
+                const int n0 = t / tiles_m * kPairN;
+                const uint32_t bar = at_rank(&full[at], 0), dst = smem_u32(smem + at * kPairStage);
+                if (rank == 0) mbar_arrive_expect_tx(&full[at], 2u * kPairStage);
+                tma_load_2d_pair(dst + kCodeTile, &map_w, bar, s * (kStageK / 2), n0 + (int)rank * (kPairN / 2));
+                tma_load_2d_pair(dst + kPairCodes + 1024, &map_ws, bar, 0, n0 / 128 * pieces + 2 * s);
+                tma_load_2d_pair(dst + kPairCodes + 2048, &map_ws, bar, 0, (n0 / 128 + 1) * pieces + 2 * s);
+            };
+            const auto rows = [&](unsigned at, int t, int s) {
+                const int m = t % tiles_m * 2 + (int)rank;
+                const uint32_t bar = at_rank(&full[at], 0), dst = smem_u32(smem + at * kPairStage);
+                tma_load_2d_pair(dst, &map_a, bar, s * (kStageK / 2), m * 128);
+                tma_load_2d_pair(dst + kPairCodes, &map_as, bar, 0, m * pieces + 2 * s);
+            };
+            unsigned i = 0;
+            int t = pair, s = 0;
+            const auto next = [&]() {
+                ++i;
+                if (++s == n_stage) s = 0, t += pairs;
+            };
+            while (i < kPairStages && t < n_tiles) { weights(i, t, s); next(); }
+            const unsigned ahead = i;
+            asm volatile("griddepcontrol.wait;" ::: "memory");
+            i = 0; t = pair; s = 0;
+            while (i < ahead) { rows(i, t, s); next(); }
+            for (; t < n_tiles; next()) {
+                const unsigned at = i % kPairStages;
+                if (!lane_wait(&empty[at], ((i / kPairStages) & 1u) ^ 1u, p.polls)) { ok = false; break; }
+                weights(at, t, s);
+                rows(at, t, s);
+            }
+            // (the leader's last commits arrive here: not after this CTA has gone)
+            for (unsigned j = i > (unsigned)kPairStages ? i - kPairStages : 0; j < i && ok; ++j) ok = lane_wait(&empty[j % kPairStages], (j / kPairStages) & 1u, p.polls);
+            // (nor do copies arrive that were issued before a wait ran out)
+            for (unsigned j = i > (unsigned)kPairStages ? i - kPairStages : 0; j < i && !ok && rank == 0; ++j)
+                (void)lane_wait(&full[j % kPairStages], (j / kPairStages) & 1u, p.polls);
+        }
+    } else if (warp == 1) {
+        if (rank == 0) {
+            const uint32_t two = mx_idesc(kPairN, 0) ^ (3u << 27), idesc[2] = {two, two | (mx_idesc(0, 1) ^ mx_idesc(0, 0))};      // M = 256
+            unsigned i = 0, it = 0;
+            for (int t = pair; t < n_tiles && ok; t += pairs, ++it) {
+                if (!pair_wait(&t_empty[it & 1u], ((it >> 1) & 1u) ^ 1u, p.polls)) { ok = false; break; }
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint32_t d = tmem + (it & 1u) * kPairN, shift = t / tiles_m & 1 ? 2 : 0;
+                for (int s = 0; s < n_stage; ++s, ++i) {
+                    const unsigned at = i % kPairStages;
+                    if (!pair_wait(&full[at], (i / kPairStages) & 1u, p.polls)) { ok = false; break; }
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint32_t base = smem_u32(smem + at * kPairStage);
+                    const uint64_t adesc = umma_desc(base), bdesc = umma_desc(base + kCodeTile);
+                    const uint32_t sa = tmem + 2 * kPairN + (i & 3u) * 32, sb = sa + 8;
+                    const int here = min(2, pieces - 2 * s);
+                    if (elect_one_sync()) {
+                        for (int c = 0; c < here; ++c) {
+                            scales_to_tmem_pair(sa + 4 * c, scale_desc(base + kPairCodes + c * kMxScaleBytes));
+                            scales_to_tmem_pair(sb + 8 * c, scale_desc(base + kPairCodes + 1024 + c * kMxScaleBytes));
+                            scales_to_tmem_pair(sb + 8 * c + 4, scale_desc(base + kPairCodes + 2048 + c * kMxScaleBytes));
+                        }
+                        for (int c = 0; c < here; ++c)
+#pragma unroll
+                            for (int j = 0; j < 2; ++j)
+                                umma_mxfp4_pair(d, adesc + 4 * c + 2 * j, bdesc + 4 * c + 2 * j, idesc[j], sa + 4 * c, sb + 8 * c + shift, (s | c | j) != 0 ? 1u : 0u);
+                        umma_commit_pair(&empty[at]);
+                        if (s == n_stage - 1) umma_commit_pair(&t_full[it & 1u]);
+                    }
+                    __syncwarp();
+                }
+            }
+        }
+    } else {
+        constexpr int kUnits = kPairN / Out<TYPE>::kUnit;     // three or six: the two warps of a quarter take the middle one in turns, or half of them each
+        const int q = warp & 3, second = (warp - 2) >> 2;
+        unsigned char* const blk = turn + (warp - 2) * 4096;
+        const bool wide = whole_pieces<TYPE>(p);
+        unsigned it = 0;
+        for (int t = pair; t < n_tiles; t += pairs, ++it) {
+            const int n0 = t / tiles_m * kPairN, row0 = t % tiles_m * 256 + (int)rank * 128 + q * 32, rows = min(32, p.M - row0);
+            const int border = (kUnits + (int)(it & 1u)) / 2;
+            ok = ok && pair_wait(&t_full[it & 1u], (it >> 1) & 1u, p.polls);
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll 1
+            for (int u = second ? border : 0; u < (second ? kUnits : border); ++u) {
+                const int c = u * Out<TYPE>::kUnit;
+                if (n0 + c >= p.N || rows <= 0) break;
+                take_out<TYPE>(tmem + ((uint32_t)(q * 32) << 16) + (it & 1u) * kPairN + c, blk, p, row0, rows, n0 + c, lane, ok, wide);
+            }
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(at_rank(&t_empty[it & 1u], 0)) : "memory");
+        }
+    }
+    if (!ok && lane == 0 && p.ran_out) {
+        *reinterpret_cast<volatile int*>(p.ran_out) = 1;
+        __threadfence_system();
+    }
+    __syncwarp();
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    cluster_sync_all();                                       // neither CTA's memory goes while the other still reads it or arrives there
+    if (warp == 1) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
     }
 }
 
@@ -418,7 +643,7 @@ __device__ __forceinline__ void put1(void* y, int type, size_t at, float v) {
     else reinterpret_cast<__half*>(y)[at] = __float2half_rn(v);
 }
 
-__global__ void __launch_bounds__(kThreads4, 1) mxfp4_few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ FewProduct p) {
+__global__ void __launch_bounds__(kFewThreads, 1) mxfp4_few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ FewProduct p) {
     constexpr int kSlot = kCodeTile + 1024, kRows = NB * 128 + 1024;       // a stage of weights, of rows
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -453,16 +678,16 @@ __global__ void __launch_bounds__(kThreads4, 1) mxfp4_few_rows_kernel(const __gr
     const auto take = [&](auto type, auto wide) {
         constexpr int TYPE = decltype(type)::value, kBatch = TYPE == kTypeF32 ? 4 : 8;
         constexpr bool WIDE = decltype(wide)::value;
-        for (int i0 = tid; i0 < items; i0 += kThreads4 * kBatch) {           // (a warp is in or out as a whole)
+        for (int i0 = tid; i0 < items; i0 += kFewThreads * kBatch) {           // (a warp is in or out as a whole)
             Eight<TYPE, WIDE> x8[kBatch];
 #pragma unroll
             for (int b = 0; b < kBatch; ++b) {
-                const int i = i0 + b * kThreads4, m = i / per_row, k = s0 * kStageK + 8 * (i - m * per_row);
+                const int i = i0 + b * kFewThreads, m = i / per_row, k = s0 * kStageK + 8 * (i - m * per_row);
                 x8[b].fetch(reinterpret_cast<const char*>(p.a) + (long long)m * p.lda * (TYPE == kTypeF32 ? 4 : 2), k, i < items ? p.K - k : 0);
             }
 #pragma unroll
             for (int b = 0; b < kBatch; ++b) {
-                const int i = i0 + b * kThreads4, m = i / per_row, c = i - m * per_row;
+                const int i = i0 + b * kFewThreads, m = i / per_row, c = i - m * per_row;
                 if (i >= items) break;
                 float v[8];
                 x8[b].widen(v);
@@ -479,7 +704,7 @@ __global__ void __launch_bounds__(kThreads4, 1) mxfp4_few_rows_kernel(const __gr
     if (p.a_type == kTypeF32) take_type(std::integral_constant<int, kTypeF32>());
     else if (p.a_type == kTypeBf16) take_type(std::integral_constant<int, kTypeBf16>());
     else take_type(std::integral_constant<int, kTypeF16>());
-    for (int i = tid; i < (NB - M) * per_row; i += kThreads4) {               // columns that no row uses
+    for (int i = tid; i < (NB - M) * per_row; i += kFewThreads) {               // columns that no row uses
         const int m = M + i / per_row, c = i % per_row;
         *reinterpret_cast<uint32_t*>(place(m, c)) = 0u;
         if ((c & 3) == 0) rows[(c >> 5) * kRows + NB * 128 + ((c & 31) >> 4) * kMxScaleBytes + (m & 31) * 16 + (m >> 5) * 4 + ((c >> 2) & 3)] = 0;
@@ -554,7 +779,7 @@ __global__ void __launch_bounds__(kThreads4, 1) mxfp4_few_rows_kernel(const __gr
     if (S > 1) {
         cluster_sync_all();
         // the outputs of the tile, dealt to the cluster's CTAs
-        for (int i = rank * kThreads4 + tid; i < M * 128; i += S * kThreads4) {
+        for (int i = rank * kFewThreads + tid; i < M * 128; i += S * kFewThreads) {
             const int m = i >> 7, n = n0 + (i & 127);
             if (n >= p.N) continue;
             float u[8];
@@ -581,24 +806,78 @@ bool codes_map(CUtensorMap* map, const void* codes, int rows, int K, int box_row
                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// scales, a row of 512 bytes per piece, two pieces at a time
+bool scales_map(CUtensorMap* map, const void* scales, int rows, int K) {
+    const EncodeTiledFn enc = encode_tiled();
+    if (!enc) return false;
+    const cuuint64_t dims[2] = {kMxScaleBytes / 4, (cuuint64_t)(mx_scale_bytes(rows, K) / kMxScaleBytes)}, strides[1] = {kMxScaleBytes};
+    const cuuint32_t box[2] = {kMxScaleBytes / 4, 2}, estr[2] = {1, 1};
+    return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, const_cast<void*>(scales), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Whether pairs of SMs are the shorter way: rounds of tiles times what a tile takes, in us.  Measured, a stage of 256 channels of a 128 x 128 tile 0.40, of a 256 x 192 tile of a
+// pair 0.45, taking a tile out 1.0 and 2.4 (4096 x 16384, both kernels: 4096 channels 179 / 134, 256 channels 29 / 45; 1024 x 8192 x 2048 15 / 13, 512 x 8192 x 2048 9 / 10).
+bool on_pairs(int M, int N, int K, int sms) {
+    const long long single = ((M + 127LL) / 128 * ((N + 127LL) / 128) + sms - 1) / sms, pairs = ((M + 255LL) / 256 * ((N + kPairN - 1LL) / kPairN) + sms / 2 - 1) / (sms / 2);
+    const double stages = (K + kStageK - 1) / kStageK;
+    return M > 128 && pairs * std::max(0.45 * stages, 2.4) + 1.0 < single * std::max(0.4 * stages, 1.0);
+}
+
+// clusters of two CTAs of the pair kernel that run at the same time
+template <int TYPE>
+cudaError_t pairs_of(int dev, int* out) {
+    static std::atomic<int> known[64];
+    if (dev >= 0 && dev < 64 && (*out = known[dev].load(std::memory_order_relaxed)) > 0) return cudaSuccess;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(2);
+    cfg.blockDim = dim3(kPairThreads);
+    cfg.dynamicSmemBytes = kPairSmem;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = 2;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    cudaError_t e = cudaFuncSetAttribute(mxfp4_pair_kernel<TYPE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem);
+    if (e == cudaSuccess) e = cudaOccupancyMaxActiveClusters(out, mxfp4_pair_kernel<TYPE>, &cfg);
+    if (e != cudaSuccess) return e;
+    if (*out < 1) return cudaErrorNotSupported;
+    if (dev >= 0 && dev < 64) known[dev].store(*out, std::memory_order_relaxed);
+    return cudaSuccess;
+}
+
 template <int TYPE>
 cudaError_t run_tiled(const Mxfp4Product& p, const uint8_t* a_codes, const uint8_t* a_scales, int dev, int sms, cudaStream_t st) {
     const cudaError_t e = ask_smem<mxfp4_product_kernel<TYPE>>(dev, kSmem4);
     if (e != cudaSuccess) return e;
-    CUtensorMap ma, mw;
-    if (!codes_map(&ma, a_codes, p.M, p.K, kBM) || !codes_map(&mw, p.w_codes, p.N, p.K, kBN)) return cudaErrorNotSupported;
     const TiledProduct q{a_scales, reinterpret_cast<const uint8_t*>(p.w_scales), p.y, p.M, p.N, p.K, p.ran_out, p.polls};
-    const long long n_tiles = (long long)((p.M + kBM - 1) / kBM) * ((p.N + kBN - 1) / kBN);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)std::min<long long>(n_tiles, sms));
-    cfg.blockDim = dim3(kThreads4);
-    cfg.dynamicSmemBytes = kSmem4;
     cfg.stream = st;
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
+    CUtensorMap ma, mw;
+    const bool pair = on_pairs(p.M, p.N, p.K, sms);
+    if (!codes_map(&ma, a_codes, p.M, p.K, kBM) || !codes_map(&mw, p.w_codes, p.N, p.K, pair ? kPairN / 2 : kBN)) return cudaErrorNotSupported;
+    if (pair) {
+        int pairs = 0;
+        CUtensorMap mas, mws;
+        const cudaError_t known = pairs_of<TYPE>(dev, &pairs);
+        if (known != cudaSuccess) return known;
+        if (!scales_map(&mas, a_scales, p.M, p.K) || !scales_map(&mws, p.w_scales, p.N, p.K)) return cudaErrorNotSupported;
+        const long long n_tiles = (long long)((p.M + 255) / 256) * ((p.N + kPairN - 1) / kPairN);
+        cfg.gridDim = dim3(2 * (unsigned)std::min<long long>(n_tiles, pairs));
+        cfg.blockDim = dim3(kPairThreads);
+        cfg.dynamicSmemBytes = kPairSmem;
+        return cudaLaunchKernelEx(&cfg, mxfp4_pair_kernel<TYPE>, ma, mw, mas, mws, q);
+    }
+    const long long n_tiles = (long long)((p.M + kBM - 1) / kBM) * ((p.N + kBN - 1) / kBN);
+    cfg.gridDim = dim3((unsigned)std::min<long long>(n_tiles, sms));
+    cfg.blockDim = dim3(kThreads4);
+    cfg.dynamicSmemBytes = kSmem4;
     return cudaLaunchKernelEx(&cfg, mxfp4_product_kernel<TYPE>, ma, mw, q);
 }
 
@@ -633,7 +912,7 @@ cudaError_t run_few(const Mxfp4Product& p, int S, int per, int slots, size_t sme
     const FewProduct q{p.a, p.lda, p.a_type, wide, reinterpret_cast<const uint8_t*>(p.w_scales), p.y, p.y_type, p.M, p.N, p.K, per, slots, p.ran_out, p.polls};
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((p.N + 127) / 128, S);
-    cfg.blockDim = dim3(kThreads4);
+    cfg.blockDim = dim3(kFewThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
