@@ -36,14 +36,20 @@ def _check_device(device: torch.device, *others: torch.Tensor) -> None:
         raise ValueError(f"operands must live on a CUDA device, not {device} (there is no CPU fallback)")
 
 
+@lru_cache(maxsize=None)
+def _function(what: str):
+    return getattr(_lm_lib.load(), "lm_b200_op_" + what)
+
+
 def _call(what: str, device: torch.device, *args) -> None:
     """The library's function ``lm_b200_op_<what>`` on the device's current stream, as its last argument."""
-    fn, stream = getattr(_lm_lib.load(), "lm_b200_op_" + what), torch._C._cuda_getCurrentRawStream(device.index)
-    if torch.cuda.current_device() == device.index:
-        rc = fn(*args, stream)
+    index = device.index
+    stream = torch._C._cuda_getCurrentRawStream(index)             # (an integer; a Stream object takes 2 us more)
+    if torch._C._cuda_getDevice() == index:
+        rc = _function(what)(*args, stream)
     else:
-        with torch.cuda.device(device.index):
-            rc = fn(*args, stream)
+        with torch.cuda.device(index):
+            rc = _function(what)(*args, stream)
     if rc:
         _lm_lib.check(rc, what)
 
@@ -153,7 +159,7 @@ def linear_mxfp4(a: torch.Tensor, w: Mxfp4, out_dtype: torch.dtype | None = None
         raise TypeError(f"out_dtype must be one of {_names(_TYPES)}, not {out_dtype}")
     _no_grad("linear_mxfp4", a)
     _check_device(device, w.data)
-    y = torch.empty((*a.shape[:-1], w.rows), dtype=out_dtype, device=device)
+    y = a.new_empty((*a.shape[:-1], w.rows), dtype=out_dtype)
     if not w.width:
         return y.zero_()
     if not y.numel():
@@ -161,7 +167,7 @@ def linear_mxfp4(a: torch.Tensor, w: Mxfp4, out_dtype: torch.dtype | None = None
     rows = _as_rows(a)
     M, at = rows.shape[0], w.data.data_ptr()
     need = _linear_work_bytes(M, w.rows, w.width)
-    work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    work = a.new_empty(need, dtype=torch.uint8) if need else None
     _call("linear_mxfp4", device, rows.data_ptr(), _TYPES[a.dtype], rows.stride(0), at, at + w.scales_at, y.data_ptr(), _TYPES[out_dtype], M,
           w.rows, w.width, work.data_ptr() if need else None, need)
     return y
@@ -190,11 +196,11 @@ def _losses(hidden, weight, targets, scale, ignore_index, reduction, keep):
     how many rows count)."""
     h, w, t = _as_rows(hidden), _as_rows(weight), targets.contiguous()
     (M, K), V, device = h.shape, w.shape[0], h.device
-    out = torch.empty(M if reduction == "none" else (), dtype=torch.float32, device=device)
-    kept = torch.empty(2 * M + 1, dtype=torch.float32, device=device) if keep else None
+    out = h.new_empty(M if reduction == "none" else (), dtype=torch.float32)
+    kept = h.new_empty(2 * M + 1, dtype=torch.float32) if keep else None
     h_at, w_at, h_type, ldh, ldw = h.data_ptr(), w.data_ptr(), _TYPES[h.dtype], h.stride(0), w.stride(0)
     need = _loss_work_bytes(h_at & 255, h_type, ldh, w_at & 255, ldw, M, V, K)
-    work = torch.empty(need, dtype=torch.uint8, device=device)
+    work = h.new_empty(need, dtype=torch.uint8)
     _call("loss", device, h_at, h_type, ldh, w_at, ldw, t.data_ptr(), t.dtype == torch.int64, ignore_index, M, V, K, scale,
           _REDUCTIONS[reduction], out.data_ptr(), kept.data_ptr() if keep else None, work.data_ptr(), need)
     return out, t, kept
@@ -217,14 +223,14 @@ class _LinearCrossEntropy(torch.autograd.Function):
         scale, ignore_index, mean = ctx.args
         need_h, need_w = ctx.needs_input_grad[:2]
         (M, K), V, device = hidden.shape, weight.shape[0], hidden.device
-        h, w, grad = _as_rows(hidden), _as_rows(weight), grad.to(torch.float32)
+        h, w = _as_rows(hidden), _as_rows(weight)
         if grad.dim() and grad.stride(0) < 0:
             grad = grad.contiguous()
-        dh = torch.empty((M, K), dtype=hidden.dtype, device=device) if need_h else None
-        dw = torch.empty((V, K), dtype=weight.dtype, device=device) if need_w else None
+        dh = hidden.new_empty((M, K)) if need_h else None
+        dw = weight.new_empty((V, K)) if need_w else None
         h_at, w_at, ldh, ldw = h.data_ptr(), w.data_ptr(), h.stride(0), w.stride(0)
         need = _loss_grad_work_bytes(h_at & 255, ldh, w_at & 255, ldw, M, V, K, need_h, need_w)
-        work = torch.empty(need, dtype=torch.uint8, device=device)
+        work = hidden.new_empty(need, dtype=torch.uint8)
         kept_at = kept.data_ptr()
         _call("loss_grad", device, h_at, ldh, w_at, ldw, t.data_ptr(), t.dtype == torch.int64, ignore_index, M, V, K, scale, kept_at,
               grad.data_ptr(), grad.stride(0) if grad.dim() else 0, kept_at + 8 * M if mean else None, dh.data_ptr() if need_h else None,
