@@ -456,6 +456,8 @@ mxfp4_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
 //   warp 0    one lane per CTA: codes and scales (TMA) of its halves; every byte of both CTAs counts on the leader's barrier
 //   warp 1    leader only: a stage's scales into the tensor memory of both, then the pair's MMAs; commits to the barriers of both
 //   warps 2-9 take the CTA's 128 rows of a finished accumulator out, half of the columns each
+// Bound: what the SMs take from L2, 11 TB/s (4096 x 16384 x 4096, us: 124; without MMAs 128 of then 132, without the copies of scales into tensor memory 131, without loading
+// scales 104 - two pieces of 512 bytes at a time they were three loads a stage, and 132 - without taking results out 127).
 constexpr int kPairN = 192, kPairStages = 6, kPairWarps = 8, kPairThreads = 64 + 32 * kPairWarps;
 constexpr int kPairCodes = kCodeTile + kPairN / 2 * 128, kPairStage = kPairCodes + 3 * 1024;
 constexpr int kPairSmem = kPairStages * kPairStage + kPairWarps * 4096 + 1024 + 256;
@@ -513,14 +515,13 @@ mxfp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                 const uint32_t bar = at_rank(&full[at], 0), dst = smem_u32(smem + at * kPairStage);
                 if (rank == 0) mbar_arrive_expect_tx(&full[at], 2u * kPairStage);
                 tma_load_2d_pair(dst + kCodeTile, &map_w, bar, s * (kStageK / 2), n0 + (int)rank * (kPairN / 2));
-                tma_load_2d_pair(dst + kPairCodes + 1024, &map_ws, bar, 0, n0 / 128 * pieces + 2 * s);
-                tma_load_2d_pair(dst + kPairCodes + 2048, &map_ws, bar, 0, (n0 / 128 + 1) * pieces + 2 * s);
+                tma_load_2d_pair(dst + kPairCodes + 1024, &map_ws, bar, s * (2 * kMxScaleBytes / 4), n0 / 128);
             };
             const auto rows = [&](unsigned at, int t, int s) {
                 const int m = t % tiles_m * 2 + (int)rank;
                 const uint32_t bar = at_rank(&full[at], 0), dst = smem_u32(smem + at * kPairStage);
                 tma_load_2d_pair(dst, &map_a, bar, s * (kStageK / 2), m * 128);
-                tma_load_2d_pair(dst + kPairCodes, &map_as, bar, 0, m * pieces + 2 * s);
+                tma_load_2d_pair(dst + kPairCodes, &map_as, bar, s * (2 * kMxScaleBytes / 4), m);
             };
             unsigned i = 0;
             int t = pair, s = 0;
@@ -806,12 +807,12 @@ bool codes_map(CUtensorMap* map, const void* codes, int rows, int K, int box_row
                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// scales, a row of 512 bytes per piece, two pieces at a time
-bool scales_map(CUtensorMap* map, const void* scales, int rows, int K) {
+// scales, a row of all pieces per block of 128 rows, two pieces of `blocks` of them at a time
+bool scales_map(CUtensorMap* map, const void* scales, int rows, int K, int blocks) {
     const EncodeTiledFn enc = encode_tiled();
     if (!enc) return false;
-    const cuuint64_t dims[2] = {kMxScaleBytes / 4, (cuuint64_t)(mx_scale_bytes(rows, K) / kMxScaleBytes)}, strides[1] = {kMxScaleBytes};
-    const cuuint32_t box[2] = {kMxScaleBytes / 4, 2}, estr[2] = {1, 1};
+    const cuuint64_t dims[2] = {(cuuint64_t)(mx_stride(K) / kMxStride * (kMxScaleBytes / 4)), (cuuint64_t)((rows + 127) / 128)}, strides[1] = {dims[0] * 4};
+    const cuuint32_t box[2] = {2 * kMxScaleBytes / 4, (cuuint32_t)blocks}, estr[2] = {1, 1};
     return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, const_cast<void*>(scales), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -867,7 +868,7 @@ cudaError_t run_tiled(const Mxfp4Product& p, const uint8_t* a_codes, const uint8
         CUtensorMap mas, mws;
         const cudaError_t known = pairs_of<TYPE>(dev, &pairs);
         if (known != cudaSuccess) return known;
-        if (!scales_map(&mas, a_scales, p.M, p.K) || !scales_map(&mws, p.w_scales, p.N, p.K)) return cudaErrorNotSupported;
+        if (!scales_map(&mas, a_scales, p.M, p.K, 1) || !scales_map(&mws, p.w_scales, p.N, p.K, 2)) return cudaErrorNotSupported;
         const long long n_tiles = (long long)((p.M + 255) / 256) * ((p.N + kPairN - 1) / kPairN);
         cfg.gridDim = dim3(2 * (unsigned)std::min<long long>(n_tiles, pairs));
         cfg.blockDim = dim3(kPairThreads);
