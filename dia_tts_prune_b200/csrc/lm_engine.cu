@@ -132,10 +132,11 @@ inline int cuda_fail(cudaError_t e) {
 inline cudaStream_t S(void* s) { return reinterpret_cast<cudaStream_t>(s); }
 
 constexpr int kMostChannels = 1 << 24;           // of a row that an operator takes (offsets inside a row stay in 32 bits)
+constexpr int kMostRows = 0x7fffffff - 256;      // (tiles of up to 256 are counted in 32 bits)
 inline bool known_type(int t) { return t == LM_B200_FP32 || t == LM_B200_BF16 || t == LM_B200_FP16; }
 inline bool loss_shape(lm::LossShape& s, const void* h, int h_type, int64_t ldh, const void* W, int64_t ldw, int M, int V, int K) {
-    constexpr int most = 0x7fffffff - 256;       // (tiles of 256 are counted in 32 bits)
-    if (!h || !W || M <= 0 || M > most || V <= 0 || V > most || K <= 0 || K > kMostChannels || (M > 1 && ldh < K) || (V > 1 && ldw < K) ||
+    const int most = h_type == LM_B200_FP32 ? kMostRows / 3 : kMostRows;         // (fp32 rows are three of bf16)
+    if (!h || !W || M <= 0 || M > most || V <= 0 || V > kMostRows || K <= 0 || K > kMostChannels || (M > 1 && ldh < K) || (V > 1 && ldw < K) ||
         (h_type != LM_B200_FP32 && h_type != LM_B200_BF16))
         return false;
     s = lm::LossShape{h, h_type, M > 1 ? ldh : K, W, V > 1 ? ldw : K, nullptr, 0, 0, M, V, K, 1.f};
@@ -1751,23 +1752,23 @@ size_t lm_b200_mxfp4_code_bytes(int rows, int K) { return rows > 0 && K > 0 ? lm
 size_t lm_b200_mxfp4_scale_bytes(int rows, int K) { return rows > 0 && K > 0 ? lm::mx_scale_bytes(rows, K) : 0; }
 
 int lm_b200_op_mxfp4_quantize(const void* x, int type, int64_t ld, int rows, int K, void* codes, void* scales, void* stream) {
-    if (!x || !codes || !scales || rows <= 0 || K <= 0 || K > kMostChannels || (rows > 1 && ld < K) || !known_type(type) || !aligned(codes, 16) || !aligned(scales, 16))
+    if (!x || !codes || !scales || rows <= 0 || rows > kMostRows || K <= 0 || K > kMostChannels || (rows > 1 && ld < K) || !known_type(type) || !aligned(codes, 16) || !aligned(scales, 16))
         return LM_B200_EINVAL;
     LCK(lm::launch_mxfp4_quantize(x, type, rows > 1 ? ld : K, rows, K, codes, scales, S(stream)));
     return LM_B200_OK;
 }
 
 int lm_b200_op_mxfp4_dequantize(const void* codes, const void* scales, int rows, int K, void* out, int type, void* stream) {
-    if (!codes || !scales || !out || rows <= 0 || K <= 0 || K > kMostChannels || !known_type(type) || !aligned(codes, 16) || !aligned(scales, 16)) return LM_B200_EINVAL;
+    if (!codes || !scales || !out || rows <= 0 || rows > kMostRows || K <= 0 || K > kMostChannels || !known_type(type) || !aligned(codes, 16) || !aligned(scales, 16)) return LM_B200_EINVAL;
     LCK(lm::launch_mxfp4_dequantize(codes, scales, rows, K, out, type, S(stream)));
     return LM_B200_OK;
 }
 
-size_t lm_b200_op_linear_mxfp4_work_bytes(int M, int N, int K) { return M > 0 && N > 0 && K > 0 ? lm::mxfp4_linear_work_bytes(M, N, K) : 0; }
+size_t lm_b200_op_linear_mxfp4_work_bytes(int M, int N, int K) { return M > 0 && M <= kMostRows && N > 0 && N <= kMostRows && K > 0 ? lm::mxfp4_linear_work_bytes(M, N, K) : 0; }
 
 int lm_b200_op_linear_mxfp4(const void* A, int a_type, int64_t lda, const void* w_codes, const void* w_scales, void* Y, int y_type, int M, int N, int K, void* work,
                             size_t work_bytes, void* stream) {
-    if (!A || !w_codes || !w_scales || !Y || M <= 0 || N <= 0 || K <= 0 || K > kMostChannels || (M > 1 && lda < K) || !known_type(a_type) || !known_type(y_type) ||
+    if (!A || !w_codes || !w_scales || !Y || M <= 0 || M > kMostRows || N <= 0 || N > kMostRows || K <= 0 || K > kMostChannels || (M > 1 && lda < K) || !known_type(a_type) || !known_type(y_type) ||
         !aligned(w_codes, 16) || !aligned(w_scales, 16) || !aligned(work, 128) || work_bytes < lm_b200_op_linear_mxfp4_work_bytes(M, N, K) || (work_bytes && !work))
         return LM_B200_EINVAL;
     LCK(lm::launch_mxfp4_linear(lm::Mxfp4Product{A, a_type, M > 1 ? lda : K, w_codes, w_scales, Y, y_type, M, N, K, nullptr, 0}, work, S(stream)));

@@ -206,7 +206,7 @@ constexpr int kBM = 128, kBN = 128, kStageK = 256;            // rows of A and o
 constexpr int kCodeTile = 128 * 128;                          // 128 rows x 256 channels, 16 KB
 constexpr int kStageBytes = 2 * kCodeTile + 2 * 1024;         // A, W, their scales
 constexpr int kStages = 5;
-constexpr int kFewThreads = 192, kWarps4 = 8, kThreads4 = 64 + 32 * kWarps4;
+constexpr int kFewThreads = 320, kWarps4 = 8, kThreads4 = 64 + 32 * kWarps4;
 constexpr int kTurnBytes = kWarps4 * 4096;
 constexpr int kSmem4 = kStages * kStageBytes + kTurnBytes + 1024 + 256;
 
@@ -644,7 +644,7 @@ __device__ __forceinline__ void put1(void* y, int type, size_t at, float v) {
     else reinterpret_cast<__half*>(y)[at] = __float2half_rn(v);
 }
 
-__global__ void __launch_bounds__(kFewThreads, 1) mxfp4_few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ FewProduct p) {
+__global__ void __launch_bounds__(kFewThreads, 2) mxfp4_few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ FewProduct p) {
     constexpr int kSlot = kCodeTile + 1024, kRows = NB * 128 + 1024;       // a stage of weights, of rows
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -677,7 +677,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) mxfp4_few_rows_kernel(const __
     const int per_row = stages * 32, items = M * per_row;
     const auto place = [&](int m, int c) { return rows + (c >> 5) * kRows + (m >> 3) * 1024 + (m & 7) * 128 + ((((c & 31) >> 2) ^ (m & 7)) << 4) + (c & 3) * 4; };
     const auto take = [&](auto type, auto wide) {
-        constexpr int TYPE = decltype(type)::value, kBatch = TYPE == kTypeF32 ? 4 : 8;
+        constexpr int TYPE = decltype(type)::value, kBatch = TYPE == kTypeF32 ? 6 : 8;
         constexpr bool WIDE = decltype(wide)::value;
         for (int i0 = tid; i0 < items; i0 += kFewThreads * kBatch) {           // (a warp is in or out as a whole)
             Eight<TYPE, WIDE> x8[kBatch];
@@ -705,11 +705,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) mxfp4_few_rows_kernel(const __
     if (p.a_type == kTypeF32) take_type(std::integral_constant<int, kTypeF32>());
     else if (p.a_type == kTypeBf16) take_type(std::integral_constant<int, kTypeBf16>());
     else take_type(std::integral_constant<int, kTypeF16>());
-    for (int i = tid; i < (NB - M) * per_row; i += kFewThreads) {               // columns that no row uses
-        const int m = M + i / per_row, c = i % per_row;
-        *reinterpret_cast<uint32_t*>(place(m, c)) = 0u;
-        if ((c & 3) == 0) rows[(c >> 5) * kRows + NB * 128 + ((c & 31) >> 4) * kMxScaleBytes + (m & 31) * 16 + (m >> 5) * 4 + ((c >> 2) & 3)] = 0;
-    }
+    // (columns beyond M multiply whatever is there and go nowhere: numbers of 4 bits are all finite, a scale that is not stays in its column)
     fence_proxy_async();
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
@@ -751,7 +747,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) mxfp4_few_rows_kernel(const __
             }
             __syncwarp();
         }
-    } else {
+    } else if (warp < 6) {
         ok = stages == 0 || pair_wait(&t_full, 0, p.polls);   // (the last CTAs of a cluster may have none: zeros)
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const int c = (warp & 3) * 32 + lane;

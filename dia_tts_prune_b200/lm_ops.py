@@ -76,7 +76,7 @@ def _as_rows(x: torch.Tensor) -> torch.Tensor:
     if x.dim() != 2:
         x = x.reshape(-1, x.shape[-1])
     rows, width = x.shape
-    if rows > 0x7fffff00 or width > 1 << 24:
+    if rows > 0x7fffff00 // 3 or width > 1 << 24:
         raise ValueError(f"{rows} rows of {width} channels are more than an operator takes")
     apart, step = x.stride()
     # (overlapping or backward rows are copied; a row stride is only read where there are several rows)
@@ -253,13 +253,15 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
     scale, ignore_index = float(scale), int(ignore_index)
     if not 0.0 < scale < float("inf"):
         raise ValueError("scale must be positive and finite")
+    if not -1 << 63 <= ignore_index < 1 << 63:
+        raise ValueError("ignore_index must fit 64 bits")
     with_grad = (hidden.requires_grad or weight.requires_grad) and torch.is_grad_enabled()
     if with_grad and hidden.dtype != torch.bfloat16:
         raise ValueError("gradients need hidden in bfloat16")
     _check_device(hidden.device, weight, targets)
-    if not targets.numel():
-        rows = hidden.new_zeros(targets.shape, dtype=torch.float32)
-        return rows if reduction == "none" else rows.sum()
+    if not targets.numel():                                       # (still a function of both, whose gradients are zeros)
+        rows = hidden.float().sum(-1)
+        return rows if reduction == "none" else rows.sum() + weight[:0].float().sum()
     rows = hidden if hidden.dim() == 2 else hidden.reshape(-1, hidden.shape[-1])
     flat = targets if targets.dim() == 1 else targets.reshape(-1)
     if with_grad:

@@ -57,7 +57,7 @@ def test_losses_that_are_refused():
     for a in ((h[:, :31], w, t), (h, w[0], t), (h, w, t[:5]), (h, w, t[:, None]), (h, w[:0], t)):
         with pytest.raises(ValueError):
             f(*a)
-    for k in (dict(reduction="max"), dict(scale=0.0), dict(scale=-1.0), dict(scale=math.inf), dict(scale=math.nan)):
+    for k in (dict(reduction="max"), dict(scale=0.0), dict(scale=-1.0), dict(scale=math.inf), dict(scale=math.nan), dict(ignore_index=1 << 63)):
         with pytest.raises(ValueError):
             f(h, w, t, **k)
     for a in ((h.float().requires_grad_(True), w, t), (h.float(), w.clone().requires_grad_(True), t)):
@@ -76,7 +76,8 @@ def test_c_entries_answer_bad_arguments():
     at, odd = 1 << 20, (1 << 20) + 8                               # (addresses that are never followed)
     q = lib.lm_b200_op_mxfp4_quantize
     for a in ((None, 0, 64, 4, 64, at, at), (at, 3, 64, 4, 64, at, at), (at, 0, 63, 4, 64, at, at), (at, 0, 64, 0, 64, at, at), (at, 0, 64, 4, 0, at, at),
-              (at, 0, 64, 4, 64, odd, at), (at, 0, 64, 4, 64, at, None), (at, 0, 1 << 30, 4, 1 << 25, at, at)):
+              (at, 0, 64, 4, 64, odd, at), (at, 0, 64, 4, 64, at, None), (at, 0, 1 << 30, 4, 1 << 25, at, at),
+              (at, 0, 64, 0x7fffffff, 64, at, at)):
         assert q(*a, None) == _lm_lib.E_INVAL
     for a in ((at, at, 0, 64, at, 0), (at, at, 4, 64, None, 0), (at, at, 4, 64, at, 7), (odd, at, 4, 64, at, 0)):
         assert lib.lm_b200_op_mxfp4_dequantize(*a, None) == _lm_lib.E_INVAL

@@ -196,3 +196,36 @@ def test_strides_leading_dimensions_and_empty():
     assert torch.equal(linear_cross_entropy(h[0], w, t[0], reduction="none"), want[0])
     assert linear_cross_entropy(h[:0], w, t[:0], reduction="none").shape == (0,)
     assert linear_cross_entropy(h[:0], w, t[:0]) == 0
+    a, b = h[:0].clone().requires_grad_(True), w.clone().requires_grad_(True)
+    loss = linear_cross_entropy(a, b, t[:0])
+    loss.backward()
+    assert loss == 0 and a.grad.shape == (0, 104) and not b.grad.any()
+
+
+@pytest.mark.parametrize("m,v,k", [(1, 40, 7), (33, 300, 100), (129, 257, 65), (300, 1025, 264)])
+def test_nothing_is_written_beside_the_results(m, v, k):
+    """Every output inside a larger buffer whose other bytes stay: losses, what the gradient needs, both gradients, the workspace."""
+    from dia_tts_prune_b200 import _lm_lib
+    lib, st = _lm_lib.load(), torch.cuda.current_stream().cuda_stream
+    h, w, t = operands(m, v, k, 3)
+
+    def room(nbytes, align=256):
+        buf = torch.full((nbytes + 4 * align,), 77, dtype=torch.uint8, device="cuda")
+        at = (buf.data_ptr() + 2 * align - 1) // align * align
+        return buf, at, at - buf.data_ptr(), nbytes
+
+    def kept(r):
+        buf, _, at, n = r
+        return bool((buf[:at] == 77).all() and (buf[at + n:] == 77).all())
+
+    each, one, keep, dh, dw = room(4 * m), room(4), room(8 * m + 4), room(2 * m * k), room(2 * v * k)
+    need = lib.lm_b200_op_loss_work_bytes(h.data_ptr(), 1, k, w.data_ptr(), k, m, v, k)
+    work = room(need)
+    for reduction, out in ((0, each), (2, one)):
+        assert lib.lm_b200_op_loss(h.data_ptr(), 1, k, w.data_ptr(), k, t.data_ptr(), 1, -100, m, v, k, 1.0, reduction, out[1], keep[1], work[1], need, st) == 0
+    need = lib.lm_b200_op_loss_grad_work_bytes(h.data_ptr(), k, w.data_ptr(), k, m, v, k, 1, 1)
+    work2, g = room(need), torch.ones((), device="cuda")
+    assert lib.lm_b200_op_loss_grad(h.data_ptr(), k, w.data_ptr(), k, t.data_ptr(), 1, -100, m, v, k, 1.0, keep[1], g.data_ptr(), 0, keep[1] + 8 * m, dh[1], dw[1],
+                                    work2[1], need, st) == 0
+    torch.cuda.synchronize()
+    assert all(kept(r) for r in (each, one, keep, dh, dw, work, work2))

@@ -73,6 +73,10 @@ def test_blocks_that_are_not_finite_stand_for_nan_alone():
     w = rows_of(64, 160, 4)
     y = lm_ops.linear_mxfp4(x, lm_ops.quantize_mxfp4(w)).cpu()
     assert y[[0, 1, 7, 129]].isnan().all() and y.isnan().sum() == 4 * 64
+    few = lm_ops.linear_mxfp4(x[:8], lm_ops.quantize_mxfp4(w)).cpu()         # (rows that are rounded inside the product)
+    assert few[[0, 1, 7]].isnan().all() and few.isnan().sum() == 3 * 64
+    few = lm_ops.linear_mxfp4(w[:3], lm_ops.quantize_mxfp4(x)).cpu()
+    assert few[:, [0, 1, 7, 129]].isnan().all() and few.isnan().sum() == 4 * 3
     y = lm_ops.linear_mxfp4(w, lm_ops.quantize_mxfp4(x)).cpu()
     assert y[:, [0, 1, 7, 129]].isnan().all() and y.isnan().sum() == 4 * 64
 
@@ -138,3 +142,34 @@ def test_many_tiles_on_every_sm_and_leading_dimensions():
     check(x, w, y.view(1030, 8200))
     assert lm_ops.linear_mxfp4(x[0], q).shape == (8200,)
     assert lm_ops.linear_mxfp4(x[:3], q, out_dtype=torch.float32).dtype == torch.float32
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("m,n,k,shift", [(1, 130, 40, 0), (5, 2047, 300, 1), (16, 64, 8200, 0), (40, 129, 130, 1), (200, 1001, 72, 0), (200, 1001, 72, 3), (513, 12290, 700, 1)])
+def test_nothing_is_written_beside_the_results(m, n, k, shift, dtype):
+    """Results, values and the 4-bit buffers inside larger ones whose other bytes stay; results may begin at any element."""
+    from dia_tts_prune_b200 import _lm_lib, lm_ops
+    lib, st = _lm_lib.load(), torch.cuda.current_stream().cuda_stream
+    x, w = rows_of(m, k, m, dtype), rows_of(n, k, n)
+    q, size, code = lm_ops.quantize_mxfp4(w), dtype.itemsize, 0 if dtype == torch.float32 else 1
+
+    def room(nbytes, off=0):
+        buf = torch.full((nbytes + 1024,), 77, dtype=torch.uint8, device="cuda")
+        at = (buf.data_ptr() + 511) // 256 * 256 + off
+        return buf, at, at - buf.data_ptr(), nbytes
+
+    def kept(r):
+        buf, _, at, nb = r
+        return bool((buf[:at] == 77).all() and (buf[at + nb:] == 77).all())
+
+    y, v, need = room(m * n * size, shift * size), room(m * k * size, shift * size), lib.lm_b200_op_linear_mxfp4_work_bytes(m, n, k)
+    work, codes, scales = room(need), room(lib.lm_b200_mxfp4_code_bytes(m, k)), room(lib.lm_b200_mxfp4_scale_bytes(m, k))
+    at = q.data.data_ptr()
+    assert lib.lm_b200_op_linear_mxfp4(x.data_ptr(), code, k, at, at + q.scales_at, y[1], code, m, n, k, work[1] if need else None, need, st) == 0
+    assert lib.lm_b200_op_mxfp4_quantize(x.data_ptr(), code, k, m, k, codes[1], scales[1], st) == 0
+    assert lib.lm_b200_op_mxfp4_dequantize(codes[1], scales[1], m, k, v[1], code, st) == 0
+    torch.cuda.synchronize()
+    assert all(kept(r) for r in (y, v, work, codes, scales))
+    got = y[0][y[2]:y[2] + y[3]].clone().view(dtype).view(m, n)
+    assert torch.equal(got, lm_ops.linear_mxfp4(x, q))
+    assert torch.equal(v[0][v[2]:v[2] + v[3]].clone().view(dtype).view(m, k), lm_ops.quantize_mxfp4(x).dequantize(dtype))
