@@ -555,28 +555,39 @@ __global__ void __launch_bounds__(kFewThreads, 2) loss_few_rows_kernel(const __g
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&t_empty[it & 1u]);
             }
+            // (rows eight at a time, side by side: one after the other each took 0.2 us a tile and as much again at the end)
 #pragma unroll
-            for (int m = 0; m < NB; ++m) {
-                if (m >= M) break;
-                if (targets[m] == n) p.hit[m] = ok ? z[m] : CUDART_NAN_F;
-                const float x = n < p.own.N ? z[m] * p.c : -CUDART_INF_F, now = fmaxf(most[m], x);
-                if (now > -CUDART_INF_F) sum[m] = sum[m] * exp2_fast(most[m] - now) + exp2_fast(n < p.own.N ? fmaf(z[m], p.c, -now) : -CUDART_INF_F);
-                else sum[m] += x != x ? x : 0.f;
-                most[m] = now;
+            for (int m0 = 0; m0 < NB; m0 += 8) {
+                if (m0 >= M) break;
+#pragma unroll
+                for (int m = m0; m < m0 + 8; ++m) {
+                    if (targets[m] == n) p.hit[m] = ok ? z[m] : CUDART_NAN_F;
+                    const float now = fmaxf(most[m], n < p.own.N ? z[m] * p.c : -CUDART_INF_F), below = now == -CUDART_INF_F ? 0.f : now;
+                    sum[m] = sum[m] * exp2_fast(most[m] - below) + exp2_fast(n < p.own.N ? fmaf(z[m], p.c, -below) : -CUDART_INF_F);
+                    most[m] = now;
+                }
             }
         }
 #pragma unroll
-        for (int m = 0; m < NB; ++m) {
-            if (m >= M) break;
-            if (!ok) most[m] = sum[m] = CUDART_NAN_F;
+        for (int m0 = 0; m0 < NB; m0 += 8) {
+            if (m0 >= M) break;
+            float top[8];
 #pragma unroll
-            for (int o = 16; o; o >>= 1) {
-                const float other = __shfl_xor_sync(0xffffffffu, most[m], o), add = __shfl_xor_sync(0xffffffffu, sum[m], o), now = fmaxf(most[m], other);
-                if (now > -CUDART_INF_F) sum[m] = sum[m] * exp2_fast(most[m] - now) + add * exp2_fast(other - now);
-                else sum[m] += add;
-                most[m] = now;
+            for (int m = 0; m < 8; ++m) top[m] = most[m0 + m];
+#pragma unroll
+            for (int o = 16; o; o >>= 1)
+#pragma unroll
+                for (int m = 0; m < 8; ++m) top[m] = fmaxf(top[m], __shfl_xor_sync(0xffffffffu, top[m], o));
+#pragma unroll
+            for (int m = 0; m < 8; ++m) sum[m0 + m] *= exp2_fast(most[m0 + m] - (top[m] == -CUDART_INF_F ? 0.f : top[m]));
+#pragma unroll
+            for (int o = 16; o; o >>= 1)
+#pragma unroll
+                for (int m = 0; m < 8; ++m) sum[m0 + m] += __shfl_xor_sync(0xffffffffu, sum[m0 + m], o);
+            if (lane == 0) {
+#pragma unroll
+                for (int m = 0; m < 8; ++m) meet[q][m0 + m] = ok ? make_float2(top[m], sum[m0 + m]) : make_float2(CUDART_NAN_F, CUDART_NAN_F);
             }
-            if (lane == 0) meet[q][m] = make_float2(most[m], sum[m]);
         }
     }
     if (!ok && lane == 0 && p.ran_out) {
