@@ -9,7 +9,7 @@
 // (8192 rows: 1.7e-3 to 1.9e-3 of the gradients' norm, of which the results' own rounding is 1.66e-3; with g inside 3.0e-3).  One g for all rows multiplies the sums; rows with
 // their own take it into h for dw (rounded to bf16) and behind the sums for dh.
 //
-// All four are one kernel on pairs of SMs: a cluster of two CTAs owns a 256 x 256 tile, tcgen05.mma (cta_group::2) multiplies the 256 rows of both by the 256 columns of
+// All of them are one kernel on pairs of SMs: a cluster of two CTAs owns a 256 x 256 tile, tcgen05.mma (cta_group::2) multiplies the 256 rows of both by the 256 columns of
 // both, and the accumulators (two per CTA: a tile is taken out while the next is multiplied) live in tensor memory.
 //   warp 0    one lane per CTA: TMA loads of its halves into a ring of stages; every byte of both CTAs counts on the leader's barrier
 //   warp 1    leader only: one elected lane issues the pair's MMAs, commits to the barriers of both CTAs
@@ -38,9 +38,10 @@ constexpr int kTileN = 256, kBK = 64, kTileBytes = 128 * kBK * 2;          // 16
 constexpr int kWarps = 8, kThreads = 64 + 32 * kWarps, kStagesMost = 6, kTurn = kWarps * 4096;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
-template <int TERMS>
+// (PAIR: see loss_product_kernel)
+template <int TERMS, bool PAIR>
 struct Ring {
-    static constexpr int kStage = (TERMS + 1) * kTileBytes, kStages = TERMS == 1 ? 6 : 3;
+    static constexpr int kStage = (TERMS + (PAIR ? 1 : 2)) * kTileBytes, kStages = TERMS == 1 ? (PAIR ? 6 : 4) : PAIR ? 3 : 2;
     static constexpr int kChunk = TERMS == 1 ? 16 : 8;       // kStats: k-blocks of an accumulator
     static constexpr int kSmem = kStages * kStage + kTurn + 1024 + 256;
 };
@@ -48,8 +49,9 @@ struct Ring {
 // Tiles of one product, and what they are made of (kGrads has two products)
 struct Tiles {
     int M, N, K;                     // rows and columns of the product, length of the contraction
+    int rows;                        // of a tile: 256, or 128 on one SM
     int splits;                      // pairs that share the contraction of a tile
-    __host__ __device__ int tiles_m() const { return (M + 255) / 256; }
+    __host__ __device__ int tiles_m() const { return (M + rows - 1) / rows; }
     __host__ __device__ int tiles_n() const { return (N + kTileN - 1) / kTileN; }
     __host__ __device__ long long tiles() const { return N > 0 ? (long long)tiles_m() * tiles_n() * splits : 0; }
     __host__ __device__ int blocks() const { return (K + kBK - 1) / kBK; }
@@ -152,12 +154,15 @@ __device__ __forceinline__ bool tile_of(const LossTiles& p, int pair, int pairs,
     return true;
 }
 
-template <int KIND, int TERMS>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+// PAIR false: one SM per 128 x 256 tile, for 128 rows and less, half of whose pair would multiply nothing (losses of 64 rows x 32768 x 2048, us, pairs / one SM: bf16
+// 37 / 32, fp32 rows 72 / 47; 131072 x 4096 bf16 233 / 199).
+template <int KIND, int TERMS, bool PAIR = true>
+__global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(kThreads, 1)
 loss_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_ha,
                     const __grid_constant__ CUtensorMap map_hb, const __grid_constant__ LossTiles p) {
     constexpr bool kStats_ = KIND == kStats;
-    constexpr int kStage = Ring<TERMS>::kStage, kStages = Ring<TERMS>::kStages, kChunk = Ring<TERMS>::kChunk;
+    constexpr int kStage = Ring<TERMS, PAIR>::kStage, kStages = Ring<TERMS, PAIR>::kStages, kChunk = Ring<TERMS, PAIR>::kChunk;
+    static_assert(PAIR || KIND != kGrads, "both gradients go on pairs");
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     unsigned char* turn = smem + kStages * kStage;
@@ -168,20 +173,29 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(t_empty + 2);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t rank = blockIdx.x & 1;
-    const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+    const uint32_t rank = PAIR ? blockIdx.x & 1 : 0;
+    const int pair = PAIR ? blockIdx.x >> 1 : blockIdx.x, pairs = PAIR ? gridDim.x >> 1 : gridDim.x;
+    const auto everyone = [] {
+        if constexpr (PAIR) cluster_sync_all();
+        else __syncthreads();
+    };
     if (KIND == kStats && blockIdx.x == 0 && threadIdx.x == 0) *p.arrived = 0u;
     if (threadIdx.x == 0) {
         for (int i = 0; i < kStages; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
-        for (int i = 0; i < 2; ++i) { mbar_init(&t_full[i], 1); mbar_init(&t_empty[i], 2 * kWarps); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&t_full[i], 1); mbar_init(&t_empty[i], (PAIR ? 2 : 1) * kWarps); }
         fence_mbar_init();
     }
     if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512));
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::);
+        if constexpr (PAIR) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512));
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::);
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512));
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+        }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-    cluster_sync_all();
+    everyone();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem_base = *tmem_slot;
     if (KIND == kStats) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -191,11 +205,11 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
             unsigned i = 0;
             Tile t;
             for (int n = 0; ok && tile_of(p, pair, pairs, n, t); ++n) {
-                const int a0 = t.m * 256 + (int)rank * 128, b0 = t.n * kTileN + (int)rank * 128;
+                const int a0 = t.m * (PAIR ? 256 : 128) + (int)rank * 128, b0 = t.n * kTileN + (int)rank * 128;
                 for (int kb = t.kb0; kb < t.kb1; ++kb, ++i) {
                     const unsigned s = i % kStages;
                     if (!lane_wait(&empty[s], ((i / kStages) & 1u) ^ 1u, p.polls)) { ok = false; break; }
-                    if (rank == 0) mbar_arrive_expect_tx(&full[s], 2u * kStage);
+                    if (rank == 0) mbar_arrive_expect_tx(&full[s], (PAIR ? 2u : 1u) * kStage);
                     const uint32_t bar = at_rank(&full[s], 0), dst = smem_u32(smem + s * kStage), k = kb * kBK;
                     if constexpr (KIND == kGrads) {
                         if (t.head) {
@@ -208,6 +222,11 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                             tma_load_2d_pair(dst + kTileBytes, &map_b, bar, b0, p.v0 + k);
                             tma_load_2d_pair(dst + kTileBytes + kTileBytes / 2, &map_b, bar, b0 + 64, p.v0 + k);
                         }
+                    } else if constexpr (!PAIR) {
+                        tma_load_2d(dst + TERMS * kTileBytes, &map_b, bar, k, p.v0 + b0);
+                        tma_load_2d(dst + (TERMS + 1) * kTileBytes, &map_b, bar, k, p.v0 + b0 + 128);
+#pragma unroll
+                        for (int tm = 0; tm < TERMS; ++tm) tma_load_2d(dst + tm * kTileBytes, &map_a, bar, k, tm * p.own.M + a0);
                     } else {
                         tma_load_2d_pair(dst + TERMS * kTileBytes, &map_b, bar, k, p.v0 + b0);
 #pragma unroll
@@ -226,8 +245,8 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
             Tile t;
             for (int n = 0; ok && tile_of(p, pair, pairs, n, t); ++n) {
                 const bool a_mn = KIND == kGrads && t.head, b_mn = KIND == kGrads;
-                // fp32 accumulators, bf16 operands, which of them are MN-major, N = 256, M = 256
-                const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(kTileN >> 3) << 17) | (16u << 24);
+                // fp32 accumulators, bf16 operands, which of them are MN-major, N = 256, M = 256 or 128
+                const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(kTileN >> 3) << 17) | ((PAIR ? 16u : 8u) << 24);
                 const uint32_t a_step = a_mn ? 2048 >> 4 : 2, b_step = b_mn ? 2048 >> 4 : 2;        // 16 of the contraction, in descriptor units
                 for (int kb = t.kb0; kb < t.kb1; ++kb, ++i) {
                     const bool first = kStats_ ? kb % kChunk == 0 : kb == t.kb0, last = kb == t.kb1 - 1 || (kStats_ && kb % kChunk == kChunk - 1);
@@ -247,11 +266,19 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                             const uint32_t a_at = at + (TERMS - 1 - u) * kTileBytes;                 // the smallest term first
                             const uint64_t adesc = a_mn ? umma_desc_mn(a_at) : umma_desc(a_at);
 #pragma unroll
-                            for (int j = 0; j < kBK / 16; ++j)
-                                umma_bf16_pair(d, adesc + a_step * j, bdesc + b_step * j, idesc, (u | j) != 0 || !first ? 1u : 0u);
+                            for (int j = 0; j < kBK / 16; ++j) {
+                                const uint32_t more = (u | j) != 0 || !first ? 1u : 0u;
+                                if constexpr (PAIR) umma_bf16_pair(d, adesc + a_step * j, bdesc + b_step * j, idesc, more);
+                                else umma_bf16(d, adesc + a_step * j, bdesc + b_step * j, idesc, more);
+                            }
                         }
-                        umma_commit_pair(&empty[s]);
-                        if (last) umma_commit_pair(&t_full[it & 1u]);
+                        if constexpr (PAIR) {
+                            umma_commit_pair(&empty[s]);
+                            if (last) umma_commit_pair(&t_full[it & 1u]);
+                        } else {
+                            umma_commit(&empty[s]);
+                            if (last) umma_commit(&t_full[it & 1u]);
+                        }
                     }
                     __syncwarp();
                     if (last) ++it;
@@ -276,7 +303,7 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
         Tile t;
         for (int tile = 0; tile_of(p, pair, pairs, tile, t); ++tile) {
             const Tiles& of = KIND == kGrads && t.head ? p.head : p.own;
-            const int n0 = t.n * kTileN + c_half, row0 = t.m * 256 + (int)rank * 128 + q * 32, rows = min(32, of.M - row0), row = row0 + lane;
+            const int n0 = t.n * kTileN + c_half, row0 = t.m * (PAIR ? 256 : 128) + (int)rank * 128 + q * 32, rows = min(32, of.M - row0), row = row0 + lane;
             const bool mine = row < of.M;
             const auto from = [&]() { return tmem_base + ((uint32_t)(q * 32) << 16) + (it & 1u) * kTileN + c_half; };
             const auto wait = [&]() {
@@ -419,10 +446,11 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
     }
     __syncwarp();
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-    cluster_sync_all();                                       // neither CTA's memory goes while the other still reads it or arrives there
+    everyone();                                               // neither CTA's memory goes while the other still reads it or arrives there
     if (warp == 1) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512));
+        if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512));
+        else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512));
     }
 }
 
@@ -752,14 +780,14 @@ cudaError_t pairs_of(int dev, int* out) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(2);
     cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = Ring<TERMS>::kSmem;
+    cfg.dynamicSmemBytes = Ring<TERMS, true>::kSmem;
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeClusterDimension;
     attr.val.clusterDim.x = 2;
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Ring<TERMS>::kSmem);
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Ring<TERMS, true>::kSmem);
     if (e == cudaSuccess) e = cudaOccupancyMaxActiveClusters(out, kernel, &cfg);
     if (e != cudaSuccess) return e;
     if (*out < 1) return cudaErrorNotSupported;
@@ -767,21 +795,34 @@ cudaError_t pairs_of(int dev, int* out) {
     return cudaSuccess;
 }
 
-// (hs, ht: the operands of dw in kGrads)
+// (hs, ht: the operands of dw in kGrads).  128 rows and less of logits go on one SM per tile
 template <int KIND, int TERMS>
 cudaError_t run_tiles(const CUtensorMap& a, const CUtensorMap& b, LossTiles p, int dev, cudaStream_t st, const CUtensorMap* hs = nullptr, const CUtensorMap* ht = nullptr) {
+    p.polls = gemm_pair_polls();
+    p.ran_out = split_attention_ran_out(dev, st);
+    p.own.rows = p.head.rows = 256;
+    if constexpr (KIND != kGrads) {
+        if (p.own.M <= 128) {
+            int sms = 0;
+            cudaError_t e = current_sms(&dev, &sms);
+            if (e == cudaSuccess) e = ask_smem<loss_product_kernel<KIND, TERMS, false>>(dev, Ring<TERMS, false>::kSmem);
+            if (e != cudaSuccess) return e;
+            p.own.rows = 128;
+            p.many = p.own.tiles_n();
+            loss_product_kernel<KIND, TERMS, false><<<std::min(p.many, sms), kThreads, Ring<TERMS, false>::kSmem, st>>>(a, b, a, b, p);
+            return cudaGetLastError();
+        }
+    }
     int pairs = 0;
     const cudaError_t e = pairs_of<KIND, TERMS>(dev, &pairs);
     if (e != cudaSuccess) return e;
-    p.polls = gemm_pair_polls();
-    p.ran_out = split_attention_ran_out(dev, st);
     const long long own = p.own.tiles(), head = p.head.tiles();
     if (own + head > 0x3fffffffLL) return cudaErrorNotSupported;
     const int long_own = p.own.share(), long_head = p.head.blocks();
     p.first_head = own == 0 || (head > 0 && long_head > long_own);
     p.many = (int)(p.first_head ? head : own);
     p.extra = own && head ? std::max(1, (p.first_head ? long_head + long_own / 2 : long_own + long_head / 2) / (p.first_head ? long_own : long_head)) : 0;
-    loss_product_kernel<KIND, TERMS><<<2 * (int)std::min<long long>(own + head, pairs), kThreads, Ring<TERMS>::kSmem, st>>>(a, b, hs ? *hs : a, ht ? *ht : b, p);
+    loss_product_kernel<KIND, TERMS><<<2 * (int)std::min<long long>(own + head, pairs), kThreads, Ring<TERMS, true>::kSmem, st>>>(a, b, hs ? *hs : a, ht ? *ht : b, p);
     return cudaGetLastError();
 }
 
