@@ -13,7 +13,7 @@
 // both, and the accumulators (two per CTA: a tile is taken out while the next is multiplied) live in tensor memory.
 //   warp 0    one lane per CTA: TMA loads of its halves into a ring of stages; every byte of both CTAs counts on the leader's barrier
 //   warp 1    leader only: one elected lane issues the pair's MMAs, commits to the barriers of both CTAs
-//   warps 2-5 epilogue of the CTA's 128 rows
+//   warps 2-9 epilogue of the CTA's 128 rows, half of the columns each
 // P w contracts over rows of w and P^T h over rows of both: those operands lie with the contraction along their rows in memory, and the MMA takes them so
 // (MN-major descriptors); nothing is transposed.
 #include <algorithm>

@@ -621,12 +621,13 @@ mxfp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
 //   all warps round the CTA's share of the rows to MXFP4, straight into the layout of the MMA
 //   warp 1    per stage the scales into tensor memory and its MMAs (M = 128, N = NB)
 //   warps 2-5 take the accumulator out (weight row = lane); with S > 1 the shares meet in shared memory, in the order of the ranges
-// Bound: the weights' bytes where there are many, latency else.  Up to 16 rows: every CTA rounds the rows by itself, which beyond takes longer than a kernel that rounds
-// them once (us, here / rounded once and 128 x 128 tiles: 2048 x 2048 8 rows 5.6 / 9.1, 16 rows 6.1 / 9.7, 32 rows 8.0 / 10.2; 32768 x 2048 13.0 / 15.2, 14.5 / 15.3, 22.7 / 15.5;
-// 8192 x 4096 12.1 / 12.3, 13.9 / 12.8, 21.4 / 13.4).  Tensor memory is taken behind the wait for the predecessor and in front of the signal to the successor:
+// Bound: the weights' bytes where there are many, latency else.  Every CTA rounds the rows by itself, which takes
+// longer than a kernel in front that rounds them once and 128 x 128 tiles from some rows times stages of a CTA on (us, here / there, weights in L2: 2048 x 2048 1 row 4.8 / 8.6,
+// 16 rows 5.8 / 9.0; 32768 x 2048 8.5 / 14.7, 8 rows 10.9 / 14.6, 16 rows - 128 stages rounded - 14.1 / 14.7; weights in memory: 32768 x 2048 8 rows 18 / 22, 16 rows
+// 23 / 22; 32768 x 4096 1 row 31 / 30, 8 rows 37 / 30, 16 rows 46 / 34).  Tensor memory is taken behind the wait for the predecessor and in front of the signal to the successor:
 // a CTA that waits for another kernel holds none of it, so neither can wait for the other.  Shared memory is asked for such that an SM holds three CTAs at most, whose
 // tensor memory fits at the same time: CTAs of a cluster wait for one another.
-constexpr int kFewMost = 16, NB = 16, kFewCols = 128, kFewSmemMost = 226 * 1024, kFewSmemLeast = 58 * 1024, kFewSlotsMost = 12;
+constexpr int kFewMost = 16, kFewRounded = 100, NB = 16, kFewCols = 128, kFewSmemMost = 226 * 1024, kFewSmemLeast = 58 * 1024, kFewSlotsMost = 12;
 static_assert(4 * kFewSmemLeast > 228 * 1024 && 4 * kFewCols <= 512, "CTAs on an SM");
 
 struct FewProduct {
@@ -891,6 +892,7 @@ bool few_plan(int M, int N, int K, int& S, int& per, int& slots, size_t& smem) {
         const size_t fixed = 1024 + each * row + (S > 1 ? NB * 512 : 0);
         if (fixed + std::min<long long>(each, 2) * slot > (size_t)kFewSmemMost) continue;
         per = (int)each;
+        if (M * each > kFewRounded) return false;
         slots = (int)std::min<long long>(each, kFewSlotsMost);
         // two CTAs on an SM where four stages fit: the next launch's weights are then requested while this one runs
         while (slots > 4 && fixed + slots * slot > (size_t)kFewSmemMost / 2) --slots;
