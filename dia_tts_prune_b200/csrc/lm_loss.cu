@@ -179,7 +179,6 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
         if constexpr (PAIR) cluster_sync_all();
         else __syncthreads();
     };
-    if (KIND == kStats && blockIdx.x == 0 && threadIdx.x == 0) *p.arrived = 0u;
     if (threadIdx.x == 0) {
         for (int i = 0; i < kStages; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
         for (int i = 0; i < 2; ++i) { mbar_init(&t_full[i], 1); mbar_init(&t_empty[i], (PAIR ? 2 : 1) * kWarps); }
@@ -198,7 +197,11 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
     everyone();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem_base = *tmem_slot;
-    if (KIND == kStats) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    // Launched while the predecessor may still run.  Tensor memory is held while this waits for it, but an SM has no room for this kernel beside another one that takes some; the
+    // successor may come as soon as every CTA has its own.
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (KIND == kStats && blockIdx.x == 0 && threadIdx.x == 0) *p.arrived = 0u;
     bool ok = true;
     if (warp == 0) {
         if (lane == 0) {
@@ -457,8 +460,7 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
 // Few rows (a token or some, up to 32): the head is the 128-row operand and streams once, the rows are the columns; float32 rows have a column for each of their three
 // terms.  A CTA walks tiles of 128 head rows, and a thread keeps for its head row of every tile, per row of h, the largest logit and the sum of the exponentials below it;
 // at the end the CTA's 128 threads meet.
-//   warp 0    one lane: the head's tile [128 x 64] of a k-block and the rows' [columns x 64] into a ring; the head's first ones before the kernel's predecessor has ended
-//             (nothing that lets its successor start early writes a head)
+//   warp 0    one lane: the head's tile [128 x 64] of a k-block and the rows' [columns x 64] into a ring
 //   warp 1    MMAs (M = 128, N = the columns), an accumulator for 16 k-blocks
 //   warps 2-5 take the accumulators out
 // Bound: the head's bytes.  Tensor memory is taken behind the wait for the predecessor and in front of the signal to the successor (see the few rows of 4-bit numbers).
@@ -500,10 +502,12 @@ __global__ void __launch_bounds__(kFewThreads, 2) loss_few_rows_kernel(const __g
         for (int i = 0; i < kSlots; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
         for (int i = 0; i < 2; ++i) { mbar_init(&t_full[i], 1); mbar_init(&t_empty[i], 4); }
         fence_mbar_init();
-        for (int i = 0; i < min(blocks, kSlots); ++i) { head_tile(i, t, kb); next(); }
     }
+    // (the head may be what the predecessor writes: a gradient, another product's result)
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (blockIdx.x == 0 && tid == 0) *p.arrived = 0u;
+    if (tid == 0)
+        for (int i = 0; i < min(blocks, kSlots); ++i) { head_tile(i, t, kb); row_tile(i, kb); next(); }
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(kFewCols));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
@@ -520,9 +524,7 @@ __global__ void __launch_bounds__(kFewThreads, 2) loss_few_rows_kernel(const __g
     bool ok = true;
     if (warp == 0) {
         if (lane == 0) {
-            int i = 0;
-            t = blockIdx.x; kb = 0;
-            for (; i < min(blocks, kSlots); ++i) { row_tile(i, kb); next(); }
+            int i = min(blocks, kSlots);
             for (; i < blocks; ++i) {
                 const int slot = i % kSlots;
                 if (!lane_wait(&empty[slot], ((i / kSlots) & 1u) ^ 1u, p.polls)) { ok = false; break; }
@@ -708,6 +710,7 @@ __global__ void __launch_bounds__(256) loss_pack_kernel(const void* __restrict__
                                                         int targets64, long long ignore, const float* grad, int grad_stride, const float* count, float scale) {
     const int per_row = ld_out / 8;
     const long long i = (long long)blockIdx.x * 256 + threadIdx.x, r = i / per_row;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (r >= M) return;
     const int k = (int)(i - r * per_row) * 8;
     const bool out_of_it = targets && target_of(targets, targets64, (int)r) == ignore;
@@ -739,6 +742,7 @@ __global__ void __launch_bounds__(256) loss_rows_out_kernel(const float* __restr
                                                             int targets64, long long ignore) {
     const int per_row = ld / 4;
     const long long i = (long long)blockIdx.x * 256 + threadIdx.x, r = i / per_row;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     if (r >= M) return;
     const int k = (int)(i - r * per_row) * 4;
     float4 v = *reinterpret_cast<const float4*>(acc + r * ld + k);
@@ -770,6 +774,22 @@ bool bf16_map(CUtensorMap* map, const void* base, long long rows, long long cols
     const cuuint32_t box[2] = {kBK, (cuuint32_t)box_rows}, estr[2] = {1, 1};
     return enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// a launch that may start while its predecessor still runs (every kernel here waits for it where it has to)
+template <typename... Params, typename... Args>
+cudaError_t launch_early(void (*kernel)(Params...), unsigned grid, unsigned threads, size_t smem, cudaStream_t st, const Args&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
 }
 
 template <int KIND, int TERMS>
@@ -809,8 +829,7 @@ cudaError_t run_tiles(const CUtensorMap& a, const CUtensorMap& b, LossTiles p, i
             if (e != cudaSuccess) return e;
             p.own.rows = 128;
             p.many = p.own.tiles_n();
-            loss_product_kernel<KIND, TERMS, false><<<std::min(p.many, sms), kThreads, Ring<TERMS, false>::kSmem, st>>>(a, b, a, b, p);
-            return cudaGetLastError();
+            return launch_early(loss_product_kernel<KIND, TERMS, false>, std::min(p.many, sms), kThreads, Ring<TERMS, false>::kSmem, st, a, b, a, b, p);
         }
     }
     int pairs = 0;
@@ -822,8 +841,7 @@ cudaError_t run_tiles(const CUtensorMap& a, const CUtensorMap& b, LossTiles p, i
     p.first_head = own == 0 || (head > 0 && long_head > long_own);
     p.many = (int)(p.first_head ? head : own);
     p.extra = own && head ? std::max(1, (p.first_head ? long_head + long_own / 2 : long_own + long_head / 2) / (p.first_head ? long_own : long_head)) : 0;
-    loss_product_kernel<KIND, TERMS><<<2 * (int)std::min<long long>(own + head, pairs), kThreads, Ring<TERMS, true>::kSmem, st>>>(a, b, hs ? *hs : a, ht ? *ht : b, p);
-    return cudaGetLastError();
+    return launch_early(loss_product_kernel<KIND, TERMS>, 2 * (int)std::min<long long>(own + head, pairs), kThreads, Ring<TERMS, true>::kSmem, st, a, b, hs ? *hs : a, ht ? *ht : b, p);
 }
 
 template <int NB, int TERMS>
@@ -832,17 +850,7 @@ cudaError_t run_few(const CUtensorMap& h, const CUtensorMap& w, LossTiles p, int
     if (e != cudaSuccess) return e;
     p.polls = gemm_pair_polls();
     p.ran_out = split_attention_ran_out(dev, st);
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(kFewThreads);
-    cfg.dynamicSmemBytes = Few<NB, TERMS>::kSmem;
-    cfg.stream = st;
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, loss_few_rows_kernel<NB, TERMS>, h, w, p);
+    return launch_early(loss_few_rows_kernel<NB, TERMS>, grid, kFewThreads, Few<NB, TERMS>::kSmem, st, h, w, p);
 }
 
 int padded(int K) { return (K + 7) / 8 * 8; }
@@ -949,17 +957,8 @@ cudaError_t launch_loss(const LossShape& s, int reduction, float* out, float* ke
     else e = f32 ? run_few<32, 3>(ma, mb, p, r.parts / 4, dev, st) : run_few<32, 1>(ma, mb, p, r.parts / 4, dev, st);
     if (e != cudaSuccess) return e;
     ++extra_launches();
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((s.M + kJoinWarps - 1) / kJoinWarps);
-    cfg.blockDim = dim3(32 * kJoinWarps);
-    cfg.stream = st;
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, loss_join_kernel, (const float2*)p.part, (const float*)p.hit, s.M, s.V, r.parts, s.targets, s.targets64, s.ignore, p.c, reduction, out,
-                              kept ? reinterpret_cast<float2*>(kept) : reinterpret_cast<float2*>(base + r.kept), p.arrived);
+    return launch_early(loss_join_kernel, (s.M + kJoinWarps - 1) / kJoinWarps, 32 * kJoinWarps, 0, st, p.part, p.hit, s.M, s.V, r.parts, s.targets, s.targets64, s.ignore, p.c,
+                        reduction, out, kept ? reinterpret_cast<float2*>(kept) : reinterpret_cast<float2*>(base + r.kept), p.arrived);
 }
 
 cudaError_t launch_loss_grad(const LossShape& s, const float* kept, const LossGrad& by, void* dh, void* dw, void* work, cudaStream_t st) {
@@ -1021,11 +1020,9 @@ cudaError_t launch_loss_grad(const LossShape& s, const float* kept, const LossGr
     if (dh) {
         const long long blocks = ((long long)s.M * (ld_acc / 4) + 255) / 256;
         if (blocks > 0x7fffffffLL) return cudaErrorNotSupported;
-        loss_rows_out_kernel<<<(unsigned)blocks, 256, 0, st>>>(acc, r.splits, s.M, s.K, ld_acc, reinterpret_cast<__nv_bfloat16*>(dh),
-                                                              s.K % 4 == 0 && (reinterpret_cast<uintptr_t>(dh) & 7) == 0, by.grad, by.grad_stride, by.count, s.scale, s.targets,
-                                                              s.targets64, s.ignore);
+        e = launch_early(loss_rows_out_kernel, (unsigned)blocks, 256, 0, st, acc, r.splits, s.M, s.K, ld_acc, reinterpret_cast<__nv_bfloat16*>(dh),
+                         (int)(s.K % 4 == 0 && (reinterpret_cast<uintptr_t>(dh) & 7) == 0), by.grad, by.grad_stride, by.count, s.scale, s.targets, s.targets64, s.ignore);
         ++extra_launches();
-        e = cudaGetLastError();
     }
     --extra_launches();                                       // (the caller counts one)
     return e;

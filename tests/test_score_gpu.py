@@ -287,3 +287,34 @@ def test_a_wait_that_ran_out_shows():
             call()
         assert torch.equal(call(), want)
     torch.autograd.grad(loss, leaf, retain_graph=True)
+
+
+def test_a_head_that_the_kernel_in_front_writes():
+    """Kernels start before their predecessor has ended; what it writes may be the head of the next loss (a product's result, a gradient)."""
+    from dia_tts_prune_b200 import lm_ops
+    g = torch.Generator(device="cuda").manual_seed(8)
+    w4 = lm_ops.quantize_mxfp4(torch.randn(4096, 512, generator=g, device="cuda") / 22)
+    xs = [torch.randn(12, 512, generator=g, device="cuda").bfloat16() for _ in range(3)]
+    h, t = torch.randn(3, 4096, generator=g, device="cuda").bfloat16(), torch.tensor([0, 5, 11], device="cuda")
+    want = []
+    for x in xs:
+        y = lm_ops.linear_mxfp4(x, w4)
+        torch.cuda.synchronize()
+        want.append(lm_ops.linear_cross_entropy(h, y, t, reduction="none"))
+    torch.cuda.synchronize()
+    for _ in range(10):
+        got = [lm_ops.linear_cross_entropy(h, lm_ops.linear_mxfp4(x, w4), t, reduction="none") for x in xs]
+        assert all(torch.equal(u, v) for u, v in zip(got, want))
+    rows = torch.randn(200, 512, generator=g, device="cuda").bfloat16()
+    head = (torch.randn(3000, 512, generator=g, device="cuda") / 22).bfloat16().requires_grad_(True)
+    targets = torch.randint(0, 3000, (200,), generator=g, device="cuda")
+
+    def loss_under_a_gradient(wait):
+        dw, = torch.autograd.grad(lm_ops.linear_cross_entropy(rows, head, targets), head)
+        if wait:
+            torch.cuda.synchronize()
+        return lm_ops.linear_cross_entropy(rows[:3] * 100, dw, targets[:3], reduction="none")
+
+    want = loss_under_a_gradient(True)
+    for _ in range(10):
+        assert torch.equal(loss_under_a_gradient(False), want)
