@@ -4,7 +4,9 @@
 //
 // Forward: one product whose epilogue keeps of a 256 x 256 tile of logits, per row, the largest one, the sum of the exponentials below it and the target's, all in fp32;
 // a second kernel joins the tiles of a row.  Backward: the vocabulary goes in pieces.  The product is taken again for a piece, its epilogue turns logits into P (bf16, a
-// piece of at most 64 MB or 4096 columns: it stays in L2), and two products take P to dh (fp32 sums over the pieces) and to the piece's rows of dw.  P is rounded without
+// piece of at most 128 MB or 4096 columns, about what L2 holds), and two products take P to dh (fp32 sums over the pieces) and to the piece's rows of dw; their tiles are dealt
+// to the pairs together.  (8192 x 32768 x 2048 and 4096 x 65536 x 1024, loss and gradients, ms, pieces of 32, 64, 128 and 256 MB: 4.55 and 1.97, 3.58 and 1.90, 3.50 and 1.80,
+// 3.52 and 1.85.)  P is rounded without
 // g: 1 - p of a row's target, which is most of its gradient, then lies just below a power of two where steps are fine, and the roundings of the rows do not go one way
 // (8192 rows: 1.7e-3 to 1.9e-3 of the gradients' norm, of which the results' own rounding is 1.66e-3; with g inside 3.0e-3).  One g for all rows multiplies the sums; rows with
 // their own take it into h for dw (rounded to bf16) and behind the sums for dh.
@@ -897,7 +899,7 @@ Room room_of(const LossShape& s, bool grad, bool rows, bool head) {
         r.arrived = take(4);
         r.kept = take((size_t)s.M * 8 + 4);
     } else {
-        const long long all = (s.V + 255) / 256 * 256LL, fit = (64LL << 20) / 2 / s.M / 256 * 256;
+        const long long all = (s.V + 255) / 256 * 256LL, fit = (128LL << 20) / 2 / s.M / 256 * 256;
         r.piece = (int)std::min(all, std::max(4096LL, fit));
         // shares of dh's contraction where its tiles leave most of the chip idle
         const long long tiles = (long long)((s.M + 255) / 256) * ((s.K + 255) / 256);
