@@ -98,6 +98,7 @@ _SIGNATURES = {
     "lm_b200_op_mxfp4_dequantize": (_ci, [_vp, _vp, _ci, _ci, _vp, _ci, _vp]),
     "lm_b200_op_linear_mxfp4_work_bytes": (C.c_size_t, [_ci, _ci, _ci]),
     "lm_b200_op_linear_mxfp4": (_ci, [_vp, _ci, C.c_int64, _vp, _vp, _vp, _ci, _ci, _ci, _ci, _vp, C.c_size_t, _vp]),
+    "lm_b200_op_loss_lay_out": (_ci, [_vp, C.c_int64, _ci, _ci, _vp, _vp]),
     "lm_b200_op_loss_work_bytes": (C.c_size_t, [_vp, _ci, C.c_int64, _vp, C.c_int64, _ci, _ci, _ci]),
     "lm_b200_op_loss": (_ci, [_vp, _ci, C.c_int64, _vp, C.c_int64, _vp, _ci, C.c_int64, _ci, _ci, _ci, _cf, _ci, _vp, _vp, _vp, C.c_size_t, _vp]),
     "lm_b200_op_loss_grad_work_bytes": (C.c_size_t, [_vp, C.c_int64, _vp, C.c_int64, _ci, _ci, _ci, _ci, _ci]),

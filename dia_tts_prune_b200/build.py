@@ -19,7 +19,7 @@ HEADERS = ["common.cuh", "engine_internal.h", "sampler.cuh", "gemm_tcgen05.h", "
 LM_LIB = CSRC / "liblm_b200.so"
 LM_SOURCES = ["lm_kernels.cu", "lm_mixers.cu", "lm_streams.cu", "lm_linear.cu", "lm_scan.cu", "lm_delta.cu", "lm_attention.cu", "lm_mxfp4.cu", "lm_loss.cu", "lm_engine.cu", "gemm_tcgen05.cu",
               "attention_split.cu"]                                # the tensor-core GEMM is shared with Dia
-LM_HEADERS = ["lm_internal.h", "lm_mxfp4.h", "lm_loss.h", "lm_device.cuh", "gemm_tcgen05.h", "attention_split.h", "common.cuh", "engine_internal.h", "fp32_pairs.cuh", "tensor_cores.cuh"]
+LM_HEADERS = ["lm_internal.h", "lm_store.cuh", "lm_mxfp4.h", "lm_loss.h", "lm_device.cuh", "gemm_tcgen05.h", "attention_split.h", "common.cuh", "engine_internal.h", "fp32_pairs.cuh", "tensor_cores.cuh"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17",
               "-Xcompiler", "-fPIC", "-shared"]
 

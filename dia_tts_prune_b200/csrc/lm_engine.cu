@@ -1775,6 +1775,12 @@ int lm_b200_op_linear_mxfp4(const void* A, int a_type, int64_t lda, const void* 
     return LM_B200_OK;
 }
 
+int lm_b200_op_loss_lay_out(const void* x, int64_t ld, int rows, int K, void* out, void* stream) {
+    if (!x || !out || rows <= 0 || rows > kMostRows || K <= 0 || K > kMostChannels || (rows > 1 && ld < K) || !aligned(out, 16)) return LM_B200_EINVAL;
+    LCK(lm::launch_loss_lay_out(x, rows > 1 ? ld : K, rows, K, out, S(stream)));
+    return LM_B200_OK;
+}
+
 size_t lm_b200_op_loss_work_bytes(const void* h, int h_type, int64_t ldh, const void* W, int64_t ldw, int M, int V, int K) {
     lm::LossShape s;
     return loss_shape(s, h, h_type, ldh, W, ldw, M, V, K) ? lm::loss_work_bytes(s) : 0;

@@ -27,6 +27,7 @@
 #include "gemm_tcgen05.h"
 #include "lm_loss.h"
 #include "lm_mxfp4.h"
+#include "lm_store.cuh"
 #include "tensor_cores.cuh"
 
 namespace lm {
@@ -95,29 +96,12 @@ __device__ __forceinline__ float exp2_fast(float x) {
     return y;
 }
 
-// 32 rows (lane = row) x 64 columns of bf16 through shared memory: whole lines of out [..][ld] from (row0, c0) on, `rows` and `cols` of them
+// 32 rows (lane = row) x 64 columns of bf16 through shared memory to out [..][ld] from (row0, c0) on, `rows` and `cols` of them
 __device__ __forceinline__ void store_64(unsigned char* blk, const uint32_t (&y)[32], __nv_bfloat16* out, long long ld, long long row0, int rows, int c0, int cols, bool wide,
                                          int lane) {
-    const int rr = lane >> 3, ch = lane & 7;
-    // its 16-byte piece c goes to place c ^ (row % 8) of the row's 128 bytes, and is read a row per eight lanes
-#pragma unroll
-    for (int c = 0; c < 8; ++c)
-        *reinterpret_cast<uint4*>(blk + lane * 128 + ((c ^ (lane & 7)) << 4)) = make_uint4(y[4 * c], y[4 * c + 1], y[4 * c + 2], y[4 * c + 3]);
+    turn_rows(blk, y, lane);
     __syncwarp();
-    if (wide) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const int r = 4 * e + rr;
-            if (r < rows && 8 * ch < cols)
-                *reinterpret_cast<uint4*>(out + (row0 + r) * ld + c0 + 8 * ch) = *reinterpret_cast<const uint4*>(blk + r * 128 + ((ch ^ (r & 7)) << 4));
-        }
-    } else {
-        for (int r = 0; r < rows; ++r)
-#pragma unroll
-            for (int c = lane; c < 64; c += 32)
-                if (c < cols)
-                    reinterpret_cast<uint16_t*>(out)[(row0 + r) * ld + c0 + c] = *reinterpret_cast<const uint16_t*>(blk + r * 128 + (((c >> 3) ^ (r & 7)) << 4) + 2 * (c & 7));
-    }
+    store_turned<2>(blk, reinterpret_cast<char*>(out + row0 * ld + c0), (size_t)ld * 2, rows, min(cols, 64), wide, lane);
     __syncwarp();
 }
 
@@ -839,7 +823,8 @@ cudaError_t run_tiles(const CUtensorMap& a, const CUtensorMap& b, LossTiles p, i
     if (e != cudaSuccess) return e;
     const long long own = p.own.tiles(), head = p.head.tiles();
     if (own + head > 0x3fffffffLL) return cudaErrorNotSupported;
-    const int long_own = p.own.share(), long_head = p.head.blocks();
+    // what a tile takes, in k-blocks; taking it out lasts as long as eight of them
+    const int long_own = std::max(p.own.share(), 8), long_head = std::max(p.head.blocks(), 8);
     p.first_head = own == 0 || (head > 0 && long_head > long_own);
     p.many = (int)(p.first_head ? head : own);
     p.extra = own && head ? std::max(1, (p.first_head ? long_head + long_own / 2 : long_own + long_head / 2) / (p.first_head ? long_own : long_head)) : 0;
@@ -921,6 +906,14 @@ LossTiles tiles_of(const LossShape& s) {
 }
 
 }  // namespace
+
+bool loss_reads(const void* x, long long ld) { return in_place(x, ld); }
+int loss_row(int K) { return padded(K); }
+cudaError_t launch_loss_lay_out(const void* x, long long ld, int rows, int K, void* out, cudaStream_t st) {
+    const cudaError_t e = pack<1, false>(x, ld, rows, K, out, nullptr, st);
+    --extra_launches();                                       // (the caller counts one)
+    return e;
+}
 
 size_t loss_work_bytes(const LossShape& s) { return room_of(s, false, false, false).all; }
 size_t loss_grad_work_bytes(const LossShape& s, bool rows, bool head) { return room_of(s, true, rows, head).all; }

@@ -15,7 +15,11 @@ struct LossShape {
     int M, V, K;
     float scale;
 };
-// The operands that are laid out again in the workspace: rows that are fp32 or not of 16 bytes, a head whose rows are not
+// bf16 rows that the kernels read where they are: 16-byte aligned, a multiple of 8 elements apart.  Others are laid out again in the workspace of every call, or by the caller
+// once for several, loss_row(K) elements apart with zeros behind the K-th
+bool loss_reads(const void* x, long long ld);
+int loss_row(int K);
+cudaError_t launch_loss_lay_out(const void* x, long long ld, int rows, int K, void* out, cudaStream_t st);
 size_t loss_work_bytes(const LossShape& s);
 // out: every loss [M], or the sum or the mean (0 where none counts) of those that count.  kept [M][2] and one more (or null), for the gradient: log sum_j exp z[i][j] and the
 // loss, and (not with kLossEach) how many rows count

@@ -13,6 +13,7 @@
 #include "engine_internal.h"
 #include "gemm_tcgen05.h"
 #include "lm_mxfp4.h"
+#include "lm_store.cuh"
 #include "tensor_cores.cuh"
 
 namespace lm {
@@ -271,48 +272,10 @@ __device__ __forceinline__ void take_out(uint32_t from, unsigned char* blk, cons
 #pragma unroll
         for (int e = 0; e < 32; ++e) w[e] = TYPE == kTypeF32 || TYPE == kTypeBf16 ? 0x7fff7fffu : 0x7e007e00u;      // (no result: NaN as one number or two)
     }
-    // a row's 16-byte piece c goes to place c ^ (row % 8) of its 128 bytes
-#pragma unroll
-    for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(blk + lane * 128 + ((c ^ (lane & 7)) << 4)) = make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+    turn_rows(blk, w, lane);
     __syncwarp();
-    const int cols = min(Out<TYPE>::kUnit, p.N - n0), rr = lane >> 3, ch = lane & 7;
-    char* const y = reinterpret_cast<char*>(p.y) + ((size_t)row0 * p.N + n0) * Out<TYPE>::kBytes;
     const size_t pitch = (size_t)p.N * Out<TYPE>::kBytes;
-    if (wide) {                                               // a row per eight lanes
-        uint4 u[8];
-#pragma unroll
-        for (int g = 0; g < 8; ++g) u[g] = *reinterpret_cast<const uint4*>(blk + (4 * g + rr) * 128 + ((ch ^ ((4 * g + rr) & 7)) << 4));
-        const bool in = ch * (16 / Out<TYPE>::kBytes) < cols;
-#pragma unroll
-        for (int g = 0; g < 8; ++g)
-            if (in && 4 * g + rr < rows) *reinterpret_cast<uint4*>(y + (4 * g + rr) * pitch + 16 * ch) = u[g];
-    } else {
-        // A row per warp, eight rows in flight, a 4-byte word per lane.  Where a row of 16-bit numbers begins half way into a word of memory, a lane's word is made of the
-        // second number of the lane in front and its own first one.
-#pragma unroll 1
-        for (int r0 = 0; r0 < rows; r0 += 8) {
-            uint32_t u[8];
-#pragma unroll
-            for (int g = 0; g < 8; ++g) u[g] = *reinterpret_cast<const uint32_t*>(blk + (r0 + g) * 128 + (((lane >> 2) ^ g) << 4) + 4 * (lane & 3));
-#pragma unroll
-            for (int g = 0; g < 8; ++g) {
-                char* const row = y + (r0 + g) * pitch;
-                if constexpr (TYPE == kTypeF32) {
-                    if (r0 + g < rows && lane < cols) *reinterpret_cast<uint32_t*>(row + 4 * lane) = u[g];
-                } else {
-                    const uint32_t front = __shfl_up_sync(0xffffffffu, u[g], 1);
-                    if (r0 + g >= rows) continue;
-                    const int off = (int)(reinterpret_cast<uintptr_t>(row) >> 1 & 1), c = 2 * lane - off;
-                    const uint32_t word = off ? __funnelshift_r(front, u[g], 16) : u[g];
-                    if (c >= 0 && c + 1 < cols) *reinterpret_cast<uint32_t*>(row + 2 * c) = word;
-                    // what stands alone at either end: the first number, the last one (of 64: a second store of the last lane)
-                    const bool front_end = c < 0, back_end = c == cols - 1, last = off && lane == 31 && cols == 64;
-                    if (front_end || back_end || last)
-                        *reinterpret_cast<uint16_t*>(row + 2 * (front_end ? 0 : back_end ? c : 63)) = (uint16_t)(front_end ? u[g] : back_end ? word : u[g] >> 16);
-                }
-            }
-        }
-    }
+    store_turned<Out<TYPE>::kBytes>(blk, reinterpret_cast<char*>(p.y) + (row0 * pitch + (size_t)n0 * Out<TYPE>::kBytes), pitch, rows, min(Out<TYPE>::kUnit, p.N - n0), wide, lane);
     __syncwarp();
 }
 

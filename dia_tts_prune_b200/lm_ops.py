@@ -188,14 +188,27 @@ def _loss_operands(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Te
         raise ValueError("weight is empty")
 
 
+def _laid_out(x: torch.Tensor) -> torch.Tensor:
+    """bfloat16 rows as the loss's kernels read them where they are: themselves, or a copy with rows of whole 16 bytes (zeros behind the
+    last channel), for operands that a forward and a backward pass read."""
+    (rows, width), device = x.shape, x.device
+    if x.dtype != torch.bfloat16 or not (x.data_ptr() & 15 or (x.stride(0) if rows > 1 else width) & 7):
+        return x
+    out = x.new_empty((rows, (width + 7) // 8 * 8))
+    _call("loss_lay_out", device, x.data_ptr(), x.stride(0), rows, width, out.data_ptr())
+    return out
+
+
 _REDUCTIONS = {"none": _lm_lib.LOSS_EACH, "sum": _lm_lib.LOSS_SUM, "mean": _lm_lib.LOSS_MEAN}
 
 
 def _losses(hidden, weight, targets, scale, ignore_index, reduction, keep):
-    """(losses or their sum or mean; the targets as they were read; with ``keep`` what the gradient needs: [log-sum, loss] of every row and
-    how many rows count)."""
+    """(losses or their sum or mean, what the gradient needs).  The latter, with ``keep``: hidden, weight and targets as they were read, and
+    [log-sum, loss] of every row and how many rows count."""
     h, w, t = _as_rows(hidden), _as_rows(weight), targets.contiguous()
     (M, K), V, device = h.shape, w.shape[0], h.device
+    if keep:
+        h, w = _laid_out(h), _laid_out(w)
     out = h.new_empty(M if reduction == "none" else (), dtype=torch.float32)
     kept = h.new_empty(2 * M + 1, dtype=torch.float32) if keep else None
     h_at, w_at, h_type, ldh, ldw = h.data_ptr(), w.data_ptr(), _TYPES[h.dtype], h.stride(0), w.stride(0)
@@ -203,7 +216,7 @@ def _losses(hidden, weight, targets, scale, ignore_index, reduction, keep):
     work = h.new_empty(need, dtype=torch.uint8)
     _call("loss", device, h_at, h_type, ldh, w_at, ldw, t.data_ptr(), t.dtype == torch.int64, ignore_index, M, V, K, scale,
           _REDUCTIONS[reduction], out.data_ptr(), kept.data_ptr() if keep else None, work.data_ptr(), need)
-    return out, t, kept
+    return out, (h, w, t, kept)
 
 
 class _LinearCrossEntropy(torch.autograd.Function):
@@ -211,19 +224,19 @@ class _LinearCrossEntropy(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, hidden, weight, targets, scale, ignore_index, reduction):
-        out, t, kept = _losses(hidden, weight, targets, scale, ignore_index, reduction, True)
-        ctx.save_for_backward(hidden, weight, t, kept)
+        out, read = _losses(hidden, weight, targets, scale, ignore_index, reduction, True)
+        # (the operands themselves are kept too where they were laid out again: a change of theirs in place shows)
+        ctx.save_for_backward(hidden, weight, *read)
         ctx.args = scale, ignore_index, reduction == "mean"
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        hidden, weight, t, kept = ctx.saved_tensors
+        hidden, weight, h, w, t, kept = ctx.saved_tensors
         scale, ignore_index, mean = ctx.args
         need_h, need_w = ctx.needs_input_grad[:2]
         (M, K), V, device = hidden.shape, weight.shape[0], hidden.device
-        h, w = _as_rows(hidden), _as_rows(weight)
         if grad.dim() and grad.stride(0) < 0:
             grad = grad.contiguous()
         dh = hidden.new_empty((M, K)) if need_h else None

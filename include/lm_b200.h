@@ -326,7 +326,10 @@ int lm_b200_op_linear_mxfp4(const void *A, int a_type, int64_t lda, const void *
  * gradient: log sum_j exp z[i][j] and the loss of every row, and behind them (with a sum or a mean) how many rows count.
  * The gradient (h in bf16): P = softmax(z) - onehot, g = scale grad [/ max(*count, 1)], dh_i = g_i P_i W (bf16 [M][K]), dW = P^T (g h) (bf16 [V][K]), either may be NULL.  grad:
  * fp32, of every loss, grad_stride apart (0: one number).  Rows that do not count have no part in either, whatever they hold; a NaN loss has NaN gradients.
- * P is kept in bf16 for a piece of the vocabulary at a time.  work: 256-byte aligned. */
+ * P is kept in bf16 for a piece of the vocabulary at a time.  work: 256-byte aligned.
+ * Rows of h and W that are bf16, 16-byte aligned and a multiple of 8 elements apart are read where they are.  Others are laid out again in the workspace of every call, or once
+ * for several by lm_b200_op_loss_lay_out: out [rows][(K + 7) / 8 * 8], zeros behind the K-th, to be handed over in their place with that stride. */
+int lm_b200_op_loss_lay_out(const void *x, int64_t ld, int rows, int K, void *out, void *stream);
 /* (of h and W the alignment counts) */
 enum lm_b200_loss_reduction { LM_B200_LOSS_EACH = 0, LM_B200_LOSS_SUM = 1, LM_B200_LOSS_MEAN = 2 };
 size_t lm_b200_op_loss_work_bytes(const void *h, int h_type, int64_t ldh, const void *W, int64_t ldw, int M, int V, int K);
