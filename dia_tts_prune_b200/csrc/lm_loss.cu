@@ -96,13 +96,13 @@ __device__ __forceinline__ float exp2_fast(float x) {
     return y;
 }
 
-// 32 rows (lane = row) x 64 columns of bf16 through shared memory to out [..][ld] from (row0, c0) on, `rows` and `cols` of them
-__device__ __forceinline__ void store_64(unsigned char* blk, const uint32_t (&y)[32], __nv_bfloat16* out, long long ld, long long row0, int rows, int c0, int cols, bool wide,
-                                         int lane) {
-    turn_rows(blk, y, lane);
-    __syncwarp();
-    store_turned<2>(blk, reinterpret_cast<char*>(out + row0 * ld + c0), (size_t)ld * 2, rows, min(cols, 64), wide, lane);
-    __syncwarp();
+// 32 rows x 128 columns of bf16, of which this warp has half the columns (lane = row), by the two warps of a quarter to out [..][ld] from (row0, c0) on, `rows` and `cols` of them
+__device__ __forceinline__ void store_128(unsigned char* panel, const uint32_t (&y)[32], __nv_bfloat16* out, long long ld, long long row0, int rows, int c0, int cols, bool wide,
+                                          int quarter, int half, int lane) {
+    fill_panel(panel, half, y, lane);
+    panel_sync(quarter);
+    store_panel<2>(panel, reinterpret_cast<char*>(out + row0 * ld + c0), (size_t)ld * 2, half, rows, min(cols, 128), wide, lane);
+    panel_sync(quarter);
 }
 
 struct Tile {
@@ -276,7 +276,9 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
         }
     } else {
         const int q = warp & 3, c_half = (warp - 2) >> 2 << 7;               // (a warp reads the 32 lanes of its number mod 4) and its half of the columns
-        unsigned char* const blk = turn + (warp - 2) * 4096;
+        const int half = (warp - 2) >> 2;
+        unsigned char* const panel = turn + q * kPanelBytes;                 // of both warps that read these lanes; blk: this one's share of it
+        unsigned char* const blk = panel + half * 4096;
         float factor = 1.f;
         if (KIND == kGrads && p.grad) {
             factor = *p.grad * p.scale;
@@ -294,7 +296,8 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
             const Tiles& of = KIND == kGrads && t.head ? p.head : p.own;
             const int n0 = t.n * kTileN + c_half, row0 = t.m * (PAIR ? 256 : 128) + (int)rank * 128 + q * 32, rows = min(32, of.M - row0), row = row0 + lane;
             const bool mine = row < of.M;
-            const auto from = [&]() { return tmem_base + ((uint32_t)(q * 32) << 16) + (it & 1u) * kTileN + c_half; };
+            const auto tile_at = [&]() { return tmem_base + ((uint32_t)(q * 32) << 16) + (it & 1u) * kTileN; };
+            const auto from = [&]() { return tile_at() + c_half; };
             const auto wait = [&]() {
                 ok = ok && pair_wait(&t_full[it & 1u], (it >> 1) & 1u, p.polls);
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -354,13 +357,14 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                 wait();
                 if (!ok) base = own = CUDART_NAN_F;
 #pragma unroll 1
-                for (int cb = 0; cb < 2; ++cb) {
+                for (int cb = 0; cb < 2; ++cb) {              // (128 columns at a time, half of them here)
                     if (rows <= 0) break;
+                    const int c0 = t.n * kTileN + cb * 128, mine0 = c0 + half * 64;
                     uint32_t v[2][32], y[32];
-                    tmem_columns32(from() + cb * 64, v[0]);
-                    tmem_columns32(from() + cb * 64 + 32, v[1]);
+                    tmem_columns32(tile_at() + cb * 128 + half * 64, v[0]);
+                    tmem_columns32(tile_at() + cb * 128 + half * 64 + 32, v[1]);
                     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                    const int at = target - (n0 + cb * 64);
+                    const int at = target - mine0;
 #pragma unroll
                     for (int e = 0; e < 32; ++e) {
                         float f[2];
@@ -373,7 +377,7 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                         const __nv_bfloat162 b = __floats2bfloat162_rn(f[0], f[1]);
                         y[e] = *reinterpret_cast<const uint32_t*>(&b);
                     }
-                    store_64(blk, y, p.p, p.ldp, row0, rows, n0 + cb * 64, 64, true, lane);
+                    store_128(panel, y, p.p, p.ldp, row0, rows, c0, 128, true, q, half, lane);
                 }
                 taken();
             } else if (!t.head) {
@@ -406,24 +410,25 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                     }
                     __syncwarp();
                 }
+                panel_sync(q);                                // (the other warp's share is a panel's too)
                 taken();
             } else {
                 wait();
                 if (!ok) factor = CUDART_NAN_F;
 #pragma unroll 1
                 for (int cb = 0; cb < 2; ++cb) {
-                    const int c0 = n0 + cb * 64;
+                    const int c0 = t.n * kTileN + cb * 128;
                     if (c0 >= of.N || rows <= 0) break;
                     uint32_t v[2][32], y[32];
-                    tmem_columns32(from() + cb * 64, v[0]);
-                    tmem_columns32(from() + cb * 64 + 32, v[1]);
+                    tmem_columns32(tile_at() + cb * 128 + half * 64, v[0]);
+                    tmem_columns32(tile_at() + cb * 128 + half * 64 + 32, v[1]);
                     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
                     for (int e = 0; e < 32; ++e) {
                         const __nv_bfloat162 b = __floats2bfloat162_rn(__uint_as_float(v[e >> 4][2 * e & 31]) * factor, __uint_as_float(v[e >> 4][(2 * e & 31) + 1]) * factor);
                         y[e] = *reinterpret_cast<const uint32_t*>(&b);
                     }
-                    store_64(blk, y, p.out, of.N, row0, rows, c0, of.N - c0, p.wide, lane);
+                    store_128(panel, y, p.out, of.N, row0, rows, c0, of.N - c0, p.wide, q, half, lane);
                 }
                 taken();
             }

@@ -240,11 +240,10 @@ struct TiledProduct {
     unsigned polls;
 };
 
-// 32 rows (lane = row) x 128 bytes of results - kUnit columns - from an accumulator, turned through shared memory so that whole lines are stored.
+// columns of a panel of results (see lm_store.cuh)
 template <int TYPE>
 struct Out {
-    static constexpr int kUnit = TYPE == kTypeF32 ? 32 : 64;
-    static constexpr int kBytes = TYPE == kTypeF32 ? 4 : 2;
+    static constexpr int kBytes = TYPE == kTypeF32 ? 4 : 2, kPanel = 256 / kBytes;
 };
 __device__ __forceinline__ uint32_t pack16(int type, float lo, float hi) {
     if (type == kTypeBf16) {
@@ -254,29 +253,34 @@ __device__ __forceinline__ uint32_t pack16(int type, float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
 }
+// A panel of an accumulator (from: its first column of the warp's 32 rows; `width` columns are there) to rows row0 .. and columns n0 .. of the result, by the two warps of a
+// quarter.
 template <int TYPE>
-__device__ __forceinline__ void take_out(uint32_t from, unsigned char* blk, const TiledProduct& p, int row0, int rows, int n0, int lane, bool ok, bool wide) {
+__device__ __forceinline__ void take_out(uint32_t from, int width, unsigned char* panel, const TiledProduct& p, int row0, int rows, int n0, int quarter, int half, int lane, bool ok,
+                                         bool wide) {
     uint32_t w[32];
-    if constexpr (TYPE == kTypeF32) {
-        tmem_columns32(from, w);
-        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-    } else {
-        uint32_t v[2][32];
-        tmem_columns32(from, v[0]);
-        tmem_columns32(from + 32, v[1]);
-        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+    if (half * (Out<TYPE>::kPanel / 2) < width) {
+        if constexpr (TYPE == kTypeF32) {
+            tmem_columns32(from + 32 * half, w);
+            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        } else {
+            uint32_t v[2][32];
+            tmem_columns32(from + 64 * half, v[0]);
+            tmem_columns32(from + 64 * half + 32, v[1]);
+            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-        for (int e = 0; e < 32; ++e) w[e] = pack16(TYPE, __uint_as_float(v[e >> 4][2 * e & 31]), __uint_as_float(v[e >> 4][(2 * e & 31) + 1]));
-    }
-    if (!ok) {
+            for (int e = 0; e < 32; ++e) w[e] = pack16(TYPE, __uint_as_float(v[e >> 4][2 * e & 31]), __uint_as_float(v[e >> 4][(2 * e & 31) + 1]));
+        }
+        if (!ok) {
 #pragma unroll
-        for (int e = 0; e < 32; ++e) w[e] = TYPE == kTypeF32 || TYPE == kTypeBf16 ? 0x7fff7fffu : 0x7e007e00u;      // (no result: NaN as one number or two)
+            for (int e = 0; e < 32; ++e) w[e] = TYPE == kTypeF16 ? 0x7e007e00u : 0x7fff7fffu;                     // (no result: NaN as one number or two)
+        }
+        fill_panel(panel, half, w, lane);
     }
-    turn_rows(blk, w, lane);
-    __syncwarp();
+    panel_sync(quarter);
     const size_t pitch = (size_t)p.N * Out<TYPE>::kBytes;
-    store_turned<Out<TYPE>::kBytes>(blk, reinterpret_cast<char*>(p.y) + (row0 * pitch + (size_t)n0 * Out<TYPE>::kBytes), pitch, rows, min(Out<TYPE>::kUnit, p.N - n0), wide, lane);
-    __syncwarp();
+    store_panel<Out<TYPE>::kBytes>(panel, reinterpret_cast<char*>(p.y) + (row0 * pitch + (size_t)n0 * Out<TYPE>::kBytes), pitch, half, rows, min(width, p.N - n0), wide, lane);
+    panel_sync(quarter);
 }
 
 template <int TYPE>
@@ -285,8 +289,7 @@ __device__ __forceinline__ bool whole_pieces(const TiledProduct& p) { return p.N
 // One CTA per SM walks 128 x 128 tiles.
 //   warp 0    one lane: a stage's codes (TMA, 128-byte swizzle) and scales (plain bulk copies)
 //   warp 1    one elected lane: the stage's scales into tensor memory, then its MMAs of 64 channels
-//   warps 2-9 take a finished accumulator out through shared memory while the next tile fills the other (with four of them 4096 x 16383 x 256, whose rows begin anywhere,
-//             took 102 us in fp32)
+//   warps 2-9 take a finished accumulator out through shared memory while the next tile fills the other (four of them took up to twice as long, rows that begin anywhere)
 template <int TYPE>
 __global__ void __launch_bounds__(kThreads4, 1)
 mxfp4_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ TiledProduct p) {
@@ -384,8 +387,8 @@ mxfp4_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
             }
         }
     } else {
-        const int q = warp & 3, c_half = ((warp - 2) >> 2) * (kBN / 2);      // (a warp reads the 32 lanes of its number mod 4) and its half of the columns
-        unsigned char* const blk = turn + (warp - 2) * 4096;
+        const int q = warp & 3, half = (warp - 2) >> 2;       // (a warp reads the 32 lanes of its number mod 4)
+        unsigned char* const panel = turn + q * kPanelBytes;
         const bool wide = whole_pieces<TYPE>(p);
         unsigned it = 0;
         for (int t = blockIdx.x; t < n_tiles; t += gridDim.x, ++it) {
@@ -393,8 +396,8 @@ mxfp4_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
             ok = ok && pair_wait(&t_full[it & 1u], (it >> 1) & 1u, p.polls);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
-            for (int c = c_half; c < c_half + kBN / 2 && n0 + c < p.N && rows > 0; c += Out<TYPE>::kUnit)
-                take_out<TYPE>(tmem + ((uint32_t)(q * 32) << 16) + (it & 1u) * kBN + c, blk, p, row0, rows, n0 + c, lane, ok, wide);
+            for (int c = 0; c < kBN && n0 + c < p.N && rows > 0; c += Out<TYPE>::kPanel)
+                take_out<TYPE>(tmem + ((uint32_t)(q * 32) << 16) + (it & 1u) * kBN + c, kBN - c, panel, p, row0, rows, n0 + c, q, half, lane, ok, wide);
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive(&t_empty[it & 1u]);
@@ -418,7 +421,7 @@ mxfp4_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
 // SM needs the scales of its own 128 rows and of all 192 columns; those of an odd tile begin half way into a block of 128, two columns further.
 //   warp 0    one lane per CTA: codes and scales (TMA) of its halves; every byte of both CTAs counts on the leader's barrier
 //   warp 1    leader only: a stage's scales into the tensor memory of both, then the pair's MMAs; commits to the barriers of both
-//   warps 2-9 take the CTA's 128 rows of a finished accumulator out, half of the columns each
+//   warps 2-9 take the CTA's 128 rows of a finished accumulator out
 // Bound: what the SMs take from L2, 11 TB/s (4096 x 16384 x 4096, us: 124; without MMAs 128 of then 132, without the copies of scales into tensor memory 131, without loading
 // scales 104 - two pieces of 512 bytes at a time they were three loads a stage, and 132 - without taking results out 127).
 constexpr int kPairN = 192, kPairStages = 6, kPairWarps = 8, kPairThreads = 64 + 32 * kPairWarps;
@@ -543,22 +546,17 @@ mxfp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
             }
         }
     } else {
-        constexpr int kUnits = kPairN / Out<TYPE>::kUnit;     // three or six: the two warps of a quarter take the middle one in turns, or half of them each
-        const int q = warp & 3, second = (warp - 2) >> 2;
-        unsigned char* const blk = turn + (warp - 2) * 4096;
+        const int q = warp & 3, half = (warp - 2) >> 2;
+        unsigned char* const panel = turn + q * kPanelBytes;
         const bool wide = whole_pieces<TYPE>(p);
         unsigned it = 0;
         for (int t = pair; t < n_tiles; t += pairs, ++it) {
             const int n0 = t / tiles_m * kPairN, row0 = t % tiles_m * 256 + (int)rank * 128 + q * 32, rows = min(32, p.M - row0);
-            const int border = (kUnits + (int)(it & 1u)) / 2;
             ok = ok && pair_wait(&t_full[it & 1u], (it >> 1) & 1u, p.polls);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
-            for (int u = second ? border : 0; u < (second ? kUnits : border); ++u) {
-                const int c = u * Out<TYPE>::kUnit;
-                if (n0 + c >= p.N || rows <= 0) break;
-                take_out<TYPE>(tmem + ((uint32_t)(q * 32) << 16) + (it & 1u) * kPairN + c, blk, p, row0, rows, n0 + c, lane, ok, wide);
-            }
+            for (int c = 0; c < kPairN && n0 + c < p.N && rows > 0; c += Out<TYPE>::kPanel)
+                take_out<TYPE>(tmem + ((uint32_t)(q * 32) << 16) + (it & 1u) * kPairN + c, kPairN - c, panel, p, row0, rows, n0 + c, q, half, lane, ok, wide);
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
             if (lane == 0) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(at_rank(&t_empty[it & 1u], 0)) : "memory");
