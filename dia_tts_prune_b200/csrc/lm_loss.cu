@@ -377,6 +377,11 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                         const __nv_bfloat162 b = __floats2bfloat162_rn(f[0], f[1]);
                         y[e] = *reinterpret_cast<const uint32_t*>(&b);
                     }
+                    // (behind the last column the contraction meets zeros, but not with an infinity: 0 there may lie far above a row's logits)
+                    if (mine0 + 64 > of.N) {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) y[e] &= mine0 + 2 * e + 1 < of.N ? 0xffffffffu : mine0 + 2 * e < of.N ? 0xffffu : 0u;
+                    }
                     store_128(panel, y, p.p, p.ldp, row0, rows, c0, 128, true, q, half, lane);
                 }
                 taken();
@@ -991,7 +996,8 @@ cudaError_t launch_loss_grad(const LossShape& s, const float* kept, const LossGr
     if (!bf16_map(&h_rows, h, s.M, s.K, ldh, 128) || !bf16_map(&w_rows, w, s.V, s.K, ldw, 128) || !bf16_map(&p_rows, probs, s.M, r.piece, r.piece, 128) ||
         (dw && !bf16_map(&h_cols, base + r.h_dw, s.M, s.K, padded(s.K), kBK)) || !bf16_map(&w_cols, w, s.V, s.K, ldw, kBK) || !bf16_map(&p_cols, probs, s.M, r.piece, r.piece, kBK))
         return cudaErrorNotSupported;
-    for (int v0 = 0; v0 < s.V; v0 += r.piece) {
+    for (long long from = 0; from < s.V; from += r.piece) {
+        const int v0 = (int)from;
         const int cols = std::min(r.piece, s.V - v0);
         LossTiles p = tiles_of(s);
         p.v0 = v0;

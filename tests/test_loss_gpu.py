@@ -175,6 +175,25 @@ def test_infinities_and_far_logits():
     assert abs(float(got) - want) <= 2.0 ** -23
 
 
+@pytest.mark.parametrize("v", [300, 4097, 513])
+def test_gradients_of_far_away_logits(v):
+    """All logits of a row hundreds below (or above) zero, a vocabulary that ends inside a tile: columns that are not there have logits of
+    zero, far above those, and no part in the gradients."""
+    from dia_tts_prune_b200.lm_ops import linear_cross_entropy
+    for m in (3, 140, 300):
+        for sign in (-1.0, 1.0):
+            h, w, t = operands(m, v, 64, 31)
+            h[:, 0], w[:, 0] = 32.0, 8.0 * sign                    # (256 of every logit)
+            e = Exact(h, w, t)
+            assert float(e.p.sum(1).sub(1).abs().max()) < 1e-9 and float((e.h @ e.w.T).mul(sign).min()) > 150
+            a, b = h.requires_grad_(True), w.requires_grad_(True)
+            loss = linear_cross_entropy(a, b, t, reduction="none")
+            within(loss, e.loss, e.loss_off)
+            got = torch.autograd.grad(loss.sum(), (a, b))
+            for x, (want, bound) in zip(got, e.gradient(torch.ones(m))):
+                within(x, want, bound)
+
+
 def test_strides_leading_dimensions_and_empty():
     from dia_tts_prune_b200.lm_ops import linear_cross_entropy
     h, w, t = operands(24, 300, 104, 9)
