@@ -237,7 +237,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
         scale, ignore_index, mean = ctx.args
         need_h, need_w = ctx.needs_input_grad[:2]
         (M, K), V, device = hidden.shape, weight.shape[0], hidden.device
-        if grad.dim() and grad.stride(0) < 0:
+        if grad.dim() and grad.stride(0) > 0x7fffffff:            # (the library takes strides of 32 bits)
             grad = grad.contiguous()
         dh = hidden.new_empty((M, K)) if need_h else None
         dw = weight.new_empty((V, K)) if need_w else None

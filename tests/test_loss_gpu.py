@@ -194,6 +194,21 @@ def test_gradients_of_far_away_logits(v):
                 within(x, want, bound)
 
 
+def test_factors_of_rows_that_lie_far_apart():
+    """Gradients of every row's loss may come with any stride."""
+    from dia_tts_prune_b200.lm_ops import linear_cross_entropy
+    h, w, t = operands(3, 40, 16, 5, ignored=0.0)
+    g = torch.tensor([1.0, -2.0, 0.5], device="cuda")
+    far = torch.empty_strided((3,), ((1 << 31) + 3,), dtype=torch.float32, device="cuda")     # (17 GB, of which three numbers are touched)
+    far.copy_(g)
+    out = []
+    for by in (g, far, torch.stack((g, g), 1)[:, 1], g.flip(0).flip(0)):
+        a, b = h.detach().requires_grad_(True), w.detach().requires_grad_(True)
+        out.append(torch.autograd.grad(linear_cross_entropy(a, b, t, reduction="none"), (a, b), by))
+    for x in out[1:]:
+        assert torch.equal(x[0], out[0][0]) and torch.equal(x[1], out[0][1])
+
+
 def test_strides_leading_dimensions_and_empty():
     from dia_tts_prune_b200.lm_ops import linear_cross_entropy
     h, w, t = operands(24, 300, 104, 9)
