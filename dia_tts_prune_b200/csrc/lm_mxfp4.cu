@@ -96,8 +96,8 @@ __device__ __forceinline__ uint32_t round_block(const float (&v)[8], uint32_t& s
 }
 
 // A CTA takes 128 rows x 256 channels, a warp 16 rows of them, a lane eight channels (four neighbours a block): kAhead rows are on their way at a time, and the scales
-// leave as the two pieces that they are.  early: the successor, a product of these rows, may start now (never where the rows are a matrix to keep: products ask for
-// theirs before their predecessor has ended).  Rows behind the last one of a piece get scales of zero.  Bound: memory (32768 x 2048 bf16, 170 MB: 75 us with an index per eight
+// leave as the two pieces that they are.  early: the successor, a product of these rows, may start now (a product asks for its weights before
+// this kernel has ended: they are never what it writes).  Rows behind the last one of a piece get scales of zero.  Bound: memory (32768 x 2048 bf16, 170 MB: 75 us with an index per eight
 // channels, whose scales went out byte by byte).
 constexpr int kQuantThreads = 256, kAhead = 8;
 template <int TYPE, bool WIDE>
@@ -577,14 +577,14 @@ mxfp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
 
 // Few rows (decoding): the weights are the 128-row operand and stream once, the rows are the columns.  A cluster of S CTAs owns 128 weight rows, each
 // CTA a range of stages.
-//   warp 0    requests the CTA's weight codes and scales ahead of the rows - before the kernel's predecessor has ended (nothing that lets its successor start early
-//             writes weights)
+//   warp 0    requests the CTA's weight codes and scales ahead of the rows, but not before the kernel's predecessor has ended, which may have written them (that takes
+//             0.2 us of 32768 x 2048 with one row, 0.7 of 4096 x 4096 read from memory by one product after the other, nothing where another kernel lies between)
 //   all warps round the CTA's share of the rows to MXFP4, straight into the layout of the MMA
 //   warp 1    per stage the scales into tensor memory and its MMAs (M = 128, N = NB)
 //   warps 2-5 take the accumulator out (weight row = lane); with S > 1 the shares meet in shared memory, in the order of the ranges
 // Bound: the weights' bytes where there are many, latency else.  Every CTA rounds the rows by itself, which takes
 // longer than a kernel in front that rounds them once and 128 x 128 tiles from some rows times stages of a CTA on (us, here / there, weights in L2: 2048 x 2048 1 row 4.8 / 8.6,
-// 16 rows 5.8 / 9.0; 32768 x 2048 8.5 / 14.7, 8 rows 10.9 / 14.6, 16 rows - 128 stages rounded - 14.1 / 14.7; weights in memory: 32768 x 2048 8 rows 18 / 22, 16 rows
+// 16 rows 5.8 / 9.0; 32768 x 2048 8.5 / 14.7, 8 rows 11.4 / 14.6, 16 rows - 128 stages rounded - 14.1 / 14.7; weights in memory: 32768 x 2048 8 rows 18 / 22, 16 rows
 // 23 / 22; 32768 x 4096 1 row 31 / 30, 8 rows 37 / 30, 16 rows 46 / 34).  Tensor memory is taken behind the wait for the predecessor and in front of the signal to the successor:
 // a CTA that waits for another kernel holds none of it, so neither can wait for the other.  Shared memory is asked for such that an SM holds three CTAs at most, whose
 // tensor memory fits at the same time: CTAs of a cluster wait for one another.
@@ -628,9 +628,10 @@ __global__ void __launch_bounds__(kFewThreads, 2) mxfp4_few_rows_kernel(const __
         for (int i = 0; i < p.slots; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
         mbar_init(&t_full, 1);
         fence_mbar_init();
-        for (int s = 0; s < min(stages, p.slots); ++s) request(s, s);
     }
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (tid == 0)
+        for (int s = 0; s < min(stages, p.slots); ++s) request(s, s);
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(kFewCols));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
@@ -855,7 +856,7 @@ bool few_plan(int M, int N, int K, int& S, int& per, int& slots, size_t& smem) {
         per = (int)each;
         if (M * each > kFewRounded) return false;
         slots = (int)std::min<long long>(each, kFewSlotsMost);
-        // two CTAs on an SM where four stages fit: the next launch's weights are then requested while this one runs
+        // two CTAs on an SM where four stages fit: more of them load at a time, and the next launch's come while this one runs (32768 x 2048, 1 row: 8.5 us, else 14.6)
         while (slots > 4 && fixed + slots * slot > (size_t)kFewSmemMost / 2) --slots;
         while (fixed + slots * slot > (size_t)kFewSmemMost) --slots;
         smem = std::max<size_t>(fixed + slots * slot, kFewSmemLeast);
