@@ -263,3 +263,45 @@ def test_nothing_is_written_beside_the_results(m, v, k):
                                     work2[1], need, st) == 0
     torch.cuda.synchronize()
     assert all(kept(r) for r in (each, one, keep, dh, dw, work, work2))
+
+
+def test_offsets_past_32_bits():
+    """Rows, and a head, of 2^31 numbers and some: losses and gradients of the last rows are what they are alone; the head's last rows have
+    the formula's gradient."""
+    from dia_tts_prune_b200.lm_ops import linear_cross_entropy
+    g = torch.Generator(device="cuda").manual_seed(2)
+    rows, k, v, last = 270000, 8192, 300, 432
+    x = torch.empty(rows, k, dtype=torch.bfloat16, device="cuda").normal_(generator=g)
+    w, t = (torch.randn(v, k, generator=g, device="cuda") / 90).bfloat16(), torch.randint(0, v, (rows,), generator=g, device="cuda")
+    got = []
+    for a, targets in ((x, t), (x[-last:], t[-last:])):
+        a = a.detach().requires_grad_(True)
+        loss = linear_cross_entropy(a, w, targets, reduction="none")
+        got.append((loss[-last:], torch.autograd.grad(loss.sum(), a)[0][-last:]))
+    # (logits alike; dh's sums over the vocabulary may be split where there are few rows: a rounding and the sums' own loss apart)
+    assert torch.equal(got[0][0], got[1][0])
+    z = (x[-last:].double() @ w.double().T).softmax(1)
+    z[torch.arange(last), t[-last:]] -= 1
+    bound = 2.0 ** -7 * got[1][1].double().abs() + 2.0 ** -18 * (z.abs() @ w.double().abs())
+    assert ((got[0][1].double() - got[1][1].double()).abs() <= bound).all()
+    del got, a, loss
+    for m in (3, 40):
+        h = (torch.randn(m, k, generator=g, device="cuda") / 30).bfloat16()
+        t = torch.randint(rows - last, rows, (m,), generator=g, device="cuda")
+        a, b = h.clone().requires_grad_(True), x.requires_grad_(True)
+        loss = linear_cross_entropy(a, b, t, reduction="none")
+        lse = torch.full((m,), -math.inf, dtype=torch.float64, device="cuda")
+        for i in range(0, rows, 27000):
+            lse = torch.logaddexp(lse, (h.double() @ x.detach()[i:i + 27000].double().T).logsumexp(1))
+        tail = x.detach()[-last:].double()
+        z = h.double() @ tail.T
+        dz = (k / 16 + 2) * 2.0 ** -22 * float((h.double().abs() @ tail.abs().T).max()) * 1.5      # (of other rows too: their largest is like that)
+        hit = z.gather(1, (t - (rows - last))[:, None])[:, 0]
+        assert ((loss.double() - (lse - hit)).abs() <= 2 * dz + 2.0 ** -20 + 2.0 ** -22 * (z.abs().amax() + loss.double())).all()
+        dw = torch.autograd.grad(loss.sum(), b)[0][-last:].double()
+        P = (z - lse[:, None]).exp()
+        dP = P * (4 * dz + 2.0 ** -18)
+        P[torch.arange(m), t - (rows - last)] -= 1
+        want = P.T @ h.double()
+        bound = 1.01 * ((dP + (2.0 ** -8 + 2.0 ** -18) * P.abs()).T @ h.double().abs()) + (m / 16 + 2) * 2.0 ** -22 * (P.abs().T @ h.double().abs())
+        assert ((dw - want).abs() <= bound + 2.0 ** -8 * want.abs() + 2.0 ** -133).all()

@@ -173,3 +173,18 @@ def test_nothing_is_written_beside_the_results(m, n, k, shift, dtype):
     got = y[0][y[2]:y[2] + y[3]].clone().view(dtype).view(m, n)
     assert torch.equal(got, lm_ops.linear_mxfp4(x, q))
     assert torch.equal(v[0][v[2]:v[2] + v[3]].clone().view(dtype).view(m, k), lm_ops.quantize_mxfp4(x).dequantize(dtype))
+
+
+def test_offsets_past_32_bits():
+    """A matrix of 2^31 numbers and some: its last rows have the values, and the products, that they have alone."""
+    from dia_tts_prune_b200.lm_ops import linear_mxfp4, quantize_mxfp4
+    g = torch.Generator(device="cuda").manual_seed(2)
+    rows, k, last = 270000, 8192, 432                              # (270000 is 2109 blocks of 128 and 48: the last 432 rows begin a block)
+    x = torch.empty(rows, k, dtype=torch.bfloat16, device="cuda").normal_(generator=g)
+    q, alone = quantize_mxfp4(x), quantize_mxfp4(x[-last:])
+    assert torch.equal(q.dequantize(torch.bfloat16)[-last:], alone.dequantize(torch.bfloat16))
+    for m in (2, 40, 300):
+        a = torch.randn(m, k, generator=g, device="cuda").bfloat16()
+        assert torch.equal(linear_mxfp4(a, q)[:, -last:], linear_mxfp4(a, alone))
+    w = quantize_mxfp4(torch.randn(8200, k, generator=g, device="cuda"))
+    assert torch.equal(linear_mxfp4(x, w)[-last:], linear_mxfp4(x[-last:], w))
