@@ -285,10 +285,11 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
             if (p.count) factor /= fmaxf(*p.count, 1.f);
         }
         unsigned it = 0;
-        const auto taken = [&]() {                            // this warp has read the accumulator
+        // this warp has read the accumulator (relaxed: a release would wait for the warp's stores to be seen, whose addresses the MMAs have nothing to do with)
+        const auto taken = [&]() {
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
-            if (lane == 0) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(at_rank(&t_empty[it & 1u], 0)) : "memory");
+            if (lane == 0) asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(at_rank(&t_empty[it & 1u], 0)) : "memory");
             ++it;
         };
         Tile t;
@@ -358,12 +359,13 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                 if (!ok) base = own = CUDART_NAN_F;
 #pragma unroll 1
                 for (int cb = 0; cb < 2; ++cb) {              // (128 columns at a time, half of them here)
-                    if (rows <= 0) break;
                     const int c0 = t.n * kTileN + cb * 128, mine0 = c0 + half * 64;
                     uint32_t v[2][32], y[32];
                     tmem_columns32(tile_at() + cb * 128 + half * 64, v[0]);
                     tmem_columns32(tile_at() + cb * 128 + half * 64 + 32, v[1]);
                     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                    if (cb == 1) taken();
+                    if (rows <= 0) continue;
                     const int at = target - mine0;
 #pragma unroll
                     for (int e = 0; e < 32; ++e) {
@@ -384,7 +386,6 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                     }
                     store_128(panel, y, p.p, p.ldp, row0, rows, c0, 128, true, q, half, lane);
                 }
-                taken();
             } else if (!t.head) {
                 const int rr = lane >> 3, ch = lane & 7;
                 float* const acc = p.acc + (size_t)t.share * of.M * p.ld_acc;
@@ -392,10 +393,11 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
 #pragma unroll 1
                 for (int cb = 0; cb < 4; ++cb) {
                     const int n = n0 + cb * 32 + 4 * ch;
-                    if (n0 + cb * 32 >= p.ld_acc || rows <= 0) break;
                     uint32_t v[32];
                     tmem_columns32(from() + cb * 32, v);
                     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                    if (cb == 3) taken();
+                    if (n0 + cb * 32 >= p.ld_acc || rows <= 0) continue;
 #pragma unroll
                     for (int c = 0; c < 8; ++c)
                         *reinterpret_cast<uint4*>(blk + lane * 128 + ((c ^ (lane & 7)) << 4)) = make_uint4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
@@ -416,18 +418,18 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                     __syncwarp();
                 }
                 panel_sync(q);                                // (the other warp's share is a panel's too)
-                taken();
             } else {
                 wait();
                 if (!ok) factor = CUDART_NAN_F;
 #pragma unroll 1
                 for (int cb = 0; cb < 2; ++cb) {
                     const int c0 = t.n * kTileN + cb * 128;
-                    if (c0 >= of.N || rows <= 0) break;
                     uint32_t v[2][32], y[32];
                     tmem_columns32(tile_at() + cb * 128 + half * 64, v[0]);
                     tmem_columns32(tile_at() + cb * 128 + half * 64 + 32, v[1]);
                     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                    if (cb == 1) taken();
+                    if (c0 >= of.N || rows <= 0) continue;
 #pragma unroll
                     for (int e = 0; e < 32; ++e) {
                         const __nv_bfloat162 b = __floats2bfloat162_rn(__uint_as_float(v[e >> 4][2 * e & 31]) * factor, __uint_as_float(v[e >> 4][(2 * e & 31) + 1]) * factor);
@@ -435,7 +437,6 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                     }
                     store_128(panel, y, p.out, of.N, row0, rows, c0, of.N - c0, p.wide, q, half, lane);
                 }
-                taken();
             }
         }
     }

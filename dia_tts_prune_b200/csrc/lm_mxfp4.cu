@@ -253,36 +253,34 @@ __device__ __forceinline__ uint32_t pack16(int type, float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
 }
-// A panel of an accumulator (from: its first column of the warp's 32 rows; `width` columns are there) to rows row0 .. and columns n0 .. of the result, by the two warps of a
-// quarter.
+// The warp's half of a panel of an accumulator (from: its first column of the warp's 32 rows)
 template <int TYPE>
-__device__ __forceinline__ void take_out(uint32_t from, int width, unsigned char* panel, const TiledProduct& p, int row0, int rows, int n0, int quarter, int half, int lane, bool ok,
-                                         bool wide) {
-    uint32_t w[32];
-    if (half * (Out<TYPE>::kPanel / 2) < width) {
-        if constexpr (TYPE == kTypeF32) {
-            tmem_columns32(from + 32 * half, w);
-            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-        } else {
-            uint32_t v[2][32];
-            tmem_columns32(from + 64 * half, v[0]);
-            tmem_columns32(from + 64 * half + 32, v[1]);
-            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+__device__ __forceinline__ void panel_half(uint32_t from, int half, uint32_t (&w)[32]) {
+    if constexpr (TYPE == kTypeF32) {
+        tmem_columns32(from + 32 * half, w);
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+    } else {
+        uint32_t v[2][32];
+        tmem_columns32(from + 64 * half, v[0]);
+        tmem_columns32(from + 64 * half + 32, v[1]);
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-            for (int e = 0; e < 32; ++e) w[e] = pack16(TYPE, __uint_as_float(v[e >> 4][2 * e & 31]), __uint_as_float(v[e >> 4][(2 * e & 31) + 1]));
-        }
-        if (!ok) {
-#pragma unroll
-            for (int e = 0; e < 32; ++e) w[e] = TYPE == kTypeF16 ? 0x7e007e00u : 0x7fff7fffu;                     // (no result: NaN as one number or two)
-        }
-        fill_panel(panel, half, w, lane);
+        for (int e = 0; e < 32; ++e) w[e] = pack16(TYPE, __uint_as_float(v[e >> 4][2 * e & 31]), __uint_as_float(v[e >> 4][(2 * e & 31) + 1]));
     }
+}
+// The warp's half (w) of a panel to rows row0 .. and columns n0 .. of the result, by the two warps of a quarter.
+template <int TYPE>
+__device__ __forceinline__ void put_out(uint32_t (&w)[32], unsigned char* panel, const TiledProduct& p, int row0, int rows, int n0, int quarter, int half, int lane, bool ok, bool wide) {
+    if (!ok) {
+#pragma unroll
+        for (int e = 0; e < 32; ++e) w[e] = TYPE == kTypeF16 ? 0x7e007e00u : 0x7fff7fffu;                         // (no result: NaN as one number or two)
+    }
+    fill_panel(panel, half, w, lane);
     panel_sync(quarter);
     const size_t pitch = (size_t)p.N * Out<TYPE>::kBytes;
-    store_panel<Out<TYPE>::kBytes>(panel, reinterpret_cast<char*>(p.y) + (row0 * pitch + (size_t)n0 * Out<TYPE>::kBytes), pitch, half, rows, min(width, p.N - n0), wide, lane);
+    store_panel<Out<TYPE>::kBytes>(panel, reinterpret_cast<char*>(p.y) + (row0 * pitch + (size_t)n0 * Out<TYPE>::kBytes), pitch, half, rows, min(Out<TYPE>::kPanel, p.N - n0), wide, lane);
     panel_sync(quarter);
 }
-
 template <int TYPE>
 __device__ __forceinline__ bool whole_pieces(const TiledProduct& p) { return p.N * Out<TYPE>::kBytes % 16 == 0 && (reinterpret_cast<uintptr_t>(p.y) & 15) == 0; }
 
@@ -396,8 +394,11 @@ mxfp4_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
             ok = ok && pair_wait(&t_full[it & 1u], (it >> 1) & 1u, p.polls);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
-            for (int c = 0; c < kBN && n0 + c < p.N && rows > 0; c += Out<TYPE>::kPanel)
-                take_out<TYPE>(tmem + ((uint32_t)(q * 32) << 16) + (it & 1u) * kBN + c, kBN - c, panel, p, row0, rows, n0 + c, q, half, lane, ok, wide);
+            for (int c = 0; c < kBN && n0 + c < p.N && rows > 0; c += Out<TYPE>::kPanel) {
+                uint32_t w[32];
+                panel_half<TYPE>(tmem + ((uint32_t)(q * 32) << 16) + (it & 1u) * kBN + c, half, w);
+                put_out<TYPE>(w, panel, p, row0, rows, n0 + c, q, half, lane, ok, wide);
+            }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive(&t_empty[it & 1u]);
@@ -416,15 +417,16 @@ mxfp4_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
     }
 }
 
-// The same on pairs of SMs: a cluster of two CTAs owns a 256 x 192 tile, an MMA of the pair multiplies the 256 rows of both by the 192 columns of both, so an SM takes 28 KB
-// of codes from L2 for 384 cycles of MMAs where the kernel above takes 32 KB for 256.  192 columns: two accumulators leave 128 columns of tensor memory for scales.  Each
-// SM needs the scales of its own 128 rows and of all 192 columns; those of an odd tile begin half way into a block of 128, two columns further.
+// The same on pairs of SMs: a cluster of two CTAs owns a 256 x 256 tile, an MMA of the pair multiplies the 256 rows of both by the 256 columns of both, so an SM takes 32 KB
+// of codes from L2 for 512 cycles of MMAs where the kernel above takes as much for 256.  Each SM needs the scales of its own 128 rows and of all 256 columns.  Two accumulators
+// and the scales of two stages are 576 columns of tensor memory, which has 512: the second accumulator begins on the last 64 columns of the first, and whichever is taken out
+// hands these over first.  (192 columns a tile, accumulators apart: 4096 x 16384 x 4096 133 us here 104, 2048 channels 75 / 60.)
 //   warp 0    one lane per CTA: codes and scales (TMA) of its halves; every byte of both CTAs counts on the leader's barrier
 //   warp 1    leader only: a stage's scales into the tensor memory of both, then the pair's MMAs; commits to the barriers of both
 //   warps 2-9 take the CTA's 128 rows of a finished accumulator out
-// Bound: what the SMs take from L2, 11 TB/s (4096 x 16384 x 4096, us: 124; without MMAs 128 of then 132, without the copies of scales into tensor memory 131, without loading
-// scales 104 - two pieces of 512 bytes at a time they were three loads a stage, and 132 - without taking results out 127).
-constexpr int kPairN = 192, kPairStages = 6, kPairWarps = 8, kPairThreads = 64 + 32 * kPairWarps;
+// Bound: what the SMs take from L2, 12 TB/s (4096 x 16384 x 4096, us with 8 of waiting for the rows: 104; without MMAs 96, without loading scales 97, without taking results
+// out 98).
+constexpr int kPairN = 256, kPairShift = 192, kPairStages = 5, kPairWarps = 8, kPairThreads = 64 + 32 * kPairWarps;
 constexpr int kPairCodes = kCodeTile + kPairN / 2 * 128, kPairStage = kPairCodes + 3 * 1024;
 constexpr int kPairSmem = kPairStages * kPairStage + kPairWarps * 4096 + 1024 + 256;
 static_assert(kPairStage % 1024 == 0 && kPairSmem <= 227 * 1024, "shared memory");
@@ -451,7 +453,8 @@ mxfp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
     uint64_t* full = reinterpret_cast<uint64_t*>(turn + kPairWarps * 4096);  // (the leader's alone)
     uint64_t* empty = full + kPairStages;
     uint64_t* t_full = empty + kPairStages;
-    uint64_t* t_empty = t_full + 2;                                          // (the leader's alone)
+    uint64_t* t_early = t_full + 2;                                          // (these two the leader's alone)
+    uint64_t* t_empty = t_early + 2;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(t_empty + 2);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = blockIdx.x & 1;
@@ -461,7 +464,7 @@ mxfp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < kPairStages; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
-        for (int i = 0; i < 2; ++i) { mbar_init(&t_full[i], 1); mbar_init(&t_empty[i], 2 * kPairWarps); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&t_full[i], 1); mbar_init(&t_early[i], 2 * kPairWarps); mbar_init(&t_empty[i], 2 * kPairWarps); }
         fence_mbar_init();
     }
     if (warp == 1) {
@@ -517,16 +520,16 @@ mxfp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
             const uint32_t two = mx_idesc(kPairN, 0) ^ (3u << 27), idesc[2] = {two, two | (mx_idesc(0, 1) ^ mx_idesc(0, 0))};      // M = 256
             unsigned i = 0, it = 0;
             for (int t = pair; t < n_tiles && ok; t += pairs, ++it) {
-                if (!pair_wait(&t_empty[it & 1u], ((it >> 1) & 1u) ^ 1u, p.polls)) { ok = false; break; }
+                if (!pair_wait(&t_empty[it & 1u], ((it >> 1) & 1u) ^ 1u, p.polls) || (it && !pair_wait(&t_early[(it & 1u) ^ 1u], ((it - 1) >> 1) & 1u, p.polls))) { ok = false; break; }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint32_t d = tmem + (it & 1u) * kPairN, shift = t / tiles_m & 1 ? 2 : 0;
+                const uint32_t d = tmem + (it & 1u) * kPairShift;
                 for (int s = 0; s < n_stage; ++s, ++i) {
                     const unsigned at = i % kPairStages;
                     if (!pair_wait(&full[at], (i / kPairStages) & 1u, p.polls)) { ok = false; break; }
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     const uint32_t base = smem_u32(smem + at * kPairStage);
                     const uint64_t adesc = umma_desc(base), bdesc = umma_desc(base + kCodeTile);
-                    const uint32_t sa = tmem + 2 * kPairN + (i & 3u) * 32, sb = sa + 8;
+                    const uint32_t sa = tmem + kPairShift + kPairN + (i & 1u) * 32, sb = sa + 8;
                     const int here = min(2, pieces - 2 * s);
                     if (elect_one_sync()) {
                         for (int c = 0; c < here; ++c) {
@@ -537,7 +540,7 @@ mxfp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                         for (int c = 0; c < here; ++c)
 #pragma unroll
                             for (int j = 0; j < 2; ++j)
-                                umma_mxfp4_pair(d, adesc + 4 * c + 2 * j, bdesc + 4 * c + 2 * j, idesc[j], sa + 4 * c, sb + 8 * c + shift, (s | c | j) != 0 ? 1u : 0u);
+                                umma_mxfp4_pair(d, adesc + 4 * c + 2 * j, bdesc + 4 * c + 2 * j, idesc[j], sa + 4 * c, sb + 8 * c, (s | c | j) != 0 ? 1u : 0u);
                         umma_commit_pair(&empty[at]);
                         if (s == n_stage - 1) umma_commit_pair(&t_full[it & 1u]);
                     }
@@ -549,17 +552,29 @@ mxfp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
         const int q = warp & 3, half = (warp - 2) >> 2;
         unsigned char* const panel = turn + q * kPanelBytes;
         const bool wide = whole_pieces<TYPE>(p);
+        constexpr int kPanels = kPairN / Out<TYPE>::kPanel;
         unsigned it = 0;
         for (int t = pair; t < n_tiles; t += pairs, ++it) {
             const int n0 = t / tiles_m * kPairN, row0 = t % tiles_m * 256 + (int)rank * 128 + q * 32, rows = min(32, p.M - row0);
             ok = ok && pair_wait(&t_full[it & 1u], (it >> 1) & 1u, p.polls);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            // (relaxed: a release would wait for this warp's stores of earlier tiles to be seen, with which the MMAs have nothing to do; 1024 channels took 66 us, not 46)
+            const auto taken = [&](uint64_t* bar) {
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(at_rank(bar, 0)) : "memory");
+            };
+            // the panel that the next tile's accumulator lies on goes first
 #pragma unroll 1
-            for (int c = 0; c < kPairN && n0 + c < p.N && rows > 0; c += Out<TYPE>::kPanel)
-                take_out<TYPE>(tmem + ((uint32_t)(q * 32) << 16) + (it & 1u) * kPairN + c, kPairN - c, panel, p, row0, rows, n0 + c, q, half, lane, ok, wide);
-            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(at_rank(&t_empty[it & 1u], 0)) : "memory");
+            for (int i = 0; i < kPanels; ++i) {
+                const int c = (it & 1u ? i : kPanels - 1 - i) * Out<TYPE>::kPanel;
+                const bool there = n0 + c < p.N && rows > 0;
+                uint32_t w[32];
+                if (there) panel_half<TYPE>(tmem + ((uint32_t)(q * 32) << 16) + (it & 1u) * kPairShift + c, half, w);
+                if (i == 0) taken(&t_early[it & 1u]);
+                if (i == kPanels - 1) taken(&t_empty[it & 1u]);
+                if (there) put_out<TYPE>(w, panel, p, row0, rows, n0 + c, q, half, lane, ok, wide);
+            }
         }
     }
     if (!ok && lane == 0 && p.ran_out) {
@@ -776,8 +791,9 @@ bool scales_map(CUtensorMap* map, const void* scales, int rows, int K, int block
                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Whether pairs of SMs are the shorter way: rounds of tiles times what a tile takes, in us.  Measured, a stage of 256 channels of a 128 x 128 tile 0.40, of a 256 x 192 tile of a
-// pair 0.45, taking a tile out 1.0 and 2.4 (4096 x 16384, both kernels: 4096 channels 179 / 134, 256 channels 29 / 45; 1024 x 8192 x 2048 15 / 13, 512 x 8192 x 2048 9 / 10).
+// Whether pairs of SMs are the shorter way: rounds of tiles times what a tile takes, in us.  Measured, a stage of 256 channels of a 128 x 128 tile 0.40, of a 256 x 256 tile of a
+// pair 0.45, taking a tile out 1.0 and 2.4 (4096 x 16384, with the rounding of the rows, tiles of one SM / of pairs: 4096 channels 189 / 115, 1024 57 / 46, 256 35 / 40;
+// 1000 x 8192 x 2048 20 / 17, 200 x 32768 x 256 11.3 / 11.8).
 bool on_pairs(int M, int N, int K, int sms) {
     const long long single = ((M + 127LL) / 128 * ((N + 127LL) / 128) + sms - 1) / sms, pairs = ((M + 255LL) / 256 * ((N + kPairN - 1LL) / kPairN) + sms / 2 - 1) / (sms / 2);
     const double stages = (K + kStageK - 1) / kStageK;
