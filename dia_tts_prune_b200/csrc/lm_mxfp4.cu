@@ -24,16 +24,23 @@ using namespace dia;
 // ---- rounding and values -------------------------------------------------------------------------------------------------------------------
 
 // Eight neighbouring channels of a row as they lie in memory.  WIDE: rows of whole 16 bytes whose channels are a multiple of eight, all eight are there or none; else those
-// at or beyond `n` are zero.  (Fetching and widening are apart: widened at once, a load is waited for before the next one goes out.)
-template <int TYPE, bool WIDE>
+// at or beyond `n` are zero.  ONCE: an SM reads them once, so that L1 does without them (32768 x 2048 fp32 rounded in 42 us, not 48).  (Fetching and widening are apart:
+// widened at once, a load is waited for before the next one goes out.)
+template <int TYPE, bool WIDE, bool ONCE>
 struct Eight {
+    static __device__ __forceinline__ uint4 load(const uint4* p) {
+        if constexpr (!ONCE) return __ldg(p);
+        uint4 v;
+        asm("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+        return v;
+    }
     uint4 w[TYPE == kTypeF32 ? 2 : 1];
     __device__ __forceinline__ void fetch(const void* row, int k, int n) {
         constexpr int kWords = TYPE == kTypeF32 ? 2 : 1;
         if constexpr (WIDE) {
 #pragma unroll
             for (int i = 0; i < kWords; ++i)
-                w[i] = n > 0 ? __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(row) + (size_t)k * (TYPE == kTypeF32 ? 4 : 2)) + i) : make_uint4(0u, 0u, 0u, 0u);
+                w[i] = n > 0 ? load(reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(row) + (size_t)k * (TYPE == kTypeF32 ? 4 : 2)) + i) : make_uint4(0u, 0u, 0u, 0u);
         } else {
             uint32_t u[4 * kWords];
 #pragma unroll
@@ -95,11 +102,11 @@ __device__ __forceinline__ uint32_t round_block(const float (&v)[8], uint32_t& s
     return codes;
 }
 
-// A CTA takes 128 rows x 256 channels, a warp 16 rows of them, a lane eight channels (four neighbours a block): kAhead rows are on their way at a time, and the scales
-// leave as the two pieces that they are.  early: the successor, a product of these rows, may start now (a product asks for its weights before
-// this kernel has ended: they are never what it writes).  Rows behind the last one of a piece get scales of zero.  Bound: memory (32768 x 2048 bf16, 170 MB: 75 us with an index per eight
-// channels, whose scales went out byte by byte).
-constexpr int kQuantThreads = 256, kAhead = 8;
+// A CTA takes 128 rows x 256 channels, a warp 16 rows of them, a lane eight channels (four neighbours a block): kAhead rows are on their way at a time, eight loads, and the
+// scales leave as the two pieces that they are.  early: the successor, a product of these rows, may start now (a product asks for its weights before this kernel has ended:
+// they are never what it writes).  Rows behind the last one of a piece get scales of zero.  Bound: memory, instructions next (32768 x 2048 bf16, 170 MB: 31 us; 75 with an index
+// per eight channels, whose scales went out byte by byte; fp32, 304 MB: 42, and 48 with eight rows on their way, whose registers leave fewer warps).
+constexpr int kQuantThreads = 256;
 template <int TYPE, bool WIDE>
 __global__ void __launch_bounds__(kQuantThreads) mxfp4_quantize_kernel(const void* __restrict__ x, long long ld, int rows, int K, uint32_t* __restrict__ codes,
                                                                        uint8_t* __restrict__ scales, int early) {
@@ -108,9 +115,10 @@ __global__ void __launch_bounds__(kQuantThreads) mxfp4_quantize_kernel(const voi
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, pieces = (K + 127) / 128, c0 = blockIdx.x * 32 + lane, k = 8 * c0;
     const long long row0 = (long long)blockIdx.y * 128 + warp * 16;
     const bool kept = c0 < pieces * 16;                       // (a row's codes go on to the end of its last piece)
+    constexpr int kAhead = TYPE == kTypeF32 ? 4 : 8;
 #pragma unroll
     for (int r0 = 0; r0 < 16; r0 += kAhead) {
-        Eight<TYPE, WIDE> x8[kAhead];
+        Eight<TYPE, WIDE, true> x8[kAhead];
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) {
             const long long r = row0 + r0 + j;
@@ -658,7 +666,7 @@ __global__ void __launch_bounds__(kFewThreads, 2) mxfp4_few_rows_kernel(const __
         constexpr int TYPE = decltype(type)::value, kBatch = TYPE == kTypeF32 ? 6 : 8;
         constexpr bool WIDE = decltype(wide)::value;
         for (int i0 = tid; i0 < items; i0 += kFewThreads * kBatch) {           // (a warp is in or out as a whole)
-            Eight<TYPE, WIDE> x8[kBatch];
+            Eight<TYPE, WIDE, false> x8[kBatch];
 #pragma unroll
             for (int b = 0; b < kBatch; ++b) {
                 const int i = i0 + b * kFewThreads, m = i / per_row, k = s0 * kStageK + 8 * (i - m * per_row);
