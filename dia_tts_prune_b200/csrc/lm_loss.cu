@@ -900,7 +900,8 @@ Room room_of(const LossShape& s, bool grad, bool rows, bool head) {
         // shares of dh's contraction where its tiles leave most of the chip idle
         const long long tiles = (long long)((s.M + 255) / 256) * ((s.K + 255) / 256);
         while (r.splits < 16 && 2 * r.splits * tiles <= 74 && r.piece / kBK >= 16 * r.splits) r.splits *= 2;
-        r.splits = shares_of(r.piece, r.splits);
+        // (of the columns that are there, not of the padded piece: the first piece writes every share, later ones add to the first of them)
+        r.splits = shares_of(std::min(r.piece, s.V), r.splits);
         r.p = take((size_t)s.M * r.piece * 2);
         r.acc = take(rows ? (size_t)r.splits * s.M * ((s.K + 3) / 4 * 4) * 4 : 0);
     }
@@ -1011,7 +1012,8 @@ cudaError_t launch_loss_grad(const LossShape& s, const float* kept, const LossGr
         LossTiles q = tiles_of(s);
         q.v0 = v0;
         if (dh) {
-            q.own.M = s.M; q.own.N = s.K; q.own.K = cols; q.own.splits = shares_of(cols, r.splits);
+            q.own.M = s.M; q.own.N = s.K; q.own.K = cols;
+            q.own.splits = v0 ? shares_of(cols, r.splits) : r.splits;
             q.acc = acc; q.ld_acc = ld_acc; q.add = v0 > 0;
         }
         if (dw) {

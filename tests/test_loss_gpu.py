@@ -305,3 +305,38 @@ def test_offsets_past_32_bits():
         want = P.T @ h.double()
         bound = 1.01 * ((dP + (2.0 ** -8 + 2.0 ** -18) * P.abs()).T @ h.double().abs()) + (m / 16 + 2) * 2.0 ** -22 * (P.abs().T @ h.double().abs())
         assert ((dw - want).abs() <= bound + 2.0 ** -8 * want.abs() + 2.0 ** -133).all()
+
+
+@pytest.mark.parametrize("m,v,k", [(129, 8500, 1000), (40, 8449, 64), (1, 9473, 96), (256, 14400, 512), (1000, 13313, 200), (3, 12290, 4)])
+def test_every_share_of_the_rows_gradient_is_written(m, v, k):
+    """The gradient by the rows is a sum of shares of the vocabulary.  These end short of a whole piece of it, so that dividing the piece and
+    dividing the columns that are there give different numbers of shares; the workspace holds NaN beforehand."""
+    from dia_tts_prune_b200 import _lm_lib
+    from dia_tts_prune_b200.lm_ops import linear_cross_entropy
+    lib, st = _lm_lib.load(), torch.cuda.current_stream().cuda_stream
+    h, w, t = operands(m, v, k, m + v)
+    e = Exact(h, w, t, 0.5)
+    n = max(int(e.keep.sum()), 1)
+    (want_h, off_h), (want_w, off_w) = e.gradient(torch.full((m,), 1.0 / n))
+    ld = (k + 7) // 8 * 8
+    a, b = (torch.nn.functional.pad(x, (0, ld - k)) for x in (h, w))
+    kept, out = torch.empty(2 * m + 1, device="cuda"), torch.empty((), device="cuda")
+    need = lib.lm_b200_op_loss_work_bytes(a.data_ptr(), 1, ld, b.data_ptr(), ld, m, v, k)
+    work = torch.full((need,), 255, dtype=torch.uint8, device="cuda")
+    assert lib.lm_b200_op_loss(a.data_ptr(), 1, ld, b.data_ptr(), ld, t.data_ptr(), 1, -100, m, v, k, 0.5, 2, out.data_ptr(), kept.data_ptr(), work.data_ptr(), need, st) == 0
+    one = torch.ones((), device="cuda")
+    for rows, head in ((True, True), (True, False), (False, True)):
+        dh, dw = (torch.full(s, math.nan, dtype=torch.bfloat16, device="cuda") for s in ((m, k), (v, k)))
+        need = lib.lm_b200_op_loss_grad_work_bytes(a.data_ptr(), ld, b.data_ptr(), ld, m, v, k, rows, head)
+        work = torch.full((need,), 255, dtype=torch.uint8, device="cuda")
+        assert lib.lm_b200_op_loss_grad(a.data_ptr(), ld, b.data_ptr(), ld, t.data_ptr(), 1, -100, m, v, k, 0.5, kept.data_ptr(), one.data_ptr(), 0, kept.data_ptr() + 8 * m,
+                                        dh.data_ptr() if rows else None, dw.data_ptr() if head else None, work.data_ptr(), need, st) == 0
+        if rows:
+            within(dh, want_h, off_h)
+        if head:
+            within(dw, want_w, off_w)
+    # and as a program calls it, behind others whose workspaces it takes over
+    x, y = h.requires_grad_(True), w.requires_grad_(True)
+    for _ in range(3):
+        torch.full((need,), 255, dtype=torch.uint8, device="cuda")
+        within(torch.autograd.grad(linear_cross_entropy(x, y, t, scale=0.5), x)[0], want_h, off_h)
