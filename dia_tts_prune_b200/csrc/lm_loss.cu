@@ -156,7 +156,9 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
     uint64_t* empty = full + kStagesMost;
     uint64_t* t_full = empty + kStagesMost;
     uint64_t* t_empty = t_full + 2;                                          // (the leader's alone)
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(t_empty + 2);
+    PairEnd* end = reinterpret_cast<PairEnd*>(t_empty + 2);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(end + 1);
+    static_assert((2 * kStagesMost + 4) * 8 + sizeof(PairEnd) + 4 <= 256, "barrier region");
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = PAIR ? blockIdx.x & 1 : 0;
@@ -168,6 +170,7 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
     if (threadIdx.x == 0) {
         for (int i = 0; i < kStages; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
         for (int i = 0; i < 2; ++i) { mbar_init(&t_full[i], 1); mbar_init(&t_empty[i], (PAIR ? 2 : 1) * kWarps); }
+        pair_begin(end);
         fence_mbar_init();
     }
     if (warp == 1) {
@@ -225,8 +228,8 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
             }
             // (the leader's last commits arrive here: not after this CTA has gone)
             for (unsigned j = i > (unsigned)kStages ? i - kStages : 0; j < i && ok; ++j) ok = lane_wait(&empty[j % kStages], (j / kStages) & 1u, p.polls);
-            // (nor do copies arrive that were issued before a wait ran out)
-            for (unsigned j = i > (unsigned)kStages ? i - kStages : 0; j < i && !ok && rank == 0; ++j) (void)lane_wait(&full[j % kStages], (j / kStages) & 1u, p.polls);
+            if constexpr (PAIR) pair_issued(end, rank, i);
+            else copies_landed(full, kStages, i);
         }
     } else if (warp == 1) {
         if (rank == 0) {
@@ -273,6 +276,7 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                     if (last) ++it;
                 }
             }
+            mmas_ended<PAIR>(&end->done);
         }
     } else {
         const int q = warp & 3, c_half = (warp - 2) >> 2 << 7;               // (a warp reads the 32 lanes of its number mod 4) and its half of the columns
@@ -440,13 +444,18 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
             }
         }
     }
-    if (!ok && lane == 0 && p.ran_out) {
-        *reinterpret_cast<volatile int*>(p.ran_out) = 1;
-        __threadfence_system();
+    if (!ok && lane == 0) {
+        if constexpr (PAIR) pair_gave_up(end);
+        if (p.ran_out) {
+            *reinterpret_cast<volatile int*>(p.ran_out) = 1;
+            __threadfence_system();
+        }
     }
     __syncwarp();
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-    everyone();                                               // neither CTA's memory goes while the other still reads it or arrives there
+    // neither CTA's memory goes while the other still reads it or arrives there
+    if constexpr (PAIR) pair_end(end, rank, full, kStages, kStage);
+    else __syncthreads();
     if (warp == 1) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512));
@@ -476,7 +485,7 @@ __global__ void __launch_bounds__(kFewThreads, 2) loss_few_rows_kernel(const __g
     constexpr int kCols = Few<NB, TERMS>::kCols, kSlot = Few<NB, TERMS>::kSlot, kSlots = Few<NB, TERMS>::kSlots;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    __shared__ uint64_t full[kSlots], empty[kSlots], t_full[2], t_empty[2];
+    __shared__ uint64_t full[kSlots], empty[kSlots], t_full[2], t_empty[2], done;
     __shared__ uint32_t tmem_slot;
     __shared__ int targets[NB];
     __shared__ float2 meet[4][NB];
@@ -498,6 +507,7 @@ __global__ void __launch_bounds__(kFewThreads, 2) loss_few_rows_kernel(const __g
     if (tid == 0) {
         for (int i = 0; i < kSlots; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
         for (int i = 0; i < 2; ++i) { mbar_init(&t_full[i], 1); mbar_init(&t_empty[i], 4); }
+        mbar_init(&done, 1);
         fence_mbar_init();
     }
     // (the head may be what the predecessor writes: a gradient, another product's result)
@@ -529,8 +539,7 @@ __global__ void __launch_bounds__(kFewThreads, 2) loss_few_rows_kernel(const __g
                 row_tile(slot, kb);
                 next();
             }
-            // (copies in flight arrive before the CTA goes)
-            for (int j = max(0, i - kSlots); j < i && !ok; ++j) (void)lane_wait(&full[j % kSlots], (j / kSlots) & 1u, p.polls);
+            copies_landed(full, kSlots, i);
         }
     } else if (warp == 1) {
         const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(kCols >> 3) << 17) | (8u << 24);
@@ -554,6 +563,7 @@ __global__ void __launch_bounds__(kFewThreads, 2) loss_few_rows_kernel(const __g
             __syncwarp();
             if (last) ++it;
         }
+        mmas_ended<false>(&done);
     } else {
         const int q = warp & 3, c = q * 32 + lane;
         float most[NB], sum[NB];                              // of c z, of 2^(c z - most)

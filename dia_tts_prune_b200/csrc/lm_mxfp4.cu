@@ -306,7 +306,8 @@ mxfp4_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
     uint64_t* empty = full + kStages;
     uint64_t* t_full = empty + kStages;
     uint64_t* t_empty = t_full + 2;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(t_empty + 2);
+    uint64_t* done = t_empty + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int pieces = (p.K + 127) / 128, n_stage = (pieces + 1) / 2;
     const int tiles_m = (p.M + kBM - 1) / kBM, n_tiles = tiles_m * ((p.N + kBN - 1) / kBN);
@@ -314,6 +315,7 @@ mxfp4_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
     if (threadIdx.x == 0) {
         for (int i = 0; i < kStages; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
         for (int i = 0; i < 2; ++i) { mbar_init(&t_full[i], 1); mbar_init(&t_empty[i], kWarps4); }
+        mbar_init(done, 1);
         fence_mbar_init();
     }
     if (warp == 1) {
@@ -359,8 +361,7 @@ mxfp4_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
                 weights(at, t, s);
                 rows(at, t, s);
             }
-            // (copies in flight arrive before the CTA goes)
-            for (unsigned j = i > (unsigned)kStages ? i - kStages : 0; j < i && !ok; ++j) (void)lane_wait(&full[j % kStages], (j / kStages) & 1u, p.polls);
+            copies_landed(full, kStages, i);
         }
     } else if (warp == 1) {
         const uint32_t idesc[2] = {mx_idesc(kBN, 0), mx_idesc(kBN, 1)};
@@ -392,6 +393,7 @@ mxfp4_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
                 __syncwarp();
             }
         }
+        mmas_ended<false>(done);
     } else {
         const int q = warp & 3, half = (warp - 2) >> 2;       // (a warp reads the 32 lanes of its number mod 4)
         unsigned char* const panel = turn + q * kPanelBytes;
@@ -463,7 +465,9 @@ mxfp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
     uint64_t* t_full = empty + kPairStages;
     uint64_t* t_early = t_full + 2;                                          // (these two the leader's alone)
     uint64_t* t_empty = t_early + 2;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(t_empty + 2);
+    PairEnd* end = reinterpret_cast<PairEnd*>(t_empty + 2);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(end + 1);
+    static_assert((2 * kPairStages + 6) * 8 + sizeof(PairEnd) + 4 <= 256, "barrier region");
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = blockIdx.x & 1;
     const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
@@ -473,6 +477,7 @@ mxfp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
     if (threadIdx.x == 0) {
         for (int i = 0; i < kPairStages; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
         for (int i = 0; i < 2; ++i) { mbar_init(&t_full[i], 1); mbar_init(&t_early[i], 2 * kPairWarps); mbar_init(&t_empty[i], 2 * kPairWarps); }
+        pair_begin(end);
         fence_mbar_init();
     }
     if (warp == 1) {
@@ -519,9 +524,7 @@ mxfp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
             }
             // (the leader's last commits arrive here: not after this CTA has gone)
             for (unsigned j = i > (unsigned)kPairStages ? i - kPairStages : 0; j < i && ok; ++j) ok = lane_wait(&empty[j % kPairStages], (j / kPairStages) & 1u, p.polls);
-            // (nor do copies arrive that were issued before a wait ran out)
-            for (unsigned j = i > (unsigned)kPairStages ? i - kPairStages : 0; j < i && !ok && rank == 0; ++j)
-                (void)lane_wait(&full[j % kPairStages], (j / kPairStages) & 1u, p.polls);
+            pair_issued(end, rank, i);
         }
     } else if (warp == 1) {
         if (rank == 0) {
@@ -555,6 +558,7 @@ mxfp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                     __syncwarp();
                 }
             }
+            mmas_ended<true>(&end->done);
         }
     } else {
         const int q = warp & 3, half = (warp - 2) >> 2;
@@ -585,13 +589,16 @@ mxfp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
             }
         }
     }
-    if (!ok && lane == 0 && p.ran_out) {
-        *reinterpret_cast<volatile int*>(p.ran_out) = 1;
-        __threadfence_system();
+    if (!ok && lane == 0) {
+        pair_gave_up(end);
+        if (p.ran_out) {
+            *reinterpret_cast<volatile int*>(p.ran_out) = 1;
+            __threadfence_system();
+        }
     }
     __syncwarp();
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-    cluster_sync_all();                                       // neither CTA's memory goes while the other still reads it or arrives there
+    pair_end(end, rank, full, kPairStages, kPairStage);       // neither CTA's memory goes while the other still reads it or arrives there
     if (warp == 1) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
@@ -633,7 +640,7 @@ __global__ void __launch_bounds__(kFewThreads, 2) mxfp4_few_rows_kernel(const __
     constexpr int kSlot = kCodeTile + 1024, kRows = NB * 128 + 1024;       // a stage of weights, of rows
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    __shared__ uint64_t full[kFewSlotsMost], empty[kFewSlotsMost], t_full;
+    __shared__ uint64_t full[kFewSlotsMost], empty[kFewSlotsMost], t_full, done;
     __shared__ uint32_t tmem_slot;
     unsigned char* const ring = smem;
     unsigned char* const rows = ring + p.slots * kSlot;                     // [per][NB x 128 bytes | 2 x 512 bytes of scales]
@@ -650,6 +657,7 @@ __global__ void __launch_bounds__(kFewThreads, 2) mxfp4_few_rows_kernel(const __
     if (tid == 0) {
         for (int i = 0; i < p.slots; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
         mbar_init(&t_full, 1);
+        mbar_init(&done, 1);
         fence_mbar_init();
     }
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -701,13 +709,13 @@ __global__ void __launch_bounds__(kFewThreads, 2) mxfp4_few_rows_kernel(const __
     bool ok = true;
     if (warp == 0) {
         if (lane == 0) {
-            for (int s = p.slots; s < stages && ok; ++s) {
+            int s = min(stages, p.slots);
+            for (; s < stages; ++s) {
                 const int slot = s % p.slots;
-                ok = lane_wait(&empty[slot], ((s / p.slots) & 1u) ^ 1u, p.polls);
-                if (ok) request(s, slot);
+                if (!lane_wait(&empty[slot], ((s / p.slots) & 1u) ^ 1u, p.polls)) { ok = false; break; }
+                request(s, slot);
             }
-            if (!ok)                                          // (copies in flight arrive before the CTA goes)
-                for (int s = 0; s < min(stages, p.slots); ++s) (void)lane_wait(&full[s], 0, p.polls);
+            copies_landed(full, p.slots, s);
         }
     } else if (warp == 1) {
         const uint32_t idesc[2] = {mx_idesc(NB, 0), mx_idesc(NB, 1)};
@@ -733,6 +741,7 @@ __global__ void __launch_bounds__(kFewThreads, 2) mxfp4_few_rows_kernel(const __
             }
             __syncwarp();
         }
+        mmas_ended<false>(&done);
     } else if (warp < 6) {
         ok = stages == 0 || pair_wait(&t_full, 0, p.polls);   // (the last CTAs of a cluster may have none: zeros)
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");

@@ -68,6 +68,61 @@ __device__ __forceinline__ void cluster_sync_all() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
+// ---- how a kernel leaves: nothing that it issued arrives behind it, whichever of its waits ran out ----
+// Looks at a barrier for what the kernel has issued itself and what therefore comes, in microseconds: tens of milliseconds, whatever limit its other waits have.
+constexpr unsigned kDrainPolls = 1u << 16;
+
+// one thread: the copies of a ring's last uses have landed, where this CTA armed its barriers for all of them (`issued` uses in turn, `stages` of them at a time)
+__device__ __forceinline__ void copies_landed(uint64_t* full, unsigned stages, unsigned issued) {
+    for (unsigned j = issued > stages ? issued - stages : 0; j < issued; ++j) (void)lane_wait(&full[j % stages], (j / stages) & 1u, kDrainPolls);
+}
+// the warp that issued them: its MMAs have ended, and what they committed has arrived (done: a barrier of one arrival that nothing else uses)
+template <bool PAIR>
+__device__ __forceinline__ void mmas_ended(uint64_t* done) {
+    if (elect_one_sync()) {
+        if constexpr (PAIR) asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(done)) : "memory");
+        else umma_commit(done);
+    }
+    __syncwarp();
+    (void)pair_wait(done, 0u, kDrainPolls);
+}
+
+// A pair's copies count on the leader's barriers, and either CTA's loader may be the one that gives up.  Both say how many uses of the ring they filled; where a wait ran out,
+// the leader stands in for what the other one did not do.
+struct PairEnd {
+    uint64_t done;                                            // see mmas_ended
+    uint32_t issued[2];                                       // the leader's: uses of the ring that either CTA has filled
+    uint32_t gave_up;                                         // in both
+};
+__device__ __forceinline__ void store_remote(const uint32_t* local, uint32_t rank, uint32_t v) {
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at_rank(local, rank)), "r"(v) : "memory");
+}
+__device__ __forceinline__ void pair_begin(PairEnd* end) {    // one thread, in front of a cluster barrier
+    mbar_init(&end->done, 1);
+    end->gave_up = 0;
+}
+__device__ __forceinline__ void pair_issued(PairEnd* end, uint32_t rank, unsigned issued) { store_remote(&end->issued[rank], 0, issued); }      // the loader, behind its last copy
+__device__ __forceinline__ void pair_gave_up(PairEnd* end) {                                // any thread, in front of pair_end
+    store_remote(&end->gave_up, 0, 1u);
+    store_remote(&end->gave_up, 1, 1u);
+}
+// Every thread of both CTAs, converged.  (A use beyond the other's last one lies less than a ring ahead: the slot was free, so both had filled it before.)
+__device__ __forceinline__ void pair_end(PairEnd* end, uint32_t rank, uint64_t* full, unsigned stages, uint32_t bytes) {
+    cluster_sync_all();
+    if (!*reinterpret_cast<volatile uint32_t*>(&end->gave_up)) return;
+    if (rank == 0 && threadIdx.x == 0) {
+        const unsigned mine = end->issued[0], other = end->issued[1], most = max(mine, other);
+        for (unsigned j = most > stages ? most - stages : 0; j < most; ++j) {
+            uint64_t* const bar = &full[j % stages];
+            if (j >= mine) mbar_arrive_expect_tx(bar, bytes);                                // (armed for one CTA's bytes)
+            else if (j >= other) asm volatile("mbarrier.complete_tx.relaxed.cluster.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+            (void)lane_wait(bar, (j / stages) & 1u, kDrainPolls);
+        }
+    }
+    __syncwarp();
+    cluster_sync_all();
+}
+
 __device__ __forceinline__ void tmem_columns16(uint32_t addr, uint32_t (&v)[16]) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"

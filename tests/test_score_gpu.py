@@ -318,3 +318,70 @@ def test_a_head_that_the_kernel_in_front_writes():
     want = loss_under_a_gradient(True)
     for _ in range(10):
         assert torch.equal(loss_under_a_gradient(False), want)
+
+
+@pytest.mark.parametrize("m,n,k", [(300, 512, 2000), (2048, 16384, 1024), (2100, 12290, 72), (3, 4096, 8192), (1, 130, 40)])
+def test_products_whose_waits_ran_out_leave_in_order(m, n, k):
+    """No looks at any barrier, with copies on their way that are asked for ahead of the first wait: tiles of one SM, of pairs, few rows.  Results
+    are NaN, the next call reports it, and what runs on the SMs behind it is whole."""
+    import ctypes as C
+
+    from dia_tts_prune_b200 import _lm_lib, lm_ops
+    g = torch.Generator(device="cuda").manual_seed(m)
+    x, w4 = torch.randn(m, k, generator=g, device="cuda").bfloat16(), lm_ops.quantize_mxfp4(torch.randn(n, k, generator=g, device="cuda"))
+    polls = getattr(_lm_lib.load(), "_ZN3dia15gemm_pair_pollsEv")
+    polls.restype = C.POINTER(C.c_uint)
+    want, kept = lm_ops.linear_mxfp4(x, w4), polls()[0]
+    polls()[0] = 0
+    try:
+        got = lm_ops.linear_mxfp4(x, w4)
+    finally:
+        polls()[0] = kept
+    behind = want.float() * 2                                      # (another kernel on the SMs that were given up)
+    torch.cuda.synchronize()
+    assert got.isnan().all() and torch.equal(behind, want.float() + want.float())
+    with pytest.raises(RuntimeError):
+        lm_ops.linear_mxfp4(x, w4)
+    for _ in range(3):
+        assert torch.equal(lm_ops.linear_mxfp4(x, w4), want)
+
+
+def test_gradients_whose_waits_ran_out_leave_in_order():
+    import ctypes as C
+
+    from dia_tts_prune_b200 import _lm_lib, lm_ops
+    g = torch.Generator(device="cuda").manual_seed(3)
+    h, w = torch.randn(300, 512, generator=g, device="cuda").bfloat16().requires_grad_(True), (torch.randn(3000, 512, generator=g, device="cuda") / 22).bfloat16().requires_grad_(True)
+    t = torch.randint(0, 3000, (300,), generator=g, device="cuda")
+    polls = getattr(_lm_lib.load(), "_ZN3dia15gemm_pair_pollsEv")
+    polls.restype = C.POINTER(C.c_uint)
+    out = torch.empty(1, device="cuda")
+    for rows in (300, 100):                                        # (pairs of SMs, one SM per tile)
+        loss = lm_ops.linear_cross_entropy(h[:rows], w, t[:rows])
+        want = torch.autograd.grad(loss, (h, w), retain_graph=True)
+        # the launches go by the limit of the thread that makes them: the C entry, from this one
+        lib, st = _lm_lib.load(), torch.cuda.current_stream().cuda_stream
+        kept = torch.empty(2 * rows + 1, device="cuda")
+        need = lib.lm_b200_op_loss_work_bytes(h.data_ptr(), 1, 512, w.data_ptr(), 512, rows, 3000, 512)
+        work = torch.empty(need, dtype=torch.uint8, device="cuda")
+        assert lib.lm_b200_op_loss(h.data_ptr(), 1, 512, w.data_ptr(), 512, t.data_ptr(), 1, -100, rows, 3000, 512, 1.0, 2, out.data_ptr(), kept.data_ptr(), work.data_ptr(), need, st) == 0
+        need = lib.lm_b200_op_loss_grad_work_bytes(h.data_ptr(), 512, w.data_ptr(), 512, rows, 3000, 512, 1, 1)
+        work, one = torch.empty(need, dtype=torch.uint8, device="cuda"), torch.ones((), device="cuda")
+        dh, dw = torch.zeros_like(h[:rows]), torch.zeros_like(w)
+
+        def backward():
+            return lib.lm_b200_op_loss_grad(h.data_ptr(), 512, w.data_ptr(), 512, t.data_ptr(), 1, -100, rows, 3000, 512, 1.0, kept.data_ptr(), one.data_ptr(), 0,
+                                            kept.data_ptr() + 8 * rows, dh.data_ptr(), dw.data_ptr(), work.data_ptr(), need, st)
+
+        torch.cuda.synchronize()
+        limit = polls()[0]
+        polls()[0] = 0
+        try:
+            assert backward() == 0
+        finally:
+            polls()[0] = limit
+        torch.cuda.synchronize()
+        assert dh.isnan().all() and dw.isnan().all()
+        assert backward() != 0                                     # (says that a wait ran out)
+        assert backward() == 0
+        assert torch.equal(dh, want[0][:rows]) and torch.equal(dw, want[1])
