@@ -483,7 +483,7 @@ struct Pair {
 };
 constexpr int kPairStagesMost = 8, kPairChunk = 4;
 constexpr unsigned kPairPolls = 4000000u;                     // a few seconds
-static_assert((2 * kPairStagesMost + 4) * 8 + 8 <= 256, "barrier region");
+static_assert((2 * kPairStagesMost + 4) * 8 + sizeof(PairEnd) + 4 <= 256, "barrier region");
 
 struct PairProduct {
     float* y; const float* residual;
@@ -552,7 +552,8 @@ dia_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
     uint64_t* empty = full + kPairStagesMost;
     uint64_t* t_full = empty + kPairStagesMost;
     uint64_t* t_empty = t_full + 2;                                              // (the leader's alone)
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(t_empty + 2);
+    PairEnd* end = reinterpret_cast<PairEnd*>(t_empty + 2);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(end + 1);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = blockIdx.x & 1;
@@ -566,6 +567,7 @@ dia_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
     if (threadIdx.x == 0) {
         for (int i = 0; i < kPairStagesMost; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
         for (int i = 0; i < 2; ++i) { mbar_init(&t_full[i], 1); mbar_init(&t_empty[i], 2 * Pair<SUMS, GLU>::kWarps); }
+        pair_begin(end);
         fence_mbar_init();
     }
     if (warp == 1) {
@@ -598,8 +600,7 @@ dia_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
                 }
                 // (the leader's last commits arrive here: not after this CTA has gone)
                 for (unsigned j = i > (unsigned)n_stages ? i - n_stages : 0; j < i && ok; ++j) ok = lane_wait(&empty[j % n_stages], (j / n_stages) & 1u, p.polls);
-                // (nor do copies arrive that were issued before a wait ran out)
-                for (unsigned j = i > (unsigned)n_stages ? i - n_stages : 0; j < i && !ok && rank == 0; ++j) (void)lane_wait(&full[j % n_stages], (j / n_stages) & 1u, p.polls);
+                pair_issued(end, rank, i);
             }
         } else if (warp == 1) {
             if (rank == 0) {
@@ -635,6 +636,7 @@ dia_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
                         if (last) ++it;
                     }
                 }
+                mmas_ended<true>(&end->done);
             }
         }
     } else if constexpr (SUMS) {
@@ -844,13 +846,16 @@ dia_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
             ++it;
         }
     }
-    if (!ok && lane == 0 && p.ran_out) {
-        *reinterpret_cast<volatile int*>(p.ran_out) = 1;
-        __threadfence_system();
+    if (!ok && lane == 0) {
+        pair_gave_up(end);
+        if (p.ran_out) {
+            *reinterpret_cast<volatile int*>(p.ran_out) = 1;
+            __threadfence_system();
+        }
     }
     __syncwarp();
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-    cluster_sync_all();                                       // neither CTA's memory goes while the other still reads it or arrives there
+    pair_end(end, rank, full, n_stages, stage_bytes);         // neither CTA's memory goes while the other still reads it or arrives there
     if (warp == 1) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512));
