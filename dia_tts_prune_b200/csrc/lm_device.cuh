@@ -16,7 +16,8 @@ __device__ __forceinline__ float dyt(float x, float alpha, float w, float b) { r
 
 // Programmatic dependent launch: a kernel of a short step lets the next one start as soon as it runs itself
 // (pdl_release) and reads what earlier kernels wrote - or writes anything - only after pdl_wait.  Before the wait a
-// kernel may fetch weights, which no kernel writes.  Launched without the attribute both are no-ops.
+// kernel may fetch weights, which no kernel of a step writes (weights that a caller hands in may be what the kernel in
+// front writes: launched without the attribute).  Launched without it both are no-ops.
 __device__ __forceinline__ void pdl_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 

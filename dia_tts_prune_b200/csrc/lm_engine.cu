@@ -1711,7 +1711,8 @@ int lm_b200_op_token_input(lm_b200_engine* e, int layer, const float* x, const i
 
 int lm_b200_op_linear(const float* A, const void* W_bf16, float* Y, int M, int N, int K, void* stream) {
     if (!A || !W_bf16 || !Y || M <= 0 || N <= 0 || K <= 0) return LM_B200_EINVAL;
-    LCK(lm::launch_linear(A, K, W_bf16, 0, Y, N, M, N, K, nullptr, S(stream)));
+    // (the weights are the caller's: a 4-bit product's result, the gradient of a loss, whose kernels let this one start before they have written it)
+    LCK(lm::launch_linear(A, K, W_bf16, 0, Y, N, M, N, K, nullptr, S(stream), lm::kActNone, false));
     return LM_B200_OK;
 }
 

@@ -48,8 +48,9 @@ cudaError_t launch_dyt_tapmix(const float* x, const NormW& n, const float* cw, i
                               float* out, void* out_bf16, int M, int D, cudaStream_t st);
 cudaError_t launch_tapmix_tail(const float* x, const NormW& n, int taps, float* tail, const SeqMeta& sm, int n_seq, int D,
                                cudaStream_t st);
+// early: the kernel may start, and fetch weights, before its predecessor has ended - not one that writes them, which a caller's predecessor may be
 cudaError_t launch_linear(const float* A, int lda, const void* W_bf16, long long w_expert_stride, float* Y, int ldy, int M,
-                          int N, int K, const GroupMap* gm, cudaStream_t st, int act = kActNone);
+                          int N, int K, const GroupMap* gm, cudaStream_t st, int act = kActNone, bool early = true);
 // the fused forms for a step of at most kRowsKernelMax rows
 cudaError_t launch_dyt_tapmix_seq(const float* x, const NormW& n, const float* cw, int taps, float* tail, const SeqMeta& sm,
                                   const RowMeta& rm, int n_seq, float* out, int D, cudaStream_t st);

@@ -1279,7 +1279,7 @@ bool vectors_ok(const float* A, int lda, const void* W, int K) {
 }  // namespace
 
 cudaError_t launch_linear(const float* A, int lda, const void* W, long long w_expert_stride, float* Y, int ldy, int M, int N,
-                          int K, const GroupMap* gm, cudaStream_t st, int act) {
+                          int K, const GroupMap* gm, cudaStream_t st, int act, bool early) {
     if (act == kActXielu) return cudaErrorNotSupported;       // (its two numbers are not handed in here)
     const int* a_row = gm ? gm->a_row : nullptr;
     const float* a_scale = gm ? gm->a_scale : nullptr;
@@ -1287,13 +1287,13 @@ cudaError_t launch_linear(const float* A, int lda, const void* W, long long w_ex
     const int* n_slots = gm ? gm->n_slots : nullptr;
     const __nv_bfloat16* w = reinterpret_cast<const __nv_bfloat16*>(W);
     if (!gm && act == kActNone && N <= kRowsKernelMaxOut && (long long)M * std::min(N, 8) >= kNarrowWorkMin && vectors_ok(A, lda, w, K))
-        return launch_pdl(linear_narrow_kernel, dim3((M + 8 * kNarrowRows - 1) / (8 * kNarrowRows)), dim3(256), 0, st, A, lda, w, Y, ldy, M, N, K);
+        return launch_pdl_if(early, linear_narrow_kernel, dim3((M + 8 * kNarrowRows - 1) / (8 * kNarrowRows)), dim3(256), 0, st, A, lda, w, Y, ldy, M, N, K);
     // a few rows, or a few outputs (router logits: the same order of operations for every step length, so that the choice of experts
     // does not depend on how a prompt was cut)
     if (M <= kRowsKernelMax || (N <= kRowsKernelMaxOut && M <= 65535))
-        return launch_pdl(linear_rows_kernel, dim3((N + 7) / 8, M), dim3(256), 0, st, A, lda, w, w_expert_stride, Y, ldy, M, N, K,
-                          a_row, a_scale, a_expert, n_slots, (float*)nullptr, (const float*)nullptr, (const float*)nullptr, 0.f,
-                          TapOut{}, act);
+        return launch_pdl_if(early, linear_rows_kernel, dim3((N + 7) / 8, M), dim3(256), 0, st, A, lda, w, w_expert_stride, Y, ldy, M, N, K,
+                             a_row, a_scale, a_expert, n_slots, (float*)nullptr, (const float*)nullptr, (const float*)nullptr, 0.f,
+                             TapOut{}, act);
     else
         linear_tile_kernel<<<dim3((N + BN - 1) / BN, (M + BM - 1) / BM), 256, 0, st>>>(A, lda, w, w_expert_stride, Y, ldy, M, N,
                                                                                       K, a_row, a_scale, a_expert, n_slots, act);

@@ -385,3 +385,38 @@ def test_gradients_whose_waits_ran_out_leave_in_order():
         assert backward() != 0                                     # (says that a wait ran out)
         assert backward() == 0
         assert torch.equal(dh, want[0][:rows]) and torch.equal(dw, want[1])
+
+
+def test_weights_that_the_kernel_in_front_writes():
+    """``lm_engine.linear`` takes bfloat16 weights where they are: a 4-bit product's result, the gradient of a loss by its head alone, whose kernels
+    let their successor start before they have written it."""
+    from dia_tts_prune_b200 import lm_engine, lm_ops
+    g = torch.Generator(device="cuda").manual_seed(12)
+    w4 = lm_ops.quantize_mxfp4(torch.randn(2048, 512, generator=g, device="cuda") / 22)
+    xs = [torch.randn(16, 512, generator=g, device="cuda").bfloat16() for _ in range(4)]
+    a, wide = torch.randn(2, 2048, generator=g, device="cuda"), torch.randn(3000, 2048, generator=g, device="cuda")   # (a few rows; many rows and few outputs)
+    rows = torch.randn(200, 512, generator=g, device="cuda").bfloat16()
+    heads = [(torch.randn(3000, 512, generator=g, device="cuda") / 22).bfloat16().requires_grad_(True) for _ in range(3)]
+    targets, b = torch.randint(0, 3000, (200,), generator=g, device="cuda"), torch.randn(2, 512, generator=g, device="cuda")
+
+    def product(x, act, wait):
+        y = lm_ops.linear_mxfp4(x, w4)
+        if wait:
+            torch.cuda.synchronize()
+        return lm_engine.linear(act, y)
+
+    def gradient(head, wait):
+        dw, = torch.autograd.grad(lm_ops.linear_cross_entropy(rows, head, targets), head)
+        if wait:
+            torch.cuda.synchronize()
+        return lm_engine.linear(b, dw)
+
+    for act in (a, wide):
+        want = [product(x, act, True) for x in xs]
+        torch.cuda.synchronize()
+        for _ in range(20):
+            assert all(torch.equal(u, v) for u, v in zip([product(x, act, False) for x in xs], want))
+    want = [gradient(h, True) for h in heads]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        assert all(torch.equal(u, v) for u, v in zip([gradient(h, False) for h in heads], want))
