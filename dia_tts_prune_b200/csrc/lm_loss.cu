@@ -642,8 +642,9 @@ __global__ void __launch_bounds__(kFewThreads, 2) loss_few_rows_kernel(const __g
 }
 
 // The tiles of a row joined, a warp per row; where their sum or mean is asked for, the last block to come sums the rows, in their order.
+// (part, hit: their writer may still run when this kernel starts, so not by the read-only path, which __restrict__ would allow)
 constexpr int kJoinWarps = 8;
-__global__ void __launch_bounds__(32 * kJoinWarps) loss_join_kernel(const float2* __restrict__ part, const float* __restrict__ hit, int M, int V, int tiles, const void* targets,
+__global__ void __launch_bounds__(32 * kJoinWarps) loss_join_kernel(const float2* part, const float* hit, int M, int V, int tiles, const void* targets,
                                                                     int targets64, long long ignore, float c, int reduction, float* __restrict__ out, float2* kept,
                                                                     unsigned* arrived) {
     const int lane = threadIdx.x & 31, row = blockIdx.x * kJoinWarps + (threadIdx.x >> 5);
@@ -743,9 +744,9 @@ __global__ void __launch_bounds__(256) loss_pack_kernel(const void* __restrict__
     for (int q = 0; q < TERMS; ++q) *reinterpret_cast<uint4*>(out + ((size_t)q * M + r) * ld_out + k) = *reinterpret_cast<const uint4*>(t[q]);
 }
 
-// dh = the sum of the shares of the contraction, times grad scale [/ *count]
-__global__ void __launch_bounds__(256) loss_rows_out_kernel(const float* __restrict__ acc, int splits, int M, int K, int ld, __nv_bfloat16* __restrict__ out, int wide,
-                                                            const float* __restrict__ grad, int grad_stride, const float* __restrict__ count, float scale, const void* targets,
+// dh = the sum of the shares of the contraction, times grad scale [/ *count]  (acc, grad and count: as part and hit above)
+__global__ void __launch_bounds__(256) loss_rows_out_kernel(const float* acc, int splits, int M, int K, int ld, __nv_bfloat16* __restrict__ out, int wide,
+                                                            const float* grad, int grad_stride, const float* count, float scale, const void* targets,
                                                             int targets64, long long ignore) {
     const int per_row = ld / 4;
     const long long i = (long long)blockIdx.x * 256 + threadIdx.x, r = i / per_row;

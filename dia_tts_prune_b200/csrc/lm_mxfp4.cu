@@ -24,12 +24,13 @@ using namespace dia;
 // ---- rounding and values -------------------------------------------------------------------------------------------------------------------
 
 // Eight neighbouring channels of a row as they lie in memory.  WIDE: rows of whole 16 bytes whose channels are a multiple of eight, all eight are there or none; else those
-// at or beyond `n` are zero.  ONCE: an SM reads them once, so that L1 does without them (32768 x 2048 fp32 rounded in 42 us, not 48).  (Fetching and widening are apart:
-// widened at once, a load is waited for before the next one goes out.)
+// at or beyond `n` are zero.  ONCE: an SM reads them once, so that L1 does without them (32768 x 2048 fp32 rounded in 42 us, not 48), and no kernel writes them meanwhile (the
+// read-only path; a kernel that starts before its predecessor has ended does without it).  (Fetching and widening are apart: widened at once, a load is waited for before the
+// next one goes out.)
 template <int TYPE, bool WIDE, bool ONCE>
 struct Eight {
     static __device__ __forceinline__ uint4 load(const uint4* p) {
-        if constexpr (!ONCE) return __ldg(p);
+        if constexpr (!ONCE) return *p;
         uint4 v;
         asm("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
         return v;

@@ -420,3 +420,29 @@ def test_weights_that_the_kernel_in_front_writes():
     torch.cuda.synchronize()
     for _ in range(20):
         assert all(torch.equal(u, v) for u, v in zip([gradient(h, False) for h in heads], want))
+
+
+def test_rows_that_the_kernel_in_front_writes():
+    """Products of few rows, losses and gradients read what the kernel in front has just written, over and over in the same memory."""
+    from dia_tts_prune_b200 import lm_ops
+    g = torch.Generator(device="cuda").manual_seed(14)
+    ws = [lm_ops.quantize_mxfp4(torch.randn(1024, 1024, generator=g, device="cuda") / 32) for _ in range(6)]
+    head, t = (torch.randn(2000, 1024, generator=g, device="cuda") / 32).bfloat16(), torch.randint(0, 2000, (16,), generator=g, device="cuda")
+    xs = [torch.randn(16, 1024, generator=g, device="cuda").to(d) for d in (torch.bfloat16, torch.float32) for _ in range(3)]
+
+    def through(x, wait):
+        for w in ws:
+            x = lm_ops.linear_mxfp4(x, w)
+            if wait:
+                torch.cuda.synchronize()
+        losses = lm_ops.linear_cross_entropy(x, head, t, reduction="none")
+        if x.dtype == torch.float32:
+            return x, losses
+        a = x.detach().requires_grad_(True)
+        return x, losses, torch.autograd.grad(lm_ops.linear_cross_entropy(a, head, t), a)[0]
+
+    want = [through(x, True) for x in xs]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for x, ref in zip(xs, want):
+            assert all(torch.equal(u, v) for u, v in zip(through(x, False), ref))
