@@ -273,8 +273,8 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
         raise ValueError("gradients need hidden in bfloat16")
     _check_device(hidden.device, weight, targets)
     if not targets.numel():                                       # (still a function of both, whose gradients are zeros)
-        rows = hidden.float().sum(-1)
-        return rows if reduction == "none" else rows.sum() + weight[:0].float().sum()
+        rows = hidden.float().sum(-1) + weight[:0].float().sum()
+        return rows if reduction == "none" else rows.sum()
     rows = hidden if hidden.dim() == 2 else hidden.reshape(-1, hidden.shape[-1])
     flat = targets if targets.dim() == 1 else targets.reshape(-1)
     if with_grad:

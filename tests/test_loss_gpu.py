@@ -340,3 +340,23 @@ def test_every_share_of_the_rows_gradient_is_written(m, v, k):
     for _ in range(3):
         torch.full((need,), 255, dtype=torch.uint8, device="cuda")
         within(torch.autograd.grad(linear_cross_entropy(x, y, t, scale=0.5), x)[0], want_h, off_h)
+
+
+@pytest.mark.parametrize("reduction", ["none", "sum", "mean"])
+@pytest.mark.parametrize("shape", [(0,), (3, 0)])
+def test_losses_of_nothing_have_gradients_of_zeros(shape, reduction):
+    """Whichever of the two asks for one."""
+    from dia_tts_prune_b200.lm_ops import linear_cross_entropy
+    t = torch.zeros(shape, dtype=torch.long, device="cuda")
+    for rows, head in ((True, True), (True, False), (False, True)):
+        h = torch.zeros(*shape, 16, dtype=torch.bfloat16, device="cuda", requires_grad=rows)
+        w = torch.full((40, 16), math.inf, dtype=torch.bfloat16, device="cuda", requires_grad=head)
+        loss = linear_cross_entropy(h, w, t, reduction=reduction)
+        assert loss.dtype == torch.float32 and loss.shape == (shape if reduction == "none" else ())
+        loss.sum().backward()
+        assert loss.sum() == 0
+        if rows:
+            assert h.grad.shape == h.shape
+        if head:
+            assert w.grad.shape == w.shape and not w.grad.any()
+    assert not linear_cross_entropy(h.detach(), w.detach(), t, reduction=reduction).requires_grad
