@@ -3,7 +3,7 @@ entropy of rows under a head with its gradient.
 
 They stand beside ``lm_engine.linear``: torch tensors on a CUDA device in, new tensors out, queued on the current stream of the tensors'
 device.  Workspaces come from torch's allocator for the length of a call, so calls on several streams and in captured graphs do not share
-any.  Arguments are checked on the host (``ValueError``, ``TypeError``); there is no CPU fallback.
+any.  Arguments are checked on the host (``ValueError``, ``TypeError``); there is no CPU fallback, and forward-mode tangents are refused.
 """
 
 from __future__ import annotations
@@ -11,6 +11,7 @@ from __future__ import annotations
 from functools import lru_cache
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lm_lib
 
@@ -83,7 +84,14 @@ def _as_rows(x: torch.Tensor) -> torch.Tensor:
     return x if (width == 1 or step == 1) and (rows <= 1 or apart >= width) else x.contiguous()
 
 
+def _no_tangent(what: str, *xs: torch.Tensor) -> None:
+    for x in xs:
+        if forward_ad.unpack_dual(x).tangent is not None:
+            raise ValueError(f"{what} takes no forward-mode tangents")
+
+
 def _no_grad(what: str, x: torch.Tensor) -> None:
+    _no_tangent(what, x)
     if x.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{what} has no gradient: detach its rows or call it under torch.no_grad()")
 
@@ -271,6 +279,7 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
     with_grad = (hidden.requires_grad or weight.requires_grad) and torch.is_grad_enabled()
     if with_grad and hidden.dtype != torch.bfloat16:
         raise ValueError("gradients need hidden in bfloat16")
+    _no_tangent("linear_cross_entropy", hidden, weight)
     _check_device(hidden.device, weight, targets)
     if not targets.numel():                                       # (still a function of both, whose gradients are zeros)
         rows = hidden.float().sum(-1) + weight[:0].float().sum()

@@ -128,3 +128,21 @@ def test_score_command_parses():
         main(["score", "--model", "x"])
     with pytest.raises(SystemExit):
         main(["generate", "--model", "x", "--prompt", "1", "--head-format", "int4"])
+
+
+def test_forward_mode_tangents_are_refused():
+    """They would be lost: the operators' results are new tensors."""
+    from torch.autograd import forward_ad
+    x, h, w = torch.randn(4, 64), torch.randn(4, 64).bfloat16(), torch.randn(10, 64).bfloat16()
+    q, t = lm_ops.Mxfp4(8, 64, torch.device("cpu")), torch.zeros(4, dtype=torch.long)
+    calls = [lambda a: lm_ops.quantize_mxfp4(a(x)), lambda a: lm_ops.linear_mxfp4(a(x), q), lambda a: lm_ops.linear_cross_entropy(a(h), w, t),
+             lambda a: lm_ops.linear_cross_entropy(h, a(w), t), lambda a: lm_ops.linear_cross_entropy(a(h[:0]), w, t[:0])]
+    with forward_ad.dual_level():
+        for call in calls:
+            with pytest.raises(ValueError, match="tangent"):
+                call(lambda v: forward_ad.make_dual(v, torch.ones_like(v)))
+            with pytest.raises(ValueError, match="CUDA"):          # (without one inside a level)
+                call(lambda v: v)
+    for call, v in zip(calls[:3], (x, x, h)):
+        with pytest.raises(ValueError, match="tangent"):
+            torch.func.jvp(lambda u: call(lambda _: u), (v,), (torch.ones_like(v),))
