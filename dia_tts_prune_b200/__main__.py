@@ -3,7 +3,7 @@
   generate  --model DIR --prompt "1 2 3" [--prompt ...] [--max-new-tokens N] [--temperature T] ...
             continue prompts given as token ids with the model of DIR (chosen by its config.json)
   score     --model DIR --tokens "1 2 3" [--tokens ...] [--head-format bfloat16|mxfp4]
-            log-probabilities of texts given as token ids, one JSON object per text
+            log-probabilities of texts given as token ids, one JSON object per text (null: not a finite number)
   trace     --model DIR --dtype bfloat16|float32 --out DIR --max-tokens N
             replay a trace of steps from standard input and write the logits asked for (``bin/trace_run``)
   build     compile the CUDA libraries
@@ -42,14 +42,24 @@ def _cmd_score(a) -> int:
     import math
 
     from .registry import load_model
+
+    def number(x: float) -> float | None:
+        return x if math.isfinite(x) else None                   # (JSON has neither infinities nor NaN)
+
+    def perplexity(loss: float) -> float | None:
+        try:
+            return number(math.exp(loss))
+        except OverflowError:                                    # a mean loss beyond 709 nats
+            return None
+
     model = load_model(a.model, dtype=a.dtype, max_tokens=a.max_tokens, head_format=a.head_format)
     if not hasattr(model, "score"):
         print("score: this command serves the language models", file=sys.stderr)
         return 2
     for logprobs in model.score([[int(t) for t in p.replace(",", " ").split()] for p in a.tokens]):
-        total = math.fsum(logprobs)
-        print(json.dumps({"tokens": len(logprobs), "logprob": total, "perplexity": math.exp(-total / len(logprobs)) if logprobs else None,
-                          "logprobs": logprobs}))
+        total = math.fsum(logprobs) if all(map(math.isfinite, logprobs)) else sum(logprobs)       # (fsum refuses infinities of both signs)
+        print(json.dumps({"tokens": len(logprobs), "logprob": number(total), "perplexity": perplexity(-total / len(logprobs)) if logprobs else None,
+                          "logprobs": [number(x) for x in logprobs]}, allow_nan=False))
     return 0
 
 

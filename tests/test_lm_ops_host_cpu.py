@@ -146,3 +146,26 @@ def test_forward_mode_tangents_are_refused():
     for call, v in zip(calls[:3], (x, x, h)):
         with pytest.raises(ValueError, match="tangent"):
             torch.func.jvp(lambda u: call(lambda _: u), (v,), (torch.ones_like(v),))
+
+
+def test_score_command_prints_json_whatever_the_scores(monkeypatch, capsys):
+    """One object per text: null for what is not a finite number and for a perplexity beyond float64's largest; texts behind it are still there."""
+    import json
+
+    from dia_tts_prune_b200 import __main__, registry
+
+    class Model:
+        def score(self, texts):
+            return [[-1.0, -2.0], [-900.0], [math.nan, -1.0], [-math.inf, -1.0], [], [-math.inf, math.inf], [-0.5]]
+
+    monkeypatch.setattr(registry, "load_model", lambda *a, **k: Model())
+    assert __main__.main(["score", "--model", "x"] + ["--tokens", "1 2"] * 7) == 0
+
+    def refuse(name):
+        raise AssertionError(f"{name} is not JSON")
+
+    got = [json.loads(line, parse_constant=refuse) for line in capsys.readouterr().out.strip().splitlines()]
+    assert [g["tokens"] for g in got] == [2, 1, 2, 2, 0, 2, 1]
+    assert [g["logprob"] for g in got] == [-3.0, -900.0, None, None, 0, None, -0.5]
+    assert [g["logprobs"] for g in got] == [[-1.0, -2.0], [-900.0], [None, -1.0], [None, -1.0], [], [None, None], [-0.5]]
+    assert [g["perplexity"] for g in got] == [math.exp(1.5), None, None, None, None, None, math.exp(0.5)]
