@@ -45,9 +45,15 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 template <int TERMS, bool PAIR>
 struct Ring {
     static constexpr int kStage = (TERMS + (PAIR ? 1 : 2)) * kTileBytes, kStages = TERMS == 1 ? (PAIR ? 6 : 4) : PAIR ? 3 : 2;
-    static constexpr int kChunk = TERMS == 1 ? 16 : 8;       // kStats: k-blocks of an accumulator
     static constexpr int kSmem = kStages * kStage + kTurn + 1024 + 256;
 };
+
+// k-blocks of an accumulator.  The tensor core cuts its sum off at every step of 16, by up to 2^-23 of it, so that a sum of terms of one sign drifts towards zero.  The losses'
+// logits: 1024 products of one term, 512 of three (64 and 96 steps: 2^-16 of them).  Of P, which is rounded to bf16 behind, 4096 channels (256 steps: 2^-15 of a logit), and of the
+// gradients, whose results are bf16, 32768 rows or columns (2048 steps: 2^-12 of the sum, a sixteenth of that rounding).  What is longer is summed in fp32.
+template <int KIND, int TERMS>
+constexpr int kChunkOf = KIND == kStats ? (TERMS == 1 ? 16 : 8) : KIND == kProbs ? 64 : 512;
+constexpr int kSumsCtas = 148, kSumsFloats = 128 * kTileN;      // sums of the pieces that came before the last one: CTAs that have room for them, numbers of each
 
 // Tiles of one product, and what they are made of (kGrads has two products)
 struct Tiles {
@@ -73,6 +79,7 @@ struct LossTiles {
     __nv_bfloat16* p; int ldp;
     float* acc; int ld_acc, add;     // kGrads, dh: [splits][M][ld_acc]; add: to what is there
     __nv_bfloat16* out; int wide;    // dw: [M][N]; wide: 16-byte stores
+    float* sums;                     // kProbs, dw: [CTA][kSumsFloats] where an accumulator does not take the whole contraction
     const float *grad, *count; float scale;        // dw: what the sums are multiplied by (grad null: nothing)
     int* ran_out;
     unsigned polls;
@@ -146,8 +153,7 @@ template <int KIND, int TERMS, bool PAIR = true>
 __global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(kThreads, 1)
 loss_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_ha,
                     const __grid_constant__ CUtensorMap map_hb, const __grid_constant__ LossTiles p) {
-    constexpr bool kStats_ = KIND == kStats;
-    constexpr int kStage = Ring<TERMS, PAIR>::kStage, kStages = Ring<TERMS, PAIR>::kStages, kChunk = Ring<TERMS, PAIR>::kChunk;
+    constexpr int kStage = Ring<TERMS, PAIR>::kStage, kStages = Ring<TERMS, PAIR>::kStages, kChunk = kChunkOf<KIND, TERMS>;
     static_assert(PAIR || KIND != kGrads, "both gradients go on pairs");
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -241,7 +247,7 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                 const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(kTileN >> 3) << 17) | ((PAIR ? 16u : 8u) << 24);
                 const uint32_t a_step = a_mn ? 2048 >> 4 : 2, b_step = b_mn ? 2048 >> 4 : 2;        // 16 of the contraction, in descriptor units
                 for (int kb = t.kb0; kb < t.kb1; ++kb, ++i) {
-                    const bool first = kStats_ ? kb % kChunk == 0 : kb == t.kb0, last = kb == t.kb1 - 1 || (kStats_ && kb % kChunk == kChunk - 1);
+                    const bool first = (kb - t.kb0) % kChunk == 0, last = kb == t.kb1 - 1 || (kb - t.kb0) % kChunk == kChunk - 1;
                     if (first) {
                         if (!pair_wait(&t_empty[it & 1u], ((it >> 1) & 1u) ^ 1u, p.polls)) { ok = false; break; }
                         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -307,9 +313,33 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                 ok = ok && pair_wait(&t_full[it & 1u], (it >> 1) & 1u, p.polls);
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             };
+            // A contraction longer than an accumulator's: the pieces before the last one, added in this thread's own place; what came before columns 32 j .. of the warp's (of the
+            // two times 64 that it stores) is then added to the last piece.
+            const int chunks = (t.kb1 - t.kb0 + kChunk - 1) / kChunk;
+            float* const sums = p.sums + (size_t)blockIdx.x * kSumsFloats + (threadIdx.x - 64);
+            const auto add_earlier = [&](uint32_t (&v)[32], int j) {
+#pragma unroll
+                for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) + sums[(j * 32 + e) * 32 * kWarps]);
+            };
+            const auto earlier = [&]() {
+#pragma unroll 1
+                for (int c = 0; c + 1 < chunks; ++c) {
+                    wait();
+#pragma unroll 1
+                    for (int j = 0; j < 4; ++j) {
+                        uint32_t v[32];
+                        tmem_columns32(tile_at() + (j >> 1) * 128 + half * 64 + (j & 1) * 32, v);
+                        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                        if (c) add_earlier(v, j);
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) sums[(j * 32 + e) * 32 * kWarps] = __uint_as_float(v[e]);
+                    }
+                    taken();
+                }
+            };
             if constexpr (KIND == kStats) {
                 const long long target = mine ? target_of(p.targets, p.targets64, row) : -1;
-                // The tensor core cuts its sum off at every step, so an accumulator lives for a piece of the contraction and the pieces meet in registers.
+                // (the pieces meet in registers)
                 float z[128];
 #pragma unroll
                 for (int e = 0; e < 128; ++e) z[e] = 0.f;
@@ -359,6 +389,7 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                     own = expm1f(-kept.y);                    // p - 1 of the target: keeps its digits where p is next to one
                     if (there) target = (int)to - p.v0;
                 }
+                earlier();
                 wait();
                 if (!ok) base = own = CUDART_NAN_F;
 #pragma unroll 1
@@ -370,6 +401,7 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
                     if (cb == 1) taken();
                     if (rows <= 0) continue;
+                    if (chunks > 1) { add_earlier(v[0], 2 * cb); add_earlier(v[1], 2 * cb + 1); }
                     const int at = target - mine0;
 #pragma unroll
                     for (int e = 0; e < 32; ++e) {
@@ -393,9 +425,10 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
             } else if (!t.head) {
                 const int rr = lane >> 3, ch = lane & 7;
                 float* const acc = p.acc + (size_t)t.share * of.M * p.ld_acc;
-                wait();
 #pragma unroll 1
-                for (int cb = 0; cb < 4; ++cb) {
+                for (int c = 0; c < 4 * chunks; ++c) {        // (a longer contraction is added to what is there, as that of later pieces of the vocabulary)
+                    const int cb = c & 3;
+                    if (cb == 0) wait();
                     const int n = n0 + cb * 32 + 4 * ch;
                     uint32_t v[32];
                     tmem_columns32(from() + cb * 32, v);
@@ -403,8 +436,8 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                     if (cb == 3) taken();
                     if (n0 + cb * 32 >= p.ld_acc || rows <= 0) continue;
 #pragma unroll
-                    for (int c = 0; c < 8; ++c)
-                        *reinterpret_cast<uint4*>(blk + lane * 128 + ((c ^ (lane & 7)) << 4)) = make_uint4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+                    for (int g = 0; g < 8; ++g)
+                        *reinterpret_cast<uint4*>(blk + lane * 128 + ((g ^ (lane & 7)) << 4)) = make_uint4(v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]);
                     __syncwarp();
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
@@ -413,7 +446,7 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                         float4 f = *reinterpret_cast<const float4*>(blk + r * 128 + ((ch ^ (r & 7)) << 4));
                         float4* const to = reinterpret_cast<float4*>(acc + (size_t)(row0 + r) * p.ld_acc + n);
                         if (!ok) f.x = f.y = f.z = f.w = CUDART_NAN_F;
-                        if (p.add) {
+                        if (p.add || c > 3) {
                             const float4 o = *to;
                             f.x += o.x; f.y += o.y; f.z += o.z; f.w += o.w;
                         }
@@ -423,6 +456,7 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                 }
                 panel_sync(q);                                // (the other warp's share is a panel's too)
             } else {
+                earlier();
                 wait();
                 if (!ok) factor = CUDART_NAN_F;
 #pragma unroll 1
@@ -434,6 +468,7 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
                     if (cb == 1) taken();
                     if (c0 >= of.N || rows <= 0) continue;
+                    if (chunks > 1) { add_earlier(v[0], 2 * cb); add_earlier(v[1], 2 * cb + 1); }
 #pragma unroll
                     for (int e = 0; e < 32; ++e) {
                         const __nv_bfloat162 b = __floats2bfloat162_rn(__uint_as_float(v[e >> 4][2 * e & 31]) * factor, __uint_as_float(v[e >> 4][(2 * e & 31) + 1]) * factor);
@@ -837,12 +872,13 @@ cudaError_t run_tiles(const CUtensorMap& a, const CUtensorMap& b, LossTiles p, i
             if (e != cudaSuccess) return e;
             p.own.rows = 128;
             p.many = p.own.tiles_n();
-            return launch_early(loss_product_kernel<KIND, TERMS, false>, std::min(p.many, sms), kThreads, Ring<TERMS, false>::kSmem, st, a, b, a, b, p);
+            return launch_early(loss_product_kernel<KIND, TERMS, false>, std::min(p.many, p.sums ? std::min(sms, kSumsCtas) : sms), kThreads, Ring<TERMS, false>::kSmem, st, a, b, a, b, p);
         }
     }
     int pairs = 0;
     const cudaError_t e = pairs_of<KIND, TERMS>(dev, &pairs);
     if (e != cudaSuccess) return e;
+    if (p.sums) pairs = std::min(pairs, kSumsCtas / 2);
     const long long own = p.own.tiles(), head = p.head.tiles();
     if (own + head > 0x3fffffffLL) return cudaErrorNotSupported;
     // what a tile takes, in k-blocks; taking it out lasts as long as eight of them
@@ -885,8 +921,8 @@ int shares_of(int length, int most) {
 
 // What a call keeps in its workspace, one after the other
 struct Room {
-    size_t h = 0, h_dw = 0, w = 0, part = 0, hit = 0, arrived = 0, kept = 0, p = 0, acc = 0, all = 0;      // offsets
-    bool few = false;
+    size_t h = 0, h_dw = 0, w = 0, part = 0, hit = 0, arrived = 0, kept = 0, p = 0, acc = 0, sums = 0, all = 0;      // offsets
+    bool few = false, long_p = false, long_dw = false;                                  // (contractions that an accumulator does not take)
     int parts = 0;                                                                      // of a row's logits
     int piece = 0, splits = 1;                                                          // columns of a piece of the vocabulary, shares of dh's contraction
 };
@@ -915,6 +951,9 @@ Room room_of(const LossShape& s, bool grad, bool rows, bool head) {
         r.splits = shares_of(std::min(r.piece, s.V), r.splits);
         r.p = take((size_t)s.M * r.piece * 2);
         r.acc = take(rows ? (size_t)r.splits * s.M * ((s.K + 3) / 4 * 4) * 4 : 0);
+        r.long_p = s.K > kChunkOf<kProbs, 1> * kBK;
+        r.long_dw = head && s.M > kChunkOf<kGrads, 1> * kBK;
+        r.sums = take(r.long_p || r.long_dw ? (size_t)kSumsCtas * kSumsFloats * 4 : 0);
     }
     r.all = at;
     return r;
@@ -1017,6 +1056,7 @@ cudaError_t launch_loss_grad(const LossShape& s, const float* kept, const LossGr
         p.own.M = s.M; p.own.N = cols; p.own.K = s.K;
         p.kept = reinterpret_cast<const float2*>(kept);
         p.p = probs; p.ldp = r.piece;
+        if (r.long_p) p.sums = reinterpret_cast<float*>(base + r.sums);
         e = run_tiles<kProbs, 1>(h_rows, w_rows, p, dev, st);
         if (e != cudaSuccess) return e;
         ++extra_launches();
@@ -1028,6 +1068,7 @@ cudaError_t launch_loss_grad(const LossShape& s, const float* kept, const LossGr
             q.acc = acc; q.ld_acc = ld_acc; q.add = v0 > 0;
         }
         if (dw) {
+            if (r.long_dw) q.sums = reinterpret_cast<float*>(base + r.sums);
             q.head.M = cols; q.head.N = s.K; q.head.K = s.M;
             q.out = reinterpret_cast<__nv_bfloat16*>(dw) + (size_t)v0 * s.K;
             if (!by.grad_stride) q.grad = by.grad, q.count = by.count, q.scale = s.scale;      // (else the rows have theirs)

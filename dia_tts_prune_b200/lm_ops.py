@@ -153,8 +153,8 @@ def quantize_mxfp4(x: torch.Tensor) -> Mxfp4:
 
 def linear_mxfp4(a: torch.Tensor, w: Mxfp4, out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """``a [..., width] @ w [out, width]^T`` with both sides in MXFP4: the rows of ``a`` are rounded on the way (as
-    :func:`quantize_mxfp4` does), products are exact and sums float32, and the result has ``a``'s type unless ``out_dtype`` says another.
-    For serving: it has no gradient."""
+    :func:`quantize_mxfp4` does), products are exact and sums float32 (a tensor core's, which cuts off up to ``2 ** -23`` of a sum at every
+    64 channels), and the result has ``a``'s type unless ``out_dtype`` says another.  For serving: it has no gradient."""
     _check_rows(a, "a")
     if not isinstance(w, Mxfp4):
         raise TypeError("w must be an Mxfp4 (see quantize_mxfp4)")

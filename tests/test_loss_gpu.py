@@ -360,3 +360,37 @@ def test_losses_of_nothing_have_gradients_of_zeros(shape, reduction):
         if head:
             assert w.grad.shape == w.shape and not w.grad.any()
     assert not linear_cross_entropy(h.detach(), w.detach(), t, reduction=reduction).requires_grad
+
+
+@pytest.mark.parametrize("m,v,k", [(40, 300, 4104), (200, 520, 8200), (129, 257, 4097), (33000, 300, 40), (70000, 513, 24), (1, 600000, 8), (257, 32900, 4700)])
+def test_contractions_longer_than_an_accumulator(m, v, k):
+    """Channels beyond 4096 (P), rows beyond 32768 (the head's gradient), columns of a share beyond 32768 (the rows')."""
+    test_gradients(m, v, k)
+
+
+def test_long_sums_of_one_sign_do_not_drift():
+    """Sums whose terms have one sign, which a tensor-core accumulator cuts off at every step (16 terms, up to 2^-23 of the sum).
+
+    Head: probabilities of one half (no logit differs), so that its second row's gradient is half the sum of 2^23 positive rows: 2^-12 for
+    the 2048 steps of an accumulator, 2^-16 for 256 float32 sums of them, 2^-8 for the result's rounding, each relative.
+    Rows of 2^18 channels with logits of about 40: P by one accumulator for 4096 channels (256 steps, 2^-15 of the logit) and 64 sums in
+    float32 (2^-18), the log-sum by one for 1024 (64 steps, 2^-17) and 256 sums (2^-16)."""
+    from dia_tts_prune_b200.lm_ops import linear_cross_entropy
+    g = torch.Generator(device="cuda").manual_seed(1)
+    h = (1 + torch.rand(1 << 23, 8, generator=g, device="cuda")).bfloat16()
+    w = torch.zeros(2, 8, dtype=torch.bfloat16, device="cuda", requires_grad=True)
+    dw, = torch.autograd.grad(linear_cross_entropy(h, w, torch.zeros(1 << 23, dtype=torch.int32, device="cuda"), reduction="sum"), w)
+    want = 0.5 * h.double().sum(0)
+    assert ((dw[1].double() / want - 1).abs() <= 2.0 ** -8 + 2.0 ** -12 + 2.0 ** -15).all(), (dw[1].double() / want - 1).tolist()
+    assert torch.equal(dw[0], -dw[1])
+    del h
+    k = 1 << 18
+    h = (1 + torch.rand(40, k, generator=g, device="cuda")).bfloat16()
+    w = ((1 + torch.rand(64, k, generator=g, device="cuda")) * (40 / 2.25 / k)).bfloat16()
+    t = torch.randint(0, 64, (40,), generator=g, device="cuda")
+    e = Exact(h, w, t)
+    e.dz = (2.0 ** -15 + 2.0 ** -18 + 2.0 ** -17 + 2.0 ** -16) / 4 * (e.h.abs() @ e.w.abs().T).amax(1)      # (the bound of P has it four times)
+    a, b = h.requires_grad_(True), w.requires_grad_(True)
+    got = torch.autograd.grad(linear_cross_entropy(a, b, t, reduction="sum"), (a, b))
+    for x, (ref, bound) in zip(got, e.gradient(torch.ones(40))):
+        within(x, ref, bound)
