@@ -188,3 +188,18 @@ def test_offsets_past_32_bits():
         assert torch.equal(linear_mxfp4(a, q)[:, -last:], linear_mxfp4(a, alone))
     w = quantize_mxfp4(torch.randn(8200, k, generator=g, device="cuda"))
     assert torch.equal(linear_mxfp4(x, w)[-last:], linear_mxfp4(x[-last:], w))
+
+
+@pytest.mark.parametrize("m,k", [(1, 1), (3, 33), (7, 128), (129, 257), (300, 2048)])
+def test_values_in_float16(m, k):
+    """The nearest float16 of every value: exact in its normal range, subnormal numbers below (half way: to the even one), infinities from 65520 on."""
+    from dia_tts_prune_b200 import lm_ops
+    x = rows_of(m, k, m + k)
+    scale = 2.0 ** torch.linspace(-40, 24, m)[:, None].round().cuda()
+    for y in (x, x * scale, x.half(), torch.full_like(x, 65504.0), torch.full_like(x, 2.0 ** -24), torch.full_like(x, 2.0 ** -25), torch.full_like(x, 3.0 * 2.0 ** -26)):
+        want = values(y).float().half()                            # (float32 holds the values as they are)
+        got = lm_ops.quantize_mxfp4(y).dequantize(torch.float16)
+        assert got.dtype == torch.float16 and same(got, want.double())
+    y = x.clone()
+    y[0, 0] = math.nan
+    assert same(lm_ops.quantize_mxfp4(y).dequantize(torch.float16), values(y).float().half().double())

@@ -446,3 +446,86 @@ def test_rows_that_the_kernel_in_front_writes():
     for _ in range(20):
         for x, ref in zip(xs, want):
             assert all(torch.equal(u, v) for u, v in zip(through(x, False), ref))
+
+
+def exact_logprobs(hidden, engine, targets):
+    """log-probabilities in 64 bits of the rows as the engine multiplies them (as they are, in bfloat16, in 4 bits), and the losses' own bound (see
+    test_loss_gpu.py): sums of 16 products lose 2^-22 of the magnitudes a step, exponentials and logarithms 2^-20."""
+    from dia_tts_prune_b200 import lm_ops
+    head, terms = engine.head, 1
+    if isinstance(head, lm_ops.Mxfp4):
+        rows, head = lm_ops.quantize_mxfp4(hidden).dequantize(), head.dequantize()
+    elif engine.precision == "float32":
+        rows, terms = hidden, 3
+    else:
+        rows = hidden.bfloat16()
+    h, w, t = rows.double().cpu(), head.double().cpu(), targets.cpu().long()
+    z = h @ w.T
+    loss = -torch.log_softmax(z, 1).gather(1, t[:, None])[:, 0]
+    dz = (h.shape[1] / 16 + 2) * terms * 2.0 ** -22 * (h.abs() @ w.abs().T).amax(1)
+    return -loss, 2 * dz + 2.0 ** -20 + 2.0 ** -22 * (z.abs().amax(1) + loss)
+
+
+@pytest.mark.parametrize("design", ["pubopel", "kupelix", "fipadra"])
+@pytest.mark.parametrize("dtype,head_format", [("float32", "bfloat16"), ("bfloat16", "bfloat16"), ("float32", "mxfp4"), ("bfloat16", "mxfp4")])
+def test_scores_are_the_losses_of_the_rows_that_were_scored(design, dtype, head_format, monkeypatch):
+    """The scores against the rows and targets of the same step, at the losses' own bound; every row's target is the token behind it."""
+    m = model(design, dtype, head_format=head_format)
+    sequences, seen, plain = texts((40, 2, 150, 1, 3, 0, 64, 90), seed=5), [], m.engine.token_losses
+
+    def record(hidden, targets):
+        seen.append((hidden.clone(), targets.clone()))
+        return plain(hidden, targets)
+
+    monkeypatch.setattr(m.engine, "token_losses", record)
+    got = m.score(sequences)
+    assert len(seen) > 1
+    hidden, targets = torch.cat([h for h, _ in seen]), torch.cat([t for _, t in seen])
+    assert targets.tolist() == [t for s in sequences for t in s[1:]]
+    want, off = exact_logprobs(hidden, m.engine, targets)
+    assert ((torch.tensor([x for g in got for x in g], dtype=torch.float64) - want).abs() <= off).all()
+    # rows in their order: the same texts one at a time go through kernels for other numbers of rows, whose bfloat16 products differ by some 2^-8
+    # of a row; other rows are far away
+    alone = torch.cat([h for s in sequences if len(s) > 1 for h in rows_of(m, [s])]).double()
+    near = torch.cdist(alone, hidden.double())
+    same = torch.tensor([[a == b for b in targets.tolist()] for a in targets.tolist()])
+    assert (near.diagonal() <= 0.1 * alone.norm(dim=1)).all()
+    apart = near.cpu() + torch.where(same, 1e9, 0.0)
+    assert (apart.amin(1) > near.diagonal().cpu()).float().mean() > 0.99
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("design", ["pubopel", "kupelix", "fipadra"])
+def test_logits_of_a_head_in_4_bits_are_its_product(design, dtype):
+    """Every logit of a step against the product of the same rows with the same head in 64 bits, at the product's own bound (64 exact products
+    at a time, 2^-22 of the magnitudes a step, see test_mxfp4_gpu.py); and the product called by itself has the step's bits."""
+    from dia_tts_prune_b200 import lm_ops
+    m = model(design, dtype, head_format="mxfp4", step_graphs=False)
+    head = m.engine.head.dequantize().double()
+    for n, wants in ((1, [0]), (40, [39]), (40, [3, 17]), (64, list(range(64)))):
+        s, out = texts((n,), seed=n)[0], []
+        for hidden in (False, True):
+            a = m.state.open("a")
+            out.append(m.engine.step([(a, s, wants)], hidden=hidden))
+            m.state.close("a")
+        logits, hidden = out
+        rows = lm_ops.quantize_mxfp4(hidden).dequantize().double()
+        bound = (hidden.shape[1] / 64 + 2) * 2.0 ** -22 * (rows.abs() @ head.abs().T) + 2.0 ** -24 * (rows @ head.T).abs()
+        assert ((logits.double() - rows @ head.T).abs() <= bound).all()
+        assert torch.equal(logits, lm_ops.linear_mxfp4(hidden, m.engine.head))
+
+
+@pytest.mark.parametrize("design", ["pubopel", "kupelix", "fipadra"])
+def test_captured_steps_of_a_head_in_4_bits(design):
+    """Steps of a few rows are captured with the head's product inside: the bits of steps that are not, as the sequences go on."""
+    a, b = (model(design, "bfloat16", head_format="mxfp4", step_graphs=g) for g in (True, False))
+    prompts = texts((5, 9, 2), seed=8)
+    open_ = [[m.state.open(f"s{i}") for i in range(3)] for m in (a, b)]
+    for _ in range(2):                                             # (captured once, replayed afterwards)
+        for k in (1, 2, 3):
+            out = [m.engine.step([(seq, p, [len(p) - 1]) for seq, p in zip(seqs[:k], prompts)]) for m, seqs in zip((a, b), open_)]
+            assert torch.equal(*out)
+            for _ in range(3):
+                tokens = out[0].argmax(1).tolist()
+                out = [m.engine.step([(seq, [t], [0]) for seq, t in zip(seqs[:k], tokens)]) for m, seqs in zip((a, b), open_)]
+                assert torch.equal(*out)
