@@ -272,8 +272,8 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
     if reduction not in _REDUCTIONS:
         raise ValueError("reduction must be 'none', 'sum' or 'mean'")
     scale, ignore_index = float(scale), int(ignore_index)
-    if not 0.0 < scale < float("inf"):
-        raise ValueError("scale must be positive and finite")
+    if not 2.0 ** -126 <= scale <= 2.0 ** 126:                    # (the kernels hold it, and its product with log2(e), in float32)
+        raise ValueError("scale must be positive, from 2 ** -126 to 2 ** 126")
     if not -1 << 63 <= ignore_index < 1 << 63:
         raise ValueError("ignore_index must fit 64 bits")
     with_grad = (hidden.requires_grad or weight.requires_grad) and torch.is_grad_enabled()

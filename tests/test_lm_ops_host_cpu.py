@@ -169,3 +169,19 @@ def test_score_command_prints_json_whatever_the_scores(monkeypatch, capsys):
     assert [g["logprob"] for g in got] == [-3.0, -900.0, None, None, 0, None, -0.5]
     assert [g["logprobs"] for g in got] == [[-1.0, -2.0], [-900.0], [None, -1.0], [None, -1.0], [], [None, None], [-0.5]]
     assert [g["perplexity"] for g in got] == [math.exp(1.5), None, None, None, None, None, math.exp(0.5)]
+
+
+def test_scales_that_float32_does_not_hold_are_refused():
+    """By the operator and by the C entries: too small, too large, or finite but not so times log2(e)."""
+    lib, at = _lm_lib.load(), 1 << 20
+    h, w, t = torch.randn(6, 32).bfloat16(), torch.randn(10, 32).bfloat16(), torch.zeros(6, dtype=torch.long)
+    loss = [at, 1, 64, at, 64, at, 1, -100, 100, 300, 64, 1.0, 2, at, at, None, 1 << 30]
+    grad = [at, 64, at, 64, at, 1, -100, 100, 300, 64, 1.0, at, at, 0, None, at, at, None, 1 << 30]
+    for scale in (1e-46, 2.0 ** -127, 2.0 ** 127, 3e38, 1e39, 1e300):
+        with pytest.raises(ValueError, match="scale"):
+            lm_ops.linear_cross_entropy(h, w, t, scale=scale)
+        loss[11] = grad[10] = scale
+        assert lib.lm_b200_op_loss(*loss, None) == lib.lm_b200_op_loss_grad(*grad, None) == _lm_lib.E_INVAL
+    for scale in (2.0 ** -126, 2.0 ** 126):
+        with pytest.raises(ValueError, match="CUDA"):
+            lm_ops.linear_cross_entropy(h, w, t, scale=scale)
