@@ -164,8 +164,16 @@ typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t,
                                   const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
+// (The driver encodes maps on threads that have a context, which the runtime gives a thread with its first call that needs one: a thread of the caller's, or the one that a
+// backward pass begins on, may not have made any.)
 static EncodeTiledFn encode_tiled() {
     static EncodeTiledFn fn = nullptr;
+    static thread_local bool bound = false;
+    if (!bound) {
+        int dev = 0;
+        if (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess) return nullptr;
+        bound = true;
+    }
     if (!fn) {
         void* p = nullptr;
         cudaDriverEntryPointQueryResult q;

@@ -529,3 +529,41 @@ def test_captured_steps_of_a_head_in_4_bits(design):
                 tokens = out[0].argmax(1).tolist()
                 out = [m.engine.step([(seq, [t], [0]) for seq, t in zip(seqs[:k], tokens)]) for m, seqs in zip((a, b), open_)]
                 assert torch.equal(*out)
+
+
+def test_a_thread_that_has_not_used_the_device():
+    """Its first call is an operator's, with memory that torch has at hand."""
+    import threading
+
+    from dia_tts_prune_b200 import lm_ops
+    x, w4, head, t = inputs(300, 9)
+    y = lm_ops.linear_mxfp4(x, w4)
+    calls = [lambda: lm_ops.linear_mxfp4(x[:2], w4), lambda: lm_ops.linear_mxfp4(x, w4), lambda: lm_ops.linear_cross_entropy(y, head, t, reduction="none"),
+             lambda: lm_ops.linear_cross_entropy(y[:3], head, t[:3], reduction="none"), lambda: lm_ops.quantize_mxfp4(y).dequantize()]
+    for call in calls:
+        call()                                                     # (its workspace is at hand afterwards)
+        want, got = call(), []
+        thread = threading.Thread(target=lambda: got.append(call()))
+        thread.start()
+        thread.join()
+        assert torch.equal(got[0], want)
+
+
+def test_the_first_backward_pass_of_a_program():
+    """By the rows alone: its thread has not used the device, and nothing else is launched in front.  (P and the result are rounded to bfloat16, 2^-8
+    each, and what the gradient sums are a target's row and a mean of many: next to no cancellation.)"""
+    import subprocess
+    import sys
+    program = """
+import torch
+from dia_tts_prune_b200.lm_ops import linear_cross_entropy
+h = torch.randn(40, 64, device="cuda").bfloat16().requires_grad_(True)
+w, t = torch.randn(300, 64, device="cuda").bfloat16(), torch.arange(40, device="cuda")
+linear_cross_entropy(h, w, t).backward()
+p = torch.softmax(h.detach().double() @ w.double().T, 1)
+p[torch.arange(40), t] -= 1
+want = p @ w.double() / 40
+assert ((h.grad.double() - want).norm() <= 2.0 ** -7 * want.norm())
+"""
+    done = subprocess.run([sys.executable, "-c", program], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
