@@ -394,3 +394,21 @@ def test_long_sums_of_one_sign_do_not_drift():
     got = torch.autograd.grad(linear_cross_entropy(a, b, t, reduction="sum"), (a, b))
     for x, (ref, bound) in zip(got, e.gradient(torch.ones(40))):
         within(x, ref, bound)
+
+
+@pytest.mark.parametrize("m", [3, 50, 300])
+@pytest.mark.parametrize("scale", [2.0 ** -126, 2.0 ** 126])
+def test_the_smallest_and_largest_scale(m, scale):
+    """Logits next to zero: the loss is the vocabulary's logarithm (2^-20 for exponentials and logarithms), the gradient zero times the scale or
+    as small as that."""
+    from dia_tts_prune_b200.lm_ops import linear_cross_entropy
+    h, w, t = operands(m, 300, 72, m, ignored=0.0)
+    if scale > 1:
+        h.zero_()
+    h.requires_grad_(True)
+    loss = linear_cross_entropy(h, w, t, scale=scale, reduction="none")
+    assert ((loss.double() - math.log(300)).abs() <= 2.0 ** -18).all()
+    dh, = torch.autograd.grad(loss.sum(), h)
+    want = (torch.full((m, 300), 1 / 300, device="cuda", dtype=torch.float64).scatter_add_(1, t[:, None], -torch.ones(m, 1, device="cuda", dtype=torch.float64)) @ w.double())
+    bound = 2.0 ** -8 * want.abs() + 2.0 ** -7 * (1 / 300 * w.double().abs().sum(0) + w.double().abs()[t])
+    assert ((dh.double() / scale - want).abs() <= bound + 2.0 ** -133 / scale).all()
