@@ -1791,7 +1791,7 @@ size_t lm_b200_op_loss_work_bytes(const void* h, int h_type, int64_t ldh, const 
 int lm_b200_op_loss(const void* h, int h_type, int64_t ldh, const void* W, int64_t ldw, const void* targets, int targets64, int64_t ignore, int M, int V, int K, float scale,
                     int reduction, float* out, float* kept, void* work, size_t work_bytes, void* stream) {
     lm::LossShape s;
-    if (!loss_shape(s, h, h_type, ldh, W, ldw, M, V, K) || !targets || !loss_scale(scale) || reduction < LM_B200_LOSS_EACH || reduction > LM_B200_LOSS_MEAN || !out || !work || !aligned(work, 256) ||
+    if (!loss_shape(s, h, h_type, ldh, W, ldw, M, V, K) || !targets || !loss_scale(scale) || reduction < LM_B200_LOSS_EACH || reduction > LM_B200_LOSS_MEAN || !out || !aligned(kept, 8) || !work || !aligned(work, 256) ||
         work_bytes < lm::loss_work_bytes(s))
         return LM_B200_EINVAL;
     s.targets = targets; s.targets64 = targets64; s.ignore = ignore; s.scale = scale;
@@ -1807,7 +1807,7 @@ size_t lm_b200_op_loss_grad_work_bytes(const void* h, int64_t ldh, const void* W
 int lm_b200_op_loss_grad(const void* h, int64_t ldh, const void* W, int64_t ldw, const void* targets, int targets64, int64_t ignore, int M, int V, int K, float scale,
                          const float* kept, const float* grad, int grad_stride, const float* count, void* dh, void* dW, void* work, size_t work_bytes, void* stream) {
     lm::LossShape s;
-    if (!loss_shape(s, h, LM_B200_BF16, ldh, W, ldw, M, V, K) || !targets || !loss_scale(scale) || !kept || !grad || grad_stride < 0 || (!dh && !dW) ||
+    if (!loss_shape(s, h, LM_B200_BF16, ldh, W, ldw, M, V, K) || !targets || !loss_scale(scale) || !kept || !aligned(kept, 8) || !grad || grad_stride < 0 || (!dh && !dW) ||
         !work || !aligned(work, 256) || work_bytes < lm::loss_grad_work_bytes(s, dh != nullptr, dW != nullptr))
         return LM_B200_EINVAL;
     s.targets = targets; s.targets64 = targets64; s.ignore = ignore; s.scale = scale;

@@ -322,7 +322,7 @@ int lm_b200_op_linear_mxfp4(const void *A, int a_type, int64_t lda, const void *
 /* ---- cross entropy of rows under a head, and its gradient, without the logits in memory ----
  * z = scale h W^T (h [M][K] fp32 or bf16, row stride ldh; W [V][K] bf16, row stride ldw; scale 2^-126 .. 2^126); loss[i] = log sum_j exp z[i][j] - z[i][target[i]], 0 for a row whose
  * target is `ignore`, NaN for one whose target is neither that nor in [0, V).  targets: int32, or int64 where targets64 != 0.  Operands of fp32 rows are exact to 24 bits
- * (three bf16 terms), sums fp32.  out: every loss [M], or one number, the sum or the mean over the rows that count (0 where none does).  kept [2 M + 1] (or NULL), for the
+ * (three bf16 terms), sums fp32.  out: every loss [M], or one number, the sum or the mean over the rows that count (0 where none does).  kept [2 M + 1] (8-byte aligned, or NULL), for the
  * gradient: log sum_j exp z[i][j] and the loss of every row, and behind them (with a sum or a mean) how many rows count.
  * The gradient (h in bf16): P = softmax(z) - onehot, g = scale grad [/ max(*count, 1)], dh_i = g_i P_i W (bf16 [M][K]), dW = P^T (g h) (bf16 [V][K]), either may be NULL.  grad:
  * fp32, of every loss, grad_stride apart (0: one number).  Rows that do not count have no part in either, whatever they hold; a NaN loss has NaN gradients.

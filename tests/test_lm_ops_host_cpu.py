@@ -185,3 +185,11 @@ def test_scales_that_float32_does_not_hold_are_refused():
     for scale in (2.0 ** -126, 2.0 ** 126):
         with pytest.raises(ValueError, match="CUDA"):
             lm_ops.linear_cross_entropy(h, w, t, scale=scale)
+
+
+def test_pairs_of_numbers_that_lie_askew_are_refused():
+    """What a loss keeps for its gradient is written and read two numbers at a time."""
+    lib, at = _lm_lib.load(), 1 << 20
+    loss = [at, 1, 64, at, 64, at, 1, -100, 100, 300, 64, 1.0, 2, at, at + 4, at, 1 << 30]
+    grad = [at, 64, at, 64, at, 1, -100, 100, 300, 64, 1.0, at + 4, at, 0, None, at, at, at, 1 << 30]
+    assert lib.lm_b200_op_loss(*loss, None) == lib.lm_b200_op_loss_grad(*grad, None) == _lm_lib.E_INVAL
