@@ -24,9 +24,14 @@ def _cmd_build(a) -> int:
     return 0
 
 
-def _cmd_generate(a) -> int:
+def _load(a):
     from .registry import load_model
-    model = load_model(a.model, dtype=a.dtype, max_tokens=a.max_tokens, head_format=a.head_format)
+    # (a loader that an application has registered need not know the formats of a head unless one is asked for)
+    return load_model(a.model, dtype=a.dtype, max_tokens=a.max_tokens, **({"head_format": a.head_format} if a.head_format != "bfloat16" else {}))
+
+
+def _cmd_generate(a) -> int:
+    model = _load(a)
     if not hasattr(model, "generate") or not hasattr(model, "run_step"):
         print("generate: this command serves the language models; use the Dia API for speech", file=sys.stderr)
         return 2
@@ -41,8 +46,6 @@ def _cmd_generate(a) -> int:
 def _cmd_score(a) -> int:
     import math
 
-    from .registry import load_model
-
     def number(x: float) -> float | None:
         return x if math.isfinite(x) else None                   # (JSON has neither infinities nor NaN)
 
@@ -52,7 +55,7 @@ def _cmd_score(a) -> int:
         except OverflowError:                                    # a mean loss beyond 709 nats
             return None
 
-    model = load_model(a.model, dtype=a.dtype, max_tokens=a.max_tokens, head_format=a.head_format)
+    model = _load(a)
     if not hasattr(model, "score"):
         print("score: this command serves the language models", file=sys.stderr)
         return 2

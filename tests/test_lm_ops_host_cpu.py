@@ -193,3 +193,27 @@ def test_pairs_of_numbers_that_lie_askew_are_refused():
     loss = [at, 1, 64, at, 64, at, 1, -100, 100, 300, 64, 1.0, 2, at, at + 4, at, 1 << 30]
     grad = [at, 64, at, 64, at, 1, -100, 100, 300, 64, 1.0, at + 4, at, 0, None, at, at, at, 1 << 30]
     assert lib.lm_b200_op_loss(*loss, None) == lib.lm_b200_op_loss_grad(*grad, None) == _lm_lib.E_INVAL
+
+
+def test_commands_and_loaders_of_an_application(tmp_path, monkeypatch, capsys):
+    """A loader registered by an application, without a word of heads: the commands serve its model; a format that it does not know is its to refuse."""
+    from dia_tts_prune_b200 import __main__, registry
+
+    class Model:
+        def generate(self, prompts, **k):
+            return [[1, 2] for _ in prompts]
+
+        def run_step(self):
+            pass
+
+        def score(self, texts):
+            return [[-1.0] for _ in texts]
+
+    registry.architectures()                                       # (the built-in ones are registered first)
+    monkeypatch.setattr(registry, "_LOADERS", dict(registry._LOADERS))
+    registry.register("Mine", lambda folder, dtype, device=None, max_tokens=0: Model())
+    (tmp_path / "config.json").write_text('{"architecture": "Mine"}')
+    assert __main__.main(["generate", "--model", str(tmp_path), "--prompt", "1 2"]) == 0
+    assert __main__.main(["score", "--model", str(tmp_path), "--tokens", "1 2"]) == 0
+    with pytest.raises(TypeError):
+        __main__.main(["score", "--model", str(tmp_path), "--tokens", "1 2", "--head-format", "mxfp4"])
