@@ -227,6 +227,18 @@ def _losses(hidden, weight, targets, scale, ignore_index, reduction, keep):
     return out, (h, w, t, kept)
 
 
+class _OnceDifferentiable(torch.autograd.Function):
+    """Gradients as they are, of which a further derivative by what they were made of is refused (it would else be taken for zero)."""
+
+    @staticmethod
+    def forward(ctx, grad, hidden, weight, *results):
+        return tuple(x.view_as(x) for x in results)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("linear_cross_entropy has no second derivative")
+
+
 class _LinearCrossEntropy(torch.autograd.Function):
     """Losses of rows, or (mean, sum) their total; rows are two-dimensional here."""
 
@@ -239,9 +251,17 @@ class _LinearCrossEntropy(torch.autograd.Function):
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        hidden, weight, h, w, t, kept = ctx.saved_tensors
+        hidden, weight, *read = ctx.saved_tensors
+        if not torch.is_grad_enabled():
+            return *_LinearCrossEntropy.gradients(ctx, grad, hidden, weight, *read), None, None, None, None
+        with torch.no_grad():
+            got = _LinearCrossEntropy.gradients(ctx, grad, hidden, weight, *read)
+        there = iter(_OnceDifferentiable.apply(grad, hidden, weight, *(x for x in got if x is not None)))
+        return *(x if x is None else next(there) for x in got), None, None, None, None
+
+    @staticmethod
+    def gradients(ctx, grad, hidden, weight, h, w, t, kept):
         scale, ignore_index, mean = ctx.args
         need_h, need_w = ctx.needs_input_grad[:2]
         (M, K), V, device = hidden.shape, weight.shape[0], hidden.device
@@ -256,7 +276,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
         _call("loss_grad", device, h_at, ldh, w_at, ldw, t.data_ptr(), t.dtype == torch.int64, ignore_index, M, V, K, scale, kept_at,
               grad.data_ptr(), grad.stride(0) if grad.dim() else 0, kept_at + 8 * M if mean else None, dh.data_ptr() if need_h else None,
               dw.data_ptr() if need_w else None, work.data_ptr(), need)
-        return dh, dw, None, None, None, None
+        return dh, dw
 
 
 def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, *, scale: float = 1.0,
@@ -267,6 +287,7 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
 
     ``weight`` is bfloat16; ``hidden`` is bfloat16, or float32, which is then multiplied as it is (24 bits) and has no gradient.  The
     gradients by ``hidden`` and ``weight`` take the vocabulary in pieces; rows that do not count have no part in them, whatever they hold.
+    There is no second derivative.
     """
     _loss_operands(hidden, weight, targets)
     if reduction not in _REDUCTIONS:

@@ -412,3 +412,25 @@ def test_the_smallest_and_largest_scale(m, scale):
     want = (torch.full((m, 300), 1 / 300, device="cuda", dtype=torch.float64).scatter_add_(1, t[:, None], -torch.ones(m, 1, device="cuda", dtype=torch.float64)) @ w.double())
     bound = 2.0 ** -8 * want.abs() + 2.0 ** -7 * (1 / 300 * w.double().abs().sum(0) + w.double().abs()[t])
     assert ((dh.double() / scale - want).abs() <= bound + 2.0 ** -133 / scale).all()
+
+
+def test_second_derivatives_are_refused():
+    """A gradient taken with its graph may be used, but not differentiated: not alone, and not beside a term that has a derivative."""
+    from dia_tts_prune_b200.lm_ops import linear_cross_entropy
+    h, w, t = operands(20, 300, 64, 4)
+    for rows, head in ((True, True), (True, False), (False, True)):
+        a, b = h.clone().requires_grad_(rows), w.clone().requires_grad_(head)
+        leaves = [x for x in (a, b) if x.requires_grad]
+        loss = linear_cross_entropy(a, b, t)
+        want = torch.autograd.grad(loss, leaves, retain_graph=True)
+        got = torch.autograd.grad(loss, leaves, create_graph=True)
+        assert all(torch.equal(u, v) for u, v in zip(got, want)) and all(x.requires_grad for x in got)
+        with pytest.raises(RuntimeError, match="second derivative"):
+            torch.autograd.grad(sum(x.float().square().sum() for x in got), leaves, retain_graph=True)
+        with pytest.raises(RuntimeError, match="second derivative"):
+            (loss + got[0].float().square().sum()).backward()
+        # kept, but not differentiated
+        loss = linear_cross_entropy(a, b, t)
+        loss.backward(create_graph=True)
+        assert torch.equal((a if rows else b).grad, want[0])
+        a.grad = b.grad = None
