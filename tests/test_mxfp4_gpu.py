@@ -203,3 +203,20 @@ def test_values_in_float16(m, k):
     y = x.clone()
     y[0, 0] = math.nan
     assert same(lm_ops.quantize_mxfp4(y).dequantize(torch.float16), values(y).float().half().double())
+
+
+def test_more_rows_than_a_grid_has_room_for():
+    """65535 x 128 rows and some: rounding, values and products of the rows on either side of the border are what they are alone."""
+    from dia_tts_prune_b200.lm_ops import linear_mxfp4, quantize_mxfp4
+    rows, k, at = 65535 * 128 + 300, 40, 65535 * 128 - 200
+    x = torch.empty(rows, k, dtype=torch.bfloat16, device="cuda").normal_(generator=torch.Generator(device="cuda").manual_seed(6))
+    q = quantize_mxfp4(x)
+    for part in (slice(0, 300), slice(at, rows)):
+        assert same(q.dequantize()[part], values(x[part]))
+    w = rows_of(12, k, 3, torch.bfloat16)
+    w4 = quantize_mxfp4(w)
+    y = linear_mxfp4(x, w4)
+    check(x[at:], w, y[at:])
+    assert torch.equal(y[at:], linear_mxfp4(x[at:], w4)) and torch.equal(y[:1000], linear_mxfp4(x[:1000], w4))
+    z = linear_mxfp4(w, q)                                         # (as the matrix of a product)
+    assert torch.equal(z[:, at:], linear_mxfp4(w, quantize_mxfp4(x[at - 56:]))[:, 56:])      # (from a block of 128 rows on)
