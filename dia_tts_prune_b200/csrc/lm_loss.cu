@@ -6,10 +6,13 @@
 // a second kernel joins the tiles of a row.  Backward: the vocabulary goes in pieces.  The product is taken again for a piece, its epilogue turns logits into P (bf16, a
 // piece of at most 128 MB or 4096 columns, about what L2 holds), and two products take P to dh (fp32 sums over the pieces) and to the piece's rows of dw; their tiles are dealt
 // to the pairs together.  (8192 x 32768 x 2048 and 4096 x 65536 x 1024, loss and gradients, ms, pieces of 32, 64, 128 and 256 MB: 4.55 and 1.97, 3.58 and 1.90, 3.50 and 1.80,
-// 3.52 and 1.85.)  P is rounded without
-// g: 1 - p of a row's target, which is most of its gradient, then lies just below a power of two where steps are fine, and the roundings of the rows do not go one way
-// (8192 rows: 1.7e-3 to 1.9e-3 of the gradients' norm, of which the results' own rounding is 1.66e-3; with g inside 3.0e-3).  One g for all rows multiplies the sums; rows with
-// their own take it into h for dw (rounded to bf16) and behind the sums for dh.
+// 3.52 and 1.85.)
+//
+// What is rounded to fewer than 32 bits.  P, to bf16: as an operand of the tensor cores; in two terms the three products would take 12 M V K operations, not 8, for results that are
+// bf16 themselves.  It is rounded without g: 1 - p of a row's target, which is most of its gradient, then lies just below a power of two where steps are fine, and the roundings of
+// the rows do not go one way (8192 rows: 1.7e-3 to 1.9e-3 of the gradients' norm, of which the results' own rounding is 1.66e-3; with g inside 3.0e-3).  One g for all rows
+// multiplies the sums; rows with their own take it into h for dw, rounded once more by half a step of bf16 (it belongs inside that contraction), and behind the sums for dh.  fp32
+// rows of the forward pass are three bf16 terms, 24 bits; their losses are 8.4e-7 off where elementary fp32 operations are 2.9e-7 off (the tensor core's sums are cut off, not rounded).
 //
 // All of them are one kernel on pairs of SMs: a cluster of two CTAs owns a 256 x 256 tile, tcgen05.mma (cta_group::2) multiplies the 256 rows of both by the 256 columns of
 // both, and the accumulators (two per CTA: a tile is taken out while the next is multiplied) live in tensor memory.
