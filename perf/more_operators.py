@@ -82,7 +82,7 @@ def draw(rng):
         heads = min(48, kv * rng.choice([1, 2, 3, 4, 6, 8, 16]))
         heads -= heads % kv
         case = dict(kind=kind, heads=heads, kv_heads=kv, dim=rng.choice([64, 128, 128, 96, 80, rng.randint(8, 256)]), page=rng.choice([16, 16, 32, 64, 128]),
-                    format=rng.choice(["e4m3", "int8"]), dtype=rng.choice(["bfloat16", "bfloat16", "float32"] + (["float16"] if kind != "attend" else [])))
+                    format=rng.choice(["e4m3", "int8"]), dtype=rng.choice(["bfloat16", "bfloat16", "float32", "float16"]))
         sequences = _log_uniform(rng, 1, 64)
         if kind == "read":
             rows = [_log_uniform(rng, 1, 65536) for _ in range(sequences)]
