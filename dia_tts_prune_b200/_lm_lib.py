@@ -24,6 +24,7 @@ ABI_VERSION = 7
 PRECISION_FP32, PRECISION_BF16 = 0, 1
 TYPE_FP32, TYPE_BF16, TYPE_FP16 = 0, 1, 2
 LOSS_EACH, LOSS_SUM, LOSS_MEAN = 0, 1, 2
+KV8_E4M3, KV8_INT8 = 0, 1
 E_OK, E_INVAL, E_CUDA, E_NOMEM, E_UNSUPPORTED = 0, -1, -2, -3, -5
 
 _vp, _i, _f = C.c_void_p, C.c_int32, C.c_float
@@ -70,6 +71,14 @@ class Model(C.Structure):
                 ("token_pages", _vp), ("head_codes", _vp), ("head_scales", _vp)]
 
 
+class Kv8(C.Structure):
+    _fields_ = [("keys", _vp), ("values", _vp), ("key_scales", _vp), ("value_scales", _vp), ("pages", _i), ("kv_heads", _i), ("page_size", _i), ("dim", _i), ("format", _i)]
+
+
+class Kv8Step(C.Structure):
+    _fields_ = [("table", _vp), ("table_ld", C.c_int64), ("past", _vp), ("first", _vp), ("max_pages", _i), ("n_seq", _i), ("rows", _i)]
+
+
 _ci = C.c_int
 _cf = C.c_float
 _SIGNATURES = {
@@ -104,6 +113,10 @@ _SIGNATURES = {
     "lm_b200_op_loss_grad_work_bytes": (C.c_size_t, [_vp, C.c_int64, _vp, C.c_int64, _ci, _ci, _ci, _ci, _ci]),
     "lm_b200_op_loss_grad": (_ci, [_vp, C.c_int64, _vp, C.c_int64, _vp, _ci, C.c_int64, _ci, _ci, _ci, _cf, _vp, _vp, _ci, _vp, _vp, _vp, _vp, C.c_size_t,
                                    _vp]),
+    "lm_b200_op_kv8_append": (_ci, [_vp, _vp, _vp, C.c_int64, C.c_int64, _vp, C.c_int64, C.c_int64, _ci, _vp]),
+    "lm_b200_op_kv8_read": (_ci, [_vp, _vp, _vp, _vp, _ci, _vp]),
+    "lm_b200_op_kv8_attention_work_bytes": (C.c_size_t, [_vp, _vp, _ci, _ci]),
+    "lm_b200_op_kv8_attention": (_ci, [_vp, _vp, _vp, C.c_int64, C.c_int64, _ci, _ci, _cf, _ci, _vp, _vp, _vp, C.c_size_t, _vp]),
     "lm_b200_argmax_rows": (_ci, [_vp, _ci, _ci, _vp, _vp]),
 }
 

@@ -98,6 +98,7 @@
 #include "gemm_tcgen05.h"
 #include "lm_b200.h"
 #include "lm_internal.h"
+#include "lm_kv8.h"
 #include "lm_loss.h"
 #include "lm_mxfp4.h"
 
@@ -144,6 +145,26 @@ inline bool loss_shape(lm::LossShape& s, const void* h, int h_type, int64_t ldh,
 }
 inline bool loss_scale(float scale) { return scale >= 0x1p-126f && scale <= 0x1p126f; }       // (times log2(e) is finite too)
 inline bool aligned(const void* p, unsigned to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
+
+bool kv8_cache(lm::Kv8Cache& c, const lm_b200_kv8* k) {
+    if (!k || !k->keys || !k->values || !k->key_scales || !k->value_scales || !aligned(k->keys, 16) || !aligned(k->values, 16) || k->pages <= 0 || k->kv_heads <= 0 || k->kv_heads > lm::kKvMostHeads ||
+        k->page_size < lm::kKvBlock || k->page_size > lm::kKvMostPage || (k->page_size & (k->page_size - 1)) || k->dim <= 0 || k->dim > lm::kKvMostDim ||
+        (k->format != LM_B200_KV8_E4M3 && k->format != LM_B200_KV8_INT8))
+        return false;
+    int shift = 4;
+    while (1 << shift < k->page_size) ++shift;
+    c = lm::Kv8Cache{reinterpret_cast<uint8_t*>(k->keys), reinterpret_cast<uint8_t*>(k->values), k->key_scales, k->value_scales, k->pages, k->kv_heads, shift, k->dim, (k->dim + 15) / 16 * 16, k->format};
+    return true;
+}
+bool kv8_step(lm::Kv8Step& s, const lm_b200_kv8_step* p) {
+    if (!p || !p->table || !p->past || p->max_pages <= 0 || (p->n_seq > 1 && p->table_ld < 0) || p->n_seq <= 0 || p->n_seq > kMostRows || p->rows <= 0 || p->rows > kMostRows || (!p->first && p->rows != p->n_seq))
+        return false;
+    s = lm::Kv8Step{p->table, p->table_ld, p->max_pages, p->past, p->first, p->n_seq, p->rows};
+    return true;
+}
+bool kv8_heads(const lm::Kv8Cache& c, const lm::Kv8Step& s, int heads) {
+    return heads > 0 && heads % c.kv_heads == 0 && heads <= lm::kKvMostHeads && s.rows <= kMostRows / heads;        // (a tile counts rows times heads in 32 bits)
+}
 inline lm::NormW N(const lm_b200_norm& n) { return lm::NormW{n.w, n.b, n.alpha}; }
 
 }  // namespace
@@ -1812,6 +1833,40 @@ int lm_b200_op_loss_grad(const void* h, int64_t ldh, const void* W, int64_t ldw,
         return LM_B200_EINVAL;
     s.targets = targets; s.targets64 = targets64; s.ignore = ignore; s.scale = scale;
     LCK(lm::launch_loss_grad(s, kept, lm::LossGrad{grad, grad_stride, count}, dh, dW, work, S(stream)));
+    return LM_B200_OK;
+}
+
+size_t lm_b200_op_kv8_attention_work_bytes(const lm_b200_kv8* cache, const lm_b200_kv8_step* step, int heads, int type) {
+    lm::Kv8Cache c;
+    lm::Kv8Step s;
+    return kv8_cache(c, cache) && kv8_step(s, step) && kv8_heads(c, s, heads) && known_type(type) ? lm::kv8_attention_work_bytes(c, s, heads, type) : 0;
+}
+
+int lm_b200_op_kv8_append(const lm_b200_kv8* cache, const lm_b200_kv8_step* step, const void* k, int64_t k_row, int64_t k_head, const void* v, int64_t v_row, int64_t v_head, int type,
+                          void* stream) {
+    lm::Kv8Cache c;
+    lm::Kv8Step s;
+    if (!kv8_cache(c, cache) || !kv8_step(s, step) || !k || !v || !known_type(type) || k_row < 0 || k_head < 0 || v_row < 0 || v_head < 0) return LM_B200_EINVAL;
+    LCK(lm::launch_kv8_append(c, s, lm::Kv8Rows{k, k_row, k_head}, lm::Kv8Rows{v, v_row, v_head}, type, S(stream)));
+    return LM_B200_OK;
+}
+
+int lm_b200_op_kv8_read(const lm_b200_kv8* cache, const lm_b200_kv8_step* step, void* k, void* v, int type, void* stream) {
+    lm::Kv8Cache c;
+    lm::Kv8Step s;
+    if (!kv8_cache(c, cache) || !kv8_step(s, step) || !k || !v || !known_type(type)) return LM_B200_EINVAL;
+    LCK(lm::launch_kv8_read(c, s, k, v, type, S(stream)));
+    return LM_B200_OK;
+}
+
+int lm_b200_op_kv8_attention(const lm_b200_kv8* cache, const lm_b200_kv8_step* step, const void* q, int64_t q_row, int64_t q_head, int heads, int type, float scale, int window,
+                             const float* sinks, void* out, void* work, size_t work_bytes, void* stream) {
+    lm::Kv8Cache c;
+    lm::Kv8Step s;
+    if (!kv8_cache(c, cache) || !kv8_step(s, step) || !kv8_heads(c, s, heads) || !q || q_row < 0 || q_head < 0 || !known_type(type) || !loss_scale(scale) || window < 0 || !out || !work ||
+        !aligned(work, 256) || work_bytes < lm::kv8_attention_work_bytes(c, s, heads, type))
+        return LM_B200_EINVAL;
+    LCK(lm::launch_kv8_attention(c, s, lm::Kv8Attention{lm::Kv8Rows{q, q_row, q_head}, out, heads, type, scale, window, sinks}, work, S(stream)));
     return LM_B200_OK;
 }
 

@@ -8,6 +8,7 @@ any.  Arguments are checked on the host (``ValueError``, ``TypeError``); there i
 
 from __future__ import annotations
 
+import ctypes as C
 from functools import lru_cache
 
 import torch
@@ -312,3 +313,158 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
     else:
         loss = _losses(rows, weight, flat, scale, ignore_index, reduction, False)[0]
     return loss.view(targets.shape) if reduction == "none" and targets.dim() != 1 else loss
+
+
+_KV8_FORMATS = {"e4m3": _lm_lib.KV8_E4M3, "int8": _lm_lib.KV8_INT8}
+_KV8_PAGES = (16, 32, 64, 128)
+
+
+class Kv8:
+    """Keys and values of sequences in pages, 8 bits a number: ``keys`` and ``values`` hold codes ``[pages, kv_heads, page_size, stride]`` (uint8;
+    E4M3, or two's complement for ``"int8"``; ``stride`` is ``dim`` padded to 16 with zeros), ``key_scales`` and ``value_scales`` ``[pages, kv_heads]``
+    (float32) one power of two for the tokens of a page and head.  A number is its code times that scale.
+
+    Which pages a sequence has is the caller's to keep (``PagedState`` does it for served models): every call takes a ``table [sequences, n]`` of
+    page numbers, int32, whose unused places may hold anything.  Together with ``past [sequences]`` and ``first [sequences + 1]`` (int32, on the
+    device, so that a captured graph reads them anew) it describes the rows of a step: sequence ``i`` has rows ``first[i]`` to ``first[i + 1]`` of the
+    packed ones, at positions ``past[i]`` and on; without ``first``, row ``i`` alone.  A token whose place lies beyond the table, or whose page is not
+    in the pool, is not there: it is not written, not seen, and reads as zeros.  A sequence whose ``past`` is negative has no tokens."""
+    __slots__ = ("keys", "values", "key_scales", "value_scales", "pages", "kv_heads", "page_size", "dim", "format", "_handle")
+
+    def __init__(self, pages: int, kv_heads: int, dim: int, *, page_size: int = 16, format: str = "e4m3", device: torch.device | str = "cuda"):
+        """Room for ``pages`` pages (1 <= dim <= 256; page_size 16, 32, 64 or 128), all zeros."""
+        if format not in _KV8_FORMATS:
+            raise ValueError("format must be 'e4m3' or 'int8'")
+        if page_size not in _KV8_PAGES:
+            raise ValueError(f"page_size must be one of {', '.join(map(str, _KV8_PAGES))}")
+        if not 1 <= dim <= 256:
+            raise ValueError("dim must be from 1 to 256")
+        if not (1 <= pages < 1 << 31 and 1 <= kv_heads <= 4096):
+            raise ValueError("pages and kv_heads must be positive (kv_heads at most 4096)")
+        self.pages, self.kv_heads, self.dim, self.page_size, self.format = int(pages), int(kv_heads), int(dim), int(page_size), format
+        shape = (self.pages, self.kv_heads, self.page_size, (self.dim + 15) // 16 * 16)
+        self.keys, self.values = (torch.zeros(shape, dtype=torch.uint8, device=device) for _ in range(2))
+        self.key_scales, self.value_scales = (torch.zeros(shape[:2], dtype=torch.float32, device=device) for _ in range(2))
+        self._handle = _lm_lib.Kv8(self.keys.data_ptr(), self.values.data_ptr(), self.key_scales.data_ptr(), self.value_scales.data_ptr(), self.pages,
+                                   self.kv_heads, self.page_size, self.dim, _KV8_FORMATS[format])
+
+    @property
+    def device(self) -> torch.device:
+        return self.keys.device
+
+    @property
+    def nbytes(self) -> int:
+        return 2 * (self.keys.numel() + 4 * self.key_scales.numel())
+
+    def append(self, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, past: torch.Tensor, first: torch.Tensor | None = None) -> None:
+        """Writes ``k`` and ``v [rows, kv_heads, dim]`` (float32, bfloat16 or float16; rows and heads of any stride) behind the ``past[i]`` tokens that
+        sequence ``i`` holds.  A page's exponent is the smallest, at least -100, for which its largest magnitude so far is at most 448 (``"int8"``: 127)
+        times the power; codes go to the nearest, half way to the even one.  Where a page that holds earlier tokens needs a larger exponent, their codes
+        are rounded again.  The first token of a page starts it anew, whatever it held.  A number that is not finite makes the page's head stand for NaNs
+        until then.  No page may belong to two sequences of a call."""
+        _check_rows(k, "k")
+        _check_rows(v, "v")
+        if k.dim() != 3 or k.shape[1] != self.kv_heads or k.shape[2] != self.dim or v.shape != k.shape or v.dtype != k.dtype:
+            raise ValueError(f"k {tuple(k.shape)} {k.dtype} and v {tuple(v.shape)} {v.dtype} must be [rows, {self.kv_heads}, {self.dim}] of one type")
+        _no_grad("Kv8.append", k)
+        _no_grad("Kv8.append", v)
+        step = _kv8_step(self, table, past, first, k.shape[0])
+        _check_device(self.keys.device, k, v)
+        if step is None:
+            return
+        k, v = _neighbouring(k), _neighbouring(v)
+        _call("kv8_append", self.keys.device, C.addressof(self._handle), C.addressof(step), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
+              v.stride(1), _TYPES[k.dtype])
+
+    def read(self, table: torch.Tensor, past: torch.Tensor, first: torch.Tensor | None, rows: int, dtype: torch.dtype = torch.float32) -> tuple[torch.Tensor, torch.Tensor]:
+        """Keys and values ``[rows, kv_heads, dim]`` of the tokens at positions ``past[i]`` and on, as many as ``first`` gives sequence ``i`` rows.  Rows of no
+        sequence are zeros."""
+        if dtype not in _TYPES:
+            raise TypeError(f"dtype must be one of {_names(_TYPES)}, not {dtype}")
+        rows = int(rows)
+        if rows < 0:
+            raise ValueError("rows must not be negative")
+        step = _kv8_step(self, table, past, first, rows)
+        device = self.keys.device
+        k, v = (torch.empty((rows, self.kv_heads, self.dim), dtype=dtype, device=device) for _ in range(2))
+        if step is None:
+            return k.zero_(), v.zero_()
+        _call("kv8_read", device, C.addressof(self._handle), C.addressof(step), k.data_ptr(), v.data_ptr(), _TYPES[dtype])
+        return k, v
+
+
+def _neighbouring(x: torch.Tensor) -> torch.Tensor:
+    return x if x.shape[-1] == 1 or x.stride(-1) == 1 else x.contiguous()
+
+
+def _kv8_step(cache: Kv8, table: torch.Tensor, past: torch.Tensor, first: torch.Tensor | None, rows: int):
+    """The description of a step's rows as the library takes it (None: no row of any sequence)."""
+    for name, t in (("table", table), ("past", past), ("first", first)):
+        if t is None and name == "first":
+            continue
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be a tensor")
+        if t.dtype != torch.int32:
+            raise TypeError(f"{name} must be int32, not {t.dtype}")
+    if table.dim() != 2 or (table.shape[1] > 1 and table.stride(1) != 1):
+        raise ValueError("table must be [sequences, pages of one] with neighbouring page numbers")
+    n = table.shape[0]
+    if past.dim() != 1 or past.shape[0] != n or not past.is_contiguous():
+        raise ValueError(f"past must hold one number for each of {n} sequences")
+    if first is None:
+        if rows != n:
+            raise ValueError(f"{rows} rows of {n} sequences need first")
+        _check_device(cache.keys.device, table, past)
+    else:
+        if first.dim() != 1 or first.shape[0] != n + 1 or not first.is_contiguous():
+            raise ValueError(f"first must hold {n + 1} numbers")
+        _check_device(cache.keys.device, table, past, first)
+    if rows > 0x7fffff00:
+        raise ValueError(f"{rows} rows are more than an operator takes")
+    if not (n and rows and table.shape[1]):
+        return None
+    return _lm_lib.Kv8Step(table.data_ptr(), table.stride(0), past.data_ptr(), None if first is None else first.data_ptr(), table.shape[1], n, rows)
+
+
+def attention_kv8(q: torch.Tensor, cache: Kv8, table: torch.Tensor, past: torch.Tensor, first: torch.Tensor | None = None, *, scale: float | None = None,
+                  window: int | None = None, sinks: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal grouped-query attention of ``q [rows, heads, dim]`` (float32, bfloat16 or float16; any stride of rows and heads) over the tokens in ``cache``: a row
+    sees the tokens at its position and before it, the last ``window`` of them where that is given, so its own have to be there
+    (:meth:`Kv8.append` with the same ``table``, ``past`` and ``first``).  Query head ``h`` reads key head ``h // (heads / kv_heads)``; weights are
+    ``exp(scale * q . k)``, ``scale`` ``dim ** -0.5`` unless given, and ``sinks [heads]`` (float32) adds ``exp(sinks[h])`` to the denominator.  A row that sees
+    nothing, and a row of no sequence, is zeros.
+
+    float32 rows are multiplied with 22 bits, as the language models' attention does; weights are rounded to 22 bits for them, to 11 for the other types.
+    Maxima, sums and outputs are float32 until the result.  It has no gradient."""
+    _check_rows(q, "q")
+    if not isinstance(cache, Kv8):
+        raise TypeError("cache must be a Kv8")
+    if q.dim() != 3 or q.shape[2] != cache.dim or not q.shape[1] or q.shape[1] % cache.kv_heads or q.shape[1] > 4096:
+        raise ValueError(f"q {tuple(q.shape)} does not go with {cache.kv_heads} key heads of {cache.dim}")
+    scale = cache.dim ** -0.5 if scale is None else float(scale)
+    if not 2.0 ** -126 <= scale <= 2.0 ** 126:
+        raise ValueError("scale must be positive, from 2 ** -126 to 2 ** 126")
+    if window is not None and not 1 <= int(window) < 1 << 31:
+        raise ValueError("window must be positive")
+    _no_grad("attention_kv8", q)
+    rows, heads, device = q.shape[0], q.shape[1], cache.keys.device
+    step = _kv8_step(cache, table, past, first, rows)
+    _check_device(device, q)
+    if sinks is not None:
+        _check_rows(sinks, "sinks", (torch.float32,))
+        if sinks.shape != (heads,):
+            raise ValueError(f"sinks must hold one number for each of {heads} heads")
+        _check_device(device, sinks)
+        sinks = sinks.contiguous()
+    if rows > (0x7fffff00 // heads):
+        raise ValueError(f"{rows} rows of {heads} heads are more than an operator takes")
+    if step is None:
+        return q.new_zeros(q.shape)
+    out = q.new_empty(q.shape)
+    q = _neighbouring(q)
+    handle, rows_at = C.addressof(cache._handle), C.addressof(step)
+    need = _function("kv8_attention_work_bytes")(handle, rows_at, heads, _TYPES[q.dtype])
+    work = q.new_empty(need, dtype=torch.uint8)
+    _call("kv8_attention", device, handle, rows_at, q.data_ptr(), q.stride(0), q.stride(1), heads, _TYPES[q.dtype], scale, int(window or 0),
+          None if sinks is None else sinks.data_ptr(), out.data_ptr(), work.data_ptr(), need)
+    return out

@@ -339,6 +339,38 @@ size_t lm_b200_op_loss_grad_work_bytes(const void *h, int64_t ldh, const void *W
 int lm_b200_op_loss_grad(const void *h, int64_t ldh, const void *W, int64_t ldw, const void *targets, int targets64, int64_t ignore, int M, int V, int K, float scale,
                          const float *kept, const float *grad, int grad_stride, const float *count, void *dh, void *dW, void *work, size_t work_bytes, void *stream);
 
+/* ---- keys and values of sequences in 8 bits, and the attention over them, for callers with rows of their own ----
+ * Pages [pages][kv_heads][page_size][stride] of codes (E4M3, or two's complement), stride = dim padded to 16 with zeros, and per page and head a power of two (fp32), the same
+ * for its tokens: a number is code * scale.  The exponent is the smallest, at least -100, for which the page's largest magnitude so far is at most 448 (127) times the power; codes
+ * are to the nearest, half way to the even one.  A number that is not finite makes the scale NaN: the page's head then stands for NaNs, until its first token is written again. */
+enum lm_b200_kv8_format { LM_B200_KV8_E4M3 = 0, LM_B200_KV8_INT8 = 1 };
+typedef struct lm_b200_kv8 {
+    void *keys, *values;           /* 16-byte aligned */
+    float *key_scales, *value_scales;
+    int32_t pages, kv_heads, page_size, dim, format; /* page_size 16, 32, 64 or 128; dim 1 .. 256 */
+} lm_b200_kv8;
+/* The rows of a step (arrays on the device): sequence i has rows first[i] .. first[i + 1] of them (first NULL: row i alone, n_seq == rows), at positions past[i] and on; its page of
+ * position p is table[i * table_ld + p / page_size].  A token whose place lies beyond max_pages, or whose page is not 0 .. pages - 1, is not there: not written, not seen, zeros when
+ * read.  A sequence whose past is negative has no tokens. */
+typedef struct lm_b200_kv8_step {
+    const int32_t *table;
+    int64_t table_ld;
+    const int32_t *past, *first;
+    int32_t max_pages, n_seq, rows;
+} lm_b200_kv8_step;
+/* k, v [rows][kv_heads][dim] of `type` (neighbouring channels; k_row, k_head, .. elements from one row or head to the next) into the pages.  A page that holds earlier tokens of its
+ * sequence keeps them; they are rounded again where its exponent has to grow.  No page may belong to two sequences of a call. */
+int lm_b200_op_kv8_append(const lm_b200_kv8 *cache, const lm_b200_kv8_step *step, const void *k, int64_t k_row, int64_t k_head, const void *v, int64_t v_row, int64_t v_head,
+                          int type, void *stream);
+/* the numbers of positions past[i] and on: k, v [rows][kv_heads][dim] of `type`; rows of no sequence are zeros */
+int lm_b200_op_kv8_read(const lm_b200_kv8 *cache, const lm_b200_kv8_step *step, void *k, void *v, int type, void *stream);
+/* out [rows][heads][dim] = attention of q (the same, q_row and q_head apart, of `type`; fp32 is multiplied with 22 bits, fp16 and bf16 as they are) over the tokens at a row's position and
+ * before it, the last `window` of them (0: all): weights exp(scale q.k), in the denominator exp(sinks[head]) too (NULL: nothing).  Query head h reads key head h / (heads / kv_heads).  A row
+ * that sees nothing, and a row of no sequence, is zeros.  work: lm_b200_op_kv8_attention_work_bytes bytes, 256-byte aligned. */
+size_t lm_b200_op_kv8_attention_work_bytes(const lm_b200_kv8 *cache, const lm_b200_kv8_step *step, int heads, int type);
+int lm_b200_op_kv8_attention(const lm_b200_kv8 *cache, const lm_b200_kv8_step *step, const void *q, int64_t q_row, int64_t q_head, int heads, int type, float scale, int window,
+                             const float *sinks, void *out, void *work, size_t work_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
