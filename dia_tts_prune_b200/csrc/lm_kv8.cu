@@ -12,25 +12,13 @@
 
 #include "gemm_tcgen05.h"
 #include "lm_device.cuh"
+#include "lm_kv8.cuh"
 #include "lm_kv8.h"
 
 namespace lm {
 namespace {
 
 constexpr int kLowestExp = -100;
-
-template <int TYPE> struct ElementOf { using type = float; };
-template <> struct ElementOf<kTypeBf16> { using type = __nv_bfloat16; };
-template <> struct ElementOf<kTypeF16> { using type = __half; };
-template <int TYPE> using Element = typename ElementOf<TYPE>::type;
-
-__device__ __forceinline__ float widen(float v) { return v; }
-__device__ __forceinline__ float widen(__nv_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ float widen(__half v) { return __half2float(v); }
-template <typename E> __device__ __forceinline__ E narrow(float v);
-template <> __device__ __forceinline__ float narrow<float>(float v) { return v; }
-template <> __device__ __forceinline__ __nv_bfloat16 narrow<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
-template <> __device__ __forceinline__ __half narrow<__half>(float v) { return __float2half_rn(v); }
 
 // 2^e, e from -126 to 127; smaller ones are 0 (a code times that rounds to zero)
 __device__ __forceinline__ float power(int e) { return e < -126 ? 0.f : __uint_as_float((unsigned)(e + 127) << 23); }
@@ -57,32 +45,6 @@ __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) 
     }
     return r;
 }
-// Four codes as two pairs of fp16, which holds both formats' numbers as they are.
-template <int FORMAT>
-__device__ __forceinline__ void decode4(uint32_t w, uint32_t& lo, uint32_t& hi) {
-    if constexpr (FORMAT == kKvE4m3) {
-        asm("{\n\t.reg .b16 a, b;\n\t"
-            "mov.b32 {a, b}, %2;\n\t"
-            "cvt.rn.f16x2.e4m3x2 %0, a;\n\t"
-            "cvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
-            : "=r"(lo), "=r"(hi) : "r"(w));
-    } else {
-        const uint32_t u = w ^ 0x80808080u;                    // code + 128; with 0x64 above it, 1152 + code in fp16
-        const __half2 bias = __half2half2(__ushort_as_half(0x6480));
-        uint32_t x = __byte_perm(u, 0x64646464u, 0x4140), y = __byte_perm(u, 0x64646464u, 0x4342);
-        __half2 p = __hsub2(*reinterpret_cast<__half2*>(&x), bias), q = __hsub2(*reinterpret_cast<__half2*>(&y), bias);
-        lo = *reinterpret_cast<uint32_t*>(&p);
-        hi = *reinterpret_cast<uint32_t*>(&q);
-    }
-}
-template <int FORMAT>
-__device__ __forceinline__ float4 values4(uint32_t w, float scale) {
-    uint32_t lo, hi;
-    decode4<FORMAT>(w, lo, hi);
-    const float2 a = __half22float2(*reinterpret_cast<__half2*>(&lo)), b = __half22float2(*reinterpret_cast<__half2*>(&hi));
-    return make_float4(a.x * scale, a.y * scale, b.x * scale, b.y * scale);
-}
-
 // Eight channels of a row from channel k on, those at or beyond n are zero.  WIDE: rows of whole 16 bytes, n is a multiple of 8.
 template <int TYPE, bool WIDE>
 struct Eight {
@@ -283,7 +245,6 @@ __global__ void __launch_bounds__(kReadThreads) kv8_read_kernel(Kv8Cache c, Kv8S
 // row's largest), or two (fp32: 22 bits).  Weights: the page's value scale is part of the exponent, 2^(x + e - max (x + e)) 2^14, so that the largest contribution, not the largest
 // weight, is what fp16's 11 bits count from (fp32 rows: two terms, 22 bits); sums, maxima and outputs are fp32, and the denominator is summed from fp32 weights without the scale.
 constexpr int kRowTile = 16, kFewWarps = 4, kFewThreads = 32 * kFewWarps, kMetaBlocks = 256;
-constexpr float kLog2e = 1.4426950408889634f, kWeightBits = 14.f;
 constexpr int kMinBlocks = 8;                                  // of a CTA's run
 
 template <int DP, int TERMS>
@@ -296,21 +257,11 @@ struct Few {
     static constexpr int kCtas = DP == 256 ? 1 : DP * TERMS > 128 ? 2 : 3;
 };
 
-__device__ __forceinline__ float exp2_fast(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint32_t pack_half(float a, float b) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-
 // where 16-byte piece `c` of row `r` of a block lies
 template <int DP>
 __device__ __forceinline__ int piece_at(int r, int c) {
@@ -323,7 +274,8 @@ struct Span {
     int begin, n, past, low, blocks, tiles;                   // low: the first block
     __device__ __forceinline__ long long units(int kv_heads) const { return (long long)kv_heads * tiles * blocks; }
 };
-__device__ __forceinline__ Span span_of(const Kv8Step& s, int i, int group, int page_shift, int window) {
+__device__ __forceinline__ Span span_of(const Kv8Step& s, const Kv8Attention& a, int i, int group, int page_shift) {
+    const int window = a.window;
     Span p;
     p.begin = s.begin(i);
     p.n = max(s.end(i) - p.begin, 0);
@@ -331,7 +283,7 @@ __device__ __forceinline__ Span span_of(const Kv8Step& s, int i, int group, int 
     p.low = window > 0 ? (int)(max(0ll, (long long)p.past + 1 - window) / kKvBlock) : 0;
     const long long end = min((long long)max(p.past, 0) + p.n, (long long)s.max_pages << page_shift);
     p.blocks = max(1, (int)((end + kKvBlock - 1) / kKvBlock) - p.low);
-    p.tiles = (int)(((long long)p.n * group + kRowTile - 1) / kRowTile);
+    p.tiles = (long long)p.n * group > a.few_most ? 0 : (p.n * group + kRowTile - 1) / kRowTile;
     return p;
 }
 
@@ -340,12 +292,12 @@ struct Place {
     int seq;
     long long base, per, total;
 };
-__device__ __forceinline__ Place find_place(const Kv8Step& s, int kv_heads, int group, int page_shift, int window, int ctas, int nth) {
+__device__ __forceinline__ Place find_place(const Kv8Step& s, const Kv8Attention& a, int kv_heads, int group, int page_shift, int ctas, int nth) {
     __shared__ long long sums[kFewWarps];
     __shared__ Place found;
     const int each = (s.sequences + kFewThreads - 1) / kFewThreads, i0 = threadIdx.x * each, i1 = min(i0 + each, s.sequences);
     long long mine = 0;
-    for (int i = i0; i < i1; ++i) mine += span_of(s, i, group, page_shift, window).units(kv_heads);
+    for (int i = i0; i < i1; ++i) mine += span_of(s, a, i, group, page_shift).units(kv_heads);
     long long upto = mine;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -366,7 +318,7 @@ __device__ __forceinline__ Place find_place(const Kv8Step& s, int kv_heads, int 
         long long base = upto - mine;
         int i = i0;
         for (;; ++i) {
-            const long long u = span_of(s, i, group, page_shift, window).units(kv_heads);
+            const long long u = span_of(s, a, i, group, page_shift).units(kv_heads);
             if (unit < base + u) break;
             base += u;
         }
@@ -375,34 +327,6 @@ __device__ __forceinline__ Place find_place(const Kv8Step& s, int kv_heads, int 
     __syncthreads();
     return found;
 }
-
-// (max, max with value scales, sum) of a row in a run, as they are left for the second kernel
-struct RowStats {
-    float m, w, l;
-};
-
-__device__ __forceinline__ void store_out(const Kv8Attention& a, size_t at, float v) {
-    if (a.type == kTypeF32) reinterpret_cast<float*>(a.out)[at] = v;
-    else if (a.type == kTypeBf16) reinterpret_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(v);
-    else reinterpret_cast<__half*>(a.out)[at] = __float2half_rn(v);
-}
-__device__ __forceinline__ float load_q(const Kv8Attention& a, long long at) {
-    if (a.type == kTypeF32) return reinterpret_cast<const float*>(a.q.x)[at];
-    if (a.type == kTypeBf16) return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(a.q.x)[at]);
-    return __half2float(reinterpret_cast<const __half*>(a.q.x)[at]);
-}
-// what the sums of a row are times to be its output
-__device__ __forceinline__ float row_factor(const Kv8Attention& a, int head, float m, float w, float l) {
-    const float sink = a.sinks ? a.sinks[head] * kLog2e : -INFINITY;
-    if (sink != -INFINITY) {
-        const float top = fmaxf(m, sink);
-        l = (m == -INFINITY ? l : l * exp2_fast(m - top)) + exp2_fast(sink - top);
-        m = top;
-    }
-    if (l == 0.f || w == -INFINITY) return l != l ? l : 0.f;    // nothing was seen (or what was seen is NaN)
-    return exp2_fast(w - m - kWeightBits) / l;
-}
-__device__ __forceinline__ float lower_to(float from, float to) { return from == -INFINITY ? 0.f : exp2_fast(from - to); }      // 2^(from - to)
 
 template <int DP, int FORMAT, int TERMS>
 __global__ void __launch_bounds__(kFewThreads, Few<DP, TERMS>::kCtas) kv8_attention_few_kernel(Kv8Cache c, Kv8Step s, Kv8Attention a, float* part, RowStats* part_stats) {
@@ -420,22 +344,17 @@ __global__ void __launch_bounds__(kFewThreads, Few<DP, TERMS>::kCtas) kv8_attent
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, group = a.heads / c.kv_heads;
-    // rows of no sequence
-    if (s.first) {
-        const int begin = min(max(s.first[0], 0), s.rows), end = min(max(s.first[s.sequences], begin), s.rows), width = a.heads * c.dim;
-        for (long long i = (long long)blockIdx.x * kFewThreads + threadIdx.x; i < (long long)(begin + s.rows - end) * width; i += (long long)gridDim.x * kFewThreads)
-            store_out(a, i < (long long)begin * width ? i : i + (long long)(end - begin) * width, 0.f);
-    }
-    Place at = find_place(s, c.kv_heads, group, c.page_shift, a.window, gridDim.x, blockIdx.x);
+    zero_rows_of_none(s, a, c.dim);
+    Place at = find_place(s, a, c.kv_heads, group, c.page_shift, gridDim.x, blockIdx.x);
     if (at.seq < 0) return;
     long long unit = at.per * blockIdx.x;
     const long long unit_end = min(unit + at.per, at.total);
-    Span sp = span_of(s, at.seq, group, c.page_shift, a.window);
+    Span sp = span_of(s, a, at.seq, group, c.page_shift);
 
     while (unit < unit_end) {
         while (unit >= at.base + sp.units(c.kv_heads)) {                             // (sequences without rows have no units)
             at.base += sp.units(c.kv_heads);
-            sp = span_of(s, ++at.seq, group, c.page_shift, a.window);
+            sp = span_of(s, a, ++at.seq, group, c.page_shift);
         }
         const long long item = (unit - at.base) / sp.blocks;
         const int b0 = (int)(unit - at.base - item * sp.blocks), count = (int)min((long long)sp.blocks - b0, unit_end - unit);
@@ -705,9 +624,9 @@ __global__ void __launch_bounds__(kFewThreads) kv8_attention_join_kernel(Kv8Cach
     __shared__ __align__(16) float sums[kFewWarps][DP];
     __shared__ float totals[kFewWarps];
     const int nth = blockIdx.x + 1, r = blockIdx.y, group = a.heads / c.kv_heads, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const Place at = find_place(s, c.kv_heads, group, c.page_shift, a.window, ctas, nth);
+    const Place at = find_place(s, a, c.kv_heads, group, c.page_shift, ctas, nth);
     if (at.seq < 0) return;
-    const Span sp = span_of(s, at.seq, group, c.page_shift, a.window);
+    const Span sp = span_of(s, a, at.seq, group, c.page_shift);
     const long long item = (at.per * nth - at.base) / sp.blocks, start = at.base + item * sp.blocks;
     const int c0 = (int)(start / at.per), c1 = (int)((start + sp.blocks - 1) / at.per);
     const int head = (int)(item / sp.tiles), tile = (int)(item - (long long)head * sp.tiles), p = tile * kRowTile + r;
@@ -814,14 +733,29 @@ cudaError_t launch_kv8_read(const Kv8Cache& c, const Kv8Step& s, void* k, void* 
     return cudaGetLastError();
 }
 
-size_t kv8_attention_work_bytes(const Kv8Cache& c, const Kv8Step&, int, int type) {
+namespace {
+// Pairs of a sequence from which on tiles of 256 rows are the shorter way
+constexpr int kFewMost = 64;
+inline bool some_in_tiles(const Kv8Cache& c, const Kv8Step& s, int heads, int type) { return kv8_tiles_ok(c, type) && (long long)s.rows * (heads / c.kv_heads) > kFewMost; }
+}  // namespace
+
+size_t kv8_attention_work_bytes(const Kv8Cache& c, const Kv8Step& s, int heads, int type) {
     const int dp = padded_dim(c);
-    return (size_t)2 * few_ctas(dp, terms_of(type)) * 16 * (dp * sizeof(float) + sizeof(RowStats));
+    const size_t few = (size_t)2 * few_ctas(dp, terms_of(type)) * 16 * (dp * sizeof(float) + sizeof(RowStats));
+    return some_in_tiles(c, s, heads, type) ? std::max(few, kv8_tiles_work_bytes(c)) : few;
 }
 
-cudaError_t launch_kv8_attention(const Kv8Cache& c, const Kv8Step& s, const Kv8Attention& a, void* work, cudaStream_t st) {
+cudaError_t launch_kv8_attention(const Kv8Cache& c, const Kv8Step& s, Kv8Attention a, void* work, cudaStream_t st) {
     const int dp = padded_dim(c);
     const bool two = terms_of(a.type) == 2;
+    a.few_most = 0x7fffffff;
+    if (some_in_tiles(c, s, a.heads, a.type)) {
+        const bool alone = s.sequences == 1;                  // (then whatever its rows are)
+        a.few_most = alone ? 0 : kFewMost;
+        const cudaError_t e = launch_kv8_tiles(c, s, a, alone, work, st);
+        if (e != cudaSuccess || alone) return e;
+        ++dia::extra_launches();
+    }
 #define KV8_FEW(DP, FORMAT) (two ? run_few<DP, FORMAT, 2>(c, s, a, work, st) : run_few<DP, FORMAT, 1>(c, s, a, work, st))
     if (c.format == kKvE4m3) return dp == 64 ? KV8_FEW(64, kKvE4m3) : dp == 128 ? KV8_FEW(128, kKvE4m3) : KV8_FEW(256, kKvE4m3);
     return dp == 64 ? KV8_FEW(64, kKvInt8) : dp == 128 ? KV8_FEW(128, kKvInt8) : KV8_FEW(256, kKvInt8);

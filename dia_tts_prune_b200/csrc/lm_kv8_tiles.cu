@@ -1,0 +1,640 @@
+// lm_kv8_tiles.cu - attention of many rows over the cache in 8 bits, on the 5th-generation tensor cores.
+//
+// A CTA takes 256 (token, query head) rows that share a key head and walks their keys 128 at a time:
+//   warps 0-3, 4-7   one thread per row, 128 rows each: scores from tensor memory, softmax weights back to it.  The two halves are in different stages of a tile, so that the
+//                    tensor cores have one half's products while the other half takes exponentials
+//   warps 8-11       codes from pages to fp16 operands in shared memory, 32 tokens each; the next tile's are on their way while they do it
+//   warp 12          one elected lane issues tcgen05.mma: S = Q K^T (M = 128, N = 128), then O += P V with P as the operand in tensor memory, where S lay
+//
+// Numbers.  t = scale log2(e) q . key + e - E in powers of two, e the exponent of the page's values and E the largest of the CTA's pages; P = 2^(t - R + 7) in fp16, with R the
+// row's reference: its largest t so far, raised (and O and the sum with it) only when one lies more than 2^8 above it, so P is at most 2^15.  That the page's value scale is inside
+// the weight lets codes be multiplied as they are, and the 11 bits of P count from the largest contribution.  The denominator takes 2^(E - e) out again, per 16 tokens.  Pages whose
+// values are 2^80 below the largest page's are taken as zeros.  Queries are scaled by a power of two per row (exact but for channels 2^-27 below the row's largest).  Sums are fp32;
+// O's live in tensor memory for the whole run of keys, and lose up to one unit in the last place per 16 keys (2^-24 on average: 2^-11 of the sum after 131072 keys, against the
+// 2^-9 of bf16).
+//
+// Bound: per 256 x 128 tile and dim 128 the tensor pipe takes 2048 cycles, the exponentials (16 a cycle) 2048, and shared memory 2048 (the scores' operands 1024, the values 512,
+// the codes turned into operands 512).
+#include <algorithm>
+
+#include "attention_split.h"
+#include "engine_internal.h"
+#include "gemm_tcgen05.h"
+#include "lm_device.cuh"
+#include "lm_kv8.cuh"
+#include "lm_kv8.h"
+#include "tensor_cores.cuh"
+
+namespace lm {
+namespace {
+
+using namespace dia;
+
+constexpr int kKeys = 128, kHalfRows = 128, kTileRows = 2 * kHalfRows, kThreads = 512, kSms = 148;
+constexpr int kBlocks = kKeys / kKvBlock;                      // blocks of 16 tokens in a tile of keys
+constexpr int kMinChunk = 4;                                   // tiles of keys that are worth a CTA of their own
+constexpr float kSlack = 8.f, kBits = 7.f, kSpread = 80.f;     // see above
+constexpr int kSoftmaxRegs = 184, kFetchRegs = 96, kIssueRegs = 48;
+static_assert(128 * (2 * kSoftmaxRegs + kFetchRegs + kIssueRegs) == kThreads * 128, "the split is the launch's registers");
+
+template <int DP>
+struct Tiles {
+    static constexpr int kStages = DP == 64 ? 4 : 2, kSide = kKeys * DP * 2, kQ = kTileRows * DP * 2;
+    static constexpr int kSmem = kQ + kStages * 2 * kSide + 1024;
+};
+
+// ---- who takes what ------------------------------------------------------------------------------------------------------------------------
+// Items are (sequence, key head, 256 rows).  Where there are fewer than SMs, the keys of an item go in chunks, as many as all of them fill the GPU once with; a second kernel
+// joins the chunks.  Items of a sequence go last rows first: those see the most keys.
+struct Sequence {
+    int begin, n, past, tiles, low, high;                     // low, high: tiles of keys that its rows look at
+};
+__device__ __forceinline__ Sequence sequence_at(const Kv8Step& s, const Kv8Attention& a, int i, int group, int page_shift) {
+    Sequence q;
+    q.begin = s.begin(i);
+    q.n = max(s.end(i) - q.begin, 0);
+    q.past = s.past[i];
+    const long long rows = (long long)q.n * group;
+    q.tiles = rows > a.few_most ? (int)((rows + kTileRows - 1) / kTileRows) : 0;
+    q.low = a.window > 0 ? (int)(max(0ll, (long long)q.past + 1 - a.window) / kKeys) : 0;
+    const long long end = min((long long)max(q.past, 0) + q.n, (long long)s.max_pages << page_shift);
+    q.high = q.past < 0 ? q.low : max((int)((end + kKeys - 1) / kKeys), q.low);
+    return q;
+}
+struct Work {
+    int seq, head, tile, chunk, chunks, first_cta, length;    // seq -1: nothing
+};
+template <int THREADS>
+__device__ __forceinline__ long long scan(long long mine, long long* sums, long long& total) {      // sum of the threads before this one
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    long long upto = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const long long o = __shfl_up_sync(0xffffffffu, upto, d);
+        if (lane >= d) upto += o;
+    }
+    if (lane == 31) sums[warp] = upto;
+    __syncthreads();
+    total = 0;
+#pragma unroll 1
+    for (int w = 0; w < THREADS / 32; ++w) {
+        if (w < warp) upto += sums[w];
+        total += sums[w];
+    }
+    __syncthreads();
+    return upto - mine;
+}
+// JOIN: `index` counts items, and only where there are chunks to join; else it counts CTAs
+template <int THREADS, bool JOIN>
+__device__ __forceinline__ Work find_work(const Kv8Cache& c, const Kv8Step& s, const Kv8Attention& a, int group, long long index) {
+    __shared__ long long sums[THREADS / 32];
+    __shared__ int longest;
+    __shared__ Work found;
+    if (threadIdx.x == 0) {
+        longest = 0;
+        found.seq = -1;
+    }
+    __syncthreads();
+    const int each = (s.sequences + THREADS - 1) / THREADS, i0 = threadIdx.x * each, i1 = min(i0 + each, s.sequences);
+    long long items = 0, total_items, ctas = 0, total;
+    int most = 0;
+    for (int i = i0; i < i1; ++i) {
+        const Sequence q = sequence_at(s, a, i, group, c.page_shift);
+        items += (long long)q.tiles * c.kv_heads;
+        if (q.tiles) most = max(most, q.high - q.low);
+    }
+    if (most) atomicMax(&longest, most);
+    const long long items_before = scan<THREADS>(items, sums, total_items);
+    if (total_items == 0 || (JOIN && total_items >= kSms)) return found;
+    const int length = total_items >= kSms ? 0x7fffffff : max(kMinChunk, (longest + kSms / (int)total_items - 1) / (kSms / (int)total_items));
+    const auto chunks_of = [&](const Sequence& q) { return length == 0x7fffffff ? 1 : max(1, (q.high - q.low + length - 1) / length); };
+    for (int i = i0; i < i1; ++i) {
+        const Sequence q = sequence_at(s, a, i, group, c.page_shift);
+        ctas += (long long)q.tiles * c.kv_heads * chunks_of(q);
+    }
+    const long long before = scan<THREADS>(ctas, sums, total);
+    long long base = JOIN ? items_before : before, cta = before;
+    if (index >= base && index < base + (JOIN ? items : ctas)) {
+        for (int i = i0;; ++i) {
+            const Sequence q = sequence_at(s, a, i, group, c.page_shift);
+            const int chunks = chunks_of(q);
+            const long long own = (long long)q.tiles * c.kv_heads, units = JOIN ? own : own * chunks;
+            if (index < base + units) {
+                const long long local = index - base, item = JOIN ? local : local / chunks;
+                found = {i, (int)(item % c.kv_heads), q.tiles - 1 - (int)(item / c.kv_heads), JOIN ? 0 : (int)(local % chunks), chunks, (int)(cta + item * chunks), length};
+                break;
+            }
+            base += units;
+            cta += own * chunks;
+        }
+    }
+    __syncthreads();
+    return found;
+}
+
+// ---- tensor memory and shared memory -------------------------------------------------------------------------------------------------------
+
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tmem_loaded() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_stored() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_load32(uint32_t addr, float* v) {
+    uint32_t u[32];
+    tmem_columns32(addr, u);
+#pragma unroll
+    for (int e = 0; e < 32; ++e) v[e] = __uint_as_float(u[e]);
+}
+__device__ __forceinline__ void tmem_store32(uint32_t addr, const uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(addr),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]),
+        "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]),
+        "r"(v[29]), "r"(v[30]), "r"(v[31])
+        : "memory");
+}
+// Operands lie in blocks of 8 rows x 16 bytes, [row / 8][channel / 8]: lead / stride are the bytes between blocks along the contraction / the rows (scores: the contraction runs
+// over channels; values: over rows, and the channels are what is far apart)
+__device__ __forceinline__ uint64_t block_desc(uint32_t addr, uint32_t lead, uint32_t stride) {
+    const uint32_t lo = ((addr & 0x3FFFFu) >> 4) | ((lead >> 4) << 16), hi = (stride >> 4) | (1u << 14);
+    return ((uint64_t)hi << 32) | lo;
+}
+__device__ __forceinline__ void mma_weights(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {      // A in tensor memory
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+template <int DP, int FORMAT>
+__global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cache c, Kv8Step s, Kv8Attention a, int alone, float* part, RowStats* part_stats, int* ran_out, unsigned polls) {
+    using T = Tiles<DP>;
+    constexpr int kStages = T::kStages, kSteps = DP / 16;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    uint8_t* const q_tile = smem;                             // [half]
+    uint8_t* const k_ring = smem + T::kQ;
+    uint8_t* const v_ring = k_ring + kStages * T::kSide;
+    __shared__ uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], s_full[2], p_ready[2], pv_done[2], done;
+    __shared__ uint32_t tmem_slot;
+    __shared__ int largest;                                   // exponent of the values' pages
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = a.heads / c.kv_heads;
+    if (alone) zero_rows_of_none(s, a, c.dim);
+    const Work work = find_work<kThreads, false>(c, s, a, group, blockIdx.x);
+    if (work.seq < 0) return;
+    const Sequence q = sequence_at(s, a, work.seq, group, c.page_shift);
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kStages; ++i) {
+            mbar_init(&k_full[i], 4);
+            mbar_init(&v_full[i], 4);
+            mbar_init(&k_empty[i], 1);
+            mbar_init(&v_empty[i], 1);
+        }
+        for (int g = 0; g < 2; ++g) {
+            mbar_init(&s_full[g], 1);
+            mbar_init(&p_ready[g], 4);
+            mbar_init(&pv_done[g], 1);
+        }
+        mbar_init(&done, 1);
+        largest = -1000;
+        fence_mbar_init();
+    }
+    if (warp == 12) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&tmem_slot)));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+    }
+    // tiles of keys: the first one, and how many of them the halves of the rows look at
+    const int pairs = q.n * group, p0 = work.tile * kTileRows;
+    const auto position = [&](int p) { return (long long)q.past + min(p, pairs - 1) / group; };
+    const long long back = a.window > 0 ? a.window - 1 : (1ll << 40);
+    const int from = max(max(q.low, (int)(max(0ll, position(p0) - back) / kKeys)), work.length == 0x7fffffff ? 0 : q.low + work.chunk * work.length);
+    const int limit = work.length == 0x7fffffff ? q.high : (int)min((long long)q.high, (long long)q.low + (long long)(work.chunk + 1) * work.length);
+    const auto tiles_of = [&](int g) {
+        if (p0 + g * kHalfRows >= pairs || q.past < 0) return 0;
+        return (int)max(0ll, min((long long)limit, position(p0 + g * kHalfRows + kHalfRows - 1) / kKeys + 1) - from);
+    };
+    const int n0 = tiles_of(0), n1 = tiles_of(1), n = max(n0, n1);
+    __syncthreads();                                          // (the largest exponent is set)
+    {
+        int most = -1000;
+        for (int b = threadIdx.x; b < n * kBlocks; b += kThreads) {
+            const int page = s.page(work.seq, ((long long)from * kKeys + (long long)b * kKvBlock) >> c.page_shift, c.pages);
+            if (page < 0) continue;
+            const uint32_t v = __float_as_uint(c.value_scales[(size_t)page * c.kv_heads + work.head]);
+            if (v < 0x7f800000u) most = max(most, (int)(v >> 23) - 127);
+        }
+        most = __reduce_max_sync(0xffffffffu, most);
+        if (lane == 0 && most > -1000) atomicMax(&largest, most);
+    }
+    // queries: a thread takes its row
+    float row_scale = 0.f;
+    if (warp < 8) {
+        const int r = threadIdx.x, p = p0 + r;
+        uint8_t* const to = q_tile + (r >> 7) * (kHalfRows * DP * 2) + ((r & 127) >> 3) * (DP * 16) + (r & 7) * 16;
+        const long long at = (q.begin + (long long)(min(p, pairs - 1) / group)) * a.q.row + (long long)(work.head * group + min(p, pairs - 1) % group) * a.q.head;
+        const bool wide = c.dim % 8 == 0 && (reinterpret_cast<uintptr_t>(a.q.x) & 15) == 0 && a.q.row % 8 == 0 && a.q.head % 8 == 0;
+        uint4 w[DP / 8];
+#pragma unroll
+        for (int j = 0; j < DP / 8; ++j) {
+            w[j] = make_uint4(0u, 0u, 0u, 0u);
+            if (p < pairs) {
+                const uint16_t* const x = reinterpret_cast<const uint16_t*>(a.q.x) + at + 8 * j;
+                if (wide) {
+                    if (8 * j < c.dim) w[j] = *reinterpret_cast<const uint4*>(x);
+                } else {
+                    uint16_t y[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) y[e] = 8 * j + e < c.dim ? x[e] : 0;
+                    memcpy(&w[j], y, 16);
+                }
+            }
+        }
+        const auto numbers = [&](uint32_t u) {
+            if (a.type == kTypeBf16) return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+            return __half22float2(*reinterpret_cast<const __half2*>(&u));
+        };
+        uint32_t most = 0;
+#pragma unroll
+        for (int j = 0; j < DP / 8; ++j) {
+            const uint32_t u[4] = {w[j].x, w[j].y, w[j].z, w[j].w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float2 f = numbers(u[e]);
+                most = max(most, max(__float_as_uint(f.x) & 0x7fffffffu, __float_as_uint(f.y) & 0x7fffffffu));
+            }
+        }
+        const uint32_t e = most == 0 ? 127u : max(most >> 23, 14u);
+        const float f = __uint_as_float((267u - e) << 23), way_back = __uint_as_float((e - 13u) << 23);       // 2^(140 - e): to below 2^14, and the way back
+        row_scale = e == 255u ? __uint_as_float(0x7fc00000u) : way_back * (a.scale * kLog2e);
+#pragma unroll
+        for (int j = 0; j < DP / 8; ++j) {
+            uint32_t u[4] = {w[j].x, w[j].y, w[j].z, w[j].w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float2 y = numbers(u[i]);
+                u[i] = e == 255u ? 0u : pack_half(y.x * f, y.y * f);
+            }
+            *reinterpret_cast<uint4*>(to + j * 128) = make_uint4(u[0], u[1], u[2], u[3]);
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = tmem_slot;                          // scores (and weights) of the halves 0, 128; outputs 256, 384
+    const float spread = (float)(largest == -1000 ? 0 : largest);
+    bool ok = true;
+
+    if (warp < 8) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+        const int g = warp >> 2, count = g ? n1 : n0;
+        const uint32_t lanes = (uint32_t)(warp & 3) * 32u << 16, t_s = tmem + lanes + 128u * g, t_o = tmem + lanes + 256u + 128u * g;
+        const int p = p0 + threadIdx.x;
+        const long long pos = position(p), first_pos = position(p0 + g * kHalfRows), last_pos = position(p0 + g * kHalfRows + kHalfRows - 1);
+        float ref = -1e30f, l = 0.f;
+        // lanes 0 .. 7 hold a block's scales each, looked up a tile ahead, and its page two tiles ahead
+        const auto page_of = [&](int i) {
+            if (lane >= kBlocks || i >= count) return -1;
+            return s.page(work.seq, (((long long)from + i) * kKeys + lane * kKvBlock) >> c.page_shift, c.pages);
+        };
+        const auto scales_of = [&](int page, float& ks, float& ev) {
+            ks = ev = 0.f;
+            if (page < 0) return;
+            const size_t at = (size_t)page * c.kv_heads + work.head;
+            const uint32_t v = __float_as_uint(c.value_scales[at]);
+            ks = c.key_scales[at];
+            ev = v >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : fmaxf((float)((int)(v >> 23) - 127) - spread, -kSpread);
+        };
+        int page = page_of(0), page_next = page_of(1);
+        float ks, ev;
+        scales_of(page, ks, ev);
+#pragma unroll 1
+        for (int i = 0; i < count; ++i) {
+            const uint32_t there = __ballot_sync(0xffffffffu, page >= 0) & 0xffu;
+            const float ks_now = ks, ev_now = ev;
+            page = page_next;
+            scales_of(page, ks, ev);
+            page_next = page_of(i + 2);
+            const long long tok = ((long long)from + i) * kKeys;
+            const bool clear = there == 0xffu && tok + kKeys - 1 <= first_pos && tok >= last_pos - back;
+            if (!pair_wait(&s_full[g], i & 1, polls)) { ok = false; break; }
+            fence_after();
+            float x[kKeys];
+#pragma unroll
+            for (int j = 0; j < kKeys; j += 32) tmem_load32(t_s + j, x + j);
+            tmem_loaded();
+            if (!clear) {
+                const int hi = (int)min(pos - tok, (long long)kKeys), lo = (int)max(pos - back - tok, -1ll);
+#pragma unroll
+                for (int e = 0; e < kKeys; ++e)
+                    if (e > hi || e < lo || !(there >> (e / kKvBlock) & 1u)) x[e] = -INFINITY;
+            }
+            float top = -INFINITY, kb[kBlocks];
+#pragma unroll
+            for (int b = 0; b < kBlocks; ++b) {
+                float m = x[16 * b];
+#pragma unroll
+                for (int e = 1; e < kKvBlock; ++e) m = fmaxf(m, x[16 * b + e]);
+                kb[b] = __shfl_sync(0xffffffffu, ks_now, b) * row_scale;
+                top = fmaxf(top, fmaf(m, kb[b], __shfl_sync(0xffffffffu, ev_now, b)));
+            }
+            if (__any_sync(0xffffffffu, top > ref + kSlack)) {
+                const float next = top > ref + kSlack ? top : ref, f = exp2_fast(ref - next);
+                ref = next;
+                l *= f;
+                if (i > 0) {
+                    if (!pair_wait(&pv_done[g], (i - 1) & 1, polls)) { ok = false; break; }
+                    fence_after();
+#pragma unroll 1
+                    for (int j = 0; j < DP; j += 32) {
+                        uint32_t o[32];
+                        tmem_columns32(t_o + j, o);
+                        tmem_loaded();
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                        tmem_store32(t_o + j, o);
+                    }
+                }
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                uint32_t w[32];
+#pragma unroll
+                for (int b4 = 0; b4 < 4; ++b4) {
+                    const int b = 4 * h + b4;
+                    const float e0 = __shfl_sync(0xffffffffu, ev_now, b);
+                    const f2 k2 = twice(kb[b]), c2 = twice(e0 - ref + kBits);
+                    f2 sum = 0;
+#pragma unroll
+                    for (int e = 0; e < kKvBlock; e += 2) {
+                        float y0, y1;
+                        unpack2(fma2(pack2(x[16 * b + e], x[16 * b + e + 1]), k2, c2), y0, y1);
+                        y0 = exp2_fast(y0);
+                        y1 = exp2_fast(y1);
+                        if (!clear) {
+                            if (x[16 * b + e] == -INFINITY) y0 = 0.f;
+                            if (x[16 * b + e + 1] == -INFINITY) y1 = 0.f;
+                        }
+                        sum = add2(sum, pack2(y0, y1));
+                        w[8 * b4 + e / 2] = pack_half(y0, y1);
+                    }
+                    float s0, s1;
+                    unpack2(sum, s0, s1);
+                    l = fmaf(s0 + s1, e0 == e0 ? __uint_as_float((uint32_t)(127 - (int)e0) << 23) : 1.f, l);
+                }
+                tmem_store32(t_s + 32 * h, w);
+            }
+            tmem_stored();
+            fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_ready[g]);
+        }
+        if (ok && count > 0 && !pair_wait(&pv_done[g], (count - 1) & 1, polls)) ok = false;
+        fence_after();
+        // out
+        float m = ref - kBits, w = m + spread + kWeightBits;
+        if (l == 0.f) m = w = -INFINITY;
+        const bool in = p < pairs, whole = work.chunks == 1;
+        const int h = work.head * group + min(p, pairs - 1) % group;
+        const size_t to = ((size_t)(q.begin + min(p, pairs - 1) / group) * a.heads + h) * c.dim;
+        float f = whole ? row_factor(a, h, m, w, l) : 1.f;
+        if (!ok) f = __uint_as_float(0x7fc00000u);
+        const size_t slot = ((size_t)work.first_cta + work.chunk) * kTileRows + threadIdx.x;
+        if (!whole && in) part_stats[slot] = {m, w, l};
+        const bool wide = c.dim % 8 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;
+#pragma unroll 1
+        for (int j = 0; j < DP; j += 32) {
+            float o[32];
+            if (count > 0) {
+                tmem_load32(t_o + j, o);
+                tmem_loaded();
+            } else {
+#pragma unroll
+                for (int e = 0; e < 32; ++e) o[e] = 0.f;
+            }
+            if (!in) continue;
+            if (!whole) {
+#pragma unroll
+                for (int e = 0; e < 32; e += 4) *reinterpret_cast<float4*>(part + slot * DP + j + e) = make_float4(o[e] * f, o[e + 1] * f, o[e + 2] * f, o[e + 3] * f);
+            } else if (wide) {
+                uint16_t* const y = reinterpret_cast<uint16_t*>(a.out) + to + j;
+#pragma unroll
+                for (int e = 0; e < 32; e += 8) {
+                    if (j + e >= c.dim) break;
+                    uint32_t u[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const float y0 = o[e + 2 * k] * f, y1 = o[e + 2 * k + 1] * f;
+                        if (a.type == kTypeBf16) {
+                            const __nv_bfloat162 b = __floats2bfloat162_rn(y0, y1);
+                            u[k] = *reinterpret_cast<const uint32_t*>(&b);
+                        } else {
+                            u[k] = pack_half(y0, y1);
+                        }
+                    }
+                    *reinterpret_cast<uint4*>(y + e) = make_uint4(u[0], u[1], u[2], u[3]);
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 32; ++e)
+                    if (j + e < c.dim) store_out(a, to + j + e, o[e] * f);
+            }
+        }
+    } else if (warp < 12) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFetchRegs));
+        // ---- codes to operands: 32 tokens of every tile, eight rows of a block a turn, a lane 16 channels of one ----
+        constexpr int kParts = DP / 64;                       // 16-byte pieces of a row that a lane takes
+        const int mine = (warp - 8) * 32, sub = lane & 7, piece = lane >> 3;
+        uint4 kc[4][kParts], vc[4][kParts];
+        const auto page_of = [&](int i, int b) { return i < n ? s.page(work.seq, (((long long)from + i) * kKeys + mine + b * kKvBlock) >> c.page_shift, c.pages) : -1; };
+        const auto fetch = [&](uint4 (&codes)[4][kParts], const uint8_t* side, int i, int pa, int pb) {
+#pragma unroll
+            for (int r8 = 0; r8 < 4; ++r8) {
+                const int page = r8 < 2 ? pa : pb;
+                const int in_page = (int)((((long long)from + i) * kKeys + mine + r8 * 8 + sub) & ((1 << c.page_shift) - 1));
+                const uint8_t* const row = side + ((((size_t)max(page, 0) * c.kv_heads + work.head) << c.page_shift) + in_page) * c.stride;
+#pragma unroll
+                for (int j = 0; j < kParts; ++j) {
+                    const int at = (piece + 4 * j) * 16;
+                    codes[r8][j] = page >= 0 && at < c.stride ? *reinterpret_cast<const uint4*>(row + at) : make_uint4(0u, 0u, 0u, 0u);
+                }
+            }
+        };
+        const auto lay = [&](const uint4 (&codes)[4][kParts], uint8_t* to, bool drop_a, bool drop_b) {
+#pragma unroll
+            for (int r8 = 0; r8 < 4; ++r8) {
+                const bool drop = r8 < 2 ? drop_a : drop_b;
+#pragma unroll
+                for (int j = 0; j < kParts; ++j) {
+                    const uint32_t w[4] = {codes[r8][j].x, codes[r8][j].y, codes[r8][j].z, codes[r8][j].w};
+                    uint32_t u[8];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) decode4<FORMAT>(drop ? 0u : w[e], u[2 * e], u[2 * e + 1]);
+                    uint8_t* const at = to + (mine / 8 + r8) * (DP * 16) + (piece + 4 * j) * 256 + sub * 16;
+                    *reinterpret_cast<uint4*>(at) = make_uint4(u[0], u[1], u[2], u[3]);
+                    *reinterpret_cast<uint4*>(at + 128) = make_uint4(u[4], u[5], u[6], u[7]);
+                }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+        };
+        const auto value_scale = [&](int page) { return page >= 0 ? __float_as_uint(c.value_scales[(size_t)page * c.kv_heads + work.head]) : 0u; };
+        const auto dropped = [&](uint32_t v) { return v < 0x7f800000u && (float)((int)(v >> 23) - 127) - spread < -kSpread; };
+        int pa = page_of(0, 0), pb = page_of(0, 1), na = page_of(1, 0), nb = page_of(1, 1);
+        fetch(kc, c.keys, 0, pa, pb);
+        fetch(vc, c.values, 0, pa, pb);
+        uint32_t va = value_scale(pa), vb = value_scale(pb);
+#pragma unroll 1
+        for (int i = 0; i < n; ++i) {
+            const int st = i % kStages;
+            const uint32_t use = (uint32_t)(i / kStages);
+            if (i >= kStages && !pair_wait(&k_empty[st], (use + 1) & 1, polls)) { ok = false; break; }
+            lay(kc, k_ring + st * T::kSide, false, false);
+            if (lane == 0) mbar_arrive(&k_full[st]);
+            if (i + 1 < n) fetch(kc, c.keys, i + 1, na, nb);
+            if (i >= kStages && !pair_wait(&v_empty[st], (use + 1) & 1, polls)) { ok = false; break; }
+            lay(vc, v_ring + st * T::kSide, dropped(va), dropped(vb));
+            if (lane == 0) mbar_arrive(&v_full[st]);
+            if (i + 1 < n) fetch(vc, c.values, i + 1, na, nb);
+            va = value_scale(na);
+            vb = value_scale(nb);
+            na = page_of(i + 2, 0);
+            nb = page_of(i + 2, 1);
+        }
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
+        if (warp == 12) {
+            const uint32_t idesc_s = (1u << 4) | ((uint32_t)(kKeys >> 3) << 17) | ((uint32_t)(kHalfRows >> 4) << 24);
+            const uint32_t idesc_o = (1u << 4) | (1u << 16) | ((uint32_t)(DP >> 3) << 17) | ((uint32_t)(kHalfRows >> 4) << 24);
+            const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0), q_at = smem_u32(q_tile), k_at = smem_u32(k_ring), v_at = smem_u32(v_ring);
+            const int u0 = __shfl_sync(0xffffffffu, n0, 0), u1 = __shfl_sync(0xffffffffu, n1, 0), un = max(u0, u1);
+            // scores of tile i for half g; behind the last half the slot is free when they are there
+            const auto scores = [&](int g, int i) {
+                if (i >= un) return;
+                if (!pair_wait(&k_full[i % kStages], (uint32_t)(i / kStages) & 1u, polls)) { ok = false; return; }
+                fence_after();
+                if (elect_one_sync()) {
+                    if (i < (g ? u1 : u0)) {
+                        const uint64_t qd = block_desc(q_at + g * (kHalfRows * DP * 2), 128u, DP * 16u), kd = block_desc(k_at + (i % kStages) * T::kSide, 128u, DP * 16u);
+#pragma unroll
+                        for (uint32_t k = 0; k < kSteps; ++k) umma_bf16(tm + 128u * g, qd + 16u * k, kd + 16u * k, idesc_s, k != 0);
+                        umma_commit(&s_full[g]);
+                    }
+                    if (g == 1) umma_commit(&k_empty[i % kStages]);
+                }
+                __syncwarp();
+            };
+            const auto values = [&](int g, int i) {
+                if (i < (g ? u1 : u0) && !pair_wait(&p_ready[g], i & 1, polls)) { ok = false; return; }
+                if (!pair_wait(&v_full[i % kStages], (uint32_t)(i / kStages) & 1u, polls)) { ok = false; return; }
+                fence_after();
+                if (elect_one_sync()) {
+                    if (i < (g ? u1 : u0)) {
+                        const uint64_t vd = block_desc(v_at + (i % kStages) * T::kSide, DP * 16u, 128u);
+#pragma unroll
+                        for (uint32_t k = 0; k < kKeys / 16; ++k) mma_weights(tm + 256u + 128u * g, tm + 128u * g + 8u * k, vd + 2u * DP * k, idesc_o, (i | k) != 0);
+                        umma_commit(&pv_done[g]);
+                    }
+                    if (g == 1) umma_commit(&v_empty[i % kStages]);
+                }
+                __syncwarp();
+            };
+            scores(0, 0);
+            if (ok) scores(1, 0);
+#pragma unroll 1
+            for (int i = 0; ok && i < un; ++i) {
+#pragma unroll 1
+                for (int g = 0; ok && g < 2; ++g) {
+                    values(g, i);
+                    if (ok) scores(g, i + 1);
+                }
+            }
+            mmas_ended<false>(&done);
+        }
+    }
+    if (!ok && lane == 0 && ran_out) {
+        *reinterpret_cast<volatile int*>(ran_out) = 1;
+        __threadfence_system();
+    }
+    __syncwarp();
+    fence_before();
+    __syncthreads();
+    if (warp == 12) {
+        fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+    }
+}
+
+// The chunks of an item: a warp per row
+constexpr int kJoinThreads = 256, kJoinCtas = 8;
+template <int DP>
+__global__ void __launch_bounds__(kJoinThreads) kv8_attention_tiles_join_kernel(Kv8Cache c, Kv8Step s, Kv8Attention a, const float* part, const RowStats* part_stats) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int group = a.heads / c.kv_heads, lane = threadIdx.x & 31;
+    const Work work = find_work<kJoinThreads, true>(c, s, a, group, blockIdx.x);
+    if (work.seq < 0 || work.chunks == 1) return;
+    const Sequence q = sequence_at(s, a, work.seq, group, c.page_shift);
+    for (int r = blockIdx.y * (kJoinThreads / 32) + (threadIdx.x >> 5); r < kTileRows; r += kJoinCtas * (kJoinThreads / 32)) {
+        const int p = work.tile * kTileRows + r;
+        if (p >= q.n * group) return;
+        float m = -INFINITY, w = -INFINITY, l = 0.f, sum[DP / 32] = {};
+        for (int i = lane; i < work.chunks; i += 32) {
+            const RowStats y = part_stats[(size_t)(work.first_cta + i) * kTileRows + r];
+            m = fmaxf(m, y.m);
+            w = fmaxf(w, y.w);
+        }
+#pragma unroll
+        for (int d = 16; d; d >>= 1) {
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+            w = fmaxf(w, __shfl_xor_sync(0xffffffffu, w, d));
+        }
+#pragma unroll 4
+        for (int i = 0; i < work.chunks; ++i) {
+            const size_t slot = (size_t)(work.first_cta + i) * kTileRows + r;
+            const RowStats y = part_stats[slot];
+            const float f = lower_to(y.w, w);
+            l += y.l * lower_to(y.m, m);
+#pragma unroll
+            for (int j = 0; j < DP / 32; ++j) sum[j] += f * part[slot * DP + lane + 32 * j];
+        }
+        const int h = work.head * group + p % group;
+        const float f = row_factor(a, h, m, w, l);
+#pragma unroll
+        for (int j = 0; j < DP / 32; ++j)
+            if (lane + 32 * j < c.dim) store_out(a, ((size_t)(q.begin + p / group) * a.heads + h) * c.dim + lane + 32 * j, f * sum[j]);
+    }
+}
+
+template <int DP, int FORMAT>
+cudaError_t run_tiles(const Kv8Cache& c, const Kv8Step& s, const Kv8Attention& a, bool alone, void* work, cudaStream_t st) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess) e = ask_smem<kv8_attention_tiles_kernel<DP, FORMAT>>(dev, Tiles<DP>::kSmem);
+    if (e != cudaSuccess) return e;
+    int* const ran_out = split_attention_ran_out(dev, st);
+    if (take_ran_out(dev, st)) return cudaErrorLaunchTimeout;
+    float* const part = reinterpret_cast<float*>(work);
+    RowStats* const stats = reinterpret_cast<RowStats*>(part + (size_t)kSms * kTileRows * DP);
+    // items there may be: full ones, and one that is not for every sequence that has enough rows
+    const long long pairs = (long long)s.rows * (a.heads / c.kv_heads), partly = std::min<long long>(s.sequences, pairs / (a.few_most + 1));
+    const long long ctas = std::max<long long>(kSms, c.kv_heads * (pairs / kTileRows + partly));
+    if (ctas > 0x7fffffff) return cudaErrorInvalidValue;
+    kv8_attention_tiles_kernel<DP, FORMAT><<<(unsigned)ctas, kThreads, Tiles<DP>::kSmem, st>>>(c, s, a, alone, part, stats, ran_out, gemm_pair_polls());
+    e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+    ++extra_launches();
+    return launch_pdl(kv8_attention_tiles_join_kernel<DP>, dim3(kSms, kJoinCtas), dim3(kJoinThreads), 0, st, c, s, a, part, stats);
+}
+
+}  // namespace
+
+bool kv8_tiles_ok(const Kv8Cache& c, int type) { return c.dim <= 128 && type != kTypeF32; }
+
+size_t kv8_tiles_work_bytes(const Kv8Cache& c) { return (size_t)kSms * kTileRows * ((c.dim <= 64 ? 64 : 128) * sizeof(float) + sizeof(RowStats)); }
+
+cudaError_t launch_kv8_tiles(const Kv8Cache& c, const Kv8Step& s, const Kv8Attention& a, bool alone, void* work, cudaStream_t st) {
+    if (c.dim <= 64) return c.format == kKvE4m3 ? run_tiles<64, kKvE4m3>(c, s, a, alone, work, st) : run_tiles<64, kKvInt8>(c, s, a, alone, work, st);
+    return c.format == kKvE4m3 ? run_tiles<128, kKvE4m3>(c, s, a, alone, work, st) : run_tiles<128, kKvInt8>(c, s, a, alone, work, st);
+}
+
+}  // namespace lm
