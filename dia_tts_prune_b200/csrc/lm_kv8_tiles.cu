@@ -1,13 +1,15 @@
 // lm_kv8_tiles.cu - attention of many rows over the cache in 8 bits, on the 5th-generation tensor cores.
 //
 // A CTA takes 256 (token, query head) rows that share a key head and walks their keys 128 at a time:
-//   warps 0-3, 4-7   one thread per row, 128 rows each: scores from tensor memory, softmax weights back to it.  The two halves are in different stages of a tile, so that the
-//                    tensor cores have one half's products while the other half takes exponentials
-//   warps 8-11       codes from pages to fp16 operands in shared memory, 32 tokens each; the next tile's are on their way while they do it
-//   warp 12          one elected lane issues tcgen05.mma: S = Q K^T (M = 128, N = 128), then O += P V with P as the operand in tensor memory, where S lay
+//   warps 0-3, 4-7   one thread per row, 128 rows each: scores from tensor memory, 32 at a time, softmax weights back to it.  The two halves are in different stages of a tile,
+//                    so that the tensor cores have one half's products while the other half takes exponentials
+//   warps 8-15       codes from pages to fp16 operands in shared memory, 16 tokens each; the next tile's are on their way while they do it
+//   warp 16          one elected lane issues tcgen05.mma: S = Q K^T (M = 128, N = 128), then O += P V with P as the operand in tensor memory, where S lay
+//   warp 17          looks up pages and scales, some tiles ahead
 //
 // Numbers.  t = scale log2(e) q . key + e - E in powers of two, e the exponent of the page's values and E the largest of the CTA's pages; P = 2^(t - R + 7) in fp16, with R the
-// row's reference: its largest t so far, raised (and O and the sum with it) only when one lies more than 2^8 above it, so P is at most 2^15.  That the page's value scale is inside
+// row's reference: about its largest t so far, raised (and with it what was made below it: O, the sum, the tile's weights) by a whole number only when a t lies more than 8 above
+// it, so P is at most 2^15.  That the page's value scale is inside
 // the weight lets codes be multiplied as they are, and the 11 bits of P count from the largest contribution.  The denominator takes 2^(E - e) out again, per 16 tokens.  Pages whose
 // values are 2^80 below the largest page's are taken as zeros.  Queries are scaled by a power of two per row (exact but for channels 2^-27 below the row's largest).  Sums are fp32;
 // O's live in tensor memory for the whole run of keys, and lose up to one unit in the last place per 16 keys (2^-24 on average: 2^-11 of the sum after 131072 keys, against the
@@ -16,6 +18,7 @@
 // Bound: per 256 x 128 tile and dim 128 the tensor pipe takes 2048 cycles, the exponentials (16 a cycle) 2048, and shared memory 2048 (the scores' operands 1024, the values 512,
 // the codes turned into operands 512).
 #include <algorithm>
+#include <type_traits>
 
 #include "attention_split.h"
 #include "engine_internal.h"
@@ -30,12 +33,14 @@ namespace {
 
 using namespace dia;
 
-constexpr int kKeys = 128, kHalfRows = 128, kTileRows = 2 * kHalfRows, kThreads = 512, kSms = 148;
+constexpr int kKeys = 128, kHalfRows = 128, kTileRows = 2 * kHalfRows, kThreads = 640, kSms = 148;
 constexpr int kBlocks = kKeys / kKvBlock;                      // blocks of 16 tokens in a tile of keys
 constexpr int kMinChunk = 4;                                   // tiles of keys that are worth a CTA of their own
-constexpr float kSlack = 8.f, kBits = 7.f, kSpread = 80.f;     // see above
-constexpr int kSoftmaxRegs = 184, kFetchRegs = 96, kIssueRegs = 48;
-static_assert(128 * (2 * kSoftmaxRegs + kFetchRegs + kIssueRegs) == kThreads * 128, "the split is the launch's registers");
+constexpr float kSlack = 8.f, kBits = 7.f;                     // see above
+constexpr int kSpread = 80;
+constexpr int kSoftmaxRegs = 136, kFetchRegs = 80, kIssueRegs = 48;
+static_assert(128 * (2 * kSoftmaxRegs + 2 * kFetchRegs + kIssueRegs) <= kThreads * 96, "the split is within the launch's registers");
+constexpr int kAhead = 8;                                      // tiles whose pages and scales are known
 
 template <int DP>
 struct Tiles {
@@ -144,14 +149,15 @@ __device__ __forceinline__ void tmem_load32(uint32_t addr, float* v) {
 #pragma unroll
     for (int e = 0; e < 32; ++e) v[e] = __uint_as_float(u[e]);
 }
-__device__ __forceinline__ void tmem_store32(uint32_t addr, const uint32_t (&v)[32]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
-        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(addr),
-        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]),
-        "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]),
-        "r"(v[29]), "r"(v[30]), "r"(v[31])
-        : "memory");
+__device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t (&v)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+                 "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+                 : "memory");
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
 }
 // Operands lie in blocks of 8 rows x 16 bytes, [row / 8][channel / 8]: lead / stride are the bytes between blocks along the contraction / the rows (scores: the contraction runs
 // over channels; values: over rows, and the channels are what is far apart)
@@ -174,7 +180,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cac
     uint8_t* const q_tile = smem;                             // [half]
     uint8_t* const k_ring = smem + T::kQ;
     uint8_t* const v_ring = k_ring + kStages * T::kSide;
-    __shared__ uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], s_full[2], p_ready[2], pv_done[2], done;
+    __shared__ uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], m_full[kAhead], m_empty[kAhead], s_full[2], p_ready[2], pv_done[2], done;
+    __shared__ float4 blocks[kAhead][kBlocks];                // (key scale, e - E, 2^(E - e), page) of 16 tokens
+    __shared__ uint2 which[kAhead];                           // of a tile's blocks: those that are there, those whose values are taken as zeros
     __shared__ uint32_t tmem_slot;
     __shared__ int largest;                                   // exponent of the values' pages
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -185,10 +193,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cac
     const Sequence q = sequence_at(s, a, work.seq, group, c.page_shift);
     if (threadIdx.x == 0) {
         for (int i = 0; i < kStages; ++i) {
-            mbar_init(&k_full[i], 4);
-            mbar_init(&v_full[i], 4);
+            mbar_init(&k_full[i], 8);
+            mbar_init(&v_full[i], 8);
             mbar_init(&k_empty[i], 1);
             mbar_init(&v_empty[i], 1);
+        }
+        for (int i = 0; i < kAhead; ++i) {
+            mbar_init(&m_full[i], 1);
+            mbar_init(&m_empty[i], 16);
         }
         for (int g = 0; g < 2; ++g) {
             mbar_init(&s_full[g], 1);
@@ -199,7 +211,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cac
         largest = -1000;
         fence_mbar_init();
     }
-    if (warp == 12) {
+    if (warp == 16) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&tmem_slot)));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
     }
@@ -290,104 +302,124 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cac
         const int g = warp >> 2, count = g ? n1 : n0;
         const uint32_t lanes = (uint32_t)(warp & 3) * 32u << 16, t_s = tmem + lanes + 128u * g, t_o = tmem + lanes + 256u + 128u * g;
         const int p = p0 + threadIdx.x;
-        const long long pos = position(p), first_pos = position(p0 + g * kHalfRows), last_pos = position(p0 + g * kHalfRows + kHalfRows - 1);
+        // the tokens that the row sees, and the ones that all 128 rows see, counted from the first tile on
+        const long long tok0 = (long long)from * kKeys;
+        const auto within = [&](long long v) { return (int)max(min(v - tok0, 0x7fffff00ll), -1ll); };
+        const int hi = within(position(p)), lo = within(position(p) - back), all_hi = within(position(p0 + g * kHalfRows)), all_lo = within(position(p0 + g * kHalfRows + kHalfRows - 1) - back);
         float ref = -1e30f, l = 0.f;
-        // lanes 0 .. 7 hold a block's scales each, looked up a tile ahead, and its page two tiles ahead
-        const auto page_of = [&](int i) {
-            if (lane >= kBlocks || i >= count) return -1;
-            return s.page(work.seq, (((long long)from + i) * kKeys + lane * kKvBlock) >> c.page_shift, c.pages);
-        };
-        const auto scales_of = [&](int page, float& ks, float& ev) {
-            ks = ev = 0.f;
-            if (page < 0) return;
-            const size_t at = (size_t)page * c.kv_heads + work.head;
-            const uint32_t v = __float_as_uint(c.value_scales[at]);
-            ks = c.key_scales[at];
-            ev = v >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : fmaxf((float)((int)(v >> 23) - 127) - spread, -kSpread);
-        };
-        int page = page_of(0), page_next = page_of(1);
-        float ks, ev;
-        scales_of(page, ks, ev);
 #pragma unroll 1
         for (int i = 0; i < count; ++i) {
-            const uint32_t there = __ballot_sync(0xffffffffu, page >= 0) & 0xffu;
-            const float ks_now = ks, ev_now = ev;
-            page = page_next;
-            scales_of(page, ks, ev);
-            page_next = page_of(i + 2);
-            const long long tok = ((long long)from + i) * kKeys;
-            const bool clear = there == 0xffu && tok + kKeys - 1 <= first_pos && tok >= last_pos - back;
+            const int slot = i % kAhead;
+            if (!pair_wait(&m_full[slot], (uint32_t)(i / kAhead) & 1u, polls)) { ok = false; break; }
+            const uint32_t there = which[slot].x;
+            const int tok = i * kKeys;
+            const bool clear = there == 0xffu && tok + kKeys - 1 <= all_hi && tok >= all_lo;
             if (!pair_wait(&s_full[g], i & 1, polls)) { ok = false; break; }
             fence_after();
-            float x[kKeys];
-#pragma unroll
-            for (int j = 0; j < kKeys; j += 32) tmem_load32(t_s + j, x + j);
-            tmem_loaded();
-            if (!clear) {
-                const int hi = (int)min(pos - tok, (long long)kKeys), lo = (int)max(pos - back - tok, -1ll);
-#pragma unroll
-                for (int e = 0; e < kKeys; ++e)
-                    if (e > hi || e < lo || !(there >> (e / kKvBlock) & 1u)) x[e] = -INFINITY;
-            }
-            float top = -INFINITY, kb[kBlocks];
-#pragma unroll
-            for (int b = 0; b < kBlocks; ++b) {
-                float m = x[16 * b];
-#pragma unroll
-                for (int e = 1; e < kKvBlock; ++e) m = fmaxf(m, x[16 * b + e]);
-                kb[b] = __shfl_sync(0xffffffffu, ks_now, b) * row_scale;
-                top = fmaxf(top, fmaf(m, kb[b], __shfl_sync(0xffffffffu, ev_now, b)));
-            }
-            if (__any_sync(0xffffffffu, top > ref + kSlack)) {
-                const float next = top > ref + kSlack ? top : ref, f = exp2_fast(ref - next);
+            // everything made with the reference that was: chunks of this tile, O, the sum
+            const auto raise = [&](float top, int chunks) {
+                const float next = top > ref + kSlack ? ceilf(top) : ref, down = ref - next;      // whole numbers: the power is exact, and so is what is times it
+                const float f = down < -126.f ? 0.f : __uint_as_float((uint32_t)((int)down + 127) << 23);
                 ref = next;
                 l *= f;
-                if (i > 0) {
-                    if (!pair_wait(&pv_done[g], (i - 1) & 1, polls)) { ok = false; break; }
-                    fence_after();
+                const __half2 f16 = __float2half2_rn(f);
+                tmem_stored();
 #pragma unroll 1
-                    for (int j = 0; j < DP; j += 32) {
-                        uint32_t o[32];
-                        tmem_columns32(t_o + j, o);
-                        tmem_loaded();
+                for (int j = 0; j < chunks; ++j) {
+                    uint32_t w[16];
+                    tmem_columns16(t_s + 16 * j, w);
+                    tmem_loaded();
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                        tmem_store32(t_o + j, o);
+                    for (int e = 0; e < 16; ++e) {
+                        const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&w[e]), f16);
+                        w[e] = *reinterpret_cast<const uint32_t*>(&y);
                     }
+                    tmem_store16(t_s + 16 * j, w);
                 }
-            }
+                if (i == 0) return;
+                if (!pair_wait(&pv_done[g], (i - 1) & 1, polls)) { ok = false; return; }
+                fence_after();
+#pragma unroll 1
+                for (int j = 0; j < DP; j += 16) {
+                    uint32_t o[16];
+                    tmem_columns16(t_o + j, o);
+                    tmem_loaded();
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                uint32_t w[32];
+                    for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                    tmem_store16(t_o + j, o);
+                }
+            };
+            const auto weigh = [&](auto some_hidden) {
+                constexpr bool kHidden = decltype(some_hidden)::value;
+                uint32_t x[2][32];
+                tmem_columns32(t_s, x[0]);
 #pragma unroll
-                for (int b4 = 0; b4 < 4; ++b4) {
-                    const int b = 4 * h + b4;
-                    const float e0 = __shfl_sync(0xffffffffu, ev_now, b);
-                    const f2 k2 = twice(kb[b]), c2 = twice(e0 - ref + kBits);
-                    f2 sum = 0;
+                for (int j = 0; j < 4; ++j) {
+                    tmem_loaded();
+                    if (j < 3) tmem_columns32(t_s + 32 * (j + 1), x[(j + 1) & 1]);
+                    float v[32];
 #pragma unroll
-                    for (int e = 0; e < kKvBlock; e += 2) {
-                        float y0, y1;
-                        unpack2(fma2(pack2(x[16 * b + e], x[16 * b + e + 1]), k2, c2), y0, y1);
-                        y0 = exp2_fast(y0);
-                        y1 = exp2_fast(y1);
-                        if (!clear) {
-                            if (x[16 * b + e] == -INFINITY) y0 = 0.f;
-                            if (x[16 * b + e + 1] == -INFINITY) y1 = 0.f;
+                    for (int e = 0; e < 32; ++e) v[e] = __uint_as_float(x[j & 1][e]);
+                    if constexpr (kHidden) {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) {
+                            const int at = tok + 32 * j + e;
+                            if (at > hi || at < lo || !(there >> (2 * j + e / 16) & 1u)) v[e] = -INFINITY;
                         }
-                        sum = add2(sum, pack2(y0, y1));
-                        w[8 * b4 + e / 2] = pack_half(y0, y1);
                     }
-                    float s0, s1;
-                    unpack2(sum, s0, s1);
-                    l = fmaf(s0 + s1, e0 == e0 ? __uint_as_float((uint32_t)(127 - (int)e0) << 23) : 1.f, l);
+                    float top = -INFINITY, kb[2], eb[2], back_out[2];
+#pragma unroll
+                    for (int b = 0; b < 2; ++b) {
+                        const float4 meta = blocks[slot][2 * j + b];
+                        float m = max3(v[16 * b], v[16 * b + 1], v[16 * b + 2]);
+#pragma unroll
+                        for (int e = 3; e < kKvBlock - 1; e += 2) m = max3(m, v[16 * b + e], v[16 * b + e + 1]);
+                        kb[b] = meta.x * row_scale;
+                        eb[b] = meta.y;
+                        back_out[b] = meta.z;
+                        top = fmaxf(top, fmaf(fmaxf(m, v[16 * b + 15]), kb[b], eb[b]));
+                    }
+                    if (__any_sync(0xffffffffu, top > ref + kSlack)) raise(top, j);
+                    uint32_t w[16];
+#pragma unroll
+                    for (int b = 0; b < 2; ++b) {
+                        const f2 k2 = twice(kb[b]), c2 = twice(eb[b] - ref + kBits);
+                        f2 sum = 0;
+#pragma unroll
+                        for (int e = 0; e < kKvBlock; e += 2) {
+                            float y0, y1;
+                            unpack2(fma2(pack2(v[16 * b + e], v[16 * b + e + 1]), k2, c2), y0, y1);
+                            y0 = exp2_fast(y0);
+                            y1 = exp2_fast(y1);
+                            if constexpr (kHidden) {                                 // (whatever the page's scales are)
+                                if (v[16 * b + e] == -INFINITY) y0 = 0.f;
+                                if (v[16 * b + e + 1] == -INFINITY) y1 = 0.f;
+                            }
+                            sum = add2(sum, pack2(y0, y1));
+                            w[8 * b + e / 2] = pack_half(y0, y1);
+                        }
+                        float s0, s1;
+                        unpack2(sum, s0, s1);
+                        l = fmaf(s0 + s1, back_out[b], l);
+                    }
+                    tmem_store16(t_s + 16 * j, w);
                 }
-                tmem_store32(t_s + 32 * h, w);
-            }
+            };
+            if (clear) weigh(std::false_type{});
+            else weigh(std::true_type{});
             tmem_stored();
             fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&p_ready[g]);
+            if (lane == 0) {
+                mbar_arrive(&m_empty[slot]);
+                mbar_arrive(&p_ready[g]);
+            }
+            if (!ok) break;
+        }
+        // (a half that looks at fewer tiles lets the others have the rest)
+        for (int i = count; ok && i < n; ++i) {
+            if (!pair_wait(&m_full[i % kAhead], (uint32_t)(i / kAhead) & 1u, polls)) ok = false;
+            else if (lane == 0) mbar_arrive(&m_empty[i % kAhead]);
         }
         if (ok && count > 0 && !pair_wait(&pv_done[g], (count - 1) & 1, polls)) ok = false;
         fence_after();
@@ -440,84 +472,92 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cac
                     if (j + e < c.dim) store_out(a, to + j + e, o[e] * f);
             }
         }
-    } else if (warp < 12) {
+    } else if (warp < 16) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFetchRegs));
-        // ---- codes to operands: 32 tokens of every tile, eight rows of a block a turn, a lane 16 channels of one ----
+        // ---- codes to operands: a block of every tile, eight rows of it a turn, a lane 16 channels of one ----
         constexpr int kParts = DP / 64;                       // 16-byte pieces of a row that a lane takes
-        const int mine = (warp - 8) * 32, sub = lane & 7, piece = lane >> 3;
-        uint4 kc[4][kParts], vc[4][kParts];
-        const auto page_of = [&](int i, int b) { return i < n ? s.page(work.seq, (((long long)from + i) * kKeys + mine + b * kKvBlock) >> c.page_shift, c.pages) : -1; };
-        const auto fetch = [&](uint4 (&codes)[4][kParts], const uint8_t* side, int i, int pa, int pb) {
-#pragma unroll
-            for (int r8 = 0; r8 < 4; ++r8) {
-                const int page = r8 < 2 ? pa : pb;
-                const int in_page = (int)((((long long)from + i) * kKeys + mine + r8 * 8 + sub) & ((1 << c.page_shift) - 1));
-                const uint8_t* const row = side + ((((size_t)max(page, 0) * c.kv_heads + work.head) << c.page_shift) + in_page) * c.stride;
-#pragma unroll
-                for (int j = 0; j < kParts; ++j) {
-                    const int at = (piece + 4 * j) * 16;
-                    codes[r8][j] = page >= 0 && at < c.stride ? *reinterpret_cast<const uint4*>(row + at) : make_uint4(0u, 0u, 0u, 0u);
-                }
-            }
+        const int block = warp - 8, sub = lane & 7, piece = lane >> 3, in_page = (int)(((long long)from * kKeys + block * kKvBlock) & ((1 << c.page_shift) - 1));
+        uint4 kc[2][kParts], vc[2][kParts];
+        size_t at = 0;                                        // of this lane's rows in the pages, for the tile that is fetched
+        bool there = false;
+        const auto find = [&](int i) {                        // (the place in a page is the same in every tile: pages are no larger)
+            const int page = __float_as_int(blocks[i % kAhead][block].w);
+            there = page >= 0;
+            at = ((((size_t)max(page, 0) * c.kv_heads + work.head) << c.page_shift) + ((in_page + i * kKeys) & ((1 << c.page_shift) - 1)) + sub) * c.stride + piece * 16;
         };
-        const auto lay = [&](const uint4 (&codes)[4][kParts], uint8_t* to, bool drop_a, bool drop_b) {
+        const auto fetch = [&](uint4 (&codes)[2][kParts], const uint8_t* side) {
 #pragma unroll
-            for (int r8 = 0; r8 < 4; ++r8) {
-                const bool drop = r8 < 2 ? drop_a : drop_b;
+            for (int r8 = 0; r8 < 2; ++r8)
+#pragma unroll
+                for (int j = 0; j < kParts; ++j)
+                    codes[r8][j] = there && piece * 16 + 64 * j < c.stride ? *reinterpret_cast<const uint4*>(side + at + (size_t)(8 * r8) * c.stride + 64 * j) : make_uint4(0u, 0u, 0u, 0u);
+        };
+        const auto lay = [&](const uint4 (&codes)[2][kParts], uint8_t* to, bool drop) {
+#pragma unroll
+            for (int r8 = 0; r8 < 2; ++r8)
 #pragma unroll
                 for (int j = 0; j < kParts; ++j) {
                     const uint32_t w[4] = {codes[r8][j].x, codes[r8][j].y, codes[r8][j].z, codes[r8][j].w};
                     uint32_t u[8];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) decode4<FORMAT>(drop ? 0u : w[e], u[2 * e], u[2 * e + 1]);
-                    uint8_t* const at = to + (mine / 8 + r8) * (DP * 16) + (piece + 4 * j) * 256 + sub * 16;
-                    *reinterpret_cast<uint4*>(at) = make_uint4(u[0], u[1], u[2], u[3]);
-                    *reinterpret_cast<uint4*>(at + 128) = make_uint4(u[4], u[5], u[6], u[7]);
+                    uint8_t* const d = to + (2 * block + r8) * (DP * 16) + (piece + 4 * j) * 256 + sub * 16;
+                    *reinterpret_cast<uint4*>(d) = make_uint4(u[0], u[1], u[2], u[3]);
+                    *reinterpret_cast<uint4*>(d + 128) = make_uint4(u[4], u[5], u[6], u[7]);
                 }
-            }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
         };
-        const auto value_scale = [&](int page) { return page >= 0 ? __float_as_uint(c.value_scales[(size_t)page * c.kv_heads + work.head]) : 0u; };
-        const auto dropped = [&](uint32_t v) { return v < 0x7f800000u && (float)((int)(v >> 23) - 127) - spread < -kSpread; };
-        int pa = page_of(0, 0), pb = page_of(0, 1), na = page_of(1, 0), nb = page_of(1, 1);
-        fetch(kc, c.keys, 0, pa, pb);
-        fetch(vc, c.values, 0, pa, pb);
-        uint32_t va = value_scale(pa), vb = value_scale(pb);
+        if (n > 0) {
+            if (pair_wait(&m_full[0], 0u, polls)) {
+                find(0);
+                fetch(kc, c.keys);
+                fetch(vc, c.values);
+            } else {
+                ok = false;
+            }
+        }
 #pragma unroll 1
-        for (int i = 0; i < n; ++i) {
-            const int st = i % kStages;
+        for (int i = 0; ok && i < n; ++i) {
+            const int st = i % kStages, next = (i + 1) % kAhead;
             const uint32_t use = (uint32_t)(i / kStages);
+            const bool more = i + 1 < n, drop = which[i % kAhead].y >> block & 1u;
+            if (more && !pair_wait(&m_full[next], (uint32_t)((i + 1) / kAhead) & 1u, polls)) { ok = false; break; }
             if (i >= kStages && !pair_wait(&k_empty[st], (use + 1) & 1, polls)) { ok = false; break; }
-            lay(kc, k_ring + st * T::kSide, false, false);
-            if (lane == 0) mbar_arrive(&k_full[st]);
-            if (i + 1 < n) fetch(kc, c.keys, i + 1, na, nb);
+            lay(kc, k_ring + st * T::kSide, false);
+            if (lane == 0) {
+                mbar_arrive(&k_full[st]);
+                mbar_arrive(&m_empty[i % kAhead]);
+            }
+            if (more) {
+                find(i + 1);
+                fetch(kc, c.keys);
+            }
             if (i >= kStages && !pair_wait(&v_empty[st], (use + 1) & 1, polls)) { ok = false; break; }
-            lay(vc, v_ring + st * T::kSide, dropped(va), dropped(vb));
+            lay(vc, v_ring + st * T::kSide, drop);
             if (lane == 0) mbar_arrive(&v_full[st]);
-            if (i + 1 < n) fetch(vc, c.values, i + 1, na, nb);
-            va = value_scale(na);
-            vb = value_scale(nb);
-            na = page_of(i + 2, 0);
-            nb = page_of(i + 2, 1);
+            if (more) fetch(vc, c.values);
         }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
-        if (warp == 12) {
+        if (warp == 16) {
             const uint32_t idesc_s = (1u << 4) | ((uint32_t)(kKeys >> 3) << 17) | ((uint32_t)(kHalfRows >> 4) << 24);
             const uint32_t idesc_o = (1u << 4) | (1u << 16) | ((uint32_t)(DP >> 3) << 17) | ((uint32_t)(kHalfRows >> 4) << 24);
-            const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0), q_at = smem_u32(q_tile), k_at = smem_u32(k_ring), v_at = smem_u32(v_ring);
-            const int u0 = __shfl_sync(0xffffffffu, n0, 0), u1 = __shfl_sync(0xffffffffu, n1, 0), un = max(u0, u1);
+            const uint32_t q_at = smem_u32(q_tile), k_at = smem_u32(k_ring), v_at = smem_u32(v_ring);
+            const int u0 = n0, u1 = n1, un = max(u0, u1);
+            // What an instruction takes is broadcast from one lane, so that it is known to be the same in every lane and stays in uniform registers.
+            const auto same = [](uint32_t v) { return __shfl_sync(0xffffffffu, v, 0); };
             // scores of tile i for half g; behind the last half the slot is free when they are there
             const auto scores = [&](int g, int i) {
                 if (i >= un) return;
                 if (!pair_wait(&k_full[i % kStages], (uint32_t)(i / kStages) & 1u, polls)) { ok = false; return; }
                 fence_after();
+                const uint32_t d = same(tmem + 128u * g), qa = same(q_at + g * (kHalfRows * DP * 2)), ka = same(k_at + (i % kStages) * T::kSide);
+                const uint64_t qd = block_desc(qa, 128u, DP * 16u), kd = block_desc(ka, 128u, DP * 16u);
                 if (elect_one_sync()) {
                     if (i < (g ? u1 : u0)) {
-                        const uint64_t qd = block_desc(q_at + g * (kHalfRows * DP * 2), 128u, DP * 16u), kd = block_desc(k_at + (i % kStages) * T::kSide, 128u, DP * 16u);
 #pragma unroll
-                        for (uint32_t k = 0; k < kSteps; ++k) umma_bf16(tm + 128u * g, qd + 16u * k, kd + 16u * k, idesc_s, k != 0);
+                        for (uint32_t k = 0; k < kSteps; ++k) umma_bf16(d, qd + 16u * k, kd + 16u * k, idesc_s, k != 0);
                         umma_commit(&s_full[g]);
                     }
                     if (g == 1) umma_commit(&k_empty[i % kStages]);
@@ -528,11 +568,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cac
                 if (i < (g ? u1 : u0) && !pair_wait(&p_ready[g], i & 1, polls)) { ok = false; return; }
                 if (!pair_wait(&v_full[i % kStages], (uint32_t)(i / kStages) & 1u, polls)) { ok = false; return; }
                 fence_after();
+                const uint32_t d = same(tmem + 256u + 128u * g), w = same(tmem + 128u * g), va = same(v_at + (i % kStages) * T::kSide), later = same(i != 0);
+                const uint64_t vd = block_desc(va, DP * 16u, 128u);
                 if (elect_one_sync()) {
                     if (i < (g ? u1 : u0)) {
-                        const uint64_t vd = block_desc(v_at + (i % kStages) * T::kSide, DP * 16u, 128u);
 #pragma unroll
-                        for (uint32_t k = 0; k < kKeys / 16; ++k) mma_weights(tm + 256u + 128u * g, tm + 128u * g + 8u * k, vd + 2u * DP * k, idesc_o, (i | k) != 0);
+                        for (uint32_t k = 0; k < kKeys / 16; ++k) mma_weights(d, w + 8u * k, vd + 2u * DP * k, idesc_o, k != 0 ? 1u : later);
                         umma_commit(&pv_done[g]);
                     }
                     if (g == 1) umma_commit(&v_empty[i % kStages]);
@@ -550,6 +591,34 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cac
                 }
             }
             mmas_ended<false>(&done);
+        } else if (warp == 17) {
+            // lanes 0 .. 7 look a block up each: its scales a tile ahead, its page two
+            const auto page_of = [&](int i) { return lane < kBlocks && i < n ? s.page(work.seq, (((long long)from + i) * kKeys + lane * kKvBlock) >> c.page_shift, c.pages) : -1; };
+            const auto scales_of = [&](int page) {
+                const size_t at = (size_t)max(page, 0) * c.kv_heads + work.head;
+                return page >= 0 ? make_float2(c.key_scales[at], c.value_scales[at]) : make_float2(0.f, 0.f);
+            };
+            int page = page_of(0), page_next = page_of(1);
+            float2 scales = scales_of(page);
+#pragma unroll 1
+            for (int i = 0; i < n; ++i) {
+                const int slot = i % kAhead, page_now = page;
+                const float2 now = scales;
+                page = page_next;
+                scales = scales_of(page);
+                page_next = page_of(i + 2);
+                const uint32_t v = __float_as_uint(now.y);
+                const bool number = v < 0x7f800000u;
+                const int e = (int)(v >> 23) - 127 - (largest == -1000 ? 0 : largest), kept = max(e, -kSpread);
+                if (i >= kAhead && !pair_wait(&m_empty[slot], (uint32_t)(i / kAhead + 1) & 1u, polls)) { ok = false; break; }
+                const uint32_t there = __ballot_sync(0xffffffffu, page_now >= 0), zeros = __ballot_sync(0xffffffffu, page_now >= 0 && number && e < -kSpread);
+                if (lane < kBlocks)
+                    blocks[slot][lane] = make_float4(now.x, page_now < 0 ? 0.f : number ? (float)kept : __uint_as_float(0x7fc00000u),
+                                                     page_now >= 0 && number ? __uint_as_float((uint32_t)(127 - kept) << 23) : 1.f, __int_as_float(page_now));
+                if (lane == 0) which[slot] = make_uint2(there & 0xffu, zeros & 0xffu);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&m_full[slot]);
+            }
         }
     }
     if (!ok && lane == 0 && ran_out) {
@@ -559,7 +628,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cac
     __syncwarp();
     fence_before();
     __syncthreads();
-    if (warp == 12) {
+    if (warp == 16) {
         fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
     }
