@@ -1,15 +1,15 @@
 // lm_kv8_tiles.cu - attention of many rows over the cache in 8 bits, on the 5th-generation tensor cores.
 //
 // A CTA takes 256 (token, query head) rows that share a key head and walks their keys 128 at a time:
-//   warps 0-3, 4-7   one thread per row, 128 rows each: scores from tensor memory, 32 at a time, softmax weights back to it.  The two halves are in different stages of a tile,
+//   warps 0-3, 4-7   one thread per row, 128 rows each: scores from tensor memory, softmax weights back to it.  The two halves are in different stages of a tile,
 //                    so that the tensor cores have one half's products while the other half takes exponentials
-//   warps 8-15       codes from pages to fp16 operands in shared memory, 16 tokens each; the next tile's are on their way while they do it
+//   warps 8-15       codes to fp16 operands, from shared memory to shared memory, 16 tokens each
 //   warp 16          one elected lane issues tcgen05.mma: S = Q K^T (M = 128, N = 128), then O += P V with P as the operand in tensor memory, where S lay
-//   warp 17          looks up pages and scales, some tiles ahead
+//   warp 17          looks up pages and scales, and fetches the next tile's codes by bulk copies
 //
 // Numbers.  t = scale log2(e) q . key + e - E in powers of two, e the exponent of the page's values and E the largest of the CTA's pages; P = 2^(t - R + 7) in fp16, with R the
-// row's reference: about its largest t so far, raised (and with it what was made below it: O, the sum, the tile's weights) by a whole number only when a t lies more than 8 above
-// it, so P is at most 2^15.  That the page's value scale is inside
+// row's reference: about its largest t so far, raised (and O and the sum with it) only when a tile's largest lies more than 8 above it, so P is at most 2^15.  That the page's value
+// scale is inside
 // the weight lets codes be multiplied as they are, and the 11 bits of P count from the largest contribution.  The denominator takes 2^(E - e) out again, per 16 tokens.  Pages whose
 // values are 2^80 below the largest page's are taken as zeros.  Queries are scaled by a power of two per row (exact but for channels 2^-27 below the row's largest).  Sums are fp32;
 // O's live in tensor memory for the whole run of keys, and lose up to one unit in the last place per 16 keys (2^-24 on average: 2^-11 of the sum after 131072 keys, against the
@@ -38,14 +38,15 @@ constexpr int kBlocks = kKeys / kKvBlock;                      // blocks of 16 t
 constexpr int kMinChunk = 4;                                   // tiles of keys that are worth a CTA of their own
 constexpr float kSlack = 8.f, kBits = 7.f;                     // see above
 constexpr int kSpread = 80;
-constexpr int kSoftmaxRegs = 136, kFetchRegs = 80, kIssueRegs = 48;
+constexpr int kSoftmaxRegs = 168, kFetchRegs = 40, kIssueRegs = 64;
 static_assert(128 * (2 * kSoftmaxRegs + 2 * kFetchRegs + kIssueRegs) <= kThreads * 96, "the split is within the launch's registers");
 constexpr int kAhead = 8;                                      // tiles whose pages and scales are known
 
 template <int DP>
 struct Tiles {
     static constexpr int kStages = DP == 64 ? 4 : 2, kSide = kKeys * DP * 2, kQ = kTileRows * DP * 2;
-    static constexpr int kSmem = kQ + kStages * 2 * kSide + 1024;
+    static constexpr int kCodes = kKeys * DP;                 // room for a tile's codes, keys or values
+    static constexpr int kSmem = kQ + kStages * 2 * kSide + 2 * kCodes;
 };
 
 // ---- who takes what ------------------------------------------------------------------------------------------------------------------------
@@ -180,9 +181,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cac
     uint8_t* const q_tile = smem;                             // [half]
     uint8_t* const k_ring = smem + T::kQ;
     uint8_t* const v_ring = k_ring + kStages * T::kSide;
-    __shared__ uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], m_full[kAhead], m_empty[kAhead], s_full[2], p_ready[2], pv_done[2], done;
+    uint8_t* const codes = v_ring + kStages * T::kSide;       // [keys, values]
+    __shared__ uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], m_full[kAhead], m_empty[kAhead], c_full[2], c_empty[2], s_full[2], p_ready[2], pv_done[2], done;
     __shared__ float4 blocks[kAhead][kBlocks];                // (key scale, e - E, 2^(E - e), page) of 16 tokens
-    __shared__ uint2 which[kAhead];                           // of a tile's blocks: those that are there, those whose values are taken as zeros
+    __shared__ uint3 which[kAhead];                           // of a tile's blocks: those that are there, whose values are taken as zeros, that stand for numbers
     __shared__ uint32_t tmem_slot;
     __shared__ int largest;                                   // exponent of the values' pages
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -203,6 +205,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cac
             mbar_init(&m_empty[i], 16);
         }
         for (int g = 0; g < 2; ++g) {
+            mbar_init(&c_full[g], 1);
+            mbar_init(&c_empty[g], 8);
             mbar_init(&s_full[g], 1);
             mbar_init(&p_ready[g], 4);
             mbar_init(&pv_done[g], 1);
@@ -311,102 +315,80 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cac
         for (int i = 0; i < count; ++i) {
             const int slot = i % kAhead;
             if (!pair_wait(&m_full[slot], (uint32_t)(i / kAhead) & 1u, polls)) { ok = false; break; }
-            const uint32_t there = which[slot].x;
+            const uint32_t there = which[slot].x, numbers = which[slot].z;
             const int tok = i * kKeys;
-            const bool clear = there == 0xffu && tok + kKeys - 1 <= all_hi && tok >= all_lo;
+            const bool clear = (there & numbers) == 0xffu && tok + kKeys - 1 <= all_hi && tok >= all_lo;
             if (!pair_wait(&s_full[g], i & 1, polls)) { ok = false; break; }
             fence_after();
-            // everything made with the reference that was: chunks of this tile, O, the sum
-            const auto raise = [&](float top, int chunks) {
-                const float next = top > ref + kSlack ? ceilf(top) : ref, down = ref - next;      // whole numbers: the power is exact, and so is what is times it
-                const float f = down < -126.f ? 0.f : __uint_as_float((uint32_t)((int)down + 127) << 23);
+            uint32_t x[4][32];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) tmem_columns32(t_s + 32 * j, x[j]);
+            tmem_loaded();
+            if (!clear) {
+#pragma unroll
+                for (int b = 0; b < kBlocks; ++b) {
+                    const bool block = there >> b & 1u;
+                    const uint32_t nan = numbers >> b & 1u ? 0u : 0x7fffffffu;      // (what a row sees of a page that stands for NaNs)
+#pragma unroll
+                    for (int e = 0; e < kKvBlock; ++e) {
+                        const int at = tok + 16 * b + e;
+                        uint32_t& v = x[b / 2][16 * (b & 1) + e];
+                        v = at > hi || at < lo || !block ? 0xff800000u : v | nan;
+                    }
+                }
+            }
+            const auto score = [&](int b, int e) { return __uint_as_float(x[b / 2][16 * (b & 1) + e]); };
+            float top = -INFINITY;
+#pragma unroll
+            for (int b = 0; b < kBlocks; ++b) {
+                const float2 meta = *reinterpret_cast<const float2*>(&blocks[slot][b]);
+                float m = max3(score(b, 0), score(b, 1), score(b, 2));
+#pragma unroll
+                for (int e = 3; e < kKvBlock - 1; e += 2) m = max3(m, score(b, e), score(b, e + 1));
+                top = fmaxf(top, fmaf(fmaxf(m, score(b, 15)), meta.x * row_scale, meta.y));
+            }
+            if (__any_sync(0xffffffffu, top > ref + kSlack)) {
+                const float next = top > ref + kSlack ? top : ref, f = exp2_fast(ref - next);
                 ref = next;
                 l *= f;
-                const __half2 f16 = __float2half2_rn(f);
-                tmem_stored();
+                if (i > 0) {
+                    if (!pair_wait(&pv_done[g], (i - 1) & 1, polls)) { ok = false; break; }
+                    fence_after();
 #pragma unroll 1
-                for (int j = 0; j < chunks; ++j) {
-                    uint32_t w[16];
-                    tmem_columns16(t_s + 16 * j, w);
-                    tmem_loaded();
+                    for (int j = 0; j < DP; j += 16) {
+                        uint32_t o[16];
+                        tmem_columns16(t_o + j, o);
+                        tmem_loaded();
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&w[e]), f16);
-                        w[e] = *reinterpret_cast<const uint32_t*>(&y);
+                        for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                        tmem_store16(t_o + j, o);
                     }
-                    tmem_store16(t_s + 16 * j, w);
                 }
-                if (i == 0) return;
-                if (!pair_wait(&pv_done[g], (i - 1) & 1, polls)) { ok = false; return; }
-                fence_after();
-#pragma unroll 1
-                for (int j = 0; j < DP; j += 16) {
-                    uint32_t o[16];
-                    tmem_columns16(t_o + j, o);
-                    tmem_loaded();
+            }
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                    tmem_store16(t_o + j, o);
+            for (int j = 0; j < 4; ++j) {
+                uint32_t w[16];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int b = 2 * j + h;
+                    const float4 meta = blocks[slot][b];
+                    const f2 k2 = twice(meta.x * row_scale), c2 = twice(meta.y - ref + kBits);
+                    f2 sum[2] = {0, 0};
+#pragma unroll
+                    for (int e = 0; e < kKvBlock; e += 2) {
+                        float y0, y1;
+                        unpack2(fma2(pack2(score(b, e), score(b, e + 1)), k2, c2), y0, y1);
+                        y0 = exp2_fast(y0);
+                        y1 = exp2_fast(y1);
+                        sum[e / 2 & 1] = add2(sum[e / 2 & 1], pack2(y0, y1));
+                        w[8 * h + e / 2] = pack_half(y0, y1);
+                    }
+                    float s0, s1;
+                    unpack2(add2(sum[0], sum[1]), s0, s1);
+                    l = fmaf(s0 + s1, meta.z, l);
                 }
-            };
-            const auto weigh = [&](auto some_hidden) {
-                constexpr bool kHidden = decltype(some_hidden)::value;
-                uint32_t x[2][32];
-                tmem_columns32(t_s, x[0]);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    tmem_loaded();
-                    if (j < 3) tmem_columns32(t_s + 32 * (j + 1), x[(j + 1) & 1]);
-                    float v[32];
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) v[e] = __uint_as_float(x[j & 1][e]);
-                    if constexpr (kHidden) {
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) {
-                            const int at = tok + 32 * j + e;
-                            if (at > hi || at < lo || !(there >> (2 * j + e / 16) & 1u)) v[e] = -INFINITY;
-                        }
-                    }
-                    float top = -INFINITY, kb[2], eb[2], back_out[2];
-#pragma unroll
-                    for (int b = 0; b < 2; ++b) {
-                        const float4 meta = blocks[slot][2 * j + b];
-                        float m = max3(v[16 * b], v[16 * b + 1], v[16 * b + 2]);
-#pragma unroll
-                        for (int e = 3; e < kKvBlock - 1; e += 2) m = max3(m, v[16 * b + e], v[16 * b + e + 1]);
-                        kb[b] = meta.x * row_scale;
-                        eb[b] = meta.y;
-                        back_out[b] = meta.z;
-                        top = fmaxf(top, fmaf(fmaxf(m, v[16 * b + 15]), kb[b], eb[b]));
-                    }
-                    if (__any_sync(0xffffffffu, top > ref + kSlack)) raise(top, j);
-                    uint32_t w[16];
-#pragma unroll
-                    for (int b = 0; b < 2; ++b) {
-                        const f2 k2 = twice(kb[b]), c2 = twice(eb[b] - ref + kBits);
-                        f2 sum = 0;
-#pragma unroll
-                        for (int e = 0; e < kKvBlock; e += 2) {
-                            float y0, y1;
-                            unpack2(fma2(pack2(v[16 * b + e], v[16 * b + e + 1]), k2, c2), y0, y1);
-                            y0 = exp2_fast(y0);
-                            y1 = exp2_fast(y1);
-                            if constexpr (kHidden) {                                 // (whatever the page's scales are)
-                                if (v[16 * b + e] == -INFINITY) y0 = 0.f;
-                                if (v[16 * b + e + 1] == -INFINITY) y1 = 0.f;
-                            }
-                            sum = add2(sum, pack2(y0, y1));
-                            w[8 * b + e / 2] = pack_half(y0, y1);
-                        }
-                        float s0, s1;
-                        unpack2(sum, s0, s1);
-                        l = fmaf(s0 + s1, back_out[b], l);
-                    }
-                    tmem_store16(t_s + 16 * j, w);
-                }
-            };
-            if (clear) weigh(std::false_type{});
-            else weigh(std::true_type{});
+                tmem_store16(t_s + 16 * j, w);
+            }
             tmem_stored();
             fence_before();
             __syncwarp();
@@ -414,7 +396,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cac
                 mbar_arrive(&m_empty[slot]);
                 mbar_arrive(&p_ready[g]);
             }
-            if (!ok) break;
         }
         // (a half that looks at fewer tiles lets the others have the rest)
         for (int i = count; ok && i < n; ++i) {
@@ -474,120 +455,119 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cac
         }
     } else if (warp < 16) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFetchRegs));
-        // ---- codes to operands: a block of every tile, eight rows of it a turn, a lane 16 channels of one ----
+        // ---- codes to operands: a block of every tile, eight rows of it a turn, a lane 16 channels of one.  Eight neighbouring lanes take eight rows and as many different pieces,
+        // so that neither what they read nor what they write meets in a bank ----
         constexpr int kParts = DP / 64;                       // 16-byte pieces of a row that a lane takes
-        const int block = warp - 8, sub = lane & 7, piece = lane >> 3, in_page = (int)(((long long)from * kKeys + block * kKvBlock) & ((1 << c.page_shift) - 1));
-        uint4 kc[2][kParts], vc[2][kParts];
-        size_t at = 0;                                        // of this lane's rows in the pages, for the tile that is fetched
-        bool there = false;
-        const auto find = [&](int i) {                        // (the place in a page is the same in every tile: pages are no larger)
-            const int page = __float_as_int(blocks[i % kAhead][block].w);
-            there = page >= 0;
-            at = ((((size_t)max(page, 0) * c.kv_heads + work.head) << c.page_shift) + ((in_page + i * kKeys) & ((1 << c.page_shift) - 1)) + sub) * c.stride + piece * 16;
-        };
-        const auto fetch = [&](uint4 (&codes)[2][kParts], const uint8_t* side) {
-#pragma unroll
-            for (int r8 = 0; r8 < 2; ++r8)
-#pragma unroll
-                for (int j = 0; j < kParts; ++j)
-                    codes[r8][j] = there && piece * 16 + 64 * j < c.stride ? *reinterpret_cast<const uint4*>(side + at + (size_t)(8 * r8) * c.stride + 64 * j) : make_uint4(0u, 0u, 0u, 0u);
-        };
-        const auto lay = [&](const uint4 (&codes)[2][kParts], uint8_t* to, bool drop) {
+        const int block = warp - 8, sub = lane & 7;
+        const auto lay = [&](const uint8_t* from, uint8_t* to, bool zeros) {
 #pragma unroll
             for (int r8 = 0; r8 < 2; ++r8)
 #pragma unroll
                 for (int j = 0; j < kParts; ++j) {
-                    const uint32_t w[4] = {codes[r8][j].x, codes[r8][j].y, codes[r8][j].z, codes[r8][j].w};
-                    uint32_t u[8];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) decode4<FORMAT>(drop ? 0u : w[e], u[2 * e], u[2 * e + 1]);
-                    uint8_t* const d = to + (2 * block + r8) * (DP * 16) + (piece + 4 * j) * 256 + sub * 16;
-                    *reinterpret_cast<uint4*>(d) = make_uint4(u[0], u[1], u[2], u[3]);
-                    *reinterpret_cast<uint4*>(d + 128) = make_uint4(u[4], u[5], u[6], u[7]);
+                    const int piece = DP == 64 ? ((sub >> 1) + (lane >> 3)) & 3 : (sub + (lane >> 3) + 4 * j) & 7;
+                    uint4 w = make_uint4(0u, 0u, 0u, 0u);
+                    if (!zeros && piece * 16 < c.stride) w = *reinterpret_cast<const uint4*>(from + (block * kKvBlock + 8 * r8 + sub) * c.stride + piece * 16);
+                    uint4 lo, hi;
+                    decode4<FORMAT>(w.x, lo.x, lo.y);
+                    decode4<FORMAT>(w.y, lo.z, lo.w);
+                    decode4<FORMAT>(w.z, hi.x, hi.y);
+                    decode4<FORMAT>(w.w, hi.z, hi.w);
+                    uint8_t* const d = to + (2 * block + r8) * (DP * 16) + piece * 256 + sub * 16;
+                    *reinterpret_cast<uint4*>(d) = lo;
+                    *reinterpret_cast<uint4*>(d + 128) = hi;
                 }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
         };
-        if (n > 0) {
-            if (pair_wait(&m_full[0], 0u, polls)) {
-                find(0);
-                fetch(kc, c.keys);
-                fetch(vc, c.values);
-            } else {
-                ok = false;
-            }
-        }
 #pragma unroll 1
-        for (int i = 0; ok && i < n; ++i) {
-            const int st = i % kStages, next = (i + 1) % kAhead;
+        for (int i = 0; i < n; ++i) {
+            const int st = i % kStages;
             const uint32_t use = (uint32_t)(i / kStages);
-            const bool more = i + 1 < n, drop = which[i % kAhead].y >> block & 1u;
-            if (more && !pair_wait(&m_full[next], (uint32_t)((i + 1) / kAhead) & 1u, polls)) { ok = false; break; }
-            if (i >= kStages && !pair_wait(&k_empty[st], (use + 1) & 1, polls)) { ok = false; break; }
-            lay(kc, k_ring + st * T::kSide, false);
+            if (!pair_wait(&c_full[0], i & 1, polls) || (i >= kStages && !pair_wait(&k_empty[st], (use + 1) & 1, polls))) { ok = false; break; }
+            const uint3 of = which[i % kAhead];
+            const bool there = of.x >> block & 1u, zeros = !there || (of.y >> block & 1u);
+            lay(codes, k_ring + st * T::kSide, !there);
             if (lane == 0) {
                 mbar_arrive(&k_full[st]);
+                mbar_arrive(&c_empty[0]);
+            }
+            if (!pair_wait(&c_full[1], i & 1, polls) || (i >= kStages && !pair_wait(&v_empty[st], (use + 1) & 1, polls))) { ok = false; break; }
+            lay(codes + T::kCodes, v_ring + st * T::kSide, zeros);
+            if (lane == 0) {
+                mbar_arrive(&v_full[st]);
+                mbar_arrive(&c_empty[1]);
                 mbar_arrive(&m_empty[i % kAhead]);
             }
-            if (more) {
-                find(i + 1);
-                fetch(kc, c.keys);
-            }
-            if (i >= kStages && !pair_wait(&v_empty[st], (use + 1) & 1, polls)) { ok = false; break; }
-            lay(vc, v_ring + st * T::kSide, drop);
-            if (lane == 0) mbar_arrive(&v_full[st]);
-            if (more) fetch(vc, c.values);
         }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
         if (warp == 16) {
             const uint32_t idesc_s = (1u << 4) | ((uint32_t)(kKeys >> 3) << 17) | ((uint32_t)(kHalfRows >> 4) << 24);
             const uint32_t idesc_o = (1u << 4) | (1u << 16) | ((uint32_t)(DP >> 3) << 17) | ((uint32_t)(kHalfRows >> 4) << 24);
+            // What an instruction takes is known to be the same in every lane (broadcast from one, where it is used: kept over a turn, the operands of all would take more
+            // registers than there are)
+            const auto same = [](uint32_t v) {
+                asm volatile("" : "+r"(v));
+                return __shfl_sync(0xffffffffu, v, 0);
+            };
             const uint32_t q_at = smem_u32(q_tile), k_at = smem_u32(k_ring), v_at = smem_u32(v_ring);
-            const int u0 = n0, u1 = n1, un = max(u0, u1);
-            // What an instruction takes is broadcast from one lane, so that it is known to be the same in every lane and stays in uniform registers.
-            const auto same = [](uint32_t v) { return __shfl_sync(0xffffffffu, v, 0); };
+            const int u0 = (int)same((uint32_t)n0), u1 = (int)same((uint32_t)n1), un = max(u0, u1);
             // scores of tile i for half g; behind the last half the slot is free when they are there
-            const auto scores = [&](int g, int i) {
+            const auto scores = [&](auto half, auto slot, int i) {
+                constexpr uint32_t g = decltype(half)::value, st = decltype(slot)::value;
                 if (i >= un) return;
-                if (!pair_wait(&k_full[i % kStages], (uint32_t)(i / kStages) & 1u, polls)) { ok = false; return; }
+                if (!pair_wait(&k_full[st], (uint32_t)(i / kStages) & 1u, polls)) { ok = false; return; }
                 fence_after();
-                const uint32_t d = same(tmem + 128u * g), qa = same(q_at + g * (kHalfRows * DP * 2)), ka = same(k_at + (i % kStages) * T::kSide);
-                const uint64_t qd = block_desc(qa, 128u, DP * 16u), kd = block_desc(ka, 128u, DP * 16u);
+                const bool mine = i < (g ? u1 : u0);
+                const uint32_t tm = same(tmem), qa = same(q_at + g * (kHalfRows * DP * 2)), ka = same(k_at + st * T::kSide);
                 if (elect_one_sync()) {
-                    if (i < (g ? u1 : u0)) {
+                    if (mine) {
+                        const uint64_t qd = block_desc(qa, 128u, DP * 16u), kd = block_desc(ka, 128u, DP * 16u);
 #pragma unroll
-                        for (uint32_t k = 0; k < kSteps; ++k) umma_bf16(d, qd + 16u * k, kd + 16u * k, idesc_s, k != 0);
+                        for (uint32_t k = 0; k < kSteps; ++k) umma_bf16(tm + 128u * g, qd + 16u * k, kd + 16u * k, idesc_s, k != 0);
                         umma_commit(&s_full[g]);
                     }
-                    if (g == 1) umma_commit(&k_empty[i % kStages]);
+                    if (g == 1) umma_commit(&k_empty[st]);
                 }
                 __syncwarp();
             };
-            const auto values = [&](int g, int i) {
-                if (i < (g ? u1 : u0) && !pair_wait(&p_ready[g], i & 1, polls)) { ok = false; return; }
-                if (!pair_wait(&v_full[i % kStages], (uint32_t)(i / kStages) & 1u, polls)) { ok = false; return; }
+            const auto values = [&](auto half, auto slot, int i) {
+                constexpr uint32_t g = decltype(half)::value, st = decltype(slot)::value;
+                const bool mine = i < (g ? u1 : u0);
+                if (mine && !pair_wait(&p_ready[g], i & 1, polls)) { ok = false; return; }
+                if (!pair_wait(&v_full[st], (uint32_t)(i / kStages) & 1u, polls)) { ok = false; return; }
                 fence_after();
-                const uint32_t d = same(tmem + 256u + 128u * g), w = same(tmem + 128u * g), va = same(v_at + (i % kStages) * T::kSide), later = same(i != 0);
-                const uint64_t vd = block_desc(va, DP * 16u, 128u);
+                const uint32_t later = i != 0, tm = same(tmem), va = same(v_at + st * T::kSide);
                 if (elect_one_sync()) {
-                    if (i < (g ? u1 : u0)) {
+                    if (mine) {
+                        const uint64_t vd = block_desc(va, DP * 16u, 128u);
 #pragma unroll
-                        for (uint32_t k = 0; k < kKeys / 16; ++k) mma_weights(d, w + 8u * k, vd + 2u * DP * k, idesc_o, k != 0 ? 1u : later);
+                        for (uint32_t k = 0; k < kKeys / 16; ++k) mma_weights(tm + 256u + 128u * g, tm + 128u * g + 8u * k, vd + 2u * DP * k, idesc_o, k != 0 ? 1u : later);
                         umma_commit(&pv_done[g]);
                     }
-                    if (g == 1) umma_commit(&v_empty[i % kStages]);
+                    if (g == 1) umma_commit(&v_empty[st]);
                 }
                 __syncwarp();
             };
-            scores(0, 0);
-            if (ok) scores(1, 0);
+            using First = std::integral_constant<uint32_t, 0>;
+            using Second = std::integral_constant<uint32_t, 1>;
+            const auto turn = [&](auto slot, int i) {
+                constexpr uint32_t st = decltype(slot)::value;
+                using Next = std::integral_constant<uint32_t, (st + 1) % kStages>;
+                if (ok && i < un) values(First{}, slot, i);
+                if (ok && i < un) scores(First{}, Next{}, i + 1);
+                if (ok && i < un) values(Second{}, slot, i);
+                if (ok && i < un) scores(Second{}, Next{}, i + 1);
+            };
+            scores(First{}, First{}, 0);
+            if (ok) scores(Second{}, First{}, 0);
 #pragma unroll 1
-            for (int i = 0; ok && i < un; ++i) {
-#pragma unroll 1
-                for (int g = 0; ok && g < 2; ++g) {
-                    values(g, i);
-                    if (ok) scores(g, i + 1);
+            for (int i = 0; ok && i < un; i += kStages) {
+                turn(First{}, i);
+                turn(Second{}, i + 1);
+                if constexpr (kStages == 4) {
+                    turn(std::integral_constant<uint32_t, 2>{}, i + 2);
+                    turn(std::integral_constant<uint32_t, 3>{}, i + 3);
                 }
             }
             mmas_ended<false>(&done);
@@ -599,6 +579,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cac
                 return page >= 0 ? make_float2(c.key_scales[at], c.value_scales[at]) : make_float2(0.f, 0.f);
             };
             int page = page_of(0), page_next = page_of(1);
+            unsigned issued = 0;                              // of the copies, keys and values in turn
             float2 scales = scales_of(page);
 #pragma unroll 1
             for (int i = 0; i < n; ++i) {
@@ -607,17 +588,32 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cac
                 page = page_next;
                 scales = scales_of(page);
                 page_next = page_of(i + 2);
-                const uint32_t v = __float_as_uint(now.y);
-                const bool number = v < 0x7f800000u;
-                const int e = (int)(v >> 23) - 127 - (largest == -1000 ? 0 : largest), kept = max(e, -kSpread);
+                // (a page that is not there, or stands for NaNs: the scores say so, and what is times them is finite)
+                const uint32_t k = __float_as_uint(now.x), v = __float_as_uint(now.y);
+                const bool number = page_now >= 0 && k < 0x7f800000u && v < 0x7f800000u;
+                const int e = (int)(v >> 23) - 127 - (largest == -1000 ? 0 : largest), kept = number ? max(e, -kSpread) : 0;
                 if (i >= kAhead && !pair_wait(&m_empty[slot], (uint32_t)(i / kAhead + 1) & 1u, polls)) { ok = false; break; }
-                const uint32_t there = __ballot_sync(0xffffffffu, page_now >= 0), zeros = __ballot_sync(0xffffffffu, page_now >= 0 && number && e < -kSpread);
-                if (lane < kBlocks)
-                    blocks[slot][lane] = make_float4(now.x, page_now < 0 ? 0.f : number ? (float)kept : __uint_as_float(0x7fc00000u),
-                                                     page_now >= 0 && number ? __uint_as_float((uint32_t)(127 - kept) << 23) : 1.f, __int_as_float(page_now));
-                if (lane == 0) which[slot] = make_uint2(there & 0xffu, zeros & 0xffu);
+                const uint32_t there = __ballot_sync(0xffffffffu, page_now >= 0), zeros = __ballot_sync(0xffffffffu, number && e < -kSpread), numbers = __ballot_sync(0xffffffffu, number || page_now < 0);
+                if (lane < kBlocks) blocks[slot][lane] = make_float4(number ? fmaxf(now.x, 0x1p-126f) : 1.f, (float)kept, __uint_as_float((uint32_t)(127 - kept) << 23), __int_as_float(page_now));
+                if (lane == 0) which[slot] = make_uint3(there & 0xffu, zeros & 0xffu, numbers & 0xffu);
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&m_full[slot]);
+                // the tile's codes, a copy per block, as soon as the last ones have been read
+                const uint32_t bytes = (uint32_t)(kKvBlock * c.stride);
+                const size_t at = ((((size_t)max(page_now, 0) * c.kv_heads + work.head) << c.page_shift) + (size_t)((((long long)from + i) * kKeys + lane * kKvBlock) & ((1 << c.page_shift) - 1))) * c.stride;
+                for (int side = 0; ok && side < 2; ++side) {
+                    if (i > 0 && !pair_wait(&c_empty[side], (i + 1) & 1, polls)) { ok = false; break; }
+                    if (lane == 0) mbar_arrive_expect_tx(&c_full[side], bytes * __popc(there & 0xffu));
+                    __syncwarp();
+                    if (lane < kBlocks && page_now >= 0) bulk_g2s(codes + side * T::kCodes + lane * bytes, (side ? c.values : c.keys) + at, bytes, &c_full[side]);
+                    issued = 2 * i + side + 1;
+                }
+                if (!ok) break;
+            }
+            // (copies in flight where a wait ran out)
+            if (lane == 0 && !ok) {
+                if (issued > 0) (void)lane_wait(&c_full[0], ((issued - 1) >> 1) & 1u, kDrainPolls);
+                if (issued > 1) (void)lane_wait(&c_full[1], ((issued - 2) >> 1) & 1u, kDrainPolls);
             }
         }
     }
