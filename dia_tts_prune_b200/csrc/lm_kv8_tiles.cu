@@ -1,14 +1,14 @@
 // lm_kv8_tiles.cu - attention of many rows over the cache in 8 bits, on the 5th-generation tensor cores.
 //
 // A CTA takes 256 (token, query head) rows that share a key head and walks their keys 128 at a time:
-//   warps 0-3, 4-7   one thread per row, 128 rows each: scores from tensor memory, softmax weights back to it.  The two halves are in different stages of a tile,
-//                    so that the tensor cores have one half's products while the other half takes exponentials
+//   warps 0-3, 4-7   one thread per row, 128 rows each: 64 scores at a time from tensor memory, softmax weights back to where they lay.  A half has two places for scores, so
+//                    that the next ones are there when it has weighed these
 //   warps 8-15       codes to fp16 operands, from shared memory to shared memory, 16 tokens each
-//   warp 16          one elected lane issues tcgen05.mma: S = Q K^T (M = 128, N = 128), then O += P V with P as the operand in tensor memory, where S lay
+//   warp 16          one elected lane issues tcgen05.mma: S = Q K^T (M = 128, N = 64), and O += P V with P as the operand in tensor memory
 //   warp 17          looks up pages and scales, and fetches the next tile's codes by bulk copies
 //
 // Numbers.  t = scale log2(e) q . key + e - E in powers of two, e the exponent of the page's values and E the largest of the CTA's pages; P = 2^(t - R + 7) in fp16, with R the
-// row's reference: about its largest t so far, raised (and O and the sum with it) only when a tile's largest lies more than 8 above it, so P is at most 2^15.  That the page's value
+// row's reference: about its largest t so far, raised (and O and the sum with it) only when one of 64 scores lies more than 8 above it, so P is at most 2^15.  That the page's value
 // scale is inside
 // the weight lets codes be multiplied as they are, and the 11 bits of P count from the largest contribution.  The denominator takes 2^(E - e) out again, per 16 tokens.  Pages whose
 // values are 2^80 below the largest page's are taken as zeros.  Queries are scaled by a power of two per row (exact but for channels 2^-27 below the row's largest).  Sums are fp32;
@@ -33,14 +33,15 @@ namespace {
 
 using namespace dia;
 
-constexpr int kKeys = 128, kHalfRows = 128, kTileRows = 2 * kHalfRows, kThreads = 640, kSms = 148;
+constexpr int kKeys = 128, kStepKeys = 64, kHalfRows = 128, kTileRows = 2 * kHalfRows, kThreads = 640, kSms = 148;
 constexpr int kBlocks = kKeys / kKvBlock;                      // blocks of 16 tokens in a tile of keys
 constexpr int kMinChunk = 4;                                   // tiles of keys that are worth a CTA of their own
 constexpr float kSlack = 8.f, kBits = 7.f;                     // see above
 constexpr int kSpread = 80;
-constexpr int kSoftmaxRegs = 168, kFetchRegs = 40, kIssueRegs = 64;
-static_assert(128 * (2 * kSoftmaxRegs + 2 * kFetchRegs + kIssueRegs) <= kThreads * 96, "the split is within the launch's registers");
-constexpr int kAhead = 8;                                      // tiles whose pages and scales are known
+constexpr int kLaunchRegs = 96, kSoftmaxRegs = 144, kFetchRegs = 48, kIssueRegs = 88;
+static_assert(128 * (2 * kSoftmaxRegs + 2 * kFetchRegs + kIssueRegs) <= kThreads * kLaunchRegs, "the split is within the launch's registers");
+static_assert(kSoftmaxRegs >= kLaunchRegs && kFetchRegs <= kLaunchRegs && kIssueRegs <= kLaunchRegs, "who gives registers and who takes them");
+constexpr int kAhead = 4;                                      // tiles whose pages and scales are known
 
 template <int DP>
 struct Tiles {
@@ -82,7 +83,7 @@ __device__ __forceinline__ long long scan(long long mine, long long* sums, long 
     if (lane == 31) sums[warp] = upto;
     __syncthreads();
     total = 0;
-#pragma unroll 1
+#pragma unroll
     for (int w = 0; w < THREADS / 32; ++w) {
         if (w < warp) upto += sums[w];
         total += sums[w];
@@ -104,8 +105,10 @@ __device__ __forceinline__ Work find_work(const Kv8Cache& c, const Kv8Step& s, c
     const int each = (s.sequences + THREADS - 1) / THREADS, i0 = threadIdx.x * each, i1 = min(i0 + each, s.sequences);
     long long items = 0, total_items, ctas = 0, total;
     int most = 0;
+    const Sequence mine = sequence_at(s, a, min(i0, s.sequences - 1), group, c.page_shift);       // (a thread's only one, mostly)
+    const auto at = [&](int i) { return i == i0 ? mine : sequence_at(s, a, i, group, c.page_shift); };
     for (int i = i0; i < i1; ++i) {
-        const Sequence q = sequence_at(s, a, i, group, c.page_shift);
+        const Sequence q = at(i);
         items += (long long)q.tiles * c.kv_heads;
         if (q.tiles) most = max(most, q.high - q.low);
     }
@@ -115,14 +118,14 @@ __device__ __forceinline__ Work find_work(const Kv8Cache& c, const Kv8Step& s, c
     const int length = total_items >= kSms ? 0x7fffffff : max(kMinChunk, (longest + kSms / (int)total_items - 1) / (kSms / (int)total_items));
     const auto chunks_of = [&](const Sequence& q) { return length == 0x7fffffff ? 1 : max(1, (q.high - q.low + length - 1) / length); };
     for (int i = i0; i < i1; ++i) {
-        const Sequence q = sequence_at(s, a, i, group, c.page_shift);
+        const Sequence q = at(i);
         ctas += (long long)q.tiles * c.kv_heads * chunks_of(q);
     }
     const long long before = scan<THREADS>(ctas, sums, total);
     long long base = JOIN ? items_before : before, cta = before;
     if (index >= base && index < base + (JOIN ? items : ctas)) {
         for (int i = i0;; ++i) {
-            const Sequence q = sequence_at(s, a, i, group, c.page_shift);
+            const Sequence q = at(i);
             const int chunks = chunks_of(q);
             const long long own = (long long)q.tiles * c.kv_heads, units = JOIN ? own : own * chunks;
             if (index < base + units) {
@@ -150,10 +153,14 @@ __device__ __forceinline__ void tmem_load32(uint32_t addr, float* v) {
 #pragma unroll
     for (int e = 0; e < 32; ++e) v[e] = __uint_as_float(u[e]);
 }
-__device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t (&v)[16]) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]),
-                 "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
-                 : "memory");
+__device__ __forceinline__ void tmem_store32(uint32_t addr, const uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(addr),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]),
+        "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]),
+        "r"(v[29]), "r"(v[30]), "r"(v[31])
+        : "memory");
 }
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
@@ -182,7 +189,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cac
     uint8_t* const k_ring = smem + T::kQ;
     uint8_t* const v_ring = k_ring + kStages * T::kSide;
     uint8_t* const codes = v_ring + kStages * T::kSide;       // [keys, values]
-    __shared__ uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], m_full[kAhead], m_empty[kAhead], c_full[2], c_empty[2], s_full[2], p_ready[2], pv_done[2], done;
+    __shared__ uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], m_full[kAhead], m_empty[kAhead], c_full[2], c_empty[2], s_full[2][2], p_ready[2][2], pv_done[2][2], done;
     __shared__ float4 blocks[kAhead][kBlocks];                // (key scale, e - E, 2^(E - e), page) of 16 tokens
     __shared__ uint3 which[kAhead];                           // of a tile's blocks: those that are there, whose values are taken as zeros, that stand for numbers
     __shared__ uint32_t tmem_slot;
@@ -207,9 +214,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cac
         for (int g = 0; g < 2; ++g) {
             mbar_init(&c_full[g], 1);
             mbar_init(&c_empty[g], 8);
-            mbar_init(&s_full[g], 1);
-            mbar_init(&p_ready[g], 4);
-            mbar_init(&pv_done[g], 1);
+            for (int i = 0; i < 2; ++i) {
+                mbar_init(&s_full[g][i], 1);
+                mbar_init(&p_ready[g][i], 4);
+                mbar_init(&pv_done[g][i], 1);
+            }
         }
         mbar_init(&done, 1);
         largest = -1000;
@@ -225,15 +234,17 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cac
     const long long back = a.window > 0 ? a.window - 1 : (1ll << 40);
     const int from = max(max(q.low, (int)(max(0ll, position(p0) - back) / kKeys)), work.length == 0x7fffffff ? 0 : q.low + work.chunk * work.length);
     const int limit = work.length == 0x7fffffff ? q.high : (int)min((long long)q.high, (long long)q.low + (long long)(work.chunk + 1) * work.length);
-    const auto tiles_of = [&](int g) {
+    const auto steps_of = [&](int g) {
         if (p0 + g * kHalfRows >= pairs || q.past < 0) return 0;
-        return (int)max(0ll, min((long long)limit, position(p0 + g * kHalfRows + kHalfRows - 1) / kKeys + 1) - from);
+        const long long end = min((long long)limit * kKeys, position(p0 + g * kHalfRows + kHalfRows - 1) + 1) - (long long)from * kKeys;
+        return (int)max(0ll, (end + kStepKeys - 1) / kStepKeys);
     };
-    const int n0 = tiles_of(0), n1 = tiles_of(1), n = max(n0, n1);
+    const int n0 = steps_of(0), n1 = steps_of(1), n = (max(n0, n1) + 1) / 2;       // steps of the halves, tiles
     __syncthreads();                                          // (the largest exponent is set)
-    {
+    float row_scale = 0.f;
+    if (warp >= 8) {
         int most = -1000;
-        for (int b = threadIdx.x; b < n * kBlocks; b += kThreads) {
+        for (int b = threadIdx.x - 256; b < n * kBlocks; b += kThreads - 256) {
             const int page = s.page(work.seq, ((long long)from * kKeys + (long long)b * kKvBlock) >> c.page_shift, c.pages);
             if (page < 0) continue;
             const uint32_t v = __float_as_uint(c.value_scales[(size_t)page * c.kv_heads + work.head]);
@@ -241,27 +252,28 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cac
         }
         most = __reduce_max_sync(0xffffffffu, most);
         if (lane == 0 && most > -1000) atomicMax(&largest, most);
-    }
-    // queries: a thread takes its row
-    float row_scale = 0.f;
-    if (warp < 8) {
-        const int r = threadIdx.x, p = p0 + r;
-        uint8_t* const to = q_tile + (r >> 7) * (kHalfRows * DP * 2) + ((r & 127) >> 3) * (DP * 16) + (r & 7) * 16;
-        const long long at = (q.begin + (long long)(min(p, pairs - 1) / group)) * a.q.row + (long long)(work.head * group + min(p, pairs - 1) % group) * a.q.head;
+    } else {
+        // queries: a warp takes its 32 rows, eight at a time, a lane DP / 4 channels of one in pieces of eight
+        constexpr int kPieces = DP / 32;
+        const int sub = lane & 7;
         const bool wide = c.dim % 8 == 0 && (reinterpret_cast<uintptr_t>(a.q.x) & 15) == 0 && a.q.row % 8 == 0 && a.q.head % 8 == 0;
-        uint4 w[DP / 8];
+        uint4 w[4][kPieces];
 #pragma unroll
-        for (int j = 0; j < DP / 8; ++j) {
-            w[j] = make_uint4(0u, 0u, 0u, 0u);
-            if (p < pairs) {
-                const uint16_t* const x = reinterpret_cast<const uint16_t*>(a.q.x) + at + 8 * j;
+        for (int r8 = 0; r8 < 4; ++r8) {
+            const int p = p0 + warp * 32 + r8 * 8 + sub, in = min(p, pairs - 1);
+            const uint16_t* const row = reinterpret_cast<const uint16_t*>(a.q.x) + (q.begin + (long long)(in / group)) * a.q.row + (long long)(work.head * group + in % group) * a.q.head;
+#pragma unroll
+            for (int j = 0; j < kPieces; ++j) {
+                const int d = 8 * ((lane >> 3) + 4 * j);
+                w[r8][j] = make_uint4(0u, 0u, 0u, 0u);
+                if (p >= pairs || d >= c.dim) continue;
                 if (wide) {
-                    if (8 * j < c.dim) w[j] = *reinterpret_cast<const uint4*>(x);
+                    w[r8][j] = *reinterpret_cast<const uint4*>(row + d);
                 } else {
                     uint16_t y[8];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) y[e] = 8 * j + e < c.dim ? x[e] : 0;
-                    memcpy(&w[j], y, 16);
+                    for (int e = 0; e < 8; ++e) y[e] = d + e < c.dim ? row[d + e] : 0;
+                    memcpy(&w[r8][j], y, 16);
                 }
             }
         }
@@ -269,28 +281,34 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cac
             if (a.type == kTypeBf16) return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
             return __half22float2(*reinterpret_cast<const __half2*>(&u));
         };
-        uint32_t most = 0;
 #pragma unroll
-        for (int j = 0; j < DP / 8; ++j) {
-            const uint32_t u[4] = {w[j].x, w[j].y, w[j].z, w[j].w};
+        for (int r8 = 0; r8 < 4; ++r8) {
+            uint32_t most = 0;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float2 f = numbers(u[e]);
-                most = max(most, max(__float_as_uint(f.x) & 0x7fffffffu, __float_as_uint(f.y) & 0x7fffffffu));
+            for (int j = 0; j < kPieces; ++j) {
+                const uint32_t u[4] = {w[r8][j].x, w[r8][j].y, w[r8][j].z, w[r8][j].w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float2 f = numbers(u[e]);
+                    most = max(most, max(__float_as_uint(f.x) & 0x7fffffffu, __float_as_uint(f.y) & 0x7fffffffu));
+                }
             }
-        }
-        const uint32_t e = most == 0 ? 127u : max(most >> 23, 14u);
-        const float f = __uint_as_float((267u - e) << 23), way_back = __uint_as_float((e - 13u) << 23);       // 2^(140 - e): to below 2^14, and the way back
-        row_scale = e == 255u ? __uint_as_float(0x7fc00000u) : way_back * (a.scale * kLog2e);
+            most = max(most, __shfl_xor_sync(0xffffffffu, most, 8));
+            most = max(most, __shfl_xor_sync(0xffffffffu, most, 16));
+            const uint32_t e = most == 0 ? 127u : max(most >> 23, 14u);
+            const float f = __uint_as_float((267u - e) << 23), way_back = __uint_as_float((e - 13u) << 23);       // 2^(140 - e): to below 2^14, and the way back
+            if (r8 == lane >> 3) row_scale = e == 255u ? __uint_as_float(0x7fc00000u) : way_back * (a.scale * kLog2e);      // (a thread's own row is 8 r8 + sub of its warp's)
+            uint8_t* const to = q_tile + (warp >> 2) * (kHalfRows * DP * 2) + ((warp & 3) * 4 + r8) * (DP * 16) + sub * 16;
 #pragma unroll
-        for (int j = 0; j < DP / 8; ++j) {
-            uint32_t u[4] = {w[j].x, w[j].y, w[j].z, w[j].w};
+            for (int j = 0; j < kPieces; ++j) {
+                uint32_t u[4] = {w[r8][j].x, w[r8][j].y, w[r8][j].z, w[r8][j].w};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float2 y = numbers(u[i]);
-                u[i] = e == 255u ? 0u : pack_half(y.x * f, y.y * f);
+                for (int i = 0; i < 4; ++i) {
+                    const float2 y = numbers(u[i]);
+                    u[i] = e == 255u ? 0u : pack_half(y.x * f, y.y * f);
+                }
+                *reinterpret_cast<uint4*>(to + ((lane >> 3) + 4 * j) * 128) = make_uint4(u[0], u[1], u[2], u[3]);
             }
-            *reinterpret_cast<uint4*>(to + j * 128) = make_uint4(u[0], u[1], u[2], u[3]);
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
@@ -304,29 +322,32 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cac
     if (warp < 8) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
         const int g = warp >> 2, count = g ? n1 : n0;
-        const uint32_t lanes = (uint32_t)(warp & 3) * 32u << 16, t_s = tmem + lanes + 128u * g, t_o = tmem + lanes + 256u + 128u * g;
+        const uint32_t lanes = (uint32_t)(warp & 3) * 32u << 16, t_scores = tmem + lanes + 128u * g, t_o = tmem + lanes + 256u + 128u * g;
         const int p = p0 + threadIdx.x;
         // the tokens that the row sees, and the ones that all 128 rows see, counted from the first tile on
         const long long tok0 = (long long)from * kKeys;
         const auto within = [&](long long v) { return (int)max(min(v - tok0, 0x7fffff00ll), -1ll); };
         const int hi = within(position(p)), lo = within(position(p) - back), all_hi = within(position(p0 + g * kHalfRows)), all_lo = within(position(p0 + g * kHalfRows + kHalfRows - 1) - back);
         float ref = -1e30f, l = 0.f;
+        // (A step's scores come behind the value product of two steps before, not of the last one: what is told of every step has a barrier for the even ones and one for the odd.)
 #pragma unroll 1
-        for (int i = 0; i < count; ++i) {
-            const int slot = i % kAhead;
-            if (!pair_wait(&m_full[slot], (uint32_t)(i / kAhead) & 1u, polls)) { ok = false; break; }
-            const uint32_t there = which[slot].x, numbers = which[slot].z;
-            const int tok = i * kKeys;
-            const bool clear = (there & numbers) == 0xffu && tok + kKeys - 1 <= all_hi && tok >= all_lo;
-            if (!pair_wait(&s_full[g], i & 1, polls)) { ok = false; break; }
+        for (int t = 0; t < count; ++t) {
+            const int i = t >> 1, half = t & 1, slot = i % kAhead;
+            if (half == 0 && !pair_wait(&m_full[slot], (uint32_t)(i / kAhead) & 1u, polls)) { ok = false; break; }
+            const uint32_t there = which[slot].x >> (4 * half), numbers = which[slot].z >> (4 * half);
+            const float4* const meta_of = &blocks[slot][4 * half];
+            const int tok = t * kStepKeys;
+            const uint32_t t_s = t_scores + kStepKeys * half;
+            const bool clear = (there & numbers & 0xfu) == 0xfu && tok + kStepKeys - 1 <= all_hi && tok >= all_lo;
+            if (!pair_wait(&s_full[g][half], i & 1, polls)) { ok = false; break; }
             fence_after();
-            uint32_t x[4][32];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) tmem_columns32(t_s + 32 * j, x[j]);
+            uint32_t x[2][32];
+            tmem_columns32(t_s, x[0]);
+            tmem_columns32(t_s + 32, x[1]);
             tmem_loaded();
             if (!clear) {
 #pragma unroll
-                for (int b = 0; b < kBlocks; ++b) {
+                for (int b = 0; b < 4; ++b) {
                     const bool block = there >> b & 1u;
                     const uint32_t nan = numbers >> b & 1u ? 0u : 0x7fffffffu;      // (what a row sees of a page that stands for NaNs)
 #pragma unroll
@@ -340,8 +361,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cac
             const auto score = [&](int b, int e) { return __uint_as_float(x[b / 2][16 * (b & 1) + e]); };
             float top = -INFINITY;
 #pragma unroll
-            for (int b = 0; b < kBlocks; ++b) {
-                const float2 meta = *reinterpret_cast<const float2*>(&blocks[slot][b]);
+            for (int b = 0; b < 4; ++b) {
+                const float2 meta = *reinterpret_cast<const float2*>(meta_of + b);
                 float m = max3(score(b, 0), score(b, 1), score(b, 2));
 #pragma unroll
                 for (int e = 3; e < kKvBlock - 1; e += 2) m = max3(m, score(b, e), score(b, e + 1));
@@ -351,58 +372,54 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cac
                 const float next = top > ref + kSlack ? top : ref, f = exp2_fast(ref - next);
                 ref = next;
                 l *= f;
-                if (i > 0) {
-                    if (!pair_wait(&pv_done[g], (i - 1) & 1, polls)) { ok = false; break; }
+                if (t > 0) {
+                    if (!pair_wait(&pv_done[g][half ^ 1], (uint32_t)((t - 1) >> 1) & 1u, polls)) { ok = false; break; }
                     fence_after();
 #pragma unroll 1
-                    for (int j = 0; j < DP; j += 16) {
-                        uint32_t o[16];
-                        tmem_columns16(t_o + j, o);
+                    for (int j = 0; j < DP; j += 32) {
+                        uint32_t o[32];
+                        tmem_columns32(t_o + j, o);
                         tmem_loaded();
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                        tmem_store16(t_o + j, o);
+                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                        tmem_store32(t_o + j, o);
                     }
                 }
             }
+            uint32_t w[32];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                uint32_t w[16];
+            for (int b = 0; b < 4; ++b) {
+                const float4 meta = meta_of[b];
+                const f2 k2 = twice(meta.x * row_scale), c2 = twice(meta.y - ref + kBits);
+                f2 sum[2] = {0, 0};
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int b = 2 * j + h;
-                    const float4 meta = blocks[slot][b];
-                    const f2 k2 = twice(meta.x * row_scale), c2 = twice(meta.y - ref + kBits);
-                    f2 sum[2] = {0, 0};
-#pragma unroll
-                    for (int e = 0; e < kKvBlock; e += 2) {
-                        float y0, y1;
-                        unpack2(fma2(pack2(score(b, e), score(b, e + 1)), k2, c2), y0, y1);
-                        y0 = exp2_fast(y0);
-                        y1 = exp2_fast(y1);
-                        sum[e / 2 & 1] = add2(sum[e / 2 & 1], pack2(y0, y1));
-                        w[8 * h + e / 2] = pack_half(y0, y1);
-                    }
-                    float s0, s1;
-                    unpack2(add2(sum[0], sum[1]), s0, s1);
-                    l = fmaf(s0 + s1, meta.z, l);
+                for (int e = 0; e < kKvBlock; e += 2) {
+                    float y0, y1;
+                    unpack2(fma2(pack2(score(b, e), score(b, e + 1)), k2, c2), y0, y1);
+                    y0 = exp2_fast(y0);
+                    y1 = exp2_fast(y1);
+                    sum[e / 2 & 1] = add2(sum[e / 2 & 1], pack2(y0, y1));
+                    w[8 * b + e / 2] = pack_half(y0, y1);
                 }
-                tmem_store16(t_s + 16 * j, w);
+                float s0, s1;
+                unpack2(add2(sum[0], sum[1]), s0, s1);
+                l = fmaf(s0 + s1, meta.z, l);
             }
+            tmem_store32(t_s, w);
             tmem_stored();
             fence_before();
             __syncwarp();
             if (lane == 0) {
-                mbar_arrive(&m_empty[slot]);
-                mbar_arrive(&p_ready[g]);
+                mbar_arrive(&p_ready[g][half]);
+                if (half == 1 || t + 1 == count) mbar_arrive(&m_empty[slot]);
             }
         }
         // (a half that looks at fewer tiles lets the others have the rest)
-        for (int i = count; ok && i < n; ++i) {
+        for (int i = (count + 1) / 2; ok && i < n; ++i) {
             if (!pair_wait(&m_full[i % kAhead], (uint32_t)(i / kAhead) & 1u, polls)) ok = false;
             else if (lane == 0) mbar_arrive(&m_empty[i % kAhead]);
         }
-        if (ok && count > 0 && !pair_wait(&pv_done[g], (count - 1) & 1, polls)) ok = false;
+        if (ok && count > 0 && !pair_wait(&pv_done[g][(count - 1) & 1], (uint32_t)((count - 1) >> 1) & 1u, polls)) ok = false;
         fence_after();
         // out
         float m = ref - kBits, w = m + spread + kWeightBits;
@@ -502,7 +519,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cac
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
         if (warp == 16) {
-            const uint32_t idesc_s = (1u << 4) | ((uint32_t)(kKeys >> 3) << 17) | ((uint32_t)(kHalfRows >> 4) << 24);
+            const uint32_t idesc_s = (1u << 4) | ((uint32_t)(kStepKeys >> 3) << 17) | ((uint32_t)(kHalfRows >> 4) << 24);
             const uint32_t idesc_o = (1u << 4) | (1u << 16) | ((uint32_t)(DP >> 3) << 17) | ((uint32_t)(kHalfRows >> 4) << 24);
             // What an instruction takes is known to be the same in every lane (broadcast from one, where it is used: kept over a turn, the operands of all would take more
             // registers than there are)
@@ -512,62 +529,75 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cac
             };
             const uint32_t q_at = smem_u32(q_tile), k_at = smem_u32(k_ring), v_at = smem_u32(v_ring);
             const int u0 = (int)same((uint32_t)n0), u1 = (int)same((uint32_t)n1), un = max(u0, u1);
-            // scores of tile i for half g; behind the last half the slot is free when they are there
-            const auto scores = [&](auto half, auto slot, int i) {
-                constexpr uint32_t g = decltype(half)::value, st = decltype(slot)::value;
-                if (i >= un) return;
-                if (!pair_wait(&k_full[st], (uint32_t)(i / kStages) & 1u, polls)) { ok = false; return; }
-                fence_after();
-                const bool mine = i < (g ? u1 : u0);
-                const uint32_t tm = same(tmem), qa = same(q_at + g * (kHalfRows * DP * 2)), ka = same(k_at + st * T::kSide);
-                if (elect_one_sync()) {
-                    if (mine) {
-                        const uint64_t qd = block_desc(qa, 128u, DP * 16u), kd = block_desc(ka, 128u, DP * 16u);
+            uint32_t tm_now, q_now, k_now;
+            // A turn of half g behind its weights of step t: their values, and the scores two steps on, whose place the weights had.  A slot's last products free it.
+            const auto scores = [&](auto half_, auto slot_, auto step_, int t) {          // (one lane)
+                constexpr uint32_t g = decltype(half_)::value, st = decltype(slot_)::value, h = decltype(step_)::value;
+                const uint64_t qd = block_desc(q_now, 128u, DP * 16u), kd = block_desc(k_now, 128u, DP * 16u);
+                if (t < (g ? u1 : u0)) {
 #pragma unroll
-                        for (uint32_t k = 0; k < kSteps; ++k) umma_bf16(tm + 128u * g, qd + 16u * k, kd + 16u * k, idesc_s, k != 0);
-                        umma_commit(&s_full[g]);
-                    }
-                    if (g == 1) umma_commit(&k_empty[st]);
+                    for (uint32_t k = 0; k < kSteps; ++k) umma_bf16(tm_now + 128u * g + kStepKeys * h, qd + 16u * k, kd + 16u * k, idesc_s, k != 0);
+                    umma_commit(&s_full[g][h]);
                 }
-                __syncwarp();
+                if (g == 1 && h == 1) umma_commit(&k_empty[st]);
             };
-            const auto values = [&](auto half, auto slot, int i) {
-                constexpr uint32_t g = decltype(half)::value, st = decltype(slot)::value;
-                const bool mine = i < (g ? u1 : u0);
-                if (mine && !pair_wait(&p_ready[g], i & 1, polls)) { ok = false; return; }
-                if (!pair_wait(&v_full[st], (uint32_t)(i / kStages) & 1u, polls)) { ok = false; return; }
-                fence_after();
-                const uint32_t later = i != 0, tm = same(tmem), va = same(v_at + st * T::kSide);
-                if (elect_one_sync()) {
-                    if (mine) {
-                        const uint64_t vd = block_desc(va, DP * 16u, 128u);
-#pragma unroll
-                        for (uint32_t k = 0; k < kKeys / 16; ++k) mma_weights(tm + 256u + 128u * g, tm + 128u * g + 8u * k, vd + 2u * DP * k, idesc_o, k != 0 ? 1u : later);
-                        umma_commit(&pv_done[g]);
-                    }
-                    if (g == 1) umma_commit(&v_empty[st]);
-                }
-                __syncwarp();
-            };
-            using First = std::integral_constant<uint32_t, 0>;
-            using Second = std::integral_constant<uint32_t, 1>;
-            const auto turn = [&](auto slot, int i) {
-                constexpr uint32_t st = decltype(slot)::value;
+            const auto turn = [&](auto half_, auto slot_, auto step_, int t) {
+                constexpr uint32_t g = decltype(half_)::value, st = decltype(slot_)::value, h = decltype(step_)::value;
                 using Next = std::integral_constant<uint32_t, (st + 1) % kStages>;
-                if (ok && i < un) values(First{}, slot, i);
-                if (ok && i < un) scores(First{}, Next{}, i + 1);
-                if (ok && i < un) values(Second{}, slot, i);
-                if (ok && i < un) scores(Second{}, Next{}, i + 1);
+                const bool mine = t < (g ? u1 : u0), more = t + 2 < un;
+                if (!ok || t >= un) return;
+                if (mine && !pair_wait(&p_ready[g][h], (uint32_t)(t >> 1) & 1u, polls)) { ok = false; return; }
+                if (g == 0 && h == 0 && !pair_wait(&v_full[st], (uint32_t)((t >> 1) / kStages) & 1u, polls)) { ok = false; return; }
+                if (g == 0 && h == 0 && more && !pair_wait(&k_full[Next::value], (uint32_t)(((t >> 1) + 1) / kStages) & 1u, polls)) { ok = false; return; }
+                fence_after();
+                tm_now = same(tmem);
+                q_now = same(q_at + g * (kHalfRows * DP * 2));
+                k_now = same(k_at + Next::value * T::kSide + h * (T::kSide / 2));
+                const uint32_t v_now = same(v_at + st * T::kSide + h * (T::kSide / 2)), later = t != 0;
+                if (elect_one_sync()) {
+                    if (mine) {
+                        const uint64_t vd = block_desc(v_now, DP * 16u, 128u);
+#pragma unroll
+                        for (uint32_t k = 0; k < kStepKeys / 16; ++k)
+                            mma_weights(tm_now + 256u + 128u * g, tm_now + 128u * g + kStepKeys * h + 8u * k, vd + 2u * DP * k, idesc_o, k != 0 ? 1u : later);
+                        umma_commit(&pv_done[g][h]);
+                    }
+                    if (g == 1 && h == 1) umma_commit(&v_empty[st]);
+                    if (more) scores(half_, Next{}, step_, t + 2);
+                }
+                __syncwarp();
             };
-            scores(First{}, First{}, 0);
-            if (ok) scores(Second{}, First{}, 0);
+            using Zero = std::integral_constant<uint32_t, 0>;
+            using One = std::integral_constant<uint32_t, 1>;
+            const auto tile = [&](auto slot, int t) {
+                turn(Zero{}, slot, Zero{}, t);
+                turn(One{}, slot, Zero{}, t);
+                turn(Zero{}, slot, One{}, t + 1);
+                turn(One{}, slot, One{}, t + 1);
+            };
+            if (un > 0 && !pair_wait(&k_full[0], 0u, polls)) ok = false;
+            if (ok && un > 0) {
+                fence_after();
+                const auto begin = [&](auto half_, auto step_) {
+                    constexpr uint32_t g = decltype(half_)::value, h = decltype(step_)::value;
+                    tm_now = same(tmem);
+                    q_now = same(q_at + g * (kHalfRows * DP * 2));
+                    k_now = same(k_at + h * (T::kSide / 2));
+                    if (h < (uint32_t)un && elect_one_sync()) scores(half_, Zero{}, step_, (int)h);
+                    __syncwarp();
+                };
+                begin(Zero{}, Zero{});
+                begin(One{}, Zero{});
+                begin(Zero{}, One{});
+                begin(One{}, One{});
+            }
 #pragma unroll 1
-            for (int i = 0; ok && i < un; i += kStages) {
-                turn(First{}, i);
-                turn(Second{}, i + 1);
+            for (int t = 0; ok && t < un; t += 2 * kStages) {
+                tile(Zero{}, t);
+                tile(One{}, t + 2);
                 if constexpr (kStages == 4) {
-                    turn(std::integral_constant<uint32_t, 2>{}, i + 2);
-                    turn(std::integral_constant<uint32_t, 3>{}, i + 3);
+                    tile(std::integral_constant<uint32_t, 2>{}, t + 4);
+                    tile(std::integral_constant<uint32_t, 3>{}, t + 6);
                 }
             }
             mmas_ended<false>(&done);
