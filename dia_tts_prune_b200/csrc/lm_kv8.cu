@@ -344,7 +344,7 @@ __global__ void __launch_bounds__(kFewThreads, Few<DP, TERMS>::kCtas) kv8_attent
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, group = a.heads / c.kv_heads;
-    zero_rows_of_none(s, a, c.dim);
+    zero_rows_of_none(s, a, c.dim, (long long)blockIdx.x * kFewThreads + threadIdx.x, (long long)gridDim.x * kFewThreads);
     Place at = find_place(s, a, c.kv_heads, group, c.page_shift, gridDim.x, blockIdx.x);
     if (at.seq < 0) return;
     long long unit = at.per * blockIdx.x;

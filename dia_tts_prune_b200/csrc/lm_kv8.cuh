@@ -88,12 +88,11 @@ __device__ __forceinline__ float row_factor(const Kv8Attention& a, int head, flo
 }
 __device__ __forceinline__ float lower_to(float from, float to) { return from == -INFINITY ? 0.f : exp2_fast(from - to); }      // 2^(from - to)
 
-
-// rows that no sequence has (all CTAs of a kernel)
-__device__ __forceinline__ void zero_rows_of_none(const Kv8Step& s, const Kv8Attention& a, int dim) {
+// rows that no sequence has (all of `threads`, who know which they are)
+__device__ __forceinline__ void zero_rows_of_none(const Kv8Step& s, const Kv8Attention& a, int dim, long long thread, long long threads) {
     if (!s.first) return;
     const int begin = min(max(s.first[0], 0), s.rows), end = min(max(s.first[s.sequences], begin), s.rows), width = a.heads * dim;
-    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < (long long)(begin + s.rows - end) * width; i += (long long)gridDim.x * blockDim.x)
+    for (long long i = thread; i < (long long)(begin + s.rows - end) * width; i += threads)
         store_out(a, i < (long long)begin * width ? i : i + (long long)(end - begin) * width, 0.f);
 }
 

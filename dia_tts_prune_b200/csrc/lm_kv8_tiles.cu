@@ -4,8 +4,8 @@
 //   warps 0-3, 4-7   one thread per row, 128 rows each: 64 scores at a time from tensor memory, softmax weights back to where they lay.  A half has two places for scores, so
 //                    that the next ones are there when it has weighed these
 //   warps 8-15       codes to fp16 operands, from shared memory to shared memory, 16 tokens each
-//   warp 16          one elected lane issues tcgen05.mma: S = Q K^T (M = 128, N = 64), and O += P V with P as the operand in tensor memory
-//   warp 17          looks up pages and scales, and fetches the next tile's codes by bulk copies
+//   warps 16, 17     one elected lane each issues tcgen05.mma for a half: S = Q K^T (M = 128, N = 64), and O += P V with P as the operand in tensor memory
+//   warp 18          looks up pages and scales, and fetches the next tile's codes by bulk copies
 //
 // Numbers.  t = scale log2(e) q . key + e - E in powers of two, e the exponent of the page's values and E the largest of the CTA's pages; P = 2^(t - R + 7) in fp16, with R the
 // row's reference: about its largest t so far, raised (and O and the sum with it) only when one of 64 scores lies more than 8 above it, so P is at most 2^15.  That the page's value
@@ -69,76 +69,60 @@ __device__ __forceinline__ Sequence sequence_at(const Kv8Step& s, const Kv8Atten
     return q;
 }
 struct Work {
-    int seq, head, tile, chunk, chunks, first_cta, length;    // seq -1: nothing
+    int seq, head, tile, chunk, chunks, first_cta, length;    // seq -1: nothing; length: of a chunk in tiles of keys
 };
-template <int THREADS>
-__device__ __forceinline__ long long scan(long long mine, long long* sums, long long& total) {      // sum of the threads before this one
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    long long upto = mine;
+constexpr int kWhole = 0x7fffffff;
+// One warp.  JOIN: `index` counts items, and only where there are chunks to join; else it counts CTAs
+template <bool JOIN>
+__device__ __forceinline__ Work find_work(const Kv8Cache& c, const Kv8Step& s, const Kv8Attention& a, int group, int index) {
+    const int lane = threadIdx.x & 31, each = (s.sequences + 31) / 32, i0 = lane * each, i1 = min(i0 + each, s.sequences);
+    const auto before = [&](int v) {                          // sums of the lanes before this one, and of all
+        int upto = v;
 #pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-        const long long o = __shfl_up_sync(0xffffffffu, upto, d);
-        if (lane >= d) upto += o;
-    }
-    if (lane == 31) sums[warp] = upto;
-    __syncthreads();
-    total = 0;
-#pragma unroll
-    for (int w = 0; w < THREADS / 32; ++w) {
-        if (w < warp) upto += sums[w];
-        total += sums[w];
-    }
-    __syncthreads();
-    return upto - mine;
-}
-// JOIN: `index` counts items, and only where there are chunks to join; else it counts CTAs
-template <int THREADS, bool JOIN>
-__device__ __forceinline__ Work find_work(const Kv8Cache& c, const Kv8Step& s, const Kv8Attention& a, int group, long long index) {
-    __shared__ long long sums[THREADS / 32];
-    __shared__ int longest;
-    __shared__ Work found;
-    if (threadIdx.x == 0) {
-        longest = 0;
-        found.seq = -1;
-    }
-    __syncthreads();
-    const int each = (s.sequences + THREADS - 1) / THREADS, i0 = threadIdx.x * each, i1 = min(i0 + each, s.sequences);
-    long long items = 0, total_items, ctas = 0, total;
-    int most = 0;
-    const Sequence mine = sequence_at(s, a, min(i0, s.sequences - 1), group, c.page_shift);       // (a thread's only one, mostly)
+        for (int d = 1; d < 32; d <<= 1) {
+            const int o = __shfl_up_sync(0xffffffffu, upto, d);
+            if (lane >= d) upto += o;
+        }
+        return make_int2(upto - v, __shfl_sync(0xffffffffu, upto, 31));
+    };
+    const Sequence mine = sequence_at(s, a, min(i0, s.sequences - 1), group, c.page_shift);       // (a lane's only one, mostly)
     const auto at = [&](int i) { return i == i0 ? mine : sequence_at(s, a, i, group, c.page_shift); };
+    int items = 0, most = 0, ctas = 0;
     for (int i = i0; i < i1; ++i) {
         const Sequence q = at(i);
-        items += (long long)q.tiles * c.kv_heads;
+        items += q.tiles * c.kv_heads;
         if (q.tiles) most = max(most, q.high - q.low);
     }
-    if (most) atomicMax(&longest, most);
-    const long long items_before = scan<THREADS>(items, sums, total_items);
-    if (total_items == 0 || (JOIN && total_items >= kSms)) return found;
-    const int length = total_items >= kSms ? 0x7fffffff : max(kMinChunk, (longest + kSms / (int)total_items - 1) / (kSms / (int)total_items));
-    const auto chunks_of = [&](const Sequence& q) { return length == 0x7fffffff ? 1 : max(1, (q.high - q.low + length - 1) / length); };
+    const int2 of_items = before(items);
+    const int longest = (int)__reduce_max_sync(0xffffffffu, (unsigned)most);
+    Work work{-1, 0, 0, 0, 1, 0, kWhole};
+    if (of_items.y == 0 || (JOIN && of_items.y >= kSms)) return work;
+    const int share = of_items.y >= kSms ? 0 : kSms / of_items.y;
+    const int length = share == 0 ? kWhole : max(kMinChunk, (longest + share - 1) / share);
+    const auto chunks_of = [&](const Sequence& q) { return length == kWhole ? 1 : max(1, (q.high - q.low + length - 1) / length); };
     for (int i = i0; i < i1; ++i) {
         const Sequence q = at(i);
-        ctas += (long long)q.tiles * c.kv_heads * chunks_of(q);
+        ctas += q.tiles * c.kv_heads * chunks_of(q);
     }
-    const long long before = scan<THREADS>(ctas, sums, total);
-    long long base = JOIN ? items_before : before, cta = before;
-    if (index >= base && index < base + (JOIN ? items : ctas)) {
+    int cta = before(ctas).x, base = JOIN ? of_items.x : cta;
+    const bool here = index >= base && index < base + (JOIN ? items : ctas);
+    if (here) {
         for (int i = i0;; ++i) {
             const Sequence q = at(i);
-            const int chunks = chunks_of(q);
-            const long long own = (long long)q.tiles * c.kv_heads, units = JOIN ? own : own * chunks;
+            const int chunks = chunks_of(q), own = q.tiles * c.kv_heads, units = JOIN ? own : own * chunks;
             if (index < base + units) {
-                const long long local = index - base, item = JOIN ? local : local / chunks;
-                found = {i, (int)(item % c.kv_heads), q.tiles - 1 - (int)(item / c.kv_heads), JOIN ? 0 : (int)(local % chunks), chunks, (int)(cta + item * chunks), length};
+                const unsigned local = index - base, item = JOIN ? local : local / (unsigned)chunks;
+                work = {i, (int)(item % (unsigned)c.kv_heads), q.tiles - 1 - (int)(item / (unsigned)c.kv_heads), JOIN ? 0 : (int)(local - item * chunks), chunks, cta + (int)item * chunks, length};
                 break;
             }
             base += units;
             cta += own * chunks;
         }
     }
-    __syncthreads();
-    return found;
+    const unsigned who = __ballot_sync(0xffffffffu, here);
+    const int from = who ? __ffs(who) - 1 : 0;
+    const auto told = [&](int v) { return __shfl_sync(0xffffffffu, v, from); };
+    return {told(work.seq), told(work.head), told(work.tile), told(work.chunk), told(work.chunks), told(work.first_cta), told(work.length)};
 }
 
 // ---- tensor memory and shared memory -------------------------------------------------------------------------------------------------------
@@ -189,23 +173,28 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cac
     uint8_t* const k_ring = smem + T::kQ;
     uint8_t* const v_ring = k_ring + kStages * T::kSide;
     uint8_t* const codes = v_ring + kStages * T::kSide;       // [keys, values]
-    __shared__ uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], m_full[kAhead], m_empty[kAhead], c_full[2], c_empty[2], s_full[2][2], p_ready[2][2], pv_done[2][2], done;
+    __shared__ uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], m_full[kAhead], m_empty[kAhead], c_full[2], c_empty[2], s_full[2][2], p_ready[2][2], pv_done[2][2], done[2];
     __shared__ float4 blocks[kAhead][kBlocks];                // (key scale, e - E, 2^(E - e), page) of 16 tokens
     __shared__ uint3 which[kAhead];                           // of a tile's blocks: those that are there, whose values are taken as zeros, that stand for numbers
     __shared__ uint32_t tmem_slot;
     __shared__ int largest;                                   // exponent of the values' pages
+    __shared__ uint64_t q_ready;
+    __shared__ Work found;
+    __shared__ Sequence found_rows;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = a.heads / c.kv_heads;
-    if (alone) zero_rows_of_none(s, a, c.dim);
-    const Work work = find_work<kThreads, false>(c, s, a, group, blockIdx.x);
-    if (work.seq < 0) return;
-    const Sequence q = sequence_at(s, a, work.seq, group, c.page_shift);
-    if (threadIdx.x == 0) {
+    if (warp == 0) {
+        const Work work = find_work<false>(c, s, a, group, blockIdx.x);
+        if (lane == 0) {
+            found = work;
+            if (work.seq >= 0) found_rows = sequence_at(s, a, work.seq, group, c.page_shift);
+        }
+    } else if (threadIdx.x == 32) {
         for (int i = 0; i < kStages; ++i) {
             mbar_init(&k_full[i], 8);
             mbar_init(&v_full[i], 8);
-            mbar_init(&k_empty[i], 1);
-            mbar_init(&v_empty[i], 1);
+            mbar_init(&k_empty[i], 2);
+            mbar_init(&v_empty[i], 2);
         }
         for (int i = 0; i < kAhead; ++i) {
             mbar_init(&m_full[i], 1);
@@ -219,30 +208,40 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cac
                 mbar_init(&p_ready[g][i], 4);
                 mbar_init(&pv_done[g][i], 1);
             }
+            mbar_init(&done[g], 1);
         }
-        mbar_init(&done, 1);
+        mbar_init(&q_ready, 8);
         largest = -1000;
         fence_mbar_init();
-    }
-    if (warp == 16) {
+    } else if (warp == 16) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&tmem_slot)));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+    } else if (warp == 19 && alone) {
+        zero_rows_of_none(s, a, c.dim, (long long)blockIdx.x * 32 + lane, (long long)gridDim.x * 32);
     }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = tmem_slot;                          // scores (and weights) of the halves 0, 128; outputs 256, 384
+    const Work work = found;
+    if (work.seq < 0) {
+        if (warp == 16) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+        return;
+    }
+    const Sequence q = found_rows;
     // tiles of keys: the first one, and how many of them the halves of the rows look at
     const int pairs = q.n * group, p0 = work.tile * kTileRows;
     const auto position = [&](int p) { return (long long)q.past + min(p, pairs - 1) / group; };
     const long long back = a.window > 0 ? a.window - 1 : (1ll << 40);
-    const int from = max(max(q.low, (int)(max(0ll, position(p0) - back) / kKeys)), work.length == 0x7fffffff ? 0 : q.low + work.chunk * work.length);
-    const int limit = work.length == 0x7fffffff ? q.high : (int)min((long long)q.high, (long long)q.low + (long long)(work.chunk + 1) * work.length);
+    const int from = max(max(q.low, (int)(max(0ll, position(p0) - back) / kKeys)), work.length == kWhole ? 0 : q.low + work.chunk * work.length);
+    const int limit = work.length == kWhole ? q.high : (int)min((long long)q.high, (long long)q.low + (long long)(work.chunk + 1) * work.length);
     const auto steps_of = [&](int g) {
         if (p0 + g * kHalfRows >= pairs || q.past < 0) return 0;
         const long long end = min((long long)limit * kKeys, position(p0 + g * kHalfRows + kHalfRows - 1) + 1) - (long long)from * kKeys;
         return (int)max(0ll, (end + kStepKeys - 1) / kStepKeys);
     };
     const int n0 = steps_of(0), n1 = steps_of(1), n = (max(n0, n1) + 1) / 2;       // steps of the halves, tiles
-    __syncthreads();                                          // (the largest exponent is set)
-    float row_scale = 0.f;
-    if (warp >= 8) {
+    const auto find_largest = [&] {                           // the largest exponent of the values' pages (all warps but the rows')
         int most = -1000;
         for (int b = threadIdx.x - 256; b < n * kBlocks; b += kThreads - 256) {
             const int page = s.page(work.seq, ((long long)from * kKeys + (long long)b * kKvBlock) >> c.page_shift, c.pages);
@@ -252,75 +251,75 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cac
         }
         most = __reduce_max_sync(0xffffffffu, most);
         if (lane == 0 && most > -1000) atomicMax(&largest, most);
-    } else {
-        // queries: a warp takes its 32 rows, eight at a time, a lane DP / 4 channels of one in pieces of eight
-        constexpr int kPieces = DP / 32;
-        const int sub = lane & 7;
-        const bool wide = c.dim % 8 == 0 && (reinterpret_cast<uintptr_t>(a.q.x) & 15) == 0 && a.q.row % 8 == 0 && a.q.head % 8 == 0;
-        uint4 w[4][kPieces];
-#pragma unroll
-        for (int r8 = 0; r8 < 4; ++r8) {
-            const int p = p0 + warp * 32 + r8 * 8 + sub, in = min(p, pairs - 1);
-            const uint16_t* const row = reinterpret_cast<const uint16_t*>(a.q.x) + (q.begin + (long long)(in / group)) * a.q.row + (long long)(work.head * group + in % group) * a.q.head;
-#pragma unroll
-            for (int j = 0; j < kPieces; ++j) {
-                const int d = 8 * ((lane >> 3) + 4 * j);
-                w[r8][j] = make_uint4(0u, 0u, 0u, 0u);
-                if (p >= pairs || d >= c.dim) continue;
-                if (wide) {
-                    w[r8][j] = *reinterpret_cast<const uint4*>(row + d);
-                } else {
-                    uint16_t y[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) y[e] = d + e < c.dim ? row[d + e] : 0;
-                    memcpy(&w[r8][j], y, 16);
-                }
-            }
-        }
-        const auto numbers = [&](uint32_t u) {
-            if (a.type == kTypeBf16) return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
-            return __half22float2(*reinterpret_cast<const __half2*>(&u));
-        };
-#pragma unroll
-        for (int r8 = 0; r8 < 4; ++r8) {
-            uint32_t most = 0;
-#pragma unroll
-            for (int j = 0; j < kPieces; ++j) {
-                const uint32_t u[4] = {w[r8][j].x, w[r8][j].y, w[r8][j].z, w[r8][j].w};
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float2 f = numbers(u[e]);
-                    most = max(most, max(__float_as_uint(f.x) & 0x7fffffffu, __float_as_uint(f.y) & 0x7fffffffu));
-                }
-            }
-            most = max(most, __shfl_xor_sync(0xffffffffu, most, 8));
-            most = max(most, __shfl_xor_sync(0xffffffffu, most, 16));
-            const uint32_t e = most == 0 ? 127u : max(most >> 23, 14u);
-            const float f = __uint_as_float((267u - e) << 23), way_back = __uint_as_float((e - 13u) << 23);       // 2^(140 - e): to below 2^14, and the way back
-            if (r8 == lane >> 3) row_scale = e == 255u ? __uint_as_float(0x7fc00000u) : way_back * (a.scale * kLog2e);      // (a thread's own row is 8 r8 + sub of its warp's)
-            uint8_t* const to = q_tile + (warp >> 2) * (kHalfRows * DP * 2) + ((warp & 3) * 4 + r8) * (DP * 16) + sub * 16;
-#pragma unroll
-            for (int j = 0; j < kPieces; ++j) {
-                uint32_t u[4] = {w[r8][j].x, w[r8][j].y, w[r8][j].z, w[r8][j].w};
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float2 y = numbers(u[i]);
-                    u[i] = e == 255u ? 0u : pack_half(y.x * f, y.y * f);
-                }
-                *reinterpret_cast<uint4*>(to + ((lane >> 3) + 4 * j) * 128) = make_uint4(u[0], u[1], u[2], u[3]);
-            }
-        }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    }
-    fence_before();
-    __syncthreads();
-    fence_after();
-    const uint32_t tmem = tmem_slot;                          // scores (and weights) of the halves 0, 128; outputs 256, 384
-    const float spread = (float)(largest == -1000 ? 0 : largest);
+        asm volatile("bar.sync 1, %0;" ::"n"(kThreads - 256) : "memory");
+    };
     bool ok = true;
 
     if (warp < 8) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+        float row_scale = 0.f;
+        {
+            // queries: a warp takes its 32 rows, eight at a time, a lane DP / 4 channels of one in pieces of eight
+            constexpr int kPieces = DP / 32;
+            const int sub = lane & 7;
+            const bool wide = c.dim % 8 == 0 && (reinterpret_cast<uintptr_t>(a.q.x) & 15) == 0 && a.q.row % 8 == 0 && a.q.head % 8 == 0;
+            uint4 w[4][kPieces];
+#pragma unroll
+            for (int r8 = 0; r8 < 4; ++r8) {
+                const int p = p0 + warp * 32 + r8 * 8 + sub, in = min(p, pairs - 1);
+                const uint16_t* const row = reinterpret_cast<const uint16_t*>(a.q.x) + (q.begin + (long long)(in / group)) * a.q.row + (long long)(work.head * group + in % group) * a.q.head;
+#pragma unroll
+                for (int j = 0; j < kPieces; ++j) {
+                    const int d = 8 * ((lane >> 3) + 4 * j);
+                    w[r8][j] = make_uint4(0u, 0u, 0u, 0u);
+                    if (p >= pairs || d >= c.dim) continue;
+                    if (wide) {
+                        w[r8][j] = *reinterpret_cast<const uint4*>(row + d);
+                    } else {
+                        uint16_t y[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) y[e] = d + e < c.dim ? row[d + e] : 0;
+                        memcpy(&w[r8][j], y, 16);
+                    }
+                }
+            }
+            const auto numbers = [&](uint32_t u) {
+                if (a.type == kTypeBf16) return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+                return __half22float2(*reinterpret_cast<const __half2*>(&u));
+            };
+#pragma unroll
+            for (int r8 = 0; r8 < 4; ++r8) {
+                uint32_t most = 0;
+#pragma unroll
+                for (int j = 0; j < kPieces; ++j) {
+                    const uint32_t u[4] = {w[r8][j].x, w[r8][j].y, w[r8][j].z, w[r8][j].w};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float2 f = numbers(u[e]);
+                        most = max(most, max(__float_as_uint(f.x) & 0x7fffffffu, __float_as_uint(f.y) & 0x7fffffffu));
+                    }
+                }
+                most = max(most, __shfl_xor_sync(0xffffffffu, most, 8));
+                most = max(most, __shfl_xor_sync(0xffffffffu, most, 16));
+                const uint32_t e = most == 0 ? 127u : max(most >> 23, 14u);
+                const float f = __uint_as_float((267u - e) << 23), way_back = __uint_as_float((e - 13u) << 23);       // 2^(140 - e): to below 2^14, and the way back
+                if (r8 == lane >> 3) row_scale = e == 255u ? __uint_as_float(0x7fc00000u) : way_back * (a.scale * kLog2e);      // (a thread's own row is 8 r8 + sub of its warp's)
+                uint8_t* const to = q_tile + (warp >> 2) * (kHalfRows * DP * 2) + ((warp & 3) * 4 + r8) * (DP * 16) + sub * 16;
+#pragma unroll
+                for (int j = 0; j < kPieces; ++j) {
+                    uint32_t u[4] = {w[r8][j].x, w[r8][j].y, w[r8][j].z, w[r8][j].w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float2 y = numbers(u[i]);
+                        u[i] = e == 255u ? 0u : pack_half(y.x * f, y.y * f);
+                    }
+                    *reinterpret_cast<uint4*>(to + ((lane >> 3) + 4 * j) * 128) = make_uint4(u[0], u[1], u[2], u[3]);
+                }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&q_ready);
+        }
         const int g = warp >> 2, count = g ? n1 : n0;
         const uint32_t lanes = (uint32_t)(warp & 3) * 32u << 16, t_scores = tmem + lanes + 128u * g, t_o = tmem + lanes + 256u + 128u * g;
         const int p = p0 + threadIdx.x;
@@ -346,16 +345,20 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cac
             tmem_columns32(t_s + 32, x[1]);
             tmem_loaded();
             if (!clear) {
+                const unsigned first = (unsigned)(lo - tok), many = (unsigned)(hi - lo);      // (what it sees in turn; nothing: hi is -1, or below lo)
+                const bool none = hi < tok || hi < lo;
 #pragma unroll
-                for (int b = 0; b < 4; ++b) {
-                    const bool block = there >> b & 1u;
-                    const uint32_t nan = numbers >> b & 1u ? 0u : 0x7fffffffu;      // (what a row sees of a page that stands for NaNs)
+                for (int e = 0; e < kStepKeys; ++e)
+                    if (none || e - first > many) x[e / 32][e % 32] = 0xff800000u;
+                if ((there & numbers & 0xfu) != 0xfu) {                              // pages that are not there, and what a row sees of pages that stand for NaNs
 #pragma unroll
-                    for (int e = 0; e < kKvBlock; ++e) {
-                        const int at = tok + 16 * b + e;
-                        uint32_t& v = x[b / 2][16 * (b & 1) + e];
-                        v = at > hi || at < lo || !block ? 0xff800000u : v | nan;
-                    }
+                    for (int b = 0; b < 4; ++b)
+#pragma unroll
+                        for (int e = 0; e < kKvBlock; ++e) {
+                            uint32_t& v = x[b / 2][16 * (b & 1) + e];
+                            if (!(there >> b & 1u)) v = 0xff800000u;
+                            else if (!(numbers >> b & 1u) && v != 0xff800000u) v = 0x7fffffffu;
+                        }
                 }
             }
             const auto score = [&](int b, int e) { return __uint_as_float(x[b / 2][16 * (b & 1) + e]); };
@@ -422,6 +425,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cac
         if (ok && count > 0 && !pair_wait(&pv_done[g][(count - 1) & 1], (uint32_t)((count - 1) >> 1) & 1u, polls)) ok = false;
         fence_after();
         // out
+        const float spread = (float)(largest == -1000 ? 0 : largest);
         float m = ref - kBits, w = m + spread + kWeightBits;
         if (l == 0.f) m = w = -INFINITY;
         const bool in = p < pairs, whole = work.chunks == 1;
@@ -472,6 +476,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cac
         }
     } else if (warp < 16) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFetchRegs));
+        find_largest();
         // ---- codes to operands: a block of every tile, eight rows of it a turn, a lane 16 channels of one.  Eight neighbouring lanes take eight rows and as many different pieces,
         // so that neither what they read nor what they write meets in a bank ----
         constexpr int kParts = DP / 64;                       // 16-byte pieces of a row that a lane takes
@@ -518,90 +523,61 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cac
         }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
-        if (warp == 16) {
+        find_largest();
+        if (warp < 18) {
             const uint32_t idesc_s = (1u << 4) | ((uint32_t)(kStepKeys >> 3) << 17) | ((uint32_t)(kHalfRows >> 4) << 24);
             const uint32_t idesc_o = (1u << 4) | (1u << 16) | ((uint32_t)(DP >> 3) << 17) | ((uint32_t)(kHalfRows >> 4) << 24);
-            // What an instruction takes is known to be the same in every lane (broadcast from one, where it is used: kept over a turn, the operands of all would take more
-            // registers than there are)
+            // A warp for each half, so that one has its turn ready while the other's is in the tensor pipe.  What an instruction takes is broadcast from one lane, where it is
+            // used, so that it is known to be the same in every lane.
             const auto same = [](uint32_t v) {
                 asm volatile("" : "+r"(v));
                 return __shfl_sync(0xffffffffu, v, 0);
             };
-            const uint32_t q_at = smem_u32(q_tile), k_at = smem_u32(k_ring), v_at = smem_u32(v_ring);
-            const int u0 = (int)same((uint32_t)n0), u1 = (int)same((uint32_t)n1), un = max(u0, u1);
-            uint32_t tm_now, q_now, k_now;
-            // A turn of half g behind its weights of step t: their values, and the scores two steps on, whose place the weights had.  A slot's last products free it.
-            const auto scores = [&](auto half_, auto slot_, auto step_, int t) {          // (one lane)
-                constexpr uint32_t g = decltype(half_)::value, st = decltype(slot_)::value, h = decltype(step_)::value;
-                const uint64_t qd = block_desc(q_now, 128u, DP * 16u), kd = block_desc(k_now, 128u, DP * 16u);
-                if (t < (g ? u1 : u0)) {
+            const int g = warp - 16, mine = (int)same((uint32_t)(g ? n1 : n0)), un = (int)same((uint32_t)max(n0, n1));
+            const uint32_t q_at = smem_u32(q_tile) + g * (kHalfRows * DP * 2), k_at = smem_u32(k_ring), v_at = smem_u32(v_ring), t_g = tmem + 128u * g;
+            // scores of step t, if it is this half's (one lane); what was the slot's last use of its tile frees it
+            const auto scores = [&](uint32_t ts, uint32_t qa, uint32_t ka, int t) {
+                const uint64_t qd = block_desc(qa, 128u, DP * 16u), kd = block_desc(ka, 128u, DP * 16u);
+                if (t < mine) {
 #pragma unroll
-                    for (uint32_t k = 0; k < kSteps; ++k) umma_bf16(tm_now + 128u * g + kStepKeys * h, qd + 16u * k, kd + 16u * k, idesc_s, k != 0);
-                    umma_commit(&s_full[g][h]);
+                    for (uint32_t k = 0; k < kSteps; ++k) umma_bf16(ts, qd + 16u * k, kd + 16u * k, idesc_s, k != 0);
+                    umma_commit(&s_full[g][t & 1]);
                 }
-                if (g == 1 && h == 1) umma_commit(&k_empty[st]);
+                if (t & 1) umma_commit(&k_empty[(t >> 1) % kStages]);
             };
-            const auto turn = [&](auto half_, auto slot_, auto step_, int t) {
-                constexpr uint32_t g = decltype(half_)::value, st = decltype(slot_)::value, h = decltype(step_)::value;
-                using Next = std::integral_constant<uint32_t, (st + 1) % kStages>;
-                const bool mine = t < (g ? u1 : u0), more = t + 2 < un;
-                if (!ok || t >= un) return;
-                if (mine && !pair_wait(&p_ready[g][h], (uint32_t)(t >> 1) & 1u, polls)) { ok = false; return; }
-                if (g == 0 && h == 0 && !pair_wait(&v_full[st], (uint32_t)((t >> 1) / kStages) & 1u, polls)) { ok = false; return; }
-                if (g == 0 && h == 0 && more && !pair_wait(&k_full[Next::value], (uint32_t)(((t >> 1) + 1) / kStages) & 1u, polls)) { ok = false; return; }
+            if (un > 0 && (!pair_wait(&q_ready, 0u, polls) || !pair_wait(&k_full[0], 0u, polls))) ok = false;
+#pragma unroll 1
+            for (int t = 0; ok && t < min(un, 2); ++t) {
                 fence_after();
-                tm_now = same(tmem);
-                q_now = same(q_at + g * (kHalfRows * DP * 2));
-                k_now = same(k_at + Next::value * T::kSide + h * (T::kSide / 2));
-                const uint32_t v_now = same(v_at + st * T::kSide + h * (T::kSide / 2)), later = t != 0;
+                const uint32_t ts = same(t_g + kStepKeys * t), qa = same(q_at), ka = same(k_at + t * (T::kSide / 2));
+                if (elect_one_sync()) scores(ts, qa, ka, t);
+                __syncwarp();
+            }
+            // A turn behind the weights of step t: their values, and the scores two steps on, whose place the weights had
+#pragma unroll 1
+            for (int t = 0; ok && t < un; ++t) {
+                const int i = t >> 1, st = i % kStages, h = t & 1, next = (i + 1) % kStages;
+                const bool more = t + 2 < un;
+                if (h == 0 && !pair_wait(&v_full[st], (uint32_t)(i / kStages) & 1u, polls)) { ok = false; break; }
+                if (h == 0 && more && !pair_wait(&k_full[next], (uint32_t)((i + 1) / kStages) & 1u, polls)) { ok = false; break; }
+                if (t < mine && !pair_wait(&p_ready[g][h], (uint32_t)i & 1u, polls)) { ok = false; break; }
+                fence_after();
+                const uint32_t ts = same(t_g + kStepKeys * h), to = same(t_g + 256u), va = same(v_at + st * T::kSide + h * (T::kSide / 2)), qa = same(q_at),
+                               ka = same(k_at + next * T::kSide + h * (T::kSide / 2)), later = t != 0;
                 if (elect_one_sync()) {
-                    if (mine) {
-                        const uint64_t vd = block_desc(v_now, DP * 16u, 128u);
+                    if (t < mine) {
+                        const uint64_t vd = block_desc(va, DP * 16u, 128u);
 #pragma unroll
-                        for (uint32_t k = 0; k < kStepKeys / 16; ++k)
-                            mma_weights(tm_now + 256u + 128u * g, tm_now + 128u * g + kStepKeys * h + 8u * k, vd + 2u * DP * k, idesc_o, k != 0 ? 1u : later);
+                        for (uint32_t k = 0; k < kStepKeys / 16; ++k) mma_weights(to, ts + 8u * k, vd + 2u * DP * k, idesc_o, k != 0 ? 1u : later);
                         umma_commit(&pv_done[g][h]);
                     }
-                    if (g == 1 && h == 1) umma_commit(&v_empty[st]);
-                    if (more) scores(half_, Next{}, step_, t + 2);
+                    if (h == 1) umma_commit(&v_empty[st]);
+                    if (more) scores(ts, qa, ka, t + 2);
                 }
                 __syncwarp();
-            };
-            using Zero = std::integral_constant<uint32_t, 0>;
-            using One = std::integral_constant<uint32_t, 1>;
-            const auto tile = [&](auto slot, int t) {
-                turn(Zero{}, slot, Zero{}, t);
-                turn(One{}, slot, Zero{}, t);
-                turn(Zero{}, slot, One{}, t + 1);
-                turn(One{}, slot, One{}, t + 1);
-            };
-            if (un > 0 && !pair_wait(&k_full[0], 0u, polls)) ok = false;
-            if (ok && un > 0) {
-                fence_after();
-                const auto begin = [&](auto half_, auto step_) {
-                    constexpr uint32_t g = decltype(half_)::value, h = decltype(step_)::value;
-                    tm_now = same(tmem);
-                    q_now = same(q_at + g * (kHalfRows * DP * 2));
-                    k_now = same(k_at + h * (T::kSide / 2));
-                    if (h < (uint32_t)un && elect_one_sync()) scores(half_, Zero{}, step_, (int)h);
-                    __syncwarp();
-                };
-                begin(Zero{}, Zero{});
-                begin(One{}, Zero{});
-                begin(Zero{}, One{});
-                begin(One{}, One{});
             }
-#pragma unroll 1
-            for (int t = 0; ok && t < un; t += 2 * kStages) {
-                tile(Zero{}, t);
-                tile(One{}, t + 2);
-                if constexpr (kStages == 4) {
-                    tile(std::integral_constant<uint32_t, 2>{}, t + 4);
-                    tile(std::integral_constant<uint32_t, 3>{}, t + 6);
-                }
-            }
-            mmas_ended<false>(&done);
-        } else if (warp == 17) {
+            mmas_ended<false>(&done[warp - 16]);
+        } else if (warp == 18) {
             // lanes 0 .. 7 look a block up each: its scales a tile ahead, its page two
             const auto page_of = [&](int i) { return lane < kBlocks && i < n ? s.page(work.seq, (((long long)from + i) * kKeys + lane * kKvBlock) >> c.page_shift, c.pages) : -1; };
             const auto scales_of = [&](int page) {
@@ -666,7 +642,13 @@ template <int DP>
 __global__ void __launch_bounds__(kJoinThreads) kv8_attention_tiles_join_kernel(Kv8Cache c, Kv8Step s, Kv8Attention a, const float* part, const RowStats* part_stats) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int group = a.heads / c.kv_heads, lane = threadIdx.x & 31;
-    const Work work = find_work<kJoinThreads, true>(c, s, a, group, blockIdx.x);
+    __shared__ Work found;
+    if (threadIdx.x < 32) {
+        const Work work = find_work<true>(c, s, a, group, blockIdx.x);
+        if (lane == 0) found = work;
+    }
+    __syncthreads();
+    const Work work = found;
     if (work.seq < 0 || work.chunks == 1) return;
     const Sequence q = sequence_at(s, a, work.seq, group, c.page_shift);
     for (int r = blockIdx.y * (kJoinThreads / 32) + (threadIdx.x >> 5); r < kTileRows; r += kJoinCtas * (kJoinThreads / 32)) {
