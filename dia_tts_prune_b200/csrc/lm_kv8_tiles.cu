@@ -3,9 +3,9 @@
 // A CTA takes 256 (token, query head) rows that share a key head and walks their keys 128 at a time:
 //   warps 0-3, 4-7   one thread per row, 128 rows each: 64 scores at a time from tensor memory, softmax weights back to where they lay.  A half has two places for scores, so
 //                    that the next ones are there when it has weighed these
-//   warps 8-15       codes to fp16 operands, from shared memory to shared memory, 16 tokens each
+//   warps 8-15       codes to fp16 operands, from shared memory to shared memory: four warps the keys, four the values, 16 tokens of a step each
 //   warps 16, 17     one elected lane each issues tcgen05.mma for a half: S = Q K^T (M = 128, N = 64), and O += P V with P as the operand in tensor memory
-//   warp 18          looks up pages and scales, and fetches the next tile's codes by bulk copies
+//   warp 18          looks up pages and scales, and fetches the codes of the next four steps by bulk copies
 //
 // Numbers.  t = scale log2(e) q . key + e - E in powers of two, e the exponent of the page's values and E the largest of the CTA's pages; P = 2^(t - R + 7) in fp16, with R the
 // row's reference: about its largest t so far, raised (and O and the sum with it) only when one of 64 scores lies more than 8 above it, so P is at most 2^15.  That the page's value
@@ -45,9 +45,9 @@ constexpr int kAhead = 4;                                      // tiles whose pa
 
 template <int DP>
 struct Tiles {
-    static constexpr int kStages = DP == 64 ? 4 : 2, kSide = kKeys * DP * 2, kQ = kTileRows * DP * 2;
-    static constexpr int kCodes = kKeys * DP;                 // room for a tile's codes, keys or values
-    static constexpr int kSmem = kQ + kStages * 2 * kSide + 2 * kCodes;
+    static constexpr int kStages = DP == 64 ? 6 : 3, kSide = kStepKeys * DP * 2;      // operands of a step, keys or values
+    static constexpr int kDepth = 4, kCodes = kStepKeys * DP; // and its codes
+    static constexpr int kQ = kTileRows * DP * 2, kSmem = kQ + 2 * kStages * kSide + 2 * kDepth * kCodes;
 };
 
 // ---- who takes what ------------------------------------------------------------------------------------------------------------------------
@@ -125,6 +125,19 @@ __device__ __forceinline__ Work find_work(const Kv8Cache& c, const Kv8Step& s, c
     return {told(work.seq), told(work.head), told(work.tile), told(work.chunk), told(work.chunks), told(work.first_cta), told(work.length)};
 }
 
+// A place in a ring of N, and which of a barrier's phases is its use's
+template <int N>
+struct Turn {
+    int at = 0;
+    uint32_t phase = 0;
+    __device__ __forceinline__ void next() {
+        if (++at == N) {
+            at = 0;
+            phase ^= 1u;
+        }
+    }
+};
+
 // ---- tensor memory and shared memory -------------------------------------------------------------------------------------------------------
 
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -167,13 +180,13 @@ __device__ __forceinline__ void mma_weights(uint32_t d, uint32_t a, uint64_t b, 
 template <int DP, int FORMAT>
 __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cache c, Kv8Step s, Kv8Attention a, int alone, float* part, RowStats* part_stats, int* ran_out, unsigned polls) {
     using T = Tiles<DP>;
-    constexpr int kStages = T::kStages, kSteps = DP / 16;
+    constexpr int kStages = T::kStages, kDepth = T::kDepth, kSteps = DP / 16;
     extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t* const q_tile = smem;                             // [half]
     uint8_t* const k_ring = smem + T::kQ;
     uint8_t* const v_ring = k_ring + kStages * T::kSide;
-    uint8_t* const codes = v_ring + kStages * T::kSide;       // [keys, values]
-    __shared__ uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], m_full[kAhead], m_empty[kAhead], c_full[2], c_empty[2], s_full[2][2], p_ready[2][2], pv_done[2][2], done[2];
+    uint8_t* const codes = v_ring + kStages * T::kSide;       // [keys, values][kDepth]
+    __shared__ uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], m_full[kAhead], m_empty[kAhead], c_full[2][kDepth], c_empty[2][kDepth], s_full[2][2], p_ready[2][2], pv_done[2][2], done[2];
     __shared__ float4 blocks[kAhead][kBlocks];                // (key scale, e - E, 2^(E - e), page) of 16 tokens
     __shared__ uint3 which[kAhead];                           // of a tile's blocks: those that are there, whose values are taken as zeros, that stand for numbers
     __shared__ uint32_t tmem_slot;
@@ -191,8 +204,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cac
         }
     } else if (threadIdx.x == 32) {
         for (int i = 0; i < kStages; ++i) {
-            mbar_init(&k_full[i], 8);
-            mbar_init(&v_full[i], 8);
+            mbar_init(&k_full[i], 4);
+            mbar_init(&v_full[i], 4);
             mbar_init(&k_empty[i], 2);
             mbar_init(&v_empty[i], 2);
         }
@@ -201,8 +214,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cac
             mbar_init(&m_empty[i], 16);
         }
         for (int g = 0; g < 2; ++g) {
-            mbar_init(&c_full[g], 1);
-            mbar_init(&c_empty[g], 8);
+            for (int i = 0; i < kDepth; ++i) {
+                mbar_init(&c_full[g][i], 1);
+                mbar_init(&c_empty[g][i], 4);
+            }
             for (int i = 0; i < 2; ++i) {
                 mbar_init(&s_full[g][i], 1);
                 mbar_init(&p_ready[g][i], 4);
@@ -240,7 +255,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cac
         const long long end = min((long long)limit * kKeys, position(p0 + g * kHalfRows + kHalfRows - 1) + 1) - (long long)from * kKeys;
         return (int)max(0ll, (end + kStepKeys - 1) / kStepKeys);
     };
-    const int n0 = steps_of(0), n1 = steps_of(1), n = (max(n0, n1) + 1) / 2;       // steps of the halves, tiles
+    const int n0 = steps_of(0), n1 = steps_of(1), steps = max(n0, n1), n = (steps + 1) / 2;      // of the halves, and tiles
     const auto find_largest = [&] {                           // the largest exponent of the values' pages (all warps but the rows')
         int most = -1000;
         for (int b = threadIdx.x - 256; b < n * kBlocks; b += kThreads - 256) {
@@ -477,10 +492,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cac
     } else if (warp < 16) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFetchRegs));
         find_largest();
-        // ---- codes to operands: a block of every tile, eight rows of it a turn, a lane 16 channels of one.  Eight neighbouring lanes take eight rows and as many different pieces,
-        // so that neither what they read nor what they write meets in a bank ----
+        // ---- codes to operands: four warps the keys, four the values, a block of every step each, eight rows of it a turn, a lane 16 channels of one.  Eight neighbouring lanes
+        // take eight rows and as many different pieces, so that neither what they read nor what they write meets in a bank ----
         constexpr int kParts = DP / 64;                       // 16-byte pieces of a row that a lane takes
-        const int block = warp - 8, sub = lane & 7;
+        const int side = (warp - 8) >> 2, block = warp & 3, sub = lane & 7;
+        uint64_t* const full = side ? v_full : k_full;
+        uint64_t* const empty = side ? v_empty : k_empty;
+        uint8_t* const ring = side ? v_ring : k_ring;
+        const uint8_t* const from_codes = codes + side * kDepth * T::kCodes;
         const auto lay = [&](const uint8_t* from, uint8_t* to, bool zeros) {
 #pragma unroll
             for (int r8 = 0; r8 < 2; ++r8)
@@ -501,24 +520,18 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cac
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
         };
+        Turn<kStages> out;
+        Turn<kDepth> in;
 #pragma unroll 1
-        for (int i = 0; i < n; ++i) {
-            const int st = i % kStages;
-            const uint32_t use = (uint32_t)(i / kStages);
-            if (!pair_wait(&c_full[0], i & 1, polls) || (i >= kStages && !pair_wait(&k_empty[st], (use + 1) & 1, polls))) { ok = false; break; }
-            const uint3 of = which[i % kAhead];
-            const bool there = of.x >> block & 1u, zeros = !there || (of.y >> block & 1u);
-            lay(codes, k_ring + st * T::kSide, !there);
+        for (int t = 0; t < steps; ++t, out.next(), in.next()) {
+            if (!pair_wait(&c_full[side][in.at], in.phase, polls) || (t >= kStages && !pair_wait(&empty[out.at], out.phase ^ 1u, polls))) { ok = false; break; }
+            const int slot = (t >> 1) % kAhead, bit = 4 * (t & 1) + block;
+            const uint3 of = which[slot];
+            lay(from_codes + in.at * T::kCodes, ring + out.at * T::kSide, !(of.x >> bit & 1u) || (side && (of.y >> bit & 1u)));
             if (lane == 0) {
-                mbar_arrive(&k_full[st]);
-                mbar_arrive(&c_empty[0]);
-            }
-            if (!pair_wait(&c_full[1], i & 1, polls) || (i >= kStages && !pair_wait(&v_empty[st], (use + 1) & 1, polls))) { ok = false; break; }
-            lay(codes + T::kCodes, v_ring + st * T::kSide, zeros);
-            if (lane == 0) {
-                mbar_arrive(&v_full[st]);
-                mbar_arrive(&c_empty[1]);
-                mbar_arrive(&m_empty[i % kAhead]);
+                mbar_arrive(&full[out.at]);
+                mbar_arrive(&c_empty[side][in.at]);
+                if ((t & 1) || t + 1 == steps) mbar_arrive(&m_empty[slot]);
             }
         }
     } else {
@@ -533,37 +546,41 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cac
                 asm volatile("" : "+r"(v));
                 return __shfl_sync(0xffffffffu, v, 0);
             };
-            const int g = warp - 16, mine = (int)same((uint32_t)(g ? n1 : n0)), un = (int)same((uint32_t)max(n0, n1));
-            const uint32_t q_at = smem_u32(q_tile) + g * (kHalfRows * DP * 2), k_at = smem_u32(k_ring), v_at = smem_u32(v_ring), t_g = tmem + 128u * g;
-            // scores of step t, if it is this half's (one lane); what was the slot's last use of its tile frees it
-            const auto scores = [&](uint32_t ts, uint32_t qa, uint32_t ka, int t) {
-                const uint64_t qd = block_desc(qa, 128u, DP * 16u), kd = block_desc(ka, 128u, DP * 16u);
+            const int g = warp - 16, mine = (int)same((uint32_t)(g ? n1 : n0)), un = (int)same((uint32_t)steps);
+            const uint32_t q_at = smem_u32(q_tile) + g * (kHalfRows * DP * 2), t_g = tmem + 128u * g;
+            Turn<kStages> keys, values;
+            // The scores of step t, if it is this half's; the slot is free behind them
+            const auto scores = [&](uint32_t ts, uint32_t qa, uint32_t ka, int t) {       // (one lane)
                 if (t < mine) {
+                    const uint64_t qd = block_desc(qa, 128u, DP * 16u), kd = block_desc(ka, 128u, DP * 16u);
 #pragma unroll
                     for (uint32_t k = 0; k < kSteps; ++k) umma_bf16(ts, qd + 16u * k, kd + 16u * k, idesc_s, k != 0);
                     umma_commit(&s_full[g][t & 1]);
                 }
-                if (t & 1) umma_commit(&k_empty[(t >> 1) % kStages]);
+                umma_commit(&k_empty[keys.at]);
             };
-            if (un > 0 && (!pair_wait(&q_ready, 0u, polls) || !pair_wait(&k_full[0], 0u, polls))) ok = false;
+            if (un > 0 && !pair_wait(&q_ready, 0u, polls)) ok = false;
 #pragma unroll 1
-            for (int t = 0; ok && t < min(un, 2); ++t) {
+            for (int t = 0; ok && t < min(un, 2); ++t, keys.next()) {
+                if (!pair_wait(&k_full[keys.at], keys.phase, polls)) { ok = false; break; }
                 fence_after();
-                const uint32_t ts = same(t_g + kStepKeys * t), qa = same(q_at), ka = same(k_at + t * (T::kSide / 2));
+                const uint32_t ts = same(t_g + kStepKeys * t), qa = same(q_at), ka = same(smem_u32(k_ring + keys.at * T::kSide));
                 if (elect_one_sync()) scores(ts, qa, ka, t);
                 __syncwarp();
             }
             // A turn behind the weights of step t: their values, and the scores two steps on, whose place the weights had
 #pragma unroll 1
-            for (int t = 0; ok && t < un; ++t) {
-                const int i = t >> 1, st = i % kStages, h = t & 1, next = (i + 1) % kStages;
+            for (int t = 0; ok && t < un; ++t, values.next()) {
+                const int h = t & 1;
                 const bool more = t + 2 < un;
-                if (h == 0 && !pair_wait(&v_full[st], (uint32_t)(i / kStages) & 1u, polls)) { ok = false; break; }
-                if (h == 0 && more && !pair_wait(&k_full[next], (uint32_t)((i + 1) / kStages) & 1u, polls)) { ok = false; break; }
-                if (t < mine && !pair_wait(&p_ready[g][h], (uint32_t)i & 1u, polls)) { ok = false; break; }
+                if (!pair_wait(&v_full[values.at], values.phase, polls) || (more && !pair_wait(&k_full[keys.at], keys.phase, polls)) ||
+                    (t < mine && !pair_wait(&p_ready[g][h], (uint32_t)(t >> 1) & 1u, polls))) {
+                    ok = false;
+                    break;
+                }
                 fence_after();
-                const uint32_t ts = same(t_g + kStepKeys * h), to = same(t_g + 256u), va = same(v_at + st * T::kSide + h * (T::kSide / 2)), qa = same(q_at),
-                               ka = same(k_at + next * T::kSide + h * (T::kSide / 2)), later = t != 0;
+                const uint32_t ts = same(t_g + kStepKeys * h), to = same(t_g + 256u), va = same(smem_u32(v_ring + values.at * T::kSide)), qa = same(q_at),
+                               ka = same(smem_u32(k_ring + keys.at * T::kSide)), later = t != 0;
                 if (elect_one_sync()) {
                     if (t < mine) {
                         const uint64_t vd = block_desc(va, DP * 16u, 128u);
@@ -571,10 +588,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cac
                         for (uint32_t k = 0; k < kStepKeys / 16; ++k) mma_weights(to, ts + 8u * k, vd + 2u * DP * k, idesc_o, k != 0 ? 1u : later);
                         umma_commit(&pv_done[g][h]);
                     }
-                    if (h == 1) umma_commit(&v_empty[st]);
+                    umma_commit(&v_empty[values.at]);
                     if (more) scores(ts, qa, ka, t + 2);
                 }
                 __syncwarp();
+                if (more) keys.next();
             }
             mmas_ended<false>(&done[warp - 16]);
         } else if (warp == 18) {
@@ -585,7 +603,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cac
                 return page >= 0 ? make_float2(c.key_scales[at], c.value_scales[at]) : make_float2(0.f, 0.f);
             };
             int page = page_of(0), page_next = page_of(1);
-            unsigned issued = 0;                              // of the copies, keys and values in turn
+            unsigned issued[2] = {0, 0};                      // steps whose copies are on their way, keys and values
+            Turn<kDepth> to;
             float2 scales = scales_of(page);
 #pragma unroll 1
             for (int i = 0; i < n; ++i) {
@@ -604,22 +623,24 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cac
                 if (lane == 0) which[slot] = make_uint3(there & 0xffu, zeros & 0xffu, numbers & 0xffu);
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&m_full[slot]);
-                // the tile's codes, a copy per block, as soon as the last ones have been read
+                // the codes of its steps, a copy per block, as soon as what lay there has been read
                 const uint32_t bytes = (uint32_t)(kKvBlock * c.stride);
                 const size_t at = ((((size_t)max(page_now, 0) * c.kv_heads + work.head) << c.page_shift) + (size_t)((((long long)from + i) * kKeys + lane * kKvBlock) & ((1 << c.page_shift) - 1))) * c.stride;
-                for (int side = 0; ok && side < 2; ++side) {
-                    if (i > 0 && !pair_wait(&c_empty[side], (i + 1) & 1, polls)) { ok = false; break; }
-                    if (lane == 0) mbar_arrive_expect_tx(&c_full[side], bytes * __popc(there & 0xffu));
-                    __syncwarp();
-                    if (lane < kBlocks && page_now >= 0) bulk_g2s(codes + side * T::kCodes + lane * bytes, (side ? c.values : c.keys) + at, bytes, &c_full[side]);
-                    issued = 2 * i + side + 1;
+                for (int t = 2 * i; ok && t < min(2 * i + 2, steps); ++t, to.next()) {
+                    for (int side = 0; side < 2; ++side) {
+                        if (t >= kDepth && !pair_wait(&c_empty[side][to.at], to.phase ^ 1u, polls)) { ok = false; break; }
+                        if (lane == 0) mbar_arrive_expect_tx(&c_full[side][to.at], bytes * __popc(there >> (4 * (t & 1)) & 0xfu));
+                        __syncwarp();
+                        if (lane >> 2 == (t & 1) && page_now >= 0)
+                            bulk_g2s(codes + (side * kDepth + to.at) * T::kCodes + (lane & 3) * bytes, (side ? c.values : c.keys) + at, bytes, &c_full[side][to.at]);
+                        issued[side] = t + 1;
+                    }
                 }
                 if (!ok) break;
             }
-            // (copies in flight where a wait ran out)
-            if (lane == 0 && !ok) {
-                if (issued > 0) (void)lane_wait(&c_full[0], ((issued - 1) >> 1) & 1u, kDrainPolls);
-                if (issued > 1) (void)lane_wait(&c_full[1], ((issued - 2) >> 1) & 1u, kDrainPolls);
+            if (!ok && lane == 0) {                           // (nothing arrives behind the kernel)
+                copies_landed(c_full[0], kDepth, issued[0]);
+                copies_landed(c_full[1], kDepth, issued[1]);
             }
         }
     }
