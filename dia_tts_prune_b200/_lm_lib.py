@@ -75,10 +75,6 @@ class Kv8(C.Structure):
     _fields_ = [("keys", _vp), ("values", _vp), ("key_scales", _vp), ("value_scales", _vp), ("pages", _i), ("kv_heads", _i), ("page_size", _i), ("dim", _i), ("format", _i)]
 
 
-class Kv8Step(C.Structure):
-    _fields_ = [("table", _vp), ("table_ld", C.c_int64), ("past", _vp), ("first", _vp), ("max_pages", _i), ("n_seq", _i), ("rows", _i)]
-
-
 _ci = C.c_int
 _cf = C.c_float
 _SIGNATURES = {
@@ -115,7 +111,7 @@ _SIGNATURES = {
                                    _vp]),
     "lm_b200_op_kv8_append": (_ci, [_vp, _vp, _vp, C.c_int64, C.c_int64, _vp, C.c_int64, C.c_int64, _ci, _vp]),
     "lm_b200_op_kv8_read": (_ci, [_vp, _vp, _vp, _vp, _ci, _vp]),
-    "lm_b200_op_kv8_attention_work_bytes": (C.c_size_t, [_vp, _vp, _ci, _ci]),
+    "lm_b200_op_kv8_attention_work_bytes": (C.c_size_t, [_ci, _ci, _ci, _ci, _ci]),
     "lm_b200_op_kv8_attention": (_ci, [_vp, _vp, _vp, C.c_int64, C.c_int64, _ci, _ci, _cf, _ci, _vp, _vp, _vp, C.c_size_t, _vp]),
     "lm_b200_argmax_rows": (_ci, [_vp, _ci, _ci, _vp, _vp]),
 }

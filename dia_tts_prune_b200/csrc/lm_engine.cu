@@ -162,8 +162,8 @@ bool kv8_step(lm::Kv8Step& s, const lm_b200_kv8_step* p) {
     s = lm::Kv8Step{p->table, p->table_ld, p->max_pages, p->past, p->first, p->n_seq, p->rows};
     return true;
 }
-bool kv8_heads(const lm::Kv8Cache& c, const lm::Kv8Step& s, int heads) {
-    return heads > 0 && heads % c.kv_heads == 0 && heads <= lm::kKvMostHeads && s.rows <= kMostRows / heads;        // (a tile counts rows times heads in 32 bits)
+bool kv8_heads(int kv_heads, int rows, int heads) {
+    return kv_heads > 0 && heads > 0 && heads % kv_heads == 0 && heads <= lm::kKvMostHeads && rows > 0 && rows <= kMostRows / heads;        // (a tile counts rows times heads in 32 bits)
 }
 inline lm::NormW N(const lm_b200_norm& n) { return lm::NormW{n.w, n.b, n.alpha}; }
 
@@ -1836,10 +1836,8 @@ int lm_b200_op_loss_grad(const void* h, int64_t ldh, const void* W, int64_t ldw,
     return LM_B200_OK;
 }
 
-size_t lm_b200_op_kv8_attention_work_bytes(const lm_b200_kv8* cache, const lm_b200_kv8_step* step, int heads, int type) {
-    lm::Kv8Cache c;
-    lm::Kv8Step s;
-    return kv8_cache(c, cache) && kv8_step(s, step) && kv8_heads(c, s, heads) && known_type(type) ? lm::kv8_attention_work_bytes(c, s, heads, type) : 0;
+size_t lm_b200_op_kv8_attention_work_bytes(int kv_heads, int dim, int rows, int heads, int type) {
+    return kv8_heads(kv_heads, rows, heads) && dim > 0 && dim <= lm::kKvMostDim && known_type(type) ? lm::kv8_attention_work_bytes(kv_heads, dim, rows, heads, type) : 0;
 }
 
 int lm_b200_op_kv8_append(const lm_b200_kv8* cache, const lm_b200_kv8_step* step, const void* k, int64_t k_row, int64_t k_head, const void* v, int64_t v_row, int64_t v_head, int type,
@@ -1863,8 +1861,8 @@ int lm_b200_op_kv8_attention(const lm_b200_kv8* cache, const lm_b200_kv8_step* s
                              const float* sinks, void* out, void* work, size_t work_bytes, void* stream) {
     lm::Kv8Cache c;
     lm::Kv8Step s;
-    if (!kv8_cache(c, cache) || !kv8_step(s, step) || !kv8_heads(c, s, heads) || !q || q_row < 0 || q_head < 0 || !known_type(type) || !loss_scale(scale) || window < 0 || !out || !work ||
-        !aligned(work, 256) || work_bytes < lm::kv8_attention_work_bytes(c, s, heads, type))
+    if (!kv8_cache(c, cache) || !kv8_step(s, step) || !kv8_heads(c.kv_heads, s.rows, heads) || !q || q_row < 0 || q_head < 0 || !known_type(type) || !loss_scale(scale) || window < 0 || !out || !work ||
+        !aligned(work, 256) || work_bytes < lm::kv8_attention_work_bytes(c.kv_heads, c.dim, s.rows, heads, type))
         return LM_B200_EINVAL;
     LCK(lm::launch_kv8_attention(c, s, lm::Kv8Attention{lm::Kv8Rows{q, q_row, q_head}, out, heads, type, scale, window, sinks, 0}, work, S(stream)));
     return LM_B200_OK;

@@ -232,36 +232,50 @@ __global__ void __launch_bounds__(kReadThreads) kv8_read_kernel(Kv8Cache c, Kv8S
 // ---- attention of few rows -----------------------------------------------------------------------------------------------------------------
 // x = scale log2(e) q . key in powers of two, p = 2^(x - max x), o = sum p value / (sum p + 2^(sink log2(e) - max x)).
 //
-// What bounds it is the cache's bytes.  The 16 rows of a tile are (token, query head) pairs that share a key head, so a token's codes are read once for the group; tiles of a
-// sequence lie next to one another in the order of the work.  Work is counted in blocks of 16 tokens over all sequences, heads and tiles and dealt to the CTAs in equal runs, so that
-// one long sequence fills the GPU and lengths need not be alike; runs that share a tile leave (max, sum, output) and a second kernel joins them, always in the same order.
+// What bounds it is the cache's bytes.  The rows of a tile (8, or 16) are (token, query head) pairs that share a key head, so a token's codes are read once for the group; tiles of
+// a sequence lie next to one another in the order of the work.  Work is counted in blocks of 16 tokens over all sequences, heads and tiles and dealt to the CTAs, one on each SM, in
+// equal runs, so that one long sequence fills the GPU and lengths need not be alike; runs that share a tile leave (max, sum, output) and a second kernel joins them, always in the
+// same order.
 //
 // A warp keeps its own ring of blocks in shared memory, filled by asynchronous copies that swizzle 16-byte pieces (rows lie 128 bytes apart, which would be the same banks), and
-// multiplies on the tensor cores (mma.sync, 16 x 8 x 16: eight columns are what a token group has, and nothing is waited for across warps; the tensor pipe is far from what
-// bounds it).  A thread's four codes of a 32-bit word are four channels of a key, whichever: queries are laid out to match; a thread's word of a value is transposed against
-// those of three other tokens by byte permutations.
+// multiplies on the tensor cores (mma.sync, 16 x 8 x 16: a block's 16 tokens, or 16 channels of their values, by eight rows: what a group has, and nothing is waited for across warps).
+// A thread's four codes of a 32-bit word are four channels of a key, whichever: queries are laid out to match; a thread's word of a value is transposed against those of three other
+// tokens by byte permutations, and the weights by movmatrix.
 //
 // Codes are exact in fp16.  A row of queries is scaled by a power of two to below 2^14 and taken as one fp16 term (bf16 and fp16 rows: exact but for channels 2^-27 below the
 // row's largest), or two (fp32: 22 bits).  Weights: the page's value scale is part of the exponent, 2^(x + e - max (x + e)) 2^14, so that the largest contribution, not the largest
 // weight, is what fp16's 11 bits count from (fp32 rows: two terms, 22 bits); sums, maxima and outputs are fp32, and the denominator is summed from fp32 weights without the scale.
-constexpr int kRowTile = 16, kFewWarps = 4, kFewThreads = 32 * kFewWarps, kMetaBlocks = 256;
-constexpr int kMinBlocks = 8;                                  // of a CTA's run
+// A tensor-core sum is cut off at every step: fp32 rows add the second terms' sums and every block's outputs to theirs by fp32 additions.
+constexpr int kMetaBlocks = 256;
 
-template <int DP, int TERMS>
+template <int DP, int TERMS, int NT>
 struct Few {
+    static constexpr int kWarps = TERMS == 2 || DP == 256 ? 8 : NT == 1 ? 16 : 12, kThreads = 32 * kWarps, kRows = 8 * NT;
     static constexpr int kSide = kKvBlock * DP;               // bytes of a block's keys, or values
-    static constexpr int kStages = DP == 64 ? 8 : DP == 128 ? 4 : 3;
-    static constexpr int kRing = kFewWarps * kStages * 2 * kSide;
-    static constexpr int kQ = TERMS * (DP / 16) * 32 * 16;    // fragments of the queries
-    static constexpr int kSmem = kRing + kQ + kMetaBlocks * 12 + 16 * 4 + kFewWarps * 16 * 12 + 256;
-    static constexpr int kCtas = DP == 256 ? 1 : DP * TERMS > 128 ? 2 : 3;
+    static constexpr int kStages = 192 * 1024 / (kWarps * 2 * kSide) > 8 ? 8 : 192 * 1024 / (kWarps * 2 * kSide);
+    static constexpr int kRing = kWarps * kStages * 2 * kSide;
+    static constexpr int kQ = TERMS * NT * (DP / 16) * 32 * 8;                    // fragments of the queries
+    static constexpr int kSums = kWarps * kRows * DP * 4;                         // (where the ring lies)
+    static constexpr int kSmem = (kRing > kSums ? kRing : kSums) + kQ + kMetaBlocks * 12 + kRows * 4 + kWarps * kRows * 12 + 128;
 };
+constexpr int kFewCtas = 148, kJoinThreads = 512;
 
-__device__ __forceinline__ void mma16816(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint2 b) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b.x), "r"(b.y));
 }
+__device__ __forceinline__ uint32_t transposed(uint32_t v) {          // of 8 x 8 fp16, a row in four lanes
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+// x, y as fp16, and what that leaves
+__device__ __forceinline__ uint32_t rest_of(float x, float y, uint32_t h) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+    return pack_half(x - f.x, y - f.y);
+}
+
 // where 16-byte piece `c` of row `r` of a block lies
 template <int DP>
 __device__ __forceinline__ int piece_at(int r, int c) {
@@ -274,96 +288,139 @@ struct Span {
     int begin, n, past, low, blocks, tiles;                   // low: the first block
     __device__ __forceinline__ long long units(int kv_heads) const { return (long long)kv_heads * tiles * blocks; }
 };
+template <int ROWS>
 __device__ __forceinline__ Span span_of(const Kv8Step& s, const Kv8Attention& a, int i, int group, int page_shift) {
-    const int window = a.window;
     Span p;
     p.begin = s.begin(i);
     p.n = max(s.end(i) - p.begin, 0);
     p.past = s.past[i];
-    p.low = window > 0 ? (int)(max(0ll, (long long)p.past + 1 - window) / kKvBlock) : 0;
+    p.low = a.window > 0 ? (int)(max(0ll, (long long)p.past + 1 - a.window) / kKvBlock) : 0;
     const long long end = min((long long)max(p.past, 0) + p.n, (long long)s.max_pages << page_shift);
     p.blocks = max(1, (int)((end + kKvBlock - 1) / kKvBlock) - p.low);
-    p.tiles = (long long)p.n * group > a.few_most ? 0 : (p.n * group + kRowTile - 1) / kRowTile;
+    p.tiles = (long long)p.n * group > a.few_most ? 0 : (p.n * group + ROWS - 1) / ROWS;
     return p;
 }
 
-// The sequence that holds the unit `per * nth` of all, where per = what a CTA takes (all threads; seq < 0: there is none)
+// The sequence that holds the unit `per * nth` of all, where per = what a CTA takes: a block for every warp at least, unless that is more than any tile has (one warp; seq < 0:
+// there is none)
 struct Place {
     int seq;
     long long base, per, total;
 };
-__device__ __forceinline__ Place find_place(const Kv8Step& s, const Kv8Attention& a, int kv_heads, int group, int page_shift, int ctas, int nth) {
-    __shared__ long long sums[kFewWarps];
-    __shared__ Place found;
-    const int each = (s.sequences + kFewThreads - 1) / kFewThreads, i0 = threadIdx.x * each, i1 = min(i0 + each, s.sequences);
+template <int ROWS>
+__device__ __forceinline__ Place find_place(const Kv8Step& s, const Kv8Attention& a, int kv_heads, int group, int page_shift, int warps, int nth) {
+    const int lane = threadIdx.x & 31, each = (s.sequences + 31) / 32, i0 = lane * each, i1 = min(i0 + each, s.sequences);
     long long mine = 0;
-    for (int i = i0; i < i1; ++i) mine += span_of(s, a, i, group, page_shift).units(kv_heads);
+    int longest = 0;
+    for (int i = i0; i < i1; ++i) {
+        const Span p = span_of<ROWS>(s, a, i, group, page_shift);
+        mine += p.units(kv_heads);
+        if (p.tiles) longest = max(longest, p.blocks);
+    }
+    longest = (int)__reduce_max_sync(0xffffffffu, (unsigned)longest);
     long long upto = mine;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
         const long long o = __shfl_up_sync(0xffffffffu, upto, d);
-        if ((threadIdx.x & 31) >= d) upto += o;
+        if (lane >= d) upto += o;
     }
-    if ((threadIdx.x & 31) == 31) sums[threadIdx.x >> 5] = upto;
-    if (threadIdx.x == 0) found.seq = -1;
-    __syncthreads();
-    long long total = 0;
-#pragma unroll
-    for (int w = 0; w < kFewWarps; ++w) {
-        if (w < (threadIdx.x >> 5)) upto += sums[w];
-        total += sums[w];
-    }
-    const long long per = max((total + ctas - 1) / ctas, (long long)kMinBlocks), unit = per * nth;
-    if (unit >= upto - mine && unit < upto) {
-        long long base = upto - mine;
-        int i = i0;
-        for (;; ++i) {
-            const long long u = span_of(s, a, i, group, page_shift).units(kv_heads);
-            if (unit < base + u) break;
-            base += u;
+    Place place;
+    place.total = __shfl_sync(0xffffffffu, upto, 31);
+    place.per = max((place.total + kFewCtas - 1) / kFewCtas, (long long)max(min(warps, longest), 1));
+    place.seq = -1;
+    place.base = upto - mine;
+    const long long unit = place.per * nth;
+    const bool here = unit >= place.base && unit < upto;
+    if (here) {
+        for (place.seq = i0;; ++place.seq) {
+            const long long u = span_of<ROWS>(s, a, place.seq, group, page_shift).units(kv_heads);
+            if (unit < place.base + u) break;
+            place.base += u;
         }
-        found = {i, base, per, total};
     }
-    __syncthreads();
-    return found;
+    const unsigned who = __ballot_sync(0xffffffffu, here);
+    const int from = who ? __ffs(who) - 1 : 0;
+    place.seq = __shfl_sync(0xffffffffu, place.seq, from);
+    place.base = __shfl_sync(0xffffffffu, place.base, from);
+    return place;
 }
 
-template <int DP, int FORMAT, int TERMS>
-__global__ void __launch_bounds__(kFewThreads, Few<DP, TERMS>::kCtas) kv8_attention_few_kernel(Kv8Cache c, Kv8Step s, Kv8Attention a, float* part, RowStats* part_stats) {
-    using F = Few<DP, TERMS>;
-    constexpr int kSteps = DP / 16, kHalves = DP == 256 ? 2 : 1, kWords = DP == 64 ? 2 : 4, kCols = kHalves * kWords * 4;
+template <int DP, int FORMAT, int TERMS, int NT>
+__global__ void __launch_bounds__(Few<DP, TERMS, NT>::kThreads, 1) kv8_attention_few_kernel(Kv8Cache c, Kv8Step s, Kv8Attention a, float* part, RowStats* part_stats) {
+    using F = Few<DP, TERMS, NT>;
+    constexpr int kSteps = DP / 16, kHalves = DP == 256 ? 2 : 1, kWords = DP == 64 ? 2 : 4, kCols = kHalves * kWords * 2, kWarps = F::kWarps, kRows = F::kRows;
     extern __shared__ __align__(128) uint8_t smem[];
     uint8_t* const ring = smem + (threadIdx.x >> 5) * (F::kStages * 2 * F::kSide);
-    uint4* const q_frags = reinterpret_cast<uint4*>(smem + F::kRing);
-    int* const meta_page = reinterpret_cast<int*>(smem + F::kRing + F::kQ);
+    float* const sums = reinterpret_cast<float*>(smem);                            // [warps][rows][DP], when the ring is empty
+    uint2* const q_frags = reinterpret_cast<uint2*>(smem + (F::kRing > F::kSums ? F::kRing : F::kSums));
+    int* const meta_page = reinterpret_cast<int*>(q_frags + F::kQ / 8);
     float* const meta_ks = reinterpret_cast<float*>(meta_page + kMetaBlocks);
     float* const meta_ev = meta_ks + kMetaBlocks;
-    float* const row_scale = meta_ev + kMetaBlocks;                                // [16] of the queries, with the scores' scale
-    RowStats* const stats = reinterpret_cast<RowStats*>(row_scale + 16);           // [warps][16]
-    float* const sums = reinterpret_cast<float*>(smem);                            // [warps][16][DP], when the ring is empty
+    float* const row_scale = meta_ev + kMetaBlocks;                                // [rows] of the queries, with the scores' scale
+    RowStats* const stats = reinterpret_cast<RowStats*>(row_scale + kRows);        // [warps][rows]
+    __shared__ Place place;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, group = a.heads / c.kv_heads;
-    zero_rows_of_none(s, a, c.dim, (long long)blockIdx.x * kFewThreads + threadIdx.x, (long long)gridDim.x * kFewThreads);
-    Place at = find_place(s, a, c.kv_heads, group, c.page_shift, gridDim.x, blockIdx.x);
+    if (warp == 0) {
+        const Place found = find_place<kRows>(s, a, c.kv_heads, group, c.page_shift, kWarps, blockIdx.x);
+        if (lane == 0) place = found;
+    }
+    zero_rows_of_none(s, a, c.dim, (long long)blockIdx.x * F::kThreads + threadIdx.x, (long long)gridDim.x * F::kThreads);
+    __syncthreads();
+    Place at = place;
     if (at.seq < 0) return;
     long long unit = at.per * blockIdx.x;
     const long long unit_end = min(unit + at.per, at.total);
-    Span sp = span_of(s, a, at.seq, group, c.page_shift);
+    Span sp = span_of<kRows>(s, a, at.seq, group, c.page_shift);
 
     while (unit < unit_end) {
         while (unit >= at.base + sp.units(c.kv_heads)) {                             // (sequences without rows have no units)
             at.base += sp.units(c.kv_heads);
-            sp = span_of(s, a, ++at.seq, group, c.page_shift);
+            sp = span_of<kRows>(s, a, ++at.seq, group, c.page_shift);
         }
         const long long item = (unit - at.base) / sp.blocks;
         const int b0 = (int)(unit - at.base - item * sp.blocks), count = (int)min((long long)sp.blocks - b0, unit_end - unit);
         const int head = (int)(item / sp.tiles), tile = (int)(item - (long long)head * sp.tiles);
-        const int rows = min(kRowTile, sp.n * group - tile * kRowTile), p0 = tile * kRowTile;
+        const int p0 = tile * kRows, rows = min(kRows, sp.n * group - p0);
         unit += count;
-
-        // queries: a warp scales four rows and leaves them as the products' fragments
-        for (int r = warp; r < kRowTile; r += kFewWarps) {
+        // positions of the tile's rows, first and last
+        const auto position = [&](int r) { return (long long)sp.past + (p0 + min(r, rows - 1)) / group; };
+        const long long back = a.window > 0 ? a.window - 1 : (1ll << 40);
+        const long long pos_a = position(0), pos_b = position(kRows), seen_from = max(0ll, pos_a - back), clear_from = max(0ll, pos_b - back);
+        const auto token = [&](int i) { return (long long)(sp.low + b0 + i) * kKvBlock; };      // of block i of the run
+        const auto look_up = [&](int m_at, int m_n) {                                // pages and scales of the run's blocks from m_at on
+            for (int i = threadIdx.x; i < m_n; i += F::kThreads) {
+                const long long tok = token(m_at + i);
+                int page = -1;
+                if (sp.past >= 0 && tok <= pos_b && tok + kKvBlock > seen_from) page = s.page(at.seq, tok >> c.page_shift, c.pages);
+                meta_page[i] = page;
+                if (page >= 0) {
+                    const size_t ph = (size_t)page * c.kv_heads + head;
+                    const uint32_t vs = __float_as_uint(c.value_scales[ph]);
+                    meta_ks[i] = c.key_scales[ph];
+                    meta_ev[i] = vs >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : (float)((int)(vs >> 23) - 127);
+                }
+            }
+        };
+        const auto issue = [&](int m_at, int m_n, int i, int stage) {                // block i of the list into a slot of the ring
+            if (i < m_n && meta_page[i] >= 0) {
+                const size_t from = ((((size_t)meta_page[i] * c.kv_heads + head) << c.page_shift) + (size_t)(token(m_at + i) & ((1 << c.page_shift) - 1))) * c.stride;
+                const uint32_t to = (uint32_t)__cvta_generic_to_shared(ring + stage * 2 * F::kSide);
+#pragma unroll
+                for (int j = 0; j < DP / 32; ++j) {
+                    const int x = lane + 32 * j, r = x / (DP / 16), p = x % (DP / 16), n = p * 16 < c.stride ? 16 : 0;
+                    const size_t off = from + (size_t)r * c.stride + (n ? p * 16 : 0);
+                    const uint32_t d = to + piece_at<DP>(r, p);
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(c.keys + off), "r"(n) : "memory");
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d + F::kSide), "l"(c.values + off), "r"(n) : "memory");
+                }
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+        look_up(0, min(kMetaBlocks, count));
+        // queries: a warp scales some rows and leaves them as the products' fragments
+        for (int r = warp; r < kRows; r += kWarps) {
             const int p = p0 + r, row = sp.begin + p / group;
             const long long q_at = row * a.q.row + (head * group + p % group) * a.q.head;
             float v[DP / 32];
@@ -376,240 +433,227 @@ __global__ void __launch_bounds__(kFewThreads, Few<DP, TERMS>::kCtas) kv8_attent
             }
             most = __reduce_max_sync(0xffffffffu, most);
             const uint32_t e = most == 0 ? 127u : max(most >> 23, 14u);
-            const float f = __uint_as_float((267u - e) << 23), back = __uint_as_float((e - 13u) << 23);      // 2^(140 - e): to below 2^14, and the way back
-            if (lane == 0) row_scale[r] = e == 255u ? __uint_as_float(0x7fc00000u) : back * (a.scale * kLog2e);
+            const float f = __uint_as_float((267u - e) << 23), way_back = __uint_as_float((e - 13u) << 23);      // 2^(140 - e): to below 2^14, and the way back
+            if (lane == 0) row_scale[r] = e == 255u ? __uint_as_float(0x7fc00000u) : way_back * (a.scale * kLog2e);
 #pragma unroll
             for (int j = 0; j < DP / 32; ++j) {
-                const int d = lane + 32 * j, chunk = d >> 4, step = (chunk >> 2) * 4 + ((d & 15) >> 2), x = d & 3, reg = (x >> 1) * 2 + (r >> 3);
-                __half* const to = reinterpret_cast<__half*>(q_frags) + ((step * 32 + (r & 7) * 4 + (chunk & 3)) * 4 + reg) * 2 + (x & 1);
+                const int d = lane + 32 * j, chunk = d >> 4, step = (chunk >> 2) * 4 + ((d & 15) >> 2), x = d & 3;
+                __half* const to = reinterpret_cast<__half*>(q_frags) + ((((r >> 3) * kSteps + step) * 32 + (r & 7) * 4 + (chunk & 3)) * 2 + (x >> 1)) * 2 + (x & 1);
                 const float y = e == 255u ? 0.f : v[j] * f;
                 const __half hi = __float2half_rn(y);
                 to[0] = hi;
-                if constexpr (TERMS == 2) to[kSteps * 32 * 8] = __float2half_rn(y - __half2float(hi));
+                if constexpr (TERMS == 2) to[NT * kSteps * 32 * 4] = __float2half_rn(y - __half2float(hi));
             }
         }
         __syncthreads();
-        constexpr bool kInRegs = DP * TERMS <= 128;
-        uint4 qf[kInRegs ? TERMS * kSteps : 1];
+        // the thread's rows of each tile of eight: 2 t and 2 t + 1
+        float scale_of[NT][2], m[NT][2], w[NT][2], l[NT][2], o[NT][kCols][4];
+        constexpr bool kInRegs = DP * TERMS * NT <= 256;
+        uint2 qf[kInRegs ? TERMS * NT * kSteps : 1];
         if constexpr (kInRegs) {
 #pragma unroll
-            for (int j = 0; j < TERMS * kSteps; ++j) qf[j] = q_frags[j * 32 + lane];
+            for (int j = 0; j < TERMS * NT * kSteps; ++j) qf[j] = q_frags[j * 32 + lane];
         }
-        const float f0 = row_scale[g], f1 = row_scale[g + 8];
-        // positions of the tile's rows, first and last, and of this thread's two
-        const long long pos_a = (long long)sp.past + p0 / group, pos_b = (long long)sp.past + (p0 + rows - 1) / group;
-        const long long pos0 = (long long)sp.past + min(p0 + g, p0 + rows - 1) / group, pos1 = (long long)sp.past + min(p0 + g + 8, p0 + rows - 1) / group;
-        const long long back = a.window > 0 ? a.window - 1 : (1ll << 40);
-        const long long seen_from = max(0ll, pos_a - back), clear_from = max(0ll, pos_b - back);
-
-        float o[kCols][4], m0 = -INFINITY, m1 = -INFINITY, w0 = -INFINITY, w1 = -INFINITY, l0 = 0.f, l1 = 0.f;
 #pragma unroll
-        for (int j = 0; j < kCols; ++j)
+        for (int n = 0; n < NT; ++n) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[j][e] = 0.f;
+            for (int e = 0; e < 2; ++e) {
+                scale_of[n][e] = row_scale[8 * n + 2 * t + e];
+                m[n][e] = w[n][e] = -INFINITY;
+                l[n][e] = 0.f;
+            }
+#pragma unroll
+            for (int j = 0; j < kCols; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[n][j][e] = 0.f;
+        }
 
         for (int m_at = 0; m_at < count; m_at += kMetaBlocks) {
             const int m_n = min(kMetaBlocks, count - m_at);
-            if (m_at) __syncthreads();                                               // (the last ones have been read)
-            for (int i = threadIdx.x; i < m_n; i += kFewThreads) {
-                const long long tok = (long long)(sp.low + b0 + m_at + i) * kKvBlock;
-                int page = -1;
-                if (sp.past >= 0 && tok <= pos_b && tok + kKvBlock > seen_from) page = s.page(at.seq, tok >> c.page_shift, c.pages);
-                meta_page[i] = page;
-                if (page >= 0) {
-                    const size_t ph = (size_t)page * c.kv_heads + head;
-                    const uint32_t vs = __float_as_uint(c.value_scales[ph]);
-                    meta_ks[i] = c.key_scales[ph];
-                    meta_ev[i] = vs >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : (float)((int)(vs >> 23) - 127);
-                }
+            if (m_at) {
+                __syncthreads();                                                     // (the last ones have been read)
+                look_up(m_at, m_n);
+                __syncthreads();
             }
-            __syncthreads();
-            const auto issue = [&](int i, int stage) {                               // block i of the list into a slot of the ring
-                if (i < m_n && meta_page[i] >= 0) {
-                    const long long tok = (long long)(sp.low + b0 + m_at + i) * kKvBlock;
-                    const size_t from = ((((size_t)meta_page[i] * c.kv_heads + head) << c.page_shift) + (size_t)(tok & ((1 << c.page_shift) - 1))) * c.stride;
-                    const uint32_t to = (uint32_t)__cvta_generic_to_shared(ring + stage * 2 * F::kSide);
-#pragma unroll
-                    for (int j = 0; j < DP / 32; ++j) {
-                        const int x = lane + 32 * j, r = x / (DP / 16), p = x % (DP / 16), n = p * 16 < c.stride ? 16 : 0;
-                        const size_t off = from + (size_t)r * c.stride + (n ? p * 16 : 0);
-                        const uint32_t d = to + piece_at<DP>(r, p);
-                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(c.keys + off), "r"(n) : "memory");
-                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d + F::kSide), "l"(c.values + off), "r"(n) : "memory");
-                    }
-                }
-                asm volatile("cp.async.commit_group;" ::: "memory");
-            };
-#pragma unroll
-            for (int j = 0; j < F::kStages - 1; ++j) issue(warp + kFewWarps * j, j);
+#pragma unroll 1
+            for (int j = 0; j < F::kStages - 1; ++j) issue(m_at, m_n, warp + kWarps * j, j);
             int stage = 0;
-            for (int i = warp; i < m_n; i += kFewWarps) {
+#pragma unroll 1
+            for (int i = warp; i < m_n; i += kWarps) {
                 asm volatile("cp.async.wait_group %0;" ::"n"(F::kStages - 2) : "memory");
                 __syncwarp();                                                        // the block is there for every lane, and the slot in front has been read by all
-                issue(i + kFewWarps * (F::kStages - 1), stage == 0 ? F::kStages - 1 : stage - 1);
+                issue(m_at, m_n, i + kWarps * (F::kStages - 1), stage == 0 ? F::kStages - 1 : stage - 1);
                 const uint8_t* const keys = ring + stage * 2 * F::kSide;
                 const uint8_t* const values = keys + F::kSide;
                 stage = stage + 1 == F::kStages ? 0 : stage + 1;
                 if (meta_page[i] < 0) continue;
 
-                float x[2][4] = {};
+                // scores: token g of row 2 t and of row 2 t + 1, token g + 8 of either
+                float x[NT][4], rest[TERMS == 2 ? NT : 1][4];
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[n][e] = rest[TERMS == 2 ? n : 0][e] = 0.f;
 #pragma unroll
                 for (int h = 0; h < DP / 64; ++h) {
+                    const uint4 u4 = *reinterpret_cast<const uint4*>(keys + piece_at<DP>(g, t + 4 * h)), v4 = *reinterpret_cast<const uint4*>(keys + piece_at<DP>(8 + g, t + 4 * h));
+                    const uint32_t u[4] = {u4.x, u4.y, u4.z, u4.w}, v[4] = {v4.x, v4.y, v4.z, v4.w};
 #pragma unroll
-                    for (int b = 0; b < 2; ++b) {
-                        const uint4 w4 = *reinterpret_cast<const uint4*>(keys + piece_at<DP>(8 * b + g, t + 4 * h));
-                        const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+                    for (int j = 0; j < 4; ++j) {
+                        uint32_t a0, a1, a2, a3;
+                        decode4<FORMAT>(u[j], a0, a2);
+                        decode4<FORMAT>(v[j], a1, a3);
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            uint32_t lo, hi;
-                            decode4<FORMAT>(w[j], lo, hi);
-#pragma unroll
-                            for (int e = 0; e < TERMS; ++e) {
-                                const int f = e * kSteps + 4 * h + j;
-                                mma16816(x[b], kInRegs ? qf[kInRegs ? f : 0] : q_frags[f * 32 + lane], lo, hi);
-                            }
+                        for (int n = 0; n < NT; ++n) {
+                            const int f = n * kSteps + 4 * h + j;
+                            mma16816(x[n], a0, a1, a2, a3, kInRegs ? qf[kInRegs ? f : 0] : q_frags[f * 32 + lane]);
+                            if constexpr (TERMS == 2) mma16816(rest[n], a0, a1, a2, a3, kInRegs ? qf[kInRegs ? NT * kSteps + f : 0] : q_frags[(NT * kSteps + f) * 32 + lane]);
                         }
                     }
                 }
-                const float ks = meta_ks[i], ev = meta_ev[i], k0 = f0 * ks, k1 = f1 * ks;
-#pragma unroll
-                for (int b = 0; b < 2; ++b) { x[b][0] *= k0; x[b][1] *= k0; x[b][2] *= k1; x[b][3] *= k1; }
-                const long long tok = (long long)(sp.low + b0 + m_at + i) * kKvBlock;
+                const float ks = meta_ks[i], ev = meta_ev[i];
+                const long long tok = token(m_at + i);
                 const bool clear = tok + kKvBlock - 1 <= pos_a && tok >= clear_from;   // every row sees all of the block
-                uint32_t hidden = 0;
-                if (!clear) {
+                uint2 hi[NT], lo[TERMS == 2 ? NT : 1];
 #pragma unroll
-                    for (int b = 0; b < 2; ++b)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const long long key = tok + 8 * b + 2 * t + (e & 1), pos = e < 2 ? pos0 : pos1;
-                            if (key > pos || key < pos - back) {
-                                x[b][e] = -INFINITY;
-                                hidden |= 1u << (4 * b + e);
-                            }
-                        }
-                }
-                float t0 = fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[1][0], x[1][1])), t1 = fmaxf(fmaxf(x[0][2], x[0][3]), fmaxf(x[1][2], x[1][3]));
-                t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, 1));
-                t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, 1));
-                t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, 2));
-                t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, 2));
-                const float n0 = fmaxf(m0, t0), n1 = fmaxf(m1, t1), u0 = fmaxf(w0, t0 + ev), u1 = fmaxf(w1, t1 + ev);
-                if (__any_sync(0xffffffffu, n0 > m0 || n1 > m1 || u0 > w0 || u1 > w1)) {
-                    const float a0 = lower_to(m0, n0), a1 = lower_to(m1, n1), c0 = lower_to(w0, u0), c1 = lower_to(w1, u1);
-                    l0 *= a0;
-                    l1 *= a1;
-#pragma unroll
-                    for (int j = 0; j < kCols; ++j) { o[j][0] *= c0; o[j][1] *= c0; o[j][2] *= c1; o[j][3] *= c1; }
-                    m0 = n0; m1 = n1; w0 = u0; w1 = u1;
-                }
-                // (rows that have seen nothing yet: any reference will do)
-                const float r0 = m0 == -INFINITY ? 0.f : m0, r1 = m1 == -INFINITY ? 0.f : m1;
-                const float s0 = (w0 == -INFINITY ? 0.f : w0) - ev - kWeightBits, s1 = (w1 == -INFINITY ? 0.f : w1) - ev - kWeightBits;
-                float p[2][4];
-#pragma unroll
-                for (int b = 0; b < 2; ++b) {
-                    l0 += exp2_fast(x[b][0] - r0) + exp2_fast(x[b][1] - r0);
-                    l1 += exp2_fast(x[b][2] - r1) + exp2_fast(x[b][3] - r1);
+                for (int n = 0; n < NT; ++n) {
+                    uint32_t hidden = 0;
+                    float top[2];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        p[b][e] = exp2_fast(x[b][e] - (e < 2 ? s0 : s1));
-                        if (!clear && (hidden >> (4 * b + e) & 1)) p[b][e] = 0.f;     // (whatever the page's scales are)
+                        if constexpr (TERMS == 2) x[n][e] += rest[n][e];
+                        x[n][e] *= scale_of[n][e & 1] * ks;
                     }
-                }
-                const uint4 hi = make_uint4(pack_half(p[0][0], p[0][1]), pack_half(p[0][2], p[0][3]), pack_half(p[1][0], p[1][1]), pack_half(p[1][2], p[1][3]));
-                uint4 lo = hi;
-                if constexpr (TERMS == 2) {
-                    const auto rest = [](float x, float y, uint32_t h) {
-                        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
-                        return pack_half(x - f.x, y - f.y);
-                    };
-                    lo = make_uint4(rest(p[0][0], p[0][1], hi.x), rest(p[0][2], p[0][3], hi.y), rest(p[1][0], p[1][1], hi.z), rest(p[1][2], p[1][3], hi.w));
+                    if (!clear) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const long long key = tok + g + 8 * (e >> 1), pos = position(8 * n + 2 * t + (e & 1));
+                            if (key > pos || key < pos - back) {
+                                x[n][e] = -INFINITY;
+                                hidden |= 1u << e;
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        top[e] = fmaxf(x[n][e], x[n][e + 2]);
+                        top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 4));
+                        top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 8));
+                        top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 16));
+                    }
+                    const float m0 = fmaxf(m[n][0], top[0]), m1 = fmaxf(m[n][1], top[1]), w0 = fmaxf(w[n][0], top[0] + ev), w1 = fmaxf(w[n][1], top[1] + ev);
+                    if (__any_sync(0xffffffffu, m0 > m[n][0] || m1 > m[n][1] || w0 > w[n][0] || w1 > w[n][1])) {
+                        const float c0 = lower_to(w[n][0], w0), c1 = lower_to(w[n][1], w1);
+                        l[n][0] *= lower_to(m[n][0], m0);
+                        l[n][1] *= lower_to(m[n][1], m1);
+#pragma unroll
+                        for (int j = 0; j < kCols; ++j) { o[n][j][0] *= c0; o[n][j][1] *= c1; o[n][j][2] *= c0; o[n][j][3] *= c1; }
+                        m[n][0] = m0; m[n][1] = m1; w[n][0] = w0; w[n][1] = w1;
+                    }
+                    float p[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        // (rows that have seen nothing yet: any reference will do)
+                        const float r = m[n][e & 1] == -INFINITY ? 0.f : m[n][e & 1], q = (w[n][e & 1] == -INFINITY ? 0.f : w[n][e & 1]) - ev - kWeightBits;
+                        l[n][e & 1] += exp2_fast(x[n][e] - r);
+                        p[e] = exp2_fast(x[n][e] - q);
+                        if (!clear && (hidden >> e & 1)) p[e] = 0.f;                  // (whatever the page's scales are)
+                    }
+                    const uint32_t h0 = pack_half(p[0], p[1]), h1 = pack_half(p[2], p[3]);
+                    hi[n] = make_uint2(transposed(h0), transposed(h1));
+                    if constexpr (TERMS == 2) lo[n] = make_uint2(transposed(rest_of(p[0], p[1], h0)), transposed(rest_of(p[2], p[3], h1)));
                 }
 #pragma unroll
                 for (int h = 0; h < kHalves; ++h) {
-                    uint32_t w[4][4];                                                // [token 2 t, 2 t + 1, 2 t + 8, 2 t + 9][word]
+                    uint32_t v[4][4];                                                // [token 2 t, 2 t + 1, 2 t + 8, 2 t + 9][word]
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const int r = 2 * t + (e & 1) + 8 * (e >> 1);
                         if constexpr (DP == 64) {
                             const uint2 v2 = *reinterpret_cast<const uint2*>(values + piece_at<DP>(r, g >> 1) + 8 * (g & 1));
-                            w[e][0] = v2.x; w[e][1] = v2.y;
+                            v[e][0] = v2.x; v[e][1] = v2.y;
                         } else {
                             const uint4 v4 = *reinterpret_cast<const uint4*>(values + piece_at<DP>(r, 8 * h + g));
-                            w[e][0] = v4.x; w[e][1] = v4.y; w[e][2] = v4.z; w[e][3] = v4.w;
+                            v[e][0] = v4.x; v[e][1] = v4.y; v[e][2] = v4.z; v[e][3] = v4.w;
                         }
                     }
 #pragma unroll
-                    for (int j = 0; j < kWords; ++j) {
-                        uint32_t b0[4], b1[4];                                       // of four channels: the pairs of tokens
-                        decode4<FORMAT>(__byte_perm(w[0][j], w[1][j], 0x5140), b0[0], b0[1]);
-                        decode4<FORMAT>(__byte_perm(w[0][j], w[1][j], 0x7362), b0[2], b0[3]);
-                        decode4<FORMAT>(__byte_perm(w[2][j], w[3][j], 0x5140), b1[0], b1[1]);
-                        decode4<FORMAT>(__byte_perm(w[2][j], w[3][j], 0x7362), b1[2], b1[3]);
+                    for (int j = 0; j < kWords; ++j)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            mma16816(o[(h * kWords + j) * 4 + e], hi, b0[e], b1[e]);
-                            if constexpr (TERMS == 2) mma16816(o[(h * kWords + j) * 4 + e], lo, b0[e], b1[e]);
+                        for (int e = 0; e < 2; ++e) {                                // channels 2 e and 2 e + 1 of the word
+                            uint32_t a0, a1, a2, a3;
+                            decode4<FORMAT>(__byte_perm(v[0][j], v[1][j], e ? 0x7362 : 0x5140), a0, a1);
+                            decode4<FORMAT>(__byte_perm(v[2][j], v[3][j], e ? 0x7362 : 0x5140), a2, a3);
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) {
+                                float (&to)[4] = o[n][(h * kWords + j) * 2 + e];
+                                if constexpr (TERMS == 2) {
+                                    float y[4] = {0.f, 0.f, 0.f, 0.f};
+                                    mma16816(y, a0, a1, a2, a3, lo[n]);
+                                    mma16816(y, a0, a1, a2, a3, hi[n]);
+#pragma unroll
+                                    for (int z = 0; z < 4; ++z) to[z] += y[z];
+                                } else {
+                                    mma16816(to, a0, a1, a2, a3, hi[n]);
+                                }
+                            }
                         }
-                    }
                 }
             }
             asm volatile("cp.async.wait_group 0;" ::: "memory");
         }
 
         // the warps' sums meet in shared memory
-        l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
-        l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
-        l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
-        l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
         __syncthreads();                                                             // every warp is done with its ring
-        if (t == 0) {
-            stats[warp * 16 + g] = {m0, w0, l0};
-            stats[warp * 16 + g + 8] = {m1, w1, l1};
-        }
-        // column 2 t (or 2 t + 1) of product (h, j) is channel 128 h + 16 (2 t) + j, eight products of 64 channels 8 (2 t) + j
-        constexpr int kRun = DP == 64 ? 8 : 16;
 #pragma unroll
-        for (int h = 0; h < kHalves; ++h)
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                float* const to = sums + (size_t)(warp * 16 + g + 8 * (e >> 1)) * DP + 128 * h + kRun * (2 * t + (e & 1));
+            for (int e = 0; e < 2; ++e) {
+                const int r = 8 * n + 2 * t + e;
 #pragma unroll
-                for (int j = 0; j < kRun; j += 4)
-                    *reinterpret_cast<float4*>(to + j) = make_float4(o[h * 16 + j][e], o[h * 16 + j + 1][e], o[h * 16 + j + 2][e], o[h * 16 + j + 3][e]);
+                for (int d = 4; d < 32; d <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], d);
+                if (g == 0) stats[warp * kRows + r] = {m[n][e], w[n][e], l[n][e]};
+                if (r >= rows) continue;
+                // products (h, j) of this thread are channels 128 h + 16 g + 2 j and the next one (of 64 channels: 8 g + 2 j)
+                constexpr int kRun = DP == 64 ? 8 : 16;
+#pragma unroll
+                for (int h = 0; h < kHalves; ++h)
+#pragma unroll
+                    for (int j = 0; j < kRun; j += 4)
+                        *reinterpret_cast<float4*>(sums + (size_t)(warp * kRows + r) * DP + 128 * h + kRun * g + j) =
+                            make_float4(o[n][h * 8 + j / 2][e], o[n][h * 8 + j / 2][e + 2], o[n][h * 8 + j / 2 + 1][e], o[n][h * 8 + j / 2 + 1][e + 2]);
             }
         __syncthreads();
         const bool whole = b0 == 0 && count == sp.blocks;
         const size_t slot = 2 * (size_t)blockIdx.x + (b0 == 0);
-        for (int i = threadIdx.x; i < rows * (DP / 4); i += kFewThreads) {
+        for (int i = threadIdx.x; i < rows * (DP / 4); i += F::kThreads) {
             const int r = i / (DP / 4), d = i % (DP / 4) * 4;
-            float m = -INFINITY, w = -INFINITY, l = 0.f;
+            float mm = -INFINITY, ww = -INFINITY, ll = 0.f;
 #pragma unroll
-            for (int v = 0; v < kFewWarps; ++v) {
-                m = fmaxf(m, stats[v * 16 + r].m);
-                w = fmaxf(w, stats[v * 16 + r].w);
+            for (int v = 0; v < kWarps; ++v) {
+                mm = fmaxf(mm, stats[v * kRows + r].m);
+                ww = fmaxf(ww, stats[v * kRows + r].w);
             }
             float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-            for (int v = 0; v < kFewWarps; ++v) {
-                const RowStats y = stats[v * 16 + r];
-                const float f = lower_to(y.w, w);
-                const float4 z = *reinterpret_cast<const float4*>(sums + (size_t)(v * 16 + r) * DP + d);
-                l += y.l * lower_to(y.m, m);
+#pragma unroll 4
+            for (int v = 0; v < kWarps; ++v) {
+                const RowStats y = stats[v * kRows + r];
+                const float f = lower_to(y.w, ww);
+                const float4 z = *reinterpret_cast<const float4*>(sums + (size_t)(v * kRows + r) * DP + d);
+                ll += y.l * lower_to(y.m, mm);
                 sum.x += f * z.x; sum.y += f * z.y; sum.z += f * z.z; sum.w += f * z.w;
             }
             if (whole) {
                 const int p = p0 + r, h = head * group + p % group;
-                const float f = row_factor(a, h, m, w, l);
+                const float f = row_factor(a, h, mm, ww, ll);
                 const size_t to = ((size_t)(sp.begin + p / group) * a.heads + h) * c.dim + d;
                 const float y[4] = {sum.x, sum.y, sum.z, sum.w};
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
                     if (d + e < c.dim) store_out(a, to + e, f * y[e]);
             } else {
-                *reinterpret_cast<float4*>(part + (slot * 16 + r) * DP + d) = sum;
-                if (d == 0) part_stats[slot * 16 + r] = {m, w, l};
+                *reinterpret_cast<float4*>(part + (slot * kRows + r) * DP + d) = sum;
+                if (d == 0) part_stats[slot * kRows + r] = {mm, ww, ll};
             }
         }
         __syncthreads();                                                             // (the ring and the queries' room are taken again)
@@ -617,92 +661,85 @@ __global__ void __launch_bounds__(kFewThreads, Few<DP, TERMS>::kCtas) kv8_attent
 }
 
 // A tile that several runs share: a CTA per border between runs, and per row.  The first border inside the tile joins it.
-template <int DP>
-__global__ void __launch_bounds__(kFewThreads) kv8_attention_join_kernel(Kv8Cache c, Kv8Step s, Kv8Attention a, int ctas, const float* part, const RowStats* part_stats) {
+template <int DP, int NT>
+__global__ void __launch_bounds__(kJoinThreads) kv8_attention_join_kernel(Kv8Cache c, Kv8Step s, Kv8Attention a, int warps, const float* part, const RowStats* part_stats) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    __shared__ float tops[kFewWarps][2];
-    __shared__ __align__(16) float sums[kFewWarps][DP];
-    __shared__ float totals[kFewWarps];
+    constexpr int kRows = 8 * NT, kWarps = kJoinThreads / 32, kEach = DP / 32;
+    __shared__ __align__(16) float sums[kWarps][DP];
+    __shared__ RowStats tops[kWarps];
+    __shared__ Place place;
     const int nth = blockIdx.x + 1, r = blockIdx.y, group = a.heads / c.kv_heads, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const Place at = find_place(s, a, c.kv_heads, group, c.page_shift, ctas, nth);
+    if (warp == 0) {
+        const Place found = find_place<kRows>(s, a, c.kv_heads, group, c.page_shift, warps, nth);
+        if (lane == 0) place = found;
+    }
+    __syncthreads();
+    const Place at = place;
     if (at.seq < 0) return;
-    const Span sp = span_of(s, a, at.seq, group, c.page_shift);
+    const Span sp = span_of<kRows>(s, a, at.seq, group, c.page_shift);
     const long long item = (at.per * nth - at.base) / sp.blocks, start = at.base + item * sp.blocks;
     const int c0 = (int)(start / at.per), c1 = (int)((start + sp.blocks - 1) / at.per);
-    const int head = (int)(item / sp.tiles), tile = (int)(item - (long long)head * sp.tiles), p = tile * kRowTile + r;
+    const int head = (int)(item / sp.tiles), tile = (int)(item - (long long)head * sp.tiles), p = tile * kRows + r;
     if (start == at.per * nth || nth != c0 + 1 || p >= sp.n * group) return;
-    const auto slot = [&](int i) { return ((size_t)2 * i + (i == c0)) * 16 + r; };
-    float m = -INFINITY, w = -INFINITY;
-    for (int i = c0 + threadIdx.x; i <= c1; i += kFewThreads) {
-        const RowStats y = part_stats[slot(i)];
-        m = fmaxf(m, y.m);
-        w = fmaxf(w, y.w);
-    }
-#pragma unroll
-    for (int d = 16; d; d >>= 1) {
-        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-        w = fmaxf(w, __shfl_xor_sync(0xffffffffu, w, d));
-    }
-    if (lane == 0) { tops[warp][0] = m; tops[warp][1] = w; }
-    __syncthreads();
-#pragma unroll
-    for (int v = 0; v < kFewWarps; ++v) { m = fmaxf(m, tops[v][0]); w = fmaxf(w, tops[v][1]); }
-    constexpr int kEach = DP / 32;
-    float sum[kEach] = {}, l = 0.f;
+    // a warp takes every so many-th run, below maxima of its own
+    float sum[kEach] = {};
+    RowStats mine{-INFINITY, -INFINITY, 0.f};
 #pragma unroll 4
-    for (int i = c0 + warp; i <= c1; i += kFewWarps) {
-        const RowStats y = part_stats[slot(i)];
-        const float f = lower_to(y.w, w);
-        l += y.l * lower_to(y.m, m);
+    for (int i = c0 + warp; i <= c1; i += kWarps) {
+        const size_t slot = ((size_t)2 * i + (i == c0)) * kRows + r;
+        const RowStats y = part_stats[slot];
+        const float m = fmaxf(mine.m, y.m), w = fmaxf(mine.w, y.w), f = lower_to(mine.w, w), z = lower_to(y.w, w);
+        mine = {m, w, mine.l * lower_to(mine.m, m) + y.l * lower_to(y.m, m)};
 #pragma unroll
-        for (int j = 0; j < kEach; ++j) sum[j] += f * part[slot(i) * DP + lane + 32 * j];
+        for (int j = 0; j < kEach; ++j) sum[j] = f * sum[j] + z * part[slot * DP + lane + 32 * j];
     }
 #pragma unroll
     for (int j = 0; j < kEach; ++j) sums[warp][lane + 32 * j] = sum[j];
-    if (lane == 0) totals[warp] = l;
+    if (lane == 0) tops[warp] = mine;
     __syncthreads();
-    const int h = head * group + p % group;
-    l = 0.f;
+    if (threadIdx.x >= c.dim) return;
+    float m = -INFINITY, w = -INFINITY, l = 0.f, y = 0.f;
 #pragma unroll
-    for (int v = 0; v < kFewWarps; ++v) l += totals[v];
-    const float f = row_factor(a, h, m, w, l);
-    for (int d = threadIdx.x; d < c.dim; d += kFewThreads) {
-        float y = 0.f;
+    for (int v = 0; v < kWarps; ++v) { m = fmaxf(m, tops[v].m); w = fmaxf(w, tops[v].w); }
 #pragma unroll
-        for (int v = 0; v < kFewWarps; ++v) y += sums[v][d];
-        store_out(a, ((size_t)(sp.begin + p / group) * a.heads + h) * c.dim + d, f * y);
+    for (int v = 0; v < kWarps; ++v) {
+        l += tops[v].l * lower_to(tops[v].m, m);
+        y += sums[v][threadIdx.x] * lower_to(tops[v].w, w);
     }
+    const int h = head * group + p % group;
+    store_out(a, ((size_t)(sp.begin + p / group) * a.heads + h) * c.dim + threadIdx.x, row_factor(a, h, m, w, l) * y);
 }
 
 inline bool wide(const Kv8Rows& x, int type, int dim) {
     const long long b = type_bytes(type);
     return (reinterpret_cast<uintptr_t>(x.x) & 15) == 0 && x.row * b % 16 == 0 && x.head * b % 16 == 0 && dim % 8 == 0;
 }
-inline int padded_dim(const Kv8Cache& c) { return c.dim <= 64 ? 64 : c.dim <= 128 ? 128 : 256; }
+inline int padded_dim(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 inline int terms_of(int type) { return type == kTypeF32 ? 2 : 1; }
-constexpr int kFewSms = 148;
-template <int DP, int TERMS> constexpr int few_ctas() { return kFewSms * Few<DP, TERMS>::kCtas; }
-inline int few_ctas(int dp, int terms) {
-    return dp == 64 ? (terms == 2 ? few_ctas<64, 2>() : few_ctas<64, 1>()) : dp == 128 ? (terms == 2 ? few_ctas<128, 2>() : few_ctas<128, 1>()) : (terms == 2 ? few_ctas<256, 2>() : few_ctas<256, 1>());
-}
 
-template <int DP, int FORMAT, int TERMS>
+template <int DP, int FORMAT, int TERMS, int NT>
 cudaError_t run_few(const Kv8Cache& c, const Kv8Step& s, const Kv8Attention& a, void* work, cudaStream_t st) {
-    using F = Few<DP, TERMS>;
-    constexpr int kCtas = few_ctas<DP, TERMS>();
+    using F = Few<DP, TERMS, NT>;
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
-    e = dia::ask_smem<kv8_attention_few_kernel<DP, FORMAT, TERMS>>(dev, F::kSmem);
+    e = dia::ask_smem<kv8_attention_few_kernel<DP, FORMAT, TERMS, NT>>(dev, F::kSmem);
     if (e != cudaSuccess) return e;
     float* const part = reinterpret_cast<float*>(work);
-    RowStats* const stats = reinterpret_cast<RowStats*>(part + (size_t)2 * kCtas * 16 * DP);
-    kv8_attention_few_kernel<DP, FORMAT, TERMS><<<kCtas, kFewThreads, F::kSmem, st>>>(c, s, a, part, stats);
+    RowStats* const stats = reinterpret_cast<RowStats*>(part + (size_t)2 * kFewCtas * F::kRows * DP);
+    kv8_attention_few_kernel<DP, FORMAT, TERMS, NT><<<kFewCtas, F::kThreads, F::kSmem, st>>>(c, s, a, part, stats);
     e = cudaGetLastError();
     if (e != cudaSuccess) return e;
     ++dia::extra_launches();
-    const int most = (int)std::min<long long>(kRowTile, (long long)s.rows * (a.heads / c.kv_heads));
-    return launch_pdl(kv8_attention_join_kernel<DP>, dim3(kCtas - 1, most), dim3(kFewThreads), 0, st, c, s, a, kCtas, part, stats);
+    const int most = (int)std::min<long long>(F::kRows, (long long)s.rows * (a.heads / c.kv_heads));
+    return launch_pdl(kv8_attention_join_kernel<DP, NT>, dim3(kFewCtas - 1, most), dim3(kJoinThreads), 0, st, c, s, a, (int)F::kWarps, part, stats);
+}
+template <int DP, int FORMAT>
+cudaError_t run_few(const Kv8Cache& c, const Kv8Step& s, const Kv8Attention& a, void* work, cudaStream_t st) {
+    // tiles of eight rows where sequences have no more of them on average (the products of 16 rows take twice the registers and the tensor cores' time)
+    const bool eight = (long long)s.rows * (a.heads / c.kv_heads) <= 8ll * s.sequences;
+    if (terms_of(a.type) == 2) return eight ? run_few<DP, FORMAT, 2, 1>(c, s, a, work, st) : run_few<DP, FORMAT, 2, 2>(c, s, a, work, st);
+    return eight ? run_few<DP, FORMAT, 1, 1>(c, s, a, work, st) : run_few<DP, FORMAT, 1, 2>(c, s, a, work, st);
 }
 
 }  // namespace
@@ -736,30 +773,27 @@ cudaError_t launch_kv8_read(const Kv8Cache& c, const Kv8Step& s, void* k, void* 
 namespace {
 // Pairs of a sequence from which on tiles of 256 rows are the shorter way
 constexpr int kFewMost = 64;
-inline bool some_in_tiles(const Kv8Cache& c, const Kv8Step& s, int heads, int type) { return kv8_tiles_ok(c, type) && (long long)s.rows * (heads / c.kv_heads) > kFewMost; }
+inline bool some_in_tiles(int kv_heads, int dim, int rows, int heads, int type) { return kv8_tiles_ok(dim, type) && (long long)rows * (heads / kv_heads) > kFewMost; }
 }  // namespace
 
-size_t kv8_attention_work_bytes(const Kv8Cache& c, const Kv8Step& s, int heads, int type) {
-    const int dp = padded_dim(c);
-    const size_t few = (size_t)2 * few_ctas(dp, terms_of(type)) * 16 * (dp * sizeof(float) + sizeof(RowStats));
-    return some_in_tiles(c, s, heads, type) ? std::max(few, kv8_tiles_work_bytes(c)) : few;
+size_t kv8_attention_work_bytes(int kv_heads, int dim, int rows, int heads, int type) {
+    const int dp = padded_dim(dim);
+    const size_t few = (size_t)2 * kFewCtas * 16 * (dp * sizeof(float) + sizeof(RowStats));
+    return some_in_tiles(kv_heads, dim, rows, heads, type) ? std::max(few, kv8_tiles_work_bytes(dim)) : few;
 }
 
 cudaError_t launch_kv8_attention(const Kv8Cache& c, const Kv8Step& s, Kv8Attention a, void* work, cudaStream_t st) {
-    const int dp = padded_dim(c);
-    const bool two = terms_of(a.type) == 2;
+    const int dp = padded_dim(c.dim);
     a.few_most = 0x7fffffff;
-    if (some_in_tiles(c, s, a.heads, a.type)) {
+    if (some_in_tiles(c.kv_heads, c.dim, s.rows, a.heads, a.type)) {
         const bool alone = s.sequences == 1;                  // (then whatever its rows are)
         a.few_most = alone ? 0 : kFewMost;
         const cudaError_t e = launch_kv8_tiles(c, s, a, alone, work, st);
         if (e != cudaSuccess || alone) return e;
         ++dia::extra_launches();
     }
-#define KV8_FEW(DP, FORMAT) (two ? run_few<DP, FORMAT, 2>(c, s, a, work, st) : run_few<DP, FORMAT, 1>(c, s, a, work, st))
-    if (c.format == kKvE4m3) return dp == 64 ? KV8_FEW(64, kKvE4m3) : dp == 128 ? KV8_FEW(128, kKvE4m3) : KV8_FEW(256, kKvE4m3);
-    return dp == 64 ? KV8_FEW(64, kKvInt8) : dp == 128 ? KV8_FEW(128, kKvInt8) : KV8_FEW(256, kKvInt8);
-#undef KV8_FEW
+    if (c.format == kKvE4m3) return dp == 64 ? run_few<64, kKvE4m3>(c, s, a, work, st) : dp == 128 ? run_few<128, kKvE4m3>(c, s, a, work, st) : run_few<256, kKvE4m3>(c, s, a, work, st);
+    return dp == 64 ? run_few<64, kKvInt8>(c, s, a, work, st) : dp == 128 ? run_few<128, kKvInt8>(c, s, a, work, st) : run_few<256, kKvInt8>(c, s, a, work, st);
 }
 
 }  // namespace lm

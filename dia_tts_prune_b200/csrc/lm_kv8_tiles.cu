@@ -726,9 +726,9 @@ cudaError_t run_tiles(const Kv8Cache& c, const Kv8Step& s, const Kv8Attention& a
 
 }  // namespace
 
-bool kv8_tiles_ok(const Kv8Cache& c, int type) { return c.dim <= 128 && type != kTypeF32; }
+bool kv8_tiles_ok(int dim, int type) { return dim <= 128 && type != kTypeF32; }
 
-size_t kv8_tiles_work_bytes(const Kv8Cache& c) { return (size_t)kSms * kTileRows * ((c.dim <= 64 ? 64 : 128) * sizeof(float) + sizeof(RowStats)); }
+size_t kv8_tiles_work_bytes(int dim) { return (size_t)kSms * kTileRows * ((dim <= 64 ? 64 : 128) * sizeof(float) + sizeof(RowStats)); }
 
 cudaError_t launch_kv8_tiles(const Kv8Cache& c, const Kv8Step& s, const Kv8Attention& a, bool alone, void* work, cudaStream_t st) {
     if (c.dim <= 64) return c.format == kKvE4m3 ? run_tiles<64, kKvE4m3>(c, s, a, alone, work, st) : run_tiles<64, kKvInt8>(c, s, a, alone, work, st);

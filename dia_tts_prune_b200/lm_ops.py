@@ -9,6 +9,7 @@ any.  Arguments are checked on the host (``ValueError``, ``TypeError``); there i
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from functools import lru_cache
 
 import torch
@@ -86,6 +87,8 @@ def _as_rows(x: torch.Tensor) -> torch.Tensor:
 
 
 def _no_tangent(what: str, *xs: torch.Tensor) -> None:
+    if forward_ad._current_level < 0:                              # (nothing has a tangent outside of a forward-mode level; asking takes 1 us)
+        return
     for x in xs:
         if forward_ad.unpack_dual(x).tangent is not None:
             raise ValueError(f"{what} takes no forward-mode tangents")
@@ -329,7 +332,7 @@ class Kv8:
     device, so that a captured graph reads them anew) it describes the rows of a step: sequence ``i`` has rows ``first[i]`` to ``first[i + 1]`` of the
     packed ones, at positions ``past[i]`` and on; without ``first``, row ``i`` alone.  A token whose place lies beyond the table, or whose page is not
     in the pool, is not there: it is not written, not seen, and reads as zeros.  A sequence whose ``past`` is negative has no tokens."""
-    __slots__ = ("keys", "values", "key_scales", "value_scales", "pages", "kv_heads", "page_size", "dim", "format", "_handle")
+    __slots__ = ("keys", "values", "key_scales", "value_scales", "pages", "kv_heads", "page_size", "dim", "format", "_handle", "_at", "_index")
 
     def __init__(self, pages: int, kv_heads: int, dim: int, *, page_size: int = 16, format: str = "e4m3", device: torch.device | str = "cuda"):
         """Room for ``pages`` pages (1 <= dim <= 256; page_size 16, 32, 64 or 128), all zeros."""
@@ -347,6 +350,7 @@ class Kv8:
         self.key_scales, self.value_scales = (torch.zeros(shape[:2], dtype=torch.float32, device=device) for _ in range(2))
         self._handle = _lm_lib.Kv8(self.keys.data_ptr(), self.values.data_ptr(), self.key_scales.data_ptr(), self.value_scales.data_ptr(), self.pages,
                                    self.kv_heads, self.page_size, self.dim, _KV8_FORMATS[format])
+        self._at, self._index = C.addressof(self._handle), self.keys.get_device()
 
     @property
     def device(self) -> torch.device:
@@ -364,17 +368,21 @@ class Kv8:
         until then.  No page may belong to two sequences of a call."""
         _check_rows(k, "k")
         _check_rows(v, "v")
-        if k.dim() != 3 or k.shape[1] != self.kv_heads or k.shape[2] != self.dim or v.shape != k.shape or v.dtype != k.dtype:
+        shape = k.shape
+        if len(shape) != 3 or shape[1] != self.kv_heads or shape[2] != self.dim or v.shape != shape or v.dtype != k.dtype:
             raise ValueError(f"k {tuple(k.shape)} {k.dtype} and v {tuple(v.shape)} {v.dtype} must be [rows, {self.kv_heads}, {self.dim}] of one type")
         _no_grad("Kv8.append", k)
         _no_grad("Kv8.append", v)
-        step = _kv8_step(self, table, past, first, k.shape[0])
-        _check_device(self.keys.device, k, v)
+        step = _kv8_step(self, table, past, first, shape[0])
+        if not k.get_device() == v.get_device() == self._index >= 0:
+            _check_device(self.keys.device, k, v)
         if step is None:
             return
-        k, v = _neighbouring(k), _neighbouring(v)
-        _call("kv8_append", self.keys.device, C.addressof(self._handle), C.addressof(step), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
-              v.stride(1), _TYPES[k.dtype])
+        (k_row, k_head, k_step), (v_row, v_head, v_step) = k.stride(), v.stride()
+        if self.dim > 1 and (k_step != 1 or v_step != 1):
+            k, v = k.contiguous(), v.contiguous()
+            (k_row, k_head, _), (v_row, v_head, _) = k.stride(), v.stride()
+        _call("kv8_append", self.keys.device, self._at, step, k.data_ptr(), k_row, k_head, v.data_ptr(), v_row, v_head, _TYPES[k.dtype])
 
     def read(self, table: torch.Tensor, past: torch.Tensor, first: torch.Tensor | None, rows: int, dtype: torch.dtype = torch.float32) -> tuple[torch.Tensor, torch.Tensor]:
         """Keys and values ``[rows, kv_heads, dim]`` of the tokens at positions ``past[i]`` and on, as many as ``first`` gives sequence ``i`` rows.  Rows of no
@@ -385,45 +393,54 @@ class Kv8:
         if rows < 0:
             raise ValueError("rows must not be negative")
         step = _kv8_step(self, table, past, first, rows)
-        device = self.keys.device
-        k, v = (torch.empty((rows, self.kv_heads, self.dim), dtype=dtype, device=device) for _ in range(2))
+        k, v = self.key_scales.new_empty((2, rows, self.kv_heads, self.dim), dtype=dtype).unbind()
         if step is None:
             return k.zero_(), v.zero_()
-        _call("kv8_read", device, C.addressof(self._handle), C.addressof(step), k.data_ptr(), v.data_ptr(), _TYPES[dtype])
+        _call("kv8_read", self.keys.device, self._at, step, k.data_ptr(), v.data_ptr(), _TYPES[dtype])
         return k, v
 
 
-def _neighbouring(x: torch.Tensor) -> torch.Tensor:
-    return x if x.shape[-1] == 1 or x.stride(-1) == 1 else x.contiguous()
+# lm_b200_kv8_step: table, table_ld, past, first, max_pages, n_seq, rows (a ctypes structure takes 1 us more)
+_KV8_STEP = struct.Struct("@PqPPiii")
 
 
-def _kv8_step(cache: Kv8, table: torch.Tensor, past: torch.Tensor, first: torch.Tensor | None, rows: int):
+def _kv8_step(cache: Kv8, table: torch.Tensor, past: torch.Tensor, first: torch.Tensor | None, rows: int) -> bytes | None:
     """The description of a step's rows as the library takes it (None: no row of any sequence)."""
     for name, t in (("table", table), ("past", past), ("first", first)):
         if t is None and name == "first":
             continue
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{name} must be a tensor")
-        if t.dtype != torch.int32:
+        if t.dtype is not torch.int32:
             raise TypeError(f"{name} must be int32, not {t.dtype}")
-    if table.dim() != 2 or (table.shape[1] > 1 and table.stride(1) != 1):
-        raise ValueError("table must be [sequences, pages of one] with neighbouring page numbers")
-    n = table.shape[0]
-    if past.dim() != 1 or past.shape[0] != n or not past.is_contiguous():
+    if table.dim() != 2:
+        raise ValueError("table must be [sequences, pages of one]")
+    (n, width), (apart, step) = table.shape, table.stride()
+    if width > 1 and step != 1:
+        raise ValueError("table must have a sequence's page numbers beside one another")
+    if past.shape != (n,) or not past.is_contiguous():
         raise ValueError(f"past must hold one number for each of {n} sequences")
+    index = cache._index
     if first is None:
         if rows != n:
             raise ValueError(f"{rows} rows of {n} sequences need first")
-        _check_device(cache.keys.device, table, past)
+        if not table.get_device() == past.get_device() == index >= 0:
+            _check_device(cache.keys.device, table, past)
     else:
-        if first.dim() != 1 or first.shape[0] != n + 1 or not first.is_contiguous():
+        if first.shape != (n + 1,) or not first.is_contiguous():
             raise ValueError(f"first must hold {n + 1} numbers")
-        _check_device(cache.keys.device, table, past, first)
+        if not table.get_device() == past.get_device() == first.get_device() == index >= 0:
+            _check_device(cache.keys.device, table, past, first)
     if rows > 0x7fffff00:
         raise ValueError(f"{rows} rows are more than an operator takes")
-    if not (n and rows and table.shape[1]):
+    if not (n and rows and width):
         return None
-    return _lm_lib.Kv8Step(table.data_ptr(), table.stride(0), past.data_ptr(), None if first is None else first.data_ptr(), table.shape[1], n, rows)
+    return _KV8_STEP.pack(table.data_ptr(), apart, past.data_ptr(), 0 if first is None else first.data_ptr(), width, n, rows)
+
+
+@lru_cache(maxsize=1024)
+def _kv8_work_bytes(kv_heads: int, dim: int, rows: int, heads: int, kind: int) -> int:
+    return _lm_lib.load().lm_b200_op_kv8_attention_work_bytes(kv_heads, dim, rows, heads, kind)
 
 
 def attention_kv8(q: torch.Tensor, cache: Kv8, table: torch.Tensor, past: torch.Tensor, first: torch.Tensor | None = None, *, scale: float | None = None,
@@ -439,32 +456,38 @@ def attention_kv8(q: torch.Tensor, cache: Kv8, table: torch.Tensor, past: torch.
     _check_rows(q, "q")
     if not isinstance(cache, Kv8):
         raise TypeError("cache must be a Kv8")
-    if q.dim() != 3 or q.shape[2] != cache.dim or not q.shape[1] or q.shape[1] % cache.kv_heads or q.shape[1] > 4096:
-        raise ValueError(f"q {tuple(q.shape)} does not go with {cache.kv_heads} key heads of {cache.dim}")
+    shape = q.shape
+    if len(shape) != 3 or shape[2] != cache.dim or not shape[1] or shape[1] % cache.kv_heads or shape[1] > 4096:
+        raise ValueError(f"q {tuple(shape)} does not go with {cache.kv_heads} key heads of {cache.dim}")
     scale = cache.dim ** -0.5 if scale is None else float(scale)
     if not 2.0 ** -126 <= scale <= 2.0 ** 126:
         raise ValueError("scale must be positive, from 2 ** -126 to 2 ** 126")
-    if window is not None and not 1 <= int(window) < 1 << 31:
+    if window is None:
+        window = 0
+    elif not 1 <= (window := int(window)) < 1 << 31:
         raise ValueError("window must be positive")
     _no_grad("attention_kv8", q)
-    rows, heads, device = q.shape[0], q.shape[1], cache.keys.device
+    rows, heads, _ = shape
     step = _kv8_step(cache, table, past, first, rows)
-    _check_device(device, q)
+    if not q.get_device() == cache._index >= 0:
+        _check_device(cache.keys.device, q)
     if sinks is not None:
         _check_rows(sinks, "sinks", (torch.float32,))
         if sinks.shape != (heads,):
             raise ValueError(f"sinks must hold one number for each of {heads} heads")
-        _check_device(device, sinks)
+        _check_device(cache.keys.device, sinks)
         sinks = sinks.contiguous()
-    if rows > (0x7fffff00 // heads):
+    if rows > 0x7fffff00 // heads:
         raise ValueError(f"{rows} rows of {heads} heads are more than an operator takes")
     if step is None:
-        return q.new_zeros(q.shape)
-    out = q.new_empty(q.shape)
-    q = _neighbouring(q)
-    handle, rows_at = C.addressof(cache._handle), C.addressof(step)
-    need = _function("kv8_attention_work_bytes")(handle, rows_at, heads, _TYPES[q.dtype])
-    work = q.new_empty(need, dtype=torch.uint8)
-    _call("kv8_attention", device, handle, rows_at, q.data_ptr(), q.stride(0), q.stride(1), heads, _TYPES[q.dtype], scale, int(window or 0),
-          None if sinks is None else sinks.data_ptr(), out.data_ptr(), work.data_ptr(), need)
+        return q.new_zeros(shape)
+    q_row, q_head, q_step = q.stride()
+    if q_step != 1 and cache.dim > 1:
+        q = q.contiguous()
+        q_row, q_head, _ = q.stride()
+    kind = _TYPES[q.dtype]
+    need = _kv8_work_bytes(cache.kv_heads, cache.dim, rows, heads, kind)
+    out, work = q.new_empty(shape), q.new_empty(need, dtype=torch.uint8)
+    _call("kv8_attention", cache.keys.device, cache._at, step, q.data_ptr(), q_row, q_head, heads, kind, scale, window, None if sinks is None else sinks.data_ptr(),
+          out.data_ptr(), work.data_ptr(), need)
     return out
