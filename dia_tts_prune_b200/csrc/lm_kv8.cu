@@ -256,7 +256,7 @@ struct Few {
     static constexpr int kRing = kWarps * kStages * 2 * kSide;
     static constexpr int kQ = TERMS * NT * (DP / 16) * 32 * 8;                    // fragments of the queries
     static constexpr int kSums = kWarps * kRows * DP * 4;                         // (where the ring lies)
-    static constexpr int kSmem = (kRing > kSums ? kRing : kSums) + kQ + kMetaBlocks * 12 + kRows * 4 + kWarps * kRows * 12 + 128;
+    static constexpr int kSmem = (kRing > kSums ? kRing : kSums) + kQ + kMetaBlocks * 16 + kRows * 4 + kWarps * kRows * 12 + 128;
 };
 constexpr int kFewCtas = 148, kJoinThreads = 512;
 
@@ -353,15 +353,17 @@ __global__ void __launch_bounds__(Few<DP, TERMS, NT>::kThreads, 1) kv8_attention
     uint8_t* const ring = smem + (threadIdx.x >> 5) * (F::kStages * 2 * F::kSide);
     float* const sums = reinterpret_cast<float*>(smem);                            // [warps][rows][DP], when the ring is empty
     uint2* const q_frags = reinterpret_cast<uint2*>(smem + (F::kRing > F::kSums ? F::kRing : F::kSums));
-    int* const meta_page = reinterpret_cast<int*>(q_frags + F::kQ / 8);
-    float* const meta_ks = reinterpret_cast<float*>(meta_page + kMetaBlocks);
-    float* const meta_ev = meta_ks + kMetaBlocks;
-    float* const row_scale = meta_ev + kMetaBlocks;                                // [rows] of the queries, with the scores' scale
+    long long* const meta_at = reinterpret_cast<long long*>(q_frags + F::kQ / 8);  // where a block's codes lie; -1: it is not there
+    float2* const meta = reinterpret_cast<float2*>(meta_at + kMetaBlocks);         // (key scale, exponent of the values)
+    float* const row_scale = reinterpret_cast<float*>(meta + kMetaBlocks);         // [rows] of the queries, with the scores' scale
     RowStats* const stats = reinterpret_cast<RowStats*>(row_scale + kRows);        // [warps][rows]
     __shared__ Place place;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, group = a.heads / c.kv_heads;
+    // a lane's pieces of 16 bytes: row lane / (DP / 16) and so on, where they go, and whether rows have them (zeros come in their place)
+    const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring), swizzled = piece_at<DP>(lane / (DP / 16), lane % (DP / 16));
+    const int lane_bytes = lane % (DP / 16) * 16 < c.stride ? 16 : 0, lane_off = lane / (DP / 16) * c.stride + (lane_bytes ? lane % (DP / 16) * 16 : 0);
     if (warp == 0) {
         const Place found = find_place<kRows>(s, a, c.kv_heads, group, c.page_shift, kWarps, blockIdx.x);
         if (lane == 0) place = found;
@@ -394,26 +396,27 @@ __global__ void __launch_bounds__(Few<DP, TERMS, NT>::kThreads, 1) kv8_attention
                 const long long tok = token(m_at + i);
                 int page = -1;
                 if (sp.past >= 0 && tok <= pos_b && tok + kKvBlock > seen_from) page = s.page(at.seq, tok >> c.page_shift, c.pages);
-                meta_page[i] = page;
                 if (page >= 0) {
                     const size_t ph = (size_t)page * c.kv_heads + head;
                     const uint32_t vs = __float_as_uint(c.value_scales[ph]);
-                    meta_ks[i] = c.key_scales[ph];
-                    meta_ev[i] = vs >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : (float)((int)(vs >> 23) - 127);
+                    meta_at[i] = (long long)(((ph << c.page_shift) + (size_t)(tok & ((1 << c.page_shift) - 1))) * c.stride);
+                    meta[i] = make_float2(c.key_scales[ph], vs >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : (float)((int)(vs >> 23) - 127));
+                } else {
+                    meta_at[i] = -1;
                 }
             }
         };
-        const auto issue = [&](int m_at, int m_n, int i, int stage) {                // block i of the list into a slot of the ring
-            if (i < m_n && meta_page[i] >= 0) {
-                const size_t from = ((((size_t)meta_page[i] * c.kv_heads + head) << c.page_shift) + (size_t)(token(m_at + i) & ((1 << c.page_shift) - 1))) * c.stride;
-                const uint32_t to = (uint32_t)__cvta_generic_to_shared(ring + stage * 2 * F::kSide);
+        const auto issue = [&](int m_n, int i, int stage) {                          // block i of the list into a slot of the ring
+            const long long from = i < m_n ? meta_at[i] : -1;
+            if (from >= 0) {
+                const uint32_t to = ring_at + stage * 2 * F::kSide;
 #pragma unroll
                 for (int j = 0; j < DP / 32; ++j) {
-                    const int x = lane + 32 * j, r = x / (DP / 16), p = x % (DP / 16), n = p * 16 < c.stride ? 16 : 0;
-                    const size_t off = from + (size_t)r * c.stride + (n ? p * 16 : 0);
-                    const uint32_t d = to + piece_at<DP>(r, p);
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(c.keys + off), "r"(n) : "memory");
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d + F::kSide), "l"(c.values + off), "r"(n) : "memory");
+                    // (a lane's pieces lie 32 on from one to the next: the swizzle differs by what it does to those bits of the row)
+                    const uint32_t d = to + 512 * j + (DP == 64 ? swizzled : DP == 128 ? swizzled ^ ((j & 1) << 6) : swizzled ^ ((j & 1) << 5) ^ ((j & 2) << 5));
+                    const size_t off = (size_t)from + (uint32_t)(lane_off + j * (512 / DP) * c.stride);
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(c.keys + off), "r"(lane_bytes) : "memory");
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d + F::kSide), "l"(c.values + off), "r"(lane_bytes) : "memory");
                 }
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
@@ -476,17 +479,17 @@ __global__ void __launch_bounds__(Few<DP, TERMS, NT>::kThreads, 1) kv8_attention
                 __syncthreads();
             }
 #pragma unroll 1
-            for (int j = 0; j < F::kStages - 1; ++j) issue(m_at, m_n, warp + kWarps * j, j);
+            for (int j = 0; j < F::kStages - 1; ++j) issue(m_n, warp + kWarps * j, j);
             int stage = 0;
 #pragma unroll 1
             for (int i = warp; i < m_n; i += kWarps) {
                 asm volatile("cp.async.wait_group %0;" ::"n"(F::kStages - 2) : "memory");
                 __syncwarp();                                                        // the block is there for every lane, and the slot in front has been read by all
-                issue(m_at, m_n, i + kWarps * (F::kStages - 1), stage == 0 ? F::kStages - 1 : stage - 1);
+                issue(m_n, i + kWarps * (F::kStages - 1), stage == 0 ? F::kStages - 1 : stage - 1);
                 const uint8_t* const keys = ring + stage * 2 * F::kSide;
                 const uint8_t* const values = keys + F::kSide;
                 stage = stage + 1 == F::kStages ? 0 : stage + 1;
-                if (meta_page[i] < 0) continue;
+                if (meta_at[i] < 0) continue;
 
                 // scores: token g of row 2 t and of row 2 t + 1, token g + 8 of either
                 float x[NT][4], rest[TERMS == 2 ? NT : 1][4];
@@ -511,7 +514,7 @@ __global__ void __launch_bounds__(Few<DP, TERMS, NT>::kThreads, 1) kv8_attention
                         }
                     }
                 }
-                const float ks = meta_ks[i], ev = meta_ev[i];
+                const float ks = meta[i].x, ev = meta[i].y;
                 const long long tok = token(m_at + i);
                 const bool clear = tok + kKvBlock - 1 <= pos_a && tok >= clear_from;   // every row sees all of the block
                 uint2 hi[NT], lo[TERMS == 2 ? NT : 1];
