@@ -233,7 +233,7 @@ __global__ void __launch_bounds__(kReadThreads) kv8_read_kernel(Kv8Cache c, Kv8S
 // x = scale log2(e) q . key in powers of two, p = 2^(x - max x), o = sum p value / (sum p + 2^(sink log2(e) - max x)).
 //
 // What bounds it is the cache's bytes.  The rows of a tile (8, or 16) are (token, query head) pairs that share a key head, so a token's codes are read once for the group; tiles of
-// a sequence lie next to one another in the order of the work.  Work is counted in blocks of 16 tokens over all sequences, heads and tiles and dealt to the CTAs, one on each SM, in
+// a sequence lie next to one another in the order of the work.  Work is counted in blocks of 16 tokens over all sequences, heads and tiles and dealt to the CTAs in
 // equal runs, so that one long sequence fills the GPU and lengths need not be alike; runs that share a tile leave (max, sum, output) and a second kernel joins them, always in the
 // same order.
 //
@@ -250,15 +250,17 @@ constexpr int kMetaBlocks = 256;
 
 template <int DP, int TERMS, int NT>
 struct Few {
-    static constexpr int kWarps = TERMS == 2 || DP == 256 ? 8 : NT == 1 ? 16 : 12, kThreads = 32 * kWarps, kRows = 8 * NT;
+    // Two CTAs on an SM where registers allow: one computes while the other is between two tiles
+    static constexpr int kPerSm = TERMS == 2 || DP == 256 ? 1 : 2, kCtas = 148 * kPerSm;
+    static constexpr int kWarps = kPerSm == 1 ? 8 : NT == 1 ? 8 : 6, kThreads = 32 * kWarps, kRows = 8 * NT;
     static constexpr int kSide = kKvBlock * DP;               // bytes of a block's keys, or values
-    static constexpr int kStages = 192 * 1024 / (kWarps * 2 * kSide) > 8 ? 8 : 192 * 1024 / (kWarps * 2 * kSide);
+    static constexpr int kStages = 192 * 1024 / kPerSm / (kWarps * 2 * kSide) > 8 ? 8 : 192 * 1024 / kPerSm / (kWarps * 2 * kSide);
     static constexpr int kRing = kWarps * kStages * 2 * kSide;
     static constexpr int kQ = TERMS * NT * (DP / 16) * 32 * 8;                    // fragments of the queries
     static constexpr int kSums = kWarps * kRows * DP * 4;                         // (where the ring lies)
     static constexpr int kSmem = (kRing > kSums ? kRing : kSums) + kQ + kMetaBlocks * 16 + kRows * 4 + kWarps * kRows * 12 + 128;
 };
-constexpr int kFewCtas = 148, kJoinThreads = 512;
+constexpr int kMostCtas = 2 * 148, kJoinThreads = 512;
 
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint2 b) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -308,7 +310,7 @@ struct Place {
     long long base, per, total;
 };
 template <int ROWS>
-__device__ __forceinline__ Place find_place(const Kv8Step& s, const Kv8Attention& a, int kv_heads, int group, int page_shift, int warps, int nth) {
+__device__ __forceinline__ Place find_place(const Kv8Step& s, const Kv8Attention& a, int kv_heads, int group, int page_shift, int ctas, int warps, int nth) {
     const int lane = threadIdx.x & 31, each = (s.sequences + 31) / 32, i0 = lane * each, i1 = min(i0 + each, s.sequences);
     long long mine = 0;
     int longest = 0;
@@ -326,7 +328,7 @@ __device__ __forceinline__ Place find_place(const Kv8Step& s, const Kv8Attention
     }
     Place place;
     place.total = __shfl_sync(0xffffffffu, upto, 31);
-    place.per = max((place.total + kFewCtas - 1) / kFewCtas, (long long)max(min(warps, longest), 1));
+    place.per = max((place.total + ctas - 1) / ctas, (long long)max(min(warps, longest), 1));
     place.seq = -1;
     place.base = upto - mine;
     const long long unit = place.per * nth;
@@ -346,7 +348,7 @@ __device__ __forceinline__ Place find_place(const Kv8Step& s, const Kv8Attention
 }
 
 template <int DP, int FORMAT, int TERMS, int NT>
-__global__ void __launch_bounds__(Few<DP, TERMS, NT>::kThreads, 1) kv8_attention_few_kernel(Kv8Cache c, Kv8Step s, Kv8Attention a, float* part, RowStats* part_stats) {
+__global__ void __launch_bounds__(Few<DP, TERMS, NT>::kThreads, Few<DP, TERMS, NT>::kPerSm) kv8_attention_few_kernel(Kv8Cache c, Kv8Step s, Kv8Attention a, float* part, RowStats* part_stats) {
     using F = Few<DP, TERMS, NT>;
     constexpr int kSteps = DP / 16, kHalves = DP == 256 ? 2 : 1, kWords = DP == 64 ? 2 : 4, kCols = kHalves * kWords * 2, kWarps = F::kWarps, kRows = F::kRows;
     extern __shared__ __align__(128) uint8_t smem[];
@@ -365,7 +367,7 @@ __global__ void __launch_bounds__(Few<DP, TERMS, NT>::kThreads, 1) kv8_attention
     const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring), swizzled = piece_at<DP>(lane / (DP / 16), lane % (DP / 16));
     const int lane_bytes = lane % (DP / 16) * 16 < c.stride ? 16 : 0, lane_off = lane / (DP / 16) * c.stride + (lane_bytes ? lane % (DP / 16) * 16 : 0);
     if (warp == 0) {
-        const Place found = find_place<kRows>(s, a, c.kv_heads, group, c.page_shift, kWarps, blockIdx.x);
+        const Place found = find_place<kRows>(s, a, c.kv_heads, group, c.page_shift, F::kCtas, kWarps, blockIdx.x);
         if (lane == 0) place = found;
     }
     zero_rows_of_none(s, a, c.dim, (long long)blockIdx.x * F::kThreads + threadIdx.x, (long long)gridDim.x * F::kThreads);
@@ -665,7 +667,7 @@ __global__ void __launch_bounds__(Few<DP, TERMS, NT>::kThreads, 1) kv8_attention
 
 // A tile that several runs share: a CTA per border between runs, and per row.  The first border inside the tile joins it.
 template <int DP, int NT>
-__global__ void __launch_bounds__(kJoinThreads) kv8_attention_join_kernel(Kv8Cache c, Kv8Step s, Kv8Attention a, int warps, const float* part, const RowStats* part_stats) {
+__global__ void __launch_bounds__(kJoinThreads) kv8_attention_join_kernel(Kv8Cache c, Kv8Step s, Kv8Attention a, int ctas, int warps, const float* part, const RowStats* part_stats) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     constexpr int kRows = 8 * NT, kWarps = kJoinThreads / 32, kEach = DP / 32;
     __shared__ __align__(16) float sums[kWarps][DP];
@@ -673,7 +675,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv8_attention_join_kernel(Kv8Cac
     __shared__ Place place;
     const int nth = blockIdx.x + 1, r = blockIdx.y, group = a.heads / c.kv_heads, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (warp == 0) {
-        const Place found = find_place<kRows>(s, a, c.kv_heads, group, c.page_shift, warps, nth);
+        const Place found = find_place<kRows>(s, a, c.kv_heads, group, c.page_shift, ctas, warps, nth);
         if (lane == 0) place = found;
     }
     __syncthreads();
@@ -729,13 +731,13 @@ cudaError_t run_few(const Kv8Cache& c, const Kv8Step& s, const Kv8Attention& a, 
     e = dia::ask_smem<kv8_attention_few_kernel<DP, FORMAT, TERMS, NT>>(dev, F::kSmem);
     if (e != cudaSuccess) return e;
     float* const part = reinterpret_cast<float*>(work);
-    RowStats* const stats = reinterpret_cast<RowStats*>(part + (size_t)2 * kFewCtas * F::kRows * DP);
-    kv8_attention_few_kernel<DP, FORMAT, TERMS, NT><<<kFewCtas, F::kThreads, F::kSmem, st>>>(c, s, a, part, stats);
+    RowStats* const stats = reinterpret_cast<RowStats*>(part + (size_t)2 * F::kCtas * F::kRows * DP);
+    kv8_attention_few_kernel<DP, FORMAT, TERMS, NT><<<F::kCtas, F::kThreads, F::kSmem, st>>>(c, s, a, part, stats);
     e = cudaGetLastError();
     if (e != cudaSuccess) return e;
     ++dia::extra_launches();
     const int most = (int)std::min<long long>(F::kRows, (long long)s.rows * (a.heads / c.kv_heads));
-    return launch_pdl(kv8_attention_join_kernel<DP, NT>, dim3(kFewCtas - 1, most), dim3(kJoinThreads), 0, st, c, s, a, (int)F::kWarps, part, stats);
+    return launch_pdl(kv8_attention_join_kernel<DP, NT>, dim3(F::kCtas - 1, most), dim3(kJoinThreads), 0, st, c, s, a, (int)F::kCtas, (int)F::kWarps, part, stats);
 }
 template <int DP, int FORMAT>
 cudaError_t run_few(const Kv8Cache& c, const Kv8Step& s, const Kv8Attention& a, void* work, cudaStream_t st) {
@@ -781,7 +783,7 @@ inline bool some_in_tiles(int kv_heads, int dim, int rows, int heads, int type) 
 
 size_t kv8_attention_work_bytes(int kv_heads, int dim, int rows, int heads, int type) {
     const int dp = padded_dim(dim);
-    const size_t few = (size_t)2 * kFewCtas * 16 * (dp * sizeof(float) + sizeof(RowStats));
+    const size_t few = (size_t)2 * kMostCtas * 16 * (dp * sizeof(float) + sizeof(RowStats));
     return some_in_tiles(kv_heads, dim, rows, heads, type) ? std::max(few, kv8_tiles_work_bytes(dim)) : few;
 }
 
