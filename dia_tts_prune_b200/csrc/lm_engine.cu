@@ -1864,7 +1864,7 @@ int lm_b200_op_kv8_attention(const lm_b200_kv8* cache, const lm_b200_kv8_step* s
     if (!kv8_cache(c, cache) || !kv8_step(s, step) || !kv8_heads(c.kv_heads, s.rows, heads) || !q || q_row < 0 || q_head < 0 || !known_type(type) || !loss_scale(scale) || window < 0 || !out || !work ||
         !aligned(work, 256) || work_bytes < lm::kv8_attention_work_bytes(c.kv_heads, c.dim, s.rows, heads, type))
         return LM_B200_EINVAL;
-    LCK(lm::launch_kv8_attention(c, s, lm::Kv8Attention{lm::Kv8Rows{q, q_row, q_head}, out, heads, type, scale, window, sinks, 0}, work, S(stream)));
+    LCK(lm::launch_kv8_attention(c, s, lm::Kv8Attention{lm::Kv8Rows{q, q_row, q_head}, out, heads, type, scale, window, sinks, 0, 0}, work, S(stream)));
     return LM_B200_OK;
 }
 

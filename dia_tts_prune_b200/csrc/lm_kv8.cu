@@ -234,8 +234,8 @@ __global__ void __launch_bounds__(kReadThreads) kv8_read_kernel(Kv8Cache c, Kv8S
 //
 // What bounds it is the cache's bytes.  The rows of a tile (8, or 16) are (token, query head) pairs that share a key head, so a token's codes are read once for the group; tiles of
 // a sequence lie next to one another in the order of the work.  Work is counted in blocks of 16 tokens over all sequences, heads and tiles and dealt to the CTAs in
-// equal runs, so that one long sequence fills the GPU and lengths need not be alike; runs that share a tile leave (max, sum, output) and a second kernel joins them, always in the
-// same order.
+// equal runs, so that one long sequence fills the GPU and lengths need not be alike; runs that share a tile leave (max, sum, output), and the last one to come joins them, always in
+// the same order (a second kernel for that took 6 us after one request's 1024 tokens, 11 after 131072, 26 after 64 requests).
 //
 // A warp keeps its own ring of blocks in shared memory, filled by asynchronous copies that swizzle 16-byte pieces (rows lie 128 bytes apart, which would be the same banks), and
 // multiplies on the tensor cores (mma.sync, 16 x 8 x 16: a block's 16 tokens, or 16 channels of their values, by eight rows: what a group has, and nothing is waited for across warps).
@@ -257,10 +257,10 @@ struct Few {
     static constexpr int kStages = 192 * 1024 / kPerSm / (kWarps * 2 * kSide) > 8 ? 8 : 192 * 1024 / kPerSm / (kWarps * 2 * kSide);
     static constexpr int kRing = kWarps * kStages * 2 * kSide;
     static constexpr int kQ = TERMS * NT * (DP / 16) * 32 * 8;                    // fragments of the queries
-    static constexpr int kSums = kWarps * kRows * DP * 4;                         // (where the ring lies)
+    static constexpr int kSums = kWarps * kRows * DP * 4 + kCtas * kRows * 4;     // and the weights of runs that share a tile (where the ring lies)
     static constexpr int kSmem = (kRing > kSums ? kRing : kSums) + kQ + kMetaBlocks * 16 + kRows * 4 + kWarps * kRows * 12 + 128;
 };
-constexpr int kMostCtas = 2 * 148, kJoinThreads = 512;
+constexpr int kMostCtas = 2 * 148;
 
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint2 b) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -287,8 +287,8 @@ __device__ __forceinline__ int piece_at(int r, int c) {
 
 // Blocks of 16 tokens that a sequence's rows look at, and its share of the work
 struct Span {
-    int begin, n, past, low, blocks, tiles;                   // low: the first block
-    __device__ __forceinline__ long long units(int kv_heads) const { return (long long)kv_heads * tiles * blocks; }
+    int begin, n, past, low, blocks, tiles, share;            // low: the first block; share: units of work in a tile: its blocks, or 1 where none is shared
+    __device__ __forceinline__ long long units(int kv_heads) const { return (long long)kv_heads * tiles * share; }
 };
 template <int ROWS>
 __device__ __forceinline__ Span span_of(const Kv8Step& s, const Kv8Attention& a, int i, int group, int page_shift) {
@@ -300,6 +300,7 @@ __device__ __forceinline__ Span span_of(const Kv8Step& s, const Kv8Attention& a,
     const long long end = min((long long)max(p.past, 0) + p.n, (long long)s.max_pages << page_shift);
     p.blocks = max(1, (int)((end + kKvBlock - 1) / kKvBlock) - p.low);
     p.tiles = (long long)p.n * group > a.few_most ? 0 : (p.n * group + ROWS - 1) / ROWS;
+    p.share = a.whole ? 1 : p.blocks;
     return p;
 }
 
@@ -317,7 +318,7 @@ __device__ __forceinline__ Place find_place(const Kv8Step& s, const Kv8Attention
     for (int i = i0; i < i1; ++i) {
         const Span p = span_of<ROWS>(s, a, i, group, page_shift);
         mine += p.units(kv_heads);
-        if (p.tiles) longest = max(longest, p.blocks);
+        if (p.tiles) longest = max(longest, p.share);
     }
     longest = (int)__reduce_max_sync(0xffffffffu, (unsigned)longest);
     long long upto = mine;
@@ -348,7 +349,7 @@ __device__ __forceinline__ Place find_place(const Kv8Step& s, const Kv8Attention
 }
 
 template <int DP, int FORMAT, int TERMS, int NT>
-__global__ void __launch_bounds__(Few<DP, TERMS, NT>::kThreads, Few<DP, TERMS, NT>::kPerSm) kv8_attention_few_kernel(Kv8Cache c, Kv8Step s, Kv8Attention a, float* part, RowStats* part_stats) {
+__global__ void __launch_bounds__(Few<DP, TERMS, NT>::kThreads, Few<DP, TERMS, NT>::kPerSm) kv8_attention_few_kernel(Kv8Cache c, Kv8Step s, Kv8Attention a, float* part, RowStats* part_stats, unsigned* arrived) {
     using F = Few<DP, TERMS, NT>;
     constexpr int kSteps = DP / 16, kHalves = DP == 256 ? 2 : 1, kWords = DP == 64 ? 2 : 4, kCols = kHalves * kWords * 2, kWarps = F::kWarps, kRows = F::kRows;
     extern __shared__ __align__(128) uint8_t smem[];
@@ -360,7 +361,7 @@ __global__ void __launch_bounds__(Few<DP, TERMS, NT>::kThreads, Few<DP, TERMS, N
     float* const row_scale = reinterpret_cast<float*>(meta + kMetaBlocks);         // [rows] of the queries, with the scores' scale
     RowStats* const stats = reinterpret_cast<RowStats*>(row_scale + kRows);        // [warps][rows]
     __shared__ Place place;
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    __shared__ int last;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, group = a.heads / c.kv_heads;
     // a lane's pieces of 16 bytes: row lane / (DP / 16) and so on, where they go, and whether rows have them (zeros come in their place)
@@ -373,21 +374,20 @@ __global__ void __launch_bounds__(Few<DP, TERMS, NT>::kThreads, Few<DP, TERMS, N
     zero_rows_of_none(s, a, c.dim, (long long)blockIdx.x * F::kThreads + threadIdx.x, (long long)gridDim.x * F::kThreads);
     __syncthreads();
     Place at = place;
-    if (at.seq < 0) return;
-    long long unit = at.per * blockIdx.x;
+    long long unit = at.seq < 0 ? at.total : at.per * blockIdx.x;
     const long long unit_end = min(unit + at.per, at.total);
-    Span sp = span_of<kRows>(s, a, at.seq, group, c.page_shift);
+    Span sp = span_of<kRows>(s, a, max(at.seq, 0), group, c.page_shift);
 
     while (unit < unit_end) {
         while (unit >= at.base + sp.units(c.kv_heads)) {                             // (sequences without rows have no units)
             at.base += sp.units(c.kv_heads);
             sp = span_of<kRows>(s, a, ++at.seq, group, c.page_shift);
         }
-        const long long item = (unit - at.base) / sp.blocks;
-        const int b0 = (int)(unit - at.base - item * sp.blocks), count = (int)min((long long)sp.blocks - b0, unit_end - unit);
+        const long long item = (unit - at.base) / sp.share;
+        const int b0 = (int)(unit - at.base - item * sp.share), taken = (int)min((long long)sp.share - b0, unit_end - unit), count = a.whole ? sp.blocks : taken;
         const int head = (int)(item / sp.tiles), tile = (int)(item - (long long)head * sp.tiles);
         const int p0 = tile * kRows, rows = min(kRows, sp.n * group - p0);
-        unit += count;
+        unit += taken;
         // positions of the tile's rows, first and last
         const auto position = [&](int r) { return (long long)sp.past + (p0 + min(r, rows - 1)) / group; };
         const long long back = a.window > 0 ? a.window - 1 : (1ll << 40);
@@ -630,121 +630,139 @@ __global__ void __launch_bounds__(Few<DP, TERMS, NT>::kThreads, Few<DP, TERMS, N
             }
         __syncthreads();
         const bool whole = b0 == 0 && count == sp.blocks;
-        const size_t slot = 2 * (size_t)blockIdx.x + (b0 == 0);
-        for (int i = threadIdx.x; i < rows * (DP / 4); i += F::kThreads) {
-            const int r = i / (DP / 4), d = i % (DP / 4) * 4;
-            float mm = -INFINITY, ww = -INFINITY, ll = 0.f;
+        const auto write = [&](int r, int d, float f, const float4& sum) {
+            const int p = p0 + r, h = head * group + p % group;
+            const size_t to = ((size_t)(sp.begin + p / group) * a.heads + h) * c.dim + d;
+            const float y[4] = {sum.x, sum.y, sum.z, sum.w};
 #pragma unroll
-            for (int v = 0; v < kWarps; ++v) {
-                mm = fmaxf(mm, stats[v * kRows + r].m);
-                ww = fmaxf(ww, stats[v * kRows + r].w);
+            for (int e = 0; e < 4; ++e)
+                if (d + e < c.dim) store_out(a, to + e, f * y[e]);
+        };
+        // sums of `n` parts of row r below their common maxima, channels d to d + 3
+        const auto meet = [&](int n, const RowStats* of, const float* from, int stride, int r, int d, RowStats& top) {
+            top = {-INFINITY, -INFINITY, 0.f};
+            for (int v = 0; v < n; ++v) {
+                top.m = fmaxf(top.m, of[v * stride + r].m);
+                top.w = fmaxf(top.w, of[v * stride + r].w);
             }
             float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-            for (int v = 0; v < kWarps; ++v) {
-                const RowStats y = stats[v * kRows + r];
-                const float f = lower_to(y.w, ww);
-                const float4 z = *reinterpret_cast<const float4*>(sums + (size_t)(v * kRows + r) * DP + d);
-                ll += y.l * lower_to(y.m, mm);
+            for (int v = 0; v < n; ++v) {
+                const RowStats y = of[v * stride + r];
+                const float f = lower_to(y.w, top.w);
+                const float4 z = *reinterpret_cast<const float4*>(from + (size_t)(v * stride + r) * DP + d);
+                top.l += y.l * lower_to(y.m, top.m);
                 sum.x += f * z.x; sum.y += f * z.y; sum.z += f * z.z; sum.w += f * z.w;
             }
+            return sum;
+        };
+        const int tasks = rows * (DP / 4);
+        const size_t slot = 2 * (size_t)blockIdx.x + (b0 == 0);
+        for (int i = threadIdx.x; i < tasks; i += F::kThreads) {
+            const int r = i / (DP / 4), d = i % (DP / 4) * 4;
+            RowStats top;
+            const float4 sum = meet(kWarps, stats, sums, kRows, r, d, top);
             if (whole) {
-                const int p = p0 + r, h = head * group + p % group;
-                const float f = row_factor(a, h, mm, ww, ll);
-                const size_t to = ((size_t)(sp.begin + p / group) * a.heads + h) * c.dim + d;
-                const float y[4] = {sum.x, sum.y, sum.z, sum.w};
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (d + e < c.dim) store_out(a, to + e, f * y[e]);
+                write(r, d, row_factor(a, head * group + (p0 + r) % group, top.m, top.w, top.l), sum);
             } else {
                 *reinterpret_cast<float4*>(part + (slot * kRows + r) * DP + d) = sum;
-                if (d == 0) part_stats[slot * kRows + r] = {mm, ww, ll};
+                if (d == 0) part_stats[slot * kRows + r] = top;
+            }
+        }
+        if (!whole) {
+            // Runs c0 to c1 share the tile; the last of them to come joins all, in their order.  (A run is the first one of at most one shared tile, whose counter it lends.)
+            const long long start = at.base + item * sp.share;
+            const int c0 = (int)(start / at.per), c1 = (int)((start + sp.share - 1) / at.per);
+            __threadfence();
+            __syncthreads();
+            if (threadIdx.x == 0) last = atomicAdd(arrived + c0, 1u) == (unsigned)(c1 - c0);
+            __syncthreads();
+            if (last) {
+                __threadfence();
+                // rows' weights of the runs first, where the rings lay, then their channels; threads that these leave over take runs of their own
+                float* const weights = sums + kWarps * kRows * DP;                   // [run][row]
+                const int n = c1 - c0 + 1, groups = max(1, min(F::kThreads / tasks, kWarps)), mine = threadIdx.x / tasks;
+                const auto at_run = [&](int v, int r) { return ((size_t)2 * (c0 + v) + (v == 0)) * kRows + r; };
+                for (int r = warp; r < rows; r += kWarps) {
+                    RowStats top{-INFINITY, -INFINITY, 0.f};
+                    for (int v = lane; v < n; v += 32) {
+                        top.m = fmaxf(top.m, __ldcg(&part_stats[at_run(v, r)].m));
+                        top.w = fmaxf(top.w, __ldcg(&part_stats[at_run(v, r)].w));
+                    }
+#pragma unroll
+                    for (int d = 16; d; d >>= 1) {
+                        top.m = fmaxf(top.m, __shfl_xor_sync(0xffffffffu, top.m, d));
+                        top.w = fmaxf(top.w, __shfl_xor_sync(0xffffffffu, top.w, d));
+                    }
+                    for (int v = lane; v < n; v += 32) {
+                        const RowStats* const y = &part_stats[at_run(v, r)];
+                        top.l += __ldcg(&y->l) * lower_to(__ldcg(&y->m), top.m);
+                        weights[v * kRows + r] = lower_to(__ldcg(&y->w), top.w);
+                    }
+#pragma unroll
+                    for (int d = 16; d; d >>= 1) top.l += __shfl_xor_sync(0xffffffffu, top.l, d);
+                    if (lane == 0) row_scale[r] = row_factor(a, head * group + (p0 + r) % group, top.m, top.w, top.l);
+                }
+                __syncthreads();
+                for (int i = groups == 1 ? threadIdx.x : threadIdx.x % tasks; i < tasks && mine < groups; i += groups == 1 ? F::kThreads : tasks) {
+                    const int r = i / (DP / 4), d = i % (DP / 4) * 4;
+                    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 16
+                    for (int v = groups == 1 ? 0 : mine; v < n; v += groups) {
+                        const float4 z = __ldcg(reinterpret_cast<const float4*>(part + at_run(v, r) * DP + d));
+                        const float f = weights[v * kRows + r];
+                        sum = make_float4(sum.x + f * z.x, sum.y + f * z.y, sum.z + f * z.z, sum.w + f * z.w);
+                    }
+                    if (groups == 1) write(r, d, row_scale[r], sum);
+                    else *reinterpret_cast<float4*>(sums + (size_t)(mine * kRows + r) * DP + d) = sum;
+                }
+                if (groups > 1) {
+                    __syncthreads();
+                    if (threadIdx.x < tasks) {
+                        const int r = threadIdx.x / (DP / 4), d = threadIdx.x % (DP / 4) * 4;
+                        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+                        for (int v = 0; v < groups; ++v) {
+                            const float4 z = *reinterpret_cast<const float4*>(sums + (size_t)(v * kRows + r) * DP + d);
+                            sum = make_float4(sum.x + z.x, sum.y + z.y, sum.z + z.z, sum.w + z.w);
+                        }
+                        write(r, d, row_scale[r], sum);
+                    }
+                }
             }
         }
         __syncthreads();                                                             // (the ring and the queries' room are taken again)
     }
-}
-
-// A tile that several runs share: a CTA per border between runs, and per row.  The first border inside the tile joins it.
-template <int DP, int NT>
-__global__ void __launch_bounds__(kJoinThreads) kv8_attention_join_kernel(Kv8Cache c, Kv8Step s, Kv8Attention a, int ctas, int warps, const float* part, const RowStats* part_stats) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    constexpr int kRows = 8 * NT, kWarps = kJoinThreads / 32, kEach = DP / 32;
-    __shared__ __align__(16) float sums[kWarps][DP];
-    __shared__ RowStats tops[kWarps];
-    __shared__ Place place;
-    const int nth = blockIdx.x + 1, r = blockIdx.y, group = a.heads / c.kv_heads, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (warp == 0) {
-        const Place found = find_place<kRows>(s, a, c.kv_heads, group, c.page_shift, ctas, warps, nth);
-        if (lane == 0) place = found;
-    }
-    __syncthreads();
-    const Place at = place;
-    if (at.seq < 0) return;
-    const Span sp = span_of<kRows>(s, a, at.seq, group, c.page_shift);
-    const long long item = (at.per * nth - at.base) / sp.blocks, start = at.base + item * sp.blocks;
-    const int c0 = (int)(start / at.per), c1 = (int)((start + sp.blocks - 1) / at.per);
-    const int head = (int)(item / sp.tiles), tile = (int)(item - (long long)head * sp.tiles), p = tile * kRows + r;
-    if (start == at.per * nth || nth != c0 + 1 || p >= sp.n * group) return;
-    // a warp takes every so many-th run, below maxima of its own
-    float sum[kEach] = {};
-    RowStats mine{-INFINITY, -INFINITY, 0.f};
-#pragma unroll 4
-    for (int i = c0 + warp; i <= c1; i += kWarps) {
-        const size_t slot = ((size_t)2 * i + (i == c0)) * kRows + r;
-        const RowStats y = part_stats[slot];
-        const float m = fmaxf(mine.m, y.m), w = fmaxf(mine.w, y.w), f = lower_to(mine.w, w), z = lower_to(y.w, w);
-        mine = {m, w, mine.l * lower_to(mine.m, m) + y.l * lower_to(y.m, m)};
-#pragma unroll
-        for (int j = 0; j < kEach; ++j) sum[j] = f * sum[j] + z * part[slot * DP + lane + 32 * j];
-    }
-#pragma unroll
-    for (int j = 0; j < kEach; ++j) sums[warp][lane + 32 * j] = sum[j];
-    if (lane == 0) tops[warp] = mine;
-    __syncthreads();
-    if (threadIdx.x >= c.dim) return;
-    float m = -INFINITY, w = -INFINITY, l = 0.f, y = 0.f;
-#pragma unroll
-    for (int v = 0; v < kWarps; ++v) { m = fmaxf(m, tops[v].m); w = fmaxf(w, tops[v].w); }
-#pragma unroll
-    for (int v = 0; v < kWarps; ++v) {
-        l += tops[v].l * lower_to(tops[v].m, m);
-        y += sums[v][threadIdx.x] * lower_to(tops[v].w, w);
-    }
-    const int h = head * group + p % group;
-    store_out(a, ((size_t)(sp.begin + p / group) * a.heads + h) * c.dim + threadIdx.x, row_factor(a, h, m, w, l) * y);
+    asm volatile("griddepcontrol.wait;" ::: "memory");        // (the sequences of many rows, which may still be on their way beside this)
 }
 
 inline bool wide(const Kv8Rows& x, int type, int dim) {
     const long long b = type_bytes(type);
     return (reinterpret_cast<uintptr_t>(x.x) & 15) == 0 && x.row * b % 16 == 0 && x.head * b % 16 == 0 && dim % 8 == 0;
 }
+// Room of the runs' parts, and how many of a shared tile's have come
+struct FewWork {
+    float* part;
+    RowStats* stats;
+    unsigned* arrived;
+};
 inline int padded_dim(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 inline int terms_of(int type) { return type == kTypeF32 ? 2 : 1; }
 
 template <int DP, int FORMAT, int TERMS, int NT>
-cudaError_t run_few(const Kv8Cache& c, const Kv8Step& s, const Kv8Attention& a, void* work, cudaStream_t st) {
+cudaError_t run_few(const Kv8Cache& c, const Kv8Step& s, const Kv8Attention& a, bool beside, const FewWork& work, cudaStream_t st) {
     using F = Few<DP, TERMS, NT>;
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess) e = dia::ask_smem<kv8_attention_few_kernel<DP, FORMAT, TERMS, NT>>(dev, F::kSmem);
     if (e != cudaSuccess) return e;
-    e = dia::ask_smem<kv8_attention_few_kernel<DP, FORMAT, TERMS, NT>>(dev, F::kSmem);
-    if (e != cudaSuccess) return e;
-    float* const part = reinterpret_cast<float*>(work);
-    RowStats* const stats = reinterpret_cast<RowStats*>(part + (size_t)2 * F::kCtas * F::kRows * DP);
-    kv8_attention_few_kernel<DP, FORMAT, TERMS, NT><<<F::kCtas, F::kThreads, F::kSmem, st>>>(c, s, a, part, stats);
-    e = cudaGetLastError();
-    if (e != cudaSuccess) return e;
-    ++dia::extra_launches();
-    const int most = (int)std::min<long long>(F::kRows, (long long)s.rows * (a.heads / c.kv_heads));
-    return launch_pdl(kv8_attention_join_kernel<DP, NT>, dim3(F::kCtas - 1, most), dim3(kJoinThreads), 0, st, c, s, a, (int)F::kCtas, (int)F::kWarps, part, stats);
+    return launch_pdl_if(beside, kv8_attention_few_kernel<DP, FORMAT, TERMS, NT>, dim3(F::kCtas), dim3(F::kThreads), F::kSmem, st, c, s, a, work.part, work.stats, work.arrived);
 }
 template <int DP, int FORMAT>
-cudaError_t run_few(const Kv8Cache& c, const Kv8Step& s, const Kv8Attention& a, void* work, cudaStream_t st) {
+cudaError_t run_few(const Kv8Cache& c, const Kv8Step& s, const Kv8Attention& a, bool beside, const FewWork& work, cudaStream_t st) {
     // tiles of eight rows where sequences have no more of them on average (the products of 16 rows take twice the registers and the tensor cores' time)
     const bool eight = (long long)s.rows * (a.heads / c.kv_heads) <= 8ll * s.sequences;
-    if (terms_of(a.type) == 2) return eight ? run_few<DP, FORMAT, 2, 1>(c, s, a, work, st) : run_few<DP, FORMAT, 2, 2>(c, s, a, work, st);
-    return eight ? run_few<DP, FORMAT, 1, 1>(c, s, a, work, st) : run_few<DP, FORMAT, 1, 2>(c, s, a, work, st);
+    if (terms_of(a.type) == 2) return eight ? run_few<DP, FORMAT, 2, 1>(c, s, a, beside, work, st) : run_few<DP, FORMAT, 2, 2>(c, s, a, beside, work, st);
+    return eight ? run_few<DP, FORMAT, 1, 1>(c, s, a, beside, work, st) : run_few<DP, FORMAT, 1, 2>(c, s, a, beside, work, st);
 }
 
 }  // namespace
@@ -778,27 +796,39 @@ cudaError_t launch_kv8_read(const Kv8Cache& c, const Kv8Step& s, void* k, void* 
 namespace {
 // Pairs of a sequence from which on tiles of 256 rows are the shorter way
 constexpr int kFewMost = 64;
+// Tables of up to so many tokens: no tile is shared by several CTAs
+constexpr int kWholeTokens = 2048;
 inline bool some_in_tiles(int kv_heads, int dim, int rows, int heads, int type) { return kv8_tiles_ok(dim, type) && (long long)rows * (heads / kv_heads) > kFewMost; }
 }  // namespace
 
+// Counters first: those of both kernels are set to zero in one go.
+namespace {
+constexpr size_t kCounters = (kMostCtas + kKvTileCounters) * sizeof(unsigned);
+inline size_t few_bytes(int dp) { return (size_t)2 * kMostCtas * 16 * (dp * sizeof(float) + sizeof(RowStats)); }
+inline size_t rounded(size_t bytes) { return (bytes + 255) / 256 * 256; }
+}  // namespace
+
 size_t kv8_attention_work_bytes(int kv_heads, int dim, int rows, int heads, int type) {
-    const int dp = padded_dim(dim);
-    const size_t few = (size_t)2 * kMostCtas * 16 * (dp * sizeof(float) + sizeof(RowStats));
-    return some_in_tiles(kv_heads, dim, rows, heads, type) ? std::max(few, kv8_tiles_work_bytes(dim)) : few;
+    return rounded(kCounters) + rounded(few_bytes(padded_dim(dim))) + (some_in_tiles(kv_heads, dim, rows, heads, type) ? kv8_tiles_work_bytes(dim) : 0);
 }
 
 cudaError_t launch_kv8_attention(const Kv8Cache& c, const Kv8Step& s, Kv8Attention a, void* work, cudaStream_t st) {
     const int dp = padded_dim(c.dim);
-    a.few_most = 0x7fffffff;
-    if (some_in_tiles(c.kv_heads, c.dim, s.rows, a.heads, a.type)) {
-        const bool alone = s.sequences == 1;                  // (then whatever its rows are)
-        a.few_most = alone ? 0 : kFewMost;
-        const cudaError_t e = launch_kv8_tiles(c, s, a, alone, work, st);
+    const bool tiles = some_in_tiles(c.kv_heads, c.dim, s.rows, a.heads, a.type), alone = tiles && s.sequences == 1;        // (alone: in tiles whatever its rows are)
+    unsigned* const counters = reinterpret_cast<unsigned*>(work);
+    float* const part = reinterpret_cast<float*>(reinterpret_cast<char*>(work) + rounded(kCounters));
+    a.whole = !tiles && ((long long)s.max_pages << c.page_shift) <= kWholeTokens;
+    cudaError_t e = a.whole ? cudaSuccess : cudaMemsetAsync(counters, 0, kCounters, st);
+    if (e != cudaSuccess) return e;
+    a.few_most = !tiles ? 0x7fffffff : alone ? 0 : kFewMost;
+    if (tiles) {
+        e = launch_kv8_tiles(c, s, a, alone, reinterpret_cast<char*>(part) + rounded(few_bytes(dp)), counters + kMostCtas, st);
         if (e != cudaSuccess || alone) return e;
         ++dia::extra_launches();
     }
-    if (c.format == kKvE4m3) return dp == 64 ? run_few<64, kKvE4m3>(c, s, a, work, st) : dp == 128 ? run_few<128, kKvE4m3>(c, s, a, work, st) : run_few<256, kKvE4m3>(c, s, a, work, st);
-    return dp == 64 ? run_few<64, kKvInt8>(c, s, a, work, st) : dp == 128 ? run_few<128, kKvInt8>(c, s, a, work, st) : run_few<256, kKvInt8>(c, s, a, work, st);
+    const FewWork few{part, reinterpret_cast<RowStats*>(part + (size_t)2 * kMostCtas * 16 * dp), counters};
+    if (c.format == kKvE4m3) return dp == 64 ? run_few<64, kKvE4m3>(c, s, a, tiles, few, st) : dp == 128 ? run_few<128, kKvE4m3>(c, s, a, tiles, few, st) : run_few<256, kKvE4m3>(c, s, a, tiles, few, st);
+    return dp == 64 ? run_few<64, kKvInt8>(c, s, a, tiles, few, st) : dp == 128 ? run_few<128, kKvInt8>(c, s, a, tiles, few, st) : run_few<256, kKvInt8>(c, s, a, tiles, few, st);
 }
 
 }  // namespace lm

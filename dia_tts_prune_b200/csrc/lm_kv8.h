@@ -72,13 +72,15 @@ struct Kv8Attention {
     int window;                                           // a row sees itself and window - 1 tokens in front; 0: all
     const float* sinks;                                   // [heads] one more logit in the denominator; NULL: none
     int few_most;                                         // (token, query head) pairs per key head of a sequence that tiles of 16 of them take; others go 256 at a time
+    int whole;                                            // != 0: a CTA takes whole tiles of 16
 };
 size_t kv8_attention_work_bytes(int kv_heads, int dim, int rows, int heads, int type);
-cudaError_t launch_kv8_attention(const Kv8Cache& c, const Kv8Step& s, Kv8Attention a, void* work, cudaStream_t st);      // (sets few_most)
+cudaError_t launch_kv8_attention(const Kv8Cache& c, const Kv8Step& s, Kv8Attention a, void* work, cudaStream_t st);      // (sets few_most and whole)
 
 // lm_kv8_tiles.cu: the sequences of more than few_most pairs; bf16 or fp16 rows, dim up to 128.  alone: nothing else zeroes the rows of no sequence
 bool kv8_tiles_ok(int dim, int type);
 size_t kv8_tiles_work_bytes(int dim);
-cudaError_t launch_kv8_tiles(const Kv8Cache& c, const Kv8Step& s, const Kv8Attention& a, bool alone, void* work, cudaStream_t st);
+constexpr int kKvTileCounters = 148;                      // zeros, one for every item whose keys go in chunks
+cudaError_t launch_kv8_tiles(const Kv8Cache& c, const Kv8Step& s, const Kv8Attention& a, bool alone, void* work, unsigned* arrived, cudaStream_t st);
 
 }  // namespace lm

@@ -51,8 +51,8 @@ struct Tiles {
 };
 
 // ---- who takes what ------------------------------------------------------------------------------------------------------------------------
-// Items are (sequence, key head, 256 rows).  Where there are fewer than SMs, the keys of an item go in chunks, as many as all of them fill the GPU once with; a second kernel
-// joins the chunks.  Items of a sequence go last rows first: those see the most keys.
+// Items are (sequence, key head, 256 rows).  Where there are fewer than SMs, the keys of an item go in chunks, as many as all of them fill the GPU once with; the last
+// chunk to come joins them.  Items of a sequence go last rows first: those see the most keys.
 struct Sequence {
     int begin, n, past, tiles, low, high;                     // low, high: tiles of keys that its rows look at
 };
@@ -72,8 +72,7 @@ struct Work {
     int seq, head, tile, chunk, chunks, first_cta, length;    // seq -1: nothing; length: of a chunk in tiles of keys
 };
 constexpr int kWhole = 0x7fffffff;
-// One warp.  JOIN: `index` counts items, and only where there are chunks to join; else it counts CTAs
-template <bool JOIN>
+// One warp: what the CTA of this index takes
 __device__ __forceinline__ Work find_work(const Kv8Cache& c, const Kv8Step& s, const Kv8Attention& a, int group, int index) {
     const int lane = threadIdx.x & 31, each = (s.sequences + 31) / 32, i0 = lane * each, i1 = min(i0 + each, s.sequences);
     const auto before = [&](int v) {                          // sums of the lanes before this one, and of all
@@ -96,7 +95,7 @@ __device__ __forceinline__ Work find_work(const Kv8Cache& c, const Kv8Step& s, c
     const int2 of_items = before(items);
     const int longest = (int)__reduce_max_sync(0xffffffffu, (unsigned)most);
     Work work{-1, 0, 0, 0, 1, 0, kWhole};
-    if (of_items.y == 0 || (JOIN && of_items.y >= kSms)) return work;
+    if (of_items.y == 0) return work;
     const int share = of_items.y >= kSms ? 0 : kSms / of_items.y;
     const int length = share == 0 ? kWhole : max(kMinChunk, (longest + share - 1) / share);
     const auto chunks_of = [&](const Sequence& q) { return length == kWhole ? 1 : max(1, (q.high - q.low + length - 1) / length); };
@@ -104,19 +103,18 @@ __device__ __forceinline__ Work find_work(const Kv8Cache& c, const Kv8Step& s, c
         const Sequence q = at(i);
         ctas += q.tiles * c.kv_heads * chunks_of(q);
     }
-    int cta = before(ctas).x, base = JOIN ? of_items.x : cta;
-    const bool here = index >= base && index < base + (JOIN ? items : ctas);
+    int base = before(ctas).x;
+    const bool here = index >= base && index < base + ctas;
     if (here) {
         for (int i = i0;; ++i) {
             const Sequence q = at(i);
-            const int chunks = chunks_of(q), own = q.tiles * c.kv_heads, units = JOIN ? own : own * chunks;
+            const int chunks = chunks_of(q), units = q.tiles * c.kv_heads * chunks;
             if (index < base + units) {
-                const unsigned local = index - base, item = JOIN ? local : local / (unsigned)chunks;
-                work = {i, (int)(item % (unsigned)c.kv_heads), q.tiles - 1 - (int)(item / (unsigned)c.kv_heads), JOIN ? 0 : (int)(local - item * chunks), chunks, cta + (int)item * chunks, length};
+                const unsigned local = index - base, item = local / (unsigned)chunks;
+                work = {i, (int)(item % (unsigned)c.kv_heads), q.tiles - 1 - (int)(item / (unsigned)c.kv_heads), (int)(local - item * chunks), chunks, base + (int)item * chunks, length};
                 break;
             }
             base += units;
-            cta += own * chunks;
         }
     }
     const unsigned who = __ballot_sync(0xffffffffu, here);
@@ -178,7 +176,7 @@ __device__ __forceinline__ void mma_weights(uint32_t d, uint32_t a, uint64_t b, 
 }
 
 template <int DP, int FORMAT>
-__global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cache c, Kv8Step s, Kv8Attention a, int alone, float* part, RowStats* part_stats, int* ran_out, unsigned polls) {
+__global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cache c, Kv8Step s, Kv8Attention a, int alone, float* part, RowStats* part_stats, unsigned* arrived, int* ran_out, unsigned polls) {
     using T = Tiles<DP>;
     constexpr int kStages = T::kStages, kDepth = T::kDepth, kSteps = DP / 16;
     extern __shared__ __align__(1024) uint8_t smem[];
@@ -197,7 +195,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cac
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = a.heads / c.kv_heads;
     if (warp == 0) {
-        const Work work = find_work<false>(c, s, a, group, blockIdx.x);
+        const Work work = find_work(c, s, a, group, blockIdx.x);
         if (lane == 0) {
             found = work;
             if (work.seq >= 0) found_rows = sequence_at(s, a, work.seq, group, c.page_shift);
@@ -649,62 +647,58 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cac
         __threadfence_system();
     }
     __syncwarp();
+    if (work.chunks > 1) __threadfence();                     // (what this chunk leaves, for whoever joins)
     fence_before();
     __syncthreads();
+    if (work.chunks > 1) {
+        // the last chunk of an item to come joins all, in their order
+        if (threadIdx.x == 0) largest = atomicAdd(arrived + work.first_cta, 1u) == (unsigned)(work.chunks - 1);
+        __syncthreads();
+        if (largest) {
+            __threadfence();
+            // rows' weights of the chunks first, where the rings lay, then their channels
+            float* const weights = reinterpret_cast<float*>(smem);                   // [chunk][row], and behind them what a row's sum is times
+            const int rows = min(kTileRows, pairs - p0);
+            const RowStats* const stats = part_stats + (size_t)work.first_cta * kTileRows;
+            for (int r = threadIdx.x; r < rows; r += kThreads) {
+                float m = -INFINITY, w = -INFINITY, l = 0.f;
+                for (int i = 0; i < work.chunks; ++i) {
+                    m = fmaxf(m, __ldcg(&stats[i * kTileRows + r].m));
+                    w = fmaxf(w, __ldcg(&stats[i * kTileRows + r].w));
+                }
+                for (int i = 0; i < work.chunks; ++i) {
+                    l += __ldcg(&stats[i * kTileRows + r].l) * lower_to(__ldcg(&stats[i * kTileRows + r].m), m);
+                    weights[i * kTileRows + r] = lower_to(__ldcg(&stats[i * kTileRows + r].w), w);
+                }
+                weights[work.chunks * kTileRows + r] = row_factor(a, work.head * group + (p0 + r) % group, m, w, l);
+            }
+            __syncthreads();
+            const float* const from_part = part + (size_t)work.first_cta * kTileRows * DP;
+#pragma unroll 4
+            for (int i = threadIdx.x; i < rows * (DP / 4); i += kThreads) {
+                const int r = i / (DP / 4), d = i % (DP / 4) * 4, p = p0 + r;
+                float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+                for (int k = 0; k < work.chunks; ++k) {
+                    const float f = weights[k * kTileRows + r];
+                    const float4 z = __ldcg(reinterpret_cast<const float4*>(from_part + ((size_t)k * kTileRows + r) * DP + d));
+                    sum = make_float4(sum.x + f * z.x, sum.y + f * z.y, sum.z + f * z.z, sum.w + f * z.w);
+                }
+                const float f = weights[work.chunks * kTileRows + r], y[4] = {sum.x, sum.y, sum.z, sum.w};
+                const size_t to = ((size_t)(q.begin + p / group) * a.heads + work.head * group + p % group) * c.dim + d;
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (d + e < c.dim) store_out(a, to + e, f * y[e]);
+            }
+        }
+    }
     if (warp == 16) {
         fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
     }
 }
 
-// The chunks of an item: a warp per row
-constexpr int kJoinThreads = 256, kJoinCtas = 8;
-template <int DP>
-__global__ void __launch_bounds__(kJoinThreads) kv8_attention_tiles_join_kernel(Kv8Cache c, Kv8Step s, Kv8Attention a, const float* part, const RowStats* part_stats) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int group = a.heads / c.kv_heads, lane = threadIdx.x & 31;
-    __shared__ Work found;
-    if (threadIdx.x < 32) {
-        const Work work = find_work<true>(c, s, a, group, blockIdx.x);
-        if (lane == 0) found = work;
-    }
-    __syncthreads();
-    const Work work = found;
-    if (work.seq < 0 || work.chunks == 1) return;
-    const Sequence q = sequence_at(s, a, work.seq, group, c.page_shift);
-    for (int r = blockIdx.y * (kJoinThreads / 32) + (threadIdx.x >> 5); r < kTileRows; r += kJoinCtas * (kJoinThreads / 32)) {
-        const int p = work.tile * kTileRows + r;
-        if (p >= q.n * group) return;
-        float m = -INFINITY, w = -INFINITY, l = 0.f, sum[DP / 32] = {};
-        for (int i = lane; i < work.chunks; i += 32) {
-            const RowStats y = part_stats[(size_t)(work.first_cta + i) * kTileRows + r];
-            m = fmaxf(m, y.m);
-            w = fmaxf(w, y.w);
-        }
-#pragma unroll
-        for (int d = 16; d; d >>= 1) {
-            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-            w = fmaxf(w, __shfl_xor_sync(0xffffffffu, w, d));
-        }
-#pragma unroll 4
-        for (int i = 0; i < work.chunks; ++i) {
-            const size_t slot = (size_t)(work.first_cta + i) * kTileRows + r;
-            const RowStats y = part_stats[slot];
-            const float f = lower_to(y.w, w);
-            l += y.l * lower_to(y.m, m);
-#pragma unroll
-            for (int j = 0; j < DP / 32; ++j) sum[j] += f * part[slot * DP + lane + 32 * j];
-        }
-        const int h = work.head * group + p % group;
-        const float f = row_factor(a, h, m, w, l);
-#pragma unroll
-        for (int j = 0; j < DP / 32; ++j)
-            if (lane + 32 * j < c.dim) store_out(a, ((size_t)(q.begin + p / group) * a.heads + h) * c.dim + lane + 32 * j, f * sum[j]);
-    }
-}
-
 template <int DP, int FORMAT>
-cudaError_t run_tiles(const Kv8Cache& c, const Kv8Step& s, const Kv8Attention& a, bool alone, void* work, cudaStream_t st) {
+cudaError_t run_tiles(const Kv8Cache& c, const Kv8Step& s, const Kv8Attention& a, bool alone, void* work, unsigned* arrived, cudaStream_t st) {
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e == cudaSuccess) e = ask_smem<kv8_attention_tiles_kernel<DP, FORMAT>>(dev, Tiles<DP>::kSmem);
@@ -717,11 +711,8 @@ cudaError_t run_tiles(const Kv8Cache& c, const Kv8Step& s, const Kv8Attention& a
     const long long pairs = (long long)s.rows * (a.heads / c.kv_heads), partly = std::min<long long>(s.sequences, pairs / (a.few_most + 1));
     const long long ctas = std::max<long long>(kSms, c.kv_heads * (pairs / kTileRows + partly));
     if (ctas > 0x7fffffff) return cudaErrorInvalidValue;
-    kv8_attention_tiles_kernel<DP, FORMAT><<<(unsigned)ctas, kThreads, Tiles<DP>::kSmem, st>>>(c, s, a, alone, part, stats, ran_out, gemm_pair_polls());
-    e = cudaGetLastError();
-    if (e != cudaSuccess) return e;
-    ++extra_launches();
-    return launch_pdl(kv8_attention_tiles_join_kernel<DP>, dim3(kSms, kJoinCtas), dim3(kJoinThreads), 0, st, c, s, a, part, stats);
+    kv8_attention_tiles_kernel<DP, FORMAT><<<(unsigned)ctas, kThreads, Tiles<DP>::kSmem, st>>>(c, s, a, alone, part, stats, arrived, ran_out, gemm_pair_polls());
+    return cudaGetLastError();
 }
 
 }  // namespace
@@ -730,9 +721,9 @@ bool kv8_tiles_ok(int dim, int type) { return dim <= 128 && type != kTypeF32; }
 
 size_t kv8_tiles_work_bytes(int dim) { return (size_t)kSms * kTileRows * ((dim <= 64 ? 64 : 128) * sizeof(float) + sizeof(RowStats)); }
 
-cudaError_t launch_kv8_tiles(const Kv8Cache& c, const Kv8Step& s, const Kv8Attention& a, bool alone, void* work, cudaStream_t st) {
-    if (c.dim <= 64) return c.format == kKvE4m3 ? run_tiles<64, kKvE4m3>(c, s, a, alone, work, st) : run_tiles<64, kKvInt8>(c, s, a, alone, work, st);
-    return c.format == kKvE4m3 ? run_tiles<128, kKvE4m3>(c, s, a, alone, work, st) : run_tiles<128, kKvInt8>(c, s, a, alone, work, st);
+cudaError_t launch_kv8_tiles(const Kv8Cache& c, const Kv8Step& s, const Kv8Attention& a, bool alone, void* work, unsigned* arrived, cudaStream_t st) {
+    if (c.dim <= 64) return c.format == kKvE4m3 ? run_tiles<64, kKvE4m3>(c, s, a, alone, work, arrived, st) : run_tiles<64, kKvInt8>(c, s, a, alone, work, arrived, st);
+    return c.format == kKvE4m3 ? run_tiles<128, kKvE4m3>(c, s, a, alone, work, arrived, st) : run_tiles<128, kKvInt8>(c, s, a, alone, work, arrived, st);
 }
 
 }  // namespace lm
