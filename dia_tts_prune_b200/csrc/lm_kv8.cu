@@ -61,6 +61,16 @@ struct Eight {
             memcpy(w, v, sizeof(v));
         }
     }
+    // the largest magnitude so far, as bits (two of the 16-bit types side by side), and as those of an fp32 number
+    __device__ __forceinline__ void look(uint32_t& most) const {
+        const uint32_t* const u = &w[0].x;
+#pragma unroll
+        for (int i = 0; i < (TYPE == kTypeF32 ? 8 : 4); ++i) most = TYPE == kTypeF32 ? max(most, u[i] & 0x7fffffffu) : __vmaxu2(most, u[i] & 0x7fff7fffu);
+    }
+    static __device__ __forceinline__ uint32_t looked(uint32_t most) {
+        const uint32_t half = max(most & 0xffffu, most >> 16);
+        return TYPE == kTypeF32 ? most : TYPE == kTypeBf16 ? half << 16 : __float_as_uint(__half2float(__ushort_as_half((unsigned short)half)));
+    }
     __device__ __forceinline__ void numbers(float (&f)[8]) const {
         Element<TYPE> v[8];
         memcpy(v, w, sizeof(v));
@@ -73,23 +83,50 @@ struct Eight {
 // A warp takes what comes into one page of one head, keys or values: it reads the rows for their largest magnitude, makes the page's step as large as it has to be, rounds the
 // codes that are there if it grew, and writes the new ones.  Eight groups of eight channels a lane stay in registers in between (16 tokens of 128 channels); what is beyond is
 // read again, from L2.  `chunk` rows in turn belong to a warp: a page border or a sequence's first row among them starts a page.
-constexpr int kAppendThreads = 128, kKept = 8;
+// Bound: a chain of loads (the row's sequence, its rows and the page's number, the page's scale) for every warp; rows are asked for before the page is known.
+constexpr int kAppendThreads = 128, kKept = 8, kSearchMost = 1024;
+
+// The sequence of a row, by a warp: how many begin at or before it (one look for 32 sequences; where there are very many, by halves)
+__device__ __forceinline__ int sequence_by_warp(const Kv8Step& s, int row) {
+    if (!s.first || s.sequences > kSearchMost) return s.sequence_of(row);
+    int n = 0;
+    for (int i = 0; i <= s.sequences; i += 32) {
+        const int at = i + (threadIdx.x & 31);
+        n += __popc(__ballot_sync(0xffffffffu, at <= s.sequences && s.first[at] <= row));
+    }
+    return n > 0 && n <= s.sequences ? n - 1 : -1;
+}
+
 template <int FORMAT, int TYPE, bool WIDE>
-__global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(Kv8Cache c, Kv8Step s, Kv8Rows k, Kv8Rows v, int chunk) {
+__global__ void __launch_bounds__(kAppendThreads, 4) kv8_append_kernel(Kv8Cache c, Kv8Step s, Kv8Rows k, Kv8Rows v, int chunk) {
     const int lane = threadIdx.x & 31;
     const long long task = ((long long)blockIdx.x * kAppendThreads + threadIdx.x) >> 5;
-    const int sides = 2 * c.kv_heads, side = (int)(task % sides), head = side >> 1;
+    const int sides = 2 * c.kv_heads, side = (int)(task % sides) & 1, head = (int)(task % sides) >> 1;
     const long long row0 = task / sides * chunk;
     if (row0 >= s.rows) return;
-    const Kv8Rows in = side & 1 ? v : k;
-    uint8_t* const codes = side & 1 ? c.values : c.keys;
-    float* const scales = side & 1 ? c.value_scales : c.key_scales;
+    const Kv8Rows in = side ? v : k;
+    uint8_t* const codes = side ? c.values : c.keys;
+    float* const scales = side ? c.value_scales : c.key_scales;
     const Element<TYPE>* const x = reinterpret_cast<const Element<TYPE>*>(in.x) + head * in.head;
     const int groups = (c.dim + 7) >> 3, page_size = 1 << c.page_shift, last = (int)min(row0 + chunk, (long long)s.rows);
-    int row = (int)row0, seq = s.sequence_of(row);
+    // a lane's groups: group lane of the rows in turn, the next one 32 further on
+    struct At {
+        int r, g;
+    };
+    const int step_r = 32 / groups, step_g = 32 - step_r * groups;
+    const At first{lane / groups, lane - lane / groups * groups};
+    const auto next = [&](At& at) {
+        at.r += step_r;
+        at.g += step_g;
+        if (at.g >= groups) {
+            at.g -= groups;
+            ++at.r;
+        }
+    };
+    int row = (int)row0, seq = sequence_by_warp(s, row);
     while (row < last) {
         if (seq < 0) {                                        // no row of a sequence: on to the next one that is
-            if (++row < last) seq = s.sequence_of(row);
+            if (++row < last) seq = sequence_by_warp(s, row);
             continue;
         }
         const int begin = s.begin(seq), end = s.end(seq), past = s.past[seq];
@@ -97,34 +134,34 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(Kv8Cache c, 
         const int place = (int)(pos & (page_size - 1));
         const int ends = min(end, row + page_size - place);    // of the rows that go into this page
         if (past >= 0 && (row == begin || place == 0)) {
-            const int page = s.page(seq, pos >> c.page_shift, c.pages), n = (ends - row) * groups;
+            const int n = ends - row;
+            Eight<TYPE, WIDE> kept[kKept];
+            const auto fetch = [&](Eight<TYPE, WIDE>& e, const At& at) {
+                if (at.r < n) e.fetch(x + (row + at.r) * in.row + 8 * at.g, c.dim - 8 * at.g);
+                else e = {};
+            };
+            At beyond = first;
+#pragma unroll
+            for (int j = 0; j < kKept; ++j) {
+                fetch(kept[j], beyond);
+                next(beyond);
+            }
+            const int page = s.page(seq, pos >> c.page_shift, c.pages);
             if (page >= 0) {
-                Eight<TYPE, WIDE> kept[kKept];
+                const size_t page_head = (size_t)page * c.kv_heads + head;
+                float* const scale = scales + page_head;
+                uint8_t* const to = codes + (page_head << c.page_shift) * c.stride;
+                const uint32_t old = place ? __float_as_uint(*scale) & 0x7fffffffu : 0u;
                 uint32_t most = 0;
-                const auto fetch = [&](Eight<TYPE, WIDE>& e, int i) {
-                    const int r = i / groups, g = i - r * groups;
-                    if (i < n) e.fetch(x + (row + r) * in.row + 8 * g, c.dim - 8 * g);
-                    else e = {};
-                };
-                const auto look = [&](const Eight<TYPE, WIDE>& e) {
-                    float f[8];
-                    e.numbers(f);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) most = max(most, __float_as_uint(f[j]) & 0x7fffffffu);
-                };
-#pragma unroll
-                for (int j = 0; j < kKept; ++j) fetch(kept[j], lane + 32 * j);
-#pragma unroll
-                for (int j = 0; j < kKept; ++j) look(kept[j]);
-                for (int i = lane + 32 * kKept; i < n; i += 32) {
+                for (int j = 0; j < kKept; ++j) kept[j].look(most);
+#pragma unroll 1
+                for (At i = beyond; i.r < n; next(i)) {
                     Eight<TYPE, WIDE> e;
                     fetch(e, i);
-                    look(e);
+                    e.look(most);
                 }
-                most = __reduce_max_sync(0xffffffffu, most);
-                float* const scale = scales + (size_t)page * c.kv_heads + head;
-                uint8_t* const at = codes + (((size_t)page * c.kv_heads + head) << c.page_shift) * c.stride;
-                const uint32_t old = place ? __float_as_uint(*scale) & 0x7fffffffu : 0u;
+                most = __reduce_max_sync(0xffffffffu, Eight<TYPE, WIDE>::looked(most));
                 const bool bad = most >= 0x7f800000u || old >= 0x7f800000u;
                 int e = needed<FORMAT>(most);
                 if (place && !bad) {
@@ -133,8 +170,9 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(Kv8Cache c, 
                         e = before;
                     } else {
                         const float f = power(before - e);
+#pragma unroll 1
                         for (int i = lane; i < place * (c.stride >> 4); i += 32) {
-                            uint4* const p = reinterpret_cast<uint4*>(at) + i;
+                            uint4* const p = reinterpret_cast<uint4*>(to) + i;
                             uint4 w = *p;
                             uint32_t* const u = &w.x;
 #pragma unroll
@@ -149,21 +187,25 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(Kv8Cache c, 
                 __syncwarp();                                  // (every lane has read the old scale)
                 if (lane == 0) *scale = bad ? __uint_as_float(0x7fc00000u) : power(e);
                 const float f = power(-e);
-                const auto write = [&](const Eight<TYPE, WIDE>& g8, int i) {
-                    if (i >= n) return;
-                    const int r = i / groups, g = i - r * groups;
+                const auto write = [&](const Eight<TYPE, WIDE>& g8, const At& at) {
+                    if (at.r >= n) return;
                     float t[8];
                     g8.numbers(t);
 #pragma unroll
                     for (int j = 0; j < 8; ++j) t[j] = bad ? 0.f : t[j] * f;
                     const uint2 w = make_uint2(encode4<FORMAT>(t[0], t[1], t[2], t[3]), encode4<FORMAT>(t[4], t[5], t[6], t[7]));
-                    uint2* const p = reinterpret_cast<uint2*>(at + (size_t)(place + r) * c.stride) + g;
+                    uint2* const p = reinterpret_cast<uint2*>(to + (size_t)(place + at.r) * c.stride) + at.g;
                     p[0] = w;
-                    if (g == groups - 1 && (groups & 1)) p[1] = make_uint2(0u, 0u);        // (up to the row's 16 bytes)
+                    if (at.g == groups - 1 && (groups & 1)) p[1] = make_uint2(0u, 0u);     // (up to the row's 16 bytes)
                 };
+                At at = first;
 #pragma unroll
-                for (int j = 0; j < kKept; ++j) write(kept[j], lane + 32 * j);
-                for (int i = lane + 32 * kKept; i < n; i += 32) {
+                for (int j = 0; j < kKept; ++j) {
+                    write(kept[j], at);
+                    next(at);
+                }
+#pragma unroll 1
+                for (At i = beyond; i.r < n; next(i)) {
                     Eight<TYPE, WIDE> g8;
                     fetch(g8, i);
                     write(g8, i);
@@ -171,60 +213,90 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(Kv8Cache c, 
             }
         }
         row = ends;
-        if (row == end && row < last) seq = s.sequence_of(row);
+        if (row == end && row < last) seq = sequence_by_warp(s, row);
     }
 }
 
 // ---- numbers out of pages ------------------------------------------------------------------------------------------------------------------
-// A CTA takes kReadRows rows (fewer where there are few): where each of them lies is looked up once, then a thread takes 16 bytes of what goes out.
-constexpr int kReadThreads = 256, kReadMostRows = 32;
+// A CTA takes kReadRows rows (fewer where there are few): where each of them lies is looked up once.  A thread has 16 bytes of what goes out, the same head and channels of row
+// after row, four rows on their way at a time.
+constexpr int kReadThreads = 256, kReadMostRows = 32, kReadAhead = 4;
 template <int FORMAT, int TYPE, bool WIDE>
 __global__ void __launch_bounds__(kReadThreads) kv8_read_kernel(Kv8Cache c, Kv8Step s, Element<TYPE>* k, Element<TYPE>* v, int rows_each) {
-    __shared__ long long where[kReadMostRows];                // the row's page and place in it, in rows of a head; -1: not there
+    __shared__ int firsts[kSearchMost + 1];
+    __shared__ long long where[kReadMostRows];                // the row's page (from the 32nd bit on) and place in it; -1: not there
     const int row0 = blockIdx.x * rows_each, n = min(rows_each, s.rows - row0);
+    const bool near = s.first && s.sequences <= kSearchMost;
+    if (near) {
+        for (int i = threadIdx.x; i <= s.sequences; i += kReadThreads) firsts[i] = s.first[i];
+        __syncthreads();
+    }
     if (threadIdx.x < n) {
-        const int row = row0 + threadIdx.x, seq = s.sequence_of(row);
+        Kv8Step of = s;
+        if (near) of.first = firsts;
+        const int row = row0 + threadIdx.x, seq = of.sequence_of(row);
         long long at = -1;
         if (seq >= 0) {
             const int past = s.past[seq];
-            const long long pos = (long long)past + (row - s.begin(seq));
+            const long long pos = (long long)past + (row - of.begin(seq));
             const int page = past >= 0 ? s.page(seq, pos >> c.page_shift, c.pages) : -1;
             if (page >= 0) at = (long long)page << 32 | (pos & ((1 << c.page_shift) - 1));
         }
         where[threadIdx.x] = at;
     }
     __syncthreads();
-    constexpr int kEach = 16 / sizeof(Element<TYPE>);
-    const int parts = (c.dim + kEach - 1) / kEach, per_row = 2 * c.kv_heads * parts;
-    for (int i = threadIdx.x; i < n * per_row; i += kReadThreads) {
-        const int r = i / per_row, j = i - r * per_row, side = j / (c.kv_heads * parts), hp = j - side * c.kv_heads * parts, head = hp / parts, part = hp - head * parts;
-        const long long at = where[r];
-        Element<TYPE> out[kEach];
-        if (at >= 0) {
-            const size_t page_head = (size_t)(at >> 32) * c.kv_heads + head;
-            const uint8_t* const p = (side ? c.values : c.keys) + ((page_head << c.page_shift) + (uint32_t)at) * c.stride + part * kEach;
-            const float scale = (side ? c.value_scales : c.key_scales)[page_head];
+    constexpr int kEach = 16 / sizeof(Element<TYPE>), kCodeWords = kEach / 4;
+    const int parts = (c.dim + kEach - 1) / kEach, per_row = 2 * c.kv_heads * parts, beside = max(1, kReadThreads / per_row);
+    for (int j = per_row <= kReadThreads ? threadIdx.x % per_row : threadIdx.x; j < per_row; j += per_row <= kReadThreads ? per_row : kReadThreads) {
+        const int side = j / (c.kv_heads * parts), hp = j - side * c.kv_heads * parts, head = hp / parts, part = hp - head * parts, r0 = per_row <= kReadThreads ? threadIdx.x / per_row : 0;
+        if (r0 >= beside) break;
+        const uint8_t* const codes = (side ? c.values : c.keys) + part * kEach;
+        const float* const scales = side ? c.value_scales : c.key_scales;
+        Element<TYPE>* const to = (side ? v : k) + ((size_t)row0 * c.kv_heads + head) * c.dim + part * kEach;
+        for (int r = r0; r < n; r += beside * kReadAhead) {
+            uint32_t w[kReadAhead][kCodeWords];
+            float scale[kReadAhead];
 #pragma unroll
-            for (int e = 0; e < kEach; e += 4) {
-                const float4 t = values4<FORMAT>(*reinterpret_cast<const uint32_t*>(p + e), scale);
-                out[e] = narrow<Element<TYPE>>(t.x);
-                out[e + 1] = narrow<Element<TYPE>>(t.y);
-                out[e + 2] = narrow<Element<TYPE>>(t.z);
-                out[e + 3] = narrow<Element<TYPE>>(t.w);
+            for (int i = 0; i < kReadAhead; ++i) {
+                const long long at = r + i * beside < n ? where[r + i * beside] : -1;
+                scale[i] = 0.f;
+#pragma unroll
+                for (int e = 0; e < kCodeWords; ++e) w[i][e] = 0;
+                if (at < 0) continue;
+                const size_t page_head = (size_t)(at >> 32) * c.kv_heads + head;
+                const uint8_t* const p = codes + ((page_head << c.page_shift) + (uint32_t)at) * c.stride;
+                if constexpr (kCodeWords == 2) {
+                    const uint2 u = *reinterpret_cast<const uint2*>(p);
+                    w[i][0] = u.x;
+                    w[i][kCodeWords - 1] = u.y;
+                } else {
+                    w[i][0] = *reinterpret_cast<const uint32_t*>(p);
+                }
+                scale[i] = scales[page_head];
             }
-        } else {
 #pragma unroll
-            for (int e = 0; e < kEach; ++e) out[e] = narrow<Element<TYPE>>(0.f);
-        }
-        Element<TYPE>* const to = (side ? v : k) + ((size_t)(row0 + r) * c.kv_heads + head) * c.dim + part * kEach;
-        if constexpr (WIDE) {
-            uint4 w;
-            memcpy(&w, out, 16);
-            *reinterpret_cast<uint4*>(to) = w;
-        } else {
+            for (int i = 0; i < kReadAhead; ++i) {
+                if (r + i * beside >= n) break;
+                Element<TYPE> out[kEach];
 #pragma unroll
-            for (int e = 0; e < kEach; ++e)
-                if (part * kEach + e < c.dim) to[e] = out[e];
+                for (int e = 0; e < kEach; e += 4) {
+                    const float4 t = values4<FORMAT>(w[i][e / 4], scale[i]);      // (of a row that is not there: zeros times zero)
+                    out[e] = narrow<Element<TYPE>>(t.x);
+                    out[e + 1] = narrow<Element<TYPE>>(t.y);
+                    out[e + 2] = narrow<Element<TYPE>>(t.z);
+                    out[e + 3] = narrow<Element<TYPE>>(t.w);
+                }
+                Element<TYPE>* const p = to + (size_t)(r + i * beside) * c.kv_heads * c.dim;
+                if constexpr (WIDE) {
+                    uint4 u;
+                    memcpy(&u, out, 16);
+                    *reinterpret_cast<uint4*>(p) = u;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < kEach; ++e)
+                        if (part * kEach + e < c.dim) p[e] = out[e];
+                }
+            }
         }
     }
 }
