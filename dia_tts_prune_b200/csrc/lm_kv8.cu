@@ -755,21 +755,27 @@ __global__ void __launch_bounds__(Few<DP, TERMS, NT>::kThreads, Few<DP, TERMS, N
                 float* const weights = sums + kWarps * kRows * DP;                   // [run][row]
                 const int n = c1 - c0 + 1, groups = max(1, min(F::kThreads / tasks, kWarps)), mine = threadIdx.x / tasks;
                 const auto at_run = [&](int v, int r) { return ((size_t)2 * (c0 + v) + (v == 0)) * kRows + r; };
+                // (Loads go out many at a time: one after the other, those of 148 runs took 12 us.)
                 for (int r = warp; r < rows; r += kWarps) {
-                    RowStats top{-INFINITY, -INFINITY, 0.f};
-                    for (int v = lane; v < n; v += 32) {
-                        top.m = fmaxf(top.m, __ldcg(&part_stats[at_run(v, r)].m));
-                        top.w = fmaxf(top.w, __ldcg(&part_stats[at_run(v, r)].w));
+                    constexpr int kMine = (F::kCtas + 31) / 32;
+                    RowStats y[kMine], top{-INFINITY, -INFINITY, 0.f};
+#pragma unroll
+                    for (int j = 0; j < kMine; ++j) {
+                        const int v = lane + 32 * j;
+                        y[j] = {-INFINITY, -INFINITY, 0.f};
+                        if (v < n) y[j] = {__ldcg(&part_stats[at_run(v, r)].m), __ldcg(&part_stats[at_run(v, r)].w), __ldcg(&part_stats[at_run(v, r)].l)};
                     }
+#pragma unroll
+                    for (int j = 0; j < kMine; ++j) top = {fmaxf(top.m, y[j].m), fmaxf(top.w, y[j].w), 0.f};
 #pragma unroll
                     for (int d = 16; d; d >>= 1) {
                         top.m = fmaxf(top.m, __shfl_xor_sync(0xffffffffu, top.m, d));
                         top.w = fmaxf(top.w, __shfl_xor_sync(0xffffffffu, top.w, d));
                     }
-                    for (int v = lane; v < n; v += 32) {
-                        const RowStats* const y = &part_stats[at_run(v, r)];
-                        top.l += __ldcg(&y->l) * lower_to(__ldcg(&y->m), top.m);
-                        weights[v * kRows + r] = lower_to(__ldcg(&y->w), top.w);
+#pragma unroll
+                    for (int j = 0; j < kMine; ++j) {
+                        top.l += y[j].l * lower_to(y[j].m, top.m);
+                        if (lane + 32 * j < n) weights[(lane + 32 * j) * kRows + r] = lower_to(y[j].w, top.w);
                     }
 #pragma unroll
                     for (int d = 16; d; d >>= 1) top.l += __shfl_xor_sync(0xffffffffu, top.l, d);
@@ -779,11 +785,20 @@ __global__ void __launch_bounds__(Few<DP, TERMS, NT>::kThreads, Few<DP, TERMS, N
                 for (int i = groups == 1 ? threadIdx.x : threadIdx.x % tasks; i < tasks && mine < groups; i += groups == 1 ? F::kThreads : tasks) {
                     const int r = i / (DP / 4), d = i % (DP / 4) * 4;
                     float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 16
-                    for (int v = groups == 1 ? 0 : mine; v < n; v += groups) {
-                        const float4 z = __ldcg(reinterpret_cast<const float4*>(part + at_run(v, r) * DP + d));
-                        const float f = weights[v * kRows + r];
-                        sum = make_float4(sum.x + f * z.x, sum.y + f * z.y, sum.z + f * z.z, sum.w + f * z.w);
+                    constexpr int kAtOnce = 16;
+#pragma unroll 1
+                    for (int v0 = groups == 1 ? 0 : mine; v0 < n; v0 += kAtOnce * groups) {
+                        float4 z[kAtOnce];
+#pragma unroll
+                        for (int j = 0; j < kAtOnce; ++j) {
+                            const int v = v0 + j * groups;
+                            z[j] = v < n ? __ldcg(reinterpret_cast<const float4*>(part + at_run(v, r) * DP + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                        }
+#pragma unroll
+                        for (int j = 0; j < kAtOnce; ++j) {
+                            const float f = v0 + j * groups < n ? weights[(v0 + j * groups) * kRows + r] : 0.f;
+                            sum = make_float4(sum.x + f * z[j].x, sum.y + f * z[j].y, sum.z + f * z[j].z, sum.w + f * z[j].w);
+                        }
                     }
                     if (groups == 1) write(r, d, row_scale[r], sum);
                     else *reinterpret_cast<float4*>(sums + (size_t)(mine * kRows + r) * DP + d) = sum;
