@@ -3,9 +3,9 @@
 // A CTA takes 256 (token, query head) rows that share a key head and walks their keys 128 at a time:
 //   warps 0-3, 4-7   one thread per row, 128 rows each: 64 scores at a time from tensor memory, softmax weights back to where they lay.  A half has two places for scores, so
 //                    that the next ones are there when it has weighed these
-//   warps 8-15       codes to fp16 operands, from shared memory to shared memory: four warps the keys, four the values, 16 tokens of a step each
+//   warps 8-15       four warps the keys, four the values, 16 tokens of a step each: codes into shared memory by bulk copies, four steps ahead, and from there to fp16 operands
 //   warps 16, 17     one elected lane each issues tcgen05.mma for a half: S = Q K^T (M = 128, N = 64), and O += P V with P as the operand in tensor memory
-//   warp 18          looks up pages and scales, and fetches the codes of the next four steps by bulk copies
+//   warp 18          looks up pages and scales, some tiles ahead
 //
 // Numbers.  t = scale log2(e) q . key + e - E in powers of two, e the exponent of the page's values and E the largest of the CTA's pages; P = 2^(t - R + 7) in fp16, with R the
 // row's reference: about its largest t so far, raised (and O and the sum with it) only when one of 64 scores lies more than 8 above it, so P is at most 2^15.  That the page's value
@@ -184,7 +184,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cac
     uint8_t* const k_ring = smem + T::kQ;
     uint8_t* const v_ring = k_ring + kStages * T::kSide;
     uint8_t* const codes = v_ring + kStages * T::kSide;       // [keys, values][kDepth]
-    __shared__ uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], m_full[kAhead], m_empty[kAhead], c_full[2][kDepth], c_empty[2][kDepth], s_full[2][2], p_ready[2][2], pv_done[2][2], done[2];
+    __shared__ uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], m_full[kAhead], m_empty[kAhead], c_full[8][kDepth], s_full[2][2], p_ready[2][2], pv_done[2][2], done[2];
     __shared__ float4 blocks[kAhead][kBlocks];                // (key scale, e - E, 2^(E - e), page) of 16 tokens
     __shared__ uint3 which[kAhead];                           // of a tile's blocks: those that are there, whose values are taken as zeros, that stand for numbers
     __shared__ uint32_t tmem_slot;
@@ -211,11 +211,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cac
             mbar_init(&m_full[i], 1);
             mbar_init(&m_empty[i], 16);
         }
+        for (int w = 0; w < 8; ++w)
+            for (int i = 0; i < kDepth; ++i) mbar_init(&c_full[w][i], 1);
         for (int g = 0; g < 2; ++g) {
-            for (int i = 0; i < kDepth; ++i) {
-                mbar_init(&c_full[g][i], 1);
-                mbar_init(&c_empty[g][i], 4);
-            }
             for (int i = 0; i < 2; ++i) {
                 mbar_init(&s_full[g][i], 1);
                 mbar_init(&p_ready[g][i], 4);
@@ -497,7 +495,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cac
         uint64_t* const full = side ? v_full : k_full;
         uint64_t* const empty = side ? v_empty : k_empty;
         uint8_t* const ring = side ? v_ring : k_ring;
-        const uint8_t* const from_codes = codes + side * kDepth * T::kCodes;
+        uint8_t* const mine = codes + (warp - 8) * kDepth * (T::kCodes / 4);      // this warp's codes of so many steps
+        uint64_t* const arrived_codes = c_full[warp - 8];
         const auto lay = [&](const uint8_t* from, uint8_t* to, bool zeros) {
 #pragma unroll
             for (int r8 = 0; r8 < 2; ++r8)
@@ -505,7 +504,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cac
                 for (int j = 0; j < kParts; ++j) {
                     const int piece = DP == 64 ? ((sub >> 1) + (lane >> 3)) & 3 : (sub + (lane >> 3) + 4 * j) & 7;
                     uint4 w = make_uint4(0u, 0u, 0u, 0u);
-                    if (!zeros && piece * 16 < c.stride) w = *reinterpret_cast<const uint4*>(from + (block * kKvBlock + 8 * r8 + sub) * c.stride + piece * 16);
+                    if (!zeros && piece * 16 < c.stride) w = *reinterpret_cast<const uint4*>(from + (8 * r8 + sub) * c.stride + piece * 16);
                     uint4 lo, hi;
                     decode4<FORMAT>(w.x, lo.x, lo.y);
                     decode4<FORMAT>(w.y, lo.z, lo.w);
@@ -518,20 +517,38 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cac
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
         };
+        const uint8_t* const pages = side ? c.values : c.keys;
+        const uint32_t bytes = (uint32_t)(kKvBlock * c.stride);
+        unsigned issued = 0;
+        const auto fetch = [&](int t, int slot) {             // step t's block, if it is there, by one bulk copy (a warp that issued them for all took 200 cycles each)
+            const int i = t >> 1;
+            if (!pair_wait(&m_full[i % kAhead], (uint32_t)(i / kAhead) & 1u, polls)) { ok = false; return; }
+            if (lane == 0) {
+                const int page = __float_as_int(blocks[i % kAhead][4 * (t & 1) + block].w);
+                mbar_arrive_expect_tx(&arrived_codes[slot], page >= 0 ? bytes : 0u);
+                if (page >= 0) {
+                    const int in_page = (int)(((long long)from * kKeys + (long long)t * kStepKeys + block * kKvBlock) & ((1 << c.page_shift) - 1));
+                    bulk_g2s(mine + slot * (T::kCodes / 4), pages + ((((size_t)page * c.kv_heads + work.head) << c.page_shift) + in_page) * c.stride, bytes, &arrived_codes[slot]);
+                }
+            }
+            ++issued;
+        };
+        for (int t = 0; ok && t < min(kDepth, steps); ++t) fetch(t, t);
         Turn<kStages> out;
         Turn<kDepth> in;
 #pragma unroll 1
-        for (int t = 0; t < steps; ++t, out.next(), in.next()) {
-            if (!pair_wait(&c_full[side][in.at], in.phase, polls) || (t >= kStages && !pair_wait(&empty[out.at], out.phase ^ 1u, polls))) { ok = false; break; }
+        for (int t = 0; ok && t < steps; ++t, out.next(), in.next()) {
+            if (!pair_wait(&arrived_codes[in.at], in.phase, polls) || (t >= kStages && !pair_wait(&empty[out.at], out.phase ^ 1u, polls))) { ok = false; break; }
             const int slot = (t >> 1) % kAhead, bit = 4 * (t & 1) + block;
             const uint3 of = which[slot];
-            lay(from_codes + in.at * T::kCodes, ring + out.at * T::kSide, !(of.x >> bit & 1u) || (side && (of.y >> bit & 1u)));
+            lay(mine + in.at * (T::kCodes / 4), ring + out.at * T::kSide, !(of.x >> bit & 1u) || (side && (of.y >> bit & 1u)));
             if (lane == 0) {
                 mbar_arrive(&full[out.at]);
-                mbar_arrive(&c_empty[side][in.at]);
                 if ((t & 1) || t + 1 == steps) mbar_arrive(&m_empty[slot]);
             }
+            if (t + kDepth < steps) fetch(t + kDepth, in.at); // (all lanes have read what lay there: lay ends with a barrier of the warp)
         }
+        if (!ok && lane == 0) copies_landed(arrived_codes, kDepth, issued);              // (nothing arrives behind the kernel)
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
         find_largest();
@@ -601,8 +618,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cac
                 return page >= 0 ? make_float2(c.key_scales[at], c.value_scales[at]) : make_float2(0.f, 0.f);
             };
             int page = page_of(0), page_next = page_of(1);
-            unsigned issued[2] = {0, 0};                      // steps whose copies are on their way, keys and values
-            Turn<kDepth> to;
             float2 scales = scales_of(page);
 #pragma unroll 1
             for (int i = 0; i < n; ++i) {
@@ -621,24 +636,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cac
                 if (lane == 0) which[slot] = make_uint3(there & 0xffu, zeros & 0xffu, numbers & 0xffu);
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&m_full[slot]);
-                // the codes of its steps, a copy per block, as soon as what lay there has been read
-                const uint32_t bytes = (uint32_t)(kKvBlock * c.stride);
-                const size_t at = ((((size_t)max(page_now, 0) * c.kv_heads + work.head) << c.page_shift) + (size_t)((((long long)from + i) * kKeys + lane * kKvBlock) & ((1 << c.page_shift) - 1))) * c.stride;
-                for (int t = 2 * i; ok && t < min(2 * i + 2, steps); ++t, to.next()) {
-                    for (int side = 0; side < 2; ++side) {
-                        if (t >= kDepth && !pair_wait(&c_empty[side][to.at], to.phase ^ 1u, polls)) { ok = false; break; }
-                        if (lane == 0) mbar_arrive_expect_tx(&c_full[side][to.at], bytes * __popc(there >> (4 * (t & 1)) & 0xfu));
-                        __syncwarp();
-                        if (lane >> 2 == (t & 1) && page_now >= 0)
-                            bulk_g2s(codes + (side * kDepth + to.at) * T::kCodes + (lane & 3) * bytes, (side ? c.values : c.keys) + at, bytes, &c_full[side][to.at]);
-                        issued[side] = t + 1;
-                    }
-                }
-                if (!ok) break;
-            }
-            if (!ok && lane == 0) {                           // (nothing arrives behind the kernel)
-                copies_landed(c_full[0], kDepth, issued[0]);
-                copies_landed(c_full[1], kDepth, issued[1]);
             }
         }
     }
