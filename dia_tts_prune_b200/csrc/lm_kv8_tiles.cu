@@ -148,6 +148,11 @@ __device__ __forceinline__ void tmem_load32(uint32_t addr, float* v) {
 #pragma unroll
     for (int e = 0; e < 32; ++e) v[e] = __uint_as_float(u[e]);
 }
+__device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t (&v)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+                 "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+                 : "memory");
+}
 __device__ __forceinline__ void tmem_store32(uint32_t addr, const uint32_t (&v)[32]) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
@@ -344,34 +349,34 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cac
         for (int t = 0; t < count; ++t) {
             const int i = t >> 1, half = t & 1, slot = i % kAhead;
             if (half == 0 && !pair_wait(&m_full[slot], (uint32_t)(i / kAhead) & 1u, polls)) { ok = false; break; }
-            const uint32_t there = which[slot].x >> (4 * half), numbers = which[slot].z >> (4 * half);
+            const uint32_t numbers = which[slot].z >> (4 * half);
             const float4* const meta_of = &blocks[slot][4 * half];
             const int tok = t * kStepKeys;
             const uint32_t t_s = t_scores + kStepKeys * half;
-            const bool clear = (there & numbers & 0xfu) == 0xfu && tok + kStepKeys - 1 <= all_hi && tok >= all_lo;
+            const bool clear = (numbers & 0xfu) == 0xfu && tok + kStepKeys - 1 <= all_hi && tok >= all_lo;
             if (!pair_wait(&s_full[g][half], i & 1, polls)) { ok = false; break; }
             fence_after();
+            if (!clear) {
+                // What a row does not see is -infinity, what it sees of a page that stands for NaNs is NaN: 16 scores a turn, in tensor memory, since this code should be short (it is
+                // rarely needed, and what is in the loop at all costs all of it instruction fetches: 193 -> 181 us, 512 rows behind 16384, without 450 instructions for it)
+                const unsigned first = (unsigned)(lo - tok), many = (unsigned)(hi - lo);      // (what it sees in turn; nothing: hi is -1, or below lo)
+                const bool none = hi < tok || hi < lo;
+#pragma unroll 1
+                for (int b = 0; b < 4; ++b) {
+                    uint32_t v[16];
+                    tmem_columns16(t_s + 16 * b, v);
+                    tmem_loaded();
+                    const bool nan = !(numbers >> b & 1u);
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) v[e] = none || 16 * b + e - first > many ? 0xff800000u : nan ? 0x7fffffffu : v[e];
+                    tmem_store16(t_s + 16 * b, v);
+                }
+                tmem_stored();
+            }
             uint32_t x[2][32];
             tmem_columns32(t_s, x[0]);
             tmem_columns32(t_s + 32, x[1]);
             tmem_loaded();
-            if (!clear) {
-                const unsigned first = (unsigned)(lo - tok), many = (unsigned)(hi - lo);      // (what it sees in turn; nothing: hi is -1, or below lo)
-                const bool none = hi < tok || hi < lo;
-#pragma unroll
-                for (int e = 0; e < kStepKeys; ++e)
-                    if (none || e - first > many) x[e / 32][e % 32] = 0xff800000u;
-                if ((there & numbers & 0xfu) != 0xfu) {                              // pages that are not there, and what a row sees of pages that stand for NaNs
-#pragma unroll
-                    for (int b = 0; b < 4; ++b)
-#pragma unroll
-                        for (int e = 0; e < kKvBlock; ++e) {
-                            uint32_t& v = x[b / 2][16 * (b & 1) + e];
-                            if (!(there >> b & 1u)) v = 0xff800000u;
-                            else if (!(numbers >> b & 1u) && v != 0xff800000u) v = 0x7fffffffu;
-                        }
-                }
-            }
             const auto score = [&](int b, int e) { return __uint_as_float(x[b / 2][16 * (b & 1) + e]); };
             float top = -INFINITY;
 #pragma unroll
@@ -626,13 +631,13 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cac
                 page = page_next;
                 scales = scales_of(page);
                 page_next = page_of(i + 2);
-                // (a page that is not there, or stands for NaNs: the scores say so, and what is times them is finite)
+                // (a page that is not there: its scores are zeros, -infinity with the exponent.  One that stands for NaNs: the scores say so, and what is times them is finite.)
                 const uint32_t k = __float_as_uint(now.x), v = __float_as_uint(now.y);
                 const bool number = page_now >= 0 && k < 0x7f800000u && v < 0x7f800000u;
                 const int e = (int)(v >> 23) - 127 - (largest == -1000 ? 0 : largest), kept = number ? max(e, -kSpread) : 0;
                 if (i >= kAhead && !pair_wait(&m_empty[slot], (uint32_t)(i / kAhead + 1) & 1u, polls)) { ok = false; break; }
                 const uint32_t there = __ballot_sync(0xffffffffu, page_now >= 0), zeros = __ballot_sync(0xffffffffu, number && e < -kSpread), numbers = __ballot_sync(0xffffffffu, number || page_now < 0);
-                if (lane < kBlocks) blocks[slot][lane] = make_float4(number ? fmaxf(now.x, 0x1p-126f) : 1.f, (float)kept, __uint_as_float((uint32_t)(127 - kept) << 23), __int_as_float(page_now));
+                if (lane < kBlocks) blocks[slot][lane] = make_float4(number ? fmaxf(now.x, 0x1p-126f) : 1.f, page_now < 0 ? -INFINITY : (float)kept, __uint_as_float((uint32_t)(127 - kept) << 23), __int_as_float(page_now));
                 if (lane == 0) which[slot] = make_uint3(there & 0xffu, zeros & 0xffu, numbers & 0xffu);
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&m_full[slot]);
