@@ -352,6 +352,11 @@ class Kv8:
                                    self.kv_heads, self.page_size, self.dim, _KV8_FORMATS[format])
         self._at, self._index = C.addressof(self._handle), self.keys.get_device()
 
+    def __setattr__(self, name, value):
+        if hasattr(self, "_index"):                               # (the handle has their addresses)
+            raise AttributeError(f"{name} of a Kv8 stays what it was made with: write into its tensors instead")
+        object.__setattr__(self, name, value)
+
     @property
     def device(self) -> torch.device:
         return self.keys.device
@@ -451,8 +456,9 @@ def attention_kv8(q: torch.Tensor, cache: Kv8, table: torch.Tensor, past: torch.
     ``exp(scale * q . k)``, ``scale`` ``dim ** -0.5`` unless given, and ``sinks [heads]`` (float32) adds ``exp(sinks[h])`` to the denominator.  A row that sees
     nothing, and a row of no sequence, is zeros.
 
-    float32 rows are multiplied with 22 bits, as the language models' attention does; weights are rounded to 22 bits for them, to 11 for the other types.
-    Maxima, sums and outputs are float32 until the result.  It has no gradient."""
+    float32 rows are multiplied with 22 bits, as the language models' attention does; weights are rounded to 22 bits for them, to 11 for the other types (a
+    token whose part in a row's result is below 2^-20 of what the largest one's may be, to 2^-31 of that).  Maxima, sums and outputs are float32 until the
+    result.  Values in pages whose power is 2^80 below the largest in a sequence's pages may be taken as zeros.  It has no gradient."""
     _check_rows(q, "q")
     if not isinstance(cache, Kv8):
         raise TypeError("cache must be a Kv8")

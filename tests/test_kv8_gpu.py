@@ -3,11 +3,16 @@
 Written numbers and numbers read back are the definition's bits.  Attention: with u half a step of the output's type, w what a weight is rounded
 by (2^-11 as one fp16 term, 2^-22 as two), A the largest sum of |scale q k| of a row's tokens and B its sum of p |v| over the denominator,
 
-    |error| <= u |o| + B (w + 2 e + 2^-20),   e = A (2^-22 + (D terms / 16 + 8) 2^-23)
+    |error| <= u |o| + B (w + 2 e + 2^-20) + T V s,   e = A (2^-22 + (D terms / 16 + 8) 2^-23)
 
 e bounds a score's error: queries of fp32 rows have 22 bits, the tensor core cuts a sum off once per 16 channels and term by up to 2^-23 of it, and the scale, the page's
 power and the exponent's argument are rounded; the error of a weight relative to the others is at most twice that.  2^-20: the exponentials (2^-22 each) and the sums of
-weights and outputs."""
+weights and outputs.
+
+T V s, T tokens and V their largest value: small weights.  A weight is fp16 2^(t - R + 7), t = x + e - E with x its score in powers of two, 2^e its page's step and 2^E the largest
+page's.  Below 2^-14 fp16 has steps of 2^-24, so it is off by up to 2^-25 whatever its size.  R is the t of a token that was seen, and e <= E, so the denominator, which has that token's
+2^(x - R + 7) = 2^(t - R + 7 + E - e), is at least 2^7.  A code is at most c = 448 (127), so a token adds at most 2^-25 c 2^E / 2^7; and c 2^E < 2 V, as E is the smallest exponent for
+V.  That is s = 2^-31.  (Few rows count from 2^14, not 2^7, and the two terms of fp32 rows leave 2^-25 too: 2^-38.)"""
 
 import math
 
@@ -127,7 +132,8 @@ def check_attention(got, q, cache, table, past, counts, scale=None, window=None,
             m = min(256, n - r)
             o, A, B = exact_attention(q[at + r:at + r + m].double(), k.double(), v.double(), there, past[i] + r, scale, window, sinks)
             e = A * (2.0 ** -22 + (D * terms / 16 + 8) * 2.0 ** -23)
-            bound = HALF[dtype] * o.abs() + B * ((2.0 ** -22 if terms == 2 else 2.0 ** -11) + 2 * e + 2.0 ** -20) + (2.0 ** -25 if dtype == torch.float16 else 1e-37)
+            small = total * float(v.nan_to_num().abs().max()) * 2.0 ** (-38 if terms == 2 else -31)
+            bound = HALF[dtype] * o.abs() + small + B * ((2.0 ** -22 if terms == 2 else 2.0 ** -11) + 2 * e + 2.0 ** -20) + (2.0 ** -25 if dtype == torch.float16 else 1e-37)
             err = (got[at + r:at + r + m].double() - o).abs()
             assert torch.equal(torch.isnan(err), torch.isnan(o)), "NaN in other places"
             worst = torch.where(torch.isnan(err), 0.0, err - bound).max()
@@ -515,3 +521,130 @@ def test_another_device_than_the_current_one():
     table, past, first = (ints(y).to("cuda:1") for y in ([[0, 1]], [0], [0, 20]))
     cache.append(x[:, :2], x[:, 2:], table, past, first)
     assert torch.isfinite(lm_ops.attention_kv8(x, cache, table, past, first)).all()
+
+
+# ---- where one way of doing it ends and another begins ----------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("fmt,group,dim,page,past,counts,window,width", [
+    ("e4m3", 4, 128, 16, [0], [16], None, None),                    # 64 pairs of token and head
+    ("e4m3", 4, 128, 16, [5], [17], None, None),
+    ("int8", 4, 64, 32, [70, 3, 0, 2000], [16, 17, 64, 65], None, None),
+    ("e4m3", 1, 64, 16, [0, 0, 0, 0, 300], [64, 65, 256, 257, 1], None, None),
+    ("int8", 8, 128, 64, [5000, 9000], [33, 9], None, None),       # keys in chunks, and a sequence of few rows beside
+    ("e4m3", 8, 112, 128, [40000], [70], None, None),
+    ("e4m3", 2, 128, 16, [6000, 0, 64, 1], [129, 3, 200, 128], 777, None),
+    ("int8", 1, 80, 16, [127, 128, 129], [129, 128, 127], None, None),
+    ("e4m3", 4, 128, 16, [500, 600], [1, 2], None, 128),            # tables of 2048 tokens and of more
+    ("e4m3", 4, 128, 16, [500, 600], [1, 2], None, 129),
+    ("int8", 2, 64, 128, [2000, 17, 0], [1, 1, 1], None, 40),
+])
+def test_borders_between_ways(fmt, group, dim, page, past, counts, window, width, dtype):
+    """Scores of many sizes: every row has tokens of its own anywhere in reach that take most of its weight."""
+    g = torch.Generator().manual_seed(sum(counts) + dim)
+    total = [p + n for p, n in zip(past, counts)]
+    pages = sum(-(-t // page) for t in total) + 2
+    lists, table = tables(counts, past, page, pages, g, width)
+    cache = lm_ops.Kv8(pages, 2, dim, page_size=page, format=fmt)
+    k, v = torch.randn(sum(total), 2, dim, generator=g), torch.randn(sum(total), 2, dim, generator=g)
+    v *= torch.exp2(torch.randint(-3, 4, (sum(total), 1, 1), generator=g).double()).float()
+    q = torch.randn(sum(counts), 2 * group, dim, generator=g)
+    at = row = 0
+    for p, n in zip(past, counts):
+        for i in range(n):
+            low = max(0, p + i + 1 - (window or 1 << 40))
+            own = torch.randint(low, p + i + 1, (2 * group,), generator=g)
+            q[row + i] += k[at + own, torch.arange(2 * group) // group] * torch.randint(0, 3, (2 * group, 1), generator=g)
+        at, row = at + p + n, row + n
+    cache.append(k.to(DEV), v.to(DEV), table, ints([0] * len(past)), cumulative(total))
+    q = q.to(dtype).to(DEV)
+    got = lm_ops.attention_kv8(q, cache, table, ints(past), cumulative(counts), window=window)
+    check_attention(got, q, cache, table, past, counts, window=window, lists=lists)
+    assert torch.equal(got, lm_ops.attention_kv8(q, cache, table, ints(past), cumulative(counts), window=window))
+
+
+def test_rows_behind_the_last_sequence_and_between_none():
+    """Rows in front of the first sequence's, behind the last one's, and of sequences that have none: zeros, whichever way the others go."""
+    g = torch.Generator().manual_seed(13)
+    lists, table, cache = filled(g, "e4m3", 2, 64, 16, [30, 0, 10, 50], [20, 0, 90, 1])
+    q = torch.randn(130, 8, 64, generator=g).bfloat16().to(DEV)
+    past = ints([30, 0, 10, 50])
+    want = lm_ops.attention_kv8(q[7:118], cache, table, past, cumulative([20, 0, 90, 1]))
+    check_attention(want, q[7:118], cache, table, [30, 0, 10, 50], [20, 0, 90, 1], lists=lists)
+    got = lm_ops.attention_kv8(q, cache, table, past, ints([7, 27, 27, 117, 118]))
+    assert not got[:7].any() and not got[118:].any() and torch.equal(got[7:118], want)
+    one = lm_ops.attention_kv8(q, cache, table[2:3], past[2:3], ints([27, 117]))             # (a step of one sequence)
+    assert not one[:27].any() and not one[117:].any()
+    check_attention(one[27:117], q[27:117], cache, table[2:3], [10], [90], lists=lists[2:3])
+    none = lm_ops.attention_kv8(q, cache, table, ints([-1, -5, -2 ** 31, -1]), ints([7, 27, 27, 117, 118]))
+    assert not none.any()
+
+
+def test_positions_far_beyond_the_table():
+    """Lengths that no table holds, up to the largest there are: what is there is seen, the rest is not."""
+    g = torch.Generator().manual_seed(14)
+    cache = lm_ops.Kv8(4, 1, 64)
+    table = ints([[0, 1, 2, 3]])
+    x = torch.randn(64, 2, 64, generator=g).to(DEV)
+    cache.append(x[:, :1], x[:, 1:], table, ints([0]), ints([0, 64]))
+    keys = cache.keys.clone()
+    for rows in (1, 90):
+        q = torch.randn(rows, 4, 64, generator=g).bfloat16().to(DEV)
+        want = lm_ops.attention_kv8(q, cache, table, ints([63]), ints([0, rows]))
+        for past in (64, 100, 5000, 2 ** 30, 2 ** 31 - 1):
+            got = lm_ops.attention_kv8(q, cache, table, ints([past]), ints([0, rows]))
+            assert torch.isfinite(got).all() and (got.float() - want.float()).abs().max() < 2.0 ** -5
+            assert not lm_ops.attention_kv8(q, cache, table, ints([past]), ints([0, rows]), window=1)[1:].any()
+            y = torch.randn(rows, 2, 64, generator=g).to(DEV)
+            cache.append(y[:, :1], y[:, 1:], table, ints([past]), ints([0, rows]))
+            assert torch.equal(cache.keys, keys) and not cache.read(table, ints([past]), ints([0, rows]), rows)[0].any()
+
+
+def test_a_mixed_step_in_a_captured_graph():
+    """Prompts beside decoding sequences; which is which, and how long, is read anew by every replay.  Two graphs in turn share nothing."""
+    g = torch.Generator().manual_seed(15)
+    lists, table, cache = filled(g, "int8", 2, 128, 16, [3000, 300, 2500, 80], [64] * 4)
+    q = torch.randn(128, 8, 128, generator=g).bfloat16().to(DEV)
+    past, first = ints([0] * 4), ints([0] * 5)
+    steps = [([2990, 300, 7, 0], [1, 64, 1, 62]), ([0, 299, 2500, 80], [60, 1, 60, 1]), ([3000, 0, 1, 5], [0, 0, 64, 0]), ([2999, 17, 2000, 3], [1, 1, 1, 1])]
+    lm_ops.attention_kv8(q, cache, table, past, first)
+    graphs = []
+    for window in (None, 500):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = lm_ops.attention_kv8(q, cache, table, past, first, window=window)
+        graphs.append((graph, out, window))
+    for p, n in steps + steps[::-1]:
+        past.copy_(ints(p))
+        first.copy_(cumulative(n))
+        for graph, out, window in graphs:
+            graph.replay()
+        for graph, out, window in graphs:
+            assert torch.equal(out, lm_ops.attention_kv8(q, cache, table, past, first, window=window))
+            check_attention(out, q, cache, table, p, n, window=window, lists=lists)
+
+
+@pytest.mark.parametrize("past,counts", [([300], [200]), ([9000], [40]), ([20, 900], [100, 1])])
+def test_a_wait_that_ran_out_shows(past, counts):
+    """With no looks at any barrier every wait ends at once: results of many rows are NaN, the next call reports it, the one behind is whole again."""
+    import ctypes as C
+
+    from dia_tts_prune_b200 import _lm_lib
+    g = torch.Generator().manual_seed(16)
+    lists, table, cache = filled(g, "e4m3", 2, 128, 16, past, counts)
+    q = torch.randn(sum(counts), 8, 128, generator=g).bfloat16().to(DEV)
+    call = lambda: lm_ops.attention_kv8(q, cache, table, ints(past), cumulative(counts))          # noqa: E731
+    polls = getattr(_lm_lib.load(), "_ZN3dia15gemm_pair_pollsEv")
+    polls.restype = C.POINTER(C.c_uint)
+    want, kept = call(), polls()[0]
+    polls()[0] = 0
+    try:
+        got = call()
+    finally:
+        polls()[0] = kept
+    torch.cuda.synchronize()
+    assert got[:counts[0]].isnan().all() and torch.equal(got[counts[0]:], want[counts[0]:])
+    with pytest.raises(RuntimeError):
+        call()
+    for _ in range(3):
+        assert torch.equal(call(), want)
