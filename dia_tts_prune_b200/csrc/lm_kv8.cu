@@ -357,13 +357,16 @@ __device__ __forceinline__ int piece_at(int r, int c) {
     else return r * DP + ((c ^ ((r & 2) | (((r << 2) ^ r) & 4))) << 4);
 }
 
-// Blocks of 16 tokens that a sequence's rows look at, and its share of the work
+// Blocks of 16 tokens that a sequence's rows look at, and its share of the work.  run: blocks that a CTA takes of one tile, which then goes in equal parts of at most so many, a unit
+// each; 0: units are blocks, which CTAs take in a row across tiles, and a tile costs kTileCost more: its rows are laid out and its warps' sums met, which takes 3 us (64 requests of up to 24576
+// tokens: 252 us without, 242 with 16, 228 with 32, 226 with 48, 231 with 96; 256 requests of up to 1000: 178, 115, 101, 100, 113)
+constexpr int kWholeRun = 0x7fffffff, kTileCost = 48;
 struct Span {
-    int begin, n, past, low, blocks, tiles, share;            // low: the first block; share: units of work in a tile: its blocks, or 1 where none is shared
+    int begin, n, past, low, blocks, tiles, share;            // low: the first block; share: units of work in a tile
     __device__ __forceinline__ long long units(int kv_heads) const { return (long long)kv_heads * tiles * share; }
 };
 template <int ROWS>
-__device__ __forceinline__ Span span_of(const Kv8Step& s, const Kv8Attention& a, int i, int group, int page_shift) {
+__device__ __forceinline__ Span span_of(const Kv8Step& s, const Kv8Attention& a, int i, int group, int page_shift, int run) {
     Span p;
     p.begin = s.begin(i);
     p.n = max(s.end(i) - p.begin, 0);
@@ -372,43 +375,58 @@ __device__ __forceinline__ Span span_of(const Kv8Step& s, const Kv8Attention& a,
     const long long end = min((long long)max(p.past, 0) + p.n, (long long)s.max_pages << page_shift);
     p.blocks = max(1, (int)((end + kKvBlock - 1) / kKvBlock) - p.low);
     p.tiles = (long long)p.n * group > a.few_most ? 0 : (p.n * group + ROWS - 1) / ROWS;
-    p.share = a.whole ? 1 : p.blocks;
+    p.share = run == 0 ? p.blocks + kTileCost : (int)(((long long)p.blocks + run - 1) / run);
     return p;
 }
 
-// The sequence that holds the unit `per * nth` of all, where per = what a CTA takes: a block for every warp at least, unless that is more than any tile has (one warp; seq < 0:
-// there is none)
+// The sequence that holds the unit `per * nth` of all, where per = what a CTA takes (one warp; seq < 0: there is none).  Where there are two CTAs for a tile, no CTA has parts of two:
+// parts of `run` blocks are as many as the CTAs, and two blocks for every warp at least (eight requests of 4096 tokens: 23 us as units in a row, 21 so; five of at most 1024: 31 and 17,
+// beside prompt portions 52 with one block for a warp and 42 with two).
 struct Place {
-    int seq;
+    int seq, run;
     long long base, per, total;
 };
 template <int ROWS>
 __device__ __forceinline__ Place find_place(const Kv8Step& s, const Kv8Attention& a, int kv_heads, int group, int page_shift, int ctas, int warps, int nth) {
     const int lane = threadIdx.x & 31, each = (s.sequences + 31) / 32, i0 = lane * each, i1 = min(i0 + each, s.sequences);
-    long long mine = 0;
-    int longest = 0;
-    for (int i = i0; i < i1; ++i) {
-        const Span p = span_of<ROWS>(s, a, i, group, page_shift);
-        mine += p.units(kv_heads);
-        if (p.tiles) longest = max(longest, p.share);
+    const Span first = span_of<ROWS>(s, a, min(i0, s.sequences - 1), group, page_shift, kWholeRun);       // (a lane's only one, mostly)
+    const auto at = [&](int i, int run) {
+        if (i != i0) return span_of<ROWS>(s, a, i, group, page_shift, run);
+        Span p = first;
+        p.share = run == 0 ? p.blocks + kTileCost : (int)(((long long)p.blocks + run - 1) / run);
+        return p;
+    };
+    Place place{-1, kWholeRun, 0, 1, 0};
+    if (!a.whole) {
+        long long blocks = 0, tiles = 0;
+        for (int i = i0; i < i1; ++i) {
+            const Span p = at(i, kWholeRun);
+            tiles += p.units(kv_heads);
+            blocks += p.units(kv_heads) * p.blocks;
+        }
+#pragma unroll
+        for (int d = 16; d; d >>= 1) {
+            tiles += __shfl_xor_sync(0xffffffffu, tiles, d);
+            blocks += __shfl_xor_sync(0xffffffffu, blocks, d);
+        }
+        place.run = 2 * tiles <= ctas ? max((int)((blocks + ctas - tiles - 1) / (ctas - tiles)), 2 * warps) : 0;
     }
-    longest = (int)__reduce_max_sync(0xffffffffu, (unsigned)longest);
+    long long mine = 0;
+    for (int i = i0; i < i1; ++i) mine += at(i, place.run).units(kv_heads);
     long long upto = mine;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
         const long long o = __shfl_up_sync(0xffffffffu, upto, d);
         if (lane >= d) upto += o;
     }
-    Place place;
     place.total = __shfl_sync(0xffffffffu, upto, 31);
-    place.per = max((place.total + ctas - 1) / ctas, (long long)max(min(warps, longest), 1));
-    place.seq = -1;
+    place.per = max((place.total + ctas - 1) / ctas, place.run ? 1ll : (long long)warps);
     place.base = upto - mine;
     const long long unit = place.per * nth;
     const bool here = unit >= place.base && unit < upto;
     if (here) {
         for (place.seq = i0;; ++place.seq) {
-            const long long u = span_of<ROWS>(s, a, place.seq, group, page_shift).units(kv_heads);
+            const long long u = at(place.seq, place.run).units(kv_heads);
             if (unit < place.base + u) break;
             place.base += u;
         }
@@ -448,18 +466,20 @@ __global__ void __launch_bounds__(Few<DP, TERMS, NT>::kThreads, Few<DP, TERMS, N
     Place at = place;
     long long unit = at.seq < 0 ? at.total : at.per * blockIdx.x;
     const long long unit_end = min(unit + at.per, at.total);
-    Span sp = span_of<kRows>(s, a, max(at.seq, 0), group, c.page_shift);
+    Span sp = span_of<kRows>(s, a, max(at.seq, 0), group, c.page_shift, at.run);
 
     while (unit < unit_end) {
         while (unit >= at.base + sp.units(c.kv_heads)) {                             // (sequences without rows have no units)
             at.base += sp.units(c.kv_heads);
-            sp = span_of<kRows>(s, a, ++at.seq, group, c.page_shift);
+            sp = span_of<kRows>(s, a, ++at.seq, group, c.page_shift, at.run);
         }
         const long long item = (unit - at.base) / sp.share;
-        const int b0 = (int)(unit - at.base - item * sp.share), taken = (int)min((long long)sp.share - b0, unit_end - unit), count = a.whole ? sp.blocks : taken;
+        const int u0 = (int)(unit - at.base - item * sp.share), taken = at.run ? 1 : (int)min((long long)sp.share - u0, unit_end - unit);
+        const int b0 = at.run ? (int)((long long)u0 * sp.blocks / sp.share) : u0, b1 = at.run ? (int)((long long)(u0 + 1) * sp.blocks / sp.share) : min(u0 + taken, sp.blocks), count = b1 - b0;
         const int head = (int)(item / sp.tiles), tile = (int)(item - (long long)head * sp.tiles);
         const int p0 = tile * kRows, rows = min(kRows, sp.n * group - p0);
         unit += taken;
+        if (count <= 0) continue;                                                    // (what a tile costs besides)
         // positions of the tile's rows, first and last
         const auto position = [&](int r) { return (long long)sp.past + (p0 + min(r, rows - 1)) / group; };
         const long long back = a.window > 0 ? a.window - 1 : (1ll << 40);
@@ -744,7 +764,7 @@ __global__ void __launch_bounds__(Few<DP, TERMS, NT>::kThreads, Few<DP, TERMS, N
         if (!whole) {
             // Runs c0 to c1 share the tile; the last of them to come joins all, in their order.  (A run is the first one of at most one shared tile, whose counter it lends.)
             const long long start = at.base + item * sp.share;
-            const int c0 = (int)(start / at.per), c1 = (int)((start + sp.share - 1) / at.per);
+            const int c0 = (int)(start / at.per), c1 = (int)((start + (at.run ? sp.share : sp.blocks) - 1) / at.per);
             __threadfence();
             __syncthreads();
             if (threadIdx.x == 0) last = atomicAdd(arrived + c0, 1u) == (unsigned)(c1 - c0);
