@@ -439,7 +439,7 @@ __device__ __forceinline__ Place find_place(const Kv8Step& s, const Kv8Attention
 }
 
 template <int DP, int FORMAT, int TERMS, int NT>
-__global__ void __launch_bounds__(Few<DP, TERMS, NT>::kThreads, Few<DP, TERMS, NT>::kPerSm) kv8_attention_few_kernel(Kv8Cache c, Kv8Step s, Kv8Attention a, float* part, RowStats* part_stats, unsigned* arrived) {
+__global__ void __launch_bounds__(Few<DP, TERMS, NT>::kThreads, Few<DP, TERMS, NT>::kPerSm) kv8_attention_few_kernel(Kv8Cache c, Kv8Step s, Kv8Attention a, int beside, float* part, RowStats* part_stats, unsigned* arrived) {
     using F = Few<DP, TERMS, NT>;
     constexpr int kSteps = DP / 16, kHalves = DP == 256 ? 2 : 1, kWords = DP == 64 ? 2 : 4, kCols = kHalves * kWords * 2, kWarps = F::kWarps, kRows = F::kRows;
     extern __shared__ __align__(128) uint8_t smem[];
@@ -767,7 +767,10 @@ __global__ void __launch_bounds__(Few<DP, TERMS, NT>::kThreads, Few<DP, TERMS, N
             const int c0 = (int)(start / at.per), c1 = (int)((start + (at.run ? sp.share : sp.blocks) - 1) / at.per);
             __threadfence();
             __syncthreads();
-            if (threadIdx.x == 0) last = atomicAdd(arrived + c0, 1u) == (unsigned)(c1 - c0);
+            if (threadIdx.x == 0) {
+                if (!beside) asm volatile("griddepcontrol.wait;" ::: "memory");      // (the counters are zeros)
+                last = atomicAdd(arrived + c0, 1u) == (unsigned)(c1 - c0);
+            }
             __syncthreads();
             if (last) {
                 __threadfence();
@@ -842,6 +845,13 @@ __global__ void __launch_bounds__(Few<DP, TERMS, NT>::kThreads, Few<DP, TERMS, N
     asm volatile("griddepcontrol.wait;" ::: "memory");        // (the sequences of many rows, which may still be on their way beside this)
 }
 
+// Zeros for the counters of both kernels, which start meanwhile (a memset in front of them takes 3 us)
+constexpr int kCounterThreads = 512;
+__global__ void kv8_counters_kernel(unsigned* counters, int n) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    for (int i = threadIdx.x; i < n; i += kCounterThreads) counters[i] = 0u;
+}
+
 inline bool wide(const Kv8Rows& x, int type, int dim) {
     const long long b = type_bytes(type);
     return (reinterpret_cast<uintptr_t>(x.x) & 15) == 0 && x.row * b % 16 == 0 && x.head * b % 16 == 0 && dim % 8 == 0;
@@ -856,20 +866,21 @@ inline int padded_dim(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256;
 inline int terms_of(int type) { return type == kTypeF32 ? 2 : 1; }
 
 template <int DP, int FORMAT, int TERMS, int NT>
-cudaError_t run_few(const Kv8Cache& c, const Kv8Step& s, const Kv8Attention& a, bool beside, const FewWork& work, cudaStream_t st) {
+cudaError_t run_few(const Kv8Cache& c, const Kv8Step& s, const Kv8Attention& a, bool early, bool beside, const FewWork& work, cudaStream_t st) {
     using F = Few<DP, TERMS, NT>;
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e == cudaSuccess) e = dia::ask_smem<kv8_attention_few_kernel<DP, FORMAT, TERMS, NT>>(dev, F::kSmem);
     if (e != cudaSuccess) return e;
-    return launch_pdl_if(beside, kv8_attention_few_kernel<DP, FORMAT, TERMS, NT>, dim3(F::kCtas), dim3(F::kThreads), F::kSmem, st, c, s, a, work.part, work.stats, work.arrived);
+    return launch_pdl_if(early, kv8_attention_few_kernel<DP, FORMAT, TERMS, NT>, dim3(F::kCtas), dim3(F::kThreads), F::kSmem, st, c, s, a, beside, work.part, work.stats, work.arrived);
 }
 template <int DP, int FORMAT>
 cudaError_t run_few(const Kv8Cache& c, const Kv8Step& s, const Kv8Attention& a, bool beside, const FewWork& work, cudaStream_t st) {
+    const bool early = !a.whole;                              // (behind the counters' kernel, or the tiles')
     // tiles of eight rows where sequences have no more of them on average (the products of 16 rows take twice the registers and the tensor cores' time)
     const bool eight = (long long)s.rows * (a.heads / c.kv_heads) <= 8ll * s.sequences;
-    if (terms_of(a.type) == 2) return eight ? run_few<DP, FORMAT, 2, 1>(c, s, a, beside, work, st) : run_few<DP, FORMAT, 2, 2>(c, s, a, beside, work, st);
-    return eight ? run_few<DP, FORMAT, 1, 1>(c, s, a, beside, work, st) : run_few<DP, FORMAT, 1, 2>(c, s, a, beside, work, st);
+    if (terms_of(a.type) == 2) return eight ? run_few<DP, FORMAT, 2, 1>(c, s, a, early, beside, work, st) : run_few<DP, FORMAT, 2, 2>(c, s, a, early, beside, work, st);
+    return eight ? run_few<DP, FORMAT, 1, 1>(c, s, a, early, beside, work, st) : run_few<DP, FORMAT, 1, 2>(c, s, a, early, beside, work, st);
 }
 
 }  // namespace
@@ -925,8 +936,13 @@ cudaError_t launch_kv8_attention(const Kv8Cache& c, const Kv8Step& s, Kv8Attenti
     unsigned* const counters = reinterpret_cast<unsigned*>(work);
     float* const part = reinterpret_cast<float*>(reinterpret_cast<char*>(work) + rounded(kCounters));
     a.whole = !tiles && ((long long)s.max_pages << c.page_shift) <= kWholeTokens;
-    cudaError_t e = a.whole ? cudaSuccess : cudaMemsetAsync(counters, 0, kCounters, st);
-    if (e != cudaSuccess) return e;
+    cudaError_t e = cudaSuccess;
+    if (!a.whole) {
+        kv8_counters_kernel<<<1, kCounterThreads, 0, st>>>(counters, (int)(kCounters / sizeof(unsigned)));
+        e = cudaGetLastError();
+        if (e != cudaSuccess) return e;
+        ++dia::extra_launches();
+    }
     a.few_most = !tiles ? 0x7fffffff : alone ? 0 : kFewMost;
     if (tiles) {
         e = launch_kv8_tiles(c, s, a, alone, reinterpret_cast<char*>(part) + rounded(few_bytes(dp)), counters + kMostCtas, st);

@@ -197,7 +197,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cac
     __shared__ uint64_t q_ready;
     __shared__ Work found;
     __shared__ Sequence found_rows;
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = a.heads / c.kv_heads;
     if (warp == 0) {
         const Work work = find_work(c, s, a, group, blockIdx.x);
@@ -232,8 +231,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cac
     } else if (warp == 16) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&tmem_slot)));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
-    } else if (warp == 19 && alone) {
-        zero_rows_of_none(s, a, c.dim, (long long)blockIdx.x * 32 + lane, (long long)gridDim.x * 32);
+    } else if (warp == 19) {
+        // The counters are zeros behind this; the kernel of the sequences of few rows, which wants them too, may start (its writes are its own)
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+        if (alone) zero_rows_of_none(s, a, c.dim, (long long)blockIdx.x * 32 + lane, (long long)gridDim.x * 32);
     }
     fence_before();
     __syncthreads();
@@ -713,8 +715,7 @@ cudaError_t run_tiles(const Kv8Cache& c, const Kv8Step& s, const Kv8Attention& a
     const long long pairs = (long long)s.rows * (a.heads / c.kv_heads), partly = std::min<long long>(s.sequences, pairs / (a.few_most + 1));
     const long long ctas = std::max<long long>(kSms, c.kv_heads * (pairs / kTileRows + partly));
     if (ctas > 0x7fffffff) return cudaErrorInvalidValue;
-    kv8_attention_tiles_kernel<DP, FORMAT><<<(unsigned)ctas, kThreads, Tiles<DP>::kSmem, st>>>(c, s, a, alone, part, stats, arrived, ran_out, gemm_pair_polls());
-    return cudaGetLastError();
+    return launch_pdl(kv8_attention_tiles_kernel<DP, FORMAT>, dim3((unsigned)ctas), dim3(kThreads), Tiles<DP>::kSmem, st, c, s, a, (int)alone, part, stats, arrived, ran_out, gemm_pair_polls());
 }
 
 }  // namespace
