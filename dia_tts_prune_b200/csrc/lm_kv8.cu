@@ -332,7 +332,7 @@ struct Few {
     static constexpr int kSums = kWarps * kRows * DP * 4 + kCtas * kRows * 4;     // and the weights of runs that share a tile (where the ring lies)
     static constexpr int kSmem = (kRing > kSums ? kRing : kSums) + kQ + kMetaBlocks * 16 + kRows * 4 + kWarps * kRows * 12 + 128;
 };
-constexpr int kMostCtas = 2 * 148;
+constexpr int kMostCtas = 2 * 148, kJoin = 12;                // (runs that are joined in one go: about the root of how many there may be)
 
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint2 b) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -763,21 +763,28 @@ __global__ void __launch_bounds__(Few<DP, TERMS, NT>::kThreads, Few<DP, TERMS, N
         }
         if (!whole) {
             // Runs c0 to c1 share the tile; the last of them to come joins all, in their order.  (A run is the first one of at most one shared tile, whose counter it lends.)
+            // Where they are many, the last of every kJoin in turn joins those, in the first one's place, and the last of these their sums.  (Their counter is lent by the last run
+            // of the kJoin, which is no other tile's but as its first.)
             const long long start = at.base + item * sp.share;
-            const int c0 = (int)(start / at.per), c1 = (int)((start + (at.run ? sp.share : sp.blocks) - 1) / at.per);
-            __threadfence();
-            __syncthreads();
-            if (threadIdx.x == 0) {
-                if (!beside) asm volatile("griddepcontrol.wait;" ::: "memory");      // (the counters are zeros)
-                last = atomicAdd(arrived + c0, 1u) == (unsigned)(c1 - c0);
-            }
-            __syncthreads();
-            if (last) {
+            const int c0 = (int)(start / at.per), all = (int)((start + (at.run ? sp.share : sp.blocks) - 1) / at.per) - c0 + 1;
+            const bool twice = all > 2 * kJoin;
+            const int run0 = (int)blockIdx.x - c0;
+            int from = twice ? run0 / kJoin * kJoin : 0, n = twice ? min(kJoin, all - from) : all, apart = 1;
+#pragma unroll 1
+            for (bool ends = !twice;; ends = true) {
+                __threadfence();
+                __syncthreads();
+                if (threadIdx.x == 0) {
+                    if (!beside) asm volatile("griddepcontrol.wait;" ::: "memory");  // (the counters are zeros)
+                    last = atomicAdd(arrived + c0 + (ends ? 0 : kMostCtas + from + n - 1), 1u) == (unsigned)(n - 1);
+                }
+                __syncthreads();
+                if (!last) break;
                 __threadfence();
                 // rows' weights of the runs first, where the rings lay, then their channels; threads that these leave over take runs of their own
                 float* const weights = sums + kWarps * kRows * DP;                   // [run][row]
-                const int n = c1 - c0 + 1, groups = max(1, min(F::kThreads / tasks, kWarps)), mine = threadIdx.x / tasks;
-                const auto at_run = [&](int v, int r) { return ((size_t)2 * (c0 + v) + (v == 0)) * kRows + r; };
+                const int groups = max(1, min(F::kThreads / tasks, kWarps)), mine = threadIdx.x / tasks;
+                const auto at_run = [&](int v, int r) { const int run = from + v * apart; return ((size_t)2 * (c0 + run) + (run == 0)) * kRows + r; };
                 // (Loads go out many at a time: one after the other, those of 148 runs took 12 us.)
                 for (int r = warp; r < rows; r += kWarps) {
                     constexpr int kMine = (F::kCtas + 31) / 32;
@@ -802,9 +809,16 @@ __global__ void __launch_bounds__(Few<DP, TERMS, NT>::kThreads, Few<DP, TERMS, N
                     }
 #pragma unroll
                     for (int d = 16; d; d >>= 1) top.l += __shfl_xor_sync(0xffffffffu, top.l, d);
-                    if (lane == 0) row_scale[r] = row_factor(a, head * group + (p0 + r) % group, top.m, top.w, top.l);
+                    if (lane == 0) {
+                        row_scale[r] = row_factor(a, head * group + (p0 + r) % group, top.m, top.w, top.l);
+                        if (!ends) part_stats[at_run(0, r)] = top;
+                    }
                 }
                 __syncthreads();
+                const auto out = [&](int r, int d, const float4& sum) {
+                    if (ends) write(r, d, row_scale[r], sum);
+                    else *reinterpret_cast<float4*>(part + at_run(0, r) * DP + d) = sum;
+                };
                 for (int i = groups == 1 ? threadIdx.x : threadIdx.x % tasks; i < tasks && mine < groups; i += groups == 1 ? F::kThreads : tasks) {
                     const int r = i / (DP / 4), d = i % (DP / 4) * 4;
                     float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -823,7 +837,7 @@ __global__ void __launch_bounds__(Few<DP, TERMS, NT>::kThreads, Few<DP, TERMS, N
                             sum = make_float4(sum.x + f * z[j].x, sum.y + f * z[j].y, sum.z + f * z[j].z, sum.w + f * z[j].w);
                         }
                     }
-                    if (groups == 1) write(r, d, row_scale[r], sum);
+                    if (groups == 1) out(r, d, sum);
                     else *reinterpret_cast<float4*>(sums + (size_t)(mine * kRows + r) * DP + d) = sum;
                 }
                 if (groups > 1) {
@@ -835,9 +849,13 @@ __global__ void __launch_bounds__(Few<DP, TERMS, NT>::kThreads, Few<DP, TERMS, N
                             const float4 z = *reinterpret_cast<const float4*>(sums + (size_t)(v * kRows + r) * DP + d);
                             sum = make_float4(sum.x + z.x, sum.y + z.y, sum.z + z.z, sum.w + z.w);
                         }
-                        write(r, d, row_scale[r], sum);
+                        out(r, d, sum);
                     }
                 }
+                if (ends) break;
+                from = 0;
+                n = (all + kJoin - 1) / kJoin;
+                apart = kJoin;
             }
         }
         __syncthreads();                                                             // (the ring and the queries' room are taken again)
@@ -921,7 +939,7 @@ inline bool some_in_tiles(int kv_heads, int dim, int rows, int heads, int type) 
 
 // Counters first: those of both kernels are set to zero in one go.
 namespace {
-constexpr size_t kCounters = (kMostCtas + kKvTileCounters) * sizeof(unsigned);
+constexpr size_t kCounters = (2 * kMostCtas + kKvTileCounters) * sizeof(unsigned);
 inline size_t few_bytes(int dp) { return (size_t)2 * kMostCtas * 16 * (dp * sizeof(float) + sizeof(RowStats)); }
 inline size_t rounded(size_t bytes) { return (bytes + 255) / 256 * 256; }
 }  // namespace
@@ -945,7 +963,7 @@ cudaError_t launch_kv8_attention(const Kv8Cache& c, const Kv8Step& s, Kv8Attenti
     }
     a.few_most = !tiles ? 0x7fffffff : alone ? 0 : kFewMost;
     if (tiles) {
-        e = launch_kv8_tiles(c, s, a, alone, reinterpret_cast<char*>(part) + rounded(few_bytes(dp)), counters + kMostCtas, st);
+        e = launch_kv8_tiles(c, s, a, alone, reinterpret_cast<char*>(part) + rounded(few_bytes(dp)), counters + 2 * kMostCtas, st);
         if (e != cudaSuccess || alone) return e;
         ++dia::extra_launches();
     }

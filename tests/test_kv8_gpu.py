@@ -563,6 +563,21 @@ def test_borders_between_ways(fmt, group, dim, page, past, counts, window, width
     assert torch.equal(got, lm_ops.attention_kv8(q, cache, table, ints(past), cumulative(counts), window=window))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("step", [0, 1, 2])
+def test_long_sequences_among_many(step, dtype):
+    """Runs of work that share a tile, tens of them, beside runs that have many tiles: every border falls elsewhere."""
+    g = torch.Generator().manual_seed(17 + step)
+    past = [5] * 90 + [23000 + 1500 * i + 333 * step for i in range(12)] + [int(x) for x in torch.randint(0, 200, (230,), generator=g)]
+    counts = [1] * len(past)
+    lists, table, cache = filled(g, "e4m3", 1, 64, 16, past, counts)
+    q = torch.randn(len(past), 2, 64, generator=g).to(dtype).to(DEV)
+    got = lm_ops.attention_kv8(q, cache, table, ints(past))
+    check_attention(got, q, cache, table, past, counts, lists=lists)
+    few = lm_ops.attention_kv8(q[90:93], cache, table[90:93], ints(past[90:93]))               # (a part of a tile for every CTA)
+    check_attention(few, q[90:93], cache, table[90:93], past[90:93], [1] * 3, lists=lists[90:93])
+
+
 def test_rows_behind_the_last_sequence_and_between_none():
     """Rows in front of the first sequence's, behind the last one's, and of sequences that have none: zeros, whichever way the others go."""
     g = torch.Generator().manual_seed(13)
