@@ -935,6 +935,7 @@ constexpr int kFewMost = 64;
 // Tables of up to so many tokens: no tile is shared by several CTAs
 constexpr int kWholeTokens = 2048;
 inline bool some_in_tiles(int kv_heads, int dim, int rows, int heads, int type) { return kv8_tiles_ok(dim, type) && (long long)rows * (heads / kv_heads) > kFewMost; }
+inline bool whole_tiles(int kv_heads, int dim, int rows, int heads, int type, long long tokens) { return tokens <= kWholeTokens && !some_in_tiles(kv_heads, dim, rows, heads, type); }
 }  // namespace
 
 // Counters first: those of both kernels are set to zero in one go.
@@ -944,7 +945,8 @@ inline size_t few_bytes(int dp) { return (size_t)2 * kMostCtas * 16 * (dp * size
 inline size_t rounded(size_t bytes) { return (bytes + 255) / 256 * 256; }
 }  // namespace
 
-size_t kv8_attention_work_bytes(int kv_heads, int dim, int rows, int heads, int type) {
+size_t kv8_attention_work_bytes(int kv_heads, int dim, int rows, int heads, int type, long long tokens) {
+    if (whole_tiles(kv_heads, dim, rows, heads, type, tokens)) return 0;
     return rounded(kCounters) + rounded(few_bytes(padded_dim(dim))) + (some_in_tiles(kv_heads, dim, rows, heads, type) ? kv8_tiles_work_bytes(dim) : 0);
 }
 
@@ -953,7 +955,7 @@ cudaError_t launch_kv8_attention(const Kv8Cache& c, const Kv8Step& s, Kv8Attenti
     const bool tiles = some_in_tiles(c.kv_heads, c.dim, s.rows, a.heads, a.type), alone = tiles && s.sequences == 1;        // (alone: in tiles whatever its rows are)
     unsigned* const counters = reinterpret_cast<unsigned*>(work);
     float* const part = reinterpret_cast<float*>(reinterpret_cast<char*>(work) + rounded(kCounters));
-    a.whole = !tiles && ((long long)s.max_pages << c.page_shift) <= kWholeTokens;
+    a.whole = whole_tiles(c.kv_heads, c.dim, s.rows, a.heads, a.type, (long long)s.max_pages << c.page_shift);
     cudaError_t e = cudaSuccess;
     if (!a.whole) {
         kv8_counters_kernel<<<1, kCounterThreads, 0, st>>>(counters, (int)(kCounters / sizeof(unsigned)));

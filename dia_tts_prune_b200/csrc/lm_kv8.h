@@ -74,7 +74,8 @@ struct Kv8Attention {
     int few_most;                                         // (token, query head) pairs per key head of a sequence that tiles of 16 of them take; others go 256 at a time
     int whole;                                            // != 0: a CTA takes whole tiles of 16
 };
-size_t kv8_attention_work_bytes(int kv_heads, int dim, int rows, int heads, int type);
+// (tokens: what a row of the table has room for; 0 bytes: none are needed)
+size_t kv8_attention_work_bytes(int kv_heads, int dim, int rows, int heads, int type, long long tokens);
 cudaError_t launch_kv8_attention(const Kv8Cache& c, const Kv8Step& s, Kv8Attention a, void* work, cudaStream_t st);      // (sets few_most and whole)
 
 // lm_kv8_tiles.cu: the sequences of more than few_most pairs; bf16 or fp16 rows, dim up to 128.  alone: nothing else zeroes the rows of no sequence

@@ -398,7 +398,8 @@ class Kv8:
         if rows < 0:
             raise ValueError("rows must not be negative")
         step = _kv8_step(self, table, past, first, rows)
-        k, v = self.key_scales.new_empty((2, rows, self.kv_heads, self.dim), dtype=dtype).unbind()
+        k = self.key_scales.new_empty((rows, self.kv_heads, self.dim), dtype=dtype)
+        v = torch.empty_like(k)
         if step is None:
             return k.zero_(), v.zero_()
         _call("kv8_read", self.keys.device, self._at, step, k.data_ptr(), v.data_ptr(), _TYPES[dtype])
@@ -409,15 +410,19 @@ class Kv8:
 _KV8_STEP = struct.Struct("@PqPPiii")
 
 
+def _check_ints(t: torch.Tensor, name: str) -> None:
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a tensor")
+    if t.dtype is not torch.int32:
+        raise TypeError(f"{name} must be int32, not {t.dtype}")
+
+
 def _kv8_step(cache: Kv8, table: torch.Tensor, past: torch.Tensor, first: torch.Tensor | None, rows: int) -> bytes | None:
     """The description of a step's rows as the library takes it (None: no row of any sequence)."""
-    for name, t in (("table", table), ("past", past), ("first", first)):
-        if t is None and name == "first":
-            continue
-        if not isinstance(t, torch.Tensor):
-            raise TypeError(f"{name} must be a tensor")
-        if t.dtype is not torch.int32:
-            raise TypeError(f"{name} must be int32, not {t.dtype}")
+    _check_ints(table, "table")
+    _check_ints(past, "past")
+    if first is not None:
+        _check_ints(first, "first")
     if table.dim() != 2:
         raise ValueError("table must be [sequences, pages of one]")
     (n, width), (apart, step) = table.shape, table.stride()
@@ -444,8 +449,8 @@ def _kv8_step(cache: Kv8, table: torch.Tensor, past: torch.Tensor, first: torch.
 
 
 @lru_cache(maxsize=1024)
-def _kv8_work_bytes(kv_heads: int, dim: int, rows: int, heads: int, kind: int) -> int:
-    return _lm_lib.load().lm_b200_op_kv8_attention_work_bytes(kv_heads, dim, rows, heads, kind)
+def _kv8_work_bytes(kv_heads: int, dim: int, rows: int, heads: int, kind: int, tokens: int) -> int:
+    return _lm_lib.load().lm_b200_op_kv8_attention_work_bytes(kv_heads, dim, rows, heads, kind, tokens)
 
 
 def attention_kv8(q: torch.Tensor, cache: Kv8, table: torch.Tensor, past: torch.Tensor, first: torch.Tensor | None = None, *, scale: float | None = None,
@@ -492,8 +497,9 @@ def attention_kv8(q: torch.Tensor, cache: Kv8, table: torch.Tensor, past: torch.
         q = q.contiguous()
         q_row, q_head, _ = q.stride()
     kind = _TYPES[q.dtype]
-    need = _kv8_work_bytes(cache.kv_heads, cache.dim, rows, heads, kind)
-    out, work = q.new_empty(shape), q.new_empty(need, dtype=torch.uint8)
+    need = _kv8_work_bytes(cache.kv_heads, cache.dim, rows, heads, kind, table.size(1) * cache.page_size)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    work = q.new_empty(need, dtype=torch.uint8) if need else None
     _call("kv8_attention", cache.keys.device, cache._at, step, q.data_ptr(), q_row, q_head, heads, kind, scale, window, None if sinks is None else sinks.data_ptr(),
-          out.data_ptr(), work.data_ptr(), need)
+          out.data_ptr(), work.data_ptr() if need else None, need)
     return out

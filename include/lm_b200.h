@@ -366,8 +366,9 @@ int lm_b200_op_kv8_append(const lm_b200_kv8 *cache, const lm_b200_kv8_step *step
 int lm_b200_op_kv8_read(const lm_b200_kv8 *cache, const lm_b200_kv8_step *step, void *k, void *v, int type, void *stream);
 /* out [rows][heads][dim] = attention of q (the same, q_row and q_head apart, of `type`; fp32 is multiplied with 22 bits, fp16 and bf16 as they are) over the tokens at a row's position and
  * before it, the last `window` of them (0: all): weights exp(scale q.k), in the denominator exp(sinks[head]) too (NULL: nothing).  Query head h reads key head h / (heads / kv_heads).  A row
- * that sees nothing, and a row of no sequence, is zeros.  work: lm_b200_op_kv8_attention_work_bytes bytes, 256-byte aligned. */
-size_t lm_b200_op_kv8_attention_work_bytes(int kv_heads, int dim, int rows, int heads, int type);
+ * that sees nothing, and a row of no sequence, is zeros.  work: lm_b200_op_kv8_attention_work_bytes bytes, 256-byte aligned (0:
+ * none; tokens: max_pages x page_size). */
+size_t lm_b200_op_kv8_attention_work_bytes(int kv_heads, int dim, int rows, int heads, int type, int64_t tokens);
 int lm_b200_op_kv8_attention(const lm_b200_kv8 *cache, const lm_b200_kv8_step *step, const void *q, int64_t q_row, int64_t q_head, int heads, int type, float scale, int window,
                              const float *sinks, void *out, void *work, size_t work_bytes, void *stream);
 
