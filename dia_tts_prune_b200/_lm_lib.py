@@ -111,7 +111,7 @@ _SIGNATURES = {
                                    _vp]),
     "lm_b200_op_kv8_append": (_ci, [_vp, _vp, _vp, C.c_int64, C.c_int64, _vp, C.c_int64, C.c_int64, _ci, _vp]),
     "lm_b200_op_kv8_read": (_ci, [_vp, _vp, _vp, _vp, _ci, _vp]),
-    "lm_b200_op_kv8_attention_work_bytes": (C.c_size_t, [_ci, _ci, _ci, _ci, _ci, C.c_int64]),
+    "lm_b200_op_kv8_attention_work_bytes": (C.c_size_t, [_ci, _ci, _ci, _ci, _ci, _ci, C.c_int64]),
     "lm_b200_op_kv8_attention": (_ci, [_vp, _vp, _vp, C.c_int64, C.c_int64, _ci, _ci, _cf, _ci, _vp, _vp, _vp, C.c_size_t, _vp]),
     "lm_b200_argmax_rows": (_ci, [_vp, _ci, _ci, _vp, _vp]),
 }

@@ -1836,8 +1836,8 @@ int lm_b200_op_loss_grad(const void* h, int64_t ldh, const void* W, int64_t ldw,
     return LM_B200_OK;
 }
 
-size_t lm_b200_op_kv8_attention_work_bytes(int kv_heads, int dim, int rows, int heads, int type, int64_t tokens) {
-    return kv8_heads(kv_heads, rows, heads) && dim > 0 && dim <= lm::kKvMostDim && known_type(type) ? lm::kv8_attention_work_bytes(kv_heads, dim, rows, heads, type, tokens) : 0;
+size_t lm_b200_op_kv8_attention_work_bytes(int kv_heads, int dim, int rows, int heads, int type, int n_seq, int64_t tokens) {
+    return kv8_heads(kv_heads, rows, heads) && dim > 0 && dim <= lm::kKvMostDim && known_type(type) && n_seq > 0 ? lm::kv8_attention_work_bytes(kv_heads, dim, rows, heads, type, n_seq, tokens) : 0;
 }
 
 int lm_b200_op_kv8_append(const lm_b200_kv8* cache, const lm_b200_kv8_step* step, const void* k, int64_t k_row, int64_t k_head, const void* v, int64_t v_row, int64_t v_head, int type,
@@ -1863,7 +1863,7 @@ int lm_b200_op_kv8_attention(const lm_b200_kv8* cache, const lm_b200_kv8_step* s
     lm::Kv8Step s;
     if (!kv8_cache(c, cache) || !kv8_step(s, step) || !kv8_heads(c.kv_heads, s.rows, heads) || !q || q_row < 0 || q_head < 0 || !known_type(type) || !loss_scale(scale) || window < 0 || !out)
         return LM_B200_EINVAL;
-    const size_t need = lm::kv8_attention_work_bytes(c.kv_heads, c.dim, s.rows, heads, type, (long long)s.max_pages << c.page_shift);
+    const size_t need = lm::kv8_attention_work_bytes(c.kv_heads, c.dim, s.rows, heads, type, s.sequences, (long long)s.max_pages << c.page_shift);
     if (need > 0 && (!work || !aligned(work, 256) || work_bytes < need)) return LM_B200_EINVAL;
     LCK(lm::launch_kv8_attention(c, s, lm::Kv8Attention{lm::Kv8Rows{q, q_row, q_head}, out, heads, type, scale, window, sinks, 0, 0}, work, S(stream)));
     return LM_B200_OK;

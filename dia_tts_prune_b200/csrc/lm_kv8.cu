@@ -318,7 +318,7 @@ __global__ void __launch_bounds__(kReadThreads) kv8_read_kernel(Kv8Cache c, Kv8S
 // row's largest), or two (fp32: 22 bits).  Weights: the page's value scale is part of the exponent, 2^(x + e - max (x + e)) 2^14, so that the largest contribution, not the largest
 // weight, is what fp16's 11 bits count from (fp32 rows: two terms, 22 bits); sums, maxima and outputs are fp32, and the denominator is summed from fp32 weights without the scale.
 // A tensor-core sum is cut off at every step: fp32 rows add the second terms' sums and every block's outputs to theirs by fp32 additions.
-constexpr int kMetaBlocks = 256;
+constexpr int kMetaBlocks = 256, kMostPeers = 8;               // CTAs of a cluster
 
 template <int DP, int TERMS, int NT>
 struct Few {
@@ -438,6 +438,29 @@ __device__ __forceinline__ Place find_place(const Kv8Step& s, const Kv8Attention
     return place;
 }
 
+// Clusters of CTAs (of one, where a launch has none)
+__device__ __forceinline__ unsigned cluster_size() { unsigned v; asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(v)); return v; }
+__device__ __forceinline__ unsigned cluster_rank() { unsigned v; asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(v)); return v; }
+__device__ __forceinline__ unsigned cluster_index() { unsigned v; asm("mov.u32 %0, %%clusterid.x;" : "=r"(v)); return v; }
+__device__ __forceinline__ void cluster_met() {
+    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t shared_of(const void* p, unsigned rank) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ float load_of(uint32_t at) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 load4_of(uint32_t at) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
+    return v;
+}
+
 template <int DP, int FORMAT, int TERMS, int NT>
 __global__ void __launch_bounds__(Few<DP, TERMS, NT>::kThreads, Few<DP, TERMS, NT>::kPerSm) kv8_attention_few_kernel(Kv8Cache c, Kv8Step s, Kv8Attention a, int beside, float* part, RowStats* part_stats, unsigned* arrived) {
     using F = Few<DP, TERMS, NT>;
@@ -454,17 +477,18 @@ __global__ void __launch_bounds__(Few<DP, TERMS, NT>::kThreads, Few<DP, TERMS, N
     __shared__ int last;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, group = a.heads / c.kv_heads;
+    const int peers = (int)cluster_size(), rank = (int)cluster_rank();               // CTAs that have a part each of the same tiles
     // a lane's pieces of 16 bytes: row lane / (DP / 16) and so on, where they go, and whether rows have them (zeros come in their place)
     const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring), swizzled = piece_at<DP>(lane / (DP / 16), lane % (DP / 16));
     const int lane_bytes = lane % (DP / 16) * 16 < c.stride ? 16 : 0, lane_off = lane / (DP / 16) * c.stride + (lane_bytes ? lane % (DP / 16) * 16 : 0);
     if (warp == 0) {
-        const Place found = find_place<kRows>(s, a, c.kv_heads, group, c.page_shift, F::kCtas, kWarps, blockIdx.x);
+        const Place found = find_place<kRows>(s, a, c.kv_heads, group, c.page_shift, (int)gridDim.x / peers, kWarps, (int)cluster_index());
         if (lane == 0) place = found;
     }
     zero_rows_of_none(s, a, c.dim, (long long)blockIdx.x * F::kThreads + threadIdx.x, (long long)gridDim.x * F::kThreads);
     __syncthreads();
     Place at = place;
-    long long unit = at.seq < 0 ? at.total : at.per * blockIdx.x;
+    long long unit = at.seq < 0 ? at.total : at.per * cluster_index();
     const long long unit_end = min(unit + at.per, at.total);
     Span sp = span_of<kRows>(s, a, max(at.seq, 0), group, c.page_shift, at.run);
 
@@ -475,11 +499,13 @@ __global__ void __launch_bounds__(Few<DP, TERMS, NT>::kThreads, Few<DP, TERMS, N
         }
         const long long item = (unit - at.base) / sp.share;
         const int u0 = (int)(unit - at.base - item * sp.share), taken = at.run ? 1 : (int)min((long long)sp.share - u0, unit_end - unit);
-        const int b0 = at.run ? (int)((long long)u0 * sp.blocks / sp.share) : u0, b1 = at.run ? (int)((long long)(u0 + 1) * sp.blocks / sp.share) : min(u0 + taken, sp.blocks), count = b1 - b0;
+        // (a cluster's CTAs take a tile that nobody shares together)
+        const long long parts = (long long)sp.share * peers, nth = (long long)u0 * peers + rank;
+        const int b0 = at.run ? (int)(nth * sp.blocks / parts) : u0, b1 = at.run ? (int)((nth + 1) * sp.blocks / parts) : min(u0 + taken, sp.blocks), count = b1 - b0;
         const int head = (int)(item / sp.tiles), tile = (int)(item - (long long)head * sp.tiles);
         const int p0 = tile * kRows, rows = min(kRows, sp.n * group - p0);
         unit += taken;
-        if (count <= 0) continue;                                                    // (what a tile costs besides)
+        if (count <= 0 && !at.run) continue;                                                    // (what a tile costs besides)
         // positions of the tile's rows, first and last
         const auto position = [&](int r) { return (long long)sp.past + (p0 + min(r, rows - 1)) / group; };
         const long long back = a.window > 0 ? a.window - 1 : (1ll << 40);
@@ -721,7 +747,7 @@ __global__ void __launch_bounds__(Few<DP, TERMS, NT>::kThreads, Few<DP, TERMS, N
                             make_float4(o[n][h * 8 + j / 2][e], o[n][h * 8 + j / 2][e + 2], o[n][h * 8 + j / 2 + 1][e], o[n][h * 8 + j / 2 + 1][e + 2]);
             }
         __syncthreads();
-        const bool whole = b0 == 0 && count == sp.blocks;
+        const bool whole = peers == 1 && count == sp.blocks;
         const auto write = [&](int r, int d, float f, const float4& sum) {
             const int p = p0 + r, h = head * group + p % group;
             const size_t to = ((size_t)(sp.begin + p / group) * a.heads + h) * c.dim + d;
@@ -749,6 +775,7 @@ __global__ void __launch_bounds__(Few<DP, TERMS, NT>::kThreads, Few<DP, TERMS, N
             return sum;
         };
         const int tasks = rows * (DP / 4);
+        RowStats* const met = reinterpret_cast<RowStats*>(sums + kWarps * kRows * DP);
         const size_t slot = 2 * (size_t)blockIdx.x + (b0 == 0);
         for (int i = threadIdx.x; i < tasks; i += F::kThreads) {
             const int r = i / (DP / 4), d = i % (DP / 4) * 4;
@@ -756,12 +783,42 @@ __global__ void __launch_bounds__(Few<DP, TERMS, NT>::kThreads, Few<DP, TERMS, N
             const float4 sum = meet(kWarps, stats, sums, kRows, r, d, top);
             if (whole) {
                 write(r, d, row_factor(a, head * group + (p0 + r) % group, top.m, top.w, top.l), sum);
+            } else if (peers > 1) {
+                *reinterpret_cast<float4*>(sums + r * DP + d) = sum;                 // (where this thread has read)
+                if (d == 0) met[r] = top;
             } else {
                 *reinterpret_cast<float4*>(part + (slot * kRows + r) * DP + d) = sum;
                 if (d == 0) part_stats[slot * kRows + r] = top;
             }
         }
-        if (!whole) {
+        if (peers > 1) {
+            // every CTA joins some channels of all
+            cluster_met();
+            for (int i = threadIdx.x * peers + rank; i < tasks; i += F::kThreads * peers) {
+                const int r = i / (DP / 4), d = i % (DP / 4) * 4;
+                RowStats y[kMostPeers], top{-INFINITY, -INFINITY, 0.f};
+                float4 z[kMostPeers], sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int v = 0; v < kMostPeers; ++v) {
+                    y[v] = {-INFINITY, -INFINITY, 0.f};
+                    z[v] = sum;
+                    if (v >= peers) continue;
+                    const uint32_t of = shared_of(met + r, v);
+                    y[v] = {load_of(of), load_of(of + 4), load_of(of + 8)};
+                    z[v] = load4_of(shared_of(sums + r * DP + d, v));
+                    top.m = fmaxf(top.m, y[v].m);
+                    top.w = fmaxf(top.w, y[v].w);
+                }
+#pragma unroll
+                for (int v = 0; v < kMostPeers; ++v) {
+                    const float f = lower_to(y[v].w, top.w);
+                    top.l += y[v].l * lower_to(y[v].m, top.m);
+                    sum = make_float4(sum.x + f * z[v].x, sum.y + f * z[v].y, sum.z + f * z[v].z, sum.w + f * z[v].w);
+                }
+                write(r, d, row_factor(a, head * group + (p0 + r) % group, top.m, top.w, top.l), sum);
+            }
+            cluster_met();                                                           // (nobody reads here any more)
+        } else if (!whole) {
             // Runs c0 to c1 share the tile; the last of them to come joins all, in their order.  (A run is the first one of at most one shared tile, whose counter it lends.)
             // Where they are many, the last of every kJoin in turn joins those, in the first one's place, and the last of these their sums.  (Their counter is lent by the last run
             // of the kJoin, which is no other tile's but as its first.)
@@ -882,6 +939,8 @@ struct FewWork {
 };
 inline int padded_dim(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 inline int terms_of(int type) { return type == kTypeF32 ? 2 : 1; }
+// tiles of eight rows where sequences have no more of them on average (the products of 16 rows take twice the registers and the tensor cores' time)
+inline bool eight_rows(int kv_heads, int rows, int heads, int sequences) { return (long long)rows * (heads / kv_heads) <= 8ll * sequences; }
 
 template <int DP, int FORMAT, int TERMS, int NT>
 cudaError_t run_few(const Kv8Cache& c, const Kv8Step& s, const Kv8Attention& a, bool early, bool beside, const FewWork& work, cudaStream_t st) {
@@ -890,13 +949,27 @@ cudaError_t run_few(const Kv8Cache& c, const Kv8Step& s, const Kv8Attention& a, 
     cudaError_t e = cudaGetDevice(&dev);
     if (e == cudaSuccess) e = dia::ask_smem<kv8_attention_few_kernel<DP, FORMAT, TERMS, NT>>(dev, F::kSmem);
     if (e != cudaSuccess) return e;
-    return launch_pdl_if(early, kv8_attention_few_kernel<DP, FORMAT, TERMS, NT>, dim3(F::kCtas), dim3(F::kThreads), F::kSmem, st, c, s, a, beside, work.part, work.stats, work.arrived);
+    const auto kernel = kv8_attention_few_kernel<DP, FORMAT, TERMS, NT>;
+    if (a.whole > 1) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)(F::kCtas / a.whole * a.whole));
+        cfg.blockDim = dim3(F::kThreads);
+        cfg.dynamicSmemBytes = F::kSmem;
+        cfg.stream = st;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = (unsigned)a.whole;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        return cudaLaunchKernelEx(&cfg, kernel, c, s, a, (int)beside, work.part, work.stats, work.arrived);
+    }
+    return launch_pdl_if(early, kernel, dim3(F::kCtas), dim3(F::kThreads), F::kSmem, st, c, s, a, beside, work.part, work.stats, work.arrived);
 }
 template <int DP, int FORMAT>
 cudaError_t run_few(const Kv8Cache& c, const Kv8Step& s, const Kv8Attention& a, bool beside, const FewWork& work, cudaStream_t st) {
     const bool early = !a.whole;                              // (behind the counters' kernel, or the tiles')
-    // tiles of eight rows where sequences have no more of them on average (the products of 16 rows take twice the registers and the tensor cores' time)
-    const bool eight = (long long)s.rows * (a.heads / c.kv_heads) <= 8ll * s.sequences;
+    const bool eight = eight_rows(c.kv_heads, s.rows, a.heads, s.sequences);
     if (terms_of(a.type) == 2) return eight ? run_few<DP, FORMAT, 2, 1>(c, s, a, early, beside, work, st) : run_few<DP, FORMAT, 2, 2>(c, s, a, early, beside, work, st);
     return eight ? run_few<DP, FORMAT, 1, 1>(c, s, a, early, beside, work, st) : run_few<DP, FORMAT, 1, 2>(c, s, a, early, beside, work, st);
 }
@@ -932,10 +1005,21 @@ cudaError_t launch_kv8_read(const Kv8Cache& c, const Kv8Step& s, void* k, void* 
 namespace {
 // Pairs of a sequence from which on tiles of 256 rows are the shorter way
 constexpr int kFewMost = 64;
-// Tables of up to so many tokens: no tile is shared by several CTAs
-constexpr int kWholeTokens = 2048;
+// Tables of up to so many tokens for each of a cluster's CTAs: no tile is shared by others, which would need counters (a launch more) and sums by way of memory.  One request of 1025
+// tokens: 14.3 us by one CTA a tile, 13.2 shared, 9.7 by eight; of 4000: 11.7 and 14.0 shared; of 16000: 21.6 and 20.0; nine of 8000: 29.2 by four and 24.0.
+constexpr int kWholeTokens = 1024;
+// and at least so many (of 128 tokens: 8.1 us alone, 9.0 by eight)
+constexpr int kPeerTokens = 128;
 inline bool some_in_tiles(int kv_heads, int dim, int rows, int heads, int type) { return kv8_tiles_ok(dim, type) && (long long)rows * (heads / kv_heads) > kFewMost; }
-inline bool whole_tiles(int kv_heads, int dim, int rows, int heads, int type, long long tokens) { return tokens <= kWholeTokens && !some_in_tiles(kv_heads, dim, rows, heads, type); }
+// CTAs of a cluster that takes tiles by itself: as many as there are for each tile; 0: tables are too long for that
+inline int whole_tiles(int kv_heads, int dim, int rows, int heads, int type, int sequences, long long tokens) {
+    if (some_in_tiles(kv_heads, dim, rows, heads, type)) return 0;
+    const int each = eight_rows(kv_heads, rows, heads, sequences) ? 8 : 16, ctas = terms_of(type) == 2 || dim > 128 ? 148 : 296;      // (as Few has them)
+    const long long tiles = kv_heads * (((long long)rows * (heads / kv_heads) + (long long)std::min(sequences, rows) * (each - 1)) / each);
+    int peers = kMostPeers;
+    while (peers > 1 && (tiles * peers > ctas || tokens <= peers / 2 * kPeerTokens)) peers /= 2;
+    return tokens <= (long long)peers * kWholeTokens ? peers : 0;
+}
 }  // namespace
 
 // Counters first: those of both kernels are set to zero in one go.
@@ -945,8 +1029,8 @@ inline size_t few_bytes(int dp) { return (size_t)2 * kMostCtas * 16 * (dp * size
 inline size_t rounded(size_t bytes) { return (bytes + 255) / 256 * 256; }
 }  // namespace
 
-size_t kv8_attention_work_bytes(int kv_heads, int dim, int rows, int heads, int type, long long tokens) {
-    if (whole_tiles(kv_heads, dim, rows, heads, type, tokens)) return 0;
+size_t kv8_attention_work_bytes(int kv_heads, int dim, int rows, int heads, int type, int sequences, long long tokens) {
+    if (whole_tiles(kv_heads, dim, rows, heads, type, sequences, tokens)) return 0;
     return rounded(kCounters) + rounded(few_bytes(padded_dim(dim))) + (some_in_tiles(kv_heads, dim, rows, heads, type) ? kv8_tiles_work_bytes(dim) : 0);
 }
 
@@ -955,7 +1039,7 @@ cudaError_t launch_kv8_attention(const Kv8Cache& c, const Kv8Step& s, Kv8Attenti
     const bool tiles = some_in_tiles(c.kv_heads, c.dim, s.rows, a.heads, a.type), alone = tiles && s.sequences == 1;        // (alone: in tiles whatever its rows are)
     unsigned* const counters = reinterpret_cast<unsigned*>(work);
     float* const part = reinterpret_cast<float*>(reinterpret_cast<char*>(work) + rounded(kCounters));
-    a.whole = whole_tiles(c.kv_heads, c.dim, s.rows, a.heads, a.type, (long long)s.max_pages << c.page_shift);
+    a.whole = whole_tiles(c.kv_heads, c.dim, s.rows, a.heads, a.type, s.sequences, (long long)s.max_pages << c.page_shift);
     cudaError_t e = cudaSuccess;
     if (!a.whole) {
         kv8_counters_kernel<<<1, kCounterThreads, 0, st>>>(counters, (int)(kCounters / sizeof(unsigned)));

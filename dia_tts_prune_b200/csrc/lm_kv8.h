@@ -72,10 +72,10 @@ struct Kv8Attention {
     int window;                                           // a row sees itself and window - 1 tokens in front; 0: all
     const float* sinks;                                   // [heads] one more logit in the denominator; NULL: none
     int few_most;                                         // (token, query head) pairs per key head of a sequence that tiles of 16 of them take; others go 256 at a time
-    int whole;                                            // != 0: a CTA takes whole tiles of 16
+    int whole;                                            // CTAs of a cluster that takes whole tiles; 0: tiles are shared
 };
 // (tokens: what a row of the table has room for; 0 bytes: none are needed)
-size_t kv8_attention_work_bytes(int kv_heads, int dim, int rows, int heads, int type, long long tokens);
+size_t kv8_attention_work_bytes(int kv_heads, int dim, int rows, int heads, int type, int sequences, long long tokens);
 cudaError_t launch_kv8_attention(const Kv8Cache& c, const Kv8Step& s, Kv8Attention a, void* work, cudaStream_t st);      // (sets few_most and whole)
 
 // lm_kv8_tiles.cu: the sequences of more than few_most pairs; bf16 or fp16 rows, dim up to 128.  alone: nothing else zeroes the rows of no sequence

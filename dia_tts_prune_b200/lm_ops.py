@@ -449,8 +449,8 @@ def _kv8_step(cache: Kv8, table: torch.Tensor, past: torch.Tensor, first: torch.
 
 
 @lru_cache(maxsize=1024)
-def _kv8_work_bytes(kv_heads: int, dim: int, rows: int, heads: int, kind: int, tokens: int) -> int:
-    return _lm_lib.load().lm_b200_op_kv8_attention_work_bytes(kv_heads, dim, rows, heads, kind, tokens)
+def _kv8_work_bytes(kv_heads: int, dim: int, rows: int, heads: int, kind: int, n: int, tokens: int) -> int:
+    return _lm_lib.load().lm_b200_op_kv8_attention_work_bytes(kv_heads, dim, rows, heads, kind, n, tokens)
 
 
 def attention_kv8(q: torch.Tensor, cache: Kv8, table: torch.Tensor, past: torch.Tensor, first: torch.Tensor | None = None, *, scale: float | None = None,
@@ -497,7 +497,8 @@ def attention_kv8(q: torch.Tensor, cache: Kv8, table: torch.Tensor, past: torch.
         q = q.contiguous()
         q_row, q_head, _ = q.stride()
     kind = _TYPES[q.dtype]
-    need = _kv8_work_bytes(cache.kv_heads, cache.dim, rows, heads, kind, table.size(1) * cache.page_size)
+    n, width = table.shape
+    need = _kv8_work_bytes(cache.kv_heads, cache.dim, rows, heads, kind, n, width * cache.page_size)
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
     work = q.new_empty(need, dtype=torch.uint8) if need else None
     _call("kv8_attention", cache.keys.device, cache._at, step, q.data_ptr(), q_row, q_head, heads, kind, scale, window, None if sinks is None else sinks.data_ptr(),

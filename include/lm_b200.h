@@ -368,7 +368,7 @@ int lm_b200_op_kv8_read(const lm_b200_kv8 *cache, const lm_b200_kv8_step *step, 
  * before it, the last `window` of them (0: all): weights exp(scale q.k), in the denominator exp(sinks[head]) too (NULL: nothing).  Query head h reads key head h / (heads / kv_heads).  A row
  * that sees nothing, and a row of no sequence, is zeros.  work: lm_b200_op_kv8_attention_work_bytes bytes, 256-byte aligned (0:
  * none; tokens: max_pages x page_size). */
-size_t lm_b200_op_kv8_attention_work_bytes(int kv_heads, int dim, int rows, int heads, int type, int64_t tokens);
+size_t lm_b200_op_kv8_attention_work_bytes(int kv_heads, int dim, int rows, int heads, int type, int n_seq, int64_t tokens);
 int lm_b200_op_kv8_attention(const lm_b200_kv8 *cache, const lm_b200_kv8_step *step, const void *q, int64_t q_row, int64_t q_head, int heads, int type, float scale, int window,
                              const float *sinks, void *out, void *work, size_t work_bytes, void *stream);
 

@@ -148,11 +148,12 @@ def test_c_entries_answer_bad_arguments():
     lib = _lm_lib.load()
     at, odd = 1 << 20, (1 << 20) + 8                               # (addresses that are never followed)
     cache = dict(zip([n for n, _ in _lm_lib.Kv8._fields_], (at, at, at, at, 4, 2, 16, 64, _lm_lib.KV8_E4M3)))
-    step = (at, 300, at, at, 300, 2, 5)
-    need = lib.lm_b200_op_kv8_attention_work_bytes(2, 64, 5, 4, _lm_lib.TYPE_BF16, 4800)
-    assert need > 0 and lib.lm_b200_op_kv8_attention_work_bytes(2, 64, 5, 4, _lm_lib.TYPE_BF16, 48) == 0 and lib.lm_b200_op_kv8_attention_work_bytes(2, 64, 500, 4, _lm_lib.TYPE_BF16, 48) > need
-    for a in ((0, 64, 5, 4, 1), (2, 0, 5, 4, 1), (2, 257, 5, 4, 1), (2, 64, 0, 4, 1), (2, 64, 5, 0, 1), (2, 64, 5, 5, 1), (2, 64, 1 << 30, 4, 1), (1, 64, 5, 4097, 1), (2, 64, 5, 4, 7)):
-        assert lib.lm_b200_op_kv8_attention_work_bytes(*a, 4800) == 0
+    step = (at, 3000, at, at, 3000, 2, 5)
+    need = lib.lm_b200_op_kv8_attention_work_bytes(2, 64, 5, 4, _lm_lib.TYPE_BF16, 2, 48000)
+    assert need > 0 and lib.lm_b200_op_kv8_attention_work_bytes(2, 64, 5, 4, _lm_lib.TYPE_BF16, 2, 48) == 0 and lib.lm_b200_op_kv8_attention_work_bytes(2, 64, 500, 4, _lm_lib.TYPE_BF16, 2, 48) > need
+    for a in ((0, 64, 5, 4, 1, 2), (2, 0, 5, 4, 1, 2), (2, 257, 5, 4, 1, 2), (2, 64, 0, 4, 1, 2), (2, 64, 5, 0, 1, 2), (2, 64, 5, 5, 1, 2), (2, 64, 1 << 30, 4, 1, 2), (1, 64, 5, 4097, 1, 2),
+              (2, 64, 5, 4, 7, 2), (2, 64, 5, 4, 1, 0)):
+        assert lib.lm_b200_op_kv8_attention_work_bytes(*a, 48000) == 0
 
     def entries(cache, step, rows=(at, 128, 64), heads=4, kind=1, scale=1.0, window=0, out=at, work=at, bytes=need):
         k = _lm_lib.Kv8(*cache.values()) if cache else None
