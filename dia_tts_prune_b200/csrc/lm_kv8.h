@@ -81,7 +81,7 @@ cudaError_t launch_kv8_attention(const Kv8Cache& c, const Kv8Step& s, Kv8Attenti
 // lm_kv8_tiles.cu: the sequences of more than few_most pairs; bf16 or fp16 rows, dim up to 128.  alone: nothing else zeroes the rows of no sequence
 bool kv8_tiles_ok(int dim, int type);
 size_t kv8_tiles_work_bytes(int dim);
-constexpr int kKvTileCounters = 148;                      // zeros, one for every item whose keys go in chunks
+constexpr int kKvTileCounters = 2 * 148;                  // zeros, two for every chunk of keys that an item may go in
 cudaError_t launch_kv8_tiles(const Kv8Cache& c, const Kv8Step& s, const Kv8Attention& a, bool alone, void* work, unsigned* arrived, cudaStream_t st);
 
 }  // namespace lm

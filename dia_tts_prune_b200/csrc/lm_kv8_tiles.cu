@@ -41,6 +41,7 @@ constexpr int kSpread = 80;
 constexpr int kLaunchRegs = 96, kSoftmaxRegs = 144, kFetchRegs = 48, kIssueRegs = 88;
 static_assert(128 * (2 * kSoftmaxRegs + 2 * kFetchRegs + kIssueRegs) <= kThreads * kLaunchRegs, "the split is within the launch's registers");
 static_assert(kSoftmaxRegs >= kLaunchRegs && kFetchRegs <= kLaunchRegs && kIssueRegs <= kLaunchRegs, "who gives registers and who takes them");
+constexpr int kJoinOnce = 8;                                     // chunks that are joined in one go
 constexpr int kAhead = 4;                                      // tiles whose pages and scales are known
 
 template <int DP>
@@ -179,6 +180,10 @@ __device__ __forceinline__ void mma_weights(uint32_t d, uint32_t a, uint64_t b, 
         "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
         : "memory");
 }
+
+struct Beside {                                               // rows between neighbouring chunks, known when it is compiled
+    __device__ __forceinline__ operator int() const { return kTileRows; }
+};
 
 template <int DP, int FORMAT>
 __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cache c, Kv8Step s, Kv8Attention a, int alone, float* part, RowStats* part_stats, unsigned* arrived, int* ran_out, unsigned polls) {
@@ -655,44 +660,78 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cac
     fence_before();
     __syncthreads();
     if (work.chunks > 1) {
-        // the last chunk of an item to come joins all, in their order
-        if (threadIdx.x == 0) largest = atomicAdd(arrived + work.first_cta, 1u) == (unsigned)(work.chunks - 1);
-        __syncthreads();
-        if (largest) {
-            __threadfence();
-            // rows' weights of the chunks first, where the rings lay, then their channels
-            float* const weights = reinterpret_cast<float*>(smem);                   // [chunk][row], and behind them what a row's sum is times
-            const int rows = min(kTileRows, pairs - p0);
-            const RowStats* const stats = part_stats + (size_t)work.first_cta * kTileRows;
+        // The last chunk of an item to come joins all, in their order; where they are many, the last of every `each` in turn joins those, in the first one's place, and the last of
+        // these their sums (one CTA reads 128 KB a chunk: 32 rows behind 16384 tokens, 37 chunks, 58 us in one go and 45 in two)
+        const int rows = min(kTileRows, pairs - p0);
+        float* const weights = reinterpret_cast<float*>(smem);                       // [chunk][row], and behind them what a row's sum is times: where the rings lay
+        const auto arrive = [&](int at, int n) {              // true for the last of n
+            if (threadIdx.x == 0) largest = atomicAdd(arrived + work.first_cta + at, 1u) == (unsigned)(n - 1);
+            __syncthreads();
+            if (largest) __threadfence();
+            return largest != 0;
+        };
+        // rows' weights of n chunks that lie `next` rows apart
+        const auto weigh = [&](const RowStats* stats, int n, auto next, auto&& told) {
             for (int r = threadIdx.x; r < rows; r += kThreads) {
                 float m = -INFINITY, w = -INFINITY, l = 0.f;
-                for (int i = 0; i < work.chunks; ++i) {
-                    m = fmaxf(m, __ldcg(&stats[i * kTileRows + r].m));
-                    w = fmaxf(w, __ldcg(&stats[i * kTileRows + r].w));
+                for (int i = 0; i < n; ++i) {
+                    m = fmaxf(m, __ldcg(&stats[i * next + r].m));
+                    w = fmaxf(w, __ldcg(&stats[i * next + r].w));
                 }
-                for (int i = 0; i < work.chunks; ++i) {
-                    l += __ldcg(&stats[i * kTileRows + r].l) * lower_to(__ldcg(&stats[i * kTileRows + r].m), m);
-                    weights[i * kTileRows + r] = lower_to(__ldcg(&stats[i * kTileRows + r].w), w);
+                for (int i = 0; i < n; ++i) {
+                    l += __ldcg(&stats[i * next + r].l) * lower_to(__ldcg(&stats[i * next + r].m), m);
+                    weights[i * kTileRows + r] = lower_to(__ldcg(&stats[i * next + r].w), w);
                 }
-                weights[work.chunks * kTileRows + r] = row_factor(a, work.head * group + (p0 + r) % group, m, w, l);
+                told(r, RowStats{m, w, l});
             }
             __syncthreads();
-            const float* const from_part = part + (size_t)work.first_cta * kTileRows * DP;
+        };
+        const auto sum_of = [&](const float* from, int n, auto next, int r, int d) {
+            float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int k = 0; k < n; ++k) {
+                const float f = weights[k * kTileRows + r];
+                const float4 z = __ldcg(reinterpret_cast<const float4*>(from + ((size_t)k * next + r) * DP + d));
+                sum = make_float4(sum.x + f * z.x, sum.y + f * z.y, sum.z + f * z.z, sum.w + f * z.w);
+            }
+            return sum;
+        };
+        const Beside one;
+        int each = 1;
+        bool here = true;
+        if (work.chunks > kJoinOnce) {
+            while (each * each < work.chunks) ++each;
+            const int from = work.chunk / each * each, n = min(each, work.chunks - from);
+            here = arrive(kSms + from + n - 1, n);
+            if (here) {
+                RowStats* const stats = part_stats + (size_t)(work.first_cta + from) * kTileRows;
+                float* const sums = part + (size_t)(work.first_cta + from) * kTileRows * DP;
+                weigh(stats, n, one, [&](int r, const RowStats& top) { stats[r] = top; });
+#pragma unroll 4
+                for (int i = threadIdx.x; i < rows * (DP / 4); i += kThreads)        // (in the place that only this thread reads)
+                    *reinterpret_cast<float4*>(sums + 4 * (size_t)i) = sum_of(sums, n, one, i / (DP / 4), i % (DP / 4) * 4);
+                __threadfence();
+                __syncthreads();
+            }
+        }
+        const auto finish = [&](int n, auto next) {
+            weigh(part_stats + (size_t)work.first_cta * kTileRows, n, next, [&](int r, const RowStats& top) {
+                weights[n * kTileRows + r] = row_factor(a, work.head * group + (p0 + r) % group, top.m, top.w, top.l);
+            });
 #pragma unroll 4
             for (int i = threadIdx.x; i < rows * (DP / 4); i += kThreads) {
                 const int r = i / (DP / 4), d = i % (DP / 4) * 4, p = p0 + r;
-                float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-                for (int k = 0; k < work.chunks; ++k) {
-                    const float f = weights[k * kTileRows + r];
-                    const float4 z = __ldcg(reinterpret_cast<const float4*>(from_part + ((size_t)k * kTileRows + r) * DP + d));
-                    sum = make_float4(sum.x + f * z.x, sum.y + f * z.y, sum.z + f * z.z, sum.w + f * z.w);
-                }
-                const float f = weights[work.chunks * kTileRows + r], y[4] = {sum.x, sum.y, sum.z, sum.w};
+                const float4 sum = sum_of(part + (size_t)work.first_cta * kTileRows * DP, n, next, r, d);
+                const float f = weights[n * kTileRows + r], y[4] = {sum.x, sum.y, sum.z, sum.w};
                 const size_t to = ((size_t)(q.begin + p / group) * a.heads + work.head * group + p % group) * c.dim + d;
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
                     if (d + e < c.dim) store_out(a, to + e, f * y[e]);
             }
+        };
+        const int left = (work.chunks + each - 1) / each;
+        if (here && arrive(0, left)) {
+            if (each == 1) finish(left, one);
+            else finish(left, each * kTileRows);
         }
     }
     if (warp == 16) {
