@@ -218,7 +218,7 @@ __global__ void __launch_bounds__(kAppendThreads, 4) kv8_append_kernel(Kv8Cache 
 }
 
 // ---- numbers out of pages ------------------------------------------------------------------------------------------------------------------
-// A CTA takes kReadRows rows (fewer where there are few): where each of them lies is looked up once.  A thread has 16 bytes of what goes out, the same head and channels of row
+// A CTA takes kReadMostRows rows (8 where there are few): where each of them lies is looked up once.  A thread has 16 bytes of what goes out, the same head and channels of row
 // after row, four rows on their way at a time.
 constexpr int kReadThreads = 256, kReadMostRows = 32, kReadAhead = 4;
 template <int FORMAT, int TYPE, bool WIDE>
@@ -307,7 +307,9 @@ __global__ void __launch_bounds__(kReadThreads) kv8_read_kernel(Kv8Cache c, Kv8S
 // What bounds it is the cache's bytes.  The rows of a tile (8, or 16) are (token, query head) pairs that share a key head, so a token's codes are read once for the group; tiles of
 // a sequence lie next to one another in the order of the work.  Work is counted in blocks of 16 tokens over all sequences, heads and tiles and dealt to the CTAs in
 // equal runs, so that one long sequence fills the GPU and lengths need not be alike; runs that share a tile leave (max, sum, output), and the last one to come joins them, always in
-// the same order (a second kernel for that took 6 us after one request's 1024 tokens, 11 after 131072, 26 after 64 requests).
+// the same order (a second kernel for that took 6 us after one request's 1024 tokens, 11 after 131072, 26 after 64 requests).  Few short tiles go to a cluster each.
+// Measured: 64 requests of up to 24576 tokens 223 us (5.9 TB/s of the 6.5 that a copy reaches); one behind 131071 28 us, of which the cache's bytes are 10, the first loads 4 and the two
+// joins 9; one of 1025 9.7 us: a launch and a chain of looks at the sequence, its page, its scale, its codes.
 //
 // A warp keeps its own ring of blocks in shared memory, filled by asynchronous copies that swizzle 16-byte pieces (rows lie 128 bytes apart, which would be the same banks), and
 // multiplies on the tensor cores (mma.sync, 16 x 8 x 16: a block's 16 tokens, or 16 channels of their values, by eight rows: what a group has, and nothing is waited for across warps).
@@ -939,7 +941,8 @@ struct FewWork {
 };
 inline int padded_dim(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 inline int terms_of(int type) { return type == kTypeF32 ? 2 : 1; }
-// tiles of eight rows where sequences have no more of them on average (the products of 16 rows take twice the registers and the tensor cores' time)
+// tiles of eight rows where sequences have no more of them on average (the products of 16 rows take twice the registers and the tensor cores' time: 64 requests 226 and 305 us, eight of
+// fp32 19 and 24; two tiles of eight would read the cache twice)
 inline bool eight_rows(int kv_heads, int rows, int heads, int sequences) { return (long long)rows * (heads / kv_heads) <= 8ll * sequences; }
 
 template <int DP, int FORMAT, int TERMS, int NT>
@@ -977,7 +980,8 @@ cudaError_t run_few(const Kv8Cache& c, const Kv8Step& s, const Kv8Attention& a, 
 }  // namespace
 
 cudaError_t launch_kv8_append(const Kv8Cache& c, const Kv8Step& s, Kv8Rows k, Kv8Rows v, int type, cudaStream_t st) {
-    // a warp per row where sequences have few of them (a decoding step's pages side by side), per page's worth where they have many
+    // a warp per row where sequences have few of them (a decoding step's pages side by side: 4 us, by the page 12), per page's worth where they have many (8192 rows of prompts: 15 us, row
+    // by row 74)
     const int chunk = s.rows > 4ll * s.sequences ? 1 << c.page_shift : 1;
     const long long tasks = ((long long)s.rows + chunk - 1) / chunk * 2 * c.kv_heads, blocks = (tasks * 32 + kAppendThreads - 1) / kAppendThreads;
     if (blocks > 0x7fffffff) return cudaErrorInvalidValue;
@@ -991,6 +995,7 @@ cudaError_t launch_kv8_append(const Kv8Cache& c, const Kv8Step& s, Kv8Rows k, Kv
 }
 
 cudaError_t launch_kv8_read(const Kv8Cache& c, const Kv8Step& s, void* k, void* v, int type, cudaStream_t st) {
+    // (98304 tokens: 56 us with 32 rows a CTA, 69 with 8; 992 tokens: 7.5 with 32, 4.4 with 8)
     const int each = s.rows >= 148 * 4 * kReadMostRows ? kReadMostRows : 8;
     const unsigned blocks = (unsigned)(((long long)s.rows + each - 1) / each);
     const bool w = c.dim % (16 / type_bytes(type)) == 0 && ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) == 0;
@@ -1003,7 +1008,8 @@ cudaError_t launch_kv8_read(const Kv8Cache& c, const Kv8Step& s, void* k, void* 
 }
 
 namespace {
-// Pairs of a sequence from which on tiles of 256 rows are the shorter way
+// Pairs of a sequence up to which tiles of 16 of them are the shorter way (four heads a key head; these and those of 256 rows: 36 pairs behind 1000 tokens 14 and 22 us, behind 16000
+// 36 and 31; 68 pairs 17 and 25, 40 and 37, of eight sequences behind 8000 tokens 97 and 53)
 constexpr int kFewMost = 64;
 // Tables of up to so many tokens for each of a cluster's CTAs: no tile is shared by others, which would need counters (a launch more) and sums by way of memory.  One request of 1025
 // tokens: 14.3 us by one CTA a tile, 13.2 shared, 9.7 by eight; of 4000: 11.7 and 14.0 shared; of 16000: 21.6 and 20.0; nine of 8000: 29.2 by four and 24.0.
