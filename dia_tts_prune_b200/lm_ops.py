@@ -1,5 +1,5 @@
-"""Operators of the language models for callers that hold rows of their own: matrices in 4 bits and their products, and the cross
-entropy of rows under a head with its gradient.
+"""Operators of the language models for callers that hold rows of their own: matrices in 4 bits and their products, the cross
+entropy of rows under a head with its gradient, and a cache of keys and values in 8 bits with its attention.
 
 They stand beside ``lm_engine.linear``: torch tensors on a CUDA device in, new tensors out, queued on the current stream of the tensors'
 device.  Workspaces come from torch's allocator for the length of a call, so calls on several streams and in captured graphs do not share
