@@ -326,7 +326,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cac
                 most = max(most, __shfl_xor_sync(0xffffffffu, most, 16));
                 const uint32_t e = most == 0 ? 127u : max(most >> 23, 14u);
                 const float f = __uint_as_float((267u - e) << 23), way_back = __uint_as_float((e - 13u) << 23);       // 2^(140 - e): to below 2^14, and the way back
-                if (r8 == lane >> 3) row_scale = e == 255u ? __uint_as_float(0x7fc00000u) : way_back * (a.scale * kLog2e);      // (a thread's own row is 8 r8 + sub of its warp's)
+                // (a thread's own row is 8 r8 + sub of its warp's.  Below zero: its query is not finite, and its operand is zeros, so that what it does not see stays hidden)
+                if (r8 == lane >> 3) row_scale = e == 255u ? -1.f : way_back * (a.scale * kLog2e);
                 uint8_t* const to = q_tile + (warp >> 2) * (kHalfRows * DP * 2) + ((warp & 3) * 4 + r8) * (DP * 16) + sub * 16;
 #pragma unroll
                 for (int j = 0; j < kPieces; ++j) {
@@ -392,7 +393,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cac
                 float m = max3(score(b, 0), score(b, 1), score(b, 2));
 #pragma unroll
                 for (int e = 3; e < kKvBlock - 1; e += 2) m = max3(m, score(b, e), score(b, e + 1));
-                top = fmaxf(top, fmaf(fmaxf(m, score(b, 15)), meta.x * row_scale, meta.y));
+                top = fmaxf(top, fmaf(fmaxf(m, score(b, 15)), meta.x * fabsf(row_scale), meta.y));
             }
             if (__any_sync(0xffffffffu, top > ref + kSlack)) {
                 const float next = top > ref + kSlack ? top : ref, f = exp2_fast(ref - next);
@@ -416,7 +417,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cac
 #pragma unroll
             for (int b = 0; b < 4; ++b) {
                 const float4 meta = meta_of[b];
-                const f2 k2 = twice(meta.x * row_scale), c2 = twice(meta.y - ref + kBits);
+                const f2 k2 = twice(meta.x * fabsf(row_scale)), c2 = twice(meta.y - ref + kBits);
                 f2 sum[2] = {0, 0};
 #pragma unroll
                 for (int e = 0; e < kKvBlock; e += 2) {
@@ -447,6 +448,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cac
         }
         if (ok && count > 0 && !pair_wait(&pv_done[g][(count - 1) & 1], (uint32_t)((count - 1) >> 1) & 1u, polls)) ok = false;
         fence_after();
+        if (row_scale < 0.f && l != 0.f) l = __uint_as_float(0x7fc00000u);               // (it saw something)
         // out
         const float spread = (float)(largest == -1000 ? 0 : largest);
         float m = ref - kBits, w = m + spread + kWeightBits;

@@ -1,0 +1,44 @@
+"""What no row sees changes nothing, whatever it is: beside queries of any size, behind a sequence's last token, in front of its window.
+
+Bounds are those of the attention over the cache in 8 bits (test_kv8_gpu.py); everything else here is equal or not."""
+
+import math
+
+import pytest
+import torch
+
+from dia_tts_prune_b200 import lm_ops
+from test_kv8_gpu import DEV, check_attention, cumulative, ints
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("rows,past", [(100, 0), (12, 40)])        # (in tiles of 256 pairs, of 16)
+def test_queries_that_are_not_finite_and_see_nothing(rows, past, dtype):
+    """A row that sees nothing is zeros whatever its query; one that sees something is NaN."""
+    g = torch.Generator().manual_seed(rows)
+    cache = lm_ops.Kv8(12, 2, 64)
+    x = torch.randn(past + rows, 4, 64, generator=g).to(DEV)
+    lists = [[7, 3, -1, 12, -5, 1, 0]]                             # tokens 32 to 79 are on no page of the pool
+    table = ints(lists)
+    cache.append(x[:, :2], x[:, 2:], table, ints([0]), ints([0, past + rows]))
+    q = torch.randn(rows, 8, 64, generator=g).to(dtype).to(DEV)
+    for sinks in (None, torch.randn(8, generator=g).to(DEV)):
+        clean = lm_ops.attention_kv8(q, cache, table, ints([past]), ints([0, rows]), window=16, sinks=sinks)
+        check_attention(clean, q, cache, table, [past], [rows], window=16, sinks=sinks, lists=lists)
+        pos = past + torch.arange(rows, device=DEV)
+        blind = (pos >= 47) & (pos <= 79)
+        assert blind.any() and not blind.all() and not clean[blind].any()
+        for bad in (math.nan, math.inf, -math.inf):
+            for r in (int(blind.nonzero()[0]), int(blind.nonzero()[-1]), int((~blind).nonzero()[0]), int((~blind).nonzero()[-1])):
+                broken = q.clone()
+                broken[r, 1, 5], broken[r, 6, 63] = bad, bad
+                got = lm_ops.attention_kv8(broken, cache, table, ints([past]), ints([0, rows]), window=16, sinks=sinks)
+                want = clean.clone()
+                if not blind[r]:
+                    want[r, 1], want[r, 6] = math.nan, math.nan
+                assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(9.0), want.nan_to_num(9.0)), (bad, r)
+    none = torch.full_like(q, math.nan)                            # nothing of the sequence is there at all
+    for t, p in ((ints([[-1] * 7]), past), (table, -1)):
+        assert not lm_ops.attention_kv8(none, cache, t, ints([p]), ints([0, rows])).any()
