@@ -351,6 +351,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cac
         const long long tok0 = (long long)from * kKeys;
         const auto within = [&](long long v) { return (int)max(min(v - tok0, 0x7fffff00ll), -1ll); };
         const int hi = within(position(p)), lo = within(position(p) - back), all_hi = within(position(p0 + g * kHalfRows)), all_lo = within(position(p0 + g * kHalfRows + kHalfRows - 1) - back);
+        // What a score is times.  Hidden ones are -infinity, so it must not be zero: it is where a page of zeros' step is 2^-100, or a small query or scale comes to it.  (Scores are below
+        // 2^30, so what is raised to 2^-126 moves by 2^-96 at most.)
+        const auto factor = [&](float key_scale) { return fmaxf(key_scale * row_scale, 0x1p-126f); };
         float ref = -1e30f, l = 0.f;
         // (A step's scores come behind the value product of two steps before, not of the last one: what is told of every step has a barrier for the even ones and one for the odd.)
 #pragma unroll 1
@@ -393,7 +396,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cac
                 float m = max3(score(b, 0), score(b, 1), score(b, 2));
 #pragma unroll
                 for (int e = 3; e < kKvBlock - 1; e += 2) m = max3(m, score(b, e), score(b, e + 1));
-                top = fmaxf(top, fmaf(fmaxf(m, score(b, 15)), meta.x * fabsf(row_scale), meta.y));
+                top = fmaxf(top, fmaf(fmaxf(m, score(b, 15)), factor(meta.x), meta.y));
             }
             if (__any_sync(0xffffffffu, top > ref + kSlack)) {
                 const float next = top > ref + kSlack ? top : ref, f = exp2_fast(ref - next);
@@ -417,7 +420,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cac
 #pragma unroll
             for (int b = 0; b < 4; ++b) {
                 const float4 meta = meta_of[b];
-                const f2 k2 = twice(meta.x * fabsf(row_scale)), c2 = twice(meta.y - ref + kBits);
+                const f2 k2 = twice(factor(meta.x)), c2 = twice(meta.y - ref + kBits);
                 f2 sum[2] = {0, 0};
 #pragma unroll
                 for (int e = 0; e < kKvBlock; e += 2) {
@@ -646,7 +649,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cac
                 const int e = (int)(v >> 23) - 127 - (largest == -1000 ? 0 : largest), kept = number ? max(e, -kSpread) : 0;
                 if (i >= kAhead && !pair_wait(&m_empty[slot], (uint32_t)(i / kAhead + 1) & 1u, polls)) { ok = false; break; }
                 const uint32_t there = __ballot_sync(0xffffffffu, page_now >= 0), zeros = __ballot_sync(0xffffffffu, number && e < -kSpread), numbers = __ballot_sync(0xffffffffu, number || page_now < 0);
-                if (lane < kBlocks) blocks[slot][lane] = make_float4(number ? fmaxf(now.x, 0x1p-126f) : 1.f, page_now < 0 ? -INFINITY : (float)kept, __uint_as_float((uint32_t)(127 - kept) << 23), __int_as_float(page_now));
+                if (lane < kBlocks) blocks[slot][lane] = make_float4(number ? now.x : 1.f, page_now < 0 ? -INFINITY : (float)kept, __uint_as_float((uint32_t)(127 - kept) << 23), __int_as_float(page_now));
                 if (lane == 0) which[slot] = make_uint3(there & 0xffu, zeros & 0xffu, numbers & 0xffu);
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&m_full[slot]);

@@ -42,3 +42,41 @@ def test_queries_that_are_not_finite_and_see_nothing(rows, past, dtype):
     none = torch.full_like(q, math.nan)                            # nothing of the sequence is there at all
     for t, p in ((ints([[-1] * 7]), past), (table, -1)):
         assert not lm_ops.attention_kv8(none, cache, t, ints([p]), ints([0, rows])).any()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("fmt,dim,page,past,counts,window", [
+    ("e4m3", 128, 16, [0], [100], None),
+    ("int8", 64, 32, [300, 0], [90, 70], 40),
+    ("e4m3", 80, 16, [5000, 3], [33, 1], None),
+    ("int8", 128, 16, [100], [200], 16),
+    ("e4m3", 96, 128, [400], [129], 200),
+])
+@pytest.mark.parametrize("scale", [None, 2.0 ** -7, 2.0 ** -126])
+def test_small_queries_beside_pages_of_zeros(fmt, dim, page, past, counts, window, scale, dtype):
+    """Keys of zeros, pages that were never written, and pages that are reserved behind the last token: their steps are 2^-100 or none at all."""
+    g = torch.Generator().manual_seed(dim + page)
+    total = [p + n for p, n in zip(past, counts)]
+    slots = [-(-t // page) + 9 for t in total]
+    pages = sum(slots)
+    order = torch.randperm(pages, generator=g).tolist()
+    lists = [[order.pop() for _ in range(max(slots))] if i == 0 else [order.pop() for _ in range(min(len(order), max(slots)))] for i in range(len(total))]
+    lists = [row + [-1] * (max(slots) - len(row)) for row in lists]
+    table = ints(lists)
+    cache = lm_ops.Kv8(pages, 2, dim, page_size=page, format=fmt)
+    k, v = torch.randn(sum(total), 2, dim, generator=g), torch.randn(sum(total), 2, dim, generator=g)
+    at = 0
+    for n in total:
+        slot = torch.arange(n) // page
+        k[at:at + n][slot % 3 == 1] = 0
+        at += n
+    cache.append(k.to(DEV), v.to(DEV), table, ints([0] * len(total)), cumulative(total))
+    for row, n in zip(lists, total):
+        for p in row[3:-(-n // page):4]:                           # (given to the sequence, and not written)
+            for t in (cache.keys, cache.values, cache.key_scales, cache.value_scales):
+                t[p] = 0
+    shape = torch.randn(sum(counts), 8, dim, generator=g)
+    for size in (1.0, 2.0 ** -4, 2.0 ** -8, 2.0 ** -14, 2.0 ** -24, 2.0 ** -35, 2.0 ** -40, 0.0):
+        q = (size * shape).to(dtype).to(DEV)
+        got = lm_ops.attention_kv8(q, cache, table, ints(past), cumulative(counts), scale=scale, window=window)
+        check_attention(got, q, cache, table, past, counts, scale=scale, window=window, lists=lists)
