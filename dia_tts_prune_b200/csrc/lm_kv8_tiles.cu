@@ -264,10 +264,13 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cac
         return (int)max(0ll, (end + kStepKeys - 1) / kStepKeys);
     };
     const int n0 = steps_of(0), n1 = steps_of(1), steps = max(n0, n1), n = (steps + 1) / 2;      // of the halves, and tiles
+    // the page of a block of 16 tokens.  Places of the table behind the sequence's last token, and in front of the first one that these rows see, may hold anything: no page there
+    const long long seen_from = max(0ll, position(p0) - back), seen_to = (long long)q.past + q.n;
+    const auto page_at = [&](long long token) { return token < seen_to && token + kKvBlock > seen_from ? s.page(work.seq, token >> c.page_shift, c.pages) : -1; };
     const auto find_largest = [&] {                           // the largest exponent of the values' pages (all warps but the rows')
         int most = -1000;
         for (int b = threadIdx.x - 256; b < n * kBlocks; b += kThreads - 256) {
-            const int page = s.page(work.seq, ((long long)from * kKeys + (long long)b * kKvBlock) >> c.page_shift, c.pages);
+            const int page = page_at((long long)from * kKeys + (long long)b * kKvBlock);
             if (page < 0) continue;
             const uint32_t v = __float_as_uint(c.value_scales[(size_t)page * c.kv_heads + work.head]);
             if (v < 0x7f800000u) most = max(most, (int)(v >> 23) - 127);
@@ -629,7 +632,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cac
             mmas_ended<false>(&done[warp - 16]);
         } else if (warp == 18) {
             // lanes 0 .. 7 look a block up each: its scales a tile ahead, its page two
-            const auto page_of = [&](int i) { return lane < kBlocks && i < n ? s.page(work.seq, (((long long)from + i) * kKeys + lane * kKvBlock) >> c.page_shift, c.pages) : -1; };
+            const auto page_of = [&](int i) { return lane < kBlocks && i < n ? page_at(((long long)from + i) * kKeys + lane * kKvBlock) : -1; };
             const auto scales_of = [&](int page) {
                 const size_t at = (size_t)max(page, 0) * c.kv_heads + work.head;
                 return page >= 0 ? make_float2(c.key_scales[at], c.value_scales[at]) : make_float2(0.f, 0.f);

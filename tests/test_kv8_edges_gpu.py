@@ -80,3 +80,42 @@ def test_small_queries_beside_pages_of_zeros(fmt, dim, page, past, counts, windo
         q = (size * shape).to(dtype).to(DEV)
         got = lm_ops.attention_kv8(q, cache, table, ints(past), cumulative(counts), scale=scale, window=window)
         check_attention(got, q, cache, table, past, counts, scale=scale, window=window, lists=lists)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("fmt,page,past,counts,window", [
+    ("e4m3", 16, [0], [100], None),
+    ("int8", 32, [40, 7], [100, 200], None),
+    ("e4m3", 16, [200], [90], 30),                                 # pages in front of the window, in the first row's 128 tokens
+    ("e4m3", 64, [6000, 130], [33, 70], 3000),                     # keys in chunks
+    ("int8", 16, [129, 300], [1, 3], 50),                          # few rows
+])
+def test_unused_places_of_a_table(fmt, page, past, counts, window, dtype):
+    """Behind the page of a sequence's last token, and in front of the page of the first token that anyone sees, a table may name any page: no bit changes."""
+    g = torch.Generator().manual_seed(page + len(past))
+    total = [p + n for p, n in zip(past, counts)]
+    need = [-(-t // page) for t in total]
+    width, used = max(need) + 9, sum(need)
+    cache = lm_ops.Kv8(used + 3, 2, 64, page_size=page, format=fmt)
+    for t, fill in ((cache.keys, 120 if fmt == "e4m3" else 127), (cache.values, 120 if fmt == "e4m3" else 127), (cache.key_scales, 2.0 ** 100), (cache.value_scales, 2.0 ** 100)):
+        t[used:] = fill                                            # three pages of others, of very large numbers, one of which stands for NaNs
+    cache.value_scales[used + 1] = cache.key_scales[used + 2] = math.nan
+    order = torch.randperm(used, generator=g).tolist()
+    lists = []
+    for n in need:
+        lists.append([order.pop() for _ in range(n)] + [-1] * (width - n))
+    x = torch.randn(sum(total), 4, 64, generator=g) * 2.0 ** -20   # (its pages' steps are 2^80 below the others')
+    cache.append(x[:, :2].to(DEV) * 2.0 ** 20, x[:, 2:].to(DEV), ints(lists), ints([0] * len(total)), cumulative(total))
+    q = torch.randn(sum(counts), 8, 64, generator=g).to(dtype).to(DEV)
+    first = cumulative(counts)
+    want = lm_ops.attention_kv8(q, cache, ints(lists), ints(past), first, window=window)
+    if dtype != torch.float16:                                     # (which has no such small numbers)
+        check_attention(want, q, cache, ints(lists), past, counts, window=window, lists=lists)
+    for other in (used, used + 1, used + 2, 0):
+        changed = [list(row) for row in lists]
+        for row, p, n in zip(changed, past, need):
+            row[n:] = [other] * (width - n)
+            front = max(0, p + 1 - window) // page if window else 0
+            row[:front] = [other] * front
+        got = lm_ops.attention_kv8(q, cache, ints(changed), ints(past), first, window=window)
+        assert torch.equal(got, want), other
