@@ -77,7 +77,8 @@ __device__ __forceinline__ float load_q(const Kv8Attention& a, long long at) {
 }
 // what the sums of a row are times to be its output
 __device__ __forceinline__ float row_factor(const Kv8Attention& a, int head, float m, float w, float l) {
-    const float sink = a.sinks ? a.sinks[head] * kLog2e : -INFINITY;
+    float sink = a.sinks ? a.sinks[head] : -INFINITY;
+    sink = sink < INFINITY ? fminf(sink * kLog2e, 0x1.fffffep+127f) : sink * kLog2e;     // (a finite one stays finite: infinity less itself is no number)
     if (sink != -INFINITY) {
         const float top = fmaxf(m, sink);
         l = (m == -INFINITY ? l : l * exp2_fast(m - top)) + exp2_fast(sink - top);

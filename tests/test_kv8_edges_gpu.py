@@ -119,3 +119,29 @@ def test_unused_places_of_a_table(fmt, page, past, counts, window, dtype):
             row[:front] = [other] * front
         got = lm_ops.attention_kv8(q, cache, ints(changed), ints(past), first, window=window)
         assert torch.equal(got, want), other
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("past,counts", [([50], [1]), ([0], [100]), ([9000], [20])])
+def test_sinks_of_any_size(past, counts, dtype):
+    """Up to the largest and down to the lowest number of float32, which times log2(e) are none; the infinities: nothing in the denominator, and no number."""
+    g = torch.Generator().manual_seed(counts[0])
+    top = torch.finfo(torch.float32).max
+    lists = [list(range(-(-(past[0] + counts[0]) // 16)))]
+    table = ints(lists)
+    cache = lm_ops.Kv8(len(lists[0]), 2, 64)
+    x = torch.randn(past[0] + counts[0], 4, 64, generator=g).to(DEV)
+    cache.append(x[:, :2], x[:, 2:], table, ints([0]), cumulative([len(x)]))
+    q = torch.randn(counts[0], 8, 64, generator=g).to(dtype).to(DEV)
+    sinks = torch.tensor([top, 0.7 * top, 0.69 * top, 2.0 ** 100, -top, -0.69 * top, -math.inf, 0.0], device=DEV)
+    got = lm_ops.attention_kv8(q, cache, table, ints(past), cumulative(counts), sinks=sinks)
+    check_attention(got, q, cache, table, past, counts, sinks=sinks, lists=lists)
+    assert not got[:, :4].any()
+    bare = lm_ops.attention_kv8(q, cache, table, ints(past), cumulative(counts))
+    assert torch.equal(got[:, 4:7], bare[:, 4:7])
+    for bad in (math.inf, math.nan):
+        sinks[3] = bad
+        again = lm_ops.attention_kv8(q, cache, table, ints(past), cumulative(counts), sinks=sinks)
+        assert again[:, 3].isnan().all() and torch.equal(again[:, 4:], got[:, 4:])
+    # rows that see nothing have nothing to give, whatever the sink
+    assert not lm_ops.attention_kv8(q, cache, ints([[-1]]), ints(past), cumulative(counts), sinks=torch.full((8,), top, device=DEV)).any()
