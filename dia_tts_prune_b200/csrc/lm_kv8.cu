@@ -125,11 +125,13 @@ __global__ void __launch_bounds__(kAppendThreads, 4) kv8_append_kernel(Kv8Cache 
     };
     int row = (int)row0, seq = sequence_by_warp(s, row);
     while (row < last) {
-        if (seq < 0) {                                        // no row of a sequence: on to the next one that is
+        const int begin = s.begin(max(seq, 0)), end = s.end(max(seq, 0));
+        // no row of a sequence: on to the next one that is.  (Where `first` decreases, the look-up may name a sequence that does not have the row.  Past this a turn goes at least one row on.)
+        if (seq < 0 || row < begin || row >= end) {
             if (++row < last) seq = sequence_by_warp(s, row);
             continue;
         }
-        const int begin = s.begin(seq), end = s.end(seq), past = s.past[seq];
+        const int past = s.past[seq];
         const long long pos = (long long)past + (row - begin);
         const int place = (int)(pos & (page_size - 1));
         const int ends = min(end, row + page_size - place);    // of the rows that go into this page

@@ -330,7 +330,8 @@ class Kv8:
     Which pages a sequence has is the caller's to keep (``PagedState`` does it for served models): every call takes a ``table [sequences, n]`` of
     page numbers, int32, whose unused places may hold anything.  Together with ``past [sequences]`` and ``first [sequences + 1]`` (int32, on the
     device, so that a captured graph reads them anew) it describes the rows of a step: sequence ``i`` has rows ``first[i]`` to ``first[i + 1]`` of the
-    packed ones, at positions ``past[i]`` and on; without ``first``, row ``i`` alone.  A token whose place lies beyond the table, or whose page is not
+    packed ones, at positions ``past[i]`` and on; without ``first``, row ``i`` alone.  ``first`` does not decrease (where it does, calls still end and
+    stay within the tensors, but which rows are whose is not said).  A token whose place lies beyond the table, or whose page is not
     in the pool, is not there: it is not written, not seen, and reads as zeros.  A sequence whose ``past`` is negative has no tokens."""
     __slots__ = ("keys", "values", "key_scales", "value_scales", "pages", "kv_heads", "page_size", "dim", "format", "_handle", "_at", "_index")
 

@@ -351,7 +351,7 @@ typedef struct lm_b200_kv8 {
 } lm_b200_kv8;
 /* The rows of a step (arrays on the device): sequence i has rows first[i] .. first[i + 1] of them (first NULL: row i alone, n_seq == rows), at positions past[i] and on; its page of
  * position p is table[i * table_ld + p / page_size].  A token whose place lies beyond max_pages, or whose page is not 0 .. pages - 1, is not there: not written, not seen, zeros when
- * read.  A sequence whose past is negative has no tokens. */
+ * read.  A sequence whose past is negative has no tokens.  first does not decrease: where it does, calls still end and stay within the arrays, but which rows are whose is not said. */
 typedef struct lm_b200_kv8_step {
     const int32_t *table;
     int64_t table_ld;

@@ -145,3 +145,39 @@ def test_sinks_of_any_size(past, counts, dtype):
         assert again[:, 3].isnan().all() and torch.equal(again[:, 4:], got[:, 4:])
     # rows that see nothing have nothing to give, whatever the sink
     assert not lm_ops.attention_kv8(q, cache, ints([[-1]]), ints(past), cumulative(counts), sinks=torch.full((8,), top, device=DEV)).any()
+
+
+@pytest.mark.parametrize("order", [[0, 10, 5, 12], [0, 5, 3, 8], [7, 3, 12, 0], [12, 0, 0, 0], [-4, 9, 2, 40], [5, 1 << 30, -(1 << 31), 12]])
+@pytest.mark.parametrize("sequences", [3, 1500])
+@pytest.mark.parametrize("rows", [12, 2000])
+def test_rows_of_sequences_in_no_order(order, sequences, rows):
+    """`first` that decreases somewhere: which rows are whose is not said, but every call ends, and pages that the table does not name stay what they are."""
+    g = torch.Generator().manual_seed(rows)
+    cache = lm_ops.Kv8(2 * sequences + 8, 2, 64)
+    for t in (cache.keys, cache.values):
+        t.fill_(56)
+    for t in (cache.key_scales, cache.value_scales):
+        t.fill_(2.0)
+    before = [t.clone() for t in (cache.keys, cache.values, cache.key_scales, cache.value_scales)]
+    table = torch.arange(2 * sequences, dtype=torch.int32, device=DEV).view(sequences, 2)
+    past = ints([5, 0, 20] + [1] * (sequences - 3))
+    first = ints([v * rows // 12 if abs(v) < 100 else v for v in order] + [rows - 3] * (sequences - 3))
+    x = torch.randn(rows, 4, 64, generator=g).to(DEV)
+    cache.append(x[:, :2], x[:, 2:], table, past, first)
+    torch.cuda.synchronize()
+    for t, b in zip((cache.keys, cache.values, cache.key_scales, cache.value_scales), before):
+        assert torch.equal(t[2 * sequences:], b[2 * sequences:])
+    assert torch.isfinite(cache.key_scales).all() and torch.isfinite(cache.value_scales).all()
+    assert all(torch.isfinite(y).all() for y in cache.read(table, past, first, rows))
+    for dtype in (torch.bfloat16, torch.float32):
+        q = torch.randn(rows, 8, 64, generator=g).to(dtype).to(DEV)
+        lm_ops.attention_kv8(q, cache, table, past, first)
+    torch.cuda.synchronize()
+    # and a step in order behind it is what it should be
+    twin = lm_ops.Kv8(2 * sequences + 8, 2, 64)
+    first = ints([0, 4, 8] + [12] * (sequences - 2))
+    for c in (cache, twin):
+        c.append(x[:12, :2], x[:12, 2:], table, ints([0] * sequences), first)
+    q = torch.randn(12, 8, 64, generator=g).to(DEV)
+    got, want = (lm_ops.attention_kv8(q, c, table, ints([0] * sequences), first) for c in (cache, twin))
+    assert torch.equal(got, want)
