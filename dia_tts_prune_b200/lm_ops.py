@@ -97,7 +97,7 @@ def _no_tangent(what: str, *xs: torch.Tensor) -> None:
 def _no_grad(what: str, x: torch.Tensor) -> None:
     _no_tangent(what, x)
     if x.requires_grad and torch.is_grad_enabled():
-        raise ValueError(f"{what} has no gradient: detach its rows or call it under torch.no_grad()")
+        raise ValueError(f"{what} has no gradient: detach its operands or call it under torch.no_grad()")
 
 
 class Mxfp4:
@@ -464,7 +464,8 @@ def attention_kv8(q: torch.Tensor, cache: Kv8, table: torch.Tensor, past: torch.
 
     float32 rows are multiplied with 22 bits, as the language models' attention does; weights are rounded to 22 bits for them, to 11 for the other types (a
     token whose part in a row's result is below 2^-20 of what the largest one's may be, to 2^-31 of that).  Maxima, sums and outputs are float32 until the
-    result.  Values in pages whose power is 2^80 below the largest in a sequence's pages may be taken as zeros.  It has no gradient."""
+    result.  Values in pages whose power is 2^80 below the largest in a sequence's pages may be taken as zeros.  It has no gradient: ``q`` or ``sinks`` that want one,
+    or have a tangent, are refused."""
     _check_rows(q, "q")
     if not isinstance(cache, Kv8):
         raise TypeError("cache must be a Kv8")
@@ -487,6 +488,7 @@ def attention_kv8(q: torch.Tensor, cache: Kv8, table: torch.Tensor, past: torch.
         _check_rows(sinks, "sinks", (torch.float32,))
         if sinks.shape != (heads,):
             raise ValueError(f"sinks must hold one number for each of {heads} heads")
+        _no_grad("attention_kv8", sinks)
         _check_device(cache.keys.device, sinks)
         sinks = sinks.contiguous()
     if rows > 0x7fffff00 // heads:
