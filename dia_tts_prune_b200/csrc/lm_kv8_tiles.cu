@@ -73,6 +73,7 @@ struct Work {
     int seq, head, tile, chunk, chunks, first_cta, length;    // seq -1: nothing; length: of a chunk in tiles of keys
 };
 constexpr int kWhole = 0x7fffffff;
+constexpr int kMostItems = 0x3000000;                          // above what a launch has (2^31 pairs / 256, and / 65 for the sequences' last ones), and 32 lanes' sums are below 2^31
 // One warp: what the CTA of this index takes
 __device__ __forceinline__ Work find_work(const Kv8Cache& c, const Kv8Step& s, const Kv8Attention& a, int group, int index) {
     const int lane = threadIdx.x & 31, each = (s.sequences + 31) / 32, i0 = lane * each, i1 = min(i0 + each, s.sequences);
@@ -90,7 +91,7 @@ __device__ __forceinline__ Work find_work(const Kv8Cache& c, const Kv8Step& s, c
     int items = 0, most = 0, ctas = 0;
     for (int i = i0; i < i1; ++i) {
         const Sequence q = at(i);
-        items += q.tiles * c.kv_heads;
+        items = min(items + q.tiles * c.kv_heads, kMostItems);    // (offsets that decrease may count rows many times)
         if (q.tiles) most = max(most, q.high - q.low);
     }
     const int2 of_items = before(items);
@@ -102,7 +103,7 @@ __device__ __forceinline__ Work find_work(const Kv8Cache& c, const Kv8Step& s, c
     const auto chunks_of = [&](const Sequence& q) { return length == kWhole ? 1 : max(1, (q.high - q.low + length - 1) / length); };
     for (int i = i0; i < i1; ++i) {
         const Sequence q = at(i);
-        ctas += q.tiles * c.kv_heads * chunks_of(q);
+        ctas = min(ctas + q.tiles * c.kv_heads * chunks_of(q), kMostItems);
     }
     int base = before(ctas).x;
     const bool here = index >= base && index < base + ctas;

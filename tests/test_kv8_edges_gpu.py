@@ -181,3 +181,18 @@ def test_rows_of_sequences_in_no_order(order, sequences, rows):
     q = torch.randn(12, 8, 64, generator=g).to(DEV)
     got, want = (lm_ops.attention_kv8(q, c, table, ints([0] * sequences), first) for c in (cache, twin))
     assert torch.equal(got, want)
+
+
+def test_rows_counted_many_times():
+    """`first` that goes up and down 2049 times: what its sequences' rows come to passes 32 bits, and the call ends all the same."""
+    sequences, rows = 4098, 1 << 16
+    cache = lm_ops.Kv8(4, 1, 1)
+    q = torch.zeros(rows, 4096, 1, dtype=torch.bfloat16, device=DEV)   # 2^20 tiles of 256 pairs
+    table = torch.full((sequences, 1), -1, dtype=torch.int32, device=DEV)
+    past = torch.zeros(sequences, dtype=torch.int32, device=DEV)
+    first = torch.zeros(sequences + 1, dtype=torch.int32, device=DEV)
+    first[1::2] = rows
+    lm_ops.attention_kv8(q, cache, table, past, first)
+    torch.cuda.synchronize()
+    first[2:] = rows                                               # (the first sequence's, once)
+    assert not lm_ops.attention_kv8(q, cache, table, past, first).any()
