@@ -319,8 +319,10 @@ __global__ void __launch_bounds__(kReadThreads) kv8_read_kernel(Kv8Cache c, Kv8S
 // tokens by byte permutations, and the weights by movmatrix.
 //
 // Codes are exact in fp16.  A row of queries is scaled by a power of two to below 2^14 and taken as one fp16 term (bf16 and fp16 rows: exact but for channels 2^-27 below the
-// row's largest), or two (fp32: 22 bits).  Weights: the page's value scale is part of the exponent, 2^(x + e - max (x + e)) 2^14, so that the largest contribution, not the largest
-// weight, is what fp16's 11 bits count from (fp32 rows: two terms, 22 bits); sums, maxima and outputs are fp32, and the denominator is summed from fp32 weights without the scale.
+// row's largest), or two (fp32: 22 bits).  Weights: the page's value scale is part of the exponent, 2^(x + e - W) 2^15, W = max (ceil(x) + e), so that the largest contribution, not the largest
+// weight, is what fp16's 11 bits count from (fp32 rows: two terms, 22 bits; 11 are what results in fp16 have themselves, and three more than bf16's).  Sums, maxima and outputs are fp32, and the
+// denominator is summed from fp32 weights without the scale.  References of weights are whole numbers, so what is between two of them, or between them and a page's exponent, is exact (with
+// fractions of scores in them fp32 outputs were off by up to 8e-7 of the sum of weighted magnitudes, 3e-6 where values are 2^100; so they are by 3.3e-7).
 // A tensor-core sum is cut off at every step: fp32 rows add the second terms' sums and every block's outputs to theirs by fp32 additions.
 constexpr int kMetaBlocks = 256, kMostPeers = 8;               // CTAs of a cluster
 
@@ -668,6 +670,9 @@ __global__ void __launch_bounds__(Few<DP, TERMS, NT>::kThreads, Few<DP, TERMS, N
                         top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 8));
                         top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 16));
                     }
+                    // (references are whole: what they differ by is exact, whatever the pages' exponents are, and so is a power of two of that)
+                    top[0] = ceilf(top[0]);
+                    top[1] = ceilf(top[1]);
                     const float m0 = fmaxf(m[n][0], top[0]), m1 = fmaxf(m[n][1], top[1]), w0 = fmaxf(w[n][0], top[0] + ev), w1 = fmaxf(w[n][1], top[1] + ev);
                     if (__any_sync(0xffffffffu, m0 > m[n][0] || m1 > m[n][1] || w0 > w[n][0] || w1 > w[n][1])) {
                         const float c0 = lower_to(w[n][0], w0), c1 = lower_to(w[n][1], w1);
@@ -677,13 +682,20 @@ __global__ void __launch_bounds__(Few<DP, TERMS, NT>::kThreads, Few<DP, TERMS, N
                         for (int j = 0; j < kCols; ++j) { o[n][j][0] *= c0; o[n][j][1] *= c1; o[n][j][2] *= c0; o[n][j][3] *= c1; }
                         m[n][0] = m0; m[n][1] = m1; w[n][0] = w0; w[n][1] = w1;
                     }
-                    float p[4];
+                    // weights below the block's own largest, which the sum and the products take to their references
+                    float p[4], to_l[2], to_w[2], from[2];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const bool none = top[e] == -INFINITY;                       // (nothing of the block is seen)
+                        from[e] = none ? 0.f : top[e];
+                        to_l[e] = none ? 0.f : exp2_fast(top[e] - m[n][e]);
+                        to_w[e] = none ? 0.f : exp2_fast(top[e] + ev - w[n][e] + kWeightBits);
+                    }
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        // (rows that have seen nothing yet: any reference will do)
-                        const float r = m[n][e & 1] == -INFINITY ? 0.f : m[n][e & 1], q = (w[n][e & 1] == -INFINITY ? 0.f : w[n][e & 1]) - ev - kWeightBits;
-                        l[n][e & 1] += exp2_fast(x[n][e] - r);
-                        p[e] = exp2_fast(x[n][e] - q);
+                        const float y = exp2_fast(x[n][e] - from[e & 1]);
+                        l[n][e & 1] = fmaf(y, to_l[e & 1], l[n][e & 1]);
+                        p[e] = y * to_w[e & 1];
                         if (!clear && (hidden >> e & 1)) p[e] = 0.f;                  // (whatever the page's scales are)
                     }
                     const uint32_t h0 = pack_half(p[0], p[1]), h1 = pack_half(p[2], p[3]);

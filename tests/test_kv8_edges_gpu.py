@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from dia_tts_prune_b200 import lm_ops
-from test_kv8_gpu import DEV, check_attention, cumulative, ints
+from test_kv8_gpu import DEV, check_attention, cumulative, ints, tables
 
 pytestmark = pytest.mark.gpu
 
@@ -196,3 +196,23 @@ def test_rows_counted_many_times():
     torch.cuda.synchronize()
     first[2:] = rows                                               # (the first sequence's, once)
     assert not lm_ops.attention_kv8(q, cache, table, past, first).any()
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("size", [1.0, 2.0 ** -12])
+@pytest.mark.parametrize("past,count", [(0, 1), (30, 2), (700, 1)])
+def test_float32_rows_keep_their_bits(fmt, size, past, count):
+    """Pages of values of many powers: what the references of a row's weights are rounded by does not show in it."""
+    g = torch.Generator().manual_seed(past + count)
+    n = 100
+    counts, pasts = [count] * n, [max(0, past - i) for i in range(n)]
+    total = [p + c for p, c in zip(pasts, counts)]
+    pages = sum(-(-t // 16) for t in total)
+    lists, table = tables(counts, pasts, 16, pages, g)
+    cache = lm_ops.Kv8(pages, 2, 64, format=fmt)
+    k, v = torch.randn(sum(total), 2, 64, generator=g), torch.randn(sum(total), 2, 64, generator=g)
+    v *= torch.exp2(torch.randint(-30, 31, (len(v) // 16 + 1, 1, 1), generator=g).float())[torch.arange(len(v)) // 16]
+    cache.append(k.to(DEV), v.to(DEV), table, ints([0] * n), cumulative(total))
+    q = (size * torch.randn(sum(counts), 16, 64, generator=g)).to(DEV)
+    got = lm_ops.attention_kv8(q, cache, table, ints(pasts), cumulative(counts))
+    check_attention(got, q, cache, table, pasts, counts, lists=lists)
