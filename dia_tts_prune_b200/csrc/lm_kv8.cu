@@ -319,10 +319,11 @@ __global__ void __launch_bounds__(kReadThreads) kv8_read_kernel(Kv8Cache c, Kv8S
 // tokens by byte permutations, and the weights by movmatrix.
 //
 // Codes are exact in fp16.  A row of queries is scaled by a power of two to below 2^14 and taken as one fp16 term (bf16 and fp16 rows: exact but for channels 2^-27 below the
-// row's largest), or two (fp32: 22 bits).  Weights: the page's value scale is part of the exponent, 2^(x + e - W) 2^15, W = max (ceil(x) + e), so that the largest contribution, not the largest
-// weight, is what fp16's 11 bits count from (fp32 rows: two terms, 22 bits; 11 are what results in fp16 have themselves, and three more than bf16's).  Sums, maxima and outputs are fp32, and the
-// denominator is summed from fp32 weights without the scale.  References of weights are whole numbers, so what is between two of them, or between them and a page's exponent, is exact (with
-// fractions of scores in them fp32 outputs were off by up to 8e-7 of the sum of weighted magnitudes, 3e-6 where values are 2^100; so they are by 3.3e-7).
+// row's largest), or two (fp32: 22 bits).  Weights: the page's value scale is part of the exponent, 2^(x + e - W) 2^14, W = max (x + e), so that the largest contribution, not the largest
+// weight, is what fp16's 11 bits count from (11 are what results in fp16 have themselves, and three more than bf16's; the largest weight is a power of two and loses nothing, which is what rows
+// with one large weight live by: with W a whole number results in fp16 were off by 2.6e-4, not 2.1e-4).  fp32 rows have two terms, 22 bits, and whole references, max (floor(x) + e): what lies
+// between two of them, or between them and a page's exponent, is then exact (with fractions of scores in them outputs were off by up to 8e-7 of the sum of weighted magnitudes, 3e-6 where values
+// are 2^100; so they are by 3e-7; a prompt of 4096 takes 1 % more, single tokens no more).  Sums, maxima and outputs are fp32, and the denominator is summed from fp32 weights without the scale.
 // A tensor-core sum is cut off at every step: fp32 rows add the second terms' sums and every block's outputs to theirs by fp32 additions.
 constexpr int kMetaBlocks = 256, kMostPeers = 8;               // CTAs of a cluster
 
@@ -670,9 +671,11 @@ __global__ void __launch_bounds__(Few<DP, TERMS, NT>::kThreads, Few<DP, TERMS, N
                         top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 8));
                         top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 16));
                     }
-                    // (references are whole: what they differ by is exact, whatever the pages' exponents are, and so is a power of two of that)
-                    top[0] = ceilf(top[0]);
-                    top[1] = ceilf(top[1]);
+                    // (of two terms: whole references, so that what they differ by is exact, whatever the pages' exponents are.  Of one: the largest weight itself is 2^14, which fp16 has as it is)
+                    if constexpr (TERMS == 2) {
+                        top[0] = floorf(top[0]);
+                        top[1] = floorf(top[1]);
+                    }
                     const float m0 = fmaxf(m[n][0], top[0]), m1 = fmaxf(m[n][1], top[1]), w0 = fmaxf(w[n][0], top[0] + ev), w1 = fmaxf(w[n][1], top[1] + ev);
                     if (__any_sync(0xffffffffu, m0 > m[n][0] || m1 > m[n][1] || w0 > w[n][0] || w1 > w[n][1])) {
                         const float c0 = lower_to(w[n][0], w0), c1 = lower_to(w[n][1], w1);
@@ -682,22 +685,35 @@ __global__ void __launch_bounds__(Few<DP, TERMS, NT>::kThreads, Few<DP, TERMS, N
                         for (int j = 0; j < kCols; ++j) { o[n][j][0] *= c0; o[n][j][1] *= c1; o[n][j][2] *= c0; o[n][j][3] *= c1; }
                         m[n][0] = m0; m[n][1] = m1; w[n][0] = w0; w[n][1] = w1;
                     }
-                    // weights below the block's own largest, which the sum and the products take to their references
-                    float p[4], to_l[2], to_w[2], from[2];
+                    float p[4];
+                    if constexpr (TERMS == 2) {
+                        // counted from the block's own largest, which the sum and the products take to their references
+                        float to_l[2], to_w[2], from[2];
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const bool none = top[e] == -INFINITY;                       // (nothing of the block is seen)
-                        from[e] = none ? 0.f : top[e];
-                        to_l[e] = none ? 0.f : exp2_fast(top[e] - m[n][e]);
-                        to_w[e] = none ? 0.f : exp2_fast(top[e] + ev - w[n][e] + kWeightBits);
+                        for (int e = 0; e < 2; ++e) {
+                            const bool none = top[e] == -INFINITY;                   // (nothing of the block is seen)
+                            from[e] = none ? 0.f : top[e];
+                            to_l[e] = none ? 0.f : exp2_fast(top[e] - m[n][e]);
+                            to_w[e] = none ? 0.f : exp2_fast(top[e] + ev - w[n][e] + kWeightBits);
+                        }
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float y = exp2_fast(x[n][e] - from[e & 1]);
+                            l[n][e & 1] = fmaf(y, to_l[e & 1], l[n][e & 1]);
+                            p[e] = y * to_w[e & 1];
+                        }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            // (rows that have seen nothing yet: any reference will do)
+                            const float r = m[n][e & 1] == -INFINITY ? 0.f : m[n][e & 1], q = (w[n][e & 1] == -INFINITY ? 0.f : w[n][e & 1]) - ev - kWeightBits;
+                            l[n][e & 1] += exp2_fast(x[n][e] - r);
+                            p[e] = exp2_fast(x[n][e] - q);
+                        }
                     }
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float y = exp2_fast(x[n][e] - from[e & 1]);
-                        l[n][e & 1] = fmaf(y, to_l[e & 1], l[n][e & 1]);
-                        p[e] = y * to_w[e & 1];
+                    for (int e = 0; e < 4; ++e)
                         if (!clear && (hidden >> e & 1)) p[e] = 0.f;                  // (whatever the page's scales are)
-                    }
                     const uint32_t h0 = pack_half(p[0], p[1]), h1 = pack_half(p[2], p[3]);
                     hi[n] = make_uint2(transposed(h0), transposed(h1));
                     if constexpr (TERMS == 2) lo[n] = make_uint2(transposed(rest_of(p[0], p[1], h0)), transposed(rest_of(p[2], p[3], h1)));
@@ -956,7 +972,8 @@ struct FewWork {
 inline int padded_dim(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 inline int terms_of(int type) { return type == kTypeF32 ? 2 : 1; }
 // tiles of eight rows where sequences have no more of them on average (the products of 16 rows take twice the registers and the tensor cores' time: 64 requests 226 and 305 us, eight of
-// fp32 19 and 24; two tiles of eight would read the cache twice)
+// fp32 19 and 24; two tiles of eight would read the cache twice).  The average is over all of a step's rows: beside prompts single tokens get tiles of 16, as
+// which sequence has how many rows is known on the device alone.
 inline bool eight_rows(int kv_heads, int rows, int heads, int sequences) { return (long long)rows * (heads / kv_heads) <= 8ll * sequences; }
 
 template <int DP, int FORMAT, int TERMS, int NT>
@@ -1023,10 +1040,13 @@ cudaError_t launch_kv8_read(const Kv8Cache& c, const Kv8Step& s, void* k, void* 
 
 namespace {
 // Pairs of a sequence up to which tiles of 16 of them are the shorter way (four heads a key head; these and those of 256 rows: 36 pairs behind 1000 tokens 14 and 22 us, behind 16000
-// 36 and 31; 68 pairs 17 and 25, 40 and 37, of eight sequences behind 8000 tokens 97 and 53)
+// 36 and 31; 68 pairs 17 and 25, 40 and 37, of eight sequences behind 8000 tokens 97 and 53).  How long pasts are moves the border and is known on the device alone, as is which sequence has how many
+// rows: a step of more pairs in all gets both kernels.  So do single tokens, without `first` too, where the host could know that none of them needs the tiles': 17 of four heads a key head
+// behind 1000 tokens take 18.3 us, 16 of them 12.0.
 constexpr int kFewMost = 64;
 // Tables of up to so many tokens for each of a cluster's CTAs: no tile is shared by others, which would need counters (a launch more) and sums by way of memory.  One request of 1025
-// tokens: 14.3 us by one CTA a tile, 13.2 shared, 9.7 by eight; of 4000: 11.7 and 14.0 shared; of 16000: 21.6 and 20.0; nine of 8000: 29.2 by four and 24.0.
+// tokens: 14.3 us by one CTA a tile, 13.2 shared, 9.7 by eight; of 4000: 11.7 and 14.0 shared; of 16000: 21.6 and 20.0; nine of 8000: 29.2 by four and 24.0.  (Lengths are on the device, so that a
+// table with room for more goes the shared way however short its sequences are.)
 constexpr int kWholeTokens = 1024;
 // and at least so many (of 128 tokens: 8.1 us alone, 9.0 by eight)
 constexpr int kPeerTokens = 128;

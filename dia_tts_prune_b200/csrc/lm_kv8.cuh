@@ -48,7 +48,7 @@ __device__ __forceinline__ float4 values4(uint32_t w, float scale) {
     return make_float4(a.x * scale, a.y * scale, b.x * scale, b.y * scale);
 }
 
-constexpr float kLog2e = 1.4426950408889634f, kWeightBits = 15.f;
+constexpr float kLog2e = 1.4426950408889634f, kWeightBits = 14.f;
 
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;
@@ -80,7 +80,7 @@ __device__ __forceinline__ float row_factor(const Kv8Attention& a, int head, flo
     float sink = a.sinks ? a.sinks[head] : -INFINITY;
     sink = sink < INFINITY ? fminf(sink * kLog2e, 0x1.fffffep+127f) : sink * kLog2e;     // (a finite one stays finite: infinity less itself is no number)
     if (sink != -INFINITY) {
-        const float top = fmaxf(m, ceilf(sink));
+        const float top = fmaxf(m, a.type == kTypeF32 ? floorf(sink) : sink);       // (whole, as the references of fp32 rows are)
         l = (m == -INFINITY ? l : l * exp2_fast(m - top)) + exp2_fast(sink - top);
         m = top;
     }

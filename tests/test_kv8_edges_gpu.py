@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from dia_tts_prune_b200 import lm_ops
-from test_kv8_gpu import DEV, check_attention, cumulative, ints, tables
+from test_kv8_gpu import DEV, HALF, check_attention, cumulative, ints, tables
 
 pytestmark = pytest.mark.gpu
 
@@ -216,3 +216,69 @@ def test_float32_rows_keep_their_bits(fmt, size, past, count):
     q = (size * torch.randn(sum(counts), 16, 64, generator=g)).to(DEV)
     got = lm_ops.attention_kv8(q, cache, table, ints(pasts), cumulative(counts))
     check_attention(got, q, cache, table, pasts, counts, lists=lists)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("past,count", [(0, 1), (333, 3), (5000, 1), (0, 200), (3000, 100)])
+def test_rows_with_one_large_weight(past, count, fmt, dtype):
+    """A row whose weight lies on one token (the others have less than 2^-60 of it) is that token's values, which 8 significant bits and a power of two give every type exactly."""
+    g = torch.Generator().manual_seed(past + count)
+    n = past + count
+    lists, table = tables([count], [past], 16, -(-n // 16), g)
+    cache = lm_ops.Kv8(-(-n // 16), 2, 64, format=fmt)
+    k, v = torch.randn(n, 2, 64, generator=g), torch.randn(n, 2, 64, generator=g)
+    k /= k.norm(dim=-1, keepdim=True)
+    cache.append(k.to(DEV), v.to(DEV), table, ints([0]), ints([0, n]))
+    own = (torch.rand(count, 8, generator=g) * (past + 1 + torch.arange(count))[:, None]).long()
+    head = (torch.arange(8) // 4).expand(count, 8)
+    q = (4096 * k[own, head]).to(dtype).to(DEV)
+    read_k, read_v = (y.double() for y in cache.read(table, ints([0]), ints([0, n]), n))
+    z = torch.einsum("rhd,thd->rht", q.double(), read_k.repeat_interleave(4, 1)) / 8
+    t = torch.arange(n, device=DEV)
+    z = z.masked_fill(t > past + torch.arange(count, device=DEV)[:, None, None], -math.inf)
+    best = z.argmax(-1)
+    top = z.topk(min(2, n), -1).values
+    alone = top[..., 0] - top[..., -1] > 60 * math.log(2) if n > 1 else torch.ones(count, 8, dtype=torch.bool, device=DEV)
+    alone |= (past + torch.arange(count, device=DEV) == 0)[:, None]
+    assert alone.float().mean() > 0.9
+    got = lm_ops.attention_kv8(q, cache, table, ints([past]), ints([0, count]))
+    want = read_v[best, head.to(DEV)]
+    assert torch.equal(want, want.to(dtype).double()) and torch.equal(got[alone].double(), want[alone])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+def test_the_largest_weight_of_few_rows_is_not_rounded(fmt, dtype):
+    """Where pages' values have one power, a row's largest weight is 2^14 in fp16: what weights are rounded by (2^-11) counts for the others alone.  The rest of the bound is
+    check_attention's, of scores and sums."""
+    g = torch.Generator().manual_seed(31)
+    n = 100
+    past = [15 + i // 2 for i in range(n)]
+    total = [p + 1 for p in past]
+    lists, table = tables([1] * n, past, 16, sum(-(-t // 16) for t in total), g)
+    cache = lm_ops.Kv8(sum(-(-t // 16) for t in total), 1, 64, format=fmt)
+    k, v = torch.randn(sum(total), 1, 64, generator=g), torch.randn(sum(total), 1, 64, generator=g).clamp(-5, 5)
+    k /= k.norm(dim=-1, keepdim=True)
+    q, at = torch.empty(n, 4, 64), 0
+    for i, t in enumerate(total):
+        v[at:at + t:16, 0, 63] = 6                                 # (in every page)
+        q[i] = 60 * k[at + torch.randint(0, t, (4,), generator=g), 0]
+        at += t
+    cache.append(k.to(DEV), v.to(DEV), table, ints([0] * n), cumulative(total))
+    q = q.to(dtype).to(DEV)
+    got = lm_ops.attention_kv8(q, cache, table, ints(past))
+    assert cache.value_scales[[p for row in lists for p in row if p >= 0]].unique().numel() == 1
+    large = 0
+    for i, t in enumerate(total):
+        k1, v1 = (y.double()[:, 0] for y in cache.read(table[i:i + 1], ints([0]), ints([0, t]), t))
+        z = q[i].double() @ k1.T / 8
+        p = torch.softmax(z, -1)
+        large += int((p.amax(-1) > 0.5).sum())
+        rest = p.scatter(1, p.argmax(-1, keepdim=True), 0.0)
+        A = (q[i].double().abs() @ k1.abs().T / 8).amax(-1, keepdim=True)
+        e = A * (2.0 ** -22 + (64 / 16 + 8) * 2.0 ** -23)
+        o, B = p @ v1, p @ v1.abs()
+        bound = HALF[dtype] * o.abs() + 2.0 ** -11 * (rest @ v1.abs()) + B * (2 * e + 2.0 ** -20) + t * 6 * 2.0 ** -37 + 2.0 ** -25
+        assert ((got[i].double() - o).abs() <= bound).all(), i
+    assert large > 200
