@@ -10,10 +10,10 @@
 // Numbers.  t = scale log2(e) q . key + e - E in powers of two, e the exponent of the page's values and E the largest of the CTA's pages; P = 2^(t - R + 7) in fp16, with R the
 // row's reference: about its largest t so far, raised (and O and the sum with it) only when one of 64 scores lies more than 8 above it, so P is at most 2^15.  That the page's value
 // scale is inside
-// the weight lets codes be multiplied as they are, and the 11 bits of P count from the largest contribution.  The denominator takes 2^(E - e) out again, per 16 tokens.  Pages whose
-// values are 2^80 below the largest page's are taken as zeros.  Queries are scaled by a power of two per row (exact but for channels 2^-27 below the row's largest).  Sums are fp32;
-// O's live in tensor memory for the whole run of keys, and lose up to one unit in the last place per 16 keys (2^-24 on average: 2^-11 of the sum after 131072 keys, against the
-// 2^-9 of bf16).
+// the weight lets codes be multiplied as they are, and the 11 bits of P (a result in fp16 has no more, one in bf16 eight) count from the largest contribution.  The denominator takes
+// 2^(E - e) out again, per 16 tokens.  Pages are those that the rows see; whose values are 2^80 below the largest page's are taken as zeros.  Queries are scaled by a power of two per row
+// (exact but for channels 2^-27 below the row's largest).  Sums are fp32; O's live in tensor memory for the whole run of keys, and lose up to one unit in the last place per 16 keys (2^-24 on
+// average: 2^-11 of the sum after 131072 keys, an eighth of what the result's rounding to bf16 may be off by, and as much as that to fp16).
 //
 // Bound: per 256 x 128 tile and dim 128 the tensor pipe takes 2048 cycles, the exponentials (16 a cycle) 2048, and shared memory 2048 (the scores' operands 1024, the values 512,
 // the codes turned into operands 512).

@@ -371,7 +371,8 @@ class Kv8:
         sequence ``i`` holds.  A page's exponent is the smallest, at least -100, for which its largest magnitude so far is at most 448 (``"int8"``: 127)
         times the power; codes go to the nearest, half way to the even one.  Where a page that holds earlier tokens needs a larger exponent, their codes
         are rounded again.  The first token of a page starts it anew, whatever it held.  A number that is not finite makes the page's head stand for NaNs
-        until then.  No page may belong to two sequences of a call."""
+        until then; finite ones of about 2^128 are read as infinity where that is the nearest number.  No page may be named twice by the places that a call's
+        tokens go to."""
         _check_rows(k, "k")
         _check_rows(v, "v")
         shape = k.shape
@@ -464,8 +465,11 @@ def attention_kv8(q: torch.Tensor, cache: Kv8, table: torch.Tensor, past: torch.
 
     float32 rows are multiplied with 22 bits, as the language models' attention does; weights are rounded to 22 bits for them, to 11 for the other types (a
     token whose part in a row's result is below 2^-20 of what the largest one's may be, to 2^-31 of that).  Maxima, sums and outputs are float32 until the
-    result.  Values in pages whose power is 2^80 below the largest in a sequence's pages may be taken as zeros.  It has no gradient: ``q`` or ``sinks`` that want one,
-    or have a tangent, are refused."""
+    result; of 16-bit prompts the outputs' additions are cut off, not rounded, up to 2^-11 of their sum behind 131072 tokens.  Values in pages whose power is
+    2^80 below the largest in a sequence's pages may be taken as zeros.  A row with a number that is not finite is NaN where it sees anything.  Scores are
+    float32: a row whose largest number times ``scale``, or that times a page's power, is beyond its range may be NaN.
+
+    It has no gradient: ``q`` or ``sinks`` that want one, or have a tangent, are refused."""
     _check_rows(q, "q")
     if not isinstance(cache, Kv8):
         raise TypeError("cache must be a Kv8")

@@ -359,7 +359,7 @@ typedef struct lm_b200_kv8_step {
     int32_t max_pages, n_seq, rows;
 } lm_b200_kv8_step;
 /* k, v [rows][kv_heads][dim] of `type` (neighbouring channels; k_row, k_head, .. elements from one row or head to the next) into the pages.  A page that holds earlier tokens of its
- * sequence keeps them; they are rounded again where its exponent has to grow.  No page may belong to two sequences of a call. */
+ * sequence keeps them; they are rounded again where its exponent has to grow.  No page may be named twice by the places that a call's tokens go to. */
 int lm_b200_op_kv8_append(const lm_b200_kv8 *cache, const lm_b200_kv8_step *step, const void *k, int64_t k_row, int64_t k_head, const void *v, int64_t v_row, int64_t v_head,
                           int type, void *stream);
 /* the numbers of positions past[i] and on: k, v [rows][kv_heads][dim] of `type`; rows of no sequence are zeros */
