@@ -310,8 +310,8 @@ __global__ void __launch_bounds__(kReadThreads) kv8_read_kernel(Kv8Cache c, Kv8S
 // a sequence lie next to one another in the order of the work.  Work is counted in blocks of 16 tokens over all sequences, heads and tiles and dealt to the CTAs in
 // equal runs, so that one long sequence fills the GPU and lengths need not be alike; runs that share a tile leave (max, sum, output), and the last one to come joins them, always in
 // the same order (a second kernel for that took 6 us after one request's 1024 tokens, 11 after 131072, 26 after 64 requests).  Few short tiles go to a cluster each.
-// Measured: 64 requests of up to 24576 tokens 223 us (5.9 TB/s of the 6.5 that a copy reaches); one behind 131071 28 us, of which the cache's bytes are 10, the first loads 4 and the two
-// joins 9; one of 1025 9.7 us: a launch and a chain of looks at the sequence, its page, its scale, its codes.
+// Measured: 64 requests of up to 24576 tokens 226 us (5.9 TB/s of the 6.5 that a copy reaches); one behind 131071 28 us, of which the cache's bytes are 10, the first loads 4 and the two
+// joins 9; one of 1025 9.8 us: a launch and a chain of looks at the sequence, its page, its scale, its codes.
 //
 // A warp keeps its own ring of blocks in shared memory, filled by asynchronous copies that swizzle 16-byte pieces (rows lie 128 bytes apart, which would be the same banks), and
 // multiplies on the tensor cores (mma.sync, 16 x 8 x 16: a block's 16 tokens, or 16 channels of their values, by eight rows: what a group has, and nothing is waited for across warps).
