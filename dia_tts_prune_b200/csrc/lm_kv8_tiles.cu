@@ -355,8 +355,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_attention_tiles_kernel(Kv8Cac
         const long long tok0 = (long long)from * kKeys;
         const auto within = [&](long long v) { return (int)max(min(v - tok0, 0x7fffff00ll), -1ll); };
         const int hi = within(position(p)), lo = within(position(p) - back), all_hi = within(position(p0 + g * kHalfRows)), all_lo = within(position(p0 + g * kHalfRows + kHalfRows - 1) - back);
-        // What a score is times.  Hidden ones are -infinity, so it must not be zero: it is where a page of zeros' step is 2^-100, or a small query or scale comes to it.  (Scores are below
-        // 2^30, so what is raised to 2^-126 moves by 2^-96 at most.)
+        // What a score is times.  Hidden ones are -infinity, so it must not be zero, which the product comes to where a page's step is 2^-100 (zeros) or none (never written) and the query or
+        // the scale is small.  (Scores are below 2^30, so what is raised to 2^-126 moves by 2^-96 at most.)
         const auto factor = [&](float key_scale) { return fmaxf(key_scale * row_scale, 0x1p-126f); };
         float ref = -1e30f, l = 0.f;
         // (A step's scores come behind the value product of two steps before, not of the last one: what is told of every step has a barrier for the even ones and one for the odd.)
